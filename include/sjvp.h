@@ -36,7 +36,7 @@
  *     void*) of the CURRENT device and returns without synchronising.
  *   - Every function returns SJVP_OK (0) or a negative error code; nothing aborts or throws.
  *     Argument errors are detected before anything is launched.
- *   - Results are deterministic: no atomics are used.
+ *   - Results are deterministic: no atomics are used but among the lanes of one wave, whose order is fixed.
  */
 #ifndef SJVP_H
 #define SJVP_H
@@ -65,7 +65,8 @@ enum sjvp_status {
     SJVP_ERR_ROTARY = -9,    /* sjvp_rope: n outside 1..4, rot_dim odd, < 0 or > D, or dtypes that mix bf16 and fp16;
                                 sjvp_fwd_rotary / sjvp_bwd_rotary: a shape, dtype or table they do not serve */
     SJVP_ERR_SCALE = -10,    /* scale negative, infinite or NaN (0 selects the default)      */
-    SJVP_ERR_SCRATCH = -11   /* sjvp_bwd_noalloc: problem beyond SJVP_NOALLOC_MAX_ROWS, or no static scratch on this device */
+    SJVP_ERR_SCRATCH = -11,  /* sjvp_bwd_noalloc: problem beyond SJVP_NOALLOC_MAX_ROWS, or no static scratch on this device */
+    SJVP_ERR_BUCKETS = -12   /* sjvp_ctx_*: a bucket count or list of first distances that is not served */
 };
 
 /* Indices into the stride tables: strides[3*i + {0,1,2}] = (batch, head, sequence) strides in
@@ -273,6 +274,55 @@ int sjvp_gelu(const void* u, const void* tu, const void* dy, const void* dty, vo
 #define SJVP_CAST_MAX 16
 int sjvp_cast(int n, const void* const* x, void* const* y, const int64_t* count, int in_dtype, int out_dtype,
               void* stream);
+
+/*
+ * Attention of queries on keys of another length (cross attention to an encoder's states), optionally with a learned relative
+ * position bias, and its backward.  SJVP_BF16 or SJVP_FP16 tensors, without tangents:
+ *   s[i][j] = scale q_i.k_j + table[bucket(j - (start + i))][head]      for j < key length (causal: and j <= start + i)
+ *   lse_i = log sum_j exp s[i][j],   o_i = sum_j exp(s[i][j] - lse_i) v_j
+ * q, o, dO, dq: [B,Hq,Lq,D]; k, v, dk, dv: [B,Hkv,Lk,D]; Hq a multiple of Hkv, query head h reads key head h / (Hq / Hkv).
+ * Any strides (batch, head, sequence; unit last stride; the sequence stride of an input below 2^24) and any alignment of the rows.
+ *   key_lengths, query_lengths, query_start   device arrays [B], or NULL: every sequence is as long as its tensor, and its
+ *       query 0 has position query_start0 (which is added to query_start[b] otherwise).  Lengths are clamped to the tensor.  What
+ *       lies in rows behind a length is not used, not even NaN; results there are zeros.  query_start and query_start0 lie within +-2^29.
+ *   a row that sees no key (also: whose every key has the bias -inf) has o = 0, lse = -inf and no gradient.
+ *   table (or NULL: no bias, causal must be 0)   fp32, bf16 or fp16 [buckets of all directions][Hq] with strides table_stride
+ *       (bucket, head); entries below -2.3e38 count as that, -inf excludes its keys.  bucket_first: HOST array of `buckets` first
+ *       distances in ascending order from 0, the last one at most SJVP_CTX_MAX_DISTANCE; a distance has the last bucket that does
+ *       not begin beyond it.  bidirectional: keys behind a query (j > start + i) have buckets of their own,
+ *       buckets .. 2 buckets - 1, by their distance; otherwise they count as distance 0.
+ *   lse   [B,Hq,Lq] fp32 contiguous; the forward takes NULL where no backward follows.
+ *   dk, dv   both or neither (then without the launch that makes them)
+ *   dtable (or NULL)   in the type of table, with strides dtable_stride; summed in fp32 in a fixed order; that of an fp32 table is formed to fp32 accuracy.
+ * strides[3*i + {0,1,2}]: (batch, head, sequence) strides in elements of tensor i of sjvp_ctx_tensor.  scale 0: 1/sqrt(D).
+ * The workspace is device memory of sjvp_ctx_workspace_bytes() bytes, 16-byte aligned (0: none is needed).
+ * No counterpart in the reference, whose attention has one length, no mask and no bias.
+ */
+#define SJVP_CTX_MAX_BUCKETS 256   /* of one direction */
+#define SJVP_CTX_MAX_DISTANCE 1024
+enum sjvp_ctx_tensor { SJVP_C_Q = 0, SJVP_C_K, SJVP_C_V, SJVP_C_O, SJVP_C_DO, SJVP_C_DQ, SJVP_C_DK, SJVP_C_DV,
+                       SJVP_C_COUNT };
+typedef struct sjvp_ctx {
+    const void *q, *k, *v;
+    void* o;
+    const void* dO;
+    void *dq, *dk, *dv;
+    int64_t strides[SJVP_C_COUNT * 3];
+    float* lse;
+    const int32_t *key_lengths, *query_lengths, *query_start;
+    const void* table;
+    void* dtable;
+    int64_t table_stride[2], dtable_stride[2];
+    const int32_t* bucket_first;
+    void* workspace;
+    size_t workspace_bytes;
+    int32_t query_start0, table_dtype, buckets, bidirectional, causal;
+    int32_t B, Hq, Hkv, Lq, Lk, D;
+    float scale;
+} sjvp_ctx;
+size_t sjvp_ctx_workspace_bytes(const sjvp_ctx* t, int backward);
+int sjvp_ctx_fwd(const sjvp_ctx* t, int dtype, void* stream);
+int sjvp_ctx_bwd(const sjvp_ctx* t, int dtype, void* stream);
 
 /* Static, NUL-terminated description of a status code. */
 const char* sjvp_strerror(int status);

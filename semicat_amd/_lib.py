@@ -27,6 +27,7 @@ SJVP_ERR_PARTS = -8
 SJVP_ERR_ROTARY = -9
 SJVP_ERR_SCALE = -10
 SJVP_ERR_SCRATCH = -11
+SJVP_ERR_BUCKETS = -12
 SJVP_NOALLOC_MAX_ROWS = 1 << 20
 
 SJVP_BWD_ROW = 1
@@ -38,12 +39,18 @@ F_TENSORS = ("q", "k", "v", "tq", "tk", "tv", "o", "to")
 B_TENSORS = ("q", "k", "v", "tq", "tk", "tv", "o", "to", "dO", "dTO",
              "dq", "dk", "dv", "dtq", "dtk", "dtv")
 
+C_TENSORS = ("q", "k", "v", "o", "dO", "dq", "dk", "dv")
+SJVP_CTX_MAX_BUCKETS = 256
+SJVP_CTX_MAX_DISTANCE = 1024
+SJVP_CTX_MAX_POSITION = 1 << 29
+
 SJVP_REPAIR_OFF = 0
 SJVP_REPAIR_AUTO = 1
 SJVP_REPAIR_ALWAYS = 2
 
 EXPORTS = ("sjvp_fwd", "sjvp_bwd", "sjvp_bwd_parts", "sjvp_bwd_noalloc", "sjvp_fwd_rotary", "sjvp_bwd_rotary", "sjvp_bwd_workspace_bytes", "sjvp_rope",
            "sjvp_adaln_fwd", "sjvp_adaln_bwd", "sjvp_adaln_workspace_floats", "sjvp_gelu", "sjvp_cast",
+           "sjvp_ctx_fwd", "sjvp_ctx_bwd", "sjvp_ctx_workspace_bytes",
            "sjvp_set_row_sum_repair", "sjvp_strerror", "sjvp_version", "sjvp_build_id")
 
 
@@ -55,6 +62,18 @@ class AdaLn(ctypes.Structure):
                                                   "da", "dta", "dgate", "dtgate", "dscale", "dtscale", "dshift",
                                                   "dtshift", "dw", "db", "workspace")]
                 + [("B", ctypes.c_int), ("S", ctypes.c_int), ("W", ctypes.c_int), ("eps", ctypes.c_float)])
+
+
+class Ctx(ctypes.Structure):
+    """``struct sjvp_ctx``."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in C_TENSORS]
+                + [("strides", ctypes.c_int64 * (3 * len(C_TENSORS)))]
+                + [(n, ctypes.c_void_p) for n in ("lse", "key_lengths", "query_lengths", "query_start", "table", "dtable")]
+                + [("table_stride", ctypes.c_int64 * 2), ("dtable_stride", ctypes.c_int64 * 2)]
+                + [("bucket_first", ctypes.c_void_p), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t)]
+                + [(n, ctypes.c_int32) for n in ("query_start0", "table_dtype", "buckets", "bidirectional", "causal",
+                                                 "B", "Hq", "Hkv", "Lq", "Lk", "D")]
+                + [("scale", ctypes.c_float)])
 
 
 _lock = threading.Lock()
@@ -112,6 +131,11 @@ def load() -> ctypes.CDLL:
             lib.sjvp_adaln_workspace_floats.restype = ctypes.c_size_t
             lib.sjvp_gelu.argtypes = [vp] * 6 + [ctypes.c_int64, i, vp]
             lib.sjvp_gelu.restype = i
+            ctx = ctypes.POINTER(Ctx)
+            lib.sjvp_ctx_fwd.argtypes = lib.sjvp_ctx_bwd.argtypes = [ctx, i, vp]
+            lib.sjvp_ctx_fwd.restype = lib.sjvp_ctx_bwd.restype = i
+            lib.sjvp_ctx_workspace_bytes.argtypes = [ctx, i]
+            lib.sjvp_ctx_workspace_bytes.restype = ctypes.c_size_t
             lib.sjvp_set_row_sum_repair.argtypes = [i]
             lib.sjvp_set_row_sum_repair.restype = i
             lib.sjvp_strerror.argtypes = [i]

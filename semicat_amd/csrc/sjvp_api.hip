@@ -503,6 +503,7 @@ const char* sjvp_strerror(int status) {
         case SJVP_ERR_SCALE: return "scale must be finite and >= 0 (0 selects 1/sqrt(D))";
         case SJVP_ERR_SCRATCH: return "sjvp_bwd_noalloc: B * H * ceil(Lq/128)*128 exceeds SJVP_NOALLOC_MAX_ROWS, or the static scratch could not be located on this device";
         case SJVP_ERR_ROTARY: return "rotary embedding: sjvp_rope needs n in 1..4, rot_dim even with 0 <= rot_dim <= D, and no mix of bf16 and fp16; sjvp_fwd_rotary / sjvp_bwd_rotary need D = 64, Lk <= 128, bf16 or fp16 tensors with 16-byte aligned rows, and 16-byte aligned fp32 tables of at least max(Lq, Lk) rows with a row stride that is a multiple of 4";
+        case SJVP_ERR_BUCKETS: return "relative position bias: 1 to SJVP_CTX_MAX_BUCKETS buckets of a direction with ascending first distances from 0 to at most SJVP_CTX_MAX_DISTANCE; without a table there are no causal rows";
         default: return "unknown sjvp status";
     }
 }

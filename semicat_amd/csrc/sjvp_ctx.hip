@@ -1,0 +1,220 @@
+// C ABI of the attention on keys of another length / with a relative position bias (sjvp_ctx_fwd, sjvp_ctx_bwd): checks, how
+// the work is split, and the launches.
+#include <climits>
+#include <cmath>
+#include <type_traits>
+
+#include "sjvp_ctx_launch.hpp"
+
+namespace sjvp {
+
+// Adds up the bucket sums of the workgroups of a head: 16 threads to a bucket, each over every 16th workgroup, in a fixed order.
+__global__ __launch_bounds__(256) void ctx_table_sum(CtxParams p) {
+    __shared__ float sums[16][17];
+    const int nb = p.both ? 2 * p.buckets : p.buckets, per = (nb + 15) / 16;
+    const int head = blockIdx.x / per, col = threadIdx.x & 15, slice = threadIdx.x >> 4, bucket = (blockIdx.x % per) * 16 + col;
+    const int64_t parts = (int64_t)p.B * p.blocks * p.splits;
+    float sum = 0.0f;
+    if (bucket < nb)
+        for (int64_t i = slice; i < parts; i += 16) sum += p.tpart[((int64_t)head * parts + i) * nb + bucket];
+    sums[slice][col] = sum;
+    workgroup_barrier();
+    if (slice == 0 && bucket < nb) {
+        sum = 0.0f;
+        for (int i = 0; i < 16; ++i) sum += sums[i][col];
+        const int64_t at = bucket * p.dtsb + head * p.dtsh;
+        if (p.table_type == SJVP_FP32) reinterpret_cast<float*>(p.dtable)[at] = sum;
+        else reinterpret_cast<elem_t*>(p.dtable)[at] = (elem_t)(p.table_type == SJVP_BF16 ? Bf16::pack2(sum, 0.0f) : Fp16::pack2(sum, 0.0f));
+    }
+}
+
+namespace {
+
+constexpr int kMaxSplits = 64;
+constexpr int kLds = 160 * 1024;
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Splits of a looped axis of `steps` steps for a launch of `groups` workgroups: enough for `per_unit` to a compute unit, each
+// with `least` steps or more.
+int splits_for(int64_t groups, int64_t steps, int per_unit, int64_t least) {
+    const int64_t wanted = (int64_t)per_unit * compute_units() / groups;
+    return (int)std::max<int64_t>(1, std::min<int64_t>({wanted, steps / least, kMaxSplits}));
+}
+
+}  // namespace
+
+CtxPlan ctx_plan_fwd(const CtxParams& p) {
+    CtxPlan plan;
+    const int HD = ctx_padded(p.D), bias = p.table ? 4 * ctx_entries(p) : 0;
+    const int64_t many = (int64_t)p.B * p.Hq * ceil_div(p.Lq, kCtxOwned);
+    plan.few = (int64_t)p.G * p.Lq <= 32 || 2 * many <= compute_units();
+    if (!plan.few) {
+        plan.blocks = (int)ceil_div(p.Lq, kCtxOwned);
+        plan.units = (int64_t)p.B * p.Hkv;
+        plan.inner = (int64_t)p.G * plan.blocks;
+        plan.smem = ctx_tiles_bytes(HD) + bias;
+        return plan;
+    }
+    const int sums = kCtxWaves * 32 * (HD + 4 + 2) * 4;
+    const int heads = p.Lq < 32 ? std::min(p.G, 31 / p.Lq + 2) : 1;  // that a block of 32 rows can touch
+    plan.packed = p.Lq < 32 && sums + heads * bias <= kLds ? p.G : 1;
+    plan.smem = sums + (plan.packed > 1 ? heads : 1) * bias;
+    plan.blocks = (int)ceil_div((int64_t)plan.packed * p.Lq, 32);
+    plan.units = (int64_t)p.B * p.Hkv * (p.G / plan.packed);
+    plan.splits = splits_for(plan.units * plan.blocks, p.Lk, 2, 256);
+    plan.inner = (int64_t)plan.blocks * plan.splits;
+    return plan;
+}
+
+CtxPlan ctx_plan_row(const CtxParams& p) {
+    CtxPlan plan;
+    plan.blocks = (int)ceil_div(p.Lq, kCtxOwned);
+    plan.units = (int64_t)p.B * p.Hkv;
+    // (the bucket sums need a row's whole residue, see ctx_bwd_row)
+    plan.splits = p.tpart ? 1 : splits_for((int64_t)p.B * p.Hq * plan.blocks, ceil_div(p.Lk, kCtxTile), 1, 4);
+    plan.inner = (int64_t)p.G * plan.blocks * plan.splits;
+    plan.smem = ctx_tiles_bytes(ctx_padded(p.D)) + (p.table ? 4 * ctx_entries(p) * (p.tpart ? 1 + kCtxWaves : 1) : 0);
+    return plan;
+}
+
+CtxPlan ctx_plan_col(const CtxParams& p) {
+    CtxPlan plan;
+    plan.blocks = (int)ceil_div(p.Lk, kCtxOwned);
+    plan.units = (int64_t)p.B * p.Hkv;
+    plan.splits = splits_for(plan.units * plan.blocks, p.G * ceil_div(p.Lq, kCtxTile), 1, 4);
+    plan.inner = (int64_t)plan.blocks * plan.splits;
+    plan.smem = ctx_tiles_bytes(ctx_padded(p.D)) + 4 * kCtxTile * 4 + (p.table ? 4 * ctx_entries(p) : 0);
+    return plan;
+}
+
+namespace {
+
+int ctx_params(const sjvp_ctx* t, CtxParams& p) {
+    if (!t) return SJVP_ERR_NULL;
+    if (t->B < 1 || t->Hq < 1 || t->Hkv < 1 || t->Lq < 1 || t->Lk < 1 || t->Hq % t->Hkv || t->Lq > kCtxMost || t->Lk > kCtxMost ||
+        t->query_start0 > kCtxMost || t->query_start0 < -kCtxMost)
+        return SJVP_ERR_SHAPE;
+    if (t->D < 16 || t->D > 128) return SJVP_ERR_HEAD_DIM;
+    if (!(t->scale >= 0.0f) || !std::isfinite(t->scale)) return SJVP_ERR_SCALE;
+    CtxView* views[SJVP_C_COUNT] = {&p.q, &p.k, &p.v, &p.o, &p.g, &p.dq, &p.dk, &p.dv};
+    const void* ptrs[SJVP_C_COUNT] = {t->q, t->k, t->v, t->o, t->dO, t->dq, t->dk, t->dv};
+    for (int i = 0; i < SJVP_C_COUNT; ++i)
+        *views[i] = {static_cast<elem_t*>(const_cast<void*>(ptrs[i])), t->strides[3 * i], t->strides[3 * i + 1], t->strides[3 * i + 2]};
+    for (const CtxView* v : {&p.q, &p.k, &p.v, &p.g})
+        if (v->ptr && (v->sl < 0 || v->sl >= 1 << 24)) return SJVP_ERR_SHAPE;
+    p.lse = t->lse;
+    p.klen = t->key_lengths, p.qlen = t->query_lengths, p.start = t->query_start, p.start0 = t->query_start0;
+    p.B = t->B, p.Hq = t->Hq, p.Hkv = t->Hkv, p.G = t->Hq / t->Hkv, p.Lq = t->Lq, p.Lk = t->Lk, p.D = t->D;
+    p.scale = t->scale == 0.0f ? 1.0f / std::sqrt(static_cast<float>(t->D)) : t->scale;
+    p.c = p.scale * kLog2e;
+    p.table = t->table, p.dtable = t->dtable, p.table_type = t->table_dtype;
+    p.tsb = t->table_stride[0], p.tsh = t->table_stride[1], p.dtsb = t->dtable_stride[0], p.dtsh = t->dtable_stride[1];
+    p.both = t->bidirectional != 0, p.causal = t->causal != 0;
+    if (!t->table) return p.causal || t->dtable ? SJVP_ERR_BUCKETS : SJVP_OK;
+    if (t->table_dtype != SJVP_FP32 && t->table_dtype != SJVP_BF16 && t->table_dtype != SJVP_FP16) return SJVP_ERR_DTYPE;
+    if (!t->bucket_first) return SJVP_ERR_NULL;
+    if (t->buckets < 1 || t->buckets > kCtxBuckets || t->bucket_first[0] != 0) return SJVP_ERR_BUCKETS;
+    p.buckets = t->buckets;
+    for (int i = 0; i < t->buckets; ++i) {
+        if (t->bucket_first[i] > SJVP_CTX_MAX_DISTANCE || (i && t->bucket_first[i] < t->bucket_first[i - 1])) return SJVP_ERR_BUCKETS;
+        p.first[i] = static_cast<uint16_t>(t->bucket_first[i]);
+    }
+    p.far = std::max(1, t->bucket_first[t->buckets - 1]);
+    return SJVP_OK;
+}
+
+// The plans of a call, and where its scratch lies in the workspace (in floats).
+struct CtxLayout {
+    CtxPlan fwd, row, col;
+    size_t delta = 0, tpart = 0, stat = 0, part = 0, total = 0;
+};
+
+CtxLayout ctx_layout(CtxParams& p, bool backward) {
+    CtxLayout l;
+    const size_t HD = ctx_padded(p.D), q_rows = (size_t)p.B * p.Hq * p.Lq, k_rows = (size_t)p.B * p.Hkv * p.Lk;
+    const auto take = [&](size_t floats) {
+        const size_t at = l.total;
+        l.total += (floats + 3) / 4 * 4;
+        return at;
+    };
+    if (!backward) {
+        l.fwd = ctx_plan_fwd(p);
+        if (l.fwd.splits > 1) {
+            l.stat = take(2 * l.fwd.splits * q_rows);
+            l.part = take(l.fwd.splits * q_rows * HD);
+        }
+        return l;
+    }
+    float some;
+    p.tpart = p.dtable ? &some : nullptr;  // (whether, for the plan)
+    l.row = ctx_plan_row(p);
+    l.col = ctx_plan_col(p);
+    p.tpart = nullptr;
+    l.delta = take(q_rows);
+    if (p.dtable) l.tpart = take((size_t)p.Hq * p.B * l.row.blocks * l.row.splits * (p.both ? 2 : 1) * p.buckets);
+    // (the row-owned launch's sums are used up before the column-owned one writes its own)
+    const size_t row = l.row.splits > 1 ? l.row.splits * q_rows * HD : 0, col = l.col.splits > 1 ? 2 * l.col.splits * k_rows * HD : 0;
+    l.part = take(std::max(row, col));
+    return l;
+}
+
+bool ctx_fits(const CtxPlan& plan) { return ctx_grid((int)std::min<int64_t>(plan.units, INT_MAX), 1) * plan.inner <= INT_MAX; }
+
+int ctx_workspace(const sjvp_ctx* t, const CtxLayout& l, float*& ws) {
+    ws = static_cast<float*>(t->workspace);
+    return l.total == 0 || (ws && t->workspace_bytes >= 4 * l.total && reinterpret_cast<uintptr_t>(ws) % 16 == 0) ? SJVP_OK : SJVP_ERR_WORKSPACE;
+}
+
+}  // namespace
+}  // namespace sjvp
+
+extern "C" {
+
+using namespace sjvp;
+
+size_t sjvp_ctx_workspace_bytes(const sjvp_ctx* t, int backward) {
+    CtxParams p{};
+    if (ctx_params(t, p) != SJVP_OK) return 0;
+    return 4 * ctx_layout(p, backward != 0).total;
+}
+
+int sjvp_ctx_fwd(const sjvp_ctx* t, int dtype, void* stream) {
+    CtxParams p{};
+    const int rc = ctx_params(t, p);
+    if (rc != SJVP_OK) return rc;
+    if (dtype != SJVP_BF16 && dtype != SJVP_FP16) return SJVP_ERR_DTYPE;
+    if (!t->q || !t->k || !t->v || !t->o) return SJVP_ERR_NULL;
+    const CtxLayout l = ctx_layout(p, false);
+    if (!ctx_fits(l.fwd)) return SJVP_ERR_SHAPE;
+    float* ws;
+    if (ctx_workspace(t, l, ws) != SJVP_OK) return SJVP_ERR_WORKSPACE;
+    p.stat = ws + l.stat, p.part = ws + l.part;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    return dtype == SJVP_BF16 ? ctx_forward<Bf16>(p, l.fwd, s) : ctx_forward<Fp16>(p, l.fwd, s);
+}
+
+int sjvp_ctx_bwd(const sjvp_ctx* t, int dtype, void* stream) {
+    CtxParams p{};
+    int rc = ctx_params(t, p);
+    if (rc != SJVP_OK) return rc;
+    if (dtype != SJVP_BF16 && dtype != SJVP_FP16) return SJVP_ERR_DTYPE;
+    if (!t->q || !t->k || !t->v || !t->o || !t->dO || !t->dq || !t->dk != !t->dv || !t->lse) return SJVP_ERR_NULL;
+    const CtxLayout l = ctx_layout(p, true);
+    if (!ctx_fits(l.row) || !ctx_fits(l.col)) return SJVP_ERR_SHAPE;
+    float* ws;
+    if (ctx_workspace(t, l, ws) != SJVP_OK) return SJVP_ERR_WORKSPACE;
+    p.delta = ws + l.delta, p.part = ws + l.part, p.tpart = p.dtable ? ws + l.tpart : nullptr;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    const auto run = [&](const CtxPlan& plan, bool row) {
+        return dtype == SJVP_BF16 ? ctx_backward<Bf16>(p, plan, row, s) : ctx_backward<Fp16>(p, plan, row, s);
+    };
+    rc = run(l.row, true);
+    if (rc == SJVP_OK && t->dk) rc = run(l.col, false);
+    if (rc != SJVP_OK || !p.dtable) return rc;
+    const int per = ((p.both ? 2 : 1) * p.buckets + 15) / 16;
+    p.blocks = l.row.blocks, p.splits = l.row.splits;
+    return launch(ctx_table_sum, p.Hq * per, 0, s, p, 256);
+}
+
+}  // extern "C"

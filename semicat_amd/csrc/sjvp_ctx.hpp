@@ -1,0 +1,319 @@
+// Attention of queries on keys of another length, and with a learned relative position bias: parameters and device
+// building blocks (kernels: sjvp_ctx_fwd.hpp, sjvp_ctx_bwd.hpp).
+//
+//   s[i][j] = scale q_i.k_j + table[bucket(j - (start + i))][head]     for j < key length (and j <= start + i if causal)
+//   lse_i = log sum_j exp s[i][j],  p = exp(s - lse),  o_i = sum_j p[i][j] v_j
+//
+// A query head reads key head  head / (Hq / Hkv).  A row that sees no key has o = 0 and lse = -inf.
+//
+// Tile algebra (v_mfma_f32_32x32x16_{bf16,f16}): C[y][x] += sum_k A[y][k] B[k][x] with
+//     A: lane l holds row y = l % 32, k = 8*(l/32) + i (i < 8);   B: column x = l % 32, same k;
+//     C: lane l holds column x = l % 32 and, in register r < 16, row y = 8*(r/4) + 4*(l/32) + r%4.
+// A wave owns 32 positions as columns, one to a lane pair (l, l + 32), so that the softmax statistics of a row are one
+// register each and a reduction over the looped axis is register arithmetic and one exchange of the halves.  Its
+// operands (B) stay in registers, the looped side is A from LDS.  Registers 8m .. 8m+7 of a score tile, rounded to 16
+// bits, are the B operand of the next contraction under the numbering  k = 8h + i  <->  y = 16m + 8*(i/4) + 4h + i%4  (h = l/32);
+// A in that numbering is what two transposing LDS reads of four rows deliver.
+#pragma once
+#include "sjvp_device.hpp"
+#include "../../include/sjvp.h"
+
+namespace sjvp {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int kCtxWaves = 4;
+constexpr int kCtxThreads = 64 * kCtxWaves;
+constexpr int kCtxOwned = 32 * kCtxWaves;  // owned positions of a workgroup whose waves share their tiles
+constexpr int kCtxTile = 64;               // looped positions per tile
+constexpr int kCtxPad = 64;                // entries of the bias row beyond the last single distance, on each side
+constexpr int kCtxBuckets = SJVP_CTX_MAX_BUCKETS;
+constexpr int kCtxMost = 1 << 29;          // positions and lengths: sums of three stay within 32 bits
+
+template <typename T> struct Mma32;
+template <> struct Mma32<Bf16> {
+    static __device__ __forceinline__ f32x16 run(u32x4 a, u32x4 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+};
+template <> struct Mma32<Fp16> {
+    static __device__ __forceinline__ f32x16 run(u32x4 a, u32x4 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+};
+
+struct CtxView {
+    elem_t* ptr;
+    int64_t sb, sh, sl;
+    __device__ __forceinline__ elem_t* head(int b, int h) const { return ptr + b * sb + h * sh; }
+};
+
+struct CtxParams {
+    CtxView q, k, v, o, g, dq, dk, dv;       // g: the cotangent of o
+    float *lse, *delta;                      // [B,Hq,Lq]
+    float *part, *stat;                      // sums of split work: rows of HD floats; their (maximum, sum) pairs
+    float* tpart;                            // bucket sums of each workgroup
+    void* dtable;
+    const void* table;
+    const int *klen, *qlen, *start;          // per batch entry, or null
+    int64_t tsb, tsh, dtsb, dtsh;            // strides of table and dtable (bucket, head)
+    int start0, table_type;
+    int B, Hq, Hkv, G, Lq, Lk, D;
+    float scale, c;                          // c = scale * log2(e)
+    int buckets, both, causal, far;          // buckets of a direction; far: the first distance of the last one
+    int splits, blocks;                      // splits of the looped axis; workgroups of a split over the owned axis
+    int packed;                              // ctx_fwd_few: heads to a block of rows
+    int cols;                                // ctx_sum: dK and dV, not dQ
+    uint16_t first[kCtxBuckets];             // first distance of each bucket
+};
+
+// max / sum over the two lanes of a column
+__device__ __forceinline__ float halves_max(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float halves_sum(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// Rows start on element boundaries; 16-byte accesses need no more.  Where a row ends inside a chunk of eight columns (D is not a
+// multiple of 8), the chunk is taken from the row's last eight elements and moved down: no access leaves the row.
+typedef u32x4 __attribute__((aligned(2))) u32x4_any;
+__device__ __forceinline__ int chunk_column(int c8, int D) { return min(c8, D - 8); }
+__device__ __forceinline__ u32x4 chunk_shifted(u32x4 x, int c8, int D) {
+    const int over = c8 + 8 - D;  // elements of the chunk beyond the row
+    if (over <= 0) return x;
+    return __builtin_bit_cast(u32x4, __builtin_bit_cast(unsigned __int128, x) >> (16 * min(over, 7)));
+}
+// Eight elements of a row from column c8 on, zeros beyond D.
+__device__ __forceinline__ u32x4 load_chunk(const elem_t* p, int c8, int D) {
+    if (c8 >= D) return u32x4{0u, 0u, 0u, 0u};
+    const u32x4 x = *reinterpret_cast<const u32x4_any*>(p + chunk_column(c8, D));
+    return D % 8 ? chunk_shifted(x, c8, D) : x;
+}
+__device__ __forceinline__ void store_chunk(elem_t* p, u32x4 x, int c8, int D) {
+    if (c8 + 8 <= D) {
+        *reinterpret_cast<u32x4_any*>(p + c8) = x;
+    } else if (c8 < D) {
+#pragma unroll
+        for (int i = 0; i < 7; ++i)
+            if (c8 + i < D) p[c8 + i] = (elem_t)(x[i / 2] >> (16 * (i % 2)));
+    }
+}
+
+// LDS tiles are [rows][HD + 8]: the 16 bytes between rows spread both the row-major 16-byte reads of 16 rows and the
+// transposing reads of 4 rows over all banks.
+template <int HD> constexpr int kCtxLd = HD + 8;
+
+// B operands of this lane's own row (all chunks of 16 of the head dimension), from memory.
+template <int HD>
+__device__ __forceinline__ void own_operands(u32x4* out, const elem_t* row, bool ok, int h, int D) {
+#pragma unroll
+    for (int c = 0; c < HD / 16; ++c) out[c] = ok ? load_chunk(row, 16 * c + 8 * h, D) : u32x4{0u, 0u, 0u, 0u};
+}
+
+// A operand: rows `row0` .. row0 + 31 of a tile, chunk c of 16 columns.
+template <int HD>
+__device__ __forceinline__ u32x4 tile_rows(const elem_t* tile, int row0, int c, int lane) {
+    return *reinterpret_cast<const u32x4*>(tile + (row0 + (lane & 31)) * kCtxLd<HD> + 16 * c + 8 * (lane >> 5));
+}
+
+// A operand of an output contraction: columns 32 dt .. 32 dt + 31 (as rows of A) over the 16 rows from row0 on, in the numbering
+// at the top.  Within 16 lanes of a transposing read lane 4j + i supplies row j, columns 4i .. 4i+3, and lane n receives column n.
+template <int HD>
+__device__ __forceinline__ u32x4 tile_columns(const elem_t* tile, int row0, int dt, int lane) {
+    const int i16 = lane & 15;
+    const elem_t* p = tile + (row0 + 4 * (lane >> 5) + (i16 >> 2)) * kCtxLd<HD> + 32 * dt + (lane & 16) + 4 * (i16 & 3);
+    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+    const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p)));
+    const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 8 * kCtxLd<HD>)));
+    return u32x4{lo[0], lo[1], hi[0], hi[1]};
+}
+
+// Registers 8m .. 8m+7 of a score tile as a B operand.
+template <typename T>
+__device__ __forceinline__ u32x4 pack_scores(const f32x16& s, int m) {
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = T::pack2(s[8 * m + 2 * i], s[8 * m + 2 * i + 1]);
+    return r;
+}
+
+// Rows of a tensor from a given one on, as a buffer: reads behind the last row that exists return zeros (whatever memory holds there),
+// with no branch.  Offsets are 32 bits within a tile, so the host keeps row strides below 2^24 elements.
+typedef __amdgpu_buffer_rsrc_t Rows;
+constexpr uint32_t kNoChunk = 0x80000000u;  // an offset behind every buffer
+__device__ __forceinline__ Rows make_rows(const elem_t* base, int64_t sl, int rows, int D) {
+    const int bytes = rows > 0 ? 2 * ((min(rows, kCtxTile) - 1) * (int)sl + D) : 0;
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<elem_t*>(base), 0, bytes, 0x00020000);
+}
+__device__ __forceinline__ uint32_t chunk_offset(int row, int c8, int64_t sl, int D) {
+    return c8 < D ? 2u * (uint32_t)(row * (int)sl + chunk_column(c8, D)) : kNoChunk;
+}
+__device__ __forceinline__ u32x4 read_chunk(Rows rows, uint32_t offset) {
+    return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rows, offset, 0, 0));
+}
+
+// A tile of 64 rows on its way from memory to LDS through the registers of NT threads: any stride and alignment.
+template <int HD, int NT = kCtxThreads>
+struct TileCopy {
+    static constexpr int CH = HD / 8;
+    static constexpr int N = kCtxTile * CH / NT;
+    static_assert(kCtxTile * CH % NT == 0, "every thread copies whole chunks");
+    u32x4 r[N];
+    uint32_t offset[N];
+
+    __device__ __forceinline__ TileCopy(int64_t sl, int D, int tid) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) offset[i] = chunk_offset((tid + NT * i) / CH, 8 * ((tid + NT * i) % CH), sl, D);
+    }
+    __device__ __forceinline__ void load(const elem_t* base, int64_t sl, int rows, int D) {
+        const Rows from = make_rows(base, sl, rows, D);
+#pragma unroll
+        for (int i = 0; i < N; ++i) r[i] = read_chunk(from, offset[i]);
+    }
+    __device__ __forceinline__ void store(elem_t* tile, int D, int tid) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int x = tid + NT * i;
+            if (D % 8) r[i] = chunk_shifted(r[i], 8 * (x % CH), D);
+            *reinterpret_cast<u32x4*>(tile + (x / CH) * kCtxLd<HD> + 8 * (x % CH)) = r[i];
+        }
+    }
+};
+
+// The bucket of a position difference (key minus query): the last bucket whose first distance is not beyond the distance;
+// differences above zero have distances and buckets of their own (`both`) or distance 0.
+__device__ __forceinline__ int ctx_bucket(const CtxParams& p, int rel) {
+    const int d = min(p.both ? abs(rel) : max(-rel, 0), p.far);
+    int lo = 0, hi = p.buckets;  // first[lo] <= d < first[hi]
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (p.first[mid] <= d) lo = mid;
+        else hi = mid;
+    }
+    return lo + (p.both && rel > 0 ? p.buckets : 0);
+}
+
+__device__ __forceinline__ float ctx_table(const CtxParams& p, int bucket, int head) {
+    const int64_t at = bucket * p.tsb + head * p.tsh;
+    if (p.table_type == SJVP_FP32) return reinterpret_cast<const float*>(p.table)[at];
+    const elem_t x = reinterpret_cast<const elem_t*>(p.table)[at];
+    return p.table_type == SJVP_BF16 ? Bf16::to_float(x) : Fp16::to_float(x);
+}
+
+__device__ __forceinline__ int ctx_row_entries(const CtxParams& p) { return 2 * (p.far + kCtxPad) + 1; }
+
+// The bias of a head by position difference, entry far + pad for difference 0, in units of log2.  A difference of a 32 x 32
+// tile that is not wholly beyond `far` lies within far + 62, so the padding saves the tiles a clamp.  A table entry near
+// the lowest float32 would leave the range with the factor log2(e); it is raised to -2.3e38, still below any score.
+__device__ __forceinline__ void fill_bias_row(const CtxParams& p, float* row, int head, int tid, int threads) {
+    for (int x = tid; x < ctx_row_entries(p); x += threads) {
+        const float t = ctx_table(p, ctx_bucket(p, x - p.far - kCtxPad), head);
+        row[x] = t == -INFINITY ? t : fmaxf(t, -2.3e38f) * kLog2e;
+    }
+}
+
+struct CtxBatch {
+    int keys, rows, start;  // key length, query length, position of query 0
+    __device__ __forceinline__ CtxBatch(const CtxParams& p, int b)
+        : keys(p.klen ? min(max(p.klen[b], 0), p.Lk) : p.Lk),
+          rows(p.qlen ? min(max(p.qlen[b], 0), p.Lq) : p.Lq),
+          start(min(max(p.start ? p.start[b] : 0, -kCtxMost), kCtxMost) + p.start0) {}
+    // keys that the row sees
+    __device__ __forceinline__ int seen(const CtxParams& p, int row) const {
+        return p.causal ? max(0, min(keys, start + row + 1)) : keys;
+    }
+};
+
+// Workgroups run on XCD blockIdx % 8.  The workgroups of one (batch, key head) unit read the same rows: each XCD takes every
+// eighth unit as a whole and finds them in its L2, and batch entries of different lengths spread over all XCDs.  With few units
+// that do not divide by eight the XCDs would differ in load, and the plain order stays.
+struct CtxWork {
+    int unit, inner;
+    bool some;
+};
+inline __host__ __device__ bool ctx_by_xcd(int units) { return units % 8 == 0 || units >= 64; }
+inline __host__ __device__ int64_t ctx_grid(int units, int inner) {
+    return (int64_t)(ctx_by_xcd(units) ? (units + 7) / 8 * 8 : units) * inner;
+}
+__device__ __forceinline__ CtxWork ctx_work(int units, int inner) {
+    const int x = blockIdx.x;
+    if (!ctx_by_xcd(units)) return {x / inner, x % inner, true};
+    const int slot = x >> 3, unit = (x & 7) + 8 * (slot / inner);
+    return {unit, slot % inner, unit < units};
+}
+
+// Sums of a wave's own 32 rows, OUT^T (row of C: column of the result), as rows in memory: through the wave's own LDS region of
+// [32][HD + 8], so that rows go out in pieces of 16 bytes.
+template <typename T, int HD>
+__device__ __forceinline__ void store_rows(const f32x16* acc, float factor, elem_t* out, int64_t sl, int rows, elem_t* region,
+                                           int lane, int D) {
+    const int h = lane >> 5;
+    elem_t* mine = region + (lane & 31) * kCtxLd<HD> + 4 * h;
+#pragma unroll
+    for (int dt = 0; dt < HD / 32; ++dt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float x[4];
+            uint32_t w[2];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = factor == 0.0f ? 0.0f : acc[dt][4 * i + j] * factor;  // (sums of rows without a result may be NaN)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) w[j] = T::pack2(x[2 * j], x[2 * j + 1]);
+            *reinterpret_cast<u32x2*>(mine + 32 * dt + 8 * i) = u32x2{w[0], w[1]};
+        }
+    wave_exchange();
+    constexpr int CH = HD / 8;
+#pragma unroll
+    for (int x0 = 0; x0 < 32 * CH; x0 += 64) {
+        const int x = x0 + lane, row = x / CH, c8 = 8 * (x % CH);
+        if (row < rows) store_chunk(out + row * sl, *reinterpret_cast<const u32x4*>(region + row * kCtxLd<HD> + c8), c8, D);
+    }
+    wave_exchange();
+}
+
+// The same sums as fp32 rows of HD, for a later launch to add up; zeros for a lane that has no result.
+template <int HD>
+__device__ __forceinline__ void store_part(const f32x16* acc, bool some, float* out, int rows, int lane) {
+    if ((lane & 31) >= rows) return;
+    float* mine = out + (int64_t)(lane & 31) * HD + 4 * (lane >> 5);
+#pragma unroll
+    for (int dt = 0; dt < HD / 32; ++dt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<f32x4*>(mine + 32 * dt + 8 * i) =
+                some ? f32x4{acc[dt][4 * i], acc[dt][4 * i + 1], acc[dt][4 * i + 2], acc[dt][4 * i + 3]} : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+}
+
+// Where a 32 x 32 tile of position differences lies: entirely beyond `far` on one side (one bias for all), or not.
+enum CtxBand { kBelow, kNear, kAbove };
+__device__ __forceinline__ CtxBand ctx_band(const CtxParams& p, int least, int most) {
+    return most <= -p.far ? kBelow : least >= p.far ? kAbove : kNear;
+}
+
+// OUT^T += A^T B for the two halves of a packed score tile whose looped rows start at row0 of the tile.
+template <typename T, int HD>
+__device__ __forceinline__ void add_columns(f32x16* acc, const elem_t* tile, int row0, const f32x16& s, int lane) {
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+        const u32x4 b = pack_scores<T>(s, m);
+#pragma unroll
+        for (int dt = 0; dt < HD / 32; ++dt)
+            acc[dt] = Mma32<T>::run(tile_columns<HD>(tile, row0 + 16 * m, dt, lane), b, acc[dt]);
+    }
+}
+
+template <typename T, int HD>
+__device__ __forceinline__ f32x16 scores(const elem_t* tile, int row0, const u32x4* own, int lane) {
+    f32x16 s = {};
+#pragma unroll
+    for (int c = 0; c < HD / 16; ++c) s = Mma32<T>::run(tile_rows<HD>(tile, row0, c, lane), own[c], s);
+    return s;
+}
+
+// looped row of register r of a score tile
+__device__ __forceinline__ int tile_row(int r, int h) { return 8 * (r >> 2) + 4 * h + (r & 3); }
+
+}  // namespace sjvp

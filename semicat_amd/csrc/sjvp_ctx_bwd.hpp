@@ -1,0 +1,349 @@
+// Backward kernels of the attention on keys of another length / with a relative position bias (sjvp_ctx.hpp).
+//
+//   dP = dO V^T,  delta = rowsum(dO * O),  dS = P (dP - delta)
+//   dQ = scale dS K,  dK = scale sum_heads dS^T Q,  dV = sum_heads P^T dO,  dtable[bucket][head] = sum of dS over its differences
+//
+// A row-owned launch (dQ, delta and the bucket sums) and a column-owned one (dK, dV), both of which recompute P: 3 + 4
+// contractions against the 5 of a single launch, whose dQ would be summed by atomics in an order that changes from run to run.
+#pragma once
+#include "sjvp_ctx.hpp"
+
+namespace sjvp {
+
+__device__ __forceinline__ float wave_sum(float x) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
+    return x;
+}
+
+// dO . O of the lane's own row, from the operands of dO and from O in memory
+template <typename T, int HD>
+__device__ __forceinline__ float row_delta(const CtxParams& p, const u32x4* own_g, const elem_t* o, bool ok, int h) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int c = 0; c < HD / 16; ++c) {
+        if (!ok) continue;
+        const u32x4 x = load_chunk(o, 16 * c + 8 * h, p.D);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                sum += T::to_float((elem_t)(own_g[c][j] >> (16 * e))) *
+                       T::to_float((elem_t)(x[j] >> (16 * e)));
+    }
+    return halves_sum(sum);
+}
+
+// Row-owned: four waves of 32 query rows of one head share tiles of 64 keys.
+template <typename T, int HD, bool BIAS>
+__global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_row(CtxParams p) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    constexpr int kTile = kCtxTile * kCtxLd<HD>;
+    elem_t* tiles = reinterpret_cast<elem_t*>(smem);  // [2][K, V]
+    float* row = reinterpret_cast<float*>(tiles + 4 * kTile);
+    const int nqb = p.blocks, entries = ctx_row_entries(p);
+    const CtxWork w = ctx_work(p.B * p.Hkv, p.G * nqb * p.splits);
+    if (!w.some) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+    const int split = w.inner / (p.G * nqb), inner = w.inner % (p.G * nqb);
+    const int b = w.unit / p.Hkv, hk = w.unit % p.Hkv, hq = hk * p.G + inner / nqb;
+    const int qb = p.causal ? nqb - 1 - inner % nqb : inner % nqb;
+    const CtxBatch bt(p, b);
+    const int q0 = qb * kCtxOwned + 32 * wave, qi = q0 + (lane & 31);
+    const int rows = min(max(bt.rows - q0, 0), 32), last = min(bt.rows, (qb + 1) * kCtxOwned) - 1;
+    const int n = last >= qb * kCtxOwned ? bt.seen(p, last) : 0, n_wave = rows > 0 ? bt.seen(p, q0 + rows - 1) : 0;
+    const int n_all = bt.seen(p, q0), limit = bt.seen(p, qi), pos0 = bt.start + q0, pos = pos0 + (lane & 31);
+    const int nt = (n + kCtxTile - 1) / kCtxTile;
+    const int t0 = (int)((int64_t)nt * split / p.splits), t1 = (int)((int64_t)nt * (split + 1) / p.splits);
+    const bool with_table = BIAS && p.tpart;
+    float* hist = row + entries + wave * entries;
+
+    const int64_t stat = ((int64_t)b * p.Hq + hq) * p.Lq + qi;
+    float lse = -INFINITY;
+    if ((lane & 31) < rows) lse = p.lse[stat];
+    const bool ok = lse != -INFINITY;  // a row that sees no key has no gradient
+    lse = ok ? lse * kLog2e : INFINITY;
+    u32x4 own_q[HD / 16], own_g[HD / 16];
+    own_operands<HD>(own_q, p.q.head(b, hq) + (int64_t)qi * p.q.sl, ok, h, p.D);
+    own_operands<HD>(own_g, p.g.head(b, hq) + (int64_t)qi * p.g.sl, ok, h, p.D);
+    const float delta = row_delta<T, HD>(p, own_g, p.o.head(b, hq) + (int64_t)qi * p.o.sl, ok, h);
+
+    const elem_t *kt = p.k.head(b, hk) + (int64_t)t0 * kCtxTile * p.k.sl, *vt = p.v.head(b, hk) + (int64_t)t0 * kCtxTile * p.v.sl;
+    TileCopy<HD> kc(p.k.sl, p.D, tid), vc(p.v.sl, p.D, tid);
+    if (t0 < t1) {
+        kc.load(kt, p.k.sl, n - t0 * kCtxTile, p.D);
+        vc.load(vt, p.v.sl, n - t0 * kCtxTile, p.D);
+        kc.store(tiles, p.D, tid);
+        vc.store(tiles + kTile, p.D, tid);
+    }
+    if constexpr (BIAS) {
+        fill_bias_row(p, row, hq, tid, kCtxThreads);
+        if (with_table)
+            for (int x = lane; x < entries; x += 64) hist[x] = 0.0f;
+    }
+    workgroup_barrier();
+    // scores of 32 keys from k0 on to P, zero where hidden
+    const auto row_probabilities = [&](f32x16& s, int k0, CtxBand band) {
+        if (BIAS && band == kNear) {
+            const float* at = row + (k0 + 4 * h - pos + p.far + kCtxPad);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = fast_exp2(__builtin_fmaf(s[r], p.c, at[8 * (r >> 2) + (r & 3)]) - lse);
+        } else {
+            const float one = BIAS ? row[band == kBelow ? 0 : entries - 1] - lse : -lse;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = fast_exp2(__builtin_fmaf(s[r], p.c, one));
+        }
+        if (k0 + 32 > n_all) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (k0 + tile_row(r, h) >= limit) s[r] = 0.0f;
+        }
+    };
+    f32x16 acc[HD / 32] = {};
+    float below = 0.0f, above = 0.0f;    // sums of dS beyond the last single distance,
+    float p_below = 0.0f, p_above = 0.0f;  // and of P there
+    float residue = 0.0f;                  // sum of dS over the row
+    for (int t = t0; t < t1; ++t) {
+        const int key = t * kCtxTile, at = (t - t0) & 1;
+        if (t + 1 < t1) {
+            kt += kCtxTile * p.k.sl;
+            vt += kCtxTile * p.v.sl;
+            kc.load(kt, p.k.sl, n - key - kCtxTile, p.D);
+            vc.load(vt, p.v.sl, n - key - kCtxTile, p.D);
+        }
+        const elem_t* K = tiles + at * 2 * kTile;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int k0 = key + 32 * u;
+            if (k0 >= n_wave) continue;
+            f32x16 s = scores<T, HD>(K, 32 * u, own_q, lane), ds = scores<T, HD>(K + kTile, 32 * u, own_g, lane);
+            const CtxBand band = BIAS ? ctx_band(p, k0 - pos0 - 31, k0 + 31 - pos0) : kNear;
+            row_probabilities(s, k0, band);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) ds[r] = s[r] * (ds[r] - delta);
+            if (with_table) {
+                float sum = 0.0f, p_sum = 0.0f;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) sum += ds[r], p_sum += s[r];
+                residue += sum;
+                if (band == kNear) {
+                    // one wave's own sums, whose order of addition is the order of its instructions
+                    float* at = hist + (k0 + 4 * h - pos + p.far + kCtxPad);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        __hip_atomic_fetch_add(at + 8 * (r >> 2) + (r & 3), ds[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                } else if (band == kBelow) {
+                    below += sum, p_below += p_sum;
+                } else {
+                    above += sum, p_above += p_sum;
+                }
+            }
+            add_columns<T, HD>(acc, K, 32 * u, ds, lane);
+        }
+        if (t + 1 < t1) {
+            elem_t* next = tiles + (1 - at) * 2 * kTile;
+            kc.store(next, p.D, tid);
+            vc.store(next + kTile, p.D, tid);
+        }
+        workgroup_barrier();
+    }
+    if (with_table) {
+        // The rows of dS sum to zero but for the error of delta, which the rounding of P and O in the forward leaves in it: the
+        // residue is that error, and P times the residue what it put into dS.  Taken out again here, over the tiles near the diagonal
+        // in a second look at their scores and over all others at once; the column-owned launch gets the right delta.
+        residue = halves_sum(residue);
+        below -= residue * p_below, above -= residue * p_above;
+    }
+    if (split == 0 && h == 0 && qi < p.Lq) p.delta[stat] = delta + residue;
+    const int out_rows = min(max(p.Lq - q0, 0), 32);
+    if (p.splits > 1) {
+        const int64_t all = (int64_t)p.B * p.Hq * p.Lq;
+        store_part<HD>(acc, ok, p.part + (split * all + ((int64_t)b * p.Hq + hq) * p.Lq + q0) * HD, out_rows, lane);
+    } else {
+        store_rows<T, HD>(acc, ok ? p.scale : 0.0f, p.dq.head(b, hq) + (int64_t)q0 * p.dq.sl, p.dq.sl, out_rows,
+                          tiles + wave * 32 * kCtxLd<HD>, lane, p.D);
+    }
+    if (with_table) {
+        if (p.table_type == SJVP_FP32) {
+            // tiles with a key within `far` of a row of the workgroup
+            const int p_first = bt.start + qb * kCtxOwned;
+            const int ta = min(max(p_first - p.far + 1, 0), n) / kCtxTile, tb = (min(max(p_first + kCtxOwned - 1 + p.far, 0), n) + kCtxTile - 1) / kCtxTile;
+            kt = p.k.head(b, hk) + (int64_t)ta * kCtxTile * p.k.sl;
+            for (int t = ta; t < tb; ++t, kt += kCtxTile * p.k.sl) {
+                const int key = t * kCtxTile;
+                workgroup_barrier();
+                kc.load(kt, p.k.sl, n - key, p.D);
+                kc.store(tiles, p.D, tid);
+                workgroup_barrier();
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const int k0 = key + 32 * u;
+                    if (k0 >= n_wave || ctx_band(p, k0 - pos0 - 31, k0 + 31 - pos0) != kNear) continue;
+                    f32x16 s = scores<T, HD>(tiles, 32 * u, own_q, lane);
+                    row_probabilities(s, k0, kNear);
+                    float* at = hist + (k0 + 4 * h - pos + p.far + kCtxPad);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        __hip_atomic_fetch_add(at + 8 * (r >> 2) + (r & 3), -residue * s[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                }
+            }
+        }
+        below = wave_sum(below), above = wave_sum(above);
+        if (lane == 0) hist[0] += below, hist[entries - 1] += above;
+        workgroup_barrier();
+        const float* hists = row + entries;
+        const int nb = p.both ? 2 * p.buckets : p.buckets, zero = p.far + kCtxPad;
+        float* out = p.tpart + (((int64_t)hq * p.B + b) * nqb * p.splits + (int64_t)qb * p.splits + split) * nb;
+        for (int bucket = wave; bucket < nb; bucket += kCtxWaves) {
+            const int side = bucket >= p.buckets, j = bucket - side * p.buckets;
+            const int from = p.first[j], to = j + 1 < p.buckets ? p.first[j + 1] - 1 : zero;  // distances
+            int lo = side ? zero + max(from, 1) : zero - to, hi = side ? zero + to : zero - from;
+            if (!p.both && j == 0) hi = entries - 1;  // differences above zero count as distance 0
+            float sum = 0.0f;
+            for (int x = lo + lane; x <= hi; x += 64)
+#pragma unroll
+                for (int k = 0; k < kCtxWaves; ++k) sum += hists[k * entries + x];
+            sum = wave_sum(sum);
+            if (lane == 0) out[bucket] = sum;
+        }
+    }
+}
+
+// Column-owned: four waves of 32 keys share tiles of 64 query rows, over all heads that read the key head.
+template <typename T, int HD, bool BIAS>
+__global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_col(CtxParams p) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    constexpr int kTile = kCtxTile * kCtxLd<HD>;
+    elem_t* tiles = reinterpret_cast<elem_t*>(smem);                // [2][Q, dO]
+    float* stats = reinterpret_cast<float*>(tiles + 4 * kTile);     // [2][lse, delta][64]
+    float* bias_row = stats + 4 * kCtxTile;
+    const int nkb = p.blocks, entries = ctx_row_entries(p);
+    const CtxWork w = ctx_work(p.B * p.Hkv, nkb * p.splits);
+    if (!w.some) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+    const int split = w.inner / nkb, kb = w.inner % nkb;
+    const int b = w.unit / p.Hkv, hk = w.unit % p.Hkv;
+    const CtxBatch bt(p, b);
+    const int k0 = kb * kCtxOwned + 32 * wave, key = k0 + (lane & 31);
+    const bool ok = key < bt.keys;
+    u32x4 own_k[HD / 16], own_v[HD / 16];
+    own_operands<HD>(own_k, p.k.head(b, hk) + (int64_t)key * p.k.sl, ok, h, p.D);
+    own_operands<HD>(own_v, p.v.head(b, hk) + (int64_t)key * p.v.sl, ok, h, p.D);
+    // tiles of query rows that see a key of the workgroup
+    const int first_row = p.causal ? max(0, kb * kCtxOwned - bt.start) : 0;
+    const int ta = first_row / kCtxTile, tb = (bt.rows + kCtxTile - 1) / kCtxTile;
+    const int per_head = kb * kCtxOwned < bt.keys ? max(0, tb - ta) : 0;
+    const int64_t all = (int64_t)p.G * per_head;
+    const int x0 = (int)(all * split / p.splits), x1 = (int)(all * (split + 1) / p.splits);
+
+    TileCopy<HD> qc(p.q.sl, p.D, tid), gc(p.g.sl, p.D, tid);
+    float stat = 0.0f;
+    const auto load = [&](int x) {
+        const int hq = hk * p.G + x / per_head, r0 = (ta + x % per_head) * kCtxTile;
+        qc.load(p.q.head(b, hq) + (int64_t)r0 * p.q.sl, p.q.sl, bt.rows - r0, p.D);
+        gc.load(p.g.head(b, hq) + (int64_t)r0 * p.g.sl, p.g.sl, bt.rows - r0, p.D);
+        if (tid < 2 * kCtxTile) {
+            const int i = r0 + (tid & (kCtxTile - 1));
+            const float* from = (tid < kCtxTile ? p.lse : p.delta) + ((int64_t)b * p.Hq + hq) * p.Lq;
+            stat = i < bt.rows ? from[i] : tid < kCtxTile ? -INFINITY : 0.0f;
+        }
+    };
+    const auto store = [&](int at) {
+        qc.store(tiles + at * 2 * kTile, p.D, tid);
+        gc.store(tiles + at * 2 * kTile + kTile, p.D, tid);
+        // (a row without keys: its exponentials are zero)
+        if (tid < 2 * kCtxTile) stats[at * 2 * kCtxTile + tid] = tid >= kCtxTile ? stat : stat == -INFINITY ? INFINITY : stat * kLog2e;
+    };
+    if (x0 < x1) {
+        load(x0);
+        store(0);
+    }
+    f32x16 dk[HD / 32] = {}, dv[HD / 32] = {};
+    int head = -1;
+    for (int x = x0; x < x1; ++x) {
+        const int at = (x - x0) & 1, g = x / per_head, r0 = (ta + x % per_head) * kCtxTile;
+        if constexpr (BIAS) {
+            if (g != head) {  // (every wave is behind the barrier of the last tile)
+                head = g;
+                fill_bias_row(p, bias_row, hk * p.G + g, tid, kCtxThreads);
+            }
+        }
+        if (x == x0 || (BIAS && x % per_head == 0)) workgroup_barrier();
+        if (x + 1 < x1) load(x + 1);
+        const elem_t* Q = tiles + at * 2 * kTile;
+        const float* st = stats + at * 2 * kCtxTile;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int q0 = r0 + 32 * u, p0 = bt.start + q0;  // position of the first row
+            if (k0 >= bt.keys || (p.causal && k0 > p0 + 31)) continue;
+            f32x16 s = scores<T, HD>(Q, 32 * u, own_k, lane), ds = scores<T, HD>(Q + kTile, 32 * u, own_v, lane);
+            f32x4 lse[4], delta[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                lse[i] = *reinterpret_cast<const f32x4*>(st + 32 * u + 8 * i + 4 * h);
+                delta[i] = *reinterpret_cast<const f32x4*>(st + kCtxTile + 32 * u + 8 * i + 4 * h);
+            }
+            if constexpr (BIAS) {
+                const CtxBand band = ctx_band(p, k0 - p0 - 31, k0 + 31 - p0);
+                if (band == kNear) {
+                    const float* row = bias_row + (key - p0 - 4 * h + p.far + kCtxPad);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        s[r] = fast_exp2(__builtin_fmaf(s[r], p.c, row[-(8 * (r >> 2) + (r & 3))]) - lse[r >> 2][r & 3]);
+                } else {
+                    const float one = bias_row[band == kBelow ? 0 : entries - 1];
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[r] = fast_exp2(__builtin_fmaf(s[r], p.c, one - lse[r >> 2][r & 3]));
+                }
+            } else {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] = fast_exp2(__builtin_fmaf(s[r], p.c, -lse[r >> 2][r & 3]));
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) ds[r] = s[r] * (ds[r] - delta[r >> 2][r & 3]);
+            if (p.causal && k0 + 31 > p0) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (key > p0 + tile_row(r, h)) s[r] = ds[r] = 0.0f;
+            }
+            add_columns<T, HD>(dv, Q + kTile, 32 * u, s, lane);
+            add_columns<T, HD>(dk, Q, 32 * u, ds, lane);
+        }
+        if (x + 1 < x1) store(1 - at);
+        workgroup_barrier();
+    }
+    const int out_rows = min(max(p.Lk - k0, 0), 32);
+    if (p.splits > 1) {
+        const int64_t rows = (int64_t)p.B * p.Hkv * p.Lk, place = ((int64_t)b * p.Hkv + hk) * p.Lk + k0;
+        store_part<HD>(dk, ok, p.part + (2 * split * rows + place) * HD, out_rows, lane);
+        store_part<HD>(dv, ok, p.part + ((2 * split + 1) * rows + place) * HD, out_rows, lane);
+    } else {
+        elem_t* region = tiles + wave * 32 * kCtxLd<HD>;
+        store_rows<T, HD>(dk, ok ? p.scale : 0.0f, p.dk.head(b, hk) + (int64_t)k0 * p.dk.sl, p.dk.sl, out_rows, region, lane, p.D);
+        store_rows<T, HD>(dv, ok ? 1.0f : 0.0f, p.dv.head(b, hk) + (int64_t)k0 * p.dv.sl, p.dv.sl, out_rows, region, lane, p.D);
+    }
+}
+
+// Adds up the splits of a launch above: one thread to eight columns of a row of dQ, or of dK and dV.
+template <typename T, int HD>
+__global__ __launch_bounds__(kCtxThreads) void ctx_sum(CtxParams p) {
+    constexpr int CH = HD / 8;
+    const bool cols = p.cols;
+    const int H = cols ? p.Hkv : p.Hq, L = cols ? p.Lk : p.Lq, tensors = cols ? 2 : 1;
+    const int64_t rows = (int64_t)p.B * H * L, x = (int64_t)blockIdx.x * kCtxThreads + threadIdx.x, place = x / CH;
+    if (place >= tensors * rows) return;
+    const int c8 = 8 * (int)(x % CH), second = place >= rows;
+    f32x4 a = {}, c = {};
+    for (int s = 0; s < p.splits; ++s) {
+        const float* from = p.part + (s * tensors * rows + place) * HD + c8;
+        a += *reinterpret_cast<const f32x4*>(from);
+        c += *reinterpret_cast<const f32x4*>(from + 4);
+    }
+    const int64_t at = place - second * rows, head = at / L;
+    const CtxView& out = !cols ? p.dq : second ? p.dv : p.dk;
+    const float f = second ? 1.0f : p.scale;
+    const u32x4 y = {T::pack2(a[0] * f, a[1] * f), T::pack2(a[2] * f, a[3] * f), T::pack2(c[0] * f, c[1] * f), T::pack2(c[2] * f, c[3] * f)};
+    store_chunk(out.head((int)(head / H), (int)(head % H)) + (at % L) * out.sl, y, c8, p.D);
+}
+
+}  // namespace sjvp

@@ -1,0 +1,313 @@
+// Forward kernels of the attention on keys of another length / with a relative position bias (sjvp_ctx.hpp).
+#pragma once
+#include "sjvp_ctx.hpp"
+
+namespace sjvp {
+
+// One pass with the running maximum m and sum l of each row.  Scores are in units of log2.  The maximum that the exponentials
+// refer to is only raised when a row's has grown by more than 2^8: until then the sums keep their scale, which 16-bit
+// probabilities up to 2^8 and fp32 sums hold without loss, and the factors of the accumulators stay out of the loop.
+template <typename T, int HD, bool BIAS>
+struct RowSums {
+    f32x16 acc[HD / 32];
+    float m, ref, l;  // maximum (-inf: no key yet), what is subtracted (finite), sum of this lane's half
+
+    __device__ __forceinline__ RowSums() : acc{}, m(-INFINITY), ref(0.0f), l(0.0f) {}
+
+    // s: scores of 32 keys from `key` on.  limit: keys that this lane's row sees; all: every row sees all 32.
+    // row: the bias row of this lane's head; pos, least_pos, most_pos: positions of its query, of the wave's first and last.
+    __device__ __forceinline__ void bias(const CtxParams& p, f32x16& s, int key, int h, const float* row, int pos, int least_pos,
+                                         int most_pos) const {
+        const CtxBand band = ctx_band(p, key - most_pos, key + 31 - least_pos);
+        if (band == kNear) {
+            const float* at = row + (key + 4 * h - pos + p.far + kCtxPad);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], p.c, at[8 * (r >> 2) + (r & 3)]);
+        } else {
+            const float one = row[band == kBelow ? 0 : 2 * (p.far + kCtxPad)];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], p.c, one);
+        }
+    }
+
+    template <int N>
+    __device__ __forceinline__ void exponentials(const CtxParams& p, f32x16 (&s)[N], int key, int limit, bool all, int h) {
+        if (!all) {
+#pragma unroll
+            for (int u = 0; u < N; ++u)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (key + 32 * u + tile_row(r, h) >= limit) s[u][r] = -INFINITY;
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int u = 0; u < N; ++u)
+#pragma unroll
+            for (int r = u ? 0 : 1; r < 16; ++r) top = fmaxf(top, s[u][r]);
+        if constexpr (!BIAS) top *= p.c;
+        if (__builtin_amdgcn_ballot_w64(top > m + 8.0f)) {
+            const float grown = fmaxf(m, halves_max(top));
+            const float now = grown == -INFINITY ? 0.0f : grown;
+            const float f = m == -INFINITY ? 0.0f : fast_exp2(ref - now);
+            m = grown, ref = now;
+            l *= f;
+#pragma unroll
+            for (int dt = 0; dt < HD / 32; ++dt) acc[dt] *= f;
+        }
+        float sum = 0.0f;
+#pragma unroll
+        for (int u = 0; u < N; ++u)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[u][r] = fast_exp2(BIAS ? s[u][r] - ref : __builtin_fmaf(s[u][r], p.c, -ref));
+                sum += s[u][r];
+            }
+        l += sum;
+    }
+};
+
+__device__ __forceinline__ float ctx_lse(float ref, float l) { return (ref + fast_log2(l)) * kLn2; }
+
+// Many rows: four waves of 32 rows of one head share tiles of 64 keys.  Two tiles of K and V in LDS: the next one is on its way
+// through registers while this one is used, one barrier to a tile.
+template <typename T, int HD, bool BIAS>
+__global__ __launch_bounds__(kCtxThreads, 2) void ctx_fwd(CtxParams p) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    constexpr int kTile = kCtxTile * kCtxLd<HD>;
+    elem_t* tiles = reinterpret_cast<elem_t*>(smem);  // [2][K, V]
+    float* row = reinterpret_cast<float*>(tiles + 4 * kTile);
+    const int nqb = p.blocks;
+    const CtxWork w = ctx_work(p.B * p.Hkv, p.G * nqb);
+    if (!w.some) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+    const int b = w.unit / p.Hkv, hk = w.unit % p.Hkv, hq = hk * p.G + w.inner / nqb;
+    const int qb = p.causal ? nqb - 1 - w.inner % nqb : w.inner % nqb;  // causal: long rows first
+    const CtxBatch bt(p, b);
+    const int q0 = qb * kCtxOwned + 32 * wave;
+    const int rows = min(max(bt.rows - q0, 0), 32), last = min(bt.rows, (qb + 1) * kCtxOwned) - 1;
+    const int n = last >= qb * kCtxOwned ? bt.seen(p, last) : 0, n_wave = rows > 0 ? bt.seen(p, q0 + rows - 1) : 0;
+    const int n_all = bt.seen(p, q0), limit = bt.seen(p, q0 + (lane & 31)), pos0 = bt.start + q0, pos = pos0 + (lane & 31);
+
+    u32x4 own[HD / 16];
+    own_operands<HD>(own, p.q.head(b, hq) + (int64_t)(q0 + (lane & 31)) * p.q.sl, (lane & 31) < rows, h, p.D);
+    const elem_t *kt = p.k.head(b, hk), *vt = p.v.head(b, hk);
+    const int nt = (n + kCtxTile - 1) / kCtxTile;
+    TileCopy<HD> kc(p.k.sl, p.D, tid), vc(p.v.sl, p.D, tid);
+    if (nt) {
+        kc.load(kt, p.k.sl, n, p.D);
+        vc.load(vt, p.v.sl, n, p.D);
+    }
+    if constexpr (BIAS) fill_bias_row(p, row, hq, tid, kCtxThreads);
+    if (nt) {
+        kc.store(tiles, p.D, tid);
+        vc.store(tiles + kTile, p.D, tid);
+    }
+    workgroup_barrier();
+    RowSums<T, HD, BIAS> st;
+    for (int t = 0; t < nt; ++t) {
+        const int key = t * kCtxTile;
+        if (t + 1 < nt) {
+            kt += kCtxTile * p.k.sl;
+            vt += kCtxTile * p.v.sl;
+            kc.load(kt, p.k.sl, n - key - kCtxTile, p.D);
+            vc.load(vt, p.v.sl, n - key - kCtxTile, p.D);
+        }
+        if (key < n_wave) {
+            const elem_t* K = tiles + (t & 1) * 2 * kTile;
+            f32x16 s[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                s[u] = scores<T, HD>(K, 32 * u, own, lane);
+                if constexpr (BIAS) st.bias(p, s[u], key + 32 * u, h, row, pos, pos0, pos0 + 31);
+            }
+            st.exponentials(p, s, key, limit, key + kCtxTile <= n_all, h);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) add_columns<T, HD>(st.acc, K + kTile, 32 * u, s[u], lane);
+        }
+        if (t + 1 < nt) {
+            elem_t* next = tiles + ((t + 1) & 1) * 2 * kTile;
+            kc.store(next, p.D, tid);
+            vc.store(next + kTile, p.D, tid);
+        }
+        workgroup_barrier();
+    }
+    const int out_rows = min(max(p.Lq - q0, 0), 32);
+    const float both = halves_sum(st.l), l = (lane & 31) < rows ? both : 0.0f;
+    const float f = l == 0.0f ? 0.0f : 1.0f / l;
+    if (p.lse && h == 0 && (lane & 31) < out_rows)
+        p.lse[((int64_t)b * p.Hq + hq) * p.Lq + q0 + lane] = l == 0.0f ? -INFINITY : ctx_lse(st.ref, l);
+    elem_t* region = tiles + wave * 32 * kCtxLd<HD>;
+    store_rows<T, HD>(st.acc, f, p.o.head(b, hq) + (int64_t)q0 * p.o.sl, p.o.sl, out_rows, region, lane, p.D);
+}
+
+// Few rows: the query rows of all heads that share a key head stand in one block of 32 (row = head of the group * Lq + query), and
+// waves share out the keys: each runs over tiles of 32 keys of its own, K straight from memory into the operand's registers, V through a
+// region of LDS that no other wave reads, so that nothing but the end is synchronised.  The sums of the four waves are
+// joined in LDS; with several splits of the key axis they go to memory for ctx_join.
+// `packed` heads of a group stand in one block's rows: all of them, or one where their bias rows would not fit, or where a head has
+// 32 rows or more (so that the positions in a block lie within 31 of each other).
+template <typename T, int HD, bool BIAS>
+__global__ __launch_bounds__(kCtxThreads, 2) void ctx_fwd_few(CtxParams p) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    constexpr int kRegion = 32 * kCtxLd<HD>, kSum = HD + 4;
+    elem_t* region = reinterpret_cast<elem_t*>(smem);  // [4] V tiles, then the waves' sums [4][32][HD + 4] fp32
+    float* sums = reinterpret_cast<float*>(smem);
+    float* stats = sums + kCtxWaves * 32 * kSum;       // [4][32] maximum, [4][32] sum
+    float* bias_rows = stats + 2 * kCtxWaves * 32;
+    const int packed = p.packed, groups = p.G / packed, all_rows = packed * p.Lq;
+    const CtxWork w = ctx_work(p.B * p.Hkv * groups, p.blocks * p.splits);
+    if (!w.some) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+    const int b = w.unit / (p.Hkv * groups), hu = w.unit % (p.Hkv * groups), hk = hu / groups, hq0 = hu * packed;
+    const int rb = w.inner % p.blocks, split = w.inner / p.blocks;
+    const CtxBatch bt(p, b);
+    const int r0 = rb * 32, rows = min(all_rows - r0, 32), r = r0 + (lane & 31);
+    const int g = min(r, all_rows - 1) / p.Lq, i = min(r, all_rows - 1) % p.Lq, g0 = r0 / p.Lq;
+    const bool mine = r < all_rows && i < bt.rows;
+    // the queries of a block: consecutive ones of one head, or any where it holds the end of one
+    const bool one_head = (r0 + rows - 1) / p.Lq == g0;
+    const int i_first = one_head ? r0 % p.Lq : 0, i_last = one_head ? r0 % p.Lq + rows - 1 : p.Lq - 1;
+    const int n = bt.rows > i_first ? bt.seen(p, min(i_last, bt.rows - 1)) : 0, n_all = bt.seen(p, i_first);
+    const int limit = mine ? bt.seen(p, i) : n, pos = bt.start + i;
+    const int tiles = (n + 31) / 32;
+    const int t_first = (int)((int64_t)tiles * split / p.splits), t_end = (int)((int64_t)tiles * (split + 1) / p.splits);
+
+    u32x4 own[HD / 16];
+    own_operands<HD>(own, p.q.head(b, hq0 + g) + (int64_t)i * p.q.sl, mine, h, p.D);
+    const elem_t *kp = p.k.head(b, hk), *vp = p.v.head(b, hk);
+    constexpr int CH = HD / 8, NV = 32 * CH / 64;
+    u32x4 kr[HD / 16], vr[NV];
+    uint32_t ko[HD / 16], vo[NV];
+#pragma unroll
+    for (int c = 0; c < HD / 16; ++c) ko[c] = chunk_offset(lane & 31, 16 * c + 8 * h, p.k.sl, p.D);
+#pragma unroll
+    for (int x = 0; x < NV; ++x) vo[x] = chunk_offset((lane + 64 * x) / CH, 8 * ((lane + 64 * x) % CH), p.v.sl, p.D);
+    const auto load = [&](int t) {
+        const int key = t * 32;
+        const Rows kf = make_rows(kp + (int64_t)key * p.k.sl, p.k.sl, min(n - key, 32), p.D),
+                   vf = make_rows(vp + (int64_t)key * p.v.sl, p.v.sl, min(n - key, 32), p.D);
+#pragma unroll
+        for (int c = 0; c < HD / 16; ++c) kr[c] = read_chunk(kf, ko[c]);
+#pragma unroll
+        for (int x = 0; x < NV; ++x) vr[x] = read_chunk(vf, vo[x]);
+    };
+    int t = t_first + wave;
+    if (t < t_end) load(t);
+    const float* row = bias_rows;
+    if constexpr (BIAS) {
+        const int entries = ctx_row_entries(p), heads = (r0 + rows - 1) / p.Lq - g0 + 1;
+        for (int x = 0; x < heads; ++x) fill_bias_row(p, bias_rows + x * entries, hq0 + g0 + x, tid, kCtxThreads);
+        row = bias_rows + (g - g0) * entries;
+        workgroup_barrier();
+    }
+    RowSums<T, HD, BIAS> st;
+    elem_t* V = region + wave * kRegion;
+    for (; t < t_end; t += kCtxWaves) {
+#pragma unroll
+        for (int x = 0; x < NV; ++x) {
+            const int at = lane + 64 * x;
+            if (p.D % 8) vr[x] = chunk_shifted(vr[x], 8 * (at % CH), p.D);
+            *reinterpret_cast<u32x4*>(V + (at / CH) * kCtxLd<HD> + 8 * (at % CH)) = vr[x];
+        }
+        if (p.D % 8) {
+#pragma unroll
+            for (int c = 0; c < HD / 16; ++c) kr[c] = chunk_shifted(kr[c], 16 * c + 8 * h, p.D);
+        }
+        f32x16 s[1] = {};
+#pragma unroll
+        for (int c = 0; c < HD / 16; ++c) s[0] = Mma32<T>::run(kr[c], own[c], s[0]);
+        if (t + kCtxWaves < t_end) load(t + kCtxWaves);
+        const int key = t * 32;
+        if constexpr (BIAS) st.bias(p, s[0], key, h, row, pos, bt.start + i_first, bt.start + i_last);
+        st.exponentials(p, s, key, limit, key + 32 <= n_all, h);
+        wave_exchange();
+        add_columns<T, HD>(st.acc, V, 0, s[0], lane);
+        wave_exchange();
+    }
+    const float l = halves_sum(st.l);
+    workgroup_barrier();  // the sums take the place of the V tiles
+    if (h == 0) {
+        stats[wave * 32 + lane] = st.m == -INFINITY ? -INFINITY : st.ref;
+        stats[(kCtxWaves + wave) * 32 + lane] = l;
+    }
+    float* out = sums + (wave * 32 + (lane & 31)) * kSum + 4 * h;
+#pragma unroll
+    for (int dt = 0; dt < HD / 32; ++dt)
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+            *reinterpret_cast<f32x4*>(out + 32 * dt + 8 * x) =
+                f32x4{st.acc[dt][4 * x], st.acc[dt][4 * x + 1], st.acc[dt][4 * x + 2], st.acc[dt][4 * x + 3]};
+    workgroup_barrier();
+    for (int x = tid; x < 32 * CH; x += kCtxThreads) {
+        const int at = x / CH, c8 = 8 * (x % CH), rr = r0 + at;
+        if (at >= rows) break;
+        float top = -INFINITY, sum = 0.0f, y[8] = {};
+#pragma unroll
+        for (int k = 0; k < kCtxWaves; ++k) top = fmaxf(top, stats[k * 32 + at]);
+        const float ref = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+        for (int k = 0; k < kCtxWaves; ++k) {
+            const float f = fast_exp2(stats[k * 32 + at] - ref);
+            sum += f * stats[(kCtxWaves + k) * 32 + at];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] += f * sums[(k * 32 + at) * kSum + c8 + j];
+        }
+        const int gg = rr / p.Lq, ii = rr % p.Lq, hq = hq0 + gg;
+        const int64_t place = ((int64_t)b * p.Hq + hq) * p.Lq + ii;
+        if (ii >= bt.rows) {
+            sum = 0.0f, top = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] = 0.0f;
+        }
+        if (p.splits > 1) {
+            const int64_t part = split * ((int64_t)p.B * p.Hq * p.Lq) + place;
+            if (c8 == 0) p.stat[2 * part] = top, p.stat[2 * part + 1] = sum;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                *reinterpret_cast<f32x4*>(p.part + part * HD + c8 + 4 * j) = f32x4{y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]};
+            continue;
+        }
+        const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+        if (p.lse && c8 == 0) p.lse[place] = sum == 0.0f ? -INFINITY : ctx_lse(ref, sum);
+        u32x4 o;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float a = f == 0.0f ? 0.0f : y[2 * j] * f, c = f == 0.0f ? 0.0f : y[2 * j + 1] * f;
+            o[j] = T::pack2(a, c);
+        }
+        store_chunk(p.o.head(b, hq) + (int64_t)ii * p.o.sl, o, c8, p.D);
+    }
+}
+
+// Joins the splits of ctx_fwd_few: one thread to eight columns of a row.
+template <typename T, int HD>
+__global__ __launch_bounds__(kCtxThreads) void ctx_join(CtxParams p) {
+    constexpr int CH = HD / 8;
+    const int64_t all = (int64_t)p.B * p.Hq * p.Lq, x = (int64_t)blockIdx.x * kCtxThreads + threadIdx.x, place = x / CH;
+    if (place >= all) return;
+    const int c8 = 8 * (int)(x % CH);
+    float top = -INFINITY, sum = 0.0f, y[8] = {};
+    for (int s = 0; s < p.splits; ++s) top = fmaxf(top, p.stat[2 * (s * all + place)]);
+    const float ref = top == -INFINITY ? 0.0f : top;
+    for (int s = 0; s < p.splits; ++s) {
+        const int64_t part = s * all + place;
+        const float f = fast_exp2(p.stat[2 * part] - ref);
+        sum += f * p.stat[2 * part + 1];
+        const f32x4 a = *reinterpret_cast<const f32x4*>(p.part + part * HD + c8), c = *reinterpret_cast<const f32x4*>(p.part + part * HD + c8 + 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] += f * a[j], y[4 + j] += f * c[j];
+    }
+    const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+    if (p.lse && c8 == 0) p.lse[place] = sum == 0.0f ? -INFINITY : ctx_lse(ref, sum);
+    u32x4 o;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float a = f == 0.0f ? 0.0f : y[2 * j] * f, c = f == 0.0f ? 0.0f : y[2 * j + 1] * f;
+        o[j] = T::pack2(a, c);
+    }
+    const int64_t head = place / p.Lq;
+    const int i = (int)(place % p.Lq), hq = (int)(head % p.Hq), b = (int)(head / p.Hq);
+    store_chunk(p.o.head(b, hq) + (int64_t)i * p.o.sl, o, c8, p.D);
+}
+
+}  // namespace sjvp

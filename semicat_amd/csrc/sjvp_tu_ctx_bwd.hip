@@ -1,0 +1,26 @@
+// Translation unit: backward kernels of the attention on keys of another length for one element type (SJVP_T).
+#include <type_traits>
+
+#include "sjvp_ctx_bwd.hpp"
+#include "sjvp_ctx_launch.hpp"
+
+namespace sjvp {
+
+template <>
+int ctx_backward<SJVP_T>(CtxParams p, const CtxPlan& plan, bool row, hipStream_t stream) {
+    p.blocks = plan.blocks, p.splits = plan.splits, p.cols = !row;
+    const int grid = (int)ctx_grid((int)plan.units, (int)plan.inner);
+    return ctx_by_head(p.D, [&](auto hd) {
+        constexpr int HD = decltype(hd)::value;
+        int rc;
+        if (row) rc = p.table ? launch(ctx_bwd_row<SJVP_T, HD, true>, grid, plan.smem, stream, p, kCtxThreads)
+                              : launch(ctx_bwd_row<SJVP_T, HD, false>, grid, plan.smem, stream, p, kCtxThreads);
+        else rc = p.table ? launch(ctx_bwd_col<SJVP_T, HD, true>, grid, plan.smem, stream, p, kCtxThreads)
+                          : launch(ctx_bwd_col<SJVP_T, HD, false>, grid, plan.smem, stream, p, kCtxThreads);
+        if (rc != SJVP_OK || p.splits == 1) return rc;
+        const int64_t rows = row ? (int64_t)p.B * p.Hq * p.Lq : 2 * (int64_t)p.B * p.Hkv * p.Lk;
+        return launch(ctx_sum<SJVP_T, HD>, (int)((rows * (HD / 8) + kCtxThreads - 1) / kCtxThreads), 0, stream, p, kCtxThreads);
+    });
+}
+
+}  // namespace sjvp
