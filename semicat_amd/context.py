@@ -20,7 +20,7 @@ import torch.autograd.forward_ad as fwAD
 from torch import Tensor
 
 from . import _lib
-from .kernels import _scale_arg
+from .kernels import _host_result, _on_gpu, _scale_arg
 
 _DTYPES = {torch.bfloat16: _lib.SJVP_BF16, torch.float16: _lib.SJVP_FP16}
 _TABLE_DTYPES = {torch.bfloat16: _lib.SJVP_BF16, torch.float16: _lib.SJVP_FP16, torch.float32: _lib.SJVP_FP32}
@@ -44,6 +44,15 @@ def relative_bucket_starts(buckets: int, max_distance: int = 128) -> Tuple[int, 
             d += 1
         starts.append(d)
     return tuple(starts)
+
+
+@functools.lru_cache(maxsize=64)
+def _packed_starts(rows: int, max_distance: int, bidirectional: bool) -> bytes:
+    """The first distances as the host extension takes them, for a table of that many rows."""
+    if bidirectional and rows % 2:
+        raise ValueError(f"two directions share an even number of buckets, got {rows}")
+    starts = relative_bucket_starts(rows // 2 if bidirectional else rows, max_distance)
+    return bytes((ctypes.c_int32 * len(starts))(*starts))
 
 
 class RelativeBias:
@@ -175,7 +184,7 @@ def context_backward(q: Tensor, k: Tensor, v: Tensor, o: Tensor, lse: Tensor, dO
     ``(dq, dk, dv, dtable)``.  ``with_keys=False`` leaves out dk and dv (frozen states), ``with_table=False`` the table's."""
     _check_inputs(q, k, v, bias, key_lengths, query_lengths, query_start)
     B, H, Lq, D = q.shape
-    if dO.stride(-1) != 1:
+    if dO.stride(-1) != 1 or dO.stride(2) >= 1 << 24:
         dO = dO.contiguous()
     for name, t in (("o", o), ("dO", dO)):
         _check(name, t, q.shape, q)
@@ -225,7 +234,7 @@ class ContextAttentionBackwardFunction(torch.autograd.Function):
     """Gradients of q, k, v and the table for the cotangent of the output."""
 
     @staticmethod
-    def forward(ctx, q, k, v, table, o, lse, d_o, key_lengths, query_lengths, query_start, scale, max_distance,
+    def forward(q, k, v, table, o, lse, d_o, key_lengths, query_lengths, query_start, scale, max_distance,
                 bidirectional, causal, with_keys, with_table):
         bias = None if table is None else RelativeBias(table, max_distance, bidirectional, causal)
         heads = [None if t is None else t.transpose(1, 2) for t in (q, k, v, o, d_o)]
@@ -234,12 +243,21 @@ class ContextAttentionBackwardFunction(torch.autograd.Function):
         return *(None if t is None else t.transpose(1, 2) for t in (dq, dk, dv)), dtable
 
     @staticmethod
+    def setup_context(ctx, inputs, output) -> None:
+        pass
+
+    @staticmethod
     def backward(ctx, *grads):
         raise NotImplementedError("double backward of the context attention ops is not implemented")
 
 
 def _attend(q, k, v, table, key_lengths, query_lengths, query_start, scale, max_distance=128, bidirectional=True,
             causal=False) -> Tensor:
+    if _on_gpu(q):
+        first = None if table is None or table.ndim != 2 else _packed_starts(table.shape[0], max_distance, bool(bidirectional))
+        o = _lib.host().context(q, k, v, table, key_lengths, query_lengths, query_start, scale, first, bool(bidirectional), bool(causal))
+        if o is not None:
+            return _host_result(o)
     for t in (q, k, v, table):
         if t is not None and fwAD.unpack_dual(t).tangent is not None:
             raise NotImplementedError("forward mode of the context attention ops is not implemented")

@@ -154,7 +154,8 @@ CtxLayout ctx_layout(CtxParams& p, bool backward) {
     l.delta = take(q_rows);
     if (p.dtable) l.tpart = take((size_t)p.Hq * p.B * l.row.blocks * l.row.splits * (p.both ? 2 : 1) * p.buckets);
     // (the row-owned launch's sums are used up before the column-owned one writes its own)
-    const size_t row = l.row.splits > 1 ? l.row.splits * q_rows * HD : 0, col = l.col.splits > 1 ? 2 * l.col.splits * k_rows * HD : 0;
+    const size_t row = l.row.splits > 1 ? 2 * l.row.splits * q_rows * HD : 0, col = l.col.splits > 1 ? 2 * l.col.splits * k_rows * HD : 0;
+    l.stat = take(l.row.splits > 1 ? l.row.splits * q_rows : 0);
     l.part = take(std::max(row, col));
     return l;
 }
@@ -204,7 +205,7 @@ int sjvp_ctx_bwd(const sjvp_ctx* t, int dtype, void* stream) {
     if (!ctx_fits(l.row) || !ctx_fits(l.col)) return SJVP_ERR_SHAPE;
     float* ws;
     if (ctx_workspace(t, l, ws) != SJVP_OK) return SJVP_ERR_WORKSPACE;
-    p.delta = ws + l.delta, p.part = ws + l.part, p.tpart = p.dtable ? ws + l.tpart : nullptr;
+    p.delta = ws + l.delta, p.stat = ws + l.stat, p.part = ws + l.part, p.tpart = p.dtable ? ws + l.tpart : nullptr;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     const auto run = [&](const CtxPlan& plan, bool row) {
         return dtype == SJVP_BF16 ? ctx_backward<Bf16>(p, plan, row, s) : ctx_backward<Fp16>(p, plan, row, s);

@@ -51,7 +51,7 @@ struct CtxView {
 struct CtxParams {
     CtxView q, k, v, o, g, dq, dk, dv;       // g: the cotangent of o
     float *lse, *delta;                      // [B,Hq,Lq]
-    float *part, *stat;                      // sums of split work: rows of HD floats; their (maximum, sum) pairs
+    float *part, *stat;                      // sums of split work: rows of HD floats; their (maximum, sum) pairs or residues
     float* tpart;                            // bucket sums of each workgroup
     void* dtable;
     const void* table;
@@ -63,7 +63,6 @@ struct CtxParams {
     int buckets, both, causal, far;          // buckets of a direction; far: the first distance of the last one
     int splits, blocks;                      // splits of the looped axis; workgroups of a split over the owned axis
     int packed;                              // ctx_fwd_few: heads to a block of rows
-    int cols;                                // ctx_sum: dK and dV, not dQ
     uint16_t first[kCtxBuckets];             // first distance of each bucket
 };
 
@@ -302,6 +301,22 @@ __device__ __forceinline__ void add_columns(f32x16* acc, const elem_t* tile, int
 #pragma unroll
         for (int dt = 0; dt < HD / 32; ++dt)
             acc[dt] = Mma32<T>::run(tile_columns<HD>(tile, row0 + 16 * m, dt, lane), b, acc[dt]);
+    }
+}
+
+// The same of two score tiles, which share the reads.
+template <typename T, int HD>
+__device__ __forceinline__ void add_columns(f32x16* acc0, f32x16* acc1, const elem_t* tile, int row0, const f32x16& s0,
+                                            const f32x16& s1, int lane) {
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+        const u32x4 b0 = pack_scores<T>(s0, m), b1 = pack_scores<T>(s1, m);
+#pragma unroll
+        for (int dt = 0; dt < HD / 32; ++dt) {
+            const u32x4 a = tile_columns<HD>(tile, row0 + 16 * m, dt, lane);
+            acc0[dt] = Mma32<T>::run(a, b0, acc0[dt]);
+            acc1[dt] = Mma32<T>::run(a, b1, acc1[dt]);
+        }
     }
 }
 

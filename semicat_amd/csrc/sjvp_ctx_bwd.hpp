@@ -3,7 +3,7 @@
 //   dP = dO V^T,  delta = rowsum(dO * O),  dS = P (dP - delta)
 //   dQ = scale dS K,  dK = scale sum_heads dS^T Q,  dV = sum_heads P^T dO,  dtable[bucket][head] = sum of dS over its differences
 //
-// A row-owned launch (dQ, delta and the bucket sums) and a column-owned one (dK, dV), both of which recompute P: 3 + 4
+// A row-owned launch (dQ, delta and the bucket sums) and a column-owned one (dK, dV), both of which recompute P: 4 + 4
 // contractions against the 5 of a single launch, whose dQ would be summed by atomics in an order that changes from run to run.
 #pragma once
 #include "sjvp_ctx.hpp"
@@ -61,7 +61,7 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_row(Ctx
     const int64_t stat = ((int64_t)b * p.Hq + hq) * p.Lq + qi;
     float lse = -INFINITY;
     if ((lane & 31) < rows) lse = p.lse[stat];
-    const bool ok = lse != -INFINITY;  // a row that sees no key has no gradient
+    const bool ok = lse != -INFINITY && limit != 1;  // no gradient of the scores of a row that sees no key, or one alone
     lse = ok ? lse * kLog2e : INFINITY;
     u32x4 own_q[HD / 16], own_g[HD / 16];
     own_operands<HD>(own_q, p.q.head(b, hq) + (int64_t)qi * p.q.sl, ok, h, p.D);
@@ -99,7 +99,7 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_row(Ctx
                 if (k0 + tile_row(r, h) >= limit) s[r] = 0.0f;
         }
     };
-    f32x16 acc[HD / 32] = {};
+    f32x16 acc[HD / 32] = {}, mean[HD / 32] = {};  // dS K, P K
     float below = 0.0f, above = 0.0f;    // sums of dS beyond the last single distance,
     float p_below = 0.0f, p_above = 0.0f;  // and of P there
     float residue = 0.0f;                  // sum of dS over the row
@@ -121,11 +121,14 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_row(Ctx
             row_probabilities(s, k0, band);
 #pragma unroll
             for (int r = 0; r < 16; ++r) ds[r] = s[r] * (ds[r] - delta);
-            if (with_table) {
-                float sum = 0.0f, p_sum = 0.0f;
+            float sum = 0.0f;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) sum += ds[r], p_sum += s[r];
-                residue += sum;
+            for (int r = 0; r < 16; ++r) sum += ds[r];
+            residue += sum;
+            if (with_table) {
+                float p_sum = 0.0f;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) p_sum += s[r];
                 if (band == kNear) {
                     // one wave's own sums, whose order of addition is the order of its instructions
                     float* at = hist + (k0 + 4 * h - pos + p.far + kCtxPad);
@@ -138,7 +141,7 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_row(Ctx
                     above += sum, p_above += p_sum;
                 }
             }
-            add_columns<T, HD>(acc, K, 32 * u, ds, lane);
+            add_columns<T, HD>(acc, mean, K, 32 * u, ds, s, lane);
         }
         if (t + 1 < t1) {
             elem_t* next = tiles + (1 - at) * 2 * kTile;
@@ -147,48 +150,51 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_row(Ctx
         }
         workgroup_barrier();
     }
-    if (with_table) {
-        // The rows of dS sum to zero but for the error of delta, which the rounding of P and O in the forward leaves in it: the
-        // residue is that error, and P times the residue what it put into dS.  Taken out again here, over the tiles near the diagonal
-        // in a second look at their scores and over all others at once; the column-owned launch gets the right delta.
-        residue = halves_sum(residue);
-        below -= residue * p_below, above -= residue * p_above;
-    }
-    if (split == 0 && h == 0 && qi < p.Lq) p.delta[stat] = delta + residue;
+    // The rows of dS sum to zero but for the error of delta, which the rounding of P and O in the forward leaves in it (2^-9 of it
+    // for bf16; of a sharp row's dS more than that).  So the residue is that error, and P times the residue what it put into dS:
+    // taken out of dQ here, of the bucket sums below, and the column-owned launch gets the right delta.  (ctx_sum_rows does it for
+    // splits, which know a part of the residue each.)
+    residue = halves_sum(residue);
     const int out_rows = min(max(p.Lq - q0, 0), 32);
     if (p.splits > 1) {
-        const int64_t all = (int64_t)p.B * p.Hq * p.Lq;
-        store_part<HD>(acc, ok, p.part + (split * all + ((int64_t)b * p.Hq + hq) * p.Lq + q0) * HD, out_rows, lane);
+        const int64_t all = (int64_t)p.B * p.Hq * p.Lq, place = ((int64_t)b * p.Hq + hq) * p.Lq + q0;
+        store_part<HD>(acc, ok, p.part + (2 * split * all + place) * HD, out_rows, lane);
+        store_part<HD>(mean, ok, p.part + ((2 * split + 1) * all + place) * HD, out_rows, lane);
+        if (h == 0 && qi < p.Lq) {
+            p.stat[split * all + stat] = residue;
+            if (split == 0) p.delta[stat] = delta;
+        }
     } else {
+#pragma unroll
+        for (int dt = 0; dt < HD / 32; ++dt) acc[dt] -= residue * mean[dt];
+        if (h == 0 && qi < p.Lq) p.delta[stat] = delta + residue;
         store_rows<T, HD>(acc, ok ? p.scale : 0.0f, p.dq.head(b, hq) + (int64_t)q0 * p.dq.sl, p.dq.sl, out_rows,
                           tiles + wave * 32 * kCtxLd<HD>, lane, p.D);
     }
     if (with_table) {
-        if (p.table_type == SJVP_FP32) {
-            // tiles with a key within `far` of a row of the workgroup
-            const int p_first = bt.start + qb * kCtxOwned;
-            const int ta = min(max(p_first - p.far + 1, 0), n) / kCtxTile, tb = (min(max(p_first + kCtxOwned - 1 + p.far, 0), n) + kCtxTile - 1) / kCtxTile;
-            kt = p.k.head(b, hk) + (int64_t)ta * kCtxTile * p.k.sl;
-            for (int t = ta; t < tb; ++t, kt += kCtxTile * p.k.sl) {
-                const int key = t * kCtxTile;
-                workgroup_barrier();
-                kc.load(kt, p.k.sl, n - key, p.D);
-                kc.store(tiles, p.D, tid);
-                workgroup_barrier();
+        // tiles with a key within `far` of a row of the workgroup
+        const int p_first = bt.start + qb * kCtxOwned;
+        const int ta = min(max(p_first - p.far + 1, 0), n) / kCtxTile, tb = (min(max(p_first + kCtxOwned - 1 + p.far, 0), n) + kCtxTile - 1) / kCtxTile;
+        kt = p.k.head(b, hk) + (int64_t)ta * kCtxTile * p.k.sl;
+        for (int t = ta; t < tb; ++t, kt += kCtxTile * p.k.sl) {
+            const int key = t * kCtxTile;
+            workgroup_barrier();
+            kc.load(kt, p.k.sl, n - key, p.D);
+            kc.store(tiles, p.D, tid);
+            workgroup_barrier();
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const int k0 = key + 32 * u;
-                    if (k0 >= n_wave || ctx_band(p, k0 - pos0 - 31, k0 + 31 - pos0) != kNear) continue;
-                    f32x16 s = scores<T, HD>(tiles, 32 * u, own_q, lane);
-                    row_probabilities(s, k0, kNear);
-                    float* at = hist + (k0 + 4 * h - pos + p.far + kCtxPad);
+            for (int u = 0; u < 2; ++u) {
+                const int k0 = key + 32 * u;
+                if (k0 >= n_wave || ctx_band(p, k0 - pos0 - 31, k0 + 31 - pos0) != kNear) continue;
+                f32x16 s = scores<T, HD>(tiles, 32 * u, own_q, lane);
+                row_probabilities(s, k0, kNear);
+                float* at = hist + (k0 + 4 * h - pos + p.far + kCtxPad);
 #pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        __hip_atomic_fetch_add(at + 8 * (r >> 2) + (r & 3), -residue * s[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-                }
+                for (int r = 0; r < 16; ++r)
+                    __hip_atomic_fetch_add(at + 8 * (r >> 2) + (r & 3), -residue * s[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
             }
         }
-        below = wave_sum(below), above = wave_sum(above);
+        below = wave_sum(below - residue * p_below), above = wave_sum(above - residue * p_above);
         if (lane == 0) hist[0] += below, hist[entries - 1] += above;
         workgroup_barrier();
         const float* hists = row + entries;
@@ -303,9 +309,13 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_col(Ctx
             for (int r = 0; r < 16; ++r) ds[r] = s[r] * (ds[r] - delta[r >> 2][r & 3]);
             if (p.causal && k0 + 31 > p0) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (key > p0 + tile_row(r, h)) s[r] = ds[r] = 0.0f;
+                for (int r = 0; r < 16; ++r) {
+                    const int seen = p0 + tile_row(r, h) + 1;
+                    if (key >= seen) s[r] = 0.0f;
+                    if (key >= seen || seen == 1) ds[r] = 0.0f;  // (a row that sees one key has no gradient of its score)
+                }
             }
+            if (bt.keys == 1) ds = f32x16{};
             add_columns<T, HD>(dv, Q + kTile, 32 * u, s, lane);
             add_columns<T, HD>(dk, Q, 32 * u, ds, lane);
         }
@@ -324,26 +334,50 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_col(Ctx
     }
 }
 
-// Adds up the splits of a launch above: one thread to eight columns of a row of dQ, or of dK and dV.
+// Adds up the splits of the row-owned launch: one thread to eight columns of a row of dQ.
 template <typename T, int HD>
-__global__ __launch_bounds__(kCtxThreads) void ctx_sum(CtxParams p) {
+__global__ __launch_bounds__(kCtxThreads) void ctx_sum_rows(CtxParams p) {
     constexpr int CH = HD / 8;
-    const bool cols = p.cols;
-    const int H = cols ? p.Hkv : p.Hq, L = cols ? p.Lk : p.Lq, tensors = cols ? 2 : 1;
-    const int64_t rows = (int64_t)p.B * H * L, x = (int64_t)blockIdx.x * kCtxThreads + threadIdx.x, place = x / CH;
-    if (place >= tensors * rows) return;
+    const int64_t rows = (int64_t)p.B * p.Hq * p.Lq, x = (int64_t)blockIdx.x * kCtxThreads + threadIdx.x, place = x / CH;
+    if (place >= rows) return;
+    const int c8 = 8 * (int)(x % CH);
+    f32x4 a[4] = {};  // dS K, P K
+    float residue = 0.0f;
+    for (int s = 0; s < p.splits; ++s) {
+        residue += p.stat[s * rows + place];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            a[i] += *reinterpret_cast<const f32x4*>(p.part + ((2 * s + i / 2) * rows + place) * HD + c8 + 4 * (i % 2));
+    }
+    if (c8 == 0) p.delta[place] += residue;
+    u32x4 y;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const f32x4 d = (a[i] - residue * a[2 + i]) * p.scale;
+        y[2 * i] = T::pack2(d[0], d[1]), y[2 * i + 1] = T::pack2(d[2], d[3]);
+    }
+    const int64_t head = place / p.Lq;
+    store_chunk(p.dq.head((int)(head / p.Hq), (int)(head % p.Hq)) + (place % p.Lq) * p.dq.sl, y, c8, p.D);
+}
+
+// The same for the column-owned one: dK and dV.
+template <typename T, int HD>
+__global__ __launch_bounds__(kCtxThreads) void ctx_sum_cols(CtxParams p) {
+    constexpr int CH = HD / 8;
+    const int64_t rows = (int64_t)p.B * p.Hkv * p.Lk, x = (int64_t)blockIdx.x * kCtxThreads + threadIdx.x, place = x / CH;
+    if (place >= 2 * rows) return;
     const int c8 = 8 * (int)(x % CH), second = place >= rows;
     f32x4 a = {}, c = {};
     for (int s = 0; s < p.splits; ++s) {
-        const float* from = p.part + (s * tensors * rows + place) * HD + c8;
+        const float* from = p.part + (s * 2 * rows + place) * HD + c8;
         a += *reinterpret_cast<const f32x4*>(from);
         c += *reinterpret_cast<const f32x4*>(from + 4);
     }
-    const int64_t at = place - second * rows, head = at / L;
-    const CtxView& out = !cols ? p.dq : second ? p.dv : p.dk;
+    const int64_t at = place - second * rows, head = at / p.Lk;
+    const CtxView& out = second ? p.dv : p.dk;
     const float f = second ? 1.0f : p.scale;
     const u32x4 y = {T::pack2(a[0] * f, a[1] * f), T::pack2(a[2] * f, a[3] * f), T::pack2(c[0] * f, c[1] * f), T::pack2(c[2] * f, c[3] * f)};
-    store_chunk(out.head((int)(head / H), (int)(head % H)) + (at % L) * out.sl, y, c8, p.D);
+    store_chunk(out.head((int)(head / p.Hkv), (int)(head % p.Hkv)) + (at % p.Lk) * out.sl, y, c8, p.D);
 }
 
 }  // namespace sjvp

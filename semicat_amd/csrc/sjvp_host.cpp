@@ -37,6 +37,9 @@ struct Abi {
     decltype(&sjvp_adaln_workspace_floats) adaln_workspace_floats = nullptr;
     decltype(&sjvp_gelu) gelu = nullptr;
     decltype(&sjvp_rope) rope = nullptr;
+    decltype(&sjvp_ctx_fwd) ctx_fwd = nullptr;
+    decltype(&sjvp_ctx_bwd) ctx_bwd = nullptr;
+    decltype(&sjvp_ctx_workspace_bytes) ctx_workspace_bytes = nullptr;
 };
 Abi abi;  // filled once by bind() when the library is loaded
 
@@ -560,11 +563,214 @@ PyObject* gelu(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// The options of a context attention call beside its differentiable tensors.
+struct ContextOptions {
+    int start0 = 0, both = 0, causal = 0;
+    float scale = 0.0f;
+    std::string first;  // int32 first distances of the buckets
+    Tensor klen, qlen, start;  // or undefined
+};
+
+constexpr int64_t kMostStride = 1 << 24;  // of an input's sequence axis
+
+int type_tag(at::ScalarType t) { return t == at::kFloat ? SJVP_FP32 : t == at::kBFloat16 ? SJVP_BF16 : t == at::kHalf ? SJVP_FP16 : -1; }
+
+// The C ABI's struct for [B,S,H,D] tensors; the table may be undefined.
+sjvp_ctx context_struct(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& table, const ContextOptions& options) {
+    sjvp_ctx t{};
+    t.B = static_cast<int>(q.size(0)), t.Lq = static_cast<int>(q.size(1)), t.Hq = static_cast<int>(q.size(2)), t.D = static_cast<int>(q.size(3));
+    t.Lk = static_cast<int>(k.size(1)), t.Hkv = static_cast<int>(k.size(2));
+    t.q = q.data_ptr(), t.k = k.data_ptr(), t.v = v.data_ptr();
+    const auto indices = [](const Tensor& x) { return x.defined() ? static_cast<const int32_t*>(x.data_ptr()) : nullptr; };
+    t.key_lengths = indices(options.klen), t.query_lengths = indices(options.qlen), t.query_start = indices(options.start);
+    t.query_start0 = options.start0, t.scale = options.scale;
+    if (table.defined()) {
+        t.table = table.data_ptr(), t.table_dtype = type_tag(table.scalar_type());
+        t.table_stride[0] = table.stride(0), t.table_stride[1] = table.stride(1);
+        t.buckets = static_cast<int>(options.first.size() / sizeof(int32_t));
+        t.bucket_first = reinterpret_cast<const int32_t*>(options.first.data());
+        t.bidirectional = options.both, t.causal = options.causal;
+    }
+    return t;
+}
+
+void context_strides(sjvp_ctx& t, int at, const Tensor& x) {  // [B,S,H,D] as (batch, head, sequence)
+    t.strides[3 * at] = x.stride(0), t.strides[3 * at + 1] = x.stride(2), t.strides[3 * at + 2] = x.stride(1);
+}
+
+int context_run(sjvp_ctx& t, const Tensor& q, bool backward) {
+    const Tensor workspace = [&] {
+        t.workspace_bytes = abi.ctx_workspace_bytes(&t, backward);
+        return t.workspace_bytes ? Maker{q.device()}({static_cast<int64_t>(t.workspace_bytes)}, at::kByte) : Tensor();
+    }();
+    t.workspace = workspace.defined() ? workspace.data_ptr() : nullptr;
+    void* stream = c10::hip::getCurrentHIPStream(q.device().index()).stream();
+    return (backward ? abi.ctx_bwd : abi.ctx_fwd)(&t, type_tag(q.scalar_type()), stream);
+}
+
+void context_check(int status) { TORCH_CHECK(status == SJVP_OK, "sjvp status ", status, " from the context attention kernels"); }
+
+Tensor context_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& table, const ContextOptions& options, Tensor* lse,
+                       int& status) {
+    const c10::DeviceGuard guard(q.device());
+    const Maker make_tensor{q.device()};
+    Tensor o = make_tensor({q.size(0), q.size(1), q.size(2), q.size(3)}, q.scalar_type());
+    sjvp_ctx t = context_struct(q, k, v, table, options);
+    if (lse) {
+        *lse = make_tensor({q.size(0), q.size(2), q.size(1)}, at::kFloat);
+        t.lse = static_cast<float*>(lse->data_ptr());
+    }
+    t.o = o.data_ptr();
+    context_strides(t, SJVP_C_Q, q);
+    context_strides(t, SJVP_C_K, k);
+    context_strides(t, SJVP_C_V, v);
+    context_strides(t, SJVP_C_O, o);
+    status = context_run(t, q, false);
+    return o;
+}
+
+// Results of a backward that a graph is being made of: whoever goes through that graph is told that there is no second derivative.
+struct NoSecondDerivative : torch::autograd::Function<NoSecondDerivative> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext*, const Tensor&, const Tensor&, const Tensor&,
+                                                  const std::optional<Tensor>&, const Tensor&, torch::autograd::variable_list* grads) {
+        return std::move(*grads);
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext*, torch::autograd::variable_list) {
+        TORCH_CHECK_NOT_IMPLEMENTED(false, "double backward of the context attention ops is not implemented");
+    }
+};
+
+struct ContextNode : torch::autograd::Function<ContextNode> {
+    static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v,
+                          const std::optional<Tensor>& table, const ContextOptions* options) {
+        Tensor lse;
+        int status;
+        Tensor o = context_forward(q, k, v, table.value_or(Tensor()), *options, &lse, status);
+        context_check(status);
+        ctx->save_for_backward({q, k, v, table.value_or(Tensor()), options->klen, options->qlen, options->start, o, lse});
+        ctx->saved_data["options"] = c10::IValue(std::vector<int64_t>{options->start0, options->both, options->causal});
+        ctx->saved_data["scale"] = static_cast<double>(options->scale);
+        ctx->saved_data["first"] = options->first;
+        ctx->set_materialize_grads(false);
+        return o;
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list cotangents) {
+        torch::autograd::variable_list grads(5);
+        if (!cotangents[0].defined()) return grads;
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &table = saved[3], &o = saved[7], &lse = saved[8];
+        const std::vector<int64_t> ints = ctx->saved_data["options"].toIntVector();
+        const ContextOptions options{static_cast<int>(ints[0]), static_cast<int>(ints[1]), static_cast<int>(ints[2]),
+                                     static_cast<float>(ctx->saved_data["scale"].toDouble()), ctx->saved_data["first"].toStringRef(),
+                                     saved[4], saved[5], saved[6]};
+        const bool record = at::GradMode::is_enabled();
+        {
+            const at::NoGradGuard no_grad;
+            const c10::DeviceGuard guard(q.device());
+            const Tensor g = cotangents[0].stride(3) == 1 && cotangents[0].stride(1) < kMostStride ? cotangents[0] : cotangents[0].contiguous();
+            const Maker make_tensor{q.device()};
+            sjvp_ctx t = context_struct(q, k, v, table, options);
+            t.lse = static_cast<float*>(lse.data_ptr());
+            t.o = o.data_ptr(), t.dO = g.data_ptr();
+            grads[0] = make_tensor(q.sizes(), q.scalar_type());
+            t.dq = grads[0].data_ptr();
+            const Tensor* at[] = {&q, &k, &v, &o, &g, &grads[0], &grads[1], &grads[2]};
+            if (ctx->needs_input_grad(1) || ctx->needs_input_grad(2)) {
+                grads[1] = make_tensor(k.sizes(), k.scalar_type());
+                grads[2] = make_tensor(v.sizes(), v.scalar_type());
+                t.dk = grads[1].data_ptr(), t.dv = grads[2].data_ptr();
+            }
+            for (int i = 0; i < SJVP_C_COUNT; ++i)
+                if (at[i]->defined()) context_strides(t, i, *at[i]);
+            if (table.defined() && ctx->needs_input_grad(3)) {
+                grads[3] = make_tensor(table.sizes(), table.scalar_type());
+                t.dtable = grads[3].data_ptr();
+                t.dtable_stride[0] = grads[3].stride(0), t.dtable_stride[1] = grads[3].stride(1);
+            }
+            context_check(context_run(t, q, true));
+        }
+        if (record) {
+            torch::autograd::variable_list made;
+            for (int i = 0; i < 4; ++i)
+                if (grads[i].defined()) made.push_back(grads[i]);
+            made = NoSecondDerivative::apply(q, k, v, table.defined() ? std::optional<Tensor>(table) : std::nullopt, cotangents[0], &made);
+            for (int i = 0, n = 0; i < 4; ++i)
+                if (grads[i].defined()) grads[i] = made[n++];
+        }
+        for (int i = 0; i < 4; ++i)
+            if (grads[i].defined() && !ctx->needs_input_grad(i)) grads[i] = Tensor();
+        return grads;
+    }
+};
+
+// context(q, k, v, table, key_lengths, query_lengths, query_start, scale, first distances, bidirectional, causal) -> output:
+// [B,S,H,D] tensors; table with its first distances (bytes of int32), lengths and scale may be None, query_start is an int or a tensor
+PyObject* context(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 11 || !abi.ctx_fwd) return none();
+    const Tensor* in[3];
+    for (int i = 0; i < 3; ++i) {
+        in[i] = plain(a[i]);
+        if (!in[i] || in[i]->dim() != 4 || in[i]->stride(3) != 1 || in[i]->scalar_type() != in[0]->scalar_type() ||
+            in[i]->device() != in[0]->device() || in[i]->numel() == 0 || in[i]->stride(1) >= kMostStride || in[i]->_fw_grad(0).defined())
+            return none();
+        for (int d = 0; d < 4; ++d)
+            if (in[i]->size(d) > INT_MAX) return none();
+    }
+    const Tensor &q = *in[0], &k = *in[1], &v = *in[2];
+    if ((q.scalar_type() != at::kBFloat16 && q.scalar_type() != at::kHalf) || k.sizes() != v.sizes() || k.size(0) != q.size(0) ||
+        k.size(3) != q.size(3) || q.size(2) % k.size(2) || q.size(3) < 16 || q.size(3) > 128)
+        return none();
+    ContextOptions options;
+    Tensor table;
+    Tensor* const indices[] = {&options.klen, &options.qlen, &options.start};
+    for (int i = 0; i < 3; ++i) {
+        if (a[4 + i] == Py_None) continue;
+        if (i == 2 && PyLong_CheckExact(a[6])) {
+            const long start = PyLong_AsLong(a[6]);
+            if (PyErr_Occurred() || start < -(1 << 29) || start > 1 << 29) {
+                PyErr_Clear();
+                return none();
+            }
+            options.start0 = static_cast<int>(start);
+            continue;
+        }
+        const Tensor* x = plain(a[4 + i]);
+        if (!x || x->dim() != 1 || x->size(0) != q.size(0) || x->scalar_type() != at::kInt || x->device() != q.device() || !x->is_contiguous())
+            return none();
+        *indices[i] = *x;
+    }
+    options.scale = scale_arg(a[7]);
+    if (options.scale < 0.0f || (a[9] != Py_True && a[9] != Py_False) || (a[10] != Py_True && a[10] != Py_False)) return none();
+    if (a[3] != Py_None) {
+        const Tensor* x = plain(a[3]);
+        if (!x || !PyBytes_CheckExact(a[8]) || x->dim() != 2 || x->size(1) != q.size(2) || x->device() != q.device() ||
+            type_tag(x->scalar_type()) < 0 || x->_fw_grad(0).defined())
+            return none();
+        table = *x;
+        options.first.assign(PyBytes_AS_STRING(a[8]), static_cast<size_t>(PyBytes_GET_SIZE(a[8])));
+        options.both = a[9] == Py_True, options.causal = a[10] == Py_True;
+        if (static_cast<int64_t>(options.first.size() / sizeof(int32_t)) * (options.both ? 2 : 1) != table.size(0)) return none();
+    }
+    Tensor o;
+    int status = SJVP_OK;
+    {
+        pybind11::gil_scoped_release no_gil;
+        const bool record = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() ||
+                                                           (table.defined() && table.requires_grad()));
+        if (record) o = ContextNode::apply(q, k, v, table.defined() ? std::optional<Tensor>(table) : std::nullopt, &options);
+        else o = context_forward(q, k, v, table, options, nullptr, status);
+    }
+    if (status != SJVP_OK) return PyLong_FromLong(status);
+    return THPVariable_Wrap(std::move(o));
+    END_HANDLE_TH_ERRORS
+}
+
 // bind(addresses of the entry points, in the order of Abi)
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
-    constexpr int kEntries = 11;
+    constexpr int kEntries = 14;
     if (n != kEntries) {
-        PyErr_SetString(PyExc_TypeError, "bind() takes eleven addresses");
+        PyErr_SetString(PyExc_TypeError, "bind() takes fourteen addresses");
         return nullptr;
     }
     void* p[kEntries];
@@ -587,7 +793,10 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
            reinterpret_cast<decltype(abi.adaln_bwd)>(p[7]),
            reinterpret_cast<decltype(abi.adaln_workspace_floats)>(p[8]),
            reinterpret_cast<decltype(abi.gelu)>(p[9]),
-           reinterpret_cast<decltype(abi.rope)>(p[10])};
+           reinterpret_cast<decltype(abi.rope)>(p[10]),
+           reinterpret_cast<decltype(abi.ctx_fwd)>(p[11]),
+           reinterpret_cast<decltype(abi.ctx_bwd)>(p[12]),
+           reinterpret_cast<decltype(abi.ctx_workspace_bytes)>(p[13])};
     return none();
 }
 
@@ -603,6 +812,7 @@ PyMethodDef methods[] = {
     {"adaln", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(adaln)), METH_FASTCALL, nullptr},
     {"gelu", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(gelu)), METH_FASTCALL, nullptr},
     {"rope", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rope)), METH_FASTCALL, nullptr},
+    {"context", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(context)), METH_FASTCALL, nullptr},
     {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(bind)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 

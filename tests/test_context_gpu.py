@@ -2,10 +2,10 @@
 
 Tolerances, element by element.  Each contraction rounds one of its operands (P or dS) to 16 bits and its result once more, by at
 most half a step each, u = eps/2 of the type relative to the value.  With a = sum |p||v| (and the like for the gradients) that is
-u a + u |result|.  delta = dO.o is taken from the rounded o, which adds u b, b = |sum p k| sum |dO||o| scale and the like (the
-oracle gives a, b).  What float32 contractions of up to 128 products, the exponentials and the reduction over the keys add
-is bounded by 2^-14 (a + b).  fp16 numbers below 2^-14 are rounded in steps of 2^-24: 2^-25 c + 2^-25, c = sum |v| and the like.
-The float32 table's gradient rounds nothing to 16 bits (delta's error is taken out again): 2^-15 a."""
+u a + u |result|.  What float32 contractions of up to 128 products, the exponentials and the reduction over the keys add
+is bounded by 2^-14 (a + b), b = |sum p k| sum |dO||o| scale and the like: what a relative error of delta = dO.o would
+do, whose 16-bit part the kernels take out again, but for its products' own rounding, u^2 b.  fp16 numbers below 2^-14 are rounded in steps of 2^-24: 2^-25 c + 2^-25, c = sum |v| and the like.
+The float32 table's gradient rounds nothing to 16 bits either: 2^-15 a."""
 import pytest
 import torch
 
@@ -54,7 +54,7 @@ def check(got, x, **options):
             if t.dtype != torch.float32:  # delta from the rounded o
                 limit += u * a
         else:
-            limit = (u + 2.0 ** -14) * (a + b) + u * want[name].abs()
+            limit = u * a + (u * u + 2.0 ** -14) * (a + b) + u * want[name].abs()
         if x["q"].dtype == FP16:
             limit += 2.0 ** -25 * (1.0 + c)
         off = (t.cpu().double() - want[name]).abs()
@@ -120,6 +120,20 @@ def test_positions(start, Lq, Lk, both, causal):
     x = make(2, 2, 1, Lq, Lk, 32, BF16, table=(12, torch.float32))
     options = dict(max_distance=50, bidirectional=both, causal=causal, query_start=start)
     check(run(x, **options), x, **options)
+
+
+@pytest.mark.parametrize("relative", [False, True])
+def test_rows_that_see_one_key_have_no_score_gradient(relative):
+    """Exactly none: whoever divides by the gradient's norm sees it.  The value's gradient is the cotangent."""
+    x = make(2, 4, 2, 5, 1, 64, BF16, table=(8, torch.float32) if relative else None)
+    got = run(x)
+    assert all(got[n].eq(0).all() for n in got if n not in ("o", "dv"))
+    check({n: got[n] for n in ("o", "dv")}, x)
+    if relative:  # the first row of a causal sequence
+        x = make(2, 4, 2, 1, 7, 64, BF16, table=(8, torch.float32))
+        got = run(x, max_distance=5, bidirectional=False, causal=True)
+        assert all(got[n].eq(0).all() for n in ("dq", "dk", "dtable"))
+        check(got, x, max_distance=5, bidirectional=False, causal=True)
 
 
 def test_masking_entries_of_the_table():
@@ -328,3 +342,48 @@ def test_double_backward_and_forward_mode_are_refused():
         g.sum().backward()
     with pytest.raises(NotImplementedError):
         torch.func.jvp(lambda t: cross_attention(t, t, t), (q.detach(),), (q.detach(),))
+
+
+def test_ctypes_path_gives_the_same_bits(monkeypatch):
+    from semicat_amd import _lib
+    x = make(2, 4, 2, 50, 90, 64, BF16, table=(16, torch.float32))
+    options = dict(key_lengths=torch.tensor([70, 90], dtype=torch.int32), query_start=torch.tensor([3, -4], dtype=torch.int32), scale=0.3)
+    first = run(x, **options)
+    plain = run({n: t for n, t in x.items() if n != "table"})
+    monkeypatch.setattr(_lib, "_host", False)
+    for a, b in ((first, run(x, **options)), (plain, run({n: t for n, t in x.items() if n != "table"}))):
+        assert all(torch.equal(a[n], b[n]) for n in a)
+    q = torch.randn(1, 8, 2, 32, device="cuda", dtype=BF16, requires_grad=True)
+    test_double_backward_and_forward_mode_are_refused()
+    g = torch.func.grad(lambda t: run_sum(t))(q.detach())  # (functorch's wrappers take this path always)
+    monkeypatch.undo()
+    assert torch.equal(g, torch.func.grad(lambda t: run_sum(t))(q.detach()))
+    assert torch.equal(g, torch.autograd.grad(run_sum(q), q)[0])
+
+
+def run_sum(t):
+    from semicat_amd import cross_attention
+    return cross_attention(t, t, t).float().sum()
+
+
+def test_other_types_are_computed_in_bfloat16():
+    from semicat_amd import cross_attention
+    x = make(1, 2, 1, 20, 30, 64, BF16)
+    q, k, v = (x[n].float().cuda().requires_grad_() for n in "qkv")
+    o = cross_attention(q, k, v)
+    g = torch.autograd.grad(o, (q, k, v), x["dO"].float().cuda())
+    want = run(x)
+    assert o.dtype == torch.float32 and torch.equal(o, want["o"].float())
+    assert all(a.dtype == torch.float32 and torch.equal(a, want[n].float()) for a, n in zip(g, ("dq", "dk", "dv")))
+
+
+def test_strides_that_are_not_served():
+    from semicat_amd import _lib, cross_attention
+    buf = torch.zeros((1 << 24) + 64, device="cuda", dtype=BF16)
+    far = buf.as_strided((1, 2, 1, 32), (1 << 25, 1 << 24, 32, 1))
+    with pytest.raises(_lib.SjvpError):
+        cross_attention(far, far, far)
+    q = torch.randn(1, 2, 1, 32, device="cuda", dtype=BF16, requires_grad=True)
+    (got,) = torch.autograd.grad(cross_attention(q, q, q), q, far + 1)
+    g = far.copy_(torch.randn(1, 2, 1, 32, device="cuda"))
+    assert torch.equal(torch.autograd.grad(cross_attention(q, q, q), q, g)[0], torch.autograd.grad(cross_attention(q, q, q), q, g.contiguous())[0])
