@@ -56,13 +56,14 @@ CtxPlan ctx_plan_fwd(const CtxParams& p) {
         plan.smem = ctx_tiles_bytes(HD) + bias;
         return plan;
     }
-    const int sums = kCtxWaves * 32 * (HD + 4 + 2) * 4;
     const int heads = p.Lq < 32 ? std::min(p.G, 31 / p.Lq + 2) : 1;  // that a block of 32 rows can touch
-    plan.packed = p.Lq < 32 && sums + heads * bias <= kLds ? p.G : 1;
-    plan.smem = sums + (plan.packed > 1 ? heads : 1) * bias;
+    const auto sums = [&](int waves) { return waves * 32 * (HD + 4 + 2) * 4; };
+    plan.waves = p.Lk >= 256 && sums(8) + heads * bias <= kLds ? 8 : 4;
+    plan.packed = p.Lq < 32 && sums(plan.waves) + heads * bias <= kLds ? p.G : 1;
+    plan.smem = sums(plan.waves) + (plan.packed > 1 ? heads : 1) * bias;
     plan.blocks = (int)ceil_div((int64_t)plan.packed * p.Lq, 32);
     plan.units = (int64_t)p.B * p.Hkv * (p.G / plan.packed);
-    plan.splits = splits_for(plan.units * plan.blocks, p.Lk, 2, 256);
+    plan.splits = splits_for(plan.units * plan.blocks, p.Lk, 1, 256);
     plan.inner = (int64_t)plan.blocks * plan.splits;
     return plan;
 }
@@ -75,6 +76,10 @@ CtxPlan ctx_plan_row(const CtxParams& p) {
     plan.splits = p.tpart ? 1 : splits_for((int64_t)p.B * p.Hq * plan.blocks, ceil_div(p.Lk, kCtxTile), 1, 4);
     plan.inner = (int64_t)p.G * plan.blocks * plan.splits;
     plan.smem = ctx_tiles_bytes(ctx_padded(p.D)) + (p.table ? 4 * ctx_entries(p) * (p.tpart ? 1 + kCtxWaves : 1) : 0);
+    if (p.tpart) {
+        plan.skew = (plan.smem + 15) / 16 * 16;
+        plan.smem = plan.skew + 4 * kCtxWaves * kSkewFloats;
+    }
     return plan;
 }
 

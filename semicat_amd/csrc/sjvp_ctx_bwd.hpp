@@ -34,6 +34,24 @@ __device__ __forceinline__ float row_delta(const CtxParams& p, const u32x4* own_
     return halves_sum(sum);
 }
 
+// Sums along the diagonals of a 32 x 32 score tile (one wave's), added to the wave's sums by difference; `at`: entry of the
+// difference -31.  Through LDS: each lane writes its column's values as a row of kSkew floats of which the last 36 are zeros, so that
+// entry d + 31 of a diagonal, read at (kSkew + 1) per row, finds zeros where the diagonal has left the tile.  (LDS atomics
+// on the sums themselves took 190 cycles an instruction: B=64 H=12 L=128 D=64 160 us for the launch, 48 us this way.)
+__device__ __forceinline__ void add_diagonals(float* skew, float* at, const f32x16& x, float factor, int lane) {
+    float* mine = skew + (1 + (lane & 31)) * kSkew + 4 * (lane >> 5);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<f32x4*>(mine + 8 * i) = f32x4{x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]} * factor;
+    wave_exchange();
+    const float* from = skew + kSkew + lane - 31;
+    float sum[4] = {};
+#pragma unroll
+    for (int q = 0; q < 32; ++q) sum[q & 3] += from[q * (kSkew + 1)];
+    if (lane < 63) at[lane] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    wave_exchange();
+}
+
 // Row-owned: four waves of 32 query rows of one head share tiles of 64 keys.
 template <typename T, int HD, bool BIAS>
 __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_row(CtxParams p) {
@@ -56,7 +74,8 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_row(Ctx
     const int nt = (n + kCtxTile - 1) / kCtxTile;
     const int t0 = (int)((int64_t)nt * split / p.splits), t1 = (int)((int64_t)nt * (split + 1) / p.splits);
     const bool with_table = BIAS && p.tpart;
-    float* hist = row + entries + wave * entries;
+    float* hist = row + entries + wave * entries;  // the wave's sums of dS by difference
+    float* skew = reinterpret_cast<float*>(smem + p.skew) + wave * kSkewFloats;
 
     const int64_t stat = ((int64_t)b * p.Hq + hq) * p.Lq + qi;
     float lse = -INFINITY;
@@ -80,6 +99,8 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_row(Ctx
         fill_bias_row(p, row, hq, tid, kCtxThreads);
         if (with_table)
             for (int x = lane; x < entries; x += 64) hist[x] = 0.0f;
+        if (with_table)
+            for (int x = lane; x < kSkewFloats; x += 64) skew[x] = 0.0f;
     }
     workgroup_barrier();
     // scores of 32 keys from k0 on to P, zero where hidden
@@ -130,11 +151,7 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_row(Ctx
 #pragma unroll
                 for (int r = 0; r < 16; ++r) p_sum += s[r];
                 if (band == kNear) {
-                    // one wave's own sums, whose order of addition is the order of its instructions
-                    float* at = hist + (k0 + 4 * h - pos + p.far + kCtxPad);
-#pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        __hip_atomic_fetch_add(at + 8 * (r >> 2) + (r & 3), ds[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                    add_diagonals(skew, hist + (k0 - pos0 - 31 + p.far + kCtxPad), ds, 1.0f, lane);
                 } else if (band == kBelow) {
                     below += sum, p_below += p_sum;
                 } else {
@@ -188,10 +205,7 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_row(Ctx
                 if (k0 >= n_wave || ctx_band(p, k0 - pos0 - 31, k0 + 31 - pos0) != kNear) continue;
                 f32x16 s = scores<T, HD>(tiles, 32 * u, own_q, lane);
                 row_probabilities(s, k0, kNear);
-                float* at = hist + (k0 + 4 * h - pos + p.far + kCtxPad);
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    __hip_atomic_fetch_add(at + 8 * (r >> 2) + (r & 3), -residue * s[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                add_diagonals(skew, hist + (k0 - pos0 - 31 + p.far + kCtxPad), s, -residue, lane);
             }
         }
         below = wave_sum(below - residue * p_below), above = wave_sum(above - residue * p_above);

@@ -142,18 +142,18 @@ __global__ __launch_bounds__(kCtxThreads, 2) void ctx_fwd(CtxParams p) {
 
 // Few rows: the query rows of all heads that share a key head stand in one block of 32 (row = head of the group * Lq + query), and
 // waves share out the keys: each runs over tiles of 32 keys of its own, K straight from memory into the operand's registers, V through a
-// region of LDS that no other wave reads, so that nothing but the end is synchronised.  The sums of the four waves are
+// region of LDS that no other wave reads, so that nothing but the end is synchronised.  The sums of the waves are
 // joined in LDS; with several splits of the key axis they go to memory for ctx_join.
 // `packed` heads of a group stand in one block's rows: all of them, or one where their bias rows would not fit, or where a head has
 // 32 rows or more (so that the positions in a block lie within 31 of each other).
-template <typename T, int HD, bool BIAS>
-__global__ __launch_bounds__(kCtxThreads, 2) void ctx_fwd_few(CtxParams p) {
+template <typename T, int HD, bool BIAS, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void ctx_fwd_few(CtxParams p) {
     extern __shared__ __align__(16) unsigned char smem[];
     constexpr int kRegion = 32 * kCtxLd<HD>, kSum = HD + 4;
-    elem_t* region = reinterpret_cast<elem_t*>(smem);  // [4] V tiles, then the waves' sums [4][32][HD + 4] fp32
+    elem_t* region = reinterpret_cast<elem_t*>(smem);  // [WAVES] V tiles, then the waves' sums [WAVES][32][HD + 4] fp32
     float* sums = reinterpret_cast<float*>(smem);
-    float* stats = sums + kCtxWaves * 32 * kSum;       // [4][32] maximum, [4][32] sum
-    float* bias_rows = stats + 2 * kCtxWaves * 32;
+    float* stats = sums + WAVES * 32 * kSum;       // [WAVES][32] maximum, then sum
+    float* bias_rows = stats + 2 * WAVES * 32;
     const int packed = p.packed, groups = p.G / packed, all_rows = packed * p.Lq;
     const CtxWork w = ctx_work(p.B * p.Hkv * groups, p.blocks * p.splits);
     if (!w.some) return;
@@ -196,13 +196,13 @@ __global__ __launch_bounds__(kCtxThreads, 2) void ctx_fwd_few(CtxParams p) {
     const float* row = bias_rows;
     if constexpr (BIAS) {
         const int entries = ctx_row_entries(p), heads = (r0 + rows - 1) / p.Lq - g0 + 1;
-        for (int x = 0; x < heads; ++x) fill_bias_row(p, bias_rows + x * entries, hq0 + g0 + x, tid, kCtxThreads);
+        for (int x = 0; x < heads; ++x) fill_bias_row(p, bias_rows + x * entries, hq0 + g0 + x, tid, 64 * WAVES);
         row = bias_rows + (g - g0) * entries;
         workgroup_barrier();
     }
     RowSums<T, HD, BIAS> st;
     elem_t* V = region + wave * kRegion;
-    for (; t < t_end; t += kCtxWaves) {
+    for (; t < t_end; t += WAVES) {
 #pragma unroll
         for (int x = 0; x < NV; ++x) {
             const int at = lane + 64 * x;
@@ -216,7 +216,7 @@ __global__ __launch_bounds__(kCtxThreads, 2) void ctx_fwd_few(CtxParams p) {
         f32x16 s[1] = {};
 #pragma unroll
         for (int c = 0; c < HD / 16; ++c) s[0] = Mma32<T>::run(kr[c], own[c], s[0]);
-        if (t + kCtxWaves < t_end) load(t + kCtxWaves);
+        if (t + WAVES < t_end) load(t + WAVES);
         const int key = t * 32;
         if constexpr (BIAS) st.bias(p, s[0], key, h, row, pos, bt.start + i_first, bt.start + i_last);
         st.exponentials(p, s, key, limit, key + 32 <= n_all, h);
@@ -228,7 +228,7 @@ __global__ __launch_bounds__(kCtxThreads, 2) void ctx_fwd_few(CtxParams p) {
     workgroup_barrier();  // the sums take the place of the V tiles
     if (h == 0) {
         stats[wave * 32 + lane] = st.m == -INFINITY ? -INFINITY : st.ref;
-        stats[(kCtxWaves + wave) * 32 + lane] = l;
+        stats[(WAVES + wave) * 32 + lane] = l;
     }
     float* out = sums + (wave * 32 + (lane & 31)) * kSum + 4 * h;
 #pragma unroll
@@ -238,17 +238,17 @@ __global__ __launch_bounds__(kCtxThreads, 2) void ctx_fwd_few(CtxParams p) {
             *reinterpret_cast<f32x4*>(out + 32 * dt + 8 * x) =
                 f32x4{st.acc[dt][4 * x], st.acc[dt][4 * x + 1], st.acc[dt][4 * x + 2], st.acc[dt][4 * x + 3]};
     workgroup_barrier();
-    for (int x = tid; x < 32 * CH; x += kCtxThreads) {
+    for (int x = tid; x < 32 * CH; x += 64 * WAVES) {
         const int at = x / CH, c8 = 8 * (x % CH), rr = r0 + at;
         if (at >= rows) break;
         float top = -INFINITY, sum = 0.0f, y[8] = {};
 #pragma unroll
-        for (int k = 0; k < kCtxWaves; ++k) top = fmaxf(top, stats[k * 32 + at]);
+        for (int k = 0; k < WAVES; ++k) top = fmaxf(top, stats[k * 32 + at]);
         const float ref = top == -INFINITY ? 0.0f : top;
 #pragma unroll
-        for (int k = 0; k < kCtxWaves; ++k) {
+        for (int k = 0; k < WAVES; ++k) {
             const float f = fast_exp2(stats[k * 32 + at] - ref);
-            sum += f * stats[(kCtxWaves + k) * 32 + at];
+            sum += f * stats[(WAVES + k) * 32 + at];
 #pragma unroll
             for (int j = 0; j < 8; ++j) y[j] += f * sums[(k * 32 + at) * kSum + c8 + j];
         }
@@ -279,26 +279,44 @@ __global__ __launch_bounds__(kCtxThreads, 2) void ctx_fwd_few(CtxParams p) {
     }
 }
 
-// Joins the splits of ctx_fwd_few: one thread to eight columns of a row.
+// Joins the splits of ctx_fwd_few: 16 threads to the columns of a row (eight each), `slices` of them to the splits, which meet in
+// LDS.  (One thread over all splits: B=2 H=16 Lq=4 Lk=16385 D=128 in 64 splits 34 us.)
 template <typename T, int HD>
 __global__ __launch_bounds__(kCtxThreads) void ctx_join(CtxParams p) {
-    constexpr int CH = HD / 8;
-    const int64_t all = (int64_t)p.B * p.Hq * p.Lq, x = (int64_t)blockIdx.x * kCtxThreads + threadIdx.x, place = x / CH;
-    if (place >= all) return;
-    const int c8 = 8 * (int)(x % CH);
+    __shared__ float met[kCtxThreads / 16][16][11];
+    const int64_t all = (int64_t)p.B * p.Hq * p.Lq;
+    const int slices = min(16, 1 << (32 - __builtin_clz(p.splits - 1))), group = threadIdx.x >> 4, slice = group % slices;
+    const int64_t place = (int64_t)blockIdx.x * (16 / slices) + group / slices;
+    const int c8 = 8 * (threadIdx.x & 15);
+    const bool some = place < all && c8 < HD;
     float top = -INFINITY, sum = 0.0f, y[8] = {};
-    for (int s = 0; s < p.splits; ++s) top = fmaxf(top, p.stat[2 * (s * all + place)]);
-    const float ref = top == -INFINITY ? 0.0f : top;
-    for (int s = 0; s < p.splits; ++s) {
-        const int64_t part = s * all + place;
-        const float f = fast_exp2(p.stat[2 * part] - ref);
-        sum += f * p.stat[2 * part + 1];
-        const f32x4 a = *reinterpret_cast<const f32x4*>(p.part + part * HD + c8), c = *reinterpret_cast<const f32x4*>(p.part + part * HD + c8 + 4);
+    const auto add = [&](float other_top, float other_sum, const float* other) {
+        const float now = fmaxf(top, other_top), ref = now == -INFINITY ? 0.0f : now, f = fast_exp2(top - ref), g = fast_exp2(other_top - ref);
+        top = now;
+        sum = f * sum + g * other_sum;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) y[j] += f * a[j], y[4 + j] += f * c[j];
+        for (int j = 0; j < 8; ++j) y[j] = f * y[j] + g * other[j];
+    };
+    if (some) {
+        for (int s = slice; s < p.splits; s += slices) {
+            const int64_t part = s * all + place;
+            const f32x4 a = *reinterpret_cast<const f32x4*>(p.part + part * HD + c8), c = *reinterpret_cast<const f32x4*>(p.part + part * HD + c8 + 4);
+            const float other[8] = {a[0], a[1], a[2], a[3], c[0], c[1], c[2], c[3]};
+            add(p.stat[2 * part], p.stat[2 * part + 1], other);
+        }
+    }
+    float* mine = met[group][threadIdx.x & 15];
+    mine[0] = top, mine[1] = sum;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) mine[2 + j] = y[j];
+    workgroup_barrier();
+    if (slice || !some) return;
+    for (int s = 1; s < slices; ++s) {
+        const float* other = met[group + s][threadIdx.x & 15];
+        add(other[0], other[1], other + 2);
     }
     const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
-    if (p.lse && c8 == 0) p.lse[place] = sum == 0.0f ? -INFINITY : ctx_lse(ref, sum);
+    if (p.lse && c8 == 0) p.lse[place] = sum == 0.0f ? -INFINITY : ctx_lse(top, sum);
     u32x4 o;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {

@@ -13,10 +13,11 @@ inline int ctx_tiles_bytes(int HD) { return 4 * kCtxTile * (HD + 8) * 2; }
 // One launch's share of the work: `blocks` over the owned axis, `splits` of the looped one.
 struct CtxPlan {
     bool few = false;      // forward: ctx_fwd_few
-    int packed = 1;        // its heads to a block of rows
+    int packed = 1;        // its heads to a block of rows,
+    int waves = kCtxWaves;  // and waves to a workgroup
     int blocks = 1, splits = 1;
     int64_t units = 1, inner = 1;  // of ctx_work
-    int smem = 0;
+    int smem = 0, skew = 0;
 };
 
 CtxPlan ctx_plan_fwd(const CtxParams& p);

@@ -8,7 +8,7 @@ namespace sjvp {
 
 template <>
 int ctx_backward<SJVP_T>(CtxParams p, const CtxPlan& plan, bool row, hipStream_t stream) {
-    p.blocks = plan.blocks, p.splits = plan.splits;
+    p.blocks = plan.blocks, p.splits = plan.splits, p.skew = plan.skew;
     const int grid = (int)ctx_grid((int)plan.units, (int)plan.inner);
     return ctx_by_head(p.D, [&](auto hd) {
         constexpr int HD = decltype(hd)::value;

@@ -15,11 +15,17 @@ int ctx_forward<SJVP_T>(CtxParams p, const CtxPlan& plan, hipStream_t stream) {
         if (!plan.few) return p.table ? launch(ctx_fwd<SJVP_T, HD, true>, grid, plan.smem, stream, p, kCtxThreads)
                                       : launch(ctx_fwd<SJVP_T, HD, false>, grid, plan.smem, stream, p, kCtxThreads);
         p.packed = plan.packed;
-        const int rc = p.table ? launch(ctx_fwd_few<SJVP_T, HD, true>, grid, plan.smem, stream, p, kCtxThreads)
-                               : launch(ctx_fwd_few<SJVP_T, HD, false>, grid, plan.smem, stream, p, kCtxThreads);
+        const auto few = [&](auto waves) {
+            constexpr int W = decltype(waves)::value;
+            return p.table ? launch(ctx_fwd_few<SJVP_T, HD, true, W>, grid, plan.smem, stream, p, 64 * W)
+                           : launch(ctx_fwd_few<SJVP_T, HD, false, W>, grid, plan.smem, stream, p, 64 * W);
+        };
+        const int rc = plan.waves == 8 ? few(std::integral_constant<int, 8>{}) : few(std::integral_constant<int, 4>{});
         if (rc != SJVP_OK || p.splits == 1) return rc;
-        const int64_t threads = (int64_t)p.B * p.Hq * p.Lq * (HD / 8);
-        return launch(ctx_join<SJVP_T, HD>, (int)((threads + kCtxThreads - 1) / kCtxThreads), 0, stream, p, kCtxThreads);
+        int slices = 1;  // as in the kernel
+        while (slices < p.splits && slices < 16) slices *= 2;
+        const int64_t rows = (int64_t)p.B * p.Hq * p.Lq, per = 16 / slices;
+        return launch(ctx_join<SJVP_T, HD>, (int)((rows + per - 1) / per), 0, stream, p, kCtxThreads);
     });
 }
 
