@@ -15,6 +15,8 @@
 // bits, are the B operand of the next contraction under the numbering  k = 8h + i  <->  y = 16m + 8*(i/4) + 4h + i%4  (h = l/32);
 // A in that numbering is what two transposing LDS reads of four rows deliver.
 #pragma once
+#include <type_traits>
+
 #include "sjvp_device.hpp"
 #include "../../include/sjvp.h"
 
@@ -208,13 +210,15 @@ __device__ __forceinline__ float ctx_table(const CtxParams& p, int bucket, int h
 
 __device__ __forceinline__ int ctx_row_entries(const CtxParams& p) { return 2 * (p.far + kCtxPad) + 1; }
 
-// The bias of a head by position difference, entry far + pad for difference 0, in units of log2.  A difference of a 32 x 32
+// The bias of a head by position difference, entry far + pad for difference 0, in units of log2; -inf for keys behind a causal query,
+// so that the kernels need no other mask for these.  A difference of a 32 x 32
 // tile that is not wholly beyond `far` lies within far + 62, so the padding saves the tiles a clamp.  A table entry near
 // the lowest float32 would leave the range with the factor log2(e); it is raised to -2.3e38, still below any score.
 __device__ __forceinline__ void fill_bias_row(const CtxParams& p, float* row, int head, int tid, int threads) {
     for (int x = tid; x < ctx_row_entries(p); x += threads) {
-        const float t = ctx_table(p, ctx_bucket(p, x - p.far - kCtxPad), head);
-        row[x] = t == -INFINITY ? t : fmaxf(t, -2.3e38f) * kLog2e;
+        const int rel = x - p.far - kCtxPad;
+        const float t = ctx_table(p, ctx_bucket(p, rel), head);
+        row[x] = t == -INFINITY || (p.causal && rel > 0) ? -INFINITY : fmaxf(t, -2.3e38f) * kLog2e;
     }
 }
 
@@ -224,6 +228,8 @@ struct CtxBatch {
         : keys(p.klen ? min(max(p.klen[b], 0), p.Lk) : p.Lk),
           rows(p.qlen ? min(max(p.qlen[b], 0), p.Lq) : p.Lq),
           start(min(max(p.start ? p.start[b] : 0, -kCtxMost), kCtxMost) + p.start0) {}
+    // whether some row sees more than one key: otherwise the scores have no gradient at all
+    __device__ __forceinline__ bool any_scored(const CtxParams& p) const { return keys != 1 && !(p.causal && start + rows <= 1); }
     // keys that the row sees
     __device__ __forceinline__ int seen(const CtxParams& p, int row) const {
         return p.causal ? max(0, min(keys, start + row + 1)) : keys;

@@ -70,7 +70,7 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_row(Ctx
     const int q0 = qb * kCtxOwned + 32 * wave, qi = q0 + (lane & 31);
     const int rows = min(max(bt.rows - q0, 0), 32), last = min(bt.rows, (qb + 1) * kCtxOwned) - 1;
     const int n = last >= qb * kCtxOwned ? bt.seen(p, last) : 0, n_wave = rows > 0 ? bt.seen(p, q0 + rows - 1) : 0;
-    const int n_all = bt.seen(p, q0), limit = bt.seen(p, qi), pos0 = bt.start + q0, pos = pos0 + (lane & 31);
+    const int limit = bt.seen(p, qi), pos0 = bt.start + q0, pos = pos0 + (lane & 31);
     const int nt = (n + kCtxTile - 1) / kCtxTile;
     const int t0 = (int)((int64_t)nt * split / p.splits), t1 = (int)((int64_t)nt * (split + 1) / p.splits);
     const bool with_table = BIAS && p.tpart;
@@ -80,7 +80,8 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_row(Ctx
     const int64_t stat = ((int64_t)b * p.Hq + hq) * p.Lq + qi;
     float lse = -INFINITY;
     if ((lane & 31) < rows) lse = p.lse[stat];
-    const bool ok = lse != -INFINITY && limit != 1;  // no gradient of the scores of a row that sees no key, or one alone
+    const bool ok = lse != -INFINITY;           // a row that sees no key has no gradient,
+    const bool scored = ok && limit != 1;       // one that sees one key none of its score: exactly none, not what rounding leaves
     lse = ok ? lse * kLog2e : INFINITY;
     u32x4 own_q[HD / 16], own_g[HD / 16];
     own_operands<HD>(own_q, p.q.head(b, hq) + (int64_t)qi * p.q.sl, ok, h, p.D);
@@ -104,7 +105,7 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_row(Ctx
     }
     workgroup_barrier();
     // scores of 32 keys from k0 on to P, zero where hidden
-    const auto row_probabilities = [&](f32x16& s, int k0, CtxBand band) {
+    const auto row_probabilities = [&](f32x16& s, int k0, CtxBand band, bool masked) {
         if (BIAS && band == kNear) {
             const float* at = row + (k0 + 4 * h - pos + p.far + kCtxPad);
 #pragma unroll
@@ -114,17 +115,18 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_row(Ctx
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = fast_exp2(__builtin_fmaf(s[r], p.c, one));
         }
-        if (k0 + 32 > n_all) {
+        if (masked) {
 #pragma unroll
             for (int r = 0; r < 16; ++r)
-                if (k0 + tile_row(r, h) >= limit) s[r] = 0.0f;
+                if (tile_row(r, 0) >= bt.keys - k0 - 4 * h) s[r] = 0.0f;
         }
     };
     f32x16 acc[HD / 32] = {}, mean[HD / 32] = {};  // dS K, P K
     float below = 0.0f, above = 0.0f;    // sums of dS beyond the last single distance,
     float p_below = 0.0f, p_above = 0.0f;  // and of P there
     float residue = 0.0f;                  // sum of dS over the row
-    for (int t = t0; t < t1; ++t) {
+    // (the sequence's last tile with its mask in code of its own, as in the forward)
+    const auto tile = [&](int t, bool masked) {
         const int key = t * kCtxTile, at = (t - t0) & 1;
         if (t + 1 < t1) {
             kt += kCtxTile * p.k.sl;
@@ -139,7 +141,7 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_row(Ctx
             if (k0 >= n_wave) continue;
             f32x16 s = scores<T, HD>(K, 32 * u, own_q, lane), ds = scores<T, HD>(K + kTile, 32 * u, own_g, lane);
             const CtxBand band = BIAS ? ctx_band(p, k0 - pos0 - 31, k0 + 31 - pos0) : kNear;
-            row_probabilities(s, k0, band);
+            row_probabilities(s, k0, band, masked);
 #pragma unroll
             for (int r = 0; r < 16; ++r) ds[r] = s[r] * (ds[r] - delta);
             float sum = 0.0f;
@@ -166,7 +168,10 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_row(Ctx
             vc.store(next + kTile, p.D, tid);
         }
         workgroup_barrier();
-    }
+    };
+    const int whole = max(t0, min(t1, bt.keys / kCtxTile));
+    for (int t = t0; t < whole; ++t) tile(t, false);
+    if (whole < t1) tile(whole, true);
     // The rows of dS sum to zero but for the error of delta, which the rounding of P and O in the forward leaves in it (2^-9 of it
     // for bf16; of a sharp row's dS more than that).  So the residue is that error, and P times the residue what it put into dS:
     // taken out of dQ here, of the bucket sums below, and the column-owned launch gets the right delta.  (ctx_sum_rows does it for
@@ -175,8 +180,8 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_row(Ctx
     const int out_rows = min(max(p.Lq - q0, 0), 32);
     if (p.splits > 1) {
         const int64_t all = (int64_t)p.B * p.Hq * p.Lq, place = ((int64_t)b * p.Hq + hq) * p.Lq + q0;
-        store_part<HD>(acc, ok, p.part + (2 * split * all + place) * HD, out_rows, lane);
-        store_part<HD>(mean, ok, p.part + ((2 * split + 1) * all + place) * HD, out_rows, lane);
+        store_part<HD>(acc, scored, p.part + (2 * split * all + place) * HD, out_rows, lane);
+        store_part<HD>(mean, scored, p.part + ((2 * split + 1) * all + place) * HD, out_rows, lane);
         if (h == 0 && qi < p.Lq) {
             p.stat[split * all + stat] = residue;
             if (split == 0) p.delta[stat] = delta;
@@ -185,7 +190,7 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_row(Ctx
 #pragma unroll
         for (int dt = 0; dt < HD / 32; ++dt) acc[dt] -= residue * mean[dt];
         if (h == 0 && qi < p.Lq) p.delta[stat] = delta + residue;
-        store_rows<T, HD>(acc, ok ? p.scale : 0.0f, p.dq.head(b, hq) + (int64_t)q0 * p.dq.sl, p.dq.sl, out_rows,
+        store_rows<T, HD>(acc, scored ? p.scale : 0.0f, p.dq.head(b, hq) + (int64_t)q0 * p.dq.sl, p.dq.sl, out_rows,
                           tiles + wave * 32 * kCtxLd<HD>, lane, p.D);
     }
     if (with_table) {
@@ -204,7 +209,7 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_row(Ctx
                 const int k0 = key + 32 * u;
                 if (k0 >= n_wave || ctx_band(p, k0 - pos0 - 31, k0 + 31 - pos0) != kNear) continue;
                 f32x16 s = scores<T, HD>(tiles, 32 * u, own_q, lane);
-                row_probabilities(s, k0, kNear);
+                row_probabilities(s, k0, kNear, k0 + 32 > bt.keys);
                 add_diagonals(skew, hist + (k0 - pos0 - 31 + p.far + kCtxPad), s, -residue, lane);
             }
         }
@@ -224,7 +229,7 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_row(Ctx
 #pragma unroll
                 for (int k = 0; k < kCtxWaves; ++k) sum += hists[k * entries + x];
             sum = wave_sum(sum);
-            if (lane == 0) out[bucket] = sum;
+            if (lane == 0) out[bucket] = bt.any_scored(p) ? sum : 0.0f;
         }
     }
 }
@@ -321,29 +326,21 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_col(Ctx
             }
 #pragma unroll
             for (int r = 0; r < 16; ++r) ds[r] = s[r] * (ds[r] - delta[r >> 2][r & 3]);
-            if (p.causal && k0 + 31 > p0) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int seen = p0 + tile_row(r, h) + 1;
-                    if (key >= seen) s[r] = 0.0f;
-                    if (key >= seen || seen == 1) ds[r] = 0.0f;  // (a row that sees one key has no gradient of its score)
-                }
-            }
-            if (bt.keys == 1) ds = f32x16{};
             add_columns<T, HD>(dv, Q + kTile, 32 * u, s, lane);
             add_columns<T, HD>(dk, Q, 32 * u, ds, lane);
         }
         if (x + 1 < x1) store(1 - at);
         workgroup_barrier();
     }
+    const bool scored = ok && bt.any_scored(p);
     const int out_rows = min(max(p.Lk - k0, 0), 32);
     if (p.splits > 1) {
         const int64_t rows = (int64_t)p.B * p.Hkv * p.Lk, place = ((int64_t)b * p.Hkv + hk) * p.Lk + k0;
-        store_part<HD>(dk, ok, p.part + (2 * split * rows + place) * HD, out_rows, lane);
+        store_part<HD>(dk, scored, p.part + (2 * split * rows + place) * HD, out_rows, lane);
         store_part<HD>(dv, ok, p.part + ((2 * split + 1) * rows + place) * HD, out_rows, lane);
     } else {
         elem_t* region = tiles + wave * 32 * kCtxLd<HD>;
-        store_rows<T, HD>(dk, ok ? p.scale : 0.0f, p.dk.head(b, hk) + (int64_t)k0 * p.dk.sl, p.dk.sl, out_rows, region, lane, p.D);
+        store_rows<T, HD>(dk, scored ? p.scale : 0.0f, p.dk.head(b, hk) + (int64_t)k0 * p.dk.sl, p.dk.sl, out_rows, region, lane, p.D);
         store_rows<T, HD>(dv, ok ? 1.0f : 0.0f, p.dv.head(b, hk) + (int64_t)k0 * p.dv.sl, p.dv.sl, out_rows, region, lane, p.D);
     }
 }

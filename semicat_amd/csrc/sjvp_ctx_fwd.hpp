@@ -14,7 +14,7 @@ struct RowSums {
 
     __device__ __forceinline__ RowSums() : acc{}, m(-INFINITY), ref(0.0f), l(0.0f) {}
 
-    // s: scores of 32 keys from `key` on.  limit: keys that this lane's row sees; all: every row sees all 32.
+    // s: scores of 32 keys from `key` on.
     // row: the bias row of this lane's head; pos, least_pos, most_pos: positions of its query, of the wave's first and last.
     __device__ __forceinline__ void bias(const CtxParams& p, f32x16& s, int key, int h, const float* row, int pos, int least_pos,
                                          int most_pos) const {
@@ -30,14 +30,15 @@ struct RowSums {
         }
     }
 
+    // left: the sequence's keys from `key` on, where they do not fill the scores (masked).
     template <int N>
-    __device__ __forceinline__ void exponentials(const CtxParams& p, f32x16 (&s)[N], int key, int limit, bool all, int h) {
-        if (!all) {
+    __device__ __forceinline__ void exponentials(const CtxParams& p, f32x16 (&s)[N], int left, int h, bool masked) {
+        if (masked) {
 #pragma unroll
             for (int u = 0; u < N; ++u)
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    if (key + 32 * u + tile_row(r, h) >= limit) s[u][r] = -INFINITY;
+                    if (32 * u + tile_row(r, 0) >= left - 4 * h) s[u][r] = -INFINITY;
         }
         float top = s[0][0];
 #pragma unroll
@@ -86,7 +87,7 @@ __global__ __launch_bounds__(kCtxThreads, 2) void ctx_fwd(CtxParams p) {
     const int q0 = qb * kCtxOwned + 32 * wave;
     const int rows = min(max(bt.rows - q0, 0), 32), last = min(bt.rows, (qb + 1) * kCtxOwned) - 1;
     const int n = last >= qb * kCtxOwned ? bt.seen(p, last) : 0, n_wave = rows > 0 ? bt.seen(p, q0 + rows - 1) : 0;
-    const int n_all = bt.seen(p, q0), limit = bt.seen(p, q0 + (lane & 31)), pos0 = bt.start + q0, pos = pos0 + (lane & 31);
+    const int pos0 = bt.start + q0, pos = pos0 + (lane & 31);
 
     u32x4 own[HD / 16];
     own_operands<HD>(own, p.q.head(b, hq) + (int64_t)(q0 + (lane & 31)) * p.q.sl, (lane & 31) < rows, h, p.D);
@@ -104,7 +105,9 @@ __global__ __launch_bounds__(kCtxThreads, 2) void ctx_fwd(CtxParams p) {
     }
     workgroup_barrier();
     RowSums<T, HD, BIAS> st;
-    for (int t = 0; t < nt; ++t) {
+    // the last tile of the sequence may need a mask: it has code of its own behind the loop (as a condition within, the compiler makes the
+    // mask a select in every tile, a third of the vector instructions at D = 64)
+    const auto tile = [&](int t, bool masked) {
         const int key = t * kCtxTile;
         if (t + 1 < nt) {
             kt += kCtxTile * p.k.sl;
@@ -120,7 +123,7 @@ __global__ __launch_bounds__(kCtxThreads, 2) void ctx_fwd(CtxParams p) {
                 s[u] = scores<T, HD>(K, 32 * u, own, lane);
                 if constexpr (BIAS) st.bias(p, s[u], key + 32 * u, h, row, pos, pos0, pos0 + 31);
             }
-            st.exponentials(p, s, key, limit, key + kCtxTile <= n_all, h);
+            st.exponentials(p, s, bt.keys - key, h, masked);
 #pragma unroll
             for (int u = 0; u < 2; ++u) add_columns<T, HD>(st.acc, K + kTile, 32 * u, s[u], lane);
         }
@@ -130,7 +133,10 @@ __global__ __launch_bounds__(kCtxThreads, 2) void ctx_fwd(CtxParams p) {
             vc.store(next + kTile, p.D, tid);
         }
         workgroup_barrier();
-    }
+    };
+    const int whole = min(nt, bt.keys / kCtxTile);
+    for (int t = 0; t < whole; ++t) tile(t, false);
+    if (whole < nt) tile(whole, true);
     const int out_rows = min(max(p.Lq - q0, 0), 32);
     const float both = halves_sum(st.l), l = (lane & 31) < rows ? both : 0.0f;
     const float f = l == 0.0f ? 0.0f : 1.0f / l;
@@ -147,7 +153,7 @@ __global__ __launch_bounds__(kCtxThreads, 2) void ctx_fwd(CtxParams p) {
 // `packed` heads of a group stand in one block's rows: all of them, or one where their bias rows would not fit, or where a head has
 // 32 rows or more (so that the positions in a block lie within 31 of each other).
 template <typename T, int HD, bool BIAS, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void ctx_fwd_few(CtxParams p) {
+__global__ __launch_bounds__(64 * WAVES, HD <= 64 ? 3 : 2) void ctx_fwd_few(CtxParams p) {
     extern __shared__ __align__(16) unsigned char smem[];
     constexpr int kRegion = 32 * kCtxLd<HD>, kSum = HD + 4;
     elem_t* region = reinterpret_cast<elem_t*>(smem);  // [WAVES] V tiles, then the waves' sums [WAVES][32][HD + 4] fp32
@@ -167,8 +173,8 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void ctx_fwd_few(CtxParams p
     // the queries of a block: consecutive ones of one head, or any where it holds the end of one
     const bool one_head = (r0 + rows - 1) / p.Lq == g0;
     const int i_first = one_head ? r0 % p.Lq : 0, i_last = one_head ? r0 % p.Lq + rows - 1 : p.Lq - 1;
-    const int n = bt.rows > i_first ? bt.seen(p, min(i_last, bt.rows - 1)) : 0, n_all = bt.seen(p, i_first);
-    const int limit = mine ? bt.seen(p, i) : n, pos = bt.start + i;
+    const int n = bt.rows > i_first ? bt.seen(p, min(i_last, bt.rows - 1)) : 0;
+    const int pos = bt.start + i;
     const int tiles = (n + 31) / 32;
     const int t_first = (int)((int64_t)tiles * split / p.splits), t_end = (int)((int64_t)tiles * (split + 1) / p.splits);
 
@@ -219,7 +225,7 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void ctx_fwd_few(CtxParams p
         if (t + WAVES < t_end) load(t + WAVES);
         const int key = t * 32;
         if constexpr (BIAS) st.bias(p, s[0], key, h, row, pos, bt.start + i_first, bt.start + i_last);
-        st.exponentials(p, s, key, limit, key + 32 <= n_all, h);
+        st.exponentials(p, s, bt.keys - key, h, key + 32 > bt.keys);
         wave_exchange();
         add_columns<T, HD>(st.acc, V, 0, s[0], lane);
         wave_exchange();
