@@ -30,9 +30,9 @@ struct RowSums {
         }
     }
 
-    // left: the sequence's keys from `key` on, where they do not fill the scores (masked).
+    // The rows' maxima with these scores.  left: the sequence's keys from `key` on, where they do not fill the scores (masked).
     template <int N>
-    __device__ __forceinline__ void exponentials(const CtxParams& p, f32x16 (&s)[N], int left, int h, bool masked) {
+    __device__ __forceinline__ void raise(const CtxParams& p, f32x16 (&s)[N], int left, int h, bool masked) {
         if (masked) {
 #pragma unroll
             for (int u = 0; u < N; ++u)
@@ -55,6 +55,10 @@ struct RowSums {
 #pragma unroll
             for (int dt = 0; dt < HD / 32; ++dt) acc[dt] *= f;
         }
+    }
+
+    template <int N>
+    __device__ __forceinline__ void exponentials(const CtxParams& p, f32x16 (&s)[N]) {
         float sum = 0.0f;
 #pragma unroll
         for (int u = 0; u < N; ++u)
@@ -75,7 +79,7 @@ template <typename T, int HD, bool BIAS>
 __global__ __launch_bounds__(kCtxThreads, 2) void ctx_fwd(CtxParams p) {
     extern __shared__ __align__(16) unsigned char smem[];
     constexpr int kTile = kCtxTile * kCtxLd<HD>;
-    elem_t* tiles = reinterpret_cast<elem_t*>(smem);  // [2][K, V]
+    elem_t* tiles = reinterpret_cast<elem_t*>(smem);  // K [2], V [2]
     float* row = reinterpret_cast<float*>(tiles + 4 * kTile);
     const int nqb = p.blocks;
     const CtxWork w = ctx_work(p.B * p.Hkv, p.G * nqb);
@@ -94,49 +98,57 @@ __global__ __launch_bounds__(kCtxThreads, 2) void ctx_fwd(CtxParams p) {
     const elem_t *kt = p.k.head(b, hk), *vt = p.v.head(b, hk);
     const int nt = (n + kCtxTile - 1) / kCtxTile;
     TileCopy<HD> kc(p.k.sl, p.D, tid), vc(p.v.sl, p.D, tid);
-    if (nt) {
-        kc.load(kt, p.k.sl, n, p.D);
-        vc.load(vt, p.v.sl, n, p.D);
-    }
+    elem_t* const vtiles = tiles + 2 * kTile;
+    // tile t of K / V on its way, and into its place
+    const auto load_k = [&](int t) { kc.load(kt + (int64_t)t * kCtxTile * p.k.sl, p.k.sl, n - t * kCtxTile, p.D); };
+    const auto load_v = [&](int t) { vc.load(vt + (int64_t)t * kCtxTile * p.v.sl, p.v.sl, n - t * kCtxTile, p.D); };
+    const auto place_k = [&](int t) { kc.store(tiles + (t & 1) * kTile, p.D, tid); };
+    const auto place_v = [&](int t) { vc.store(vtiles + (t & 1) * kTile, p.D, tid); };
+    if (nt) load_k(0), load_v(0);
     if constexpr (BIAS) fill_bias_row(p, row, hq, tid, kCtxThreads);
     if (nt) {
-        kc.store(tiles, p.D, tid);
-        vc.store(tiles + kTile, p.D, tid);
+        place_k(0), place_v(0);
+        if (nt > 1) load_k(1);
     }
     workgroup_barrier();
     RowSums<T, HD, BIAS> st;
-    // the last tile of the sequence may need a mask: it has code of its own behind the loop (as a condition within, the compiler makes the
-    // mask a select in every tile, a third of the vector instructions at D = 64)
-    const auto tile = [&](int t, bool masked) {
+    f32x16 s[2], next[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) s[u] = scores<T, HD>(tiles, 32 * u, own, lane);
+    if (nt > 1) place_k(1);
+    workgroup_barrier();
+    // Scores of one tile are contracted beside the exponentials of the one before, which the vector unit is busy with.
+    // The sequence's last tile may need a mask and has code of its own behind the loop (as a condition within, the compiler makes the
+    // mask a select in every tile, a third of the vector instructions at D = 64).
+    const auto tile = [&](int t, bool masked, auto more) {
         const int key = t * kCtxTile;
-        if (t + 1 < nt) {
-            kt += kCtxTile * p.k.sl;
-            vt += kCtxTile * p.v.sl;
-            kc.load(kt, p.k.sl, n - key - kCtxTile, p.D);
-            vc.load(vt, p.v.sl, n - key - kCtxTile, p.D);
+        if (more) {
+            if (t + 2 < nt) load_k(t + 2);
+            load_v(t + 1);
         }
         if (key < n_wave) {
-            const elem_t* K = tiles + (t & 1) * 2 * kTile;
-            f32x16 s[2];
+            if constexpr (BIAS) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                s[u] = scores<T, HD>(K, 32 * u, own, lane);
-                if constexpr (BIAS) st.bias(p, s[u], key + 32 * u, h, row, pos, pos0, pos0 + 31);
+                for (int u = 0; u < 2; ++u) st.bias(p, s[u], key + 32 * u, h, row, pos, pos0, pos0 + 31);
             }
-            st.exponentials(p, s, bt.keys - key, h, masked);
+            st.raise(p, s, bt.keys - key, h, masked);
+            if constexpr (more) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) add_columns<T, HD>(st.acc, K + kTile, 32 * u, s[u], lane);
+                for (int u = 0; u < 2; ++u) next[u] = scores<T, HD>(tiles + ((t + 1) & 1) * kTile, 32 * u, own, lane);
+            }
+            st.exponentials(p, s);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) add_columns<T, HD>(st.acc, vtiles + (t & 1) * kTile, 32 * u, s[u], lane);
+            if constexpr (more) s[0] = next[0], s[1] = next[1];
         }
-        if (t + 1 < nt) {
-            elem_t* next = tiles + ((t + 1) & 1) * 2 * kTile;
-            kc.store(next, p.D, tid);
-            vc.store(next + kTile, p.D, tid);
+        if (more) {
+            if (t + 2 < nt) place_k(t + 2);
+            place_v(t + 1);
         }
         workgroup_barrier();
     };
-    const int whole = min(nt, bt.keys / kCtxTile);
-    for (int t = 0; t < whole; ++t) tile(t, false);
-    if (whole < nt) tile(whole, true);
+    for (int t = 0; t + 1 < nt; ++t) tile(t, false, std::true_type{});
+    if (nt) tile(nt - 1, nt * kCtxTile > bt.keys, std::false_type{});
     const int out_rows = min(max(p.Lq - q0, 0), 32);
     const float both = halves_sum(st.l), l = (lane & 31) < rows ? both : 0.0f;
     const float f = l == 0.0f ? 0.0f : 1.0f / l;
@@ -225,7 +237,8 @@ __global__ __launch_bounds__(64 * WAVES, HD <= 64 ? 3 : 2) void ctx_fwd_few(CtxP
         if (t + WAVES < t_end) load(t + WAVES);
         const int key = t * 32;
         if constexpr (BIAS) st.bias(p, s[0], key, h, row, pos, bt.start + i_first, bt.start + i_last);
-        st.exponentials(p, s, bt.keys - key, h, key + 32 > bt.keys);
+        st.raise(p, s, bt.keys - key, h, key + 32 > bt.keys);
+        st.exponentials(p, s);
         wave_exchange();
         add_columns<T, HD>(st.acc, V, 0, s[0], lane);
         wave_exchange();
