@@ -53,7 +53,8 @@ CtxPlan ctx_plan_fwd(const CtxParams& p) {
         plan.blocks = (int)ceil_div(p.Lq, kCtxOwned);
         plan.units = (int64_t)p.B * p.Hkv;
         plan.inner = (int64_t)p.G * plan.blocks;
-        plan.smem = ctx_tiles_bytes(HD) + bias;
+        plan.dma = ctx_dma(p, p.k, p.v);
+        plan.smem = ctx_tiles_bytes(HD, plan.dma) + bias;
         return plan;
     }
     const int heads = p.Lq < 32 ? std::min(p.G, 31 / p.Lq + 2) : 1;  // that a block of 32 rows can touch
@@ -75,8 +76,9 @@ CtxPlan ctx_plan_row(const CtxParams& p) {
     // (the bucket sums need a row's whole residue, see ctx_bwd_row)
     plan.splits = p.tpart ? 1 : splits_for((int64_t)p.B * p.Hq * plan.blocks, ceil_div(p.Lk, kCtxTile), 1, 4);
     plan.inner = (int64_t)p.G * plan.blocks * plan.splits;
-    plan.smem = ctx_tiles_bytes(ctx_padded(p.D)) + (p.table ? 4 * ctx_entries(p) * (p.tpart ? 1 + kCtxWaves : 1) : 0);
-    if (p.tpart) {
+    plan.dma = ctx_dma(p, p.k, p.v);
+    plan.smem = ctx_tiles_bytes(ctx_padded(p.D), plan.dma) + (p.table ? 4 * ctx_entries(p) * (1 + kCtxWaves) : 0);
+    if (p.table) {
         plan.skew = (plan.smem + 15) / 16 * 16;
         plan.smem = plan.skew + 4 * kCtxWaves * kSkewFloats;
     }
@@ -89,7 +91,8 @@ CtxPlan ctx_plan_col(const CtxParams& p) {
     plan.units = (int64_t)p.B * p.Hkv;
     plan.splits = splits_for(plan.units * plan.blocks, p.G * ceil_div(p.Lq, kCtxTile), 1, 4);
     plan.inner = (int64_t)plan.blocks * plan.splits;
-    plan.smem = ctx_tiles_bytes(ctx_padded(p.D)) + 4 * kCtxTile * 4 + (p.table ? 4 * ctx_entries(p) : 0);
+    plan.dma = ctx_dma(p, p.q, p.g);
+    plan.smem = ctx_tiles_bytes(ctx_padded(p.D), plan.dma) + 4 * kCtxTile * 4 + (p.table ? 4 * ctx_entries(p) : 0);
     return plan;
 }
 

@@ -107,10 +107,6 @@ __device__ __forceinline__ void store_chunk(elem_t* p, u32x4 x, int c8, int D) {
     }
 }
 
-// LDS tiles are [rows][HD + 8]: the 16 bytes between rows spread both the row-major 16-byte reads of 16 rows and the
-// transposing reads of 4 rows over all banks.
-template <int HD> constexpr int kCtxLd = HD + 8;
-
 // B operands of this lane's own row (all chunks of 16 of the head dimension), from memory.
 template <int HD>
 __device__ __forceinline__ void own_operands(u32x4* out, const elem_t* row, bool ok, int h, int D) {
@@ -118,23 +114,46 @@ __device__ __forceinline__ void own_operands(u32x4* out, const elem_t* row, bool
     for (int c = 0; c < HD / 16; ++c) out[c] = ok ? load_chunk(row, 16 * c + 8 * h, D) : u32x4{0u, 0u, 0u, 0u};
 }
 
-// A operand: rows `row0` .. row0 + 31 of a tile, chunk c of 16 columns.
-template <int HD>
-__device__ __forceinline__ u32x4 tile_rows(const elem_t* tile, int row0, int c, int lane) {
-    return *reinterpret_cast<const u32x4*>(tile + (row0 + (lane & 31)) * kCtxLd<HD> + 16 * c + 8 * (lane >> 5));
-}
+// A tile of looped rows in LDS, and where this lane reads its operands.  Tiles that come through registers are [64][HD + 8]: the 16
+// bytes between rows spread both the row-major 16-byte reads of 16 rows and the transposing reads of 4 rows over all banks.
+// LDS-DMA copies leave no gaps: there the 16-byte pieces of a row are permuted instead (swz).
+template <int HD, bool DMA>
+struct Tile {
+    static constexpr int kLd = DMA ? HD : HD + 8, kElems = kCtxTile * kLd;
+    int row[HD / 16], col[HD == 32 ? 2 : HD / 32];
 
-// A operand of an output contraction: columns 32 dt .. 32 dt + 31 (as rows of A) over the 16 rows from row0 on, in the numbering
-// at the top.  Within 16 lanes of a transposing read lane 4j + i supplies row j, columns 4i .. 4i+3, and lane n receives column n.
-template <int HD>
-__device__ __forceinline__ u32x4 tile_columns(const elem_t* tile, int row0, int dt, int lane) {
-    const int i16 = lane & 15;
-    const elem_t* p = tile + (row0 + 4 * (lane >> 5) + (i16 >> 2)) * kCtxLd<HD> + 32 * dt + (lane & 16) + 4 * (i16 & 3);
-    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-    const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p)));
-    const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 8 * kCtxLd<HD>)));
-    return u32x4{lo[0], lo[1], hi[0], hi[1]};
-}
+    __device__ __forceinline__ explicit Tile(int lane) {
+        const int y = lane & 31, h = lane >> 5, i16 = lane & 15;
+#pragma unroll
+        for (int c = 0; c < HD / 16; ++c) row[c] = DMA ? y * HD + 8 * ((2 * c + h) ^ swz<HD>(y)) : y * kLd + 16 * c + 8 * h;
+        // within 16 lanes of a transposing read lane 4j + i supplies row j, columns 4i .. 4i+3, and lane n receives column n
+        const int r = 4 * h + (i16 >> 2), chunk = 2 * ((lane >> 4) & 1) + ((i16 & 3) >> 1);
+#pragma unroll
+        for (int z = 0; z < (HD == 32 ? 2 : HD / 32); ++z)
+            col[z] = DMA ? r * HD + 8 * (chunk ^ swz<HD>(r) ^ (HD == 32 ? 2 * z : 4 * z)) + 4 * (i16 & 1) : r * kLd + 8 * chunk + 4 * (i16 & 1);
+    }
+    // A operand: rows row0 .. row0 + 31 (row0 a multiple of 32), chunk c of 16 columns
+    __device__ __forceinline__ u32x4 rows(const elem_t* tile, int row0, int c) const {
+        return *reinterpret_cast<const u32x4*>(tile + row0 * kLd + row[c]);
+    }
+    // A operand of an output contraction: columns 32 dt .. 32 dt + 31 (as rows of A) over the 16 rows from row0 on (a multiple of
+    // 16), in the numbering at the top
+    __device__ __forceinline__ u32x4 columns(const elem_t* tile, int row0, int dt) const {
+        // the permutation of rows 8 further differs in one bit, and so does the place of the next 32 columns
+        const elem_t *p = tile + row0 * kLd, *lo, *hi;
+        if constexpr (DMA) {
+            lo = p + col[HD == 32 ? 0 : dt];
+            hi = p + 8 * kLd + col[HD == 32 ? 1 : HD == 64 ? dt ^ 1 : dt ^ 2];
+        } else {
+            lo = p + col[0] + 32 * dt;
+            hi = lo + 8 * kLd;
+        }
+        typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+        const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lo)));
+        const u32x2 b = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(hi)));
+        return u32x4{a[0], a[1], b[0], b[1]};
+    }
+};
 
 // Registers 8m .. 8m+7 of a score tile as a B operand.
 template <typename T>
@@ -147,11 +166,19 @@ __device__ __forceinline__ u32x4 pack_scores(const f32x16& s, int m) {
 
 // Rows of a tensor from a given one on, as a buffer: reads behind the last row that exists return zeros (whatever memory holds there),
 // with no branch.  Offsets are 32 bits within a tile, so the host keeps row strides below 2^24 elements.
-typedef __amdgpu_buffer_rsrc_t Rows;
 constexpr uint32_t kNoChunk = 0x80000000u;  // an offset behind every buffer
+__device__ __forceinline__ int rows_bytes(int64_t sl, int rows, int D) {
+    return rows > 0 ? 2 * ((min(rows, kCtxTile) - 1) * (int)sl + D) : 0;
+}
+typedef __amdgpu_buffer_rsrc_t Rows;
+constexpr int kRowsFlags = 0x00020000;
 __device__ __forceinline__ Rows make_rows(const elem_t* base, int64_t sl, int rows, int D) {
-    const int bytes = rows > 0 ? 2 * ((min(rows, kCtxTile) - 1) * (int)sl + D) : 0;
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<elem_t*>(base), 0, bytes, 0x00020000);
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<elem_t*>(base), 0, rows_bytes(sl, rows, D), kRowsFlags);
+}
+// the four words of that descriptor
+__device__ __forceinline__ u32x4 rows_words(const elem_t* base, int64_t sl, int rows, int D) {
+    const uint64_t at = reinterpret_cast<uint64_t>(base);
+    return u32x4{(uint32_t)at, (uint32_t)(at >> 32) & 0xffffu, (uint32_t)rows_bytes(sl, rows, D), (uint32_t)kRowsFlags};
 }
 __device__ __forceinline__ uint32_t chunk_offset(int row, int c8, int64_t sl, int D) {
     return c8 < D ? 2u * (uint32_t)(row * (int)sl + chunk_column(c8, D)) : kNoChunk;
@@ -160,31 +187,53 @@ __device__ __forceinline__ u32x4 read_chunk(Rows rows, uint32_t offset) {
     return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rows, offset, 0, 0));
 }
 
-// A tile of 64 rows on its way from memory to LDS through the registers of NT threads: any stride and alignment.
-template <int HD, int NT = kCtxThreads>
-struct TileCopy {
+// A tile of 64 rows on its way from memory to LDS by NT threads: straight into LDS where rows start on 16-byte boundaries (DMA), through
+// registers at any alignment otherwise.  request() is called ahead, deliver() where the place is read next, behind it arrived()
+// and a barrier.
+template <int HD, bool DMA, int NT = kCtxThreads>
+struct TileFeed {
     static constexpr int CH = HD / 8;
     static constexpr int N = kCtxTile * CH / NT;
     static_assert(kCtxTile * CH % NT == 0, "every thread copies whole chunks");
-    u32x4 r[N];
+    u32x4 r[DMA ? 1 : N];
     uint32_t offset[N];
 
-    __device__ __forceinline__ TileCopy(int64_t sl, int D, int tid) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) offset[i] = chunk_offset((tid + NT * i) / CH, 8 * ((tid + NT * i) % CH), sl, D);
-    }
-    __device__ __forceinline__ void load(const elem_t* base, int64_t sl, int rows, int D) {
-        const Rows from = make_rows(base, sl, rows, D);
-#pragma unroll
-        for (int i = 0; i < N; ++i) r[i] = read_chunk(from, offset[i]);
-    }
-    __device__ __forceinline__ void store(elem_t* tile, int D, int tid) {
+    __device__ __forceinline__ TileFeed(int64_t sl, int D, int tid) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int x = tid + NT * i;
-            if (D % 8) r[i] = chunk_shifted(r[i], 8 * (x % CH), D);
-            *reinterpret_cast<u32x4*>(tile + (x / CH) * kCtxLd<HD> + 8 * (x % CH)) = r[i];
+            const int x = tid + NT * i, row = x / CH, c = x % CH;
+            offset[i] = chunk_offset(row, 8 * (DMA ? c ^ swz<HD>(row) : c), sl, D);
         }
+    }
+    __device__ __forceinline__ void request(const elem_t* base, int64_t sl, int rows, int D, elem_t* place, int wave) {
+        if constexpr (DMA) {
+            const u32x4 from = rows_words(base, sl, rows, D);
+            // M0 carries the LDS address; nothing else here uses it.  Counted by vmcnt, unknown to the compiler: its own waits for loads
+            // are stricter for it, never laxer, since loads return in order.
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                asm volatile("s_mov_b32 m0, %2\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
+                             :
+                             : "v"(offset[i]), "s"(from), "s"(__builtin_amdgcn_readfirstlane(lds_addr(place) + 16 * (64 * wave + NT * i)))
+                             : "memory");
+        } else {
+            const Rows from = make_rows(base, sl, rows, D);
+#pragma unroll
+            for (int i = 0; i < N; ++i) r[i] = read_chunk(from, offset[i]);
+        }
+    }
+    __device__ __forceinline__ void deliver(elem_t* place, int D, int tid) {
+        if constexpr (!DMA) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int x = tid + NT * i;
+                if (D % 8) r[i] = chunk_shifted(r[i], 8 * (x % CH), D);
+                *reinterpret_cast<u32x4*>(place + (x / CH) * Tile<HD, DMA>::kLd + 8 * (x % CH)) = r[i];
+            }
+        }
+    }
+    static __device__ __forceinline__ void arrived() {
+        if constexpr (DMA) __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
     }
 };
 
@@ -211,9 +260,8 @@ __device__ __forceinline__ float ctx_table(const CtxParams& p, int bucket, int h
 __device__ __forceinline__ int ctx_row_entries(const CtxParams& p) { return 2 * (p.far + kCtxPad) + 1; }
 
 // The bias of a head by position difference, entry far + pad for difference 0, in units of log2; -inf for keys behind a causal query,
-// so that the kernels need no other mask for these.  A difference of a 32 x 32
-// tile that is not wholly beyond `far` lies within far + 62, so the padding saves the tiles a clamp.  A table entry near
-// the lowest float32 would leave the range with the factor log2(e); it is raised to -2.3e38, still below any score.
+// so that the kernels need no other mask for these.  A table entry near the lowest float32 would leave the range with the factor
+// log2(e); it is raised to -2.3e38, still below any score.
 __device__ __forceinline__ void fill_bias_row(const CtxParams& p, float* row, int head, int tid, int threads) {
     for (int x = tid; x < ctx_row_entries(p); x += threads) {
         const int rel = x - p.far - kCtxPad;
@@ -260,7 +308,7 @@ template <typename T, int HD>
 __device__ __forceinline__ void store_rows(const f32x16* acc, float factor, elem_t* out, int64_t sl, int rows, elem_t* region,
                                            int lane, int D) {
     const int h = lane >> 5;
-    elem_t* mine = region + (lane & 31) * kCtxLd<HD> + 4 * h;
+    elem_t* mine = region + (lane & 31) * (HD + 8) + 4 * h;
 #pragma unroll
     for (int dt = 0; dt < HD / 32; ++dt)
 #pragma unroll
@@ -278,7 +326,7 @@ __device__ __forceinline__ void store_rows(const f32x16* acc, float factor, elem
 #pragma unroll
     for (int x0 = 0; x0 < 32 * CH; x0 += 64) {
         const int x = x0 + lane, row = x / CH, c8 = 8 * (x % CH);
-        if (row < rows) store_chunk(out + row * sl, *reinterpret_cast<const u32x4*>(region + row * kCtxLd<HD> + c8), c8, D);
+        if (row < rows) store_chunk(out + row * sl, *reinterpret_cast<const u32x4*>(region + row * (HD + 8) + c8), c8, D);
     }
     wave_exchange();
 }
@@ -296,45 +344,52 @@ __device__ __forceinline__ void store_part(const f32x16* acc, bool some, float* 
                 some ? f32x4{acc[dt][4 * i], acc[dt][4 * i + 1], acc[dt][4 * i + 2], acc[dt][4 * i + 3]} : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 }
 
-// Where a 32 x 32 tile of position differences lies: entirely beyond `far` on one side (one bias for all), or not.
+// Where the position differences of a tile lie: all beyond `far` on one side, which has one bias, or not.  Looped positions are walked in
+// order, so that the tiles of each kind follow each other and each kind has a loop of its own, without a branch in its body.
 enum CtxBand { kBelow, kNear, kAbove };
-__device__ __forceinline__ CtxBand ctx_band(const CtxParams& p, int least, int most) {
-    return most <= -p.far ? kBelow : least >= p.far ? kAbove : kNear;
+template <CtxBand B> using InBand = std::integral_constant<CtxBand, B>;
+// whole tiles in front of a position, of `tiles`
+__device__ __forceinline__ int tiles_before(int position, int tiles) { return min(max(position, 0) / kCtxTile, tiles); }
+
+// First entry of a bias row (or of sums by difference) for a lane or a wave that uses `count` from it on: differences wholly beyond `far`
+// have the same bias, so that their entries may be taken from the row's ends.
+__device__ __forceinline__ int row_entry(const CtxParams& p, int rel, int count) {
+    return min(max(rel + p.far + kCtxPad, 0), ctx_row_entries(p) - count);
 }
 
 // OUT^T += A^T B for the two halves of a packed score tile whose looped rows start at row0 of the tile.
-template <typename T, int HD>
-__device__ __forceinline__ void add_columns(f32x16* acc, const elem_t* tile, int row0, const f32x16& s, int lane) {
+template <typename T, int HD, bool DMA>
+__device__ __forceinline__ void add_columns(f32x16* acc, const Tile<HD, DMA>& at, const elem_t* tile, int row0, const f32x16& s) {
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
         const u32x4 b = pack_scores<T>(s, m);
 #pragma unroll
         for (int dt = 0; dt < HD / 32; ++dt)
-            acc[dt] = Mma32<T>::run(tile_columns<HD>(tile, row0 + 16 * m, dt, lane), b, acc[dt]);
+            acc[dt] = Mma32<T>::run(at.columns(tile, row0 + 16 * m, dt), b, acc[dt]);
     }
 }
 
 // The same of two score tiles, which share the reads.
-template <typename T, int HD>
-__device__ __forceinline__ void add_columns(f32x16* acc0, f32x16* acc1, const elem_t* tile, int row0, const f32x16& s0,
-                                            const f32x16& s1, int lane) {
+template <typename T, int HD, bool DMA>
+__device__ __forceinline__ void add_columns(f32x16* acc0, f32x16* acc1, const Tile<HD, DMA>& at, const elem_t* tile, int row0,
+                                            const f32x16& s0, const f32x16& s1) {
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
         const u32x4 b0 = pack_scores<T>(s0, m), b1 = pack_scores<T>(s1, m);
 #pragma unroll
         for (int dt = 0; dt < HD / 32; ++dt) {
-            const u32x4 a = tile_columns<HD>(tile, row0 + 16 * m, dt, lane);
+            const u32x4 a = at.columns(tile, row0 + 16 * m, dt);
             acc0[dt] = Mma32<T>::run(a, b0, acc0[dt]);
             acc1[dt] = Mma32<T>::run(a, b1, acc1[dt]);
         }
     }
 }
 
-template <typename T, int HD>
-__device__ __forceinline__ f32x16 scores(const elem_t* tile, int row0, const u32x4* own, int lane) {
+template <typename T, int HD, bool DMA>
+__device__ __forceinline__ f32x16 scores(const Tile<HD, DMA>& at, const elem_t* tile, int row0, const u32x4* own) {
     f32x16 s = {};
 #pragma unroll
-    for (int c = 0; c < HD / 16; ++c) s = Mma32<T>::run(tile_rows<HD>(tile, row0, c, lane), own[c], s);
+    for (int c = 0; c < HD / 16; ++c) s = Mma32<T>::run(at.rows(tile, row0, c), own[c], s);
     return s;
 }
 

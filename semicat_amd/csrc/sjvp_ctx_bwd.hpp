@@ -53,10 +53,10 @@ __device__ __forceinline__ void add_diagonals(float* skew, float* at, const f32x
 }
 
 // Row-owned: four waves of 32 query rows of one head share tiles of 64 keys.
-template <typename T, int HD, bool BIAS>
+template <typename T, int HD, bool BIAS, bool DMA>
 __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_row(CtxParams p) {
     extern __shared__ __align__(16) unsigned char smem[];
-    constexpr int kTile = kCtxTile * kCtxLd<HD>;
+    constexpr int kTile = Tile<HD, DMA>::kElems;
     elem_t* tiles = reinterpret_cast<elem_t*>(smem);  // [2][K, V]
     float* row = reinterpret_cast<float*>(tiles + 4 * kTile);
     const int nqb = p.blocks, entries = ctx_row_entries(p);
@@ -73,7 +73,6 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_row(Ctx
     const int limit = bt.seen(p, qi), pos0 = bt.start + q0, pos = pos0 + (lane & 31);
     const int nt = (n + kCtxTile - 1) / kCtxTile;
     const int t0 = (int)((int64_t)nt * split / p.splits), t1 = (int)((int64_t)nt * (split + 1) / p.splits);
-    const bool with_table = BIAS && p.tpart;
     float* hist = row + entries + wave * entries;  // the wave's sums of dS by difference
     float* skew = reinterpret_cast<float*>(smem + p.skew) + wave * kSkewFloats;
 
@@ -88,28 +87,35 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_row(Ctx
     own_operands<HD>(own_g, p.g.head(b, hq) + (int64_t)qi * p.g.sl, ok, h, p.D);
     const float delta = row_delta<T, HD>(p, own_g, p.o.head(b, hq) + (int64_t)qi * p.o.sl, ok, h);
 
-    const elem_t *kt = p.k.head(b, hk) + (int64_t)t0 * kCtxTile * p.k.sl, *vt = p.v.head(b, hk) + (int64_t)t0 * kCtxTile * p.v.sl;
-    TileCopy<HD> kc(p.k.sl, p.D, tid), vc(p.v.sl, p.D, tid);
+    const elem_t *kt = p.k.head(b, hk), *vt = p.v.head(b, hk);
+    TileFeed<HD, DMA> kf(p.k.sl, p.D, tid), vf(p.v.sl, p.D, tid);
+    const Tile<HD, DMA> at(lane);
+    const auto place = [&](int t) { return tiles + ((t - t0) & 1) * 2 * kTile; };
+    const auto request = [&](int t) {
+        kf.request(kt + (int64_t)t * kCtxTile * p.k.sl, p.k.sl, n - t * kCtxTile, p.D, place(t), wave);
+        vf.request(vt + (int64_t)t * kCtxTile * p.v.sl, p.v.sl, n - t * kCtxTile, p.D, place(t) + kTile, wave);
+    };
+    const auto deliver = [&](int t) {
+        kf.deliver(place(t), p.D, tid);
+        vf.deliver(place(t) + kTile, p.D, tid);
+    };
     if (t0 < t1) {
-        kc.load(kt, p.k.sl, n - t0 * kCtxTile, p.D);
-        vc.load(vt, p.v.sl, n - t0 * kCtxTile, p.D);
-        kc.store(tiles, p.D, tid);
-        vc.store(tiles + kTile, p.D, tid);
+        request(t0);
+        deliver(t0);
     }
     if constexpr (BIAS) {
         fill_bias_row(p, row, hq, tid, kCtxThreads);
-        if (with_table)
-            for (int x = lane; x < entries; x += 64) hist[x] = 0.0f;
-        if (with_table)
-            for (int x = lane; x < kSkewFloats; x += 64) skew[x] = 0.0f;
+        for (int x = lane; x < entries; x += 64) hist[x] = 0.0f;
+        for (int x = lane; x < kSkewFloats; x += 64) skew[x] = 0.0f;
     }
+    kf.arrived();
     workgroup_barrier();
-    // scores of 32 keys from k0 on to P, zero where hidden
-    const auto row_probabilities = [&](f32x16& s, int k0, CtxBand band, bool masked) {
-        if (BIAS && band == kNear) {
-            const float* at = row + (k0 + 4 * h - pos + p.far + kCtxPad);
+    // scores of 32 keys from k0 on to P, zero behind the sequence (masked)
+    const auto row_probabilities = [&](f32x16& s, int k0, auto band, bool masked) {
+        if constexpr (decltype(band)::value == kNear) {
+            const float* bias = row + row_entry(p, k0 + 4 * h - pos, 28);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = fast_exp2(__builtin_fmaf(s[r], p.c, at[8 * (r >> 2) + (r & 3)]) - lse);
+            for (int r = 0; r < 16; ++r) s[r] = fast_exp2(__builtin_fmaf(s[r], p.c, bias[8 * (r >> 2) + (r & 3)]) - lse);
         } else {
             const float one = BIAS ? row[band == kBelow ? 0 : entries - 1] - lse : -lse;
 #pragma unroll
@@ -122,56 +128,61 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_row(Ctx
         }
     };
     f32x16 acc[HD / 32] = {}, mean[HD / 32] = {};  // dS K, P K
-    float below = 0.0f, above = 0.0f;    // sums of dS beyond the last single distance,
-    float p_below = 0.0f, p_above = 0.0f;  // and of P there
-    float residue = 0.0f;                  // sum of dS over the row
+    float ds_below = 0.0f, ds_above = 0.0f;        // sums of dS beyond the last single distance,
+    float p_below = 0.0f, p_above = 0.0f;          // and of P there
+    float residue = 0.0f;                          // sum of dS over the row
     // (the sequence's last tile with its mask in code of its own, as in the forward)
-    const auto tile = [&](int t, bool masked) {
-        const int key = t * kCtxTile, at = (t - t0) & 1;
-        if (t + 1 < t1) {
-            kt += kCtxTile * p.k.sl;
-            vt += kCtxTile * p.v.sl;
-            kc.load(kt, p.k.sl, n - key - kCtxTile, p.D);
-            vc.load(vt, p.v.sl, n - key - kCtxTile, p.D);
-        }
-        const elem_t* K = tiles + at * 2 * kTile;
+    const auto tile = [&](int t, bool masked, auto band) {
+        const int key = t * kCtxTile;
+        if (t + 1 < t1) request(t + 1);
+        const elem_t* K = place(t);
+        if (key < n_wave) {
+            f32x16 s[2], ds[2];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int k0 = key + 32 * u;
-            if (k0 >= n_wave) continue;
-            f32x16 s = scores<T, HD>(K, 32 * u, own_q, lane), ds = scores<T, HD>(K + kTile, 32 * u, own_g, lane);
-            const CtxBand band = BIAS ? ctx_band(p, k0 - pos0 - 31, k0 + 31 - pos0) : kNear;
-            row_probabilities(s, k0, band, masked);
+            for (int u = 0; u < 2; ++u) {
+                s[u] = scores<T>(at, K, 32 * u, own_q);
+                ds[u] = scores<T>(at, K + kTile, 32 * u, own_g);
+            }
 #pragma unroll
-            for (int r = 0; r < 16; ++r) ds[r] = s[r] * (ds[r] - delta);
-            float sum = 0.0f;
+            for (int u = 0; u < 2; ++u) {
+                row_probabilities(s[u], key + 32 * u, band, masked);
+                float sum = 0.0f, p_sum = 0.0f;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) sum += ds[r];
-            residue += sum;
-            if (with_table) {
-                float p_sum = 0.0f;
+                for (int r = 0; r < 16; ++r) {
+                    ds[u][r] = s[u][r] * (ds[u][r] - delta);
+                    sum += ds[u][r];
+                }
+                residue += sum;
+                if constexpr (BIAS && decltype(band)::value == kNear) {
+                    add_diagonals(skew, hist + row_entry(p, key + 32 * u - pos0 - 31, 63), ds[u], 1.0f, lane);
+                } else if constexpr (BIAS) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) p_sum += s[r];
-                if (band == kNear) {
-                    add_diagonals(skew, hist + (k0 - pos0 - 31 + p.far + kCtxPad), ds, 1.0f, lane);
-                } else if (band == kBelow) {
-                    below += sum, p_below += p_sum;
-                } else {
-                    above += sum, p_above += p_sum;
+                    for (int r = 0; r < 16; ++r) p_sum += s[u][r];
+                    if constexpr (decltype(band)::value == kBelow) ds_below += sum, p_below += p_sum;
+                    else ds_above += sum, p_above += p_sum;
                 }
             }
-            add_columns<T, HD>(acc, mean, K, 32 * u, ds, s, lane);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) add_columns<T>(acc, mean, at, K, 32 * u, ds[u], s[u]);
         }
-        if (t + 1 < t1) {
-            elem_t* next = tiles + (1 - at) * 2 * kTile;
-            kc.store(next, p.D, tid);
-            vc.store(next + kTile, p.D, tid);
-        }
+        if (t + 1 < t1) deliver(t + 1);
+        kf.arrived();
         workgroup_barrier();
     };
-    const int whole = max(t0, min(t1, bt.keys / kCtxTile));
-    for (int t = t0; t < whole; ++t) tile(t, false);
-    if (whole < t1) tile(whole, true);
+    // the tiles near the diagonal: of the workgroup, whose positions are first .. first + 127
+    const int first = bt.start + qb * kCtxOwned;
+    const int near = tiles_before(first - p.far + 1, nt), above = tiles_before(first + kCtxOwned - 1 + p.far + kCtxTile - 1, nt);
+    const int whole = t1 * kCtxTile > bt.keys ? t1 - 1 : t1;
+    int t = t0;
+    if constexpr (BIAS) {
+        for (; t < min(near, whole); ++t) tile(t, false, InBand<kBelow>{});
+        for (; t < min(above, whole); ++t) tile(t, false, InBand<kNear>{});
+        for (; t < whole; ++t) tile(t, false, InBand<kAbove>{});
+    } else {
+        for (; t < whole; ++t) tile(t, false, InBand<kBelow>{});
+    }
+    // (differences beyond the last single distance may be summed among the others, at the row's ends)
+    if (t < t1) tile(t, true, InBand<BIAS ? kNear : kBelow>{});
     // The rows of dS sum to zero but for the error of delta, which the rounding of P and O in the forward leaves in it (2^-9 of it
     // for bf16; of a sharp row's dS more than that).  So the residue is that error, and P times the residue what it put into dS:
     // taken out of dQ here, of the bucket sums below, and the column-owned launch gets the right delta.  (ctx_sum_rows does it for
@@ -191,30 +202,30 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_row(Ctx
         for (int dt = 0; dt < HD / 32; ++dt) acc[dt] -= residue * mean[dt];
         if (h == 0 && qi < p.Lq) p.delta[stat] = delta + residue;
         store_rows<T, HD>(acc, scored ? p.scale : 0.0f, p.dq.head(b, hq) + (int64_t)q0 * p.dq.sl, p.dq.sl, out_rows,
-                          tiles + wave * 32 * kCtxLd<HD>, lane, p.D);
+                          tiles + wave * 32 * (HD + 8), lane, p.D);
     }
-    if (with_table) {
-        // tiles with a key within `far` of a row of the workgroup
-        const int p_first = bt.start + qb * kCtxOwned;
-        const int ta = min(max(p_first - p.far + 1, 0), n) / kCtxTile, tb = (min(max(p_first + kCtxOwned - 1 + p.far, 0), n) + kCtxTile - 1) / kCtxTile;
-        kt = p.k.head(b, hk) + (int64_t)ta * kCtxTile * p.k.sl;
-        for (int t = ta; t < tb; ++t, kt += kCtxTile * p.k.sl) {
-            const int key = t * kCtxTile;
-            workgroup_barrier();
-            kc.load(kt, p.k.sl, n - key, p.D);
-            kc.store(tiles, p.D, tid);
-            workgroup_barrier();
+    if constexpr (!BIAS) return;
+    if (!p.tpart) return;
+    // the tiles whose differences were summed one by one, the last among them
+    const int t_near = min(near, whole), n_near = max(0, min(above, whole) - t_near), again = n_near + (t1 - whole);
+    for (int i = 0; i < again; ++i) {
+        const int key = (i < n_near ? t_near + i : whole) * kCtxTile;
+        workgroup_barrier();
+        kf.request(kt + (int64_t)key * p.k.sl, p.k.sl, n - key, p.D, tiles, wave);
+        kf.deliver(tiles, p.D, tid);
+        kf.arrived();
+        workgroup_barrier();
+        if (key >= n_wave) continue;
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int k0 = key + 32 * u;
-                if (k0 >= n_wave || ctx_band(p, k0 - pos0 - 31, k0 + 31 - pos0) != kNear) continue;
-                f32x16 s = scores<T, HD>(tiles, 32 * u, own_q, lane);
-                row_probabilities(s, k0, kNear, k0 + 32 > bt.keys);
-                add_diagonals(skew, hist + (k0 - pos0 - 31 + p.far + kCtxPad), s, -residue, lane);
-            }
+        for (int u = 0; u < 2; ++u) {
+            f32x16 s = scores<T>(at, tiles, 32 * u, own_q);
+            row_probabilities(s, key + 32 * u, InBand<kNear>{}, key + kCtxTile > bt.keys);
+            add_diagonals(skew, hist + row_entry(p, key + 32 * u - pos0 - 31, 63), s, -residue, lane);
         }
-        below = wave_sum(below - residue * p_below), above = wave_sum(above - residue * p_above);
-        if (lane == 0) hist[0] += below, hist[entries - 1] += above;
+    }
+    {
+        const float below = wave_sum(ds_below - residue * p_below), above_sum = wave_sum(ds_above - residue * p_above);
+        if (lane == 0) hist[0] += below, hist[entries - 1] += above_sum;
         workgroup_barrier();
         const float* hists = row + entries;
         const int nb = p.both ? 2 * p.buckets : p.buckets, zero = p.far + kCtxPad;
@@ -235,10 +246,10 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_row(Ctx
 }
 
 // Column-owned: four waves of 32 keys share tiles of 64 query rows, over all heads that read the key head.
-template <typename T, int HD, bool BIAS>
+template <typename T, int HD, bool BIAS, bool DMA>
 __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_col(CtxParams p) {
     extern __shared__ __align__(16) unsigned char smem[];
-    constexpr int kTile = kCtxTile * kCtxLd<HD>;
+    constexpr int kTile = Tile<HD, DMA>::kElems;
     elem_t* tiles = reinterpret_cast<elem_t*>(smem);                // [2][Q, dO]
     float* stats = reinterpret_cast<float*>(tiles + 4 * kTile);     // [2][lse, delta][64]
     float* bias_row = stats + 4 * kCtxTile;
@@ -261,76 +272,90 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_col(Ctx
     const int64_t all = (int64_t)p.G * per_head;
     const int x0 = (int)(all * split / p.splits), x1 = (int)(all * (split + 1) / p.splits);
 
-    TileCopy<HD> qc(p.q.sl, p.D, tid), gc(p.g.sl, p.D, tid);
+    TileFeed<HD, DMA> qf(p.q.sl, p.D, tid), gf(p.g.sl, p.D, tid);
+    const Tile<HD, DMA> at(lane);
     float stat = 0.0f;
-    const auto load = [&](int x) {
+    const auto place = [&](int x) { return tiles + ((x - x0) & 1) * 2 * kTile; };
+    const auto request = [&](int x) {
         const int hq = hk * p.G + x / per_head, r0 = (ta + x % per_head) * kCtxTile;
-        qc.load(p.q.head(b, hq) + (int64_t)r0 * p.q.sl, p.q.sl, bt.rows - r0, p.D);
-        gc.load(p.g.head(b, hq) + (int64_t)r0 * p.g.sl, p.g.sl, bt.rows - r0, p.D);
+        qf.request(p.q.head(b, hq) + (int64_t)r0 * p.q.sl, p.q.sl, bt.rows - r0, p.D, place(x), wave);
+        gf.request(p.g.head(b, hq) + (int64_t)r0 * p.g.sl, p.g.sl, bt.rows - r0, p.D, place(x) + kTile, wave);
         if (tid < 2 * kCtxTile) {
             const int i = r0 + (tid & (kCtxTile - 1));
             const float* from = (tid < kCtxTile ? p.lse : p.delta) + ((int64_t)b * p.Hq + hq) * p.Lq;
             stat = i < bt.rows ? from[i] : tid < kCtxTile ? -INFINITY : 0.0f;
         }
     };
-    const auto store = [&](int at) {
-        qc.store(tiles + at * 2 * kTile, p.D, tid);
-        gc.store(tiles + at * 2 * kTile + kTile, p.D, tid);
+    const auto deliver = [&](int x) {
+        qf.deliver(place(x), p.D, tid);
+        gf.deliver(place(x) + kTile, p.D, tid);
         // (a row without keys: its exponentials are zero)
-        if (tid < 2 * kCtxTile) stats[at * 2 * kCtxTile + tid] = tid >= kCtxTile ? stat : stat == -INFINITY ? INFINITY : stat * kLog2e;
+        if (tid < 2 * kCtxTile)
+            stats[((x - x0) & 1) * 2 * kCtxTile + tid] = tid >= kCtxTile ? stat : stat == -INFINITY ? INFINITY : stat * kLog2e;
     };
     if (x0 < x1) {
-        load(x0);
-        store(0);
+        request(x0);
+        deliver(x0);
+        qf.arrived();
     }
     f32x16 dk[HD / 32] = {}, dv[HD / 32] = {};
-    int head = -1;
-    for (int x = x0; x < x1; ++x) {
-        const int at = (x - x0) & 1, g = x / per_head, r0 = (ta + x % per_head) * kCtxTile;
-        if constexpr (BIAS) {
-            if (g != head) {  // (every wave is behind the barrier of the last tile)
-                head = g;
-                fill_bias_row(p, bias_row, hk * p.G + g, tid, kCtxThreads);
+    const auto tile = [&](int x, auto band) {
+        const int p0 = bt.start + (ta + x % per_head) * kCtxTile;  // position of the first row
+        if (x + 1 < x1) request(x + 1);
+        const elem_t* Q = place(x);
+        const float* st = stats + ((x - x0) & 1) * 2 * kCtxTile;
+        if (k0 < bt.keys) {
+            f32x16 s[2], ds[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                s[u] = scores<T>(at, Q, 32 * u, own_k);
+                ds[u] = scores<T>(at, Q + kTile, 32 * u, own_v);
             }
-        }
-        if (x == x0 || (BIAS && x % per_head == 0)) workgroup_barrier();
-        if (x + 1 < x1) load(x + 1);
-        const elem_t* Q = tiles + at * 2 * kTile;
-        const float* st = stats + at * 2 * kCtxTile;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int q0 = r0 + 32 * u, p0 = bt.start + q0;  // position of the first row
-            if (k0 >= bt.keys || (p.causal && k0 > p0 + 31)) continue;
-            f32x16 s = scores<T, HD>(Q, 32 * u, own_k, lane), ds = scores<T, HD>(Q + kTile, 32 * u, own_v, lane);
-            f32x4 lse[4], delta[4];
+            for (int u = 0; u < 2; ++u) {
+                const float* bias = bias_row;
+                float one = 0.0f;
+                if constexpr (BIAS && decltype(band)::value == kNear)
+                    bias += row_entry(p, key - p0 - 32 * u - 4 * h - 27, 28) + 27;
+                else if constexpr (BIAS) one = bias_row[band == kBelow ? 0 : entries - 1];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                lse[i] = *reinterpret_cast<const f32x4*>(st + 32 * u + 8 * i + 4 * h);
-                delta[i] = *reinterpret_cast<const f32x4*>(st + kCtxTile + 32 * u + 8 * i + 4 * h);
-            }
-            if constexpr (BIAS) {
-                const CtxBand band = ctx_band(p, k0 - p0 - 31, k0 + 31 - p0);
-                if (band == kNear) {
-                    const float* row = bias_row + (key - p0 - 4 * h + p.far + kCtxPad);
+                for (int i = 0; i < 4; ++i) {
+                    const f32x4 lse = *reinterpret_cast<const f32x4*>(st + 32 * u + 8 * i + 4 * h);
+                    const f32x4 delta = *reinterpret_cast<const f32x4*>(st + kCtxTile + 32 * u + 8 * i + 4 * h);
 #pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        s[r] = fast_exp2(__builtin_fmaf(s[r], p.c, row[-(8 * (r >> 2) + (r & 3))]) - lse[r >> 2][r & 3]);
-                } else {
-                    const float one = bias_row[band == kBelow ? 0 : entries - 1];
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) s[r] = fast_exp2(__builtin_fmaf(s[r], p.c, one - lse[r >> 2][r & 3]));
+                    for (int j = 0; j < 4; ++j) {
+                        float y = s[u][4 * i + j];
+                        if constexpr (BIAS && decltype(band)::value == kNear) y = fast_exp2(__builtin_fmaf(y, p.c, bias[-(8 * i + j)]) - lse[j]);
+                        else y = fast_exp2(__builtin_fmaf(y, p.c, one - lse[j]));
+                        s[u][4 * i + j] = y;
+                        ds[u][4 * i + j] = y * (ds[u][4 * i + j] - delta[j]);
+                    }
                 }
-            } else {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] = fast_exp2(__builtin_fmaf(s[r], p.c, -lse[r >> 2][r & 3]));
             }
 #pragma unroll
-            for (int r = 0; r < 16; ++r) ds[r] = s[r] * (ds[r] - delta[r >> 2][r & 3]);
-            add_columns<T, HD>(dv, Q + kTile, 32 * u, s, lane);
-            add_columns<T, HD>(dk, Q, 32 * u, ds, lane);
+            for (int u = 0; u < 2; ++u) {
+                add_columns<T>(dv, at, Q + kTile, 32 * u, s[u]);
+                add_columns<T>(dk, at, Q, 32 * u, ds[u]);
+            }
         }
-        if (x + 1 < x1) store(1 - at);
+        if (x + 1 < x1) deliver(x + 1);
+        qf.arrived();
         workgroup_barrier();
+    };
+    // the rows of a head one after another: first those that lie far behind the keys, then those near them, then those far ahead
+    const int kb0 = kb * kCtxOwned - bt.start;
+    const int n_above = max(0, tiles_before(kb0 - p.far + 1, tb) - ta), n_near = max(n_above, tiles_before(kb0 + kCtxOwned - 1 + p.far + kCtxTile - 1, tb) - ta);
+    if (!BIAS && x0 < x1) workgroup_barrier();
+    for (int x = x0; x < x1;) {
+        const int g = x / per_head, first = g * per_head, end = min(x1, first + per_head);
+        if constexpr (BIAS) {
+            // (every wave is behind the barrier of the last tile)
+            fill_bias_row(p, bias_row, hk * p.G + g, tid, kCtxThreads);
+            workgroup_barrier();
+            for (; x < min(first + n_above, end); ++x) tile(x, InBand<kAbove>{});
+            for (; x < min(first + n_near, end); ++x) tile(x, InBand<kNear>{});
+        }
+        for (; x < end; ++x) tile(x, InBand<kBelow>{});
     }
     const bool scored = ok && bt.any_scored(p);
     const int out_rows = min(max(p.Lk - k0, 0), 32);
@@ -339,7 +364,7 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_col(Ctx
         store_part<HD>(dk, scored, p.part + (2 * split * rows + place) * HD, out_rows, lane);
         store_part<HD>(dv, ok, p.part + ((2 * split + 1) * rows + place) * HD, out_rows, lane);
     } else {
-        elem_t* region = tiles + wave * 32 * kCtxLd<HD>;
+        elem_t* region = tiles + wave * 32 * (HD + 8);
         store_rows<T, HD>(dk, scored ? p.scale : 0.0f, p.dk.head(b, hk) + (int64_t)k0 * p.dk.sl, p.dk.sl, out_rows, region, lane, p.D);
         store_rows<T, HD>(dv, ok ? 1.0f : 0.0f, p.dv.head(b, hk) + (int64_t)k0 * p.dv.sl, p.dv.sl, out_rows, region, lane, p.D);
     }

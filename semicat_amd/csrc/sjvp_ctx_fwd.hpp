@@ -7,32 +7,24 @@ namespace sjvp {
 // One pass with the running maximum m and sum l of each row.  Scores are in units of log2.  The maximum that the exponentials
 // refer to is only raised when a row's has grown by more than 2^8: until then the sums keep their scale, which 16-bit
 // probabilities up to 2^8 and fp32 sums hold without loss, and the factors of the accumulators stay out of the loop.
-template <typename T, int HD, bool BIAS>
+template <int HD>
 struct RowSums {
     f32x16 acc[HD / 32];
     float m, ref, l;  // maximum (-inf: no key yet), what is subtracted (finite), sum of this lane's half
 
     __device__ __forceinline__ RowSums() : acc{}, m(-INFINITY), ref(0.0f), l(0.0f) {}
 
-    // s: scores of 32 keys from `key` on.
-    // row: the bias row of this lane's head; pos, least_pos, most_pos: positions of its query, of the wave's first and last.
-    __device__ __forceinline__ void bias(const CtxParams& p, f32x16& s, int key, int h, const float* row, int pos, int least_pos,
-                                         int most_pos) const {
-        const CtxBand band = ctx_band(p, key - most_pos, key + 31 - least_pos);
-        if (band == kNear) {
-            const float* at = row + (key + 4 * h - pos + p.far + kCtxPad);
+    // Scores of 32 keys from `key` on with their bias.  row: the bias row of this lane's head; pos: the position of its query.
+    __device__ __forceinline__ void bias(const CtxParams& p, f32x16& s, int key, int h, const float* row, int pos) const {
+        const float* at = row + row_entry(p, key + 4 * h - pos, 28);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], p.c, at[8 * (r >> 2) + (r & 3)]);
-        } else {
-            const float one = row[band == kBelow ? 0 : 2 * (p.far + kCtxPad)];
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], p.c, one);
-        }
+        for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], p.c, at[8 * (r >> 2) + (r & 3)]);
     }
 
-    // The rows' maxima with these scores.  left: the sequence's keys from `key` on, where they do not fill the scores (masked).
-    template <int N>
-    __device__ __forceinline__ void raise(const CtxParams& p, f32x16 (&s)[N], int left, int h, bool masked) {
+    // The rows' maxima with these scores.  EVEN: they have neither factor nor bias yet, and all have the bias `one`.  left: the
+    // sequence's keys from the first of them on, where they do not fill the scores (masked).
+    template <bool EVEN, int N>
+    __device__ __forceinline__ void raise(const CtxParams& p, f32x16 (&s)[N], float one, int left, int h, bool masked) {
         if (masked) {
 #pragma unroll
             for (int u = 0; u < N; ++u)
@@ -45,7 +37,7 @@ struct RowSums {
         for (int u = 0; u < N; ++u)
 #pragma unroll
             for (int r = u ? 0 : 1; r < 16; ++r) top = fmaxf(top, s[u][r]);
-        if constexpr (!BIAS) top *= p.c;
+        if constexpr (EVEN) top = __builtin_fmaf(top, p.c, one);
         if (__builtin_amdgcn_ballot_w64(top > m + 8.0f)) {
             const float grown = fmaxf(m, halves_max(top));
             const float now = grown == -INFINITY ? 0.0f : grown;
@@ -57,14 +49,15 @@ struct RowSums {
         }
     }
 
-    template <int N>
-    __device__ __forceinline__ void exponentials(const CtxParams& p, f32x16 (&s)[N]) {
+    template <bool EVEN, int N>
+    __device__ __forceinline__ void exponentials(const CtxParams& p, f32x16 (&s)[N], float one) {
+        const float less = one - ref;
         float sum = 0.0f;
 #pragma unroll
         for (int u = 0; u < N; ++u)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                s[u][r] = fast_exp2(BIAS ? s[u][r] - ref : __builtin_fmaf(s[u][r], p.c, -ref));
+                s[u][r] = fast_exp2(EVEN ? __builtin_fmaf(s[u][r], p.c, less) : s[u][r] - ref);
                 sum += s[u][r];
             }
         l += sum;
@@ -74,11 +67,11 @@ struct RowSums {
 __device__ __forceinline__ float ctx_lse(float ref, float l) { return (ref + fast_log2(l)) * kLn2; }
 
 // Many rows: four waves of 32 rows of one head share tiles of 64 keys.  Two tiles of K and V in LDS: the next one is on its way
-// through registers while this one is used, one barrier to a tile.
-template <typename T, int HD, bool BIAS>
+// while this one is used, one barrier to a tile.
+template <typename T, int HD, bool BIAS, bool DMA>
 __global__ __launch_bounds__(kCtxThreads, 2) void ctx_fwd(CtxParams p) {
     extern __shared__ __align__(16) unsigned char smem[];
-    constexpr int kTile = kCtxTile * kCtxLd<HD>;
+    constexpr int kTile = Tile<HD, DMA>::kElems;
     elem_t* tiles = reinterpret_cast<elem_t*>(smem);  // K [2], V [2]
     float* row = reinterpret_cast<float*>(tiles + 4 * kTile);
     const int nqb = p.blocks;
@@ -91,70 +84,85 @@ __global__ __launch_bounds__(kCtxThreads, 2) void ctx_fwd(CtxParams p) {
     const int q0 = qb * kCtxOwned + 32 * wave;
     const int rows = min(max(bt.rows - q0, 0), 32), last = min(bt.rows, (qb + 1) * kCtxOwned) - 1;
     const int n = last >= qb * kCtxOwned ? bt.seen(p, last) : 0, n_wave = rows > 0 ? bt.seen(p, q0 + rows - 1) : 0;
-    const int pos0 = bt.start + q0, pos = pos0 + (lane & 31);
+    const int pos = bt.start + q0 + (lane & 31);
 
     u32x4 own[HD / 16];
     own_operands<HD>(own, p.q.head(b, hq) + (int64_t)(q0 + (lane & 31)) * p.q.sl, (lane & 31) < rows, h, p.D);
     const elem_t *kt = p.k.head(b, hk), *vt = p.v.head(b, hk);
     const int nt = (n + kCtxTile - 1) / kCtxTile;
-    TileCopy<HD> kc(p.k.sl, p.D, tid), vc(p.v.sl, p.D, tid);
-    elem_t* const vtiles = tiles + 2 * kTile;
-    // tile t of K / V on its way, and into its place
-    const auto load_k = [&](int t) { kc.load(kt + (int64_t)t * kCtxTile * p.k.sl, p.k.sl, n - t * kCtxTile, p.D); };
-    const auto load_v = [&](int t) { vc.load(vt + (int64_t)t * kCtxTile * p.v.sl, p.v.sl, n - t * kCtxTile, p.D); };
-    const auto place_k = [&](int t) { kc.store(tiles + (t & 1) * kTile, p.D, tid); };
-    const auto place_v = [&](int t) { vc.store(vtiles + (t & 1) * kTile, p.D, tid); };
-    if (nt) load_k(0), load_v(0);
+    TileFeed<HD, DMA> kf(p.k.sl, p.D, tid), vf(p.v.sl, p.D, tid);
+    const Tile<HD, DMA> at(lane);
+    const auto k_place = [&](int t) { return tiles + (t & 1) * kTile; };
+    const auto v_place = [&](int t) { return tiles + (2 + (t & 1)) * kTile; };
+    const auto k_request = [&](int t) { kf.request(kt + (int64_t)t * kCtxTile * p.k.sl, p.k.sl, n - t * kCtxTile, p.D, k_place(t), wave); };
+    const auto v_request = [&](int t) { vf.request(vt + (int64_t)t * kCtxTile * p.v.sl, p.v.sl, n - t * kCtxTile, p.D, v_place(t), wave); };
+    const auto k_deliver = [&](int t) { kf.deliver(k_place(t), p.D, tid); };
+    const auto v_deliver = [&](int t) { vf.deliver(v_place(t), p.D, tid); };
+    if (nt) k_request(0), v_request(0);
     if constexpr (BIAS) fill_bias_row(p, row, hq, tid, kCtxThreads);
     if (nt) {
-        place_k(0), place_v(0);
-        if (nt > 1) load_k(1);
+        k_deliver(0), v_deliver(0);
+        if (nt > 1) k_request(1);
     }
+    kf.arrived();
     workgroup_barrier();
-    RowSums<T, HD, BIAS> st;
+    RowSums<HD> st;
     f32x16 s[2], next[2];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) s[u] = scores<T, HD>(tiles, 32 * u, own, lane);
-    if (nt > 1) place_k(1);
+    for (int u = 0; u < 2; ++u) s[u] = scores<T>(at, tiles, 32 * u, own);
+    if (nt > 1) k_deliver(1);
     workgroup_barrier();
     // Scores of one tile are contracted beside the exponentials of the one before, which the vector unit is busy with.
-    // The sequence's last tile may need a mask and has code of its own behind the loop (as a condition within, the compiler makes the
+    // The sequence's last tile may need a mask and has code of its own behind the loops (as a condition within, the compiler makes the
     // mask a select in every tile, a third of the vector instructions at D = 64).
-    const auto tile = [&](int t, bool masked, auto more) {
+    const auto tile = [&](int t, bool masked, auto more, auto band) {
+        constexpr bool kEven = decltype(band)::value != kNear;
         const int key = t * kCtxTile;
         if (more) {
-            if (t + 2 < nt) load_k(t + 2);
-            load_v(t + 1);
+            if (t + 2 < nt) k_request(t + 2);
+            v_request(t + 1);
         }
         if (key < n_wave) {
-            if constexpr (BIAS) {
+            const float one = !BIAS ? 0.0f : row[band == kBelow ? 0 : 2 * (p.far + kCtxPad)];
+            if constexpr (!kEven) {
 #pragma unroll
-                for (int u = 0; u < 2; ++u) st.bias(p, s[u], key + 32 * u, h, row, pos, pos0, pos0 + 31);
+                for (int u = 0; u < 2; ++u) st.bias(p, s[u], key + 32 * u, h, row, pos);
             }
-            st.raise(p, s, bt.keys - key, h, masked);
+            st.template raise<kEven>(p, s, one, bt.keys - key, h, masked);
             if constexpr (more) {
 #pragma unroll
-                for (int u = 0; u < 2; ++u) next[u] = scores<T, HD>(tiles + ((t + 1) & 1) * kTile, 32 * u, own, lane);
+                for (int u = 0; u < 2; ++u) next[u] = scores<T>(at, k_place(t + 1), 32 * u, own);
             }
-            st.exponentials(p, s);
+            st.template exponentials<kEven>(p, s, one);
 #pragma unroll
-            for (int u = 0; u < 2; ++u) add_columns<T, HD>(st.acc, vtiles + (t & 1) * kTile, 32 * u, s[u], lane);
+            for (int u = 0; u < 2; ++u) add_columns<T>(st.acc, at, v_place(t), 32 * u, s[u]);
             if constexpr (more) s[0] = next[0], s[1] = next[1];
         }
         if (more) {
-            if (t + 2 < nt) place_k(t + 2);
-            place_v(t + 1);
+            if (t + 2 < nt) k_deliver(t + 2);
+            v_deliver(t + 1);
         }
+        kf.arrived();
         workgroup_barrier();
     };
-    for (int t = 0; t + 1 < nt; ++t) tile(t, false, std::true_type{});
-    if (nt) tile(nt - 1, nt * kCtxTile > bt.keys, std::false_type{});
+    const std::true_type more;
+    if constexpr (BIAS) {
+        const int first = bt.start + qb * kCtxOwned;
+        const int near = tiles_before(first - p.far + 1, nt - 1), above = tiles_before(first + kCtxOwned - 1 + p.far + kCtxTile - 1, nt - 1);
+        int t = 0;
+        for (; t < near; ++t) tile(t, false, more, InBand<kBelow>{});
+        for (; t < above; ++t) tile(t, false, more, InBand<kNear>{});
+        for (; t + 1 < nt; ++t) tile(t, false, more, InBand<kAbove>{});
+    } else {
+        for (int t = 0; t + 1 < nt; ++t) tile(t, false, more, InBand<kBelow>{});
+    }
+    if (nt) tile(nt - 1, nt * kCtxTile > bt.keys, std::false_type{}, InBand<BIAS ? kNear : kBelow>{});
     const int out_rows = min(max(p.Lq - q0, 0), 32);
     const float both = halves_sum(st.l), l = (lane & 31) < rows ? both : 0.0f;
     const float f = l == 0.0f ? 0.0f : 1.0f / l;
     if (p.lse && h == 0 && (lane & 31) < out_rows)
         p.lse[((int64_t)b * p.Hq + hq) * p.Lq + q0 + lane] = l == 0.0f ? -INFINITY : ctx_lse(st.ref, l);
-    elem_t* region = tiles + wave * 32 * kCtxLd<HD>;
+    elem_t* region = tiles + wave * 32 * (HD + 8);
     store_rows<T, HD>(st.acc, f, p.o.head(b, hq) + (int64_t)q0 * p.o.sl, p.o.sl, out_rows, region, lane, p.D);
 }
 
@@ -162,12 +170,12 @@ __global__ __launch_bounds__(kCtxThreads, 2) void ctx_fwd(CtxParams p) {
 // waves share out the keys: each runs over tiles of 32 keys of its own, K straight from memory into the operand's registers, V through a
 // region of LDS that no other wave reads, so that nothing but the end is synchronised.  The sums of the waves are
 // joined in LDS; with several splits of the key axis they go to memory for ctx_join.
-// `packed` heads of a group stand in one block's rows: all of them, or one where their bias rows would not fit, or where a head has
-// 32 rows or more (so that the positions in a block lie within 31 of each other).
+// `packed` heads of a group stand in one block's rows: all of them, or one where their bias rows would not fit or a head
+// fills a block by itself.
 template <typename T, int HD, bool BIAS, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, HD <= 64 ? 3 : 2) void ctx_fwd_few(CtxParams p) {
     extern __shared__ __align__(16) unsigned char smem[];
-    constexpr int kRegion = 32 * kCtxLd<HD>, kSum = HD + 4;
+    constexpr int kRegion = 32 * (HD + 8), kSum = HD + 4;
     elem_t* region = reinterpret_cast<elem_t*>(smem);  // [WAVES] V tiles, then the waves' sums [WAVES][32][HD + 4] fp32
     float* sums = reinterpret_cast<float*>(smem);
     float* stats = sums + WAVES * 32 * kSum;       // [WAVES][32] maximum, then sum
@@ -218,14 +226,15 @@ __global__ __launch_bounds__(64 * WAVES, HD <= 64 ? 3 : 2) void ctx_fwd_few(CtxP
         row = bias_rows + (g - g0) * entries;
         workgroup_barrier();
     }
-    RowSums<T, HD, BIAS> st;
+    RowSums<HD> st;
     elem_t* V = region + wave * kRegion;
+    const Tile<HD, false> tile(lane);
     for (; t < t_end; t += WAVES) {
 #pragma unroll
         for (int x = 0; x < NV; ++x) {
             const int at = lane + 64 * x;
             if (p.D % 8) vr[x] = chunk_shifted(vr[x], 8 * (at % CH), p.D);
-            *reinterpret_cast<u32x4*>(V + (at / CH) * kCtxLd<HD> + 8 * (at % CH)) = vr[x];
+            *reinterpret_cast<u32x4*>(V + (at / CH) * (HD + 8) + 8 * (at % CH)) = vr[x];
         }
         if (p.D % 8) {
 #pragma unroll
@@ -236,11 +245,11 @@ __global__ __launch_bounds__(64 * WAVES, HD <= 64 ? 3 : 2) void ctx_fwd_few(CtxP
         for (int c = 0; c < HD / 16; ++c) s[0] = Mma32<T>::run(kr[c], own[c], s[0]);
         if (t + WAVES < t_end) load(t + WAVES);
         const int key = t * 32;
-        if constexpr (BIAS) st.bias(p, s[0], key, h, row, pos, bt.start + i_first, bt.start + i_last);
-        st.raise(p, s, bt.keys - key, h, key + 32 > bt.keys);
-        st.exponentials(p, s);
+        if constexpr (BIAS) st.bias(p, s[0], key, h, row, pos);
+        st.template raise<!BIAS>(p, s, 0.0f, bt.keys - key, h, key + 32 > bt.keys);
+        st.template exponentials<!BIAS>(p, s, 0.0f);
         wave_exchange();
-        add_columns<T, HD>(st.acc, V, 0, s[0], lane);
+        add_columns<T>(st.acc, tile, V, 0, s[0]);
         wave_exchange();
     }
     const float l = halves_sum(st.l);

@@ -10,10 +10,11 @@ template <>
 int ctx_forward<SJVP_T>(CtxParams p, const CtxPlan& plan, hipStream_t stream) {
     p.blocks = plan.blocks, p.splits = plan.splits;
     const int grid = (int)ctx_grid((int)plan.units, (int)plan.inner);
-    return ctx_by_head(p.D, [&](auto hd) {
+    return ctx_by_head(p.D, plan.dma, [&](auto hd, auto dma) {
         constexpr int HD = decltype(hd)::value;
-        if (!plan.few) return p.table ? launch(ctx_fwd<SJVP_T, HD, true>, grid, plan.smem, stream, p, kCtxThreads)
-                                      : launch(ctx_fwd<SJVP_T, HD, false>, grid, plan.smem, stream, p, kCtxThreads);
+        constexpr bool DMA = decltype(dma)::value;
+        if (!plan.few) return p.table ? launch(ctx_fwd<SJVP_T, HD, true, DMA>, grid, plan.smem, stream, p, kCtxThreads)
+                                      : launch(ctx_fwd<SJVP_T, HD, false, DMA>, grid, plan.smem, stream, p, kCtxThreads);
         p.packed = plan.packed;
         const auto few = [&](auto waves) {
             constexpr int W = decltype(waves)::value;
