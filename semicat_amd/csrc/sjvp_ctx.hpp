@@ -69,13 +69,23 @@ struct CtxParams {
     int splits, blocks;                      // splits of the looped axis; workgroups of a split over the owned axis
     int packed;                              // ctx_fwd_few: heads to a block of rows
     int skew;                                // ctx_bwd_row: byte offset of its scratch for the bucket sums in LDS
-    uint16_t first[kCtxBuckets];             // first distance of each bucket
+    alignas(4) uint16_t first[kCtxBuckets];  // first distance of each bucket
 };
 
 // max / sum over the two lanes of a column
 __device__ __forceinline__ float halves_max(float x) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+// sum over 16 neighbouring lanes, in all of them
+__device__ __forceinline__ float sum16(float x) {
+    const auto turned = [](float y, auto by) {
+        return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(y), 0x120 | decltype(by)::value, 0xf, 0xf, false));
+    };
+    x += turned(x, std::integral_constant<int, 8>{});
+    x += turned(x, std::integral_constant<int, 4>{});
+    x += turned(x, std::integral_constant<int, 2>{});
+    return x + turned(x, std::integral_constant<int, 1>{});
 }
 __device__ __forceinline__ float halves_sum(float x) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -238,16 +248,16 @@ struct TileFeed {
 };
 
 // The bucket of a position difference (key minus query): the last bucket whose first distance is not beyond the distance;
-// differences above zero have distances and buckets of their own (`both`) or distance 0.
+// differences above zero have distances and buckets of their own (`both`) or distance 0.  The first distances are the same for all
+// lanes and come as scalars, so counting them is quicker than a search, whose every step would wait for memory.
 __device__ __forceinline__ int ctx_bucket(const CtxParams& p, int rel) {
-    const int d = min(p.both ? abs(rel) : max(-rel, 0), p.far);
-    int lo = 0, hi = p.buckets;  // first[lo] <= d < first[hi]
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (p.first[mid] <= d) lo = mid;
-        else hi = mid;
+    const int d = p.both ? abs(rel) : max(-rel, 0);
+    int bucket = -1;
+    for (int i = 0; i < p.buckets; i += 2) {
+        const uint32_t two = reinterpret_cast<const uint32_t*>(p.first)[i / 2];
+        bucket += (d >= (int)(two & 0xffffu)) + (i + 1 < p.buckets && d >= (int)(two >> 16));
     }
-    return lo + (p.both && rel > 0 ? p.buckets : 0);
+    return bucket + (p.both && rel > 0 ? p.buckets : 0);
 }
 
 __device__ __forceinline__ float ctx_table(const CtxParams& p, int bucket, int head) {

@@ -11,9 +11,8 @@
 namespace sjvp {
 
 __device__ __forceinline__ float wave_sum(float x) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
-    return x;
+    x = halves_sum(sum16(x));
+    return x + __shfl_xor(x, 16);
 }
 
 // dO . O of the lane's own row, from the operands of dO and from O in memory
@@ -76,17 +75,6 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_row(Ctx
     float* hist = row + entries + wave * entries;  // the wave's sums of dS by difference
     float* skew = reinterpret_cast<float*>(smem + p.skew) + wave * kSkewFloats;
 
-    const int64_t stat = ((int64_t)b * p.Hq + hq) * p.Lq + qi;
-    float lse = -INFINITY;
-    if ((lane & 31) < rows) lse = p.lse[stat];
-    const bool ok = lse != -INFINITY;           // a row that sees no key has no gradient,
-    const bool scored = ok && limit != 1;       // one that sees one key none of its score: exactly none, not what rounding leaves
-    lse = ok ? lse * kLog2e : INFINITY;
-    u32x4 own_q[HD / 16], own_g[HD / 16];
-    own_operands<HD>(own_q, p.q.head(b, hq) + (int64_t)qi * p.q.sl, ok, h, p.D);
-    own_operands<HD>(own_g, p.g.head(b, hq) + (int64_t)qi * p.g.sl, ok, h, p.D);
-    const float delta = row_delta<T, HD>(p, own_g, p.o.head(b, hq) + (int64_t)qi * p.o.sl, ok, h);
-
     const elem_t *kt = p.k.head(b, hk), *vt = p.v.head(b, hk);
     TileFeed<HD, DMA> kf(p.k.sl, p.D, tid), vf(p.v.sl, p.D, tid);
     const Tile<HD, DMA> at(lane);
@@ -99,15 +87,27 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_row(Ctx
         kf.deliver(place(t), p.D, tid);
         vf.deliver(place(t) + kTile, p.D, tid);
     };
-    if (t0 < t1) {
-        request(t0);
-        deliver(t0);
-    }
+    if (t0 < t1) request(t0);
+    const int64_t stat = ((int64_t)b * p.Hq + hq) * p.Lq + qi;
+    const bool mine = (lane & 31) < rows;
+    float lse = mine ? p.lse[stat] : -INFINITY;
+    u32x4 own_q[HD / 16], own_g[HD / 16];
+    own_operands<HD>(own_q, p.q.head(b, hq) + (int64_t)qi * p.q.sl, mine, h, p.D);
+    own_operands<HD>(own_g, p.g.head(b, hq) + (int64_t)qi * p.g.sl, mine, h, p.D);
     if constexpr (BIAS) {
         fill_bias_row(p, row, hq, tid, kCtxThreads);
         for (int x = lane; x < entries; x += 64) hist[x] = 0.0f;
         for (int x = lane; x < kSkewFloats; x += 64) skew[x] = 0.0f;
     }
+    const bool ok = lse != -INFINITY;      // a row that sees no key has no gradient, whatever its cotangent,
+    const bool scored = ok && limit != 1;  // one that sees one key none of its score: exactly none, not what rounding leaves
+    lse = ok ? lse * kLog2e : INFINITY;
+    if (__builtin_amdgcn_ballot_w64(mine && !ok)) {
+#pragma unroll
+        for (int c = 0; c < HD / 16; ++c) own_g[c] = ok ? own_g[c] : u32x4{0u, 0u, 0u, 0u};
+    }
+    const float delta = row_delta<T, HD>(p, own_g, p.o.head(b, hq) + (int64_t)qi * p.o.sl, ok, h);
+    if (t0 < t1) deliver(t0);
     kf.arrived();
     workgroup_barrier();
     // scores of 32 keys from k0 on to P, zero behind the sequence (masked)
@@ -208,20 +208,32 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_row(Ctx
     if (!p.tpart) return;
     // the tiles whose differences were summed one by one, the last among them
     const int t_near = min(near, whole), n_near = max(0, min(above, whole) - t_near), again = n_near + (t1 - whole);
+    const auto key_of = [&](int i) { return (i < n_near ? t_near + i : whole) * kCtxTile; };
+    const auto again_place = [&](int i) { return tiles + (i & 1) * kTile; };
+    const auto again_request = [&](int i) {
+        kf.request(kt + (int64_t)key_of(i) * p.k.sl, p.k.sl, n - key_of(i), p.D, again_place(i), wave);
+    };
+    workgroup_barrier();
+    if (again) {
+        again_request(0);
+        kf.deliver(again_place(0), p.D, tid);
+    }
+    kf.arrived();
+    workgroup_barrier();
     for (int i = 0; i < again; ++i) {
-        const int key = (i < n_near ? t_near + i : whole) * kCtxTile;
-        workgroup_barrier();
-        kf.request(kt + (int64_t)key * p.k.sl, p.k.sl, n - key, p.D, tiles, wave);
-        kf.deliver(tiles, p.D, tid);
+        const int key = key_of(i);
+        if (i + 1 < again) again_request(i + 1);
+        if (key < n_wave) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                f32x16 s = scores<T>(at, again_place(i), 32 * u, own_q);
+                row_probabilities(s, key + 32 * u, InBand<kNear>{}, key + kCtxTile > bt.keys);
+                add_diagonals(skew, hist + row_entry(p, key + 32 * u - pos0 - 31, 63), s, -residue, lane);
+            }
+        }
+        if (i + 1 < again) kf.deliver(again_place(i + 1), p.D, tid);
         kf.arrived();
         workgroup_barrier();
-        if (key >= n_wave) continue;
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            f32x16 s = scores<T>(at, tiles, 32 * u, own_q);
-            row_probabilities(s, key + 32 * u, InBand<kNear>{}, key + kCtxTile > bt.keys);
-            add_diagonals(skew, hist + row_entry(p, key + 32 * u - pos0 - 31, 63), s, -residue, lane);
-        }
     }
     {
         const float below = wave_sum(ds_below - residue * p_below), above_sum = wave_sum(ds_above - residue * p_above);
@@ -230,17 +242,17 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_row(Ctx
         const float* hists = row + entries;
         const int nb = p.both ? 2 * p.buckets : p.buckets, zero = p.far + kCtxPad;
         float* out = p.tpart + (((int64_t)hq * p.B + b) * nqb * p.splits + (int64_t)qb * p.splits + split) * nb;
-        for (int bucket = wave; bucket < nb; bucket += kCtxWaves) {
-            const int side = bucket >= p.buckets, j = bucket - side * p.buckets;
+        for (int bucket = tid / 16; bucket < (nb + 15) / 16 * 16; bucket += kCtxThreads / 16) {  // 16 lanes to a bucket
+            const int side = bucket >= p.buckets, j = min(bucket - side * p.buckets, p.buckets - 1);
             const int from = p.first[j], to = j + 1 < p.buckets ? p.first[j + 1] - 1 : zero;  // distances
-            int lo = side ? zero + max(from, 1) : zero - to, hi = side ? zero + to : zero - from;
-            if (!p.both && j == 0) hi = entries - 1;  // differences above zero count as distance 0
+            const int lo = side ? zero + max(from, 1) : zero - to;
+            const int hi = side ? zero + to : !p.both && j == 0 ? entries - 1 : zero - from;  // (above zero: distance 0)
             float sum = 0.0f;
-            for (int x = lo + lane; x <= hi; x += 64)
+            for (int x = lo + (lane & 15); x <= hi; x += 16)
 #pragma unroll
                 for (int k = 0; k < kCtxWaves; ++k) sum += hists[k * entries + x];
-            sum = wave_sum(sum);
-            if (lane == 0) out[bucket] = bt.any_scored(p) ? sum : 0.0f;
+            sum = sum16(sum);
+            if ((lane & 15) == 0 && bucket < nb) out[bucket] = bt.any_scored(p) ? sum : 0.0f;
         }
     }
 }
