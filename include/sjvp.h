@@ -291,20 +291,23 @@ int sjvp_cast(int n, const void* const* x, void* const* y, const int64_t* count,
  *       distances in ascending order from 0, the last one at most SJVP_CTX_MAX_DISTANCE; a distance has the last bucket that does
  *       not begin beyond it.  bidirectional: keys behind a query (j > start + i) have buckets of their own,
  *       buckets .. 2 buckets - 1, by their distance; otherwise they count as distance 0.
+ *   o_rest (or NULL)   what the rounding of o left, in o's type.  A forward that is given it forms o with probabilities of 16 bits or
+ *       more and stores it; the backward needs it for rowsum(dO * o), of which dS is a small difference where attention is
+ *       sharp, and which the gradient of an fp32 table (formed to some 1e-6 with it) is a sum over.
  *   lse   [B,Hq,Lq] fp32 contiguous; the forward takes NULL where no backward follows.
  *   dk, dv   both or neither (then without the launch that makes them)
- *   dtable (or NULL)   in the type of table, with strides dtable_stride; summed in fp32 in a fixed order; that of an fp32 table is formed to fp32 accuracy.
+ *   dtable (or NULL)   in the type of table, with strides dtable_stride; summed in fp32 in a fixed order.
  * strides[3*i + {0,1,2}]: (batch, head, sequence) strides in elements of tensor i of sjvp_ctx_tensor.  scale 0: 1/sqrt(D).
  * The workspace is device memory of sjvp_ctx_workspace_bytes() bytes, 16-byte aligned (0: none is needed).
  * No counterpart in the reference, whose attention has one length, no mask and no bias.
  */
 #define SJVP_CTX_MAX_BUCKETS 256   /* of one direction */
 #define SJVP_CTX_MAX_DISTANCE 1024
-enum sjvp_ctx_tensor { SJVP_C_Q = 0, SJVP_C_K, SJVP_C_V, SJVP_C_O, SJVP_C_DO, SJVP_C_DQ, SJVP_C_DK, SJVP_C_DV,
+enum sjvp_ctx_tensor { SJVP_C_Q = 0, SJVP_C_K, SJVP_C_V, SJVP_C_O, SJVP_C_O_REST, SJVP_C_DO, SJVP_C_DQ, SJVP_C_DK, SJVP_C_DV,
                        SJVP_C_COUNT };
 typedef struct sjvp_ctx {
     const void *q, *k, *v;
-    void* o;
+    void *o, *o_rest;
     const void* dO;
     void *dq, *dk, *dv;
     int64_t strides[SJVP_C_COUNT * 3];

@@ -39,7 +39,7 @@ F_TENSORS = ("q", "k", "v", "tq", "tk", "tv", "o", "to")
 B_TENSORS = ("q", "k", "v", "tq", "tk", "tv", "o", "to", "dO", "dTO",
              "dq", "dk", "dv", "dtq", "dtk", "dtv")
 
-C_TENSORS = ("q", "k", "v", "o", "dO", "dq", "dk", "dv")
+C_TENSORS = ("q", "k", "v", "o", "o_rest", "dO", "dq", "dk", "dv")
 SJVP_CTX_MAX_BUCKETS = 256
 SJVP_CTX_MAX_DISTANCE = 1024
 SJVP_CTX_MAX_POSITION = 1 << 29

@@ -124,7 +124,7 @@ def _check_inputs(q, k, v, bias, key_lengths, query_lengths, query_start) -> Non
 
 
 def _call(backward: bool, tensors, lse, bias, key_lengths, query_lengths, query_start, scale, dtable=None) -> None:
-    """``tensors``: q, k, v, o, dO, dq, dk, dv, as the C ABI orders them."""
+    """``tensors``: q, k, v, o, o_rest, dO, dq, dk, dv, as the C ABI orders them."""
     q, k = tensors[0], tensors[1]
     ptr = lambda t: None if t is None else t.data_ptr()
     t = _lib.Ctx()
@@ -160,33 +160,40 @@ def _call(backward: bool, tensors, lse, bias, key_lengths, query_lengths, query_
 
 def context_forward(q: Tensor, k: Tensor, v: Tensor, bias: Optional[RelativeBias] = None, key_lengths: Optional[Tensor] = None,
                     query_lengths: Optional[Tensor] = None, query_start: Union[int, Tensor] = 0, scale: Optional[float] = None,
-                    o: Optional[Tensor] = None, with_lse: bool = True) -> Tuple[Tensor, Optional[Tensor]]:
+                    o: Optional[Tensor] = None, o_rest: Optional[Tensor] = None, with_lse: bool = True
+                    ) -> Tuple[Tensor, Optional[Tensor]]:
     """Forward on ``[B,H,L,D]`` views: ``(o, lse)``, with ``lse`` fp32 ``[B,Hq,Lq]``, or None without ``with_lse``.  ``o`` may be
-    passed in to be filled."""
+    passed in to be filled, and ``o_rest``, a tensor like it, to receive what the rounding of ``o`` leaves, for
+    :func:`context_backward`."""
     _check_inputs(q, k, v, bias, key_lengths, query_lengths, query_start)
     B, H, Lq, D = q.shape
     if o is None:
         o = torch.empty((B, Lq, H, D), device=q.device, dtype=q.dtype).transpose(1, 2)
     _check("o", o, q.shape, q)
+    if o_rest is not None:
+        _check("o_rest", o_rest, q.shape, q)
     lse = torch.empty((B, H, Lq), device=q.device, dtype=torch.float32) if with_lse else None
     if q.numel() == 0 or k.numel() == 0:  # no row, or no key for any row
+        if o_rest is not None:
+            o_rest.zero_()
         return o.zero_(), None if lse is None else lse.fill_(-float("inf"))
-    _call(False, (q, k, v, o, None, None, None, None), lse, bias, key_lengths, query_lengths, query_start, scale)
+    _call(False, (q, k, v, o, o_rest, None, None, None, None), lse, bias, key_lengths, query_lengths, query_start, scale)
     return o, lse
 
 
 def context_backward(q: Tensor, k: Tensor, v: Tensor, o: Tensor, lse: Tensor, dO: Tensor, bias: Optional[RelativeBias] = None,
                      key_lengths: Optional[Tensor] = None, query_lengths: Optional[Tensor] = None,
-                     query_start: Union[int, Tensor] = 0, scale: Optional[float] = None,
+                     query_start: Union[int, Tensor] = 0, scale: Optional[float] = None, o_rest: Optional[Tensor] = None,
                      with_keys: bool = True, with_table: bool = True
                      ) -> Tuple[Tensor, Optional[Tensor], Optional[Tensor], Optional[Tensor]]:
     """Backward on ``[B,H,L,D]`` views for the cotangent ``dO``, with the forward's arguments and results:
-    ``(dq, dk, dv, dtable)``.  ``with_keys=False`` leaves out dk and dv (frozen states), ``with_table=False`` the table's."""
+    ``(dq, dk, dv, dtable)``.  Without ``o_rest`` the row sums of ``dO * o`` carry the rounding of ``o``, which the gradients of
+    sharp rows and of a float32 table show.  ``with_keys=False`` leaves out dk and dv (frozen states), ``with_table=False`` the table's."""
     _check_inputs(q, k, v, bias, key_lengths, query_lengths, query_start)
     B, H, Lq, D = q.shape
     if dO.stride(-1) != 1 or dO.stride(2) >= 1 << 24:
         dO = dO.contiguous()
-    for name, t in (("o", o), ("dO", dO)):
+    for name, t in (("o", o), ("dO", dO)) + ((("o_rest", o_rest),) if o_rest is not None else ()):
         _check(name, t, q.shape, q)
     if tuple(lse.shape) != (B, H, Lq) or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != q.device:
         raise AssertionError(f"lse must be a contiguous float32 tensor of shape {(B, H, Lq)}, got {tuple(lse.shape)} {lse.dtype}")
@@ -195,7 +202,7 @@ def context_backward(q: Tensor, k: Tensor, v: Tensor, o: Tensor, lse: Tensor, dO
     dtable = torch.empty(bias.table.shape, device=q.device, dtype=bias.table.dtype) if bias is not None and with_table else None
     if q.numel() == 0 or k.numel() == 0:
         return tuple(None if t is None else t.zero_() for t in (dq, dk, dv, dtable))
-    _call(True, (q, k, v, o, dO, dq, dk, dv), lse, bias, key_lengths, query_lengths, query_start, scale, dtable)
+    _call(True, (q, k, v, o, o_rest, dO, dq, dk, dv), lse, bias, key_lengths, query_lengths, query_start, scale, dtable)
     return dq, dk, dv, dtable
 
 
@@ -205,27 +212,28 @@ class ContextAttentionFunction(torch.autograd.Function):
     @staticmethod
     def forward(q, k, v, table, key_lengths, query_lengths, query_start, scale, max_distance, bidirectional, causal):
         bias = None if table is None else RelativeBias(table, max_distance, bidirectional, causal)
+        rest = torch.empty(q.shape, device=q.device, dtype=q.dtype)
         o, lse = context_forward(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), bias, key_lengths, query_lengths,
-                                 query_start, scale)
-        return o.transpose(1, 2), lse
+                                 query_start, scale, o_rest=rest.transpose(1, 2))
+        return o.transpose(1, 2), lse, rest
 
     @staticmethod
     def setup_context(ctx, inputs, output) -> None:
         q, k, v, table, key_lengths, query_lengths, query_start, *ctx.options = inputs
-        o, lse = output
+        o, lse, rest = output
         ctx.start = None if isinstance(query_start, Tensor) else query_start
-        ctx.save_for_backward(q, k, v, table, key_lengths, query_lengths, None if ctx.start is not None else query_start, o, lse)
-        ctx.mark_non_differentiable(lse)
+        ctx.save_for_backward(q, k, v, table, key_lengths, query_lengths, None if ctx.start is not None else query_start, o, lse, rest)
+        ctx.mark_non_differentiable(lse, rest)
         ctx.set_materialize_grads(False)
 
     @staticmethod
     def backward(ctx, d_o, *_):
         if d_o is None:
             return (None,) * 11
-        q, k, v, table, key_lengths, query_lengths, query_start, o, lse = ctx.saved_tensors
+        q, k, v, table, key_lengths, query_lengths, query_start, o, lse, rest = ctx.saved_tensors
         needs = ctx.needs_input_grad
         grads = ContextAttentionBackwardFunction.apply(
-            q, k, v, table, o, lse, d_o, key_lengths, query_lengths, query_start if ctx.start is None else ctx.start,
+            q, k, v, table, o, lse, rest, d_o, key_lengths, query_lengths, query_start if ctx.start is None else ctx.start,
             *ctx.options, needs[1] or needs[2], needs[3])
         return *(g if need else None for g, need in zip(grads, needs)), *(None,) * 7
 
@@ -234,12 +242,12 @@ class ContextAttentionBackwardFunction(torch.autograd.Function):
     """Gradients of q, k, v and the table for the cotangent of the output."""
 
     @staticmethod
-    def forward(q, k, v, table, o, lse, d_o, key_lengths, query_lengths, query_start, scale, max_distance,
+    def forward(q, k, v, table, o, lse, rest, d_o, key_lengths, query_lengths, query_start, scale, max_distance,
                 bidirectional, causal, with_keys, with_table):
         bias = None if table is None else RelativeBias(table, max_distance, bidirectional, causal)
-        heads = [None if t is None else t.transpose(1, 2) for t in (q, k, v, o, d_o)]
+        heads = [None if t is None else t.transpose(1, 2) for t in (q, k, v, o, d_o, rest)]
         dq, dk, dv, dtable = context_backward(*heads[:4], lse, heads[4], bias, key_lengths, query_lengths, query_start, scale,
-                                              with_keys=with_keys, with_table=with_table)
+                                              o_rest=heads[5], with_keys=with_keys, with_table=with_table)
         return *(None if t is None else t.transpose(1, 2) for t in (dq, dk, dv)), dtable
 
     @staticmethod
@@ -266,7 +274,7 @@ def _attend(q, k, v, table, key_lengths, query_lengths, query_start, scale, max_
         # the dtype policy of safe_sdpa_jvp: computed in bfloat16, handed back in the caller's type
         q, k, v = (t.to(torch.bfloat16) for t in (q, k, v))
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, table)):
-        o, _ = ContextAttentionFunction.apply(q, k, v, table, key_lengths, query_lengths, query_start, scale, max_distance,
+        o, _, _ = ContextAttentionFunction.apply(q, k, v, table, key_lengths, query_lengths, query_start, scale, max_distance,
                                               bidirectional, causal)
     else:
         bias = None if table is None else RelativeBias(table, max_distance, bidirectional, causal)

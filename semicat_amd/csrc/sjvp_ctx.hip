@@ -73,8 +73,7 @@ CtxPlan ctx_plan_row(const CtxParams& p) {
     CtxPlan plan;
     plan.blocks = (int)ceil_div(p.Lq, kCtxOwned);
     plan.units = (int64_t)p.B * p.Hkv;
-    // (the bucket sums need a row's whole residue, see ctx_bwd_row)
-    plan.splits = p.tpart ? 1 : splits_for((int64_t)p.B * p.Hq * plan.blocks, ceil_div(p.Lk, kCtxTile), 1, 4);
+    plan.splits = splits_for((int64_t)p.B * p.Hq * plan.blocks, ceil_div(p.Lk, kCtxTile), 1, 4);
     plan.inner = (int64_t)p.G * plan.blocks * plan.splits;
     plan.dma = ctx_dma(p, p.k, p.v);
     plan.smem = ctx_tiles_bytes(ctx_padded(p.D), plan.dma) + (p.table ? 4 * ctx_entries(p) * (1 + kCtxWaves) : 0);
@@ -105,8 +104,8 @@ int ctx_params(const sjvp_ctx* t, CtxParams& p) {
         return SJVP_ERR_SHAPE;
     if (t->D < 16 || t->D > 128) return SJVP_ERR_HEAD_DIM;
     if (!(t->scale >= 0.0f) || !std::isfinite(t->scale)) return SJVP_ERR_SCALE;
-    CtxView* views[SJVP_C_COUNT] = {&p.q, &p.k, &p.v, &p.o, &p.g, &p.dq, &p.dk, &p.dv};
-    const void* ptrs[SJVP_C_COUNT] = {t->q, t->k, t->v, t->o, t->dO, t->dq, t->dk, t->dv};
+    CtxView* views[SJVP_C_COUNT] = {&p.q, &p.k, &p.v, &p.o, &p.rest, &p.g, &p.dq, &p.dk, &p.dv};
+    const void* ptrs[SJVP_C_COUNT] = {t->q, t->k, t->v, t->o, t->o_rest, t->dO, t->dq, t->dk, t->dv};
     for (int i = 0; i < SJVP_C_COUNT; ++i)
         *views[i] = {static_cast<elem_t*>(const_cast<void*>(ptrs[i])), t->strides[3 * i], t->strides[3 * i + 1], t->strides[3 * i + 2]};
     for (const CtxView* v : {&p.q, &p.k, &p.v, &p.g})
@@ -138,7 +137,7 @@ struct CtxLayout {
     size_t delta = 0, tpart = 0, stat = 0, part = 0, total = 0;
 };
 
-CtxLayout ctx_layout(CtxParams& p, bool backward) {
+CtxLayout ctx_layout(const CtxParams& p, bool backward) {
     CtxLayout l;
     const size_t HD = ctx_padded(p.D), q_rows = (size_t)p.B * p.Hq * p.Lq, k_rows = (size_t)p.B * p.Hkv * p.Lk;
     const auto take = [&](size_t floats) {
@@ -154,16 +153,12 @@ CtxLayout ctx_layout(CtxParams& p, bool backward) {
         }
         return l;
     }
-    float some;
-    p.tpart = p.dtable ? &some : nullptr;  // (whether, for the plan)
     l.row = ctx_plan_row(p);
     l.col = ctx_plan_col(p);
-    p.tpart = nullptr;
     l.delta = take(q_rows);
     if (p.dtable) l.tpart = take((size_t)p.Hq * p.B * l.row.blocks * l.row.splits * (p.both ? 2 : 1) * p.buckets);
     // (the row-owned launch's sums are used up before the column-owned one writes its own)
-    const size_t row = l.row.splits > 1 ? 2 * l.row.splits * q_rows * HD : 0, col = l.col.splits > 1 ? 2 * l.col.splits * k_rows * HD : 0;
-    l.stat = take(l.row.splits > 1 ? l.row.splits * q_rows : 0);
+    const size_t row = l.row.splits > 1 ? l.row.splits * q_rows * HD : 0, col = l.col.splits > 1 ? 2 * l.col.splits * k_rows * HD : 0;
     l.part = take(std::max(row, col));
     return l;
 }
@@ -213,7 +208,7 @@ int sjvp_ctx_bwd(const sjvp_ctx* t, int dtype, void* stream) {
     if (!ctx_fits(l.row) || !ctx_fits(l.col)) return SJVP_ERR_SHAPE;
     float* ws;
     if (ctx_workspace(t, l, ws) != SJVP_OK) return SJVP_ERR_WORKSPACE;
-    p.delta = ws + l.delta, p.stat = ws + l.stat, p.part = ws + l.part, p.tpart = p.dtable ? ws + l.tpart : nullptr;
+    p.delta = ws + l.delta, p.part = ws + l.part, p.tpart = p.dtable ? ws + l.tpart : nullptr;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     const auto run = [&](const CtxPlan& plan, bool row) {
         return dtype == SJVP_BF16 ? ctx_backward<Bf16>(p, plan, row, s) : ctx_backward<Fp16>(p, plan, row, s);

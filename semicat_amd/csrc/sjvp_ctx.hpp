@@ -54,9 +54,9 @@ struct CtxView {
 };
 
 struct CtxParams {
-    CtxView q, k, v, o, g, dq, dk, dv;       // g: the cotangent of o
+    CtxView q, k, v, o, rest, g, dq, dk, dv;  // rest: o minus its rounding (or null); g: the cotangent of o
     float *lse, *delta;                      // [B,Hq,Lq]
-    float *part, *stat;                      // sums of split work: rows of HD floats; their (maximum, sum) pairs or residues
+    float *part, *stat;                      // sums of split work: rows of HD floats; their (maximum, sum) pairs
     float* tpart;                            // bucket sums of each workgroup
     void* dtable;
     const void* table;
@@ -68,6 +68,7 @@ struct CtxParams {
     int buckets, both, causal, far;          // buckets of a direction; far: the first distance of the last one
     int splits, blocks;                      // splits of the looped axis; workgroups of a split over the owned axis
     int packed;                              // ctx_fwd_few: heads to a block of rows
+    int cols;                                // ctx_sum: dK and dV, not dQ
     int skew;                                // ctx_bwd_row: byte offset of its scratch for the bucket sums in LDS
     alignas(4) uint16_t first[kCtxBuckets];  // first distance of each bucket
 };
@@ -312,11 +313,17 @@ __device__ __forceinline__ CtxWork ctx_work(int units, int inner) {
     return {unit, slot % inner, unit < units};
 }
 
+// What the rounding of two numbers to w left of them, rounded in turn.
+template <typename T>
+__device__ __forceinline__ uint32_t rest_of(uint32_t w, float lo, float hi) {
+    return T::pack2(lo - T::to_float((elem_t)w), hi - T::to_float((elem_t)(w >> 16)));
+}
+
 // Sums of a wave's own 32 rows, OUT^T (row of C: column of the result), as rows in memory: through the wave's own LDS region of
-// [32][HD + 8], so that rows go out in pieces of 16 bytes.
+// [32][HD + 8], so that rows go out in pieces of 16 bytes.  `rest`: what the rounding leaves of them.
 template <typename T, int HD>
 __device__ __forceinline__ void store_rows(const f32x16* acc, float factor, elem_t* out, int64_t sl, int rows, elem_t* region,
-                                           int lane, int D) {
+                                           int lane, int D, bool rest = false) {
     const int h = lane >> 5;
     elem_t* mine = region + (lane & 31) * (HD + 8) + 4 * h;
 #pragma unroll
@@ -328,7 +335,10 @@ __device__ __forceinline__ void store_rows(const f32x16* acc, float factor, elem
 #pragma unroll
             for (int j = 0; j < 4; ++j) x[j] = factor == 0.0f ? 0.0f : acc[dt][4 * i + j] * factor;  // (sums of rows without a result may be NaN)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) w[j] = T::pack2(x[2 * j], x[2 * j + 1]);
+            for (int j = 0; j < 2; ++j) {
+                w[j] = T::pack2(x[2 * j], x[2 * j + 1]);
+                if (rest) w[j] = rest_of<T>(w[j], x[2 * j], x[2 * j + 1]);
+            }
             *reinterpret_cast<u32x2*>(mine + 32 * dt + 8 * i) = u32x2{w[0], w[1]};
         }
     wave_exchange();
@@ -379,18 +389,20 @@ __device__ __forceinline__ void add_columns(f32x16* acc, const Tile<HD, DMA>& at
     }
 }
 
-// The same of two score tiles, which share the reads.
+// The same with what the rounding of the scores leaves: 16 bits of them or more in all.
 template <typename T, int HD, bool DMA>
-__device__ __forceinline__ void add_columns(f32x16* acc0, f32x16* acc1, const Tile<HD, DMA>& at, const elem_t* tile, int row0,
-                                            const f32x16& s0, const f32x16& s1) {
+__device__ __forceinline__ void add_columns_exact(f32x16* acc, const Tile<HD, DMA>& at, const elem_t* tile, int row0, const f32x16& s) {
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
-        const u32x4 b0 = pack_scores<T>(s0, m), b1 = pack_scores<T>(s1, m);
+        const u32x4 b = pack_scores<T>(s, m);
+        u32x4 rest;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) rest[i] = rest_of<T>(b[i], s[8 * m + 2 * i], s[8 * m + 2 * i + 1]);
 #pragma unroll
         for (int dt = 0; dt < HD / 32; ++dt) {
             const u32x4 a = at.columns(tile, row0 + 16 * m, dt);
-            acc0[dt] = Mma32<T>::run(a, b0, acc0[dt]);
-            acc1[dt] = Mma32<T>::run(a, b1, acc1[dt]);
+            acc[dt] = Mma32<T>::run(a, b, acc[dt]);
+            acc[dt] = Mma32<T>::run(a, rest, acc[dt]);
         }
     }
 }

@@ -3,7 +3,7 @@
 //   dP = dO V^T,  delta = rowsum(dO * O),  dS = P (dP - delta)
 //   dQ = scale dS K,  dK = scale sum_heads dS^T Q,  dV = sum_heads P^T dO,  dtable[bucket][head] = sum of dS over its differences
 //
-// A row-owned launch (dQ, delta and the bucket sums) and a column-owned one (dK, dV), both of which recompute P: 4 + 4
+// A row-owned launch (dQ, delta and the bucket sums) and a column-owned one (dK, dV), both of which recompute P: 3 + 4
 // contractions against the 5 of a single launch, whose dQ would be summed by atomics in an order that changes from run to run.
 #pragma once
 #include "sjvp_ctx.hpp"
@@ -15,20 +15,21 @@ __device__ __forceinline__ float wave_sum(float x) {
     return x + __shfl_xor(x, 16);
 }
 
-// dO . O of the lane's own row, from the operands of dO and from O in memory
+// dO . o of the lane's own row, from the operands of dO and from o, and what its rounding left, in memory
 template <typename T, int HD>
-__device__ __forceinline__ float row_delta(const CtxParams& p, const u32x4* own_g, const elem_t* o, bool ok, int h) {
+__device__ __forceinline__ float row_delta(const CtxParams& p, const u32x4* own_g, const elem_t* o, const elem_t* rest, bool ok, int h) {
     float sum = 0.0f;
 #pragma unroll
     for (int c = 0; c < HD / 16; ++c) {
         if (!ok) continue;
         const u32x4 x = load_chunk(o, 16 * c + 8 * h, p.D);
+        u32x4 y = {0u, 0u, 0u, 0u};
+        if (rest) y = load_chunk(rest, 16 * c + 8 * h, p.D);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
-                sum += T::to_float((elem_t)(own_g[c][j] >> (16 * e))) *
-                       T::to_float((elem_t)(x[j] >> (16 * e)));
+            for (int e = 0; e < 32; e += 16)
+                sum += T::to_float((elem_t)(own_g[c][j] >> e)) * (T::to_float((elem_t)(x[j] >> e)) + T::to_float((elem_t)(y[j] >> e)));
     }
     return halves_sum(sum);
 }
@@ -37,11 +38,11 @@ __device__ __forceinline__ float row_delta(const CtxParams& p, const u32x4* own_
 // difference -31.  Through LDS: each lane writes its column's values as a row of kSkew floats of which the last 36 are zeros, so that
 // entry d + 31 of a diagonal, read at (kSkew + 1) per row, finds zeros where the diagonal has left the tile.  (LDS atomics
 // on the sums themselves took 190 cycles an instruction: B=64 H=12 L=128 D=64 160 us for the launch, 48 us this way.)
-__device__ __forceinline__ void add_diagonals(float* skew, float* at, const f32x16& x, float factor, int lane) {
+__device__ __forceinline__ void add_diagonals(float* skew, float* at, const f32x16& x, int lane) {
     float* mine = skew + (1 + (lane & 31)) * kSkew + 4 * (lane >> 5);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-        *reinterpret_cast<f32x4*>(mine + 8 * i) = f32x4{x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]} * factor;
+        *reinterpret_cast<f32x4*>(mine + 8 * i) = f32x4{x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]};
     wave_exchange();
     const float* from = skew + kSkew + lane - 31;
     float sum[4] = {};
@@ -53,7 +54,7 @@ __device__ __forceinline__ void add_diagonals(float* skew, float* at, const f32x
 
 // Row-owned: four waves of 32 query rows of one head share tiles of 64 keys.
 template <typename T, int HD, bool BIAS, bool DMA>
-__global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_row(CtxParams p) {
+__global__ __launch_bounds__(kCtxThreads, HD <= 64 && !BIAS ? 3 : 2) void ctx_bwd_row(CtxParams p) {
     extern __shared__ __align__(16) unsigned char smem[];
     constexpr int kTile = Tile<HD, DMA>::kElems;
     elem_t* tiles = reinterpret_cast<elem_t*>(smem);  // [2][K, V]
@@ -106,7 +107,9 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_row(Ctx
 #pragma unroll
         for (int c = 0; c < HD / 16; ++c) own_g[c] = ok ? own_g[c] : u32x4{0u, 0u, 0u, 0u};
     }
-    const float delta = row_delta<T, HD>(p, own_g, p.o.head(b, hq) + (int64_t)qi * p.o.sl, ok, h);
+    const float delta = row_delta<T, HD>(p, own_g, p.o.head(b, hq) + (int64_t)qi * p.o.sl,
+                                         p.rest.ptr ? p.rest.head(b, hq) + (int64_t)qi * p.rest.sl : nullptr, ok, h);
+    if (split == 0 && h == 0 && qi < p.Lq) p.delta[stat] = delta;
     if (t0 < t1) deliver(t0);
     kf.arrived();
     workgroup_barrier();
@@ -127,10 +130,8 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_row(Ctx
                 if (tile_row(r, 0) >= bt.keys - k0 - 4 * h) s[r] = 0.0f;
         }
     };
-    f32x16 acc[HD / 32] = {}, mean[HD / 32] = {};  // dS K, P K
-    float ds_below = 0.0f, ds_above = 0.0f;        // sums of dS beyond the last single distance,
-    float p_below = 0.0f, p_above = 0.0f;          // and of P there
-    float residue = 0.0f;                          // sum of dS over the row
+    f32x16 acc[HD / 32] = {};
+    float below = 0.0f, above = 0.0f;  // sums of dS beyond the last single distance
     // (the sequence's last tile with its mask in code of its own, as in the forward)
     const auto tile = [&](int t, bool masked, auto band) {
         const int key = t * kCtxTile;
@@ -146,24 +147,20 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_row(Ctx
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 row_probabilities(s[u], key + 32 * u, band, masked);
-                float sum = 0.0f, p_sum = 0.0f;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    ds[u][r] = s[u][r] * (ds[u][r] - delta);
-                    sum += ds[u][r];
-                }
-                residue += sum;
+                for (int r = 0; r < 16; ++r) ds[u][r] = s[u][r] * (ds[u][r] - delta);
                 if constexpr (BIAS && decltype(band)::value == kNear) {
-                    add_diagonals(skew, hist + row_entry(p, key + 32 * u - pos0 - 31, 63), ds[u], 1.0f, lane);
+                    add_diagonals(skew, hist + row_entry(p, key + 32 * u - pos0 - 31, 63), ds[u], lane);
                 } else if constexpr (BIAS) {
+                    float sum = 0.0f;
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) p_sum += s[u][r];
-                    if constexpr (decltype(band)::value == kBelow) ds_below += sum, p_below += p_sum;
-                    else ds_above += sum, p_above += p_sum;
+                    for (int r = 0; r < 16; ++r) sum += ds[u][r];
+                    if constexpr (decltype(band)::value == kBelow) below += sum;
+                    else above += sum;
                 }
             }
 #pragma unroll
-            for (int u = 0; u < 2; ++u) add_columns<T>(acc, mean, at, K, 32 * u, ds[u], s[u]);
+            for (int u = 0; u < 2; ++u) add_columns<T>(acc, at, K, 32 * u, ds[u]);
         }
         if (t + 1 < t1) deliver(t + 1);
         kf.arrived();
@@ -171,73 +168,30 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_row(Ctx
     };
     // the tiles near the diagonal: of the workgroup, whose positions are first .. first + 127
     const int first = bt.start + qb * kCtxOwned;
-    const int near = tiles_before(first - p.far + 1, nt), above = tiles_before(first + kCtxOwned - 1 + p.far + kCtxTile - 1, nt);
+    const int t_near = tiles_before(first - p.far + 1, nt), t_above = tiles_before(first + kCtxOwned - 1 + p.far + kCtxTile - 1, nt);
     const int whole = t1 * kCtxTile > bt.keys ? t1 - 1 : t1;
     int t = t0;
     if constexpr (BIAS) {
-        for (; t < min(near, whole); ++t) tile(t, false, InBand<kBelow>{});
-        for (; t < min(above, whole); ++t) tile(t, false, InBand<kNear>{});
+        for (; t < min(t_near, whole); ++t) tile(t, false, InBand<kBelow>{});
+        for (; t < min(t_above, whole); ++t) tile(t, false, InBand<kNear>{});
         for (; t < whole; ++t) tile(t, false, InBand<kAbove>{});
     } else {
         for (; t < whole; ++t) tile(t, false, InBand<kBelow>{});
     }
     // (differences beyond the last single distance may be summed among the others, at the row's ends)
     if (t < t1) tile(t, true, InBand<BIAS ? kNear : kBelow>{});
-    // The rows of dS sum to zero but for the error of delta, which the rounding of P and O in the forward leaves in it (2^-9 of it
-    // for bf16; of a sharp row's dS more than that).  So the residue is that error, and P times the residue what it put into dS:
-    // taken out of dQ here, of the bucket sums below, and the column-owned launch gets the right delta.  (ctx_sum_rows does it for
-    // splits, which know a part of the residue each.)
-    residue = halves_sum(residue);
     const int out_rows = min(max(p.Lq - q0, 0), 32);
     if (p.splits > 1) {
-        const int64_t all = (int64_t)p.B * p.Hq * p.Lq, place = ((int64_t)b * p.Hq + hq) * p.Lq + q0;
-        store_part<HD>(acc, scored, p.part + (2 * split * all + place) * HD, out_rows, lane);
-        store_part<HD>(mean, scored, p.part + ((2 * split + 1) * all + place) * HD, out_rows, lane);
-        if (h == 0 && qi < p.Lq) {
-            p.stat[split * all + stat] = residue;
-            if (split == 0) p.delta[stat] = delta;
-        }
+        const int64_t all = (int64_t)p.B * p.Hq * p.Lq;
+        store_part<HD>(acc, scored, p.part + (split * all + ((int64_t)b * p.Hq + hq) * p.Lq + q0) * HD, out_rows, lane);
     } else {
-#pragma unroll
-        for (int dt = 0; dt < HD / 32; ++dt) acc[dt] -= residue * mean[dt];
-        if (h == 0 && qi < p.Lq) p.delta[stat] = delta + residue;
         store_rows<T, HD>(acc, scored ? p.scale : 0.0f, p.dq.head(b, hq) + (int64_t)q0 * p.dq.sl, p.dq.sl, out_rows,
                           tiles + wave * 32 * (HD + 8), lane, p.D);
     }
-    if constexpr (!BIAS) return;
-    if (!p.tpart) return;
-    // the tiles whose differences were summed one by one, the last among them
-    const int t_near = min(near, whole), n_near = max(0, min(above, whole) - t_near), again = n_near + (t1 - whole);
-    const auto key_of = [&](int i) { return (i < n_near ? t_near + i : whole) * kCtxTile; };
-    const auto again_place = [&](int i) { return tiles + (i & 1) * kTile; };
-    const auto again_request = [&](int i) {
-        kf.request(kt + (int64_t)key_of(i) * p.k.sl, p.k.sl, n - key_of(i), p.D, again_place(i), wave);
-    };
-    workgroup_barrier();
-    if (again) {
-        again_request(0);
-        kf.deliver(again_place(0), p.D, tid);
-    }
-    kf.arrived();
-    workgroup_barrier();
-    for (int i = 0; i < again; ++i) {
-        const int key = key_of(i);
-        if (i + 1 < again) again_request(i + 1);
-        if (key < n_wave) {
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                f32x16 s = scores<T>(at, again_place(i), 32 * u, own_q);
-                row_probabilities(s, key + 32 * u, InBand<kNear>{}, key + kCtxTile > bt.keys);
-                add_diagonals(skew, hist + row_entry(p, key + 32 * u - pos0 - 31, 63), s, -residue, lane);
-            }
-        }
-        if (i + 1 < again) kf.deliver(again_place(i + 1), p.D, tid);
-        kf.arrived();
-        workgroup_barrier();
-    }
-    {
-        const float below = wave_sum(ds_below - residue * p_below), above_sum = wave_sum(ds_above - residue * p_above);
-        if (lane == 0) hist[0] += below, hist[entries - 1] += above_sum;
+    if constexpr (BIAS) {
+        if (!p.tpart) return;
+        below = wave_sum(below), above = wave_sum(above);
+        if (lane == 0) hist[0] += below, hist[entries - 1] += above;
         workgroup_barrier();
         const float* hists = row + entries;
         const int nb = p.both ? 2 * p.buckets : p.buckets, zero = p.far + kCtxPad;
@@ -382,50 +336,25 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_col(Ctx
     }
 }
 
-// Adds up the splits of the row-owned launch: one thread to eight columns of a row of dQ.
+// Adds up the splits of a launch above: one thread to eight columns of a row of dQ, or of dK and dV.
 template <typename T, int HD>
-__global__ __launch_bounds__(kCtxThreads) void ctx_sum_rows(CtxParams p) {
+__global__ __launch_bounds__(kCtxThreads) void ctx_sum(CtxParams p) {
     constexpr int CH = HD / 8;
-    const int64_t rows = (int64_t)p.B * p.Hq * p.Lq, x = (int64_t)blockIdx.x * kCtxThreads + threadIdx.x, place = x / CH;
-    if (place >= rows) return;
-    const int c8 = 8 * (int)(x % CH);
-    f32x4 a[4] = {};  // dS K, P K
-    float residue = 0.0f;
-    for (int s = 0; s < p.splits; ++s) {
-        residue += p.stat[s * rows + place];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            a[i] += *reinterpret_cast<const f32x4*>(p.part + ((2 * s + i / 2) * rows + place) * HD + c8 + 4 * (i % 2));
-    }
-    if (c8 == 0) p.delta[place] += residue;
-    u32x4 y;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const f32x4 d = (a[i] - residue * a[2 + i]) * p.scale;
-        y[2 * i] = T::pack2(d[0], d[1]), y[2 * i + 1] = T::pack2(d[2], d[3]);
-    }
-    const int64_t head = place / p.Lq;
-    store_chunk(p.dq.head((int)(head / p.Hq), (int)(head % p.Hq)) + (place % p.Lq) * p.dq.sl, y, c8, p.D);
-}
-
-// The same for the column-owned one: dK and dV.
-template <typename T, int HD>
-__global__ __launch_bounds__(kCtxThreads) void ctx_sum_cols(CtxParams p) {
-    constexpr int CH = HD / 8;
-    const int64_t rows = (int64_t)p.B * p.Hkv * p.Lk, x = (int64_t)blockIdx.x * kCtxThreads + threadIdx.x, place = x / CH;
-    if (place >= 2 * rows) return;
+    const int H = p.cols ? p.Hkv : p.Hq, L = p.cols ? p.Lk : p.Lq, tensors = p.cols ? 2 : 1;
+    const int64_t rows = (int64_t)p.B * H * L, x = (int64_t)blockIdx.x * kCtxThreads + threadIdx.x, place = x / CH;
+    if (place >= tensors * rows) return;
     const int c8 = 8 * (int)(x % CH), second = place >= rows;
     f32x4 a = {}, c = {};
     for (int s = 0; s < p.splits; ++s) {
-        const float* from = p.part + (s * 2 * rows + place) * HD + c8;
+        const float* from = p.part + (s * tensors * rows + place) * HD + c8;
         a += *reinterpret_cast<const f32x4*>(from);
         c += *reinterpret_cast<const f32x4*>(from + 4);
     }
-    const int64_t at = place - second * rows, head = at / p.Lk;
-    const CtxView& out = second ? p.dv : p.dk;
+    const int64_t at = place - second * rows, head = at / L;
+    const CtxView& out = !p.cols ? p.dq : second ? p.dv : p.dk;
     const float f = second ? 1.0f : p.scale;
     const u32x4 y = {T::pack2(a[0] * f, a[1] * f), T::pack2(a[2] * f, a[3] * f), T::pack2(c[0] * f, c[1] * f), T::pack2(c[2] * f, c[3] * f)};
-    store_chunk(out.head((int)(head / p.Hkv), (int)(head % p.Hkv)) + (at % p.Lk) * out.sl, y, c8, p.D);
+    store_chunk(out.head((int)(head / H), (int)(head % H)) + (at % L) * out.sl, y, c8, p.D);
 }
 
 }  // namespace sjvp

@@ -66,9 +66,12 @@ struct RowSums {
 
 __device__ __forceinline__ float ctx_lse(float ref, float l) { return (ref + fast_log2(l)) * kLn2; }
 
+// REST, for a backward to follow: the gradients need delta = dO . o as it would be with unrounded probabilities (their sums over a row
+// are differences of near numbers), so P goes into the contraction with what its rounding leaves, and so does o into memory.
+//
 // Many rows: four waves of 32 rows of one head share tiles of 64 keys.  Two tiles of K and V in LDS: the next one is on its way
 // while this one is used, one barrier to a tile.
-template <typename T, int HD, bool BIAS, bool DMA>
+template <typename T, int HD, bool BIAS, bool DMA, bool REST>
 __global__ __launch_bounds__(kCtxThreads, 2) void ctx_fwd(CtxParams p) {
     extern __shared__ __align__(16) unsigned char smem[];
     constexpr int kTile = Tile<HD, DMA>::kElems;
@@ -135,7 +138,10 @@ __global__ __launch_bounds__(kCtxThreads, 2) void ctx_fwd(CtxParams p) {
             }
             st.template exponentials<kEven>(p, s, one);
 #pragma unroll
-            for (int u = 0; u < 2; ++u) add_columns<T>(st.acc, at, v_place(t), 32 * u, s[u]);
+            for (int u = 0; u < 2; ++u) {
+                if constexpr (REST) add_columns_exact<T>(st.acc, at, v_place(t), 32 * u, s[u]);
+                else add_columns<T>(st.acc, at, v_place(t), 32 * u, s[u]);
+            }
             if constexpr (more) s[0] = next[0], s[1] = next[1];
         }
         if (more) {
@@ -164,6 +170,8 @@ __global__ __launch_bounds__(kCtxThreads, 2) void ctx_fwd(CtxParams p) {
         p.lse[((int64_t)b * p.Hq + hq) * p.Lq + q0 + lane] = l == 0.0f ? -INFINITY : ctx_lse(st.ref, l);
     elem_t* region = tiles + wave * 32 * (HD + 8);
     store_rows<T, HD>(st.acc, f, p.o.head(b, hq) + (int64_t)q0 * p.o.sl, p.o.sl, out_rows, region, lane, p.D);
+    if constexpr (REST)
+        store_rows<T, HD>(st.acc, f, p.rest.head(b, hq) + (int64_t)q0 * p.rest.sl, p.rest.sl, out_rows, region, lane, p.D, true);
 }
 
 // Few rows: the query rows of all heads that share a key head stand in one block of 32 (row = head of the group * Lq + query), and
@@ -172,7 +180,7 @@ __global__ __launch_bounds__(kCtxThreads, 2) void ctx_fwd(CtxParams p) {
 // joined in LDS; with several splits of the key axis they go to memory for ctx_join.
 // `packed` heads of a group stand in one block's rows: all of them, or one where their bias rows would not fit or a head
 // fills a block by itself.
-template <typename T, int HD, bool BIAS, int WAVES>
+template <typename T, int HD, bool BIAS, bool REST, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, HD <= 64 ? 3 : 2) void ctx_fwd_few(CtxParams p) {
     extern __shared__ __align__(16) unsigned char smem[];
     constexpr int kRegion = 32 * (HD + 8), kSum = HD + 4;
@@ -249,7 +257,8 @@ __global__ __launch_bounds__(64 * WAVES, HD <= 64 ? 3 : 2) void ctx_fwd_few(CtxP
         st.template raise<!BIAS>(p, s, 0.0f, bt.keys - key, h, key + 32 > bt.keys);
         st.template exponentials<!BIAS>(p, s, 0.0f);
         wave_exchange();
-        add_columns<T>(st.acc, tile, V, 0, s[0]);
+        if constexpr (REST) add_columns_exact<T>(st.acc, tile, V, 0, s[0]);
+        else add_columns<T>(st.acc, tile, V, 0, s[0]);
         wave_exchange();
     }
     const float l = halves_sum(st.l);
@@ -297,13 +306,15 @@ __global__ __launch_bounds__(64 * WAVES, HD <= 64 ? 3 : 2) void ctx_fwd_few(CtxP
         }
         const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
         if (p.lse && c8 == 0) p.lse[place] = sum == 0.0f ? -INFINITY : ctx_lse(ref, sum);
-        u32x4 o;
+        u32x4 o, rest;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const float a = f == 0.0f ? 0.0f : y[2 * j] * f, c = f == 0.0f ? 0.0f : y[2 * j + 1] * f;
             o[j] = T::pack2(a, c);
+            rest[j] = rest_of<T>(o[j], a, c);
         }
         store_chunk(p.o.head(b, hq) + (int64_t)ii * p.o.sl, o, c8, p.D);
+        if constexpr (REST) store_chunk(p.rest.head(b, hq) + (int64_t)ii * p.rest.sl, rest, c8, p.D);
     }
 }
 
@@ -345,15 +356,17 @@ __global__ __launch_bounds__(kCtxThreads) void ctx_join(CtxParams p) {
     }
     const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
     if (p.lse && c8 == 0) p.lse[place] = sum == 0.0f ? -INFINITY : ctx_lse(top, sum);
-    u32x4 o;
+    u32x4 o, rest;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const float a = f == 0.0f ? 0.0f : y[2 * j] * f, c = f == 0.0f ? 0.0f : y[2 * j + 1] * f;
         o[j] = T::pack2(a, c);
+        rest[j] = rest_of<T>(o[j], a, c);
     }
     const int64_t head = place / p.Lq;
     const int i = (int)(place % p.Lq), hq = (int)(head % p.Hq), b = (int)(head / p.Hq);
     store_chunk(p.o.head(b, hq) + (int64_t)i * p.o.sl, o, c8, p.D);
+    if (p.rest.ptr) store_chunk(p.rest.head(b, hq) + (int64_t)i * p.rest.sl, rest, c8, p.D);
 }
 
 }  // namespace sjvp

@@ -610,8 +610,9 @@ int context_run(sjvp_ctx& t, const Tensor& q, bool backward) {
 
 void context_check(int status) { TORCH_CHECK(status == SJVP_OK, "sjvp status ", status, " from the context attention kernels"); }
 
+// lse, rest: for a backward to follow, or null
 Tensor context_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& table, const ContextOptions& options, Tensor* lse,
-                       int& status) {
+                       Tensor* rest, int& status) {
     const c10::DeviceGuard guard(q.device());
     const Maker make_tensor{q.device()};
     Tensor o = make_tensor({q.size(0), q.size(1), q.size(2), q.size(3)}, q.scalar_type());
@@ -619,6 +620,9 @@ Tensor context_forward(const Tensor& q, const Tensor& k, const Tensor& v, const 
     if (lse) {
         *lse = make_tensor({q.size(0), q.size(2), q.size(1)}, at::kFloat);
         t.lse = static_cast<float*>(lse->data_ptr());
+        *rest = make_tensor(o.sizes(), o.scalar_type());
+        t.o_rest = rest->data_ptr();
+        context_strides(t, SJVP_C_O_REST, *rest);
     }
     t.o = o.data_ptr();
     context_strides(t, SJVP_C_Q, q);
@@ -643,11 +647,11 @@ struct NoSecondDerivative : torch::autograd::Function<NoSecondDerivative> {
 struct ContextNode : torch::autograd::Function<ContextNode> {
     static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v,
                           const std::optional<Tensor>& table, const ContextOptions* options) {
-        Tensor lse;
+        Tensor lse, rest;
         int status;
-        Tensor o = context_forward(q, k, v, table.value_or(Tensor()), *options, &lse, status);
+        Tensor o = context_forward(q, k, v, table.value_or(Tensor()), *options, &lse, &rest, status);
         context_check(status);
-        ctx->save_for_backward({q, k, v, table.value_or(Tensor()), options->klen, options->qlen, options->start, o, lse});
+        ctx->save_for_backward({q, k, v, table.value_or(Tensor()), options->klen, options->qlen, options->start, o, lse, rest});
         ctx->saved_data["options"] = c10::IValue(std::vector<int64_t>{options->start0, options->both, options->causal});
         ctx->saved_data["scale"] = static_cast<double>(options->scale);
         ctx->saved_data["first"] = options->first;
@@ -658,7 +662,7 @@ struct ContextNode : torch::autograd::Function<ContextNode> {
         torch::autograd::variable_list grads(5);
         if (!cotangents[0].defined()) return grads;
         const auto saved = ctx->get_saved_variables();
-        const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &table = saved[3], &o = saved[7], &lse = saved[8];
+        const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &table = saved[3], &o = saved[7], &lse = saved[8], &rest = saved[9];
         const std::vector<int64_t> ints = ctx->saved_data["options"].toIntVector();
         const ContextOptions options{static_cast<int>(ints[0]), static_cast<int>(ints[1]), static_cast<int>(ints[2]),
                                      static_cast<float>(ctx->saved_data["scale"].toDouble()), ctx->saved_data["first"].toStringRef(),
@@ -671,10 +675,10 @@ struct ContextNode : torch::autograd::Function<ContextNode> {
             const Maker make_tensor{q.device()};
             sjvp_ctx t = context_struct(q, k, v, table, options);
             t.lse = static_cast<float*>(lse.data_ptr());
-            t.o = o.data_ptr(), t.dO = g.data_ptr();
+            t.o = o.data_ptr(), t.o_rest = rest.data_ptr(), t.dO = g.data_ptr();
             grads[0] = make_tensor(q.sizes(), q.scalar_type());
             t.dq = grads[0].data_ptr();
-            const Tensor* at[] = {&q, &k, &v, &o, &g, &grads[0], &grads[1], &grads[2]};
+            const Tensor* at[] = {&q, &k, &v, &o, &rest, &g, &grads[0], &grads[1], &grads[2]};
             if (ctx->needs_input_grad(1) || ctx->needs_input_grad(2)) {
                 grads[1] = make_tensor(k.sizes(), k.scalar_type());
                 grads[2] = make_tensor(v.sizes(), v.scalar_type());
@@ -759,7 +763,7 @@ PyObject* context(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const bool record = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() ||
                                                            (table.defined() && table.requires_grad()));
         if (record) o = ContextNode::apply(q, k, v, table.defined() ? std::optional<Tensor>(table) : std::nullopt, &options);
-        else o = context_forward(q, k, v, table, options, nullptr, status);
+        else o = context_forward(q, k, v, table, options, nullptr, nullptr, status);
     }
     if (status != SJVP_OK) return PyLong_FromLong(status);
     return THPVariable_Wrap(std::move(o));

@@ -8,7 +8,7 @@ namespace sjvp {
 
 template <>
 int ctx_backward<SJVP_T>(CtxParams p, const CtxPlan& plan, bool row, hipStream_t stream) {
-    p.blocks = plan.blocks, p.splits = plan.splits, p.skew = plan.skew;
+    p.blocks = plan.blocks, p.splits = plan.splits, p.skew = plan.skew, p.cols = !row;
     const int grid = (int)ctx_grid((int)plan.units, (int)plan.inner);
     return ctx_by_head(p.D, plan.dma, [&](auto hd, auto dma) {
         constexpr int HD = decltype(hd)::value;
@@ -20,8 +20,7 @@ int ctx_backward<SJVP_T>(CtxParams p, const CtxPlan& plan, bool row, hipStream_t
                           : launch(ctx_bwd_col<SJVP_T, HD, false, DMA>, grid, plan.smem, stream, p, kCtxThreads);
         if (rc != SJVP_OK || p.splits == 1) return rc;
         const int64_t rows = row ? (int64_t)p.B * p.Hq * p.Lq : 2 * (int64_t)p.B * p.Hkv * p.Lk;
-        return launch(row ? ctx_sum_rows<SJVP_T, HD> : ctx_sum_cols<SJVP_T, HD>, (int)((rows * (HD / 8) + kCtxThreads - 1) / kCtxThreads), 0,
-                      stream, p, kCtxThreads);
+        return launch(ctx_sum<SJVP_T, HD>, (int)((rows * (HD / 8) + kCtxThreads - 1) / kCtxThreads), 0, stream, p, kCtxThreads);
     });
 }
 

@@ -10,18 +10,19 @@ template <>
 int ctx_forward<SJVP_T>(CtxParams p, const CtxPlan& plan, hipStream_t stream) {
     p.blocks = plan.blocks, p.splits = plan.splits;
     const int grid = (int)ctx_grid((int)plan.units, (int)plan.inner);
+    p.packed = plan.packed;
     return ctx_by_head(p.D, plan.dma, [&](auto hd, auto dma) {
         constexpr int HD = decltype(hd)::value;
-        constexpr bool DMA = decltype(dma)::value;
-        if (!plan.few) return p.table ? launch(ctx_fwd<SJVP_T, HD, true, DMA>, grid, plan.smem, stream, p, kCtxThreads)
-                                      : launch(ctx_fwd<SJVP_T, HD, false, DMA>, grid, plan.smem, stream, p, kCtxThreads);
-        p.packed = plan.packed;
-        const auto few = [&](auto waves) {
-            constexpr int W = decltype(waves)::value;
-            return p.table ? launch(ctx_fwd_few<SJVP_T, HD, true, W>, grid, plan.smem, stream, p, 64 * W)
-                           : launch(ctx_fwd_few<SJVP_T, HD, false, W>, grid, plan.smem, stream, p, 64 * W);
+        const auto run = [&](auto bias, auto rest) {
+            constexpr bool BIAS = decltype(bias)::value, REST = decltype(rest)::value;
+            if (!plan.few) return launch(ctx_fwd<SJVP_T, HD, BIAS, decltype(dma)::value, REST>, grid, plan.smem, stream, p, kCtxThreads);
+            return plan.waves == 8 ? launch(ctx_fwd_few<SJVP_T, HD, BIAS, REST, 8>, grid, plan.smem, stream, p, 512)
+                                   : launch(ctx_fwd_few<SJVP_T, HD, BIAS, REST, 4>, grid, plan.smem, stream, p, 256);
         };
-        const int rc = plan.waves == 8 ? few(std::integral_constant<int, 8>{}) : few(std::integral_constant<int, 4>{});
+        const std::true_type yes;
+        const std::false_type no;
+        const int rc = p.table ? p.rest.ptr ? run(yes, yes) : run(yes, no) : p.rest.ptr ? run(no, yes) : run(no, no);
+        if (!plan.few) return rc;
         if (rc != SJVP_OK || p.splits == 1) return rc;
         int slices = 1;  // as in the kernel
         while (slices < p.splits && slices < 16) slices *= 2;
