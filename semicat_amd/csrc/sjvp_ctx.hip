@@ -77,10 +77,6 @@ CtxPlan ctx_plan_row(const CtxParams& p) {
     plan.inner = (int64_t)p.G * plan.blocks * plan.splits;
     plan.dma = ctx_dma(p, p.k, p.v);
     plan.smem = ctx_tiles_bytes(ctx_padded(p.D), plan.dma) + (p.table ? 4 * ctx_entries(p) * (1 + kCtxWaves) : 0);
-    if (p.table) {
-        plan.skew = (plan.smem + 15) / 16 * 16;
-        plan.smem = plan.skew + 4 * kCtxWaves * kSkewFloats;
-    }
     return plan;
 }
 

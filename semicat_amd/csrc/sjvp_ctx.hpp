@@ -30,9 +30,6 @@ constexpr int kCtxOwned = 32 * kCtxWaves;  // owned positions of a workgroup who
 constexpr int kCtxTile = 64;               // looped positions per tile
 constexpr int kCtxPad = 64;                // entries of the bias row beyond the last single distance, on each side
 constexpr int kCtxBuckets = SJVP_CTX_MAX_BUCKETS;
-// the scratch of a wave in the bucket sums (ctx_bwd_row), in floats
-constexpr int kSkew = 68;                     // of a row: 16-byte accesses of consecutive rows on different banks
-constexpr int kSkewFloats = 33 * kSkew + 32;  // with a row of zeros in front, and what the last lanes read behind
 constexpr int kCtxMost = 1 << 29;          // positions and lengths: sums of three stay within 32 bits
 
 template <typename T> struct Mma32;
@@ -69,7 +66,6 @@ struct CtxParams {
     int splits, blocks;                      // splits of the looped axis; workgroups of a split over the owned axis
     int packed;                              // ctx_fwd_few: heads to a block of rows
     int cols;                                // ctx_sum: dK and dV, not dQ
-    int skew;                                // ctx_bwd_row: byte offset of its scratch for the bucket sums in LDS
     alignas(4) uint16_t first[kCtxBuckets];  // first distance of each bucket
 };
 

@@ -34,22 +34,26 @@ __device__ __forceinline__ float row_delta(const CtxParams& p, const u32x4* own_
     return halves_sum(sum);
 }
 
-// Sums along the diagonals of a 32 x 32 score tile (one wave's), added to the wave's sums by difference; `at`: entry of the
-// difference -31.  Through LDS: each lane writes its column's values as a row of kSkew floats of which the last 36 are zeros, so that
-// entry d + 31 of a diagonal, read at (kSkew + 1) per row, finds zeros where the diagonal has left the tile.  (LDS atomics
-// on the sums themselves took 190 cycles an instruction: B=64 H=12 L=128 D=64 160 us for the launch, 48 us this way.)
-__device__ __forceinline__ void add_diagonals(float* skew, float* at, const f32x16& x, int lane) {
-    float* mine = skew + (1 + (lane & 31)) * kSkew + 4 * (lane >> 5);
+// Sums along the diagonals of a 32 x 32 score tile (one wave's): lane j < 63 receives that of the difference (looped row - column)
+// 31 - j.  The partial sum of a diagonal stands with the lane whose column it has reached and moves one lane up from a looped row to
+// the next; the upper half of the wave, which holds columns of its own only until they are moved below it, takes what leaves the 32
+// columns.  Registers and lane shifts alone.  (LDS atomics by difference took 190 cycles an instruction: B=64 H=12 L=128 D=64 160 us
+// for the launch; through rows of LDS 35 us and 36 KB of it; this way 32 us.)
+__device__ __forceinline__ float diagonals(const f32x16& x) {
+    float lower[16], upper[16];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        *reinterpret_cast<f32x4*>(mine + 8 * i) = f32x4{x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]};
-    wave_exchange();
-    const float* from = skew + kSkew + lane - 31;
-    float sum[4] = {};
+    for (int r = 0; r < 16; ++r) {
+        const auto halves = __builtin_amdgcn_permlane32_swap(__float_as_uint(x[r]), 0u, false, false);
+        lower[r] = __uint_as_float(halves[0]);
+        upper[r] = __uint_as_float(halves[1]);
+    }
+    float sum = 0.0f;
 #pragma unroll
-    for (int q = 0; q < 32; ++q) sum[q & 3] += from[q * (kSkew + 1)];
-    if (lane < 63) at[lane] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-    wave_exchange();
+    for (int y = 0; y < 32; ++y) {
+        const int r = 4 * (y >> 3) + (y & 3);
+        sum = __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(sum), 0x138, 0xf, 0xf, true)) + (y & 4 ? upper : lower)[r];
+    }
+    return sum;
 }
 
 // Row-owned: four waves of 32 query rows of one head share tiles of 64 keys.
@@ -74,7 +78,6 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 && !BIAS ? 3 : 2) void ctx_bw
     const int nt = (n + kCtxTile - 1) / kCtxTile;
     const int t0 = (int)((int64_t)nt * split / p.splits), t1 = (int)((int64_t)nt * (split + 1) / p.splits);
     float* hist = row + entries + wave * entries;  // the wave's sums of dS by difference
-    float* skew = reinterpret_cast<float*>(smem + p.skew) + wave * kSkewFloats;
 
     const elem_t *kt = p.k.head(b, hk), *vt = p.v.head(b, hk);
     TileFeed<HD, DMA> kf(p.k.sl, p.D, tid), vf(p.v.sl, p.D, tid);
@@ -98,7 +101,6 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 && !BIAS ? 3 : 2) void ctx_bw
     if constexpr (BIAS) {
         fill_bias_row(p, row, hq, tid, kCtxThreads);
         for (int x = lane; x < entries; x += 64) hist[x] = 0.0f;
-        for (int x = lane; x < kSkewFloats; x += 64) skew[x] = 0.0f;
     }
     const bool ok = lse != -INFINITY;      // a row that sees no key has no gradient, whatever its cotangent,
     const bool scored = ok && limit != 1;  // one that sees one key none of its score: exactly none, not what rounding leaves
@@ -150,7 +152,9 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 && !BIAS ? 3 : 2) void ctx_bw
 #pragma unroll
                 for (int r = 0; r < 16; ++r) ds[u][r] = s[u][r] * (ds[u][r] - delta);
                 if constexpr (BIAS && decltype(band)::value == kNear) {
-                    add_diagonals(skew, hist + row_entry(p, key + 32 * u - pos0 - 31, 63), ds[u], lane);
+                    const float sum = diagonals(ds[u]);
+                    if (lane < 63) hist[row_entry(p, key + 32 * u - pos0 - 31, 63) + 62 - lane] += sum;
+                    wave_exchange();  // (other lanes add to these next)
                 } else if constexpr (BIAS) {
                     float sum = 0.0f;
 #pragma unroll

@@ -26,7 +26,7 @@ struct CtxPlan {
     int waves = kCtxWaves;  // and waves to a workgroup
     int blocks = 1, splits = 1;
     int64_t units = 1, inner = 1;  // of ctx_work
-    int smem = 0, skew = 0;
+    int smem = 0;
     bool dma = false;              // tiles by LDS-DMA
 };
 

@@ -8,7 +8,7 @@ namespace sjvp {
 
 template <>
 int ctx_backward<SJVP_T>(CtxParams p, const CtxPlan& plan, bool row, hipStream_t stream) {
-    p.blocks = plan.blocks, p.splits = plan.splits, p.skew = plan.skew, p.cols = !row;
+    p.blocks = plan.blocks, p.splits = plan.splits, p.cols = !row;
     const int grid = (int)ctx_grid((int)plan.units, (int)plan.inner);
     return ctx_by_head(p.D, plan.dma, [&](auto hd, auto dma) {
         constexpr int HD = decltype(hd)::value;
