@@ -91,6 +91,18 @@ CtxPlan ctx_plan_col(const CtxParams& p) {
     return plan;
 }
 
+bool ctx_plan_one(const CtxParams& p, CtxPlan& plan) {
+    if (ctx_padded(p.D) != 64 || p.Lk > 256 || !p.dk.ptr) return false;
+    plan.waves = p.Lk > 128 ? 8 : 4;
+    plan.units = (int64_t)p.B * p.Hkv;
+    plan.dma = ctx_dma(p, p.q, p.g) && ctx_aligned(p.k);
+    const int tile = kCtxTile * (64 + (plan.dma ? 0 : 8)) * 2;
+    plan.smem = (plan.waves / 2 + 4) * tile + plan.waves / 2 * kCtxTile * 72 * 2 + 4 * kCtxTile * 4 +
+                (p.table ? 4 * (ctx_entries(p) * (1 + plan.waves) + 28) : 0);
+    // a workgroup walks all rows of its heads: with few workgroups the pair of launches spreads them over more
+    return plan.smem <= kLds && (2 * plan.units >= compute_units() || p.G * ceil_div(p.Lq, kCtxTile) <= 4);
+}
+
 namespace {
 
 int ctx_params(const sjvp_ctx* t, CtxParams& p) {
@@ -129,7 +141,8 @@ int ctx_params(const sjvp_ctx* t, CtxParams& p) {
 
 // The plans of a call, and where its scratch lies in the workspace (in floats).
 struct CtxLayout {
-    CtxPlan fwd, row, col;
+    CtxPlan fwd, row, col, one;
+    bool single = false;  // backward by ctx_bwd_one
     size_t delta = 0, tpart = 0, stat = 0, part = 0, total = 0;
 };
 
@@ -147,6 +160,11 @@ CtxLayout ctx_layout(const CtxParams& p, bool backward) {
             l.stat = take(2 * l.fwd.splits * q_rows);
             l.part = take(l.fwd.splits * q_rows * HD);
         }
+        return l;
+    }
+    l.single = ctx_plan_one(p, l.one);
+    if (l.single) {
+        if (p.dtable) l.tpart = take((size_t)p.Hq * p.B * (p.both ? 2 : 1) * p.buckets);
         return l;
     }
     l.row = ctx_plan_row(p);
@@ -200,7 +218,7 @@ int sjvp_ctx_bwd(const sjvp_ctx* t, int dtype, void* stream) {
     if (rc != SJVP_OK) return rc;
     if (dtype != SJVP_BF16 && dtype != SJVP_FP16) return SJVP_ERR_DTYPE;
     if (!t->q || !t->k || !t->v || !t->o || !t->dO || !t->dq || !t->dk != !t->dv || !t->lse) return SJVP_ERR_NULL;
-    const CtxLayout l = ctx_layout(p, true);
+    CtxLayout l = ctx_layout(p, true);
     if (!ctx_fits(l.row) || !ctx_fits(l.col)) return SJVP_ERR_SHAPE;
     float* ws;
     if (ctx_workspace(t, l, ws) != SJVP_OK) return SJVP_ERR_WORKSPACE;
@@ -209,8 +227,13 @@ int sjvp_ctx_bwd(const sjvp_ctx* t, int dtype, void* stream) {
     const auto run = [&](const CtxPlan& plan, bool row) {
         return dtype == SJVP_BF16 ? ctx_backward<Bf16>(p, plan, row, s) : ctx_backward<Fp16>(p, plan, row, s);
     };
-    rc = run(l.row, true);
-    if (rc == SJVP_OK && t->dk) rc = run(l.col, false);
+    if (l.single) {
+        rc = dtype == SJVP_BF16 ? ctx_backward_one<Bf16>(p, l.one, s) : ctx_backward_one<Fp16>(p, l.one, s);
+        l.row.blocks = l.row.splits = 1;
+    } else {
+        rc = run(l.row, true);
+        if (rc == SJVP_OK && t->dk) rc = run(l.col, false);
+    }
     if (rc != SJVP_OK || !p.dtable) return rc;
     const int per = ((p.both ? 2 : 1) * p.buckets + 15) / 16;
     p.blocks = l.row.blocks, p.splits = l.row.splits;

@@ -74,15 +74,17 @@ __device__ __forceinline__ float halves_max(float x) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
+// the values of other lanes, by a DPP pattern
+template <int PATTERN>
+__device__ __forceinline__ float lanes_turned(float x) {
+    return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), PATTERN, 0xf, 0xf, false));
+}
 // sum over 16 neighbouring lanes, in all of them
 __device__ __forceinline__ float sum16(float x) {
-    const auto turned = [](float y, auto by) {
-        return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(y), 0x120 | decltype(by)::value, 0xf, 0xf, false));
-    };
-    x += turned(x, std::integral_constant<int, 8>{});
-    x += turned(x, std::integral_constant<int, 4>{});
-    x += turned(x, std::integral_constant<int, 2>{});
-    return x + turned(x, std::integral_constant<int, 1>{});
+    x += lanes_turned<0x128>(x);  // turned by 8 of 16
+    x += lanes_turned<0x124>(x);
+    x += lanes_turned<0x122>(x);
+    return x + lanes_turned<0x121>(x);
 }
 __device__ __forceinline__ float halves_sum(float x) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -111,6 +113,18 @@ __device__ __forceinline__ void store_chunk(elem_t* p, u32x4 x, int c8, int D) {
 #pragma unroll
         for (int i = 0; i < 7; ++i)
             if (c8 + i < D) p[c8 + i] = (elem_t)(x[i / 2] >> (16 * (i % 2)));
+    }
+}
+
+// Four elements of a row from column c4 on.
+typedef u32x2 __attribute__((aligned(2))) u32x2_any;
+__device__ __forceinline__ void store_quad(elem_t* p, u32x2 x, int c4, int D) {
+    if (c4 + 4 <= D) {
+        *reinterpret_cast<u32x2_any*>(p + c4) = x;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+            if (c4 + i < D) p[c4 + i] = (elem_t)(x[i / 2] >> (16 * (i % 2)));
     }
 }
 
@@ -264,6 +278,7 @@ __device__ __forceinline__ float ctx_table(const CtxParams& p, int bucket, int h
     return p.table_type == SJVP_BF16 ? Bf16::to_float(x) : Fp16::to_float(x);
 }
 
+__device__ __forceinline__ int ctx_all_buckets(const CtxParams& p) { return p.both ? 2 * p.buckets : p.buckets; }
 __device__ __forceinline__ int ctx_row_entries(const CtxParams& p) { return 2 * (p.far + kCtxPad) + 1; }
 
 // The bias of a head by position difference, entry far + pad for difference 0, in units of log2; -inf for keys behind a causal query,

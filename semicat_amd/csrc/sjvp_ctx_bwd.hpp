@@ -15,21 +15,27 @@ __device__ __forceinline__ float wave_sum(float x) {
     return x + __shfl_xor(x, 16);
 }
 
-// dO . o of the lane's own row, from the operands of dO and from o, and what its rounding left, in memory
+// dO . (o + what its rounding left) over eight columns
+template <typename T>
+__device__ __forceinline__ float piece_delta(u32x4 g, u32x4 o, u32x4 rest) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 32; e += 16)
+            sum += T::to_float((elem_t)(g[j] >> e)) * (T::to_float((elem_t)(o[j] >> e)) + T::to_float((elem_t)(rest[j] >> e)));
+    return sum;
+}
+
+// the same over the lane's own row, from the operands of dO
 template <typename T, int HD>
 __device__ __forceinline__ float row_delta(const CtxParams& p, const u32x4* own_g, const elem_t* o, const elem_t* rest, bool ok, int h) {
     float sum = 0.0f;
 #pragma unroll
     for (int c = 0; c < HD / 16; ++c) {
         if (!ok) continue;
-        const u32x4 x = load_chunk(o, 16 * c + 8 * h, p.D);
-        u32x4 y = {0u, 0u, 0u, 0u};
-        if (rest) y = load_chunk(rest, 16 * c + 8 * h, p.D);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int e = 0; e < 32; e += 16)
-                sum += T::to_float((elem_t)(own_g[c][j] >> e)) * (T::to_float((elem_t)(x[j] >> e)) + T::to_float((elem_t)(y[j] >> e)));
+        const u32x4 none = {0u, 0u, 0u, 0u};
+        sum += piece_delta<T>(own_g[c], load_chunk(o, 16 * c + 8 * h, p.D), rest ? load_chunk(rest, 16 * c + 8 * h, p.D) : none);
     }
     return halves_sum(sum);
 }
@@ -54,6 +60,22 @@ __device__ __forceinline__ float diagonals(const f32x16& x) {
         sum = __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(sum), 0x138, 0xf, 0xf, true)) + (y & 4 ? upper : lower)[r];
     }
     return sum;
+}
+
+// From a workgroup's sums by difference (`count` waves, one after another) to its sums by bucket: 16 lanes to a bucket.
+__device__ __forceinline__ void write_buckets(const CtxParams& p, const float* hists, int count, float* out, bool any, int tid, int threads) {
+    const int nb = ctx_all_buckets(p), zero = p.far + kCtxPad, entries = ctx_row_entries(p);
+    for (int bucket = tid / 16; bucket < (nb + 15) / 16 * 16; bucket += threads / 16) {
+        const int side = bucket >= p.buckets, j = min(bucket - side * p.buckets, p.buckets - 1);
+        const int from = p.first[j], to = j + 1 < p.buckets ? p.first[j + 1] - 1 : zero;  // distances
+        const int lo = side ? zero + max(from, 1) : zero - to;
+        const int hi = side ? zero + to : !p.both && j == 0 ? entries - 1 : zero - from;  // (above zero: distance 0)
+        float sum = 0.0f;
+        for (int x = lo + (tid & 15); x <= hi; x += 16)
+            for (int k = 0; k < count; ++k) sum += hists[k * entries + x];
+        sum = sum16(sum);
+        if ((tid & 15) == 0 && bucket < nb) out[bucket] = any ? sum : 0.0f;
+    }
 }
 
 // Row-owned: four waves of 32 query rows of one head share tiles of 64 keys.
@@ -197,21 +219,8 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 && !BIAS ? 3 : 2) void ctx_bw
         below = wave_sum(below), above = wave_sum(above);
         if (lane == 0) hist[0] += below, hist[entries - 1] += above;
         workgroup_barrier();
-        const float* hists = row + entries;
-        const int nb = p.both ? 2 * p.buckets : p.buckets, zero = p.far + kCtxPad;
-        float* out = p.tpart + (((int64_t)hq * p.B + b) * nqb * p.splits + (int64_t)qb * p.splits + split) * nb;
-        for (int bucket = tid / 16; bucket < (nb + 15) / 16 * 16; bucket += kCtxThreads / 16) {  // 16 lanes to a bucket
-            const int side = bucket >= p.buckets, j = min(bucket - side * p.buckets, p.buckets - 1);
-            const int from = p.first[j], to = j + 1 < p.buckets ? p.first[j + 1] - 1 : zero;  // distances
-            const int lo = side ? zero + max(from, 1) : zero - to;
-            const int hi = side ? zero + to : !p.both && j == 0 ? entries - 1 : zero - from;  // (above zero: distance 0)
-            float sum = 0.0f;
-            for (int x = lo + (lane & 15); x <= hi; x += 16)
-#pragma unroll
-                for (int k = 0; k < kCtxWaves; ++k) sum += hists[k * entries + x];
-            sum = sum16(sum);
-            if ((lane & 15) == 0 && bucket < nb) out[bucket] = bt.any_scored(p) ? sum : 0.0f;
-        }
+        write_buckets(p, row + entries, kCtxWaves, p.tpart + (((int64_t)hq * p.B + b) * nqb * p.splits + (int64_t)qb * p.splits + split) * ctx_all_buckets(p),
+                      bt.any_scored(p), tid, kCtxThreads);
     }
 }
 
@@ -338,6 +347,171 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_col(Ctx
         store_rows<T, HD>(dk, scored ? p.scale : 0.0f, p.dk.head(b, hk) + (int64_t)k0 * p.dk.sl, p.dk.sl, out_rows, region, lane, p.D);
         store_rows<T, HD>(dv, ok ? 1.0f : 0.0f, p.dv.head(b, hk) + (int64_t)k0 * p.dv.sl, p.dv.sl, out_rows, region, lane, p.D);
     }
+}
+
+// One launch for both, where a workgroup's waves own all keys of a sequence between them (up to 32 * WAVES; head dimensions 33 to
+// 64): five contractions, and each input is read once.  Column-owned as above; a tile's dS goes to LDS as well, where the dQ of the
+// tile's rows is contracted over all keys, by a quarter of 32 rows x 32 columns for each of four waves.  With eight waves the two
+// halves of the workgroup take turns, and the other half is ahead with the next tile's scores meanwhile.
+// B=128 H=12 L=256 D=64 with bias: 132 us row-owned + 125 column-owned.
+template <typename T, bool BIAS, bool DMA, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 2) void ctx_bwd_one(CtxParams p) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    constexpr int HD = 64, NT = 64 * WAVES, kTile = Tile<HD, DMA>::kElems, kX = Tile<HD, false>::kElems;
+    elem_t* const K = reinterpret_cast<elem_t*>(smem);                   // [WAVES / 2] tiles of all keys
+    elem_t* const tiles = K + WAVES / 2 * kTile;                         // [2][Q, dO]
+    elem_t* const X = tiles + 4 * kTile;                                 // [WAVES / 2] tiles of dS, rows: keys, columns: query rows
+    float* const stats = reinterpret_cast<float*>(X + WAVES / 2 * kX);   // [2][lse, delta][64]
+    float* const bias_row = stats + 4 * kCtxTile;                        // with 28 entries of -inf behind it
+    const int entries = ctx_row_entries(p);
+    float* const hists = bias_row + entries + 28;
+    const CtxWork w = ctx_work(p.B * p.Hkv, 1);
+    if (!w.some) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+    const int b = w.unit / p.Hkv, hk = w.unit % p.Hkv;
+    const CtxBatch bt(p, b);
+    const int k0 = 32 * wave, key = k0 + (lane & 31);
+    const bool ok = key < bt.keys;
+    const int per_head = (p.Lq + kCtxTile - 1) / kCtxTile, all = p.G * per_head;
+    float* const hist = hists + wave * entries;
+
+    TileFeed<HD, DMA, NT> qf(p.q.sl, p.D, tid), gf(p.g.sl, p.D, tid), kf(p.k.sl, p.D, tid);
+    const Tile<HD, DMA> at(lane);
+    const Tile<HD, false> x_at(lane);
+    // The statistics of a tile's rows: WAVES lanes to a row, each with every WAVES-th piece of dO, o and its rest.
+    constexpr int kPieces = HD / 8 / WAVES;
+    u32x4 g_piece[kPieces], o_piece[kPieces], r_piece[kPieces];
+    float lse_next = 0.0f;
+    const auto place = [&](int x) { return tiles + (x & 1) * 2 * kTile; };
+    const auto request = [&](int x) {
+        const int hq = hk * p.G + x / per_head, r0 = x % per_head * kCtxTile;
+        qf.request(p.q.head(b, hq) + (int64_t)r0 * p.q.sl, p.q.sl, bt.rows - r0, p.D, place(x), wave);
+        gf.request(p.g.head(b, hq) + (int64_t)r0 * p.g.sl, p.g.sl, bt.rows - r0, p.D, place(x) + kTile, wave);
+        const int i = r0 + tid / WAVES;
+        const bool mine = i < bt.rows;
+        lse_next = mine ? p.lse[((int64_t)b * p.Hq + hq) * p.Lq + i] : -INFINITY;
+#pragma unroll
+        for (int j = 0; j < kPieces; ++j) {
+            const int c8 = 8 * (tid % WAVES + WAVES * j);
+            const u32x4 none = {0u, 0u, 0u, 0u};
+            g_piece[j] = mine ? load_chunk(p.g.head(b, hq) + (int64_t)i * p.g.sl, c8, p.D) : none;
+            o_piece[j] = mine ? load_chunk(p.o.head(b, hq) + (int64_t)i * p.o.sl, c8, p.D) : none;
+            r_piece[j] = mine && p.rest.ptr ? load_chunk(p.rest.head(b, hq) + (int64_t)i * p.rest.sl, c8, p.D) : none;
+        }
+    };
+    const auto deliver = [&](int x) {
+        qf.deliver(place(x), p.D, tid);
+        gf.deliver(place(x) + kTile, p.D, tid);
+        float delta = 0.0f;
+#pragma unroll
+        for (int j = 0; j < kPieces; ++j) delta += piece_delta<T>(g_piece[j], o_piece[j], r_piece[j]);
+        delta += lanes_turned<0xB1>(delta);  // lanes 1, 0, 3, 2 of four
+        delta += lanes_turned<0x4E>(delta);  // 2, 3, 0, 1
+        if (WAVES == 8) delta += lanes_turned<0x141>(delta);  // 7 .. 0 of eight
+        if (tid % WAVES == 0) {
+            float* st = stats + (x & 1) * 2 * kCtxTile + tid / WAVES;
+            st[0] = lse_next == -INFINITY ? INFINITY : lse_next * kLog2e;
+            st[kCtxTile] = delta;
+        }
+    };
+    for (int t = 0; t < WAVES / 2; ++t) {
+        kf.request(p.k.head(b, hk) + (int64_t)t * kCtxTile * p.k.sl, p.k.sl, bt.keys - t * kCtxTile, p.D, K + t * kTile, wave);
+        kf.deliver(K + t * kTile, p.D, tid);
+    }
+    request(0);
+    u32x4 own_k[HD / 16], own_v[HD / 16];
+    own_operands<HD>(own_k, p.k.head(b, hk) + (int64_t)key * p.k.sl, ok, h, p.D);
+    own_operands<HD>(own_v, p.v.head(b, hk) + (int64_t)key * p.v.sl, ok, h, p.D);
+    if (BIAS && tid < 28) bias_row[entries + tid] = -INFINITY;
+    deliver(0);
+    f32x16 dk[HD / 32] = {}, dv[HD / 32] = {};
+    for (int x = 0; x < all; ++x) {
+        const int hq = hk * p.G + x / per_head, r0 = x % per_head * kCtxTile, p0 = bt.start + r0;
+        if (BIAS && r0 == 0) {
+            fill_bias_row(p, bias_row, hq, tid, NT);
+            for (int y = lane; y < entries; y += 64) hist[y] = 0.0f;
+        }
+        if (x == 0) qf.arrived();
+        if (x == 0 || (BIAS && r0 == 0)) workgroup_barrier();
+        if (x + 1 < all) request(x + 1);
+        const elem_t* Q = place(x);
+        const float* st = stats + (x & 1) * 2 * kCtxTile;
+        f32x16 s[2], ds[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            s[u] = scores<T>(at, Q, 32 * u, own_k);
+            ds[u] = scores<T>(at, Q + kTile, 32 * u, own_v);
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            // keys that do not exist have the bias -inf
+            const float* bias = bias_row + (ok ? row_entry(p, key - p0 - 32 * u - 4 * h - 27, 28) : entries) + 27;
+            const float one = ok ? 0.0f : -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const f32x4 lse = *reinterpret_cast<const f32x4*>(st + 32 * u + 8 * i + 4 * h);
+                const f32x4 delta = *reinterpret_cast<const f32x4*>(st + kCtxTile + 32 * u + 8 * i + 4 * h);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float y = s[u][4 * i + j];
+                    if constexpr (BIAS) y = fast_exp2(__builtin_fmaf(y, p.c, bias[-(8 * i + j)]) - lse[j]);
+                    else y = fast_exp2(__builtin_fmaf(y, p.c, one - lse[j]));
+                    s[u][4 * i + j] = y;
+                    ds[u][4 * i + j] = y * (ds[u][4 * i + j] - delta[j]);
+                }
+            }
+            if constexpr (BIAS) {
+                const float sum = diagonals(ds[u]);  // (looped rows are the queries here)
+                if (lane < 63) hist[row_entry(p, k0 - p0 - 32 * u - 31, 63) + lane] += sum;
+                wave_exchange();
+            }
+        }
+        workgroup_barrier();  // the last tile's dS has been read
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<u32x2*>(X + key * (HD + 8) + 32 * u + 8 * i + 4 * h) =
+                    u32x2{T::pack2(ds[u][4 * i], ds[u][4 * i + 1]), T::pack2(ds[u][4 * i + 2], ds[u][4 * i + 3])};
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            add_columns<T>(dv, at, Q + kTile, 32 * u, s[u]);
+            add_columns<T>(dk, at, Q, 32 * u, ds[u]);
+        }
+        if (x + 1 < all) deliver(x + 1);
+        qf.arrived();
+        workgroup_barrier();
+        if (WAVES == 4 || (wave >> 2) == (x & 1)) {
+            const int dt = wave & 1, uq = wave >> 1 & 1, i = r0 + 32 * uq + (lane & 31);
+            f32x16 dq = {};
+            const int steps = (bt.keys + 15) / 16;
+#pragma unroll 4
+            for (int m = 0; m < steps; ++m)
+                dq = Mma32<T>::run(at.columns(K + (m >> 2) * kTile, 16 * (m & 3), dt), x_at.columns(X + (m >> 2) * kX, 16 * (m & 3), uq), dq);
+            // a row that sees one key has no gradient of its score: exactly none, not what rounding leaves
+            const float f = bt.seen(p, i) == 1 ? 0.0f : p.scale;
+            if (i < p.Lq) {
+                elem_t* out = p.dq.head(b, hq) + (int64_t)i * p.dq.sl;
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    float z[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) z[j] = f == 0.0f ? 0.0f : dq[4 * y + j] * f;
+                    store_quad(out, u32x2{T::pack2(z[0], z[1]), T::pack2(z[2], z[3])}, 32 * dt + 8 * y + 4 * h, p.D);
+                }
+            }
+        }
+        if (BIAS && p.tpart && r0 + kCtxTile >= p.Lq) {
+            write_buckets(p, hists, WAVES, p.tpart + ((int64_t)hq * p.B + b) * ctx_all_buckets(p), bt.any_scored(p), tid, NT);
+            workgroup_barrier();
+        }
+    }
+    workgroup_barrier();
+    const bool scored = ok && bt.any_scored(p);
+    const int out_rows = min(max(p.Lk - k0, 0), 32);
+    elem_t* region = X + wave * 32 * (HD + 8);
+    store_rows<T, HD>(dk, scored ? p.scale : 0.0f, p.dk.head(b, hk) + (int64_t)k0 * p.dk.sl, p.dk.sl, out_rows, region, lane, p.D);
+    store_rows<T, HD>(dv, ok ? 1.0f : 0.0f, p.dv.head(b, hk) + (int64_t)k0 * p.dv.sl, p.dv.sl, out_rows, region, lane, p.D);
 }
 
 // Adds up the splits of a launch above: one thread to eight columns of a row of dQ, or of dK and dV.

@@ -33,10 +33,13 @@ struct CtxPlan {
 CtxPlan ctx_plan_fwd(const CtxParams& p);
 CtxPlan ctx_plan_row(const CtxParams& p);
 CtxPlan ctx_plan_col(const CtxParams& p);
+bool ctx_plan_one(const CtxParams& p, CtxPlan& plan);  // whether one launch does the backward
 
 template <typename T> int ctx_forward(CtxParams p, const CtxPlan& plan, hipStream_t stream);
 // row: the row-owned launch (dQ, delta, bucket sums), else the column-owned one (dK, dV)
 template <typename T> int ctx_backward(CtxParams p, const CtxPlan& plan, bool row, hipStream_t stream);
+
+template <typename T> int ctx_backward_one(CtxParams p, const CtxPlan& plan, hipStream_t stream);
 
 // Calls f with the padded head dimension, and whether tiles come by LDS-DMA, as constants.
 template <typename F>

@@ -24,4 +24,18 @@ int ctx_backward<SJVP_T>(CtxParams p, const CtxPlan& plan, bool row, hipStream_t
     });
 }
 
+template <>
+int ctx_backward_one<SJVP_T>(CtxParams p, const CtxPlan& plan, hipStream_t stream) {
+    p.blocks = p.splits = 1;
+    const int grid = (int)ctx_grid((int)plan.units, 1);
+    const auto run = [&](auto bias, auto dma) {
+        constexpr bool BIAS = decltype(bias)::value, DMA = decltype(dma)::value;
+        return plan.waves == 8 ? launch(ctx_bwd_one<SJVP_T, BIAS, DMA, 8>, grid, plan.smem, stream, p, 512)
+                               : launch(ctx_bwd_one<SJVP_T, BIAS, DMA, 4>, grid, plan.smem, stream, p, 256);
+    };
+    const std::true_type yes;
+    const std::false_type no;
+    return p.table ? plan.dma ? run(yes, yes) : run(yes, no) : plan.dma ? run(no, yes) : run(no, no);
+}
+
 }  // namespace sjvp
