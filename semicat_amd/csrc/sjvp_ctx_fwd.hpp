@@ -181,7 +181,7 @@ __global__ __launch_bounds__(kCtxThreads, 2) void ctx_fwd(CtxParams p) {
 // `packed` heads of a group stand in one block's rows: all of them, or one where their bias rows would not fit or a head
 // fills a block by itself.
 template <typename T, int HD, bool BIAS, bool REST, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, HD <= 64 ? 3 : 2) void ctx_fwd_few(CtxParams p) {
+__global__ __launch_bounds__(64 * WAVES, HD <= 64 ? 4 : 2) void ctx_fwd_few(CtxParams p) {
     extern __shared__ __align__(16) unsigned char smem[];
     constexpr int kRegion = 32 * (HD + 8), kSum = HD + 4;
     elem_t* region = reinterpret_cast<elem_t*>(smem);  // [WAVES] V tiles, then the waves' sums [WAVES][32][HD + 4] fp32
