@@ -72,7 +72,7 @@ __device__ __forceinline__ float ctx_lse(float ref, float l) { return (ref + fas
 // Many rows: four waves of 32 rows of one head share tiles of 64 keys.  Two tiles of K and V in LDS: the next one is on its way
 // while this one is used, one barrier to a tile.
 template <typename T, int HD, bool BIAS, bool DMA, bool REST>
-__global__ __launch_bounds__(kCtxThreads, 2) void ctx_fwd(CtxParams p) {
+__global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 4 : 2) void ctx_fwd(CtxParams p) {
     extern __shared__ __align__(16) unsigned char smem[];
     constexpr int kTile = Tile<HD, DMA>::kElems;
     elem_t* tiles = reinterpret_cast<elem_t*>(smem);  // K [2], V [2]
@@ -105,64 +105,54 @@ __global__ __launch_bounds__(kCtxThreads, 2) void ctx_fwd(CtxParams p) {
     if constexpr (BIAS) fill_bias_row(p, row, hq, tid, kCtxThreads);
     if (nt) {
         k_deliver(0), v_deliver(0);
-        if (nt > 1) k_request(1);
     }
     kf.arrived();
     workgroup_barrier();
     RowSums<HD> st;
-    f32x16 s[2], next[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) s[u] = scores<T>(at, tiles, 32 * u, own);
-    if (nt > 1) k_deliver(1);
-    workgroup_barrier();
-    // Scores of one tile are contracted beside the exponentials of the one before, which the vector unit is busy with.
     // The sequence's last tile may need a mask and has code of its own behind the loops (as a condition within, the compiler makes the
     // mask a select in every tile, a third of the vector instructions at D = 64).
-    const auto tile = [&](int t, bool masked, auto more, auto band) {
+    const auto tile = [&](int t, bool masked, bool more, auto band) {
         constexpr bool kEven = decltype(band)::value != kNear;
         const int key = t * kCtxTile;
         if (more) {
-            if (t + 2 < nt) k_request(t + 2);
+            k_request(t + 1);
             v_request(t + 1);
         }
         if (key < n_wave) {
+            f32x16 s[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) s[u] = scores<T>(at, k_place(t), 32 * u, own);
             const float one = !BIAS ? 0.0f : row[band == kBelow ? 0 : 2 * (p.far + kCtxPad)];
             if constexpr (!kEven) {
 #pragma unroll
                 for (int u = 0; u < 2; ++u) st.bias(p, s[u], key + 32 * u, h, row, pos);
             }
             st.template raise<kEven>(p, s, one, bt.keys - key, h, masked);
-            if constexpr (more) {
-#pragma unroll
-                for (int u = 0; u < 2; ++u) next[u] = scores<T>(at, k_place(t + 1), 32 * u, own);
-            }
             st.template exponentials<kEven>(p, s, one);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 if constexpr (REST) add_columns_exact<T>(st.acc, at, v_place(t), 32 * u, s[u]);
                 else add_columns<T>(st.acc, at, v_place(t), 32 * u, s[u]);
             }
-            if constexpr (more) s[0] = next[0], s[1] = next[1];
         }
         if (more) {
-            if (t + 2 < nt) k_deliver(t + 2);
+            k_deliver(t + 1);
             v_deliver(t + 1);
         }
         kf.arrived();
         workgroup_barrier();
     };
-    const std::true_type more;
     if constexpr (BIAS) {
         const int first = bt.start + qb * kCtxOwned;
         const int near = tiles_before(first - p.far + 1, nt - 1), above = tiles_before(first + kCtxOwned - 1 + p.far + kCtxTile - 1, nt - 1);
         int t = 0;
-        for (; t < near; ++t) tile(t, false, more, InBand<kBelow>{});
-        for (; t < above; ++t) tile(t, false, more, InBand<kNear>{});
-        for (; t + 1 < nt; ++t) tile(t, false, more, InBand<kAbove>{});
+        for (; t < near; ++t) tile(t, false, true, InBand<kBelow>{});
+        for (; t < above; ++t) tile(t, false, true, InBand<kNear>{});
+        for (; t + 1 < nt; ++t) tile(t, false, true, InBand<kAbove>{});
     } else {
-        for (int t = 0; t + 1 < nt; ++t) tile(t, false, more, InBand<kBelow>{});
+        for (int t = 0; t + 1 < nt; ++t) tile(t, false, true, InBand<kBelow>{});
     }
-    if (nt) tile(nt - 1, nt * kCtxTile > bt.keys, std::false_type{}, InBand<BIAS ? kNear : kBelow>{});
+    if (nt) tile(nt - 1, nt * kCtxTile > bt.keys, false, InBand<BIAS ? kNear : kBelow>{});
     const int out_rows = min(max(p.Lq - q0, 0), 32);
     const float both = halves_sum(st.l), l = (lane & 31) < rows ? both : 0.0f;
     const float f = l == 0.0f ? 0.0f : 1.0f / l;
