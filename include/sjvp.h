@@ -36,7 +36,7 @@
  *     void*) of the CURRENT device and returns without synchronising.
  *   - Every function returns SJVP_OK (0) or a negative error code; nothing aborts or throws.
  *     Argument errors are detected before anything is launched.
- *   - Results are deterministic: no atomics are used but among the lanes of one wave, whose order is fixed.
+ *   - Results are deterministic: no atomics are used.
  */
 #ifndef SJVP_H
 #define SJVP_H
@@ -291,9 +291,10 @@ int sjvp_cast(int n, const void* const* x, void* const* y, const int64_t* count,
  *       distances in ascending order from 0, the last one at most SJVP_CTX_MAX_DISTANCE; a distance has the last bucket that does
  *       not begin beyond it.  bidirectional: keys behind a query (j > start + i) have buckets of their own,
  *       buckets .. 2 buckets - 1, by their distance; otherwise they count as distance 0.
- *   o_rest (or NULL)   what the rounding of o left, in o's type.  A forward that is given it forms o with probabilities of 16 bits or
- *       more and stores it; the backward needs it for rowsum(dO * o), of which dS is a small difference where attention is
- *       sharp, and which the gradient of an fp32 table (formed to some 1e-6 with it) is a sum over.
+ *   o_rest (or NULL)   what the rounding of o left, 16 bits to an element in a form of its own, for the backward.  A forward that is
+ *       given it forms o with probabilities of 16 bits or more (24 where the table is fp32) and stores it; the backward needs it
+ *       for rowsum(dO * o), of which dS is a small difference where attention is sharp, and which the gradient of an fp32 table
+ *       (formed to some 1e-6 with it) is a sum over.
  *   lse   [B,Hq,Lq] fp32 contiguous; the forward takes NULL where no backward follows.
  *   dk, dv   both or neither (then without the launch that makes them)
  *   dtable (or NULL)   in the type of table, with strides dtable_stride; summed in fp32 in a fixed order.

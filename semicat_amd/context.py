@@ -163,8 +163,8 @@ def context_forward(q: Tensor, k: Tensor, v: Tensor, bias: Optional[RelativeBias
                     o: Optional[Tensor] = None, o_rest: Optional[Tensor] = None, with_lse: bool = True
                     ) -> Tuple[Tensor, Optional[Tensor]]:
     """Forward on ``[B,H,L,D]`` views: ``(o, lse)``, with ``lse`` fp32 ``[B,Hq,Lq]``, or None without ``with_lse``.  ``o`` may be
-    passed in to be filled, and ``o_rest``, a tensor like it, to receive what the rounding of ``o`` leaves, for
-    :func:`context_backward`."""
+    passed in to be filled, and ``o_rest``, a tensor like it, to receive what the rounding of ``o`` leaves (16 bits
+    in a form of their own), for :func:`context_backward`."""
     _check_inputs(q, k, v, bias, key_lengths, query_lengths, query_start)
     B, H, Lq, D = q.shape
     if o is None:

@@ -51,7 +51,7 @@ struct CtxView {
 };
 
 struct CtxParams {
-    CtxView q, k, v, o, rest, g, dq, dk, dv;  // rest: o minus its rounding (or null); g: the cotangent of o
+    CtxView q, k, v, o, rest, g, dq, dk, dv;  // rest: what the rounding of o left (or null); g: the cotangent of o
     float *lse, *delta;                      // [B,Hq,Lq]
     float *part, *stat;                      // sums of split work: rows of HD floats; their (maximum, sum) pairs
     float* tpart;                            // bucket sums of each workgroup
@@ -324,10 +324,20 @@ __device__ __forceinline__ CtxWork ctx_work(int units, int inner) {
     return {unit, slot % inner, unit < units};
 }
 
-// What the rounding of two numbers to w left of them, rounded in turn.
+// What the rounding of two numbers to w left of them, as it stands in memory beside o.  fp16: the difference, which makes 22 bits in
+// all; bf16, where that would make 17: the difference of the bits as a signed number, which makes all 24.
 template <typename T>
 __device__ __forceinline__ uint32_t rest_of(uint32_t w, float lo, float hi) {
-    return T::pack2(lo - T::to_float((elem_t)w), hi - T::to_float((elem_t)(w >> 16)));
+    if constexpr (!std::is_same_v<T, Bf16>) return T::pack2(lo - T::to_float((elem_t)w), hi - T::to_float((elem_t)(w >> 16)));
+    const auto bits = [](float x, uint32_t top) {
+        return (uint32_t)min(max((int)(__float_as_uint(x) - top), -32768), 32767);
+    };
+    return (bits(lo, w << 16) & 0xffffu) | bits(hi, w & 0xffff0000u) << 16;
+}
+template <typename T>
+__device__ __forceinline__ float with_rest(elem_t o, elem_t rest) {
+    if constexpr (!std::is_same_v<T, Bf16>) return T::to_float(o) + T::to_float(rest);
+    return __uint_as_float(((uint32_t)o << 16) + (uint32_t)(int)(int16_t)rest);
 }
 
 // Sums of a wave's own 32 rows, OUT^T (row of C: column of the result), as rows in memory: through the wave's own LDS region of
@@ -400,20 +410,26 @@ __device__ __forceinline__ void add_columns(f32x16* acc, const Tile<HD, DMA>& at
     }
 }
 
-// The same with what the rounding of the scores leaves: 16 bits of them or more in all.
-template <typename T, int HD, bool DMA>
+// The same with what the rounding of the scores leaves: TERMS roundings of 8 (bf16) or 11 bits each.
+template <typename T, int TERMS, int HD, bool DMA>
 __device__ __forceinline__ void add_columns_exact(f32x16* acc, const Tile<HD, DMA>& at, const elem_t* tile, int row0, const f32x16& s) {
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
-        const u32x4 b = pack_scores<T>(s, m);
-        u32x4 rest;
+        u32x4 b[TERMS];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) rest[i] = rest_of<T>(b[i], s[8 * m + 2 * i], s[8 * m + 2 * i + 1]);
+        for (int i = 0; i < 4; ++i) {
+            float lo = s[8 * m + 2 * i], hi = s[8 * m + 2 * i + 1];
+#pragma unroll
+            for (int x = 0; x < TERMS; ++x) {
+                b[x][i] = T::pack2(lo, hi);
+                lo -= T::to_float((elem_t)b[x][i]), hi -= T::to_float((elem_t)(b[x][i] >> 16));
+            }
+        }
 #pragma unroll
         for (int dt = 0; dt < HD / 32; ++dt) {
             const u32x4 a = at.columns(tile, row0 + 16 * m, dt);
-            acc[dt] = Mma32<T>::run(a, b, acc[dt]);
-            acc[dt] = Mma32<T>::run(a, rest, acc[dt]);
+#pragma unroll
+            for (int x = 0; x < TERMS; ++x) acc[dt] = Mma32<T>::run(a, b[x], acc[dt]);
         }
     }
 }

@@ -23,7 +23,7 @@ __device__ __forceinline__ float piece_delta(u32x4 g, u32x4 o, u32x4 rest) {
     for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int e = 0; e < 32; e += 16)
-            sum += T::to_float((elem_t)(g[j] >> e)) * (T::to_float((elem_t)(o[j] >> e)) + T::to_float((elem_t)(rest[j] >> e)));
+            sum += T::to_float((elem_t)(g[j] >> e)) * with_rest<T>((elem_t)(o[j] >> e), (elem_t)(rest[j] >> e));
     return sum;
 }
 

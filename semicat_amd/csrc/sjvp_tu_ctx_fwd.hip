@@ -13,15 +13,21 @@ int ctx_forward<SJVP_T>(CtxParams p, const CtxPlan& plan, hipStream_t stream) {
     p.packed = plan.packed;
     return ctx_by_head(p.D, plan.dma, [&](auto hd, auto dma) {
         constexpr int HD = decltype(hd)::value;
-        const auto run = [&](auto bias, auto rest) {
-            constexpr bool BIAS = decltype(bias)::value, REST = decltype(rest)::value;
-            if (!plan.few) return launch(ctx_fwd<SJVP_T, HD, BIAS, decltype(dma)::value, REST>, grid, plan.smem, stream, p, kCtxThreads);
-            return plan.waves == 8 ? launch(ctx_fwd_few<SJVP_T, HD, BIAS, REST, 8>, grid, plan.smem, stream, p, 512)
-                                   : launch(ctx_fwd_few<SJVP_T, HD, BIAS, REST, 4>, grid, plan.smem, stream, p, 256);
+        const auto run = [&](auto bias, auto terms) {
+            constexpr bool BIAS = decltype(bias)::value;
+            constexpr int TERMS = decltype(terms)::value;
+            if (!plan.few) return launch(ctx_fwd<SJVP_T, HD, BIAS, decltype(dma)::value, TERMS>, grid, plan.smem, stream, p, kCtxThreads);
+            return plan.waves == 8 ? launch(ctx_fwd_few<SJVP_T, HD, BIAS, TERMS, 8>, grid, plan.smem, stream, p, 512)
+                                   : launch(ctx_fwd_few<SJVP_T, HD, BIAS, TERMS, 4>, grid, plan.smem, stream, p, 256);
         };
         const std::true_type yes;
         const std::false_type no;
-        const int rc = p.table ? p.rest.ptr ? run(yes, yes) : run(yes, no) : p.rest.ptr ? run(no, yes) : run(no, no);
+        const std::integral_constant<int, 1> one;
+        const std::integral_constant<int, 2> two;
+        const std::integral_constant<int, std::is_same_v<SJVP_T, Bf16> ? 3 : 2> most;
+        const int rc = !p.rest.ptr ? p.table ? run(yes, one) : run(no, one)
+                       : !p.table  ? run(no, two)
+                                   : p.table_type == SJVP_FP32 ? run(yes, most) : run(yes, two);
         if (!plan.few) return rc;
         if (rc != SJVP_OK || p.splits == 1) return rc;
         int slices = 1;  // as in the kernel

@@ -51,8 +51,6 @@ def check(got, x, **options):
         a, b, c = sizes[name]
         if name == "dtable":
             limit = 2.0 ** -15 * a + u * want[name].abs()
-            if t.dtype != torch.float32:  # delta from the rounded o
-                limit += u * a
         else:
             limit = u * a + (u * u + 2.0 ** -14) * (a + b) + u * want[name].abs()
         if x["q"].dtype == FP16:
