@@ -285,7 +285,7 @@ int sjvp_cast(int n, const void* const* x, void* const* y, const int64_t* count,
  *   key_lengths, query_lengths, query_start   device arrays [B], or NULL: every sequence is as long as its tensor, and its
  *       query 0 has position query_start0 (which is added to query_start[b] otherwise).  Lengths are clamped to the tensor.  What
  *       lies in rows behind a length is not used, not even NaN; results there are zeros.  query_start and query_start0 lie within +-2^29.
- *   a row that sees no key (also: whose every key has the bias -inf) has o = 0, lse = -inf and no gradient.
+ *   a row that sees no key (also: whose every key has the bias -inf) has o = 0, lse = -inf and no gradient, for any finite dO.
  *   table (or NULL: no bias, causal must be 0)   fp32, bf16 or fp16 [buckets of all directions][Hq] with strides table_stride
  *       (bucket, head); entries below -2.3e38 count as that, -inf excludes its keys.  bucket_first: HOST array of `buckets` first
  *       distances in ascending order from 0, the last one at most SJVP_CTX_MAX_DISTANCE; a distance has the last bucket that does
@@ -296,6 +296,7 @@ int sjvp_cast(int n, const void* const* x, void* const* y, const int64_t* count,
  *       for rowsum(dO * o), of which dS is a small difference where attention is sharp, and which the gradient of an fp32 table
  *       (formed to some 1e-6 with it) is a sum over.
  *   lse   [B,Hq,Lq] fp32 contiguous; the forward takes NULL where no backward follows.
+ *   dO   fp16: dS = P (dP - delta) is rounded to fp16 on its way into dQ and dK, so that losses are scaled as usual with this type.
  *   dk, dv   both or neither (then without the launch that makes them)
  *   dtable (or NULL)   in the type of table, with strides dtable_stride; summed in fp32 in a fixed order.
  * strides[3*i + {0,1,2}]: (batch, head, sequence) strides in elements of tensor i of sjvp_ctx_tensor.  scale 0: 1/sqrt(D).

@@ -105,6 +105,8 @@ def _check_inputs(q, k, v, bias, key_lengths, query_lengths, query_start) -> Non
     B, H, Lq, D = q.shape
     if D < 16 or D > 128:
         raise ValueError(f"the head dimension must lie within 16 and 128, got {D}")
+    if max(*q.shape, *k.shape) > _lib.SJVP_CTX_MAX_POSITION:
+        raise ValueError(f"sizes must not exceed {_lib.SJVP_CTX_MAX_POSITION}, got {tuple(q.shape)} and {tuple(k.shape)}")
     if k.shape[1] < 1 or H % max(k.shape[1], 1):
         raise AssertionError(f"{H} query heads cannot share {k.shape[1]} key heads")
     _check("q", q, q.shape, q)

@@ -177,7 +177,10 @@ CtxLayout ctx_layout(const CtxParams& p, bool backward) {
     return l;
 }
 
-bool ctx_fits(const CtxPlan& plan) { return ctx_grid((int)std::min<int64_t>(plan.units, INT_MAX), 1) * plan.inner <= INT_MAX; }
+// A launch holds fewer than 2^32 threads.
+bool ctx_fits(const CtxPlan& plan) {
+    return std::max(plan.units, plan.inner) <= INT_MAX && ctx_grid(plan.units, plan.inner) <= UINT32_MAX / (64 * plan.waves);
+}
 
 int ctx_workspace(const sjvp_ctx* t, const CtxLayout& l, float*& ws) {
     ws = static_cast<float*>(t->workspace);
@@ -219,7 +222,8 @@ int sjvp_ctx_bwd(const sjvp_ctx* t, int dtype, void* stream) {
     if (dtype != SJVP_BF16 && dtype != SJVP_FP16) return SJVP_ERR_DTYPE;
     if (!t->q || !t->k || !t->v || !t->o || !t->dO || !t->dq || !t->dk != !t->dv || !t->lse) return SJVP_ERR_NULL;
     CtxLayout l = ctx_layout(p, true);
-    if (!ctx_fits(l.row) || !ctx_fits(l.col)) return SJVP_ERR_SHAPE;
+    const int64_t per = ((p.both ? 2 : 1) * p.buckets + 15) / 16;  // workgroups of ctx_table_sum to a head
+    if (!ctx_fits(l.row) || !ctx_fits(l.col) || !ctx_fits(l.one) || p.Hq * per > UINT32_MAX / 256) return SJVP_ERR_SHAPE;
     float* ws;
     if (ctx_workspace(t, l, ws) != SJVP_OK) return SJVP_ERR_WORKSPACE;
     p.delta = ws + l.delta, p.part = ws + l.part, p.tpart = p.dtable ? ws + l.tpart : nullptr;
@@ -235,9 +239,8 @@ int sjvp_ctx_bwd(const sjvp_ctx* t, int dtype, void* stream) {
         if (rc == SJVP_OK && t->dk) rc = run(l.col, false);
     }
     if (rc != SJVP_OK || !p.dtable) return rc;
-    const int per = ((p.both ? 2 : 1) * p.buckets + 15) / 16;
     p.blocks = l.row.blocks, p.splits = l.row.splits;
-    return launch(ctx_table_sum, p.Hq * per, 0, s, p, 256);
+    return launch(ctx_table_sum, (int)(p.Hq * per), 0, s, p, 256);
 }
 
 }  // extern "C"

@@ -283,12 +283,12 @@ __device__ __forceinline__ int ctx_row_entries(const CtxParams& p) { return 2 * 
 
 // The bias of a head by position difference, entry far + pad for difference 0, in units of log2; -inf for keys behind a causal query,
 // so that the kernels need no other mask for these.  A table entry near the lowest float32 would leave the range with the factor
-// log2(e); it is raised to -2.3e38, still below any score.
+// log2(e); it is raised to -2.3e38, still below any score.  NaN stays.
 __device__ __forceinline__ void fill_bias_row(const CtxParams& p, float* row, int head, int tid, int threads) {
     for (int x = tid; x < ctx_row_entries(p); x += threads) {
         const int rel = x - p.far - kCtxPad;
         const float t = ctx_table(p, ctx_bucket(p, rel), head);
-        row[x] = t == -INFINITY || (p.causal && rel > 0) ? -INFINITY : fmaxf(t, -2.3e38f) * kLog2e;
+        row[x] = t == -INFINITY || (p.causal && rel > 0) ? -INFINITY : (t < -2.3e38f ? -2.3e38f : t) * kLog2e;
     }
 }
 
@@ -313,9 +313,9 @@ struct CtxWork {
     int unit, inner;
     bool some;
 };
-inline __host__ __device__ bool ctx_by_xcd(int units) { return units % 8 == 0 || units >= 64; }
-inline __host__ __device__ int64_t ctx_grid(int units, int inner) {
-    return (int64_t)(ctx_by_xcd(units) ? (units + 7) / 8 * 8 : units) * inner;
+inline __host__ __device__ bool ctx_by_xcd(int64_t units) { return units % 8 == 0 || units >= 64; }
+inline __host__ __device__ int64_t ctx_grid(int64_t units, int64_t inner) {
+    return (ctx_by_xcd(units) ? (units + 7) / 8 * 8 : units) * inner;
 }
 __device__ __forceinline__ CtxWork ctx_work(int units, int inner) {
     const int x = blockIdx.x;

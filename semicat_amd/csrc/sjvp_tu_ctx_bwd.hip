@@ -9,7 +9,7 @@ namespace sjvp {
 template <>
 int ctx_backward<SJVP_T>(CtxParams p, const CtxPlan& plan, bool row, hipStream_t stream) {
     p.blocks = plan.blocks, p.splits = plan.splits, p.cols = !row;
-    const int grid = (int)ctx_grid((int)plan.units, (int)plan.inner);
+    const int grid = (int)ctx_grid(plan.units, plan.inner);
     return ctx_by_head(p.D, plan.dma, [&](auto hd, auto dma) {
         constexpr int HD = decltype(hd)::value;
         constexpr bool DMA = decltype(dma)::value;
@@ -27,7 +27,7 @@ int ctx_backward<SJVP_T>(CtxParams p, const CtxPlan& plan, bool row, hipStream_t
 template <>
 int ctx_backward_one<SJVP_T>(CtxParams p, const CtxPlan& plan, hipStream_t stream) {
     p.blocks = p.splits = 1;
-    const int grid = (int)ctx_grid((int)plan.units, 1);
+    const int grid = (int)ctx_grid(plan.units, 1);
     const auto run = [&](auto bias, auto dma) {
         constexpr bool BIAS = decltype(bias)::value, DMA = decltype(dma)::value;
         return plan.waves == 8 ? launch(ctx_bwd_one<SJVP_T, BIAS, DMA, 8>, grid, plan.smem, stream, p, 512)

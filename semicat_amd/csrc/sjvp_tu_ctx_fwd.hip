@@ -9,7 +9,7 @@ namespace sjvp {
 template <>
 int ctx_forward<SJVP_T>(CtxParams p, const CtxPlan& plan, hipStream_t stream) {
     p.blocks = plan.blocks, p.splits = plan.splits;
-    const int grid = (int)ctx_grid((int)plan.units, (int)plan.inner);
+    const int grid = (int)ctx_grid(plan.units, plan.inner);
     p.packed = plan.packed;
     return ctx_by_head(p.D, plan.dma, [&](auto hd, auto dma) {
         constexpr int HD = decltype(hd)::value;

@@ -72,6 +72,7 @@ def _t(*shape, dtype=torch.bfloat16):
     (TypeError, lambda: context_forward(*[_t(1, 2, 3, 32)] * 3, query_lengths=_t(1, dtype=torch.float32))),
     (AssertionError, lambda: context_forward(*[_t(1, 2, 3, 32)] * 3, query_start=_t(1, 1, dtype=torch.int32))),
     (ValueError, lambda: context_forward(*[_t(1, 2, 3, 32)] * 3, query_start=1 << 30)),
+    (ValueError, lambda: context_forward(_t(1, 2, 3, 32), *[_t(1, 2, 1, 32).expand(1, 2, (1 << 32) + 3, 32)] * 2)),
     (ValueError, lambda: context_forward(*[_t(1, 2, 3, 32)] * 3, scale=-1.0)),
     (AssertionError, lambda: context_forward(*[_t(1, 2, 3, 32)] * 3, bias=RelativeBias(_t(8, 3)))),
     (ValueError, lambda: RelativeBias(_t(7, 2))),
@@ -115,8 +116,8 @@ def test_status_of_the_c_abi_beyond_the_fields():
     assert lib.sjvp_ctx_fwd(None, 0, None) == _lib.SJVP_ERR_NULL
     assert lib.sjvp_ctx_fwd(ctypes.byref(_ctx()), 2, None) == _lib.SJVP_ERR_DTYPE
     assert lib.sjvp_ctx_bwd(ctypes.byref(_ctx(dk=None)), 0, None) == _lib.SJVP_ERR_NULL
-    assert lib.sjvp_ctx_bwd(ctypes.byref(_ctx()), 0, None) == _lib.SJVP_ERR_WORKSPACE
-    assert lib.sjvp_ctx_bwd(ctypes.byref(_ctx(workspace=64, workspace_bytes=4)), 0, None) == _lib.SJVP_ERR_WORKSPACE
+    assert lib.sjvp_ctx_bwd(ctypes.byref(_ctx(Lk=300)), 0, None) == _lib.SJVP_ERR_WORKSPACE
+    assert lib.sjvp_ctx_bwd(ctypes.byref(_ctx(Lk=300, workspace=64, workspace_bytes=4)), 0, None) == _lib.SJVP_ERR_WORKSPACE
     t = _ctx()
     t.strides[2] = 1 << 24
     assert lib.sjvp_ctx_fwd(ctypes.byref(t), 0, None) == _lib.SJVP_ERR_SHAPE
@@ -124,4 +125,8 @@ def test_status_of_the_c_abi_beyond_the_fields():
         first = (ctypes.c_int32 * len(starts))(*starts)
         t = _ctx(table=64, table_dtype=2, buckets=len(starts), bucket_first=ctypes.cast(first, ctypes.c_void_p))
         assert lib.sjvp_ctx_fwd(ctypes.byref(t), 0, None) == _lib.SJVP_ERR_BUCKETS
+    # launches of too many workgroups: no work is done, and nothing wraps round
+    for sizes in (dict(B=1 << 24), dict(B=1 << 30), dict(B=(1 << 31) - 1, Lq=1), dict(B=1 << 28, Hq=16, Hkv=16), dict(Lq=1 << 29, B=64, D=96)):
+        assert lib.sjvp_ctx_fwd(ctypes.byref(_ctx(**sizes)), 0, None) == _lib.SJVP_ERR_SHAPE, sizes
+        assert lib.sjvp_ctx_bwd(ctypes.byref(_ctx(**sizes)), 0, None) == _lib.SJVP_ERR_SHAPE, sizes
     assert b"bias" in lib.sjvp_strerror(_lib.SJVP_ERR_BUCKETS)

@@ -313,6 +313,52 @@ def test_streams_and_graphs():
         both(held)
 
 
+# one launch, a pair of launches, a pair with split axes; few rows in splits
+@pytest.mark.parametrize("B,H,G,Lq,Lk,D,table", [(2, 4, 2, 70, 90, 64, None), (3, 4, 2, 70, 300, 32, (16, torch.float32)),
+                                                 (1, 2, 2, 130, 1500, 96, (8, BF16)), (2, 4, 4, 3, 3000, 128, None)])
+def test_training_passes_in_a_graph(B, H, G, Lq, Lk, D, table):
+    """Forward and backward through the autograd surface, captured and replayed on other inputs among eager passes."""
+    from semicat_amd import cross_attention, relative_attention
+    xs = [{n: t.cuda() for n, t in make(B, H, G, Lq, Lk, D, BF16, seed=s, table=table).items()} for s in range(3)]
+    lengths = [torch.tensor([Lk - s] + [Lk // (2 + s)] * (B - 1), dtype=torch.int32, device="cuda") for s in range(3)]
+
+    def step(x, n):
+        leaves = [x[m].detach().requires_grad_() for m in ("q", "k", "v", "table") if m in x]
+        o = cross_attention(*leaves, key_lengths=n) if table is None else relative_attention(*leaves, 64, key_lengths=n)
+        return o.detach(), *torch.autograd.grad(o, leaves, x["dO"])
+
+    want = [step(x, n) for x, n in zip(xs, lengths)]
+    held, n = {m: t.clone() for m, t in xs[0].items()}, lengths[0].clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(held, n)
+    for i in (0, 1, 2, 1):
+        for m, t in held.items():
+            t.copy_(xs[i][m])
+        n.copy_(lengths[i])
+        for t in out:
+            t.zero_()
+        graph.replay()
+        eager = step(xs[(i + 1) % 3], lengths[(i + 1) % 3])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want[i]))
+        assert all(torch.equal(a, b) for a, b in zip(eager, want[(i + 1) % 3]))
+
+
+@pytest.mark.parametrize("D,Lk", [(64, 100), (32, 300)])
+def test_table_entries_beyond_the_range(D, Lk):
+    """NaN in the table is not hidden where a key has it; -inf and the lowest float32 hide their keys."""
+    x = make(1, 2, 1, 40, Lk, D, BF16, table=(8, torch.float32))
+    x["table"][2, 0] = float("nan")
+    got = run(x, max_distance=16)
+    assert bool(got["o"][:, 2:, 0].isnan().all()) and bool(got["plain"][:, 2:, 0].isnan().all()) and bool(got["dtable"][2, 0].isnan())
+    assert not any(bool(got[n][:, :, 1].isnan().any()) for n in ("o", "plain", "dq", "dk", "dv")) and not bool(got["dtable"][:, 1].isnan().any())
+    for low in (float("-inf"), torch.finfo(torch.float32).min):
+        x["table"][2, 0] = low
+        check(run(x, max_distance=16), x, max_distance=16)
+
+
 def test_rows_without_work():
     """No batch entry, no query, no key."""
     from semicat_amd import cross_attention
