@@ -35,15 +35,25 @@ constexpr int kLds = 160 * 1024;
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Splits of a looped axis of `steps` steps for a launch of `groups` workgroups: enough for `per_unit` to a compute unit, each
-// with `least` steps or more.
-int splits_for(int64_t groups, int64_t steps, int per_unit, int64_t least) {
-    const int64_t wanted = (int64_t)per_unit * compute_units() / groups;
+// Splits of a looped axis of `steps` steps for a launch of `groups` workgroups: up to one workgroup to a compute unit, each with `least`
+// steps or more.
+int splits_for(int64_t groups, int64_t steps, int64_t least) {
+    const int64_t wanted = compute_units() / groups;
     return (int)std::max<int64_t>(1, std::min<int64_t>({wanted, steps / least, kMaxSplits}));
 }
 
 }  // namespace
 
+// Times of the rules below in microseconds, D = 64 unless said, (B,Hq,Lq,Lk) bf16; `rel`: with a bias.
+//
+// Few rows (ctx_fwd_few) where the rows of a key head fit one block, and where blocks of 128 rows would leave half of the compute
+// units idle: (2,8,512,1024) rel 15.2 / 31.4 by blocks of 128, (2,16,200,2000) D=128 28 / 65, (4,16,256,1024) 18.5 / 20.6; beyond
+// that (8,16,256,256) rel 21.6 / 14.4, (16,12,128,128) rel 11.8 / 10.2.
+//   waves: eight share the filling of a bias row for many keys, (2,8,512,1024) rel 11.5 / 12.7 with four; otherwise four, which end sooner:
+//     (64,12,1,400) 17.8 / 21.1 with eight, (4,12,256,256) rel 9.6 / 10.4, (2,16,4,16385) D=128 in groups of eight 15.2 / 16.3.
+//   packed heads read their keys once: (64,16,1,2048) D=128 in groups of four 45 / 160 one by one.
+//   splits: of 256 keys or more, since joining them is a launch of 4 us: (8,16,4,2000) D=128 in groups of eight 13.2 / 22.7 unsplit,
+//     (1,12,1,2000) rel 12.1 / 18.1; none up to 1024 keys at D = 64: (1,8,300,1000) 10.7 / 11.7 split, (1,12,1,600) 8.1 / 8.9.
 CtxPlan ctx_plan_fwd(const CtxParams& p) {
     CtxPlan plan;
     const int HD = ctx_padded(p.D), bias = p.table ? 4 * ctx_entries(p) : 0;
@@ -59,21 +69,24 @@ CtxPlan ctx_plan_fwd(const CtxParams& p) {
     }
     const int heads = p.Lq < 32 ? std::min(p.G, 31 / p.Lq + 2) : 1;  // that a block of 32 rows can touch
     const auto sums = [&](int waves) { return waves * 32 * (HD + 4 + 2) * 4; };
-    plan.waves = p.Lk >= 256 && sums(8) + heads * bias <= kLds ? 8 : 4;
+    plan.waves = p.table && p.Lk >= 1024 && sums(8) + heads * bias <= kLds ? 8 : 4;
     plan.packed = p.Lq < 32 && sums(plan.waves) + heads * bias <= kLds ? p.G : 1;
     plan.smem = sums(plan.waves) + (plan.packed > 1 ? heads : 1) * bias;
     plan.blocks = (int)ceil_div((int64_t)plan.packed * p.Lq, 32);
     plan.units = (int64_t)p.B * p.Hkv * (p.G / plan.packed);
-    plan.splits = splits_for(plan.units * plan.blocks, p.Lk, 1, 256);
+    plan.splits = (int64_t)p.Lk * HD <= 1024 * 64 ? 1 : splits_for(plan.units * plan.blocks, p.Lk, 256);
     plan.inner = (int64_t)plan.blocks * plan.splits;
     return plan;
 }
 
+// The backward pair splits its looped axes from ten tiles on while compute units are idle: the launch that adds up costs 4 us and the
+// partial sums their traffic.  (4,8,512,512) rel whole 42, in tiles of four 50; (2,8,512,1024) rel 44 / 49; the other way (8,8,300,300) D=36
+// rel in groups of two 52 in tiles of five, 58 whole, (1,8,300,300) D=128 rel in groups of two 54 / 64.
 CtxPlan ctx_plan_row(const CtxParams& p) {
     CtxPlan plan;
     plan.blocks = (int)ceil_div(p.Lq, kCtxOwned);
     plan.units = (int64_t)p.B * p.Hkv;
-    plan.splits = splits_for((int64_t)p.B * p.Hq * plan.blocks, ceil_div(p.Lk, kCtxTile), 1, 4);
+    plan.splits = splits_for((int64_t)p.B * p.Hq * plan.blocks, ceil_div(p.Lk, kCtxTile), 5);
     plan.inner = (int64_t)p.G * plan.blocks * plan.splits;
     plan.dma = ctx_dma(p, p.k, p.v);
     plan.smem = ctx_tiles_bytes(ctx_padded(p.D), plan.dma) + (p.table ? 4 * ctx_entries(p) * (1 + kCtxWaves) : 0);
@@ -84,13 +97,21 @@ CtxPlan ctx_plan_col(const CtxParams& p) {
     CtxPlan plan;
     plan.blocks = (int)ceil_div(p.Lk, kCtxOwned);
     plan.units = (int64_t)p.B * p.Hkv;
-    plan.splits = splits_for(plan.units * plan.blocks, p.G * ceil_div(p.Lq, kCtxTile), 1, 4);
+    plan.splits = splits_for(plan.units * plan.blocks, p.G * ceil_div(p.Lq, kCtxTile), 5);
     plan.inner = (int64_t)plan.blocks * plan.splits;
     plan.dma = ctx_dma(p, p.q, p.g);
     plan.smem = ctx_tiles_bytes(ctx_padded(p.D), plan.dma) + 4 * kCtxTile * 4 + (p.table ? 4 * ctx_entries(p) : 0);
     return plan;
 }
 
+// The single backward launch, against the pair.  Its workgroup walks all rows of its heads, so that the pair spreads few of them over
+// more compute units, unless the walk is short.  One workgroup of eight waves fills a compute unit: a last round that leaves many idle costs a
+// whole one.
+//   up to three tiles: 8 heads of 64 rows on 100 keys 8.6 / 13.0 by the pair, of 192 rows 15.7 / 16.7 (rel 26 / 25), of 256 rows rel 31 / 27;
+//     (8,12,128,128) 13.0 / 15.5, (11,16,100,200) rel 25 / 31, (8,16,128,256) 17 / 18.5
+//   four waves (up to 128 keys): (24,16,512,128) 50 / 60, (64,12,128,128) rel 50 / 59; few workgroups (4,16,256,128) 20.4 / 18.8, (4,16,1024,128) 65 / 36
+//   eight waves: (10,16,256,200) 27 / 30.5, (16,16,256,256) 30 / 34, (28,16,300,256) 65 / 70, (64,12,1024,256) 245 / 299; the other way
+//     (8,16,256,256) rel 37 / 34, (24,16,256,256) 52 / 47, (40,16,256,256) 78 / 73, (32,12,1024,256) 158 / 140
 bool ctx_plan_one(const CtxParams& p, CtxPlan& plan) {
     if (ctx_padded(p.D) != 64 || p.Lk > 256 || !p.dk.ptr) return false;
     plan.waves = p.Lk > 128 ? 8 : 4;
@@ -99,8 +120,11 @@ bool ctx_plan_one(const CtxParams& p, CtxPlan& plan) {
     const int tile = kCtxTile * (64 + (plan.dma ? 0 : 8)) * 2;
     plan.smem = (plan.waves / 2 + 4) * tile + plan.waves / 2 * kCtxTile * 72 * 2 + 4 * kCtxTile * 4 +
                 (p.table ? 4 * (ctx_entries(p) * (1 + plan.waves) + 28) : 0);
-    // a workgroup walks all rows of its heads: with few workgroups the pair of launches spreads them over more
-    return plan.smem <= kLds && (2 * plan.units >= compute_units() || p.G * ceil_div(p.Lq, kCtxTile) <= 4);
+    if (plan.smem > kLds) return false;
+    const int64_t units = plan.units, cu = compute_units(), rounds = ceil_div(units, cu);
+    if (rounds == 1 && p.G * ceil_div(p.Lq, kCtxTile) <= 3) return true;
+    if (plan.waves == 4) return 2 * units >= cu;
+    return rounds == 1 ? 5 * units >= 3 * cu : 7 * units >= 6 * rounds * cu;
 }
 
 namespace {

@@ -281,14 +281,18 @@ __device__ __forceinline__ float ctx_table(const CtxParams& p, int bucket, int h
 __device__ __forceinline__ int ctx_all_buckets(const CtxParams& p) { return p.both ? 2 * p.buckets : p.buckets; }
 __device__ __forceinline__ int ctx_row_entries(const CtxParams& p) { return 2 * (p.far + kCtxPad) + 1; }
 
-// The bias of a head by position difference, entry far + pad for difference 0, in units of log2; -inf for keys behind a causal query,
-// so that the kernels need no other mask for these.  A table entry near the lowest float32 would leave the range with the factor
-// log2(e); it is raised to -2.3e38, still below any score.  NaN stays.
-__device__ __forceinline__ void fill_bias_row(const CtxParams& p, float* row, int head, int tid, int threads) {
-    for (int x = tid; x < ctx_row_entries(p); x += threads) {
-        const int rel = x - p.far - kCtxPad;
-        const float t = ctx_table(p, ctx_bucket(p, rel), head);
-        row[x] = t == -INFINITY || (p.causal && rel > 0) ? -INFINITY : (t < -2.3e38f ? -2.3e38f : t) * kLog2e;
+// The bias of a head (of `heads` from it on, one row after another) by position difference, entry far + pad for difference 0, in units
+// of log2; -inf for keys behind a causal query, so that the kernels need no other mask for these.  A table entry near the lowest
+// float32 would leave the range with the factor log2(e); it is raised to -2.3e38, still below any score.  NaN stays.
+// (An entry's bucket serves all heads: filled head by head, eight heads of B=4 Lq=2 Lk=4096 D=64 took 16.9 us in place of 12.1.)
+__device__ __forceinline__ void fill_bias_row(const CtxParams& p, float* row, int head, int tid, int threads, int heads = 1) {
+    const int entries = ctx_row_entries(p);
+    for (int x = tid; x < entries; x += threads) {
+        const int rel = x - p.far - kCtxPad, bucket = ctx_bucket(p, rel);
+        for (int i = 0; i < heads; ++i) {
+            const float t = ctx_table(p, bucket, head + i);
+            row[i * entries + x] = t == -INFINITY || (p.causal && rel > 0) ? -INFINITY : (t < -2.3e38f ? -2.3e38f : t) * kLog2e;
+        }
     }
 }
 

@@ -78,7 +78,9 @@ __device__ __forceinline__ void write_buckets(const CtxParams& p, const float* h
     }
 }
 
-// Row-owned: four waves of 32 query rows of one head share tiles of 64 keys.
+// Row-owned: four waves of 32 query rows of one head share tiles of 64 keys.  Bound by the matrix unit and the vector instructions
+// together with the latency of a tile, two waves to a SIMD: B=8 H=16 L=4096 D=64 causal with bias 528 us (the matrix unit busy 36 %, vector instructions issued 56 %; three
+// contractions at 0.78 PFLOP/s), B=8 Hq=16 Hkv=4 Lq=2048 Lk=1024 D=128 224 us.
 template <typename T, int HD, bool BIAS, bool DMA>
 __global__ __launch_bounds__(kCtxThreads, HD <= 64 && !BIAS ? 3 : 2) void ctx_bwd_row(CtxParams p) {
     extern __shared__ __align__(16) unsigned char smem[];
@@ -224,7 +226,9 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 && !BIAS ? 3 : 2) void ctx_bw
     }
 }
 
-// Column-owned: four waves of 32 keys share tiles of 64 query rows, over all heads that read the key head.
+// Column-owned: four waves of 32 keys share tiles of 64 query rows, over all heads that read the key head.  Bound as the row-owned
+// launch, at D = 128 with one wave to a SIMD (dK, dV, K and V of a wave are 256 registers): the cases above 662 us (four
+// contractions at 0.83 PFLOP/s) and 326 us.  (Half tiles in a rolled loop: 1 % and 4 % slower.)
 template <typename T, int HD, bool BIAS, bool DMA>
 __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_col(CtxParams p) {
     extern __shared__ __align__(16) unsigned char smem[];
@@ -353,7 +357,9 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_col(Ctx
 // 64): five contractions, and each input is read once.  Column-owned as above; a tile's dS goes to LDS as well, where the dQ of the
 // tile's rows is contracted over all keys, by a quarter of 32 rows x 32 columns for each of four waves.  With eight waves the two
 // halves of the workgroup take turns, and the other half is ahead with the next tile's scores meanwhile.
-// B=128 H=12 L=256 D=64 with bias: 132 us row-owned + 125 column-owned.
+// B=128 H=12 L=256 D=64 with bias 226 us against 132 row-owned + 125 column-owned, B=64 H=12 L=128 48 against 32.5 + 27.5.  Bound by
+// the latency of a tile's chain (scores, dS to LDS, barrier, dQ): one workgroup of eight waves to a compute unit, vector instructions
+// issued 35 % of the time, the matrix unit busy 12 %.
 template <typename T, bool BIAS, bool DMA, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, 2) void ctx_bwd_one(CtxParams p) {
     extern __shared__ __align__(16) unsigned char smem[];

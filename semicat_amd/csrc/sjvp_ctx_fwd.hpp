@@ -73,7 +73,11 @@ __device__ __forceinline__ float ctx_lse(float ref, float l) { return (ref + fas
 // 1.6e-6 with three), for 2 % of a training pass at L=256 D=64 and 8 % at a causal 4096.
 //
 // Many rows: four waves of 32 rows of one head share tiles of 64 keys.  Two tiles of K and V in LDS: the next one is on its way
-// while this one is used, one barrier to a tile.
+// while this one is used, one barrier to a tile.  Bound by the issue of vector instructions and by power: of
+// B=8 H=16 Lq=4096 Lk=1024 (half of the keys there) D=64, 138 us, vector instructions are issued 81 % of the time and the matrix unit is
+// busy 47 %, at 1.7 GHz.  So the loops hold neither masks nor bounds, the running maximum is raised seldom, and up to D = 64 four
+// waves share a SIMD (128 registers), whose instructions fill each other's gaps: two waves with the scores of the next tile ahead took 150 us.
+// At D = 128 two (B=8 Hq=16 Hkv=4 Lq=2048 Lk=1024 with rests: 184 us, the matrix unit busy 47 %).
 template <typename T, int HD, bool BIAS, bool DMA, int TERMS>
 __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 4 : 2) void ctx_fwd(CtxParams p) {
     extern __shared__ __align__(16) unsigned char smem[];
@@ -170,7 +174,8 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 4 : 2) void ctx_fwd(CtxPara
 // Few rows: the query rows of all heads that share a key head stand in one block of 32 (row = head of the group * Lq + query), and
 // waves share out the keys: each runs over tiles of 32 keys of its own, K straight from memory into the operand's registers, V through a
 // region of LDS that no other wave reads, so that nothing but the end is synchronised.  The sums of the waves are
-// joined in LDS; with several splits of the key axis they go to memory for ctx_join.
+// joined in LDS; with several splits of the key axis they go to memory for ctx_join.  Bound by memory for many keys: 64 sequences of 1024 to
+// 2048 keys, Hq=16 Hkv=4 D=128, 37 us of kernel at 5.4 TB/s; by latency otherwise (one query on 128 keys: 4.7 us).
 // `packed` heads of a group stand in one block's rows: all of them, or one where their bias rows would not fit or a head
 // fills a block by itself.
 template <typename T, int HD, bool BIAS, int TERMS, int WAVES>
@@ -223,7 +228,7 @@ __global__ __launch_bounds__(64 * WAVES, HD <= 64 ? 4 : 2) void ctx_fwd_few(CtxP
     const float* row = bias_rows;
     if constexpr (BIAS) {
         const int entries = ctx_row_entries(p), heads = (r0 + rows - 1) / p.Lq - g0 + 1;
-        for (int x = 0; x < heads; ++x) fill_bias_row(p, bias_rows + x * entries, hq0 + g0 + x, tid, 64 * WAVES);
+        fill_bias_row(p, bias_rows, hq0 + g0, tid, 64 * WAVES, heads);
         row = bias_rows + (g - g0) * entries;
         workgroup_barrier();
     }

@@ -17,8 +17,9 @@ int ctx_forward<SJVP_T>(CtxParams p, const CtxPlan& plan, hipStream_t stream) {
             constexpr bool BIAS = decltype(bias)::value;
             constexpr int TERMS = decltype(terms)::value;
             if (!plan.few) return launch(ctx_fwd<SJVP_T, HD, BIAS, decltype(dma)::value, TERMS>, grid, plan.smem, stream, p, kCtxThreads);
-            return plan.waves == 8 ? launch(ctx_fwd_few<SJVP_T, HD, BIAS, TERMS, 8>, grid, plan.smem, stream, p, 512)
-                                   : launch(ctx_fwd_few<SJVP_T, HD, BIAS, TERMS, 4>, grid, plan.smem, stream, p, 256);
+            if constexpr (BIAS)
+                if (plan.waves == 8) return launch(ctx_fwd_few<SJVP_T, HD, BIAS, TERMS, 8>, grid, plan.smem, stream, p, 512);
+            return launch(ctx_fwd_few<SJVP_T, HD, BIAS, TERMS, 4>, grid, plan.smem, stream, p, 256);
         };
         const std::true_type yes;
         const std::false_type no;
