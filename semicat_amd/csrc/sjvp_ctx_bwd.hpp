@@ -62,27 +62,34 @@ __device__ __forceinline__ float diagonals(const f32x16& x) {
     return sum;
 }
 
-// From a workgroup's sums by difference (`count` waves, one after another) to its sums by bucket: 16 lanes to a bucket.
-__device__ __forceinline__ void write_buckets(const CtxParams& p, const float* hists, int count, float* out, bool any, int tid, int threads) {
+// From a workgroup's sums by difference (`count` waves, one after another) to its sums by bucket: first over the waves, then by 16 lanes to
+// a bucket.
+__device__ __forceinline__ void write_buckets(const CtxParams& p, float* hists, int count, float* out, bool any, int tid, int threads) {
     const int nb = ctx_all_buckets(p), zero = p.far + kCtxPad, entries = ctx_row_entries(p);
+    for (int x = tid; x < entries; x += threads) {
+        float sum = hists[x];
+        for (int k = 1; k < count; ++k) sum += hists[k * entries + x];
+        hists[x] = sum;
+    }
+    workgroup_barrier();
     for (int bucket = tid / 16; bucket < (nb + 15) / 16 * 16; bucket += threads / 16) {
         const int side = bucket >= p.buckets, j = min(bucket - side * p.buckets, p.buckets - 1);
         const int from = p.first[j], to = j + 1 < p.buckets ? p.first[j + 1] - 1 : zero;  // distances
         const int lo = side ? zero + max(from, 1) : zero - to;
         const int hi = side ? zero + to : !p.both && j == 0 ? entries - 1 : zero - from;  // (above zero: distance 0)
         float sum = 0.0f;
-        for (int x = lo + (tid & 15); x <= hi; x += 16)
-            for (int k = 0; k < count; ++k) sum += hists[k * entries + x];
+        for (int x = lo + (tid & 15); x <= hi; x += 16) sum += hists[x];
         sum = sum16(sum);
         if ((tid & 15) == 0 && bucket < nb) out[bucket] = any ? sum : 0.0f;
     }
 }
 
 // Row-owned: four waves of 32 query rows of one head share tiles of 64 keys.  Bound by the matrix unit and the vector instructions
-// together with the latency of a tile, two waves to a SIMD: B=8 H=16 L=4096 D=64 causal with bias 528 us (the matrix unit busy 36 %, vector instructions issued 56 %; three
-// contractions at 0.78 PFLOP/s), B=8 Hq=16 Hkv=4 Lq=2048 Lk=1024 D=128 224 us.
+// together with the latency of a tile, two waves to a SIMD: B=8 H=16 L=4096 D=64 causal with bias 528 us (three contractions at 0.78
+// PFLOP/s, the matrix unit busy 36 %, vector instructions issued 56 %), B=8 Hq=16 Hkv=4 Lq=2048 Lk=1024 D=128 224 us.
 template <typename T, int HD, bool BIAS, bool DMA>
 __global__ __launch_bounds__(kCtxThreads, HD <= 64 && !BIAS ? 3 : 2) void ctx_bwd_row(CtxParams p) {
+    if constexpr (DMA) __builtin_assume(p.D % 8 == 0);
     extern __shared__ __align__(16) unsigned char smem[];
     constexpr int kTile = Tile<HD, DMA>::kElems;
     elem_t* tiles = reinterpret_cast<elem_t*>(smem);  // [2][K, V]
@@ -231,6 +238,7 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 && !BIAS ? 3 : 2) void ctx_bw
 // contractions at 0.83 PFLOP/s) and 326 us.  (Half tiles in a rolled loop: 1 % and 4 % slower.)
 template <typename T, int HD, bool BIAS, bool DMA>
 __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_col(CtxParams p) {
+    if constexpr (DMA) __builtin_assume(p.D % 8 == 0);
     extern __shared__ __align__(16) unsigned char smem[];
     constexpr int kTile = Tile<HD, DMA>::kElems;
     elem_t* tiles = reinterpret_cast<elem_t*>(smem);                // [2][Q, dO]
@@ -362,6 +370,7 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_col(Ctx
 // issued 35 % of the time, the matrix unit busy 12 %.
 template <typename T, bool BIAS, bool DMA, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, 2) void ctx_bwd_one(CtxParams p) {
+    if constexpr (DMA) __builtin_assume(p.D % 8 == 0);
     extern __shared__ __align__(16) unsigned char smem[];
     constexpr int HD = 64, NT = 64 * WAVES, kTile = Tile<HD, DMA>::kElems, kX = Tile<HD, false>::kElems;
     elem_t* const K = reinterpret_cast<elem_t*>(smem);                   // [WAVES / 2] tiles of all keys
@@ -428,15 +437,19 @@ __global__ __launch_bounds__(64 * WAVES, 2) void ctx_bwd_one(CtxParams p) {
     u32x4 own_k[HD / 16], own_v[HD / 16];
     own_operands<HD>(own_k, p.k.head(b, hk) + (int64_t)key * p.k.sl, ok, h, p.D);
     own_operands<HD>(own_v, p.v.head(b, hk) + (int64_t)key * p.v.sl, ok, h, p.D);
-    if (BIAS && tid < 28) bias_row[entries + tid] = -INFINITY;
+    const auto new_head = [&](int hq) {
+        fill_bias_row(p, bias_row, hq, tid, NT);
+        for (int y = lane; y < entries; y += 64) hist[y] = 0.0f;
+    };
+    if constexpr (BIAS) {
+        new_head(hk * p.G);  // (while the first tile is on its way)
+        if (tid < 28) bias_row[entries + tid] = -INFINITY;
+    }
     deliver(0);
     f32x16 dk[HD / 32] = {}, dv[HD / 32] = {};
     for (int x = 0; x < all; ++x) {
         const int hq = hk * p.G + x / per_head, r0 = x % per_head * kCtxTile, p0 = bt.start + r0;
-        if (BIAS && r0 == 0) {
-            fill_bias_row(p, bias_row, hq, tid, NT);
-            for (int y = lane; y < entries; y += 64) hist[y] = 0.0f;
-        }
+        if (BIAS && r0 == 0 && x) new_head(hq);
         if (x == 0) qf.arrived();
         if (x == 0 || (BIAS && r0 == 0)) workgroup_barrier();
         if (x + 1 < all) request(x + 1);

@@ -76,10 +76,12 @@ __device__ __forceinline__ float ctx_lse(float ref, float l) { return (ref + fas
 // while this one is used, one barrier to a tile.  Bound by the issue of vector instructions and by power: of
 // B=8 H=16 Lq=4096 Lk=1024 (half of the keys there) D=64, 138 us, vector instructions are issued 81 % of the time and the matrix unit is
 // busy 47 %, at 1.7 GHz.  So the loops hold neither masks nor bounds, the running maximum is raised seldom, and up to D = 64 four
-// waves share a SIMD (128 registers), whose instructions fill each other's gaps: two waves with the scores of the next tile ahead took 150 us.
+// waves share a SIMD (128 registers), whose instructions fill each other's gaps (141 us against 145 by two waves with the scores of the
+// next tile ahead, in turn).
 // At D = 128 two (B=8 Hq=16 Hkv=4 Lq=2048 Lk=1024 with rests: 184 us, the matrix unit busy 47 %).
 template <typename T, int HD, bool BIAS, bool DMA, int TERMS>
 __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 4 : 2) void ctx_fwd(CtxParams p) {
+    if constexpr (DMA) __builtin_assume(p.D % 8 == 0);
     extern __shared__ __align__(16) unsigned char smem[];
     constexpr int kTile = Tile<HD, DMA>::kElems;
     elem_t* tiles = reinterpret_cast<elem_t*>(smem);  // K [2], V [2]
