@@ -439,8 +439,7 @@ __device__ __forceinline__ void add_columns_exact(f32x16* acc, const Tile<HD, DM
 }
 
 template <typename T, int HD, bool DMA>
-__device__ __forceinline__ f32x16 scores(const Tile<HD, DMA>& at, const elem_t* tile, int row0, const u32x4* own) {
-    f32x16 s = {};
+__device__ __forceinline__ f32x16 scores(const Tile<HD, DMA>& at, const elem_t* tile, int row0, const u32x4* own, f32x16 s = {}) {
 #pragma unroll
     for (int c = 0; c < HD / 16; ++c) s = Mma32<T>::run(at.rows(tile, row0, c), own[c], s);
     return s;

@@ -40,6 +40,20 @@ __device__ __forceinline__ float row_delta(const CtxParams& p, const u32x4* own_
     return halves_sum(sum);
 }
 
+// What LDS holds of 32 looped rows, as the registers of a score tile.  -delta is where the contraction for dP starts, an instruction less to an
+// element (B=8 Hq=16 Hkv=4 Lq=2048 Lk=1024 D=128 1.5 % of forward and backward), but not where dS is summed by bucket: the matrix unit cuts
+// off what it adds below its larger addends, and the sums of an fp32 table's gradient would be 4e-6 off in place of 1e-6.
+__device__ __forceinline__ f32x16 of_rows(const float* rows, int h) {
+    f32x16 x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const f32x4 four = *reinterpret_cast<const f32x4*>(rows + 8 * i + 4 * h);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[4 * i + j] = four[j];
+    }
+    return x;
+}
+
 // Sums along the diagonals of a 32 x 32 score tile (one wave's): lane j < 63 receives that of the difference (looped row - column)
 // 31 - j.  The partial sum of a diagonal stands with the lane whose column it has reached and moves one lane up from a looped row to
 // the next; the upper half of the wave, which holds columns of its own only until they are moved below it, takes what leaves the 32
@@ -242,7 +256,7 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_col(Ctx
     extern __shared__ __align__(16) unsigned char smem[];
     constexpr int kTile = Tile<HD, DMA>::kElems;
     elem_t* tiles = reinterpret_cast<elem_t*>(smem);                // [2][Q, dO]
-    float* stats = reinterpret_cast<float*>(tiles + 4 * kTile);     // [2][lse, delta][64]
+    float* stats = reinterpret_cast<float*>(tiles + 4 * kTile);     // [2][lse, -delta][64]
     float* bias_row = stats + 4 * kCtxTile;
     const int nkb = p.blocks, entries = ctx_row_entries(p);
     const CtxWork w = ctx_work(p.B * p.Hkv, nkb * p.splits);
@@ -282,7 +296,7 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_col(Ctx
         gf.deliver(place(x) + kTile, p.D, tid);
         // (a row without keys: its exponentials are zero)
         if (tid < 2 * kCtxTile)
-            stats[((x - x0) & 1) * 2 * kCtxTile + tid] = tid >= kCtxTile ? stat : stat == -INFINITY ? INFINITY : stat * kLog2e;
+            stats[((x - x0) & 1) * 2 * kCtxTile + tid] = tid >= kCtxTile ? -stat : stat == -INFINITY ? INFINITY : stat * kLog2e;
     };
     if (x0 < x1) {
         request(x0);
@@ -300,7 +314,7 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_col(Ctx
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 s[u] = scores<T>(at, Q, 32 * u, own_k);
-                ds[u] = scores<T>(at, Q + kTile, 32 * u, own_v);
+                ds[u] = scores<T>(at, Q + kTile, 32 * u, own_v, of_rows(st + kCtxTile + 32 * u, h));
             }
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
@@ -312,14 +326,13 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_col(Ctx
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const f32x4 lse = *reinterpret_cast<const f32x4*>(st + 32 * u + 8 * i + 4 * h);
-                    const f32x4 delta = *reinterpret_cast<const f32x4*>(st + kCtxTile + 32 * u + 8 * i + 4 * h);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         float y = s[u][4 * i + j];
                         if constexpr (BIAS && decltype(band)::value == kNear) y = fast_exp2(__builtin_fmaf(y, p.c, bias[-(8 * i + j)]) - lse[j]);
                         else y = fast_exp2(__builtin_fmaf(y, p.c, one - lse[j]));
                         s[u][4 * i + j] = y;
-                        ds[u][4 * i + j] = y * (ds[u][4 * i + j] - delta[j]);
+                        ds[u][4 * i + j] *= y;
                     }
                 }
             }
@@ -376,7 +389,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void ctx_bwd_one(CtxParams p) {
     elem_t* const K = reinterpret_cast<elem_t*>(smem);                   // [WAVES / 2] tiles of all keys
     elem_t* const tiles = K + WAVES / 2 * kTile;                         // [2][Q, dO]
     elem_t* const X = tiles + 4 * kTile;                                 // [WAVES / 2] tiles of dS, rows: keys, columns: query rows
-    float* const stats = reinterpret_cast<float*>(X + WAVES / 2 * kX);   // [2][lse, delta][64]
+    float* const stats = reinterpret_cast<float*>(X + WAVES / 2 * kX);   // [2][lse, -delta][64]
     float* const bias_row = stats + 4 * kCtxTile;                        // with 28 entries of -inf behind it
     const int entries = ctx_row_entries(p);
     float* const hists = bias_row + entries + 28;
@@ -426,7 +439,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void ctx_bwd_one(CtxParams p) {
         if (tid % WAVES == 0) {
             float* st = stats + (x & 1) * 2 * kCtxTile + tid / WAVES;
             st[0] = lse_next == -INFINITY ? INFINITY : lse_next * kLog2e;
-            st[kCtxTile] = delta;
+            st[kCtxTile] = -delta;
         }
     };
     for (int t = 0; t < WAVES / 2; ++t) {
@@ -459,7 +472,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void ctx_bwd_one(CtxParams p) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             s[u] = scores<T>(at, Q, 32 * u, own_k);
-            ds[u] = scores<T>(at, Q + kTile, 32 * u, own_v);
+            if constexpr (BIAS) ds[u] = scores<T>(at, Q + kTile, 32 * u, own_v);
+            else ds[u] = scores<T>(at, Q + kTile, 32 * u, own_v, of_rows(st + kCtxTile + 32 * u, h));
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -469,14 +483,15 @@ __global__ __launch_bounds__(64 * WAVES, 2) void ctx_bwd_one(CtxParams p) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const f32x4 lse = *reinterpret_cast<const f32x4*>(st + 32 * u + 8 * i + 4 * h);
-                const f32x4 delta = *reinterpret_cast<const f32x4*>(st + kCtxTile + 32 * u + 8 * i + 4 * h);
+                f32x4 less_delta = {};
+                if constexpr (BIAS) less_delta = *reinterpret_cast<const f32x4*>(st + kCtxTile + 32 * u + 8 * i + 4 * h);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     float y = s[u][4 * i + j];
                     if constexpr (BIAS) y = fast_exp2(__builtin_fmaf(y, p.c, bias[-(8 * i + j)]) - lse[j]);
                     else y = fast_exp2(__builtin_fmaf(y, p.c, one - lse[j]));
                     s[u][4 * i + j] = y;
-                    ds[u][4 * i + j] = y * (ds[u][4 * i + j] - delta[j]);
+                    ds[u][4 * i + j] = y * (BIAS ? ds[u][4 * i + j] + less_delta[j] : ds[u][4 * i + j]);
                 }
             }
             if constexpr (BIAS) {
