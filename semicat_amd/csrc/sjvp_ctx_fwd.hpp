@@ -70,7 +70,7 @@ __device__ __forceinline__ float ctx_lse(float ref, float l) { return (ref + fas
 // a row are differences of near numbers), so P goes into the contraction with what its rounding leaves, and so does o into memory.
 // Two terms leave 2e-6 of o in bf16, for gradients that are rounded to 16 bits in the end.  The gradient of an fp32 table in bf16 takes
 // three: a bucket's sum over all rows is far below its terms' where it all but cancels (B=H=1 L=300 D=128: 5e-6 of it with two terms,
-// 1.6e-6 with three), for 2 % of a training pass at L=256 D=64 and 8 % at a causal 4096.
+// 1.1e-6 with three), for 2 % of a training pass at L=256 D=64 and 8 % at a causal 4096.
 //
 // Many rows: four waves of 32 rows of one head share tiles of 64 keys.  Two tiles of K and V in LDS: the next one is on its way
 // while this one is used, one barrier to a tile.  Bound by the issue of vector instructions and by power: of
