@@ -6,6 +6,8 @@ u a + u |result|.  What float32 contractions of up to 128 products, the exponent
 is bounded by 2^-14 (a + b), b = |sum p k| sum |dO||o| scale and the like: what a relative error of delta = dO.o does, for which P
 and o are held to two roundings, u^2 b.  fp16 numbers below 2^-14 are rounded in steps of 2^-24: 2^-25 c + 2^-25, c = sum |v| and the like.
 The float32 table's gradient rounds nothing to 16 bits either: 2^-15 a."""
+import ctypes
+
 import pytest
 import torch
 
@@ -86,7 +88,8 @@ def test_relative(shape, buckets, distance, both, causal, dtype, table):
 
 
 @pytest.mark.parametrize("relative", [False, True])
-@pytest.mark.parametrize("shape", [(5, 4, 2, 70, 150, 64), (6, 4, 2, 65, 100, 64), (5, 2, 1, 200, 300, 64), (5, 2, 1, 3, 400, 40), (5, 4, 4, 140, 140, 128), (6, 2, 1, 1, 2, 32)])
+@pytest.mark.parametrize("shape", [(5, 4, 2, 70, 150, 64), (6, 4, 2, 65, 100, 64), (5, 2, 1, 200, 300, 64), (5, 2, 1, 3, 400, 40), (5, 4, 4, 140, 140, 128), (6, 2, 1, 1, 2, 32),
+                                   (5, 2, 1, 190, 150, 64), (6, 2, 1, 130, 100, 64), (5, 3, 3, 60, 250, 52), (6, 2, 2, 40, 128, 33)])
 def test_lengths_hide_what_lies_behind_them(shape, relative):
     """Lengths of zero, one and all; NaN and infinities behind them; results there are zeros."""
     B, _, _, Lq, Lk, _ = shape
@@ -121,10 +124,23 @@ def test_positions(start, Lq, Lk, both, causal):
     check(run(x, **options), x, **options)
 
 
-def test_many_units_with_a_bias(shape=(33, 8, 2, 150, 220, 64)):
-    """The single backward launch over several tiles and heads, each with its buckets."""
+def in_one_launch(B, H, G, Lq, Lk, D):
+    """Whether the backward of such a call is a single launch, which alone needs no workspace (without a table)."""
+    from semicat_amd import _lib
+    t = _lib.Ctx()
+    t.B, t.Hq, t.Hkv, t.Lq, t.Lk, t.D, t.dk = B, H, H // G, Lq, Lk, D, 64  # (no pointer is read)
+    return _lib.load().sjvp_ctx_workspace_bytes(ctypes.byref(t), 1) == 0
+
+
+# the single backward launch over several tiles and heads, by eight waves and by four; the pair
+@pytest.mark.parametrize("shape,one", [((40, 8, 2, 150, 220, 64), True), ((65, 4, 2, 150, 100, 64), True), ((33, 8, 2, 150, 220, 64), False),
+                                       ((2, 9, 3, 60, 256, 40), True), ((3, 2, 2, 33, 128, 50), True), ((80, 2, 1, 200, 140, 36), True)])
+def test_many_units_with_a_bias(shape, one):
     x = make(*shape, BF16, table=(32, torch.float32))
-    options = dict(max_distance=60, key_lengths=torch.randint(0, 221, (33,), generator=torch.Generator().manual_seed(0)).int())
+    B, Lk = shape[0], shape[4]
+    options = dict(max_distance=60, key_lengths=torch.randint(0, Lk + 1, (B,), generator=torch.Generator().manual_seed(0)).int())
+    if torch.cuda.get_device_properties(0).multi_processor_count == 256:  # (the rule asks for their number)
+        assert in_one_launch(*shape) == one
     check(run(x, **options), x, **options)
 
 
@@ -314,7 +330,7 @@ def test_streams_and_graphs():
 
 
 # one launch, a pair of launches, a pair with split axes; few rows in splits
-@pytest.mark.parametrize("B,H,G,Lq,Lk,D,table", [(2, 4, 2, 70, 90, 64, None), (3, 4, 2, 70, 300, 32, (16, torch.float32)),
+@pytest.mark.parametrize("B,H,G,Lq,Lk,D,table", [(2, 4, 1, 70, 90, 64, None), (3, 4, 2, 70, 300, 32, (16, torch.float32)),
                                                  (1, 2, 2, 130, 1500, 96, (8, BF16)), (2, 4, 4, 3, 3000, 128, None)])
 def test_training_passes_in_a_graph(B, H, G, Lq, Lk, D, table):
     """Forward and backward through the autograd surface, captured and replayed on other inputs among eager passes."""
