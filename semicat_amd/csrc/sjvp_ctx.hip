@@ -118,9 +118,11 @@ bool ctx_plan_one(const CtxParams& p, CtxPlan& plan) {
     plan.units = (int64_t)p.B * p.Hkv;
     plan.dma = ctx_dma(p, p.q, p.g) && ctx_aligned(p.k);
     const int tile = kCtxTile * (64 + (plan.dma ? 0 : 8)) * 2;
-    plan.smem = (plan.waves / 2 + 4) * tile + plan.waves / 2 * kCtxTile * 72 * 2 + 4 * kCtxTile * 4 +
-                (p.table ? 4 * (ctx_entries(p) * (1 + plan.waves) + 28) : 0);
+    const int ds = plan.waves / 2 * kCtxTile * 72 * 2;
+    plan.smem = (plan.waves / 2 + 4) * tile + ds + 4 * kCtxTile * 4 + (p.table ? 4 * (ctx_entries(p) * (1 + plan.waves) + 28) : 0);
     if (plan.smem > kLds) return false;
+    plan.packed = plan.waves == 8 && plan.smem + ds <= kLds ? 2 : 1;
+    plan.smem += (plan.packed - 1) * ds;
     const int64_t units = plan.units, cu = compute_units(), rounds = ceil_div(units, cu);
     if (rounds == 1 && p.G * ceil_div(p.Lq, kCtxTile) <= 3) return true;
     if (plan.waves == 4) return 2 * units >= cu;

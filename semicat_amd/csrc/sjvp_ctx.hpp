@@ -64,7 +64,7 @@ struct CtxParams {
     float scale, c;                          // c = scale * log2(e)
     int buckets, both, causal, far;          // buckets of a direction; far: the first distance of the last one
     int splits, blocks;                      // splits of the looped axis; workgroups of a split over the owned axis
-    int packed;                              // ctx_fwd_few: heads to a block of rows
+    int packed;                              // ctx_fwd_few: heads to a block of rows; ctx_bwd_one: sets of dS tiles
     int cols;                                // ctx_sum: dK and dV, not dQ
     alignas(4) uint16_t first[kCtxBuckets];  // first distance of each bucket
 };

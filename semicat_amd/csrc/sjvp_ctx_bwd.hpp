@@ -377,7 +377,8 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_col(Ctx
 // One launch for both, where a workgroup's waves own all keys of a sequence between them (up to 32 * WAVES; head dimensions 33 to
 // 64): five contractions, and each input is read once.  Column-owned as above; a tile's dS goes to LDS as well, where the dQ of the
 // tile's rows is contracted over all keys, by a quarter of 32 rows x 32 columns for each of four waves.  With eight waves the two
-// halves of the workgroup take turns, and the other half is ahead with the next tile's scores meanwhile.
+// halves of the workgroup take turns, and the other half is ahead with the next tile's scores meanwhile; where two tiles' dS fit LDS, they
+// alternate, which leaves one barrier to a tile (B=64 H=12 1024 x 256 with bias 305 us, with one 314).
 // B=128 H=12 L=256 D=64 with bias 226 us against 132 row-owned + 125 column-owned, B=64 H=12 L=128 48 against 32.5 + 27.5.  Bound by
 // the latency of a tile's chain (scores, dS to LDS, barrier, dQ): one workgroup of eight waves to a compute unit, vector instructions
 // issued 35 % of the time, the matrix unit busy 12 %.
@@ -388,8 +389,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void ctx_bwd_one(CtxParams p) {
     constexpr int HD = 64, NT = 64 * WAVES, kTile = Tile<HD, DMA>::kElems, kX = Tile<HD, false>::kElems;
     elem_t* const K = reinterpret_cast<elem_t*>(smem);                   // [WAVES / 2] tiles of all keys
     elem_t* const tiles = K + WAVES / 2 * kTile;                         // [2][Q, dO]
-    elem_t* const X = tiles + 4 * kTile;                                 // [WAVES / 2] tiles of dS, rows: keys, columns: query rows
-    float* const stats = reinterpret_cast<float*>(X + WAVES / 2 * kX);   // [2][lse, -delta][64]
+    elem_t* const X = tiles + 4 * kTile;                                 // [sets][WAVES / 2] tiles of dS, rows: keys, columns: query rows
+    const int sets = WAVES == 8 ? p.packed : 1;
+    float* const stats = reinterpret_cast<float*>(X + sets * (WAVES / 2) * kX);  // [2][lse, -delta][64]
     float* const bias_row = stats + 4 * kCtxTile;                        // with 28 entries of -inf behind it
     const int entries = ctx_row_entries(p);
     float* const hists = bias_row + entries + 28;
@@ -500,12 +502,13 @@ __global__ __launch_bounds__(64 * WAVES, 2) void ctx_bwd_one(CtxParams p) {
                 wave_exchange();
             }
         }
-        workgroup_barrier();  // the last tile's dS has been read
+        if (sets == 1) workgroup_barrier();  // the last tile's dS has been read
+        elem_t* const XT = X + (x & (sets - 1)) * (WAVES / 2) * kX;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                *reinterpret_cast<u32x2*>(X + key * (HD + 8) + 32 * u + 8 * i + 4 * h) =
+                *reinterpret_cast<u32x2*>(XT + key * (HD + 8) + 32 * u + 8 * i + 4 * h) =
                     u32x2{T::pack2(ds[u][4 * i], ds[u][4 * i + 1]), T::pack2(ds[u][4 * i + 2], ds[u][4 * i + 3])};
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -521,7 +524,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void ctx_bwd_one(CtxParams p) {
             const int steps = (bt.keys + 15) / 16;
 #pragma unroll 4
             for (int m = 0; m < steps; ++m)
-                dq = Mma32<T>::run(at.columns(K + (m >> 2) * kTile, 16 * (m & 3), dt), x_at.columns(X + (m >> 2) * kX, 16 * (m & 3), uq), dq);
+                dq = Mma32<T>::run(at.columns(K + (m >> 2) * kTile, 16 * (m & 3), dt), x_at.columns(XT + (m >> 2) * kX, 16 * (m & 3), uq), dq);
             // a row that sees one key has no gradient of its score: exactly none, not what rounding leaves
             const float f = bt.seen(p, i) == 1 ? 0.0f : p.scale;
             if (i < p.Lq) {

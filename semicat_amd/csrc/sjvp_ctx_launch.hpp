@@ -22,7 +22,7 @@ inline bool ctx_dma(const CtxParams& p, const CtxView& a, const CtxView& b) {
 // One launch's share of the work: `blocks` over the owned axis, `splits` of the looped one.
 struct CtxPlan {
     bool few = false;      // forward: ctx_fwd_few
-    int packed = 1;        // its heads to a block of rows,
+    int packed = 1;        // its heads to a block of rows (ctx_bwd_one: sets of dS tiles),
     int waves = kCtxWaves;  // and waves to a workgroup
     int blocks = 1, splits = 1;
     int64_t units = 1, inner = 1;  // of ctx_work

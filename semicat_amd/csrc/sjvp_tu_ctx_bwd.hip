@@ -26,7 +26,7 @@ int ctx_backward<SJVP_T>(CtxParams p, const CtxPlan& plan, bool row, hipStream_t
 
 template <>
 int ctx_backward_one<SJVP_T>(CtxParams p, const CtxPlan& plan, hipStream_t stream) {
-    p.blocks = p.splits = 1;
+    p.blocks = p.splits = 1, p.packed = plan.packed;
     const int grid = (int)ctx_grid(plan.units, 1);
     const auto run = [&](auto bias, auto dma) {
         constexpr bool BIAS = decltype(bias)::value, DMA = decltype(dma)::value;
