@@ -31,8 +31,9 @@ def bucket_map(Lq, Lk, start, buckets, max_distance, bidirectional):
 
 
 def attention(q, k, v, dO=None, table=None, max_distance=128, bidirectional=True, causal=False, key_lengths=None,
-              query_lengths=None, start=0, scale=None):
-    """``[B,S,H,D]`` tensors.  Returns ``(values, sizes)``, dicts of o, lse and, with dO, dq, dk, dv, dtable.  ``sizes[name]`` holds
+              query_lengths=None, start=0, scale=None, scores_in=None):
+    """``[B,S,H,D]`` tensors.  ``scores_in``: a type that the scores with their bias are rounded to (their gradient passes as it is), which
+    a bias of 1e8 or more hides the scores in.  Returns ``(values, sizes)``, dicts of o, lse and, with dO, dq, dk, dv, dtable.  ``sizes[name]`` holds
     (a, b, c): a is the magnitude that a relative rounding of the 16-bit operands of the last contraction meets (sum of
     |p||v| and the like), b what a relative error of delta = dO.o meets, c what an absolute error of those operands meets."""
     B, Lq, H, D = q.shape
@@ -60,6 +61,8 @@ def attention(q, k, v, dO=None, table=None, max_distance=128, bidirectional=True
             s = Q @ K.T * scale
             if tab is not None:
                 s = s + tab[:, h][at]
+            if scores_in is not None:
+                s = (s - s.detach()) + s.detach().to(scores_in).double()
             hidden = ~seen | (s == -math.inf)
             some = (~hidden).any(1)
             s = s.masked_fill(hidden, -math.inf)[some]

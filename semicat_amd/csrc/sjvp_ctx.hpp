@@ -402,6 +402,14 @@ __device__ __forceinline__ int row_entry(const CtxParams& p, int rel, int count)
     return min(max(rel + p.far + kCtxPad, 0), ctx_row_entries(p) - count);
 }
 
+// Whether a bias (in units of log2) is such that rounding score plus bias shows in the probabilities: 2^-14 from 2^10 on, and nothing is left of
+// the scores in the end (lowest numbers as masks).  Tiles of one bias subtract the maximum from the bias and round only then, so those with
+// such a bias go through the loop near the diagonal, which reads the ends of the bias row: every launch forms the same scores.
+__device__ __forceinline__ bool ctx_rounds(float bias) {
+    const float x = fabsf(__uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(bias))));
+    return x >= 1024.0f && x < INFINITY;
+}
+
 // OUT^T += A^T B for the two halves of a packed score tile whose looped rows start at row0 of the tile.
 template <typename T, int HD, bool DMA>
 __device__ __forceinline__ void add_columns(f32x16* acc, const Tile<HD, DMA>& at, const elem_t* tile, int row0, const f32x16& s) {

@@ -215,12 +215,13 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 && !BIAS ? 3 : 2) void ctx_bw
         kf.arrived();
         workgroup_barrier();
     };
-    // the tiles near the diagonal: of the workgroup, whose positions are first .. first + 127
+    // the tiles near the diagonal of the workgroup, whose positions are first .. first + 127
     const int first = bt.start + qb * kCtxOwned;
-    const int t_near = tiles_before(first - p.far + 1, nt), t_above = tiles_before(first + kCtxOwned - 1 + p.far + kCtxTile - 1, nt);
     const int whole = t1 * kCtxTile > bt.keys ? t1 - 1 : t1;
     int t = t0;
     if constexpr (BIAS) {
+        const int t_near = ctx_rounds(row[0]) ? 0 : tiles_before(first - p.far + 1, nt);
+        const int t_above = ctx_rounds(row[entries - 1]) ? nt : tiles_before(first + kCtxOwned - 1 + p.far + kCtxTile - 1, nt);
         for (; t < min(t_near, whole); ++t) tile(t, false, InBand<kBelow>{});
         for (; t < min(t_above, whole); ++t) tile(t, false, InBand<kNear>{});
         for (; t < whole; ++t) tile(t, false, InBand<kAbove>{});
@@ -356,8 +357,9 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_col(Ctx
             // (every wave is behind the barrier of the last tile)
             fill_bias_row(p, bias_row, hk * p.G + g, tid, kCtxThreads);
             workgroup_barrier();
-            for (; x < min(first + n_above, end); ++x) tile(x, InBand<kAbove>{});
-            for (; x < min(first + n_near, end); ++x) tile(x, InBand<kNear>{});
+            const int above = ctx_rounds(bias_row[entries - 1]) ? 0 : n_above, near = ctx_rounds(bias_row[0]) ? per_head : n_near;
+            for (; x < min(first + above, end); ++x) tile(x, InBand<kAbove>{});
+            for (; x < min(first + near, end); ++x) tile(x, InBand<kNear>{});
         }
         for (; x < end; ++x) tile(x, InBand<kBelow>{});
     }

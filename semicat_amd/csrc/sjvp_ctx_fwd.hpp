@@ -153,7 +153,8 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 4 : 2) void ctx_fwd(CtxPara
     };
     if constexpr (BIAS) {
         const int first = bt.start + qb * kCtxOwned;
-        const int near = tiles_before(first - p.far + 1, nt - 1), above = tiles_before(first + kCtxOwned - 1 + p.far + kCtxTile - 1, nt - 1);
+        const int near = ctx_rounds(row[0]) ? 0 : tiles_before(first - p.far + 1, nt - 1);
+        const int above = ctx_rounds(row[2 * (p.far + kCtxPad)]) ? nt - 1 : tiles_before(first + kCtxOwned - 1 + p.far + kCtxTile - 1, nt - 1);
         int t = 0;
         for (; t < near; ++t) tile(t, false, true, InBand<kBelow>{});
         for (; t < above; ++t) tile(t, false, true, InBand<kNear>{});
