@@ -285,7 +285,7 @@ int sjvp_cast(int n, const void* const* x, void* const* y, const int64_t* count,
  *   key_lengths, query_lengths, query_start   device arrays [B], or NULL: every sequence is as long as its tensor, and its
  *       query 0 has position query_start0 (which is added to query_start[b] otherwise).  Lengths are clamped to the tensor.  What
  *       lies in rows behind a length is not used, not even NaN; results there are zeros.  query_start and query_start0 lie within +-2^29.
- *   a row that sees no key (also: whose every key has the bias -inf) has o = 0, lse = -inf and no gradient, for any finite dO.
+ *   a row that sees no key (also: whose every key has the bias -inf) has o = 0, lse = (0, 0) and no gradient, for any finite dO.
  *   table (or NULL: no bias, causal must be 0)   fp32, bf16 or fp16 [buckets of all directions][Hq] with strides table_stride
  *       (bucket, head); entries below -2.3e38 count as that, -inf excludes its keys.  bucket_first: HOST array of `buckets` first
  *       distances in ascending order from 0, the last one at most SJVP_CTX_MAX_DISTANCE; a distance has the last bucket that does
@@ -295,7 +295,8 @@ int sjvp_cast(int n, const void* const* x, void* const* y, const int64_t* count,
  *       given it forms o with probabilities of 16 bits or more (22 or 24 where the table is fp32) and stores it; the backward needs it
  *       for rowsum(dO * o), of which dS is a small difference where attention is sharp, and which the gradient of an fp32 table
  *       (formed to some 1e-6 with it) is a sum over.
- *   lse   [B,Hq,Lq] fp32 contiguous; the forward takes NULL where no backward follows.
+ *   lse   [B,Hq,Lq][2] fp32 contiguous: m, l of each row with lse_i = m ln 2 + ln l, two numbers, since one would lose l beside large
+ *       scores or biases; the forward takes NULL where no backward follows.
  *   dO   fp16: dS = P (dP - delta) is rounded to fp16 on its way into dQ and dK, so that losses are scaled as usual with this type.
  *   dk, dv   both or neither (then without the launch that makes them)
  *   dtable (or NULL)   in the type of table, with strides dtable_stride; summed in fp32 in a fixed order.

@@ -164,8 +164,9 @@ def context_forward(q: Tensor, k: Tensor, v: Tensor, bias: Optional[RelativeBias
                     query_lengths: Optional[Tensor] = None, query_start: Union[int, Tensor] = 0, scale: Optional[float] = None,
                     o: Optional[Tensor] = None, o_rest: Optional[Tensor] = None, with_lse: bool = True
                     ) -> Tuple[Tensor, Optional[Tensor]]:
-    """Forward on ``[B,H,L,D]`` views: ``(o, lse)``, with ``lse`` fp32 ``[B,Hq,Lq]``, or None without ``with_lse``.  ``o`` may be
-    passed in to be filled, and ``o_rest``, a tensor like it, to receive what the rounding of ``o`` leaves (16 bits
+    """Forward on ``[B,H,L,D]`` views: ``(o, lse)``, with ``lse`` fp32 ``[B,Hq,Lq,2]``, or None without ``with_lse``: two numbers ``m``,
+    ``l`` to a row, of which the logarithm of the sum of its scores' exponentials is ``m ln 2 + ln l`` (in one number, ``l`` would be lost
+    beside large scores or biases), ``(0, 0)`` for a row that sees no key.  ``o`` may be passed in to be filled, and ``o_rest``, a tensor like it, to receive what the rounding of ``o`` leaves (16 bits
     in a form of their own), for :func:`context_backward`."""
     _check_inputs(q, k, v, bias, key_lengths, query_lengths, query_start)
     B, H, Lq, D = q.shape
@@ -174,11 +175,11 @@ def context_forward(q: Tensor, k: Tensor, v: Tensor, bias: Optional[RelativeBias
     _check("o", o, q.shape, q)
     if o_rest is not None:
         _check("o_rest", o_rest, q.shape, q)
-    lse = torch.empty((B, H, Lq), device=q.device, dtype=torch.float32) if with_lse else None
+    lse = torch.empty((B, H, Lq, 2), device=q.device, dtype=torch.float32) if with_lse else None
     if q.numel() == 0 or k.numel() == 0:  # no row, or no key for any row
         if o_rest is not None:
             o_rest.zero_()
-        return o.zero_(), None if lse is None else lse.fill_(-float("inf"))
+        return o.zero_(), None if lse is None else lse.zero_()
     _call(False, (q, k, v, o, o_rest, None, None, None, None), lse, bias, key_lengths, query_lengths, query_start, scale)
     return o, lse
 
@@ -197,8 +198,8 @@ def context_backward(q: Tensor, k: Tensor, v: Tensor, o: Tensor, lse: Tensor, dO
         dO = dO.contiguous()
     for name, t in (("o", o), ("dO", dO)) + ((("o_rest", o_rest),) if o_rest is not None else ()):
         _check(name, t, q.shape, q)
-    if tuple(lse.shape) != (B, H, Lq) or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != q.device:
-        raise AssertionError(f"lse must be a contiguous float32 tensor of shape {(B, H, Lq)}, got {tuple(lse.shape)} {lse.dtype}")
+    if tuple(lse.shape) != (B, H, Lq, 2) or lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != q.device:
+        raise AssertionError(f"lse must be a contiguous float32 tensor of shape {(B, H, Lq, 2)}, got {tuple(lse.shape)} {lse.dtype}")
     like = lambda t: torch.empty((t.shape[0], t.shape[2], t.shape[1], D), device=t.device, dtype=t.dtype).transpose(1, 2)
     dq, dk, dv = like(q), *((like(k), like(v)) if with_keys else (None, None))
     dtable = torch.empty(bias.table.shape, device=q.device, dtype=bias.table.dtype) if bias is not None and with_table else None

@@ -100,7 +100,7 @@ CtxPlan ctx_plan_col(const CtxParams& p) {
     plan.splits = splits_for(plan.units * plan.blocks, p.G * ceil_div(p.Lq, kCtxTile), 5);
     plan.inner = (int64_t)plan.blocks * plan.splits;
     plan.dma = ctx_dma(p, p.q, p.g);
-    plan.smem = ctx_tiles_bytes(ctx_padded(p.D), plan.dma) + 4 * kCtxTile * 4 + (p.table ? 4 * ctx_entries(p) : 0);
+    plan.smem = ctx_tiles_bytes(ctx_padded(p.D), plan.dma) + 4 * kCtxStats + (p.table ? 4 * ctx_entries(p) : 0);
     return plan;
 }
 
@@ -119,7 +119,7 @@ bool ctx_plan_one(const CtxParams& p, CtxPlan& plan) {
     plan.dma = ctx_dma(p, p.q, p.g) && ctx_aligned(p.k);
     const int tile = kCtxTile * (64 + (plan.dma ? 0 : 8)) * 2;
     const int ds = plan.waves / 2 * kCtxTile * 72 * 2;
-    plan.smem = (plan.waves / 2 + 4) * tile + ds + 4 * kCtxTile * 4 + (p.table ? 4 * (ctx_entries(p) * (1 + plan.waves) + 28) : 0);
+    plan.smem = (plan.waves / 2 + 4) * tile + ds + 4 * kCtxStats + (p.table ? 4 * (ctx_entries(p) * (1 + plan.waves) + 28) : 0);
     if (plan.smem > kLds) return false;
     plan.packed = plan.waves == 8 && plan.smem + ds <= kLds ? 2 : 1;
     plan.smem += (plan.packed - 1) * ds;
@@ -169,7 +169,7 @@ int ctx_params(const sjvp_ctx* t, CtxParams& p) {
 struct CtxLayout {
     CtxPlan fwd, row, col, one;
     bool single = false;  // backward by ctx_bwd_one
-    size_t delta = 0, tpart = 0, stat = 0, part = 0, total = 0;
+    size_t folded = 0, tpart = 0, stat = 0, part = 0, total = 0;
 };
 
 CtxLayout ctx_layout(const CtxParams& p, bool backward) {
@@ -195,7 +195,7 @@ CtxLayout ctx_layout(const CtxParams& p, bool backward) {
     }
     l.row = ctx_plan_row(p);
     l.col = ctx_plan_col(p);
-    l.delta = take(q_rows);
+    l.folded = take(3 * q_rows);
     if (p.dtable) l.tpart = take((size_t)p.Hq * p.B * l.row.blocks * l.row.splits * (p.both ? 2 : 1) * p.buckets);
     // (the row-owned launch's sums are used up before the column-owned one writes its own)
     const size_t row = l.row.splits > 1 ? l.row.splits * q_rows * HD : 0, col = l.col.splits > 1 ? 2 * l.col.splits * k_rows * HD : 0;
@@ -252,7 +252,7 @@ int sjvp_ctx_bwd(const sjvp_ctx* t, int dtype, void* stream) {
     if (!ctx_fits(l.row) || !ctx_fits(l.col) || !ctx_fits(l.one) || p.Hq * per > UINT32_MAX / 256) return SJVP_ERR_SHAPE;
     float* ws;
     if (ctx_workspace(t, l, ws) != SJVP_OK) return SJVP_ERR_WORKSPACE;
-    p.delta = ws + l.delta, p.part = ws + l.part, p.tpart = p.dtable ? ws + l.tpart : nullptr;
+    p.folded = ws + l.folded, p.part = ws + l.part, p.tpart = p.dtable ? ws + l.tpart : nullptr;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     const auto run = [&](const CtxPlan& plan, bool row) {
         return dtype == SJVP_BF16 ? ctx_backward<Bf16>(p, plan, row, s) : ctx_backward<Fp16>(p, plan, row, s);

@@ -4,7 +4,7 @@
 //   s[i][j] = scale q_i.k_j + table[bucket(j - (start + i))][head]     for j < key length (and j <= start + i if causal)
 //   lse_i = log sum_j exp s[i][j],  p = exp(s - lse),  o_i = sum_j p[i][j] v_j
 //
-// A query head reads key head  head / (Hq / Hkv).  A row that sees no key has o = 0 and lse = -inf.
+// A query head reads key head  head / (Hq / Hkv).  A row that sees no key has o = 0 and no gradient.
 //
 // Tile algebra (v_mfma_f32_32x32x16_{bf16,f16}): C[y][x] += sum_k A[y][k] B[k][x] with
 //     A: lane l holds row y = l % 32, k = 8*(l/32) + i (i < 8);   B: column x = l % 32, same k;
@@ -29,6 +29,7 @@ constexpr int kCtxThreads = 64 * kCtxWaves;
 constexpr int kCtxOwned = 32 * kCtxWaves;  // owned positions of a workgroup whose waves share their tiles
 constexpr int kCtxTile = 64;               // looped positions per tile
 constexpr int kCtxPad = 64;                // entries of the bias row beyond the last single distance, on each side
+constexpr int kCtxStats = 2 * 3 * kCtxTile; // floats of LDS for what the column-owned launches keep of two tiles' rows
 constexpr int kCtxBuckets = SJVP_CTX_MAX_BUCKETS;
 constexpr int kCtxMost = 1 << 29;          // positions and lengths: sums of three stay within 32 bits
 
@@ -52,7 +53,7 @@ struct CtxView {
 
 struct CtxParams {
     CtxView q, k, v, o, rest, g, dq, dk, dv;  // rest: what the rounding of o left (or null); g: the cotangent of o
-    float *lse, *delta;                      // [B,Hq,Lq]
+    float *lse, *folded;                     // [B,Hq,Lq][2]: (m, l) of each row; [3][B,Hq,Lq]: row_stat_folded, -delta
     float *part, *stat;                      // sums of split work: rows of HD floats; their (maximum, sum) pairs
     float* tpart;                            // bucket sums of each workgroup
     void* dtable;
@@ -309,6 +310,26 @@ struct CtxBatch {
         return p.causal ? max(0, min(keys, start + row + 1)) : keys;
     }
 };
+
+// The statistics of a row: m, which its scores (in units of log2) have subtracted, and l, the sum of their exponentials then.  Two numbers, since
+// m + log2 l in one would lose l beside a large m (1e8: P would be 1 for every key in place of 1/n).  No key: both are zero.
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef f32x2 __attribute__((aligned(4))) f32x2_any;
+__device__ __forceinline__ void store_stat(const CtxParams& p, int64_t place, float m, float l) {
+    if (p.lse) *reinterpret_cast<f32x2_any*>(p.lse + 2 * place) = f32x2{l == 0.0f ? 0.0f : m, l};
+}
+__device__ __forceinline__ f32x2 load_stat(const CtxParams& p, int64_t place) { return *reinterpret_cast<const f32x2_any*>(p.lse + 2 * place); }
+// What a backward subtracts from the row's scores, and what it multiplies the exponentials with; none of them is left in a row without keys.
+__device__ __forceinline__ f32x2 row_stat(f32x2 stat) {
+    return stat[1] == 0.0f ? f32x2{INFINITY, 0.0f} : f32x2{stat[0], 1.0f / stat[1]};
+}
+// The same for launches that walk the rows, where a factor takes reads and registers (in the single backward launch, B=64 H=12 Lq=128 Lk=256
+// forward and backward, 87 us in place of 72): it is 1 where m + log2 l is below 64, and its rounding below 1.4e-6 of P.
+__device__ __forceinline__ f32x2 row_stat_folded(f32x2 stat) {
+    if (stat[1] == 0.0f) return f32x2{INFINITY, 1.0f};
+    const float both = stat[0] + fast_log2(stat[1]);
+    return fabsf(both) < 64.0f ? f32x2{both, 1.0f} : row_stat(stat);
+}
 
 // Workgroups run on XCD blockIdx % 8.  The workgroups of one (batch, key head) unit read the same rows: each XCD takes every
 // eighth unit as a whole and finds them in its L2, and batch entries of different lengths spread over all XCDs.  With few units

@@ -54,6 +54,12 @@ __device__ __forceinline__ f32x16 of_rows(const float* rows, int h) {
     return x;
 }
 
+// P and dS of 32 rows whose factors stand in LDS.
+__device__ __forceinline__ void times_rows(f32x16& s, f32x16& ds, const float* rows, int h) {
+    const f32x16 factors = of_rows(rows, h);
+    s *= factors, ds *= factors;
+}
+
 // Sums along the diagonals of a 32 x 32 score tile (one wave's): lane j < 63 receives that of the difference (looped row - column)
 // 31 - j.  The partial sum of a diagonal stands with the lane whose column it has reached and moves one lane up from a looped row to
 // the next; the upper half of the wave, which holds columns of its own only until they are moved below it, takes what leaves the 32
@@ -139,7 +145,7 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 && !BIAS ? 3 : 2) void ctx_bw
     if (t0 < t1) request(t0);
     const int64_t stat = ((int64_t)b * p.Hq + hq) * p.Lq + qi;
     const bool mine = (lane & 31) < rows;
-    float lse = mine ? p.lse[stat] : -INFINITY;
+    const f32x2 ml = mine ? load_stat(p, stat) : f32x2{0.0f, 0.0f};
     u32x4 own_q[HD / 16], own_g[HD / 16];
     own_operands<HD>(own_q, p.q.head(b, hq) + (int64_t)qi * p.q.sl, mine, h, p.D);
     own_operands<HD>(own_g, p.g.head(b, hq) + (int64_t)qi * p.g.sl, mine, h, p.D);
@@ -147,27 +153,33 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 && !BIAS ? 3 : 2) void ctx_bw
         fill_bias_row(p, row, hq, tid, kCtxThreads);
         for (int x = lane; x < entries; x += 64) hist[x] = 0.0f;
     }
-    const bool ok = lse != -INFINITY;      // a row that sees no key has no gradient, whatever its cotangent,
+    const bool ok = ml[1] != 0.0f;         // a row that sees no key has no gradient, whatever its cotangent,
     const bool scored = ok && limit != 1;  // one that sees one key none of its score: exactly none, not what rounding leaves
-    lse = ok ? lse * kLog2e : INFINITY;
+    const f32x2 less_factor = row_stat(ml);
+    const float less = less_factor[0], factor = less_factor[1];
     if (__builtin_amdgcn_ballot_w64(mine && !ok)) {
 #pragma unroll
         for (int c = 0; c < HD / 16; ++c) own_g[c] = ok ? own_g[c] : u32x4{0u, 0u, 0u, 0u};
     }
     const float delta = row_delta<T, HD>(p, own_g, p.o.head(b, hq) + (int64_t)qi * p.o.sl,
                                          p.rest.ptr ? p.rest.head(b, hq) + (int64_t)qi * p.rest.sl : nullptr, ok, h);
-    if (split == 0 && h == 0 && qi < p.Lq) p.delta[stat] = delta;
+    if (split == 0 && h == 0 && qi < p.Lq) {
+        const int64_t all = (int64_t)p.B * p.Hq * p.Lq;
+        const f32x2 folded = row_stat_folded(ml);
+        p.folded[stat] = folded[0], p.folded[all + stat] = folded[1], p.folded[2 * all + stat] = -delta;
+    }
+    const float less_delta = -delta * factor;  // P (dP - delta) = exponential * (factor dP + less_delta)
     if (t0 < t1) deliver(t0);
     kf.arrived();
     workgroup_barrier();
-    // scores of 32 keys from k0 on to P, zero behind the sequence (masked)
-    const auto row_probabilities = [&](f32x16& s, int k0, auto band, bool masked) {
+    // scores of 32 keys from k0 on to P without its factor, zero behind the sequence (masked)
+    const auto exponentials = [&](f32x16& s, int k0, auto band, bool masked) {
         if constexpr (decltype(band)::value == kNear) {
             const float* bias = row + row_entry(p, k0 + 4 * h - pos, 28);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = fast_exp2(__builtin_fmaf(s[r], p.c, bias[8 * (r >> 2) + (r & 3)]) - lse);
+            for (int r = 0; r < 16; ++r) s[r] = fast_exp2(__builtin_fmaf(s[r], p.c, bias[8 * (r >> 2) + (r & 3)]) - less);
         } else {
-            const float one = BIAS ? row[band == kBelow ? 0 : entries - 1] - lse : -lse;
+            const float one = BIAS ? row[band == kBelow ? 0 : entries - 1] - less : -less;
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = fast_exp2(__builtin_fmaf(s[r], p.c, one));
         }
@@ -193,9 +205,9 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 && !BIAS ? 3 : 2) void ctx_bw
             }
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                row_probabilities(s[u], key + 32 * u, band, masked);
+                exponentials(s[u], key + 32 * u, band, masked);
 #pragma unroll
-                for (int r = 0; r < 16; ++r) ds[u][r] = s[u][r] * (ds[u][r] - delta);
+                for (int r = 0; r < 16; ++r) ds[u][r] = s[u][r] * __builtin_fmaf(ds[u][r], factor, less_delta);
                 if constexpr (BIAS && decltype(band)::value == kNear) {
                     const float sum = diagonals(ds[u]);
                     if (lane < 63) hist[row_entry(p, key + 32 * u - pos0 - 31, 63) + 62 - lane] += sum;
@@ -257,8 +269,8 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_col(Ctx
     extern __shared__ __align__(16) unsigned char smem[];
     constexpr int kTile = Tile<HD, DMA>::kElems;
     elem_t* tiles = reinterpret_cast<elem_t*>(smem);                // [2][Q, dO]
-    float* stats = reinterpret_cast<float*>(tiles + 4 * kTile);     // [2][lse, -delta][64]
-    float* bias_row = stats + 4 * kCtxTile;
+    float* stats = reinterpret_cast<float*>(tiles + 4 * kTile);     // [2][row_stat_folded, -delta][64]
+    float* bias_row = stats + kCtxStats;
     const int nkb = p.blocks, entries = ctx_row_entries(p);
     const CtxWork w = ctx_work(p.B * p.Hkv, nkb * p.splits);
     if (!w.some) return;
@@ -286,18 +298,16 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_col(Ctx
         const int hq = hk * p.G + x / per_head, r0 = (ta + x % per_head) * kCtxTile;
         qf.request(p.q.head(b, hq) + (int64_t)r0 * p.q.sl, p.q.sl, bt.rows - r0, p.D, place(x), wave);
         gf.request(p.g.head(b, hq) + (int64_t)r0 * p.g.sl, p.g.sl, bt.rows - r0, p.D, place(x) + kTile, wave);
-        if (tid < 2 * kCtxTile) {
+        if (tid < 3 * kCtxTile) {
             const int i = r0 + (tid & (kCtxTile - 1));
-            const float* from = (tid < kCtxTile ? p.lse : p.delta) + ((int64_t)b * p.Hq + hq) * p.Lq;
-            stat = i < bt.rows ? from[i] : tid < kCtxTile ? -INFINITY : 0.0f;
+            const float* from = p.folded + ((tid / kCtxTile * (int64_t)p.B + b) * p.Hq + hq) * p.Lq;
+            stat = i < bt.rows ? from[i] : tid < kCtxTile ? INFINITY : tid < 2 * kCtxTile ? 1.0f : 0.0f;
         }
     };
     const auto deliver = [&](int x) {
         qf.deliver(place(x), p.D, tid);
         gf.deliver(place(x) + kTile, p.D, tid);
-        // (a row without keys: its exponentials are zero)
-        if (tid < 2 * kCtxTile)
-            stats[((x - x0) & 1) * 2 * kCtxTile + tid] = tid >= kCtxTile ? -stat : stat == -INFINITY ? INFINITY : stat * kLog2e;
+        if (tid < 3 * kCtxTile) stats[((x - x0) & 1) * (kCtxStats / 2) + tid] = stat;
     };
     if (x0 < x1) {
         request(x0);
@@ -305,17 +315,21 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_col(Ctx
         qf.arrived();
     }
     f32x16 dk[HD / 32] = {}, dv[HD / 32] = {};
+    // The rows' factors (row_stat_folded) in every tile, or by a branch: B=8 Hq=16 Hkv=4 Lq=2048 Lk=1024 D=128 forward and backward 673 / 689 us;
+    // at D = 64 B=8 H=16 L=1024 196 / 192.5, causal L=4096 with bias 1776 / 1754.
+    constexpr bool kFactors = HD > 64;
     const auto tile = [&](int x, auto band) {
         const int p0 = bt.start + (ta + x % per_head) * kCtxTile;  // position of the first row
         if (x + 1 < x1) request(x + 1);
         const elem_t* Q = place(x);
-        const float* st = stats + ((x - x0) & 1) * 2 * kCtxTile;
+        const float* st = stats + ((x - x0) & 1) * (kCtxStats / 2);
         if (k0 < bt.keys) {
+            const bool factors = __builtin_amdgcn_ballot_w64(st[kCtxTile + lane] != 1.0f);
             f32x16 s[2], ds[2];
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 s[u] = scores<T>(at, Q, 32 * u, own_k);
-                ds[u] = scores<T>(at, Q + kTile, 32 * u, own_v, of_rows(st + kCtxTile + 32 * u, h));
+                ds[u] = scores<T>(at, Q + kTile, 32 * u, own_v, of_rows(st + 2 * kCtxTile + 32 * u, h));
             }
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
@@ -326,17 +340,21 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_col(Ctx
                 else if constexpr (BIAS) one = bias_row[band == kBelow ? 0 : entries - 1];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const f32x4 lse = *reinterpret_cast<const f32x4*>(st + 32 * u + 8 * i + 4 * h);
+                    const f32x4 less = *reinterpret_cast<const f32x4*>(st + 32 * u + 8 * i + 4 * h);
+                    f32x4 factor;
+                    if constexpr (kFactors) factor = *reinterpret_cast<const f32x4*>(st + kCtxTile + 32 * u + 8 * i + 4 * h);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         float y = s[u][4 * i + j];
-                        if constexpr (BIAS && decltype(band)::value == kNear) y = fast_exp2(__builtin_fmaf(y, p.c, bias[-(8 * i + j)]) - lse[j]);
-                        else y = fast_exp2(__builtin_fmaf(y, p.c, one - lse[j]));
+                        if constexpr (BIAS && decltype(band)::value == kNear) y = fast_exp2(__builtin_fmaf(y, p.c, bias[-(8 * i + j)]) - less[j]);
+                        else y = fast_exp2(__builtin_fmaf(y, p.c, BIAS ? one - less[j] : -less[j]));
+                        if constexpr (kFactors) y *= factor[j];
                         s[u][4 * i + j] = y;
                         ds[u][4 * i + j] *= y;
                     }
                 }
             }
+            if (!kFactors && factors) times_rows(s[0], ds[0], st + kCtxTile, h), times_rows(s[1], ds[1], st + kCtxTile + 32, h);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 add_columns<T>(dv, at, Q + kTile, 32 * u, s[u]);
@@ -393,8 +411,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void ctx_bwd_one(CtxParams p) {
     elem_t* const tiles = K + WAVES / 2 * kTile;                         // [2][Q, dO]
     elem_t* const X = tiles + 4 * kTile;                                 // [sets][WAVES / 2] tiles of dS, rows: keys, columns: query rows
     const int sets = WAVES == 8 ? p.packed : 1;
-    float* const stats = reinterpret_cast<float*>(X + sets * (WAVES / 2) * kX);  // [2][lse, -delta][64]
-    float* const bias_row = stats + 4 * kCtxTile;                        // with 28 entries of -inf behind it
+    float* const stats = reinterpret_cast<float*>(X + sets * (WAVES / 2) * kX);  // [2][row_stat_folded, -delta][64]
+    float* const bias_row = stats + kCtxStats;                           // with 28 entries of -inf behind it
     const int entries = ctx_row_entries(p);
     float* const hists = bias_row + entries + 28;
     const CtxWork w = ctx_work(p.B * p.Hkv, 1);
@@ -413,7 +431,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void ctx_bwd_one(CtxParams p) {
     // The statistics of a tile's rows: WAVES lanes to a row, each with every WAVES-th piece of dO, o and its rest.
     constexpr int kPieces = HD / 8 / WAVES;
     u32x4 g_piece[kPieces], o_piece[kPieces], r_piece[kPieces];
-    float lse_next = 0.0f;
+    f32x2 stat_next = {};
     const auto place = [&](int x) { return tiles + (x & 1) * 2 * kTile; };
     const auto request = [&](int x) {
         const int hq = hk * p.G + x / per_head, r0 = x % per_head * kCtxTile;
@@ -421,7 +439,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void ctx_bwd_one(CtxParams p) {
         gf.request(p.g.head(b, hq) + (int64_t)r0 * p.g.sl, p.g.sl, bt.rows - r0, p.D, place(x) + kTile, wave);
         const int i = r0 + tid / WAVES;
         const bool mine = i < bt.rows;
-        lse_next = mine ? p.lse[((int64_t)b * p.Hq + hq) * p.Lq + i] : -INFINITY;
+        stat_next = mine ? load_stat(p, ((int64_t)b * p.Hq + hq) * p.Lq + i) : f32x2{0.0f, 0.0f};
 #pragma unroll
         for (int j = 0; j < kPieces; ++j) {
             const int c8 = 8 * (tid % WAVES + WAVES * j);
@@ -441,9 +459,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void ctx_bwd_one(CtxParams p) {
         delta += lanes_turned<0x4E>(delta);  // 2, 3, 0, 1
         if (WAVES == 8) delta += lanes_turned<0x141>(delta);  // 7 .. 0 of eight
         if (tid % WAVES == 0) {
-            float* st = stats + (x & 1) * 2 * kCtxTile + tid / WAVES;
-            st[0] = lse_next == -INFINITY ? INFINITY : lse_next * kLog2e;
-            st[kCtxTile] = -delta;
+            float* st = stats + (x & 1) * (kCtxStats / 2) + tid / WAVES;
+            const f32x2 stat = row_stat_folded(stat_next);
+            st[0] = stat[0], st[kCtxTile] = stat[1];
+            st[2 * kCtxTile] = -delta;
         }
     };
     for (int t = 0; t < WAVES / 2; ++t) {
@@ -471,13 +490,14 @@ __global__ __launch_bounds__(64 * WAVES, 2) void ctx_bwd_one(CtxParams p) {
         if (x == 0 || (BIAS && r0 == 0)) workgroup_barrier();
         if (x + 1 < all) request(x + 1);
         const elem_t* Q = place(x);
-        const float* st = stats + (x & 1) * 2 * kCtxTile;
+        const float* st = stats + (x & 1) * (kCtxStats / 2);
+        const bool factors = __builtin_amdgcn_ballot_w64(st[kCtxTile + lane] != 1.0f);
         f32x16 s[2], ds[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             s[u] = scores<T>(at, Q, 32 * u, own_k);
             if constexpr (BIAS) ds[u] = scores<T>(at, Q + kTile, 32 * u, own_v);
-            else ds[u] = scores<T>(at, Q + kTile, 32 * u, own_v, of_rows(st + kCtxTile + 32 * u, h));
+            else ds[u] = scores<T>(at, Q + kTile, 32 * u, own_v, of_rows(st + 2 * kCtxTile + 32 * u, h));
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -486,18 +506,19 @@ __global__ __launch_bounds__(64 * WAVES, 2) void ctx_bwd_one(CtxParams p) {
             const float one = ok ? 0.0f : -INFINITY;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const f32x4 lse = *reinterpret_cast<const f32x4*>(st + 32 * u + 8 * i + 4 * h);
+                const f32x4 less = *reinterpret_cast<const f32x4*>(st + 32 * u + 8 * i + 4 * h);
                 f32x4 less_delta = {};
-                if constexpr (BIAS) less_delta = *reinterpret_cast<const f32x4*>(st + kCtxTile + 32 * u + 8 * i + 4 * h);
+                if constexpr (BIAS) less_delta = *reinterpret_cast<const f32x4*>(st + 2 * kCtxTile + 32 * u + 8 * i + 4 * h);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     float y = s[u][4 * i + j];
-                    if constexpr (BIAS) y = fast_exp2(__builtin_fmaf(y, p.c, bias[-(8 * i + j)]) - lse[j]);
-                    else y = fast_exp2(__builtin_fmaf(y, p.c, one - lse[j]));
+                    if constexpr (BIAS) y = fast_exp2(__builtin_fmaf(y, p.c, bias[-(8 * i + j)]) - less[j]);
+                    else y = fast_exp2(__builtin_fmaf(y, p.c, one - less[j]));
                     s[u][4 * i + j] = y;
                     ds[u][4 * i + j] = y * (BIAS ? ds[u][4 * i + j] + less_delta[j] : ds[u][4 * i + j]);
                 }
             }
+            if (factors) times_rows(s[u], ds[u], st + kCtxTile + 32 * u, h);
             if constexpr (BIAS) {
                 const float sum = diagonals(ds[u]);  // (looped rows are the queries here)
                 if (lane < 63) hist[row_entry(p, k0 - p0 - 32 * u - 31, 63) + lane] += sum;

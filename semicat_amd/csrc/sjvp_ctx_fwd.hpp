@@ -64,8 +64,6 @@ struct RowSums {
     }
 };
 
-__device__ __forceinline__ float ctx_lse(float ref, float l) { return (ref + fast_log2(l)) * kLn2; }
-
 // TERMS > 1, for a backward to follow: the gradients need delta = dO . o as it would be with unrounded probabilities (their sums over
 // a row are differences of near numbers), so P goes into the contraction with what its rounding leaves, and so does o into memory.
 // Two terms leave 2e-6 of o in bf16, for gradients that are rounded to 16 bits in the end.  The gradient of an fp32 table in bf16 takes
@@ -166,8 +164,7 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 4 : 2) void ctx_fwd(CtxPara
     const int out_rows = min(max(p.Lq - q0, 0), 32);
     const float both = halves_sum(st.l), l = (lane & 31) < rows ? both : 0.0f;
     const float f = l == 0.0f ? 0.0f : 1.0f / l;
-    if (p.lse && h == 0 && (lane & 31) < out_rows)
-        p.lse[((int64_t)b * p.Hq + hq) * p.Lq + q0 + lane] = l == 0.0f ? -INFINITY : ctx_lse(st.ref, l);
+    if (h == 0 && (lane & 31) < out_rows) store_stat(p, ((int64_t)b * p.Hq + hq) * p.Lq + q0 + lane, st.ref, l);
     elem_t* region = tiles + wave * 32 * (HD + 8);
     store_rows<T, HD>(st.acc, f, p.o.head(b, hq) + (int64_t)q0 * p.o.sl, p.o.sl, out_rows, region, lane, p.D);
     if constexpr (TERMS > 1)
@@ -306,7 +303,7 @@ __global__ __launch_bounds__(64 * WAVES, HD <= 64 ? 4 : 2) void ctx_fwd_few(CtxP
             continue;
         }
         const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
-        if (p.lse && c8 == 0) p.lse[place] = sum == 0.0f ? -INFINITY : ctx_lse(ref, sum);
+        if (c8 == 0) store_stat(p, place, ref, sum);
         u32x4 o, rest;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -356,7 +353,7 @@ __global__ __launch_bounds__(kCtxThreads) void ctx_join(CtxParams p) {
         add(other[0], other[1], other + 2);
     }
     const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
-    if (p.lse && c8 == 0) p.lse[place] = sum == 0.0f ? -INFINITY : ctx_lse(top, sum);
+    if (c8 == 0) store_stat(p, place, top == -INFINITY ? 0.0f : top, sum);
     u32x4 o, rest;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {

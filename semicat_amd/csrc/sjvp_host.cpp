@@ -618,7 +618,7 @@ Tensor context_forward(const Tensor& q, const Tensor& k, const Tensor& v, const 
     Tensor o = make_tensor({q.size(0), q.size(1), q.size(2), q.size(3)}, q.scalar_type());
     sjvp_ctx t = context_struct(q, k, v, table, options);
     if (lse) {
-        *lse = make_tensor({q.size(0), q.size(2), q.size(1)}, at::kFloat);
+        *lse = make_tensor({q.size(0), q.size(2), q.size(1), 2}, at::kFloat);
         t.lse = static_cast<float*>(lse->data_ptr());
         *rest = make_tensor(o.sizes(), o.scalar_type());
         t.o_rest = rest->data_ptr();

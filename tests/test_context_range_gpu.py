@@ -38,3 +38,42 @@ def test_a_bias_that_leaves_nothing_of_the_scores_does_so_at_every_distance(shap
     want, sizes = orc.attention(**x, max_distance=60, scores_in=torch.float32)
     x["dO"] = torch.zeros_like(x["q"])
     near(run(x, max_distance=60), want, sizes, x, ("o", "plain"))
+
+
+@pytest.mark.parametrize("value", [-1e9, LOW])
+@pytest.mark.parametrize("dtype,shape", [(BF16, s) for s in FORMS] + [(FP16, FORMS[0]), (FP16, FORMS[3])])
+def test_rows_whose_keys_all_have_one_large_bias(shape, dtype, value):
+    """Beside a bias of 1e9 nothing of the scores is left in float32: all keys of the row have the same weight, in the output
+    and in every gradient."""
+    x = make(*shape, dtype, seed=1, table=(32, torch.float32))
+    x["table"][:] = value
+    want, sizes = orc.attention(**x, max_distance=60, scores_in=torch.float32)
+    near(run(x, max_distance=60), want, sizes, x)
+
+
+@pytest.mark.parametrize("value", [-1e9, LOW])
+@pytest.mark.parametrize("shape", FORMS[:4])
+def test_rows_that_see_hidden_keys_alone_beside_others(shape, value):
+    """Causal rows near the first key see nothing but the distances that the table hides; the others see keys that it does not."""
+    x = make(*shape, BF16, seed=2, table=(24, torch.float32))
+    x["table"][:5] = value
+    options = dict(max_distance=60, bidirectional=False, causal=True, key_lengths=torch.tensor([shape[4] - 7] * shape[0], dtype=torch.int32))
+    want, sizes = orc.attention(**x, scores_in=torch.float32, **options)
+    near(run(x, **options), want, sizes, x)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("shape", FORMS)
+def test_weights_of_large_scores_sum_to_one(shape, dtype):
+    """Keys in groups of three alike, with scores of some millions: a row's weights are thirds.  With a cotangent of ones each row hands
+    a weight of one on to dv, whose sum over the keys is the number of rows: P is rounded once and so is dv, by u each, and fp16
+    numbers below 2^-14 by 2^-25."""
+    B, H, G, Lq, Lk, _ = shape
+    x = make(*shape, dtype, seed=3)
+    x["q"], x["k"] = x["q"] * 2048, x["k"][:, torch.arange(Lk) // 3] * 2048
+    x["dO"] = torch.ones_like(x["dO"])
+    got = run(x)
+    assert all(t.isfinite().all() for t in got.values())
+    total, rows = got["dv"].cpu().double().sum(1), G * Lq
+    limit = (2 * torch.finfo(dtype).eps / 2 + 2.0 ** -14) * rows + (2.0 ** -25 * Lk * (1 + rows) if dtype == FP16 else 0.0)
+    assert bool(((total - rows).abs() <= limit).all()), float((total - rows).abs().max() / limit)
