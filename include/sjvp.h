@@ -292,7 +292,8 @@ int sjvp_cast(int n, const void* const* x, void* const* y, const int64_t* count,
  *       not begin beyond it.  bidirectional: keys behind a query (j > start + i) have buckets of their own,
  *       buckets .. 2 buckets - 1, by their distance; otherwise they count as distance 0.
  *   o_rest (or NULL)   what the rounding of o left, 16 bits to an element in a form of its own, for the backward.  A forward that is
- *       given it forms o with probabilities of 16 bits or more (22 or 24 where the table is fp32) and stores it; the backward needs it
+ *       given it forms o with probabilities of 16 bits or more (22 or 24 where the table is fp32) and stores what 22 (fp16, down to
+ *       steps of 2^-35) or 24 bits hold of it; the backward needs it
  *       for rowsum(dO * o), of which dS is a small difference where attention is sharp, and which the gradient of an fp32 table
  *       (formed to some 1e-6 with it) is a sum over.
  *   lse   [B,Hq,Lq][2] fp32 contiguous: m, l of each row with lse_i = m ln 2 + ln l, two numbers, since one would lose l beside large

@@ -349,11 +349,13 @@ __device__ __forceinline__ CtxWork ctx_work(int units, int inner) {
     return {unit, slot % inner, unit < units};
 }
 
-// What the rounding of two numbers to w left of them, as it stands in memory beside o.  fp16: the difference, which makes 22 bits in
-// all; bf16, where that would make 17: the difference of the bits as a signed number, which makes all 24.
+// What the rounding of two numbers to w left of them, as it stands in memory beside o.  fp16: the difference, 2^11 times as large (at most as
+// large as the number then), which makes 22 bits in all and, for small numbers, steps of 2^-35; bf16, where the difference would make 17: the
+// difference of the bits as a signed number, which makes all 24.
+constexpr float kRestScale = 2048.0f;
 template <typename T>
 __device__ __forceinline__ uint32_t rest_of(uint32_t w, float lo, float hi) {
-    if constexpr (!std::is_same_v<T, Bf16>) return T::pack2(lo - T::to_float((elem_t)w), hi - T::to_float((elem_t)(w >> 16)));
+    if constexpr (!std::is_same_v<T, Bf16>) return T::pack2((lo - T::to_float((elem_t)w)) * kRestScale, (hi - T::to_float((elem_t)(w >> 16))) * kRestScale);
     const auto bits = [](float x, uint32_t top) {
         return (uint32_t)min(max((int)(__float_as_uint(x) - top), -32768), 32767);
     };
@@ -361,7 +363,7 @@ __device__ __forceinline__ uint32_t rest_of(uint32_t w, float lo, float hi) {
 }
 template <typename T>
 __device__ __forceinline__ float with_rest(elem_t o, elem_t rest) {
-    if constexpr (!std::is_same_v<T, Bf16>) return T::to_float(o) + T::to_float(rest);
+    if constexpr (!std::is_same_v<T, Bf16>) return __builtin_fmaf(T::to_float(rest), 1.0f / kRestScale, T::to_float(o));
     return __uint_as_float(((uint32_t)o << 16) + (uint32_t)(int)(int16_t)rest);
 }
 

@@ -77,3 +77,24 @@ def test_weights_of_large_scores_sum_to_one(shape, dtype):
     total, rows = got["dv"].cpu().double().sum(1), G * Lq
     limit = (2 * torch.finfo(dtype).eps / 2 + 2.0 ** -14) * rows + (2.0 ** -25 * Lk * (1 + rows) if dtype == FP16 else 0.0)
     assert bool(((total - rows).abs() <= limit).all()), float((total - rows).abs().max() / limit)
+
+
+def off_in_norm(x, **options):
+    """How far the table's gradient is off, relative to its norm."""
+    want = orc.attention(**x, **options)[0]["dtable"]
+    return float((run(x, **options)["dtable"].cpu().double() - want).norm() / want.norm())
+
+
+# the single backward launch by four waves and by eight, the pair, split axes, a long causal sequence
+EXACT = [((2, 4, 2, 128, 128, 64), {}), ((3, 2, 2, 200, 250, 64), {}), ((4, 2, 1, 100, 90, 32), {}), ((1, 1, 1, 300, 300, 128), {}),
+         ((1, 2, 1, 1500, 1500, 64), dict(bidirectional=False, causal=True))]
+
+
+@pytest.mark.parametrize("small", [0.01, 0.002])
+@pytest.mark.parametrize("shape,options", EXACT)
+def test_table_gradient_of_small_values_in_fp16(shape, options, small):
+    """Outputs of 1e-4: delta = dO.o is formed from o to 2^-22 of it or 2^-36, 1.5e-7 of such an output.  With what float32 adds (see
+    the next test) 3e-6 of the norm."""
+    x = make(*shape, FP16, seed=7, table=(32, torch.float32))
+    x["v"] = (x["v"].float() * small).to(FP16)
+    assert off_in_norm(x, **options) <= 3e-6
