@@ -98,3 +98,41 @@ def test_table_gradient_of_small_values_in_fp16(shape, options, small):
     x = make(*shape, FP16, seed=7, table=(32, torch.float32))
     x["v"] = (x["v"].float() * small).to(FP16)
     assert off_in_norm(x, **options) <= 3e-6
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("shape,options", EXACT + [((1, 2, 1, 512, 512, 64), {}), ((2, 4, 4, 7, 2500, 128), {})])
+@pytest.mark.parametrize("spread,added", [(1.0, 0.0), (2.0, 0.0), (1.0, 30.0)])
+def test_table_gradient_is_off_by_some_1e_6(shape, options, dtype, spread, added):
+    """Limits in the norm, which the terms of dS all but cancel in as they do in a sum of random signs, so that relative errors of single
+    terms come through as they are.  P = 2^x is off by half a step of x, i.e. by 2^-24 X ln 2 for |x| up to X, and is formed twice, for o and for dS.
+    Scores have a deviation of 1.44 spread^2 in units of log2 and the bias one of 1.44, largest among 1e5 pairs 5 of them: X is 16 for the
+    first, 32 with a spread of 2 (5 x 5.9) and 64 with 30 / ln 2 in every entry: 1.3e-6, 2.6e-6, 5.3e-6.  Contractions of 128 products and
+    delta add 2^-22 = 2.4e-7 each: 7e-7 with both.
+    P in one rounding (2^-9 of it in bf16), delta of a rounded o (2^-9, 2^-12) or, with bf16, P in two roundings (2^-18 of it at worst,
+    4e-6) do not stay below 2e-6."""
+    x = make(*shape, dtype, seed=7, table=(32, torch.float32), spread=spread)
+    x["table"] += added
+    assert off_in_norm(x, **options) <= 7e-7 + 2 * 2.0 ** -24 * 0.6932 * (64 if added else 32 if spread > 1.0 else 16)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("shape", FORMS)
+def test_backward_without_what_the_rounding_of_o_left(shape, dtype):
+    """delta is off by u |dO||o| then: u (a + b) more than the limits of single elements, for the table u a."""
+    from semicat_amd import RelativeBias, context_backward, context_forward
+    x = make(*shape, dtype, seed=8, table=(32, torch.float32))
+    d = {n: t.cuda() if n == "table" else t.cuda().transpose(1, 2) for n, t in x.items()}
+    bias = RelativeBias(d["table"], 60)
+    o, lse = context_forward(d["q"], d["k"], d["v"], bias)
+    dq, dk, dv, dtable = context_backward(d["q"], d["k"], d["v"], o, lse, d["dO"], bias)
+    got = {"o": o.transpose(1, 2), "dq": dq.transpose(1, 2), "dk": dk.transpose(1, 2), "dv": dv.transpose(1, 2), "dtable": dtable}
+    want, sizes = orc.attention(**x, max_distance=60)
+    u = torch.finfo(dtype).eps / 2
+    for name, t in got.items():
+        a, b, c = sizes[name]
+        own = torch.finfo(t.dtype).eps / 2 * want[name].abs()
+        limit = (2.0 ** -15 + u) * a + own if name == "dtable" else u * a + (u + 2.0 ** -14) * (a + b) + own
+        limit = limit + (2.0 ** -25 * (1.0 + c) if dtype == FP16 else 0.0) + 1e-30
+        off = (t.cpu().double() - want[name]).abs()
+        assert bool((off <= limit).all()), f"{name}: {float((off / limit).max()):.3g} times the limit"
