@@ -289,7 +289,7 @@ int sjvp_cast(int n, const void* const* x, void* const* y, const int64_t* count,
  *   table (or NULL: no bias, causal must be 0)   fp32, bf16 or fp16 [buckets of all directions][Hq] with strides table_stride
  *       (bucket, head); entries below -2.3e38 count as that, -inf excludes its keys.  bucket_first: HOST array of `buckets` first
  *       distances in ascending order from 0, the last one at most SJVP_CTX_MAX_DISTANCE; a distance has the last bucket that does
- *       not begin beyond it.  bidirectional: keys behind a query (j > start + i) have buckets of their own,
+ *       not begin beyond it (of equal ones all but the last are empty).  bidirectional: keys behind a query (j > start + i) have buckets of their own,
  *       buckets .. 2 buckets - 1, by their distance; otherwise they count as distance 0.
  *   o_rest (or NULL)   what the rounding of o left, 16 bits to an element in a form of its own, for the backward.  A forward that is
  *       given it forms o with probabilities of 16 bits or more (22 or 24 where the table is fp32) and stores what 22 (fp16, down to

@@ -96,7 +96,7 @@ __device__ __forceinline__ void write_buckets(const CtxParams& p, float* hists, 
         const int side = bucket >= p.buckets, j = min(bucket - side * p.buckets, p.buckets - 1);
         const int from = p.first[j], to = j + 1 < p.buckets ? p.first[j + 1] - 1 : zero;  // distances
         const int lo = side ? zero + max(from, 1) : zero - to;
-        const int hi = side ? zero + to : !p.both && j == 0 ? entries - 1 : zero - from;  // (above zero: distance 0)
+        const int hi = side ? zero + to : !p.both && from == 0 && to >= 0 ? entries - 1 : zero - from;  // (above zero: distance 0)
         float sum = 0.0f;
         for (int x = lo + (tid & 15); x <= hi; x += 16) sum += hists[x];
         sum = sum16(sum);

@@ -27,6 +27,33 @@ def near(got, want, sizes, x, names=None):
         assert bool((off <= limit).all()), f"{name}: {float((off / limit).max()):.3g} times the limit"
 
 
+@pytest.mark.parametrize("both,causal", [(False, False), (True, False), (False, True)])
+@pytest.mark.parametrize("shape", FORMS[:3])
+def test_bucket_lists_with_buckets_that_no_distance_has(shape, both, causal):
+    """Equal first distances: all but the last bucket of them are empty.  Results are those of the list without the empty ones, whose
+    entries have no gradient."""
+    from semicat_amd import RelativeBias, context_backward, context_forward
+    firsts, used = (0, 0, 0, 2, 7, 7, 40), [2, 3, 5, 6]
+    x = make(*shape, BF16, seed=5, table=(14 if both else 7, torch.float32))
+    d = {n: t.cuda() if n == "table" else t.cuda().transpose(1, 2) for n, t in x.items()}
+    rows = used + [7 + i for i in used] if both else used
+
+    def passes(table, starts):
+        bias = RelativeBias(table, 40, both, causal)
+        bias.starts = starts
+        rest = torch.empty_like(d["q"])
+        o, lse = context_forward(d["q"], d["k"], d["v"], bias, o_rest=rest)
+        return o, *context_backward(d["q"], d["k"], d["v"], o, lse, d["dO"], bias, o_rest=rest)
+
+    got = passes(d["table"], firsts)
+    want = passes(d["table"][rows].contiguous(), tuple(firsts[i] for i in used))
+    for a, b in zip(got[:-1], want[:-1]):
+        assert torch.equal(a, b)
+    full = torch.zeros_like(got[-1])
+    full[rows] = want[-1]
+    assert torch.equal(got[-1], full)
+
+
 @pytest.mark.parametrize("value", [-1e9, LOW])
 @pytest.mark.parametrize("shape", FORMS + [(6, 8, 1, 700, 900, 64), (9, 8, 2, 500, 600, 128)])
 def test_a_bias_that_leaves_nothing_of_the_scores_does_so_at_every_distance(shape, value):
