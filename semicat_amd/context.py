@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import operator
 from typing import Optional, Tuple, Union
 
 import torch
@@ -116,7 +117,7 @@ def _check_inputs(q, k, v, bias, key_lengths, query_lengths, query_start) -> Non
     _check_indices("query_lengths", query_lengths, q)
     if isinstance(query_start, Tensor):
         _check_indices("query_start", query_start, q)
-    elif not -_lib.SJVP_CTX_MAX_POSITION <= int(query_start) <= _lib.SJVP_CTX_MAX_POSITION:
+    elif not -_lib.SJVP_CTX_MAX_POSITION <= operator.index(query_start) <= _lib.SJVP_CTX_MAX_POSITION:
         raise ValueError(f"query_start must lie within +-{_lib.SJVP_CTX_MAX_POSITION}, got {query_start}")
     if bias is not None:
         if bias.table.shape[1] != H:
@@ -138,7 +139,7 @@ def _call(backward: bool, tensors, lse, bias, key_lengths, query_lengths, query_
     if isinstance(query_start, Tensor):
         t.query_start = ptr(query_start)
     else:
-        t.query_start0 = int(query_start)
+        t.query_start0 = operator.index(query_start)
     if bias is not None:
         t.table, t.table_dtype = ptr(bias.table), _TABLE_DTYPES[bias.table.dtype]
         t.table_stride[:] = bias.table.stride()

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from semicat_amd import context_backward
+from semicat_amd import RelativeBias, context_backward, context_forward, relative_bucket_starts
 from tests.test_context import _t
 
 
@@ -11,3 +11,9 @@ def test_the_statistics_of_a_row_are_two_numbers():
     for shape in ((1, 2, 3), (1, 2, 3, 1), (2, 1, 2, 3)):
         with pytest.raises(AssertionError):
             context_backward(q, q, q, q, _t(*shape, dtype=torch.float32), q)
+
+
+@pytest.mark.parametrize("start", [1.5, 2.0, "1", None])
+def test_query_start_is_a_whole_number(start):
+    with pytest.raises(TypeError):
+        context_forward(*[_t(1, 2, 3, 32)] * 3, query_start=start)
