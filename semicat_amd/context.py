@@ -27,11 +27,12 @@ _DTYPES = {torch.bfloat16: _lib.SJVP_BF16, torch.float16: _lib.SJVP_FP16}
 _TABLE_DTYPES = {torch.bfloat16: _lib.SJVP_BF16, torch.float16: _lib.SJVP_FP16, torch.float32: _lib.SJVP_FP32}
 
 
-@functools.lru_cache(maxsize=64)
+@functools.lru_cache(maxsize=64, typed=True)
 def relative_bucket_starts(buckets: int, max_distance: int = 128) -> Tuple[int, ...]:
     """The first distance of each bucket of one direction.  The lower half of the ``n`` buckets are single distances; bucket
     ``single + k`` begins at the least ``d`` with ``(d / single) ** (n - single) >= (max_distance / single) ** k``, so that the
     upper ones grow evenly in the logarithm and the last one has no end.  In whole numbers: no rounding at a border."""
+    buckets, max_distance = operator.index(buckets), operator.index(max_distance)
     single = buckets // 2
     if buckets < 2 or buckets > _lib.SJVP_CTX_MAX_BUCKETS:
         raise ValueError(f"a direction has 2 to {_lib.SJVP_CTX_MAX_BUCKETS} buckets, got {buckets}")
@@ -47,7 +48,7 @@ def relative_bucket_starts(buckets: int, max_distance: int = 128) -> Tuple[int, 
     return tuple(starts)
 
 
-@functools.lru_cache(maxsize=64)
+@functools.lru_cache(maxsize=64, typed=True)
 def _packed_starts(rows: int, max_distance: int, bidirectional: bool) -> bytes:
     """The first distances as the host extension takes them, for a table of that many rows."""
     if bidirectional and rows % 2:

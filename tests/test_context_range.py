@@ -17,3 +17,12 @@ def test_the_statistics_of_a_row_are_two_numbers():
 def test_query_start_is_a_whole_number(start):
     with pytest.raises(TypeError):
         context_forward(*[_t(1, 2, 3, 32)] * 3, query_start=start)
+
+
+@pytest.mark.parametrize("call", [lambda: relative_bucket_starts(16, 100.5), lambda: relative_bucket_starts(16.0, 128),
+                                  lambda: relative_bucket_starts(16, 128.0), lambda: RelativeBias(_t(32, 2), 128.0)])
+def test_buckets_and_distances_are_whole_numbers(call):
+    """Also where a whole number of the same value was asked for before."""
+    relative_bucket_starts(16, 128)
+    with pytest.raises(TypeError):
+        call()
