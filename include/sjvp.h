@@ -281,7 +281,7 @@ int sjvp_cast(int n, const void* const* x, void* const* y, const int64_t* count,
  *   s[i][j] = scale q_i.k_j + table[bucket(j - (start + i))][head]      for j < key length (causal: and j <= start + i)
  *   lse_i = log sum_j exp s[i][j],   o_i = sum_j exp(s[i][j] - lse_i) v_j
  * q, o, dO, dq: [B,Hq,Lq,D]; k, v, dk, dv: [B,Hkv,Lk,D]; Hq a multiple of Hkv, query head h reads key head h / (Hq / Hkv).
- * Any strides (batch, head, sequence; unit last stride; the sequence stride of an input below 2^24) and any alignment of the rows.
+ * Any strides (batch, head, sequence; unit last stride; the sequence stride of an input of two rows or more below 2^24) and any alignment of the rows.
  *   key_lengths, query_lengths, query_start   device arrays [B], or NULL: every sequence is as long as its tensor, and its
  *       query 0 has position query_start0 (which is added to query_start[b] otherwise).  Lengths are clamped to the tensor.  What
  *       lies in rows behind a length is not used, not even NaN; results there are zeros.  query_start and query_start0 lie within +-2^29.

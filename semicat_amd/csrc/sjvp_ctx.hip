@@ -142,6 +142,10 @@ int ctx_params(const sjvp_ctx* t, CtxParams& p) {
     const void* ptrs[SJVP_C_COUNT] = {t->q, t->k, t->v, t->o, t->o_rest, t->dO, t->dq, t->dk, t->dv};
     for (int i = 0; i < SJVP_C_COUNT; ++i)
         *views[i] = {static_cast<elem_t*>(const_cast<void*>(ptrs[i])), t->strides[3 * i], t->strides[3 * i + 1], t->strides[3 * i + 2]};
+    for (CtxView* v : {&p.q, &p.g})
+        if (t->Lq == 1) v->sl = t->D;  // (one row: no stride)
+    for (CtxView* v : {&p.k, &p.v})
+        if (t->Lk == 1) v->sl = t->D;
     for (const CtxView* v : {&p.q, &p.k, &p.v, &p.g})
         if (v->ptr && (v->sl < 0 || v->sl >= 1 << 24)) return SJVP_ERR_SHAPE;
     p.lse = t->lse;

@@ -571,7 +571,8 @@ struct ContextOptions {
     Tensor klen, qlen, start;  // or undefined
 };
 
-constexpr int64_t kMostStride = 1 << 24;  // of an input's sequence axis
+// whether the kernels take the stride of an input's sequence axis
+bool context_stride(const Tensor& x) { return x.size(1) == 1 || x.stride(1) < 1 << 24; }
 
 int type_tag(at::ScalarType t) { return t == at::kFloat ? SJVP_FP32 : t == at::kBFloat16 ? SJVP_BF16 : t == at::kHalf ? SJVP_FP16 : -1; }
 
@@ -671,7 +672,7 @@ struct ContextNode : torch::autograd::Function<ContextNode> {
         {
             const at::NoGradGuard no_grad;
             const c10::DeviceGuard guard(q.device());
-            const Tensor g = cotangents[0].stride(3) == 1 && cotangents[0].stride(1) < kMostStride ? cotangents[0] : cotangents[0].contiguous();
+            const Tensor g = cotangents[0].stride(3) == 1 && context_stride(cotangents[0]) ? cotangents[0] : cotangents[0].contiguous();
             const Maker make_tensor{q.device()};
             sjvp_ctx t = context_struct(q, k, v, table, options);
             t.lse = static_cast<float*>(lse.data_ptr());
@@ -716,7 +717,7 @@ PyObject* context(PyObject*, PyObject* const* a, Py_ssize_t n) {
     for (int i = 0; i < 3; ++i) {
         in[i] = plain(a[i]);
         if (!in[i] || in[i]->dim() != 4 || in[i]->stride(3) != 1 || in[i]->scalar_type() != in[0]->scalar_type() ||
-            in[i]->device() != in[0]->device() || in[i]->numel() == 0 || in[i]->stride(1) >= kMostStride || in[i]->_fw_grad(0).defined())
+            in[i]->device() != in[0]->device() || in[i]->numel() == 0 || !context_stride(*in[i]) || in[i]->_fw_grad(0).defined())
             return none();
         for (int d = 0; d < 4; ++d)
             if (in[i]->size(d) > INT_MAX) return none();

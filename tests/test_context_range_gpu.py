@@ -163,3 +163,26 @@ def test_backward_without_what_the_rounding_of_o_left(shape, dtype):
         limit = limit + (2.0 ** -25 * (1.0 + c) if dtype == FP16 else 0.0) + 1e-30
         off = (t.cpu().double() - want[name]).abs()
         assert bool((off <= limit).all()), f"{name}: {float((off / limit).max()):.3g} times the limit"
+
+
+def test_strides_of_axes_of_one_row():
+    """A sequence axis of size one has no stride that anything depends on."""
+    from semicat_amd import cross_attention
+    x = make(2, 4, 2, 1, 1, 64, BF16, seed=9)
+    y = make(2, 4, 2, 5, 7, 64, BF16, seed=9)
+
+    def far(t):
+        return t.as_strided(t.shape, (t.stride(0), (1 << 24) + 4, t.stride(2), 1))
+
+    def passes(q, k, v, dO):
+        leaves = [t.requires_grad_() for t in (q, k, v)]
+        o = cross_attention(*leaves)
+        with torch.no_grad():
+            plain = cross_attention(*leaves)
+        return (o.detach(), plain, *torch.autograd.grad(o, leaves, dO))
+
+    for a, b in ((x, x), (x, y), (y, x)):  # one row on both sides, one query, one key
+        d = [t.cuda() for t in (a["q"], b["k"], b["v"], a["dO"])]
+        want = passes(*(t.clone() for t in d))
+        got = passes(*(far(t.clone()) if t.shape[1] == 1 else t.clone() for t in d))
+        assert all(torch.equal(s, t) for s, t in zip(got, want))
