@@ -569,7 +569,10 @@ struct ContextOptions {
     float scale = 0.0f;
     std::string first;  // int32 first distances of the buckets
     Tensor klen, qlen, start;  // or undefined
+    mutable int status = SJVP_OK;  // of a forward that its node has thrown
 };
+
+constexpr int64_t kMostRows = 1 << 29;  // of any axis, and of positions
 
 // whether the kernels take the stride of an input's sequence axis
 bool context_stride(const Tensor& x) { return x.size(1) == 1 || x.stride(1) < 1 << 24; }
@@ -651,6 +654,7 @@ struct ContextNode : torch::autograd::Function<ContextNode> {
         Tensor lse, rest;
         int status;
         Tensor o = context_forward(q, k, v, table.value_or(Tensor()), *options, &lse, &rest, status);
+        options->status = status;
         context_check(status);
         ctx->save_for_backward({q, k, v, table.value_or(Tensor()), options->klen, options->qlen, options->start, o, lse, rest});
         ctx->saved_data["options"] = c10::IValue(std::vector<int64_t>{options->start0, options->both, options->causal});
@@ -720,7 +724,7 @@ PyObject* context(PyObject*, PyObject* const* a, Py_ssize_t n) {
             in[i]->device() != in[0]->device() || in[i]->numel() == 0 || !context_stride(*in[i]) || in[i]->_fw_grad(0).defined())
             return none();
         for (int d = 0; d < 4; ++d)
-            if (in[i]->size(d) > INT_MAX) return none();
+            if (in[i]->size(d) > kMostRows) return none();
     }
     const Tensor &q = *in[0], &k = *in[1], &v = *in[2];
     if ((q.scalar_type() != at::kBFloat16 && q.scalar_type() != at::kHalf) || k.sizes() != v.sizes() || k.size(0) != q.size(0) ||
@@ -733,7 +737,7 @@ PyObject* context(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (a[4 + i] == Py_None) continue;
         if (i == 2 && PyLong_CheckExact(a[6])) {
             const long start = PyLong_AsLong(a[6]);
-            if (PyErr_Occurred() || start < -(1 << 29) || start > 1 << 29) {
+            if (PyErr_Occurred() || start < -kMostRows || start > kMostRows) {
                 PyErr_Clear();
                 return none();
             }
@@ -763,8 +767,14 @@ PyObject* context(PyObject*, PyObject* const* a, Py_ssize_t n) {
         pybind11::gil_scoped_release no_gil;
         const bool record = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() ||
                                                            (table.defined() && table.requires_grad()));
-        if (record) o = ContextNode::apply(q, k, v, table.defined() ? std::optional<Tensor>(table) : std::nullopt, &options);
-        else o = context_forward(q, k, v, table, options, nullptr, nullptr, status);
+        if (record) {
+            try {
+                o = ContextNode::apply(q, k, v, table.defined() ? std::optional<Tensor>(table) : std::nullopt, &options);
+            } catch (const c10::Error&) {
+                if (options.status == SJVP_OK) throw;
+                status = options.status;  // (raised as every other status)
+            }
+        } else o = context_forward(q, k, v, table, options, nullptr, nullptr, status);
     }
     if (status != SJVP_OK) return PyLong_FromLong(status);
     return THPVariable_Wrap(std::move(o));

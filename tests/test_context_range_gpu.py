@@ -186,3 +186,16 @@ def test_strides_of_axes_of_one_row():
         want = passes(*(t.clone() for t in d))
         got = passes(*(far(t.clone()) if t.shape[1] == 1 else t.clone() for t in d))
         assert all(torch.equal(s, t) for s, t in zip(got, want))
+
+
+@pytest.mark.parametrize("training", [False, True])
+def test_sizes_beyond_the_range_raise_what_the_checks_raise(training):
+    """Expanded tensors of one row; nothing is launched.  More sequences than a launch has workgroups for: the library's own error."""
+    from semicat_amd import _lib, cross_attention
+    q, k = (torch.zeros(1, 1, 1, 16, device="cuda", dtype=BF16, requires_grad=training) for _ in range(2))
+    with pytest.raises(ValueError):
+        cross_attention(q, k.expand(1, (1 << 29) + 1, 1, 16), k.expand(1, (1 << 29) + 1, 1, 16))
+    many = (1 << 24) + 8
+    with pytest.raises(_lib.SjvpError) as info:
+        cross_attention(q.expand(many, 1, 1, 16), k.expand(many, 1, 1, 16), k.expand(many, 1, 1, 16))
+    assert info.value.status == _lib.SJVP_ERR_SHAPE
