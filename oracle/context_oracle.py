@@ -62,7 +62,7 @@ def attention(q, k, v, dO=None, table=None, max_distance=128, bidirectional=True
             if tab is not None:
                 s = s + tab[:, h][at]
             if scores_in is not None:
-                s = (s - s.detach()) + s.detach().to(scores_in).double()
+                s = s + (s.detach().to(scores_in).double() - s.detach()).nan_to_num(0.0)  # (-inf stays)
             hidden = ~seen | (s == -math.inf)
             some = (~hidden).any(1)
             s = s.masked_fill(hidden, -math.inf)[some]
