@@ -285,9 +285,11 @@ int sjvp_cast(int n, const void* const* x, void* const* y, const int64_t* count,
  *   key_lengths, query_lengths, query_start   device arrays [B], or NULL: every sequence is as long as its tensor, and its
  *       query 0 has position query_start0 (which is added to query_start[b] otherwise).  Lengths are clamped to the tensor.  What
  *       lies in rows behind a length is not used, not even NaN; results there are zeros.  query_start and query_start0 lie within +-2^29.
- *   a row that sees no key (also: whose every key has the bias -inf) has o = 0, lse = (0, 0) and no gradient, for any finite dO.
+ *   a row that sees no key (also: whose every key has the bias -inf) has o = 0, lse = (0, 0) and no gradient, for any dO whose products
+ *       with v are finite.
  *   table (or NULL: no bias, causal must be 0)   fp32, bf16 or fp16 [buckets of all directions][Hq] with strides table_stride
- *       (bucket, head); entries below -2.3e38 count as that, -inf excludes its keys.  bucket_first: HOST array of `buckets` first
+ *       (bucket, head); entries below -2.3e38 count as that, -inf excludes its keys; score and bias are added in fp32, so that nothing is
+ *       left of the scores beside a bias of 1e8 or more, and rows whose keys all have one weigh them alike.  bucket_first: HOST array of `buckets` first
  *       distances in ascending order from 0, the last one at most SJVP_CTX_MAX_DISTANCE; a distance has the last bucket that does
  *       not begin beyond it (of equal ones all but the last are empty).  bidirectional: keys behind a query (j > start + i) have buckets of their own,
  *       buckets .. 2 buckets - 1, by their distance; otherwise they count as distance 0.

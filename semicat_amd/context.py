@@ -305,7 +305,8 @@ def cross_attention(q: Tensor, k: Tensor, v: Tensor, key_lengths: Optional[Tenso
 def relative_attention(q: Tensor, k: Tensor, v: Tensor, table: Tensor, max_distance: int = 128, bidirectional: bool = True,
                        causal: bool = False, key_lengths: Optional[Tensor] = None, query_lengths: Optional[Tensor] = None,
                        query_start: Union[int, Tensor] = 0, scale: Optional[float] = None) -> Tensor:
-    """:func:`cross_attention` with ``table[bucket(j - (query_start + i)), h]`` added to the score of query ``i`` and key ``j``.
+    """:func:`cross_attention` with ``table[bucket(j - (query_start + i)), h]`` added to the score of query ``i`` and key ``j``, in float32
+    (keys that all have the lowest number weigh alike, ``-inf`` leaves its keys out).
 
     ``table`` is ``[num_buckets, Hq]`` (float32, bfloat16 or float16; its gradient is summed in float32, and formed to some
     1e-6 for a float32 table).  Buckets go by distance (:func:`relative_bucket_starts`): with ``bidirectional`` the second half of

@@ -44,7 +44,8 @@ int splits_for(int64_t groups, int64_t steps, int64_t least) {
 
 }  // namespace
 
-// Times of the rules below in microseconds, D = 64 unless said, (B,Hq,Lq,Lk) bf16; `rel`: with a bias.
+// Times of the rules below in microseconds, D = 64 unless said, (B,Hq,Lq,Lk) bf16; `rel`: with a bias.  They ask for compute units and tiles
+// alone: of D <= 32 and D > 64 the backward's were measured at the entries given, not over a range.
 //
 // Few rows (ctx_fwd_few) where the rows of a key head fit one block, and where blocks of 128 rows would leave half of the compute
 // units idle: (2,8,512,1024) rel 15.2 / 31.4 by blocks of 128, (2,16,200,2000) D=128 28 / 65, (4,16,256,1024) 18.5 / 20.6; beyond

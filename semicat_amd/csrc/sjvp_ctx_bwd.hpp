@@ -4,7 +4,8 @@
 //   dQ = scale dS K,  dK = scale sum_heads dS^T Q,  dV = sum_heads P^T dO,  dtable[bucket][head] = sum of dS over its differences
 //
 // A row-owned launch (dQ, delta and the bucket sums) and a column-owned one (dK, dV), both of which recompute P: 3 + 4
-// contractions against the 5 of a single launch, whose dQ would be summed by atomics in an order that changes from run to run.
+// contractions against the 5 of a single launch, whose dQ would be summed over workgroups by atomics in an order that changes from run
+// to run, except where a workgroup holds all keys of a sequence (ctx_bwd_one).
 #pragma once
 #include "sjvp_ctx.hpp"
 
@@ -42,7 +43,7 @@ __device__ __forceinline__ float row_delta(const CtxParams& p, const u32x4* own_
 
 // What LDS holds of 32 looped rows, as the registers of a score tile.  -delta is where the contraction for dP starts, an instruction less to an
 // element (B=8 Hq=16 Hkv=4 Lq=2048 Lk=1024 D=128 1.5 % of forward and backward), but not where dS is summed by bucket: the matrix unit cuts
-// off what it adds below its larger addends, and the sums of an fp32 table's gradient would be 4e-6 off in place of 1e-6.
+// off what it adds below its larger addends, and the gradient of an fp32 table would be some 4e-6 off.
 __device__ __forceinline__ f32x16 of_rows(const float* rows, int h) {
     f32x16 x;
 #pragma unroll
@@ -105,8 +106,8 @@ __device__ __forceinline__ void write_buckets(const CtxParams& p, float* hists, 
 }
 
 // Row-owned: four waves of 32 query rows of one head share tiles of 64 keys.  Bound by the matrix unit and the vector instructions
-// together with the latency of a tile, two waves to a SIMD: B=8 H=16 L=4096 D=64 causal with bias 528 us (three contractions at 0.78
-// PFLOP/s, the matrix unit busy 36 %, vector instructions issued 56 %), B=8 Hq=16 Hkv=4 Lq=2048 Lk=1024 D=128 224 us.
+// together with the latency of a tile, two waves to a SIMD: B=8 H=16 L=4096 D=64 causal with bias 530 us (three contractions at 0.78
+// PFLOP/s, the matrix unit busy 37 %, vector instructions issued 56 %), B=8 Hq=16 Hkv=4 Lq=2048 Lk=1024 D=128 224 us.
 template <typename T, int HD, bool BIAS, bool DMA>
 __global__ __launch_bounds__(kCtxThreads, HD <= 64 && !BIAS ? 3 : 2) void ctx_bwd_row(CtxParams p) {
     if constexpr (DMA) __builtin_assume(p.D % 8 == 0);
@@ -261,8 +262,8 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 && !BIAS ? 3 : 2) void ctx_bw
 }
 
 // Column-owned: four waves of 32 keys share tiles of 64 query rows, over all heads that read the key head.  Bound as the row-owned
-// launch, at D = 128 with one wave to a SIMD (dK, dV, K and V of a wave are 256 registers): the cases above 662 us (four
-// contractions at 0.83 PFLOP/s) and 326 us.  (Half tiles in a rolled loop: 1 % and 4 % slower.)
+// launch, at D = 128 with one wave to a SIMD (dK, dV, K and V of a wave are 256 registers): the cases above 640 us (four
+// contractions at 0.86 PFLOP/s) and 310 us.  (Half tiles in a rolled loop: 1 % and 4 % slower.)
 template <typename T, int HD, bool BIAS, bool DMA>
 __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_col(CtxParams p) {
     if constexpr (DMA) __builtin_assume(p.D % 8 == 0);
@@ -399,9 +400,9 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void ctx_bwd_col(Ctx
 // tile's rows is contracted over all keys, by a quarter of 32 rows x 32 columns for each of four waves.  With eight waves the two
 // halves of the workgroup take turns, and the other half is ahead with the next tile's scores meanwhile; where two tiles' dS fit LDS, they
 // alternate, which leaves one barrier to a tile (B=64 H=12 1024 x 256 with bias 305 us, with one 314).
-// B=128 H=12 L=256 D=64 with bias 226 us against 132 row-owned + 125 column-owned, B=64 H=12 L=128 48 against 32.5 + 27.5.  Bound by
+// B=128 H=12 L=256 D=64 with bias 212 us against 132 row-owned + 125 column-owned, B=64 H=12 L=128 48 against 32.5 + 27.5.  Bound by
 // the latency of a tile's chain (scores, dS to LDS, barrier, dQ): one workgroup of eight waves to a compute unit, vector instructions
-// issued 35 % of the time, the matrix unit busy 12 %.
+// issued 38 % of the time, the matrix unit busy 13 %.
 template <typename T, bool BIAS, bool DMA, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, 2) void ctx_bwd_one(CtxParams p) {
     if constexpr (DMA) __builtin_assume(p.D % 8 == 0);

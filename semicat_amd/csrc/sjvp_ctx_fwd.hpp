@@ -67,16 +67,16 @@ struct RowSums {
 // TERMS > 1, for a backward to follow: the gradients need delta = dO . o as it would be with unrounded probabilities (their sums over
 // a row are differences of near numbers), so P goes into the contraction with what its rounding leaves, and so does o into memory.
 // Two terms leave 2e-6 of o in bf16, for gradients that are rounded to 16 bits in the end.  The gradient of an fp32 table in bf16 takes
-// three: a bucket's sum over all rows is far below its terms' where it all but cancels (B=H=1 L=300 D=128: 5e-6 of it with two terms,
-// 1.1e-6 with three), for 2 % of a training pass at L=256 D=64 and 8 % at a causal 4096.
+// three: a bucket's sum over all rows is far below its terms' where it all but cancels (in norm, B=H=1 L=300 D=128: 2.1e-6 of it off with two
+// terms, 3.1e-7 with three), for 2 % of a training pass at L=256 D=64 and 8 % at a causal 4096.
 //
 // Many rows: four waves of 32 rows of one head share tiles of 64 keys.  Two tiles of K and V in LDS: the next one is on its way
 // while this one is used, one barrier to a tile.  Bound by the issue of vector instructions and by power: of
-// B=8 H=16 Lq=4096 Lk=1024 (half of the keys there) D=64, 138 us, vector instructions are issued 81 % of the time and the matrix unit is
+// B=8 H=16 Lq=4096 Lk=1024 (half of the keys there) D=64, 141 us, vector instructions are issued 82 % of the time and the matrix unit is
 // busy 47 %, at 1.7 GHz.  So the loops hold neither masks nor bounds, the running maximum is raised seldom, and up to D = 64 four
 // waves share a SIMD (128 registers), whose instructions fill each other's gaps (141 us against 145 by two waves with the scores of the
 // next tile ahead, in turn).
-// At D = 128 two (B=8 Hq=16 Hkv=4 Lq=2048 Lk=1024 with rests: 184 us, the matrix unit busy 47 %).
+// At D = 128 two (B=8 Hq=16 Hkv=4 Lq=2048 Lk=1024 with rests: 196 us, the matrix unit busy 47 %).
 template <typename T, int HD, bool BIAS, bool DMA, int TERMS>
 __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 4 : 2) void ctx_fwd(CtxParams p) {
     if constexpr (DMA) __builtin_assume(p.D % 8 == 0);
