@@ -281,7 +281,8 @@ int sjvp_cast(int n, const void* const* x, void* const* y, const int64_t* count,
  *   s[i][j] = scale q_i.k_j + table[bucket(j - (start + i))][head]      for j < key length (causal: and j <= start + i)
  *   lse_i = log sum_j exp s[i][j],   o_i = sum_j exp(s[i][j] - lse_i) v_j
  * q, o, dO, dq: [B,Hq,Lq,D]; k, v, dk, dv: [B,Hkv,Lk,D]; Hq a multiple of Hkv, query head h reads key head h / (Hq / Hkv).
- * Any strides (batch, head, sequence; unit last stride; the sequence stride of an input of two rows or more below 2^24) and any alignment of the rows.
+ * Any strides (batch, head, sequence; unit last stride; the sequence stride of an input of two rows or more below 2^24) and any alignment of
+ * the rows.
  *   key_lengths, query_lengths, query_start   device arrays [B], or NULL: every sequence is as long as its tensor, and its
  *       query 0 has position query_start0 (which is added to query_start[b] otherwise).  Lengths are clamped to the tensor.  What
  *       lies in rows behind a length is not used, not even NaN; results there are zeros.  query_start and query_start0 lie within +-2^29.
@@ -289,15 +290,15 @@ int sjvp_cast(int n, const void* const* x, void* const* y, const int64_t* count,
  *       with v are finite.
  *   table (or NULL: no bias, causal must be 0)   fp32, bf16 or fp16 [buckets of all directions][Hq] with strides table_stride
  *       (bucket, head); entries below -2.3e38 count as that, -inf excludes its keys; score and bias are added in fp32, so that nothing is
- *       left of the scores beside a bias of 1e8 or more, and rows whose keys all have one weigh them alike.  bucket_first: HOST array of `buckets` first
- *       distances in ascending order from 0, the last one at most SJVP_CTX_MAX_DISTANCE; a distance has the last bucket that does
- *       not begin beyond it (of equal ones all but the last are empty).  bidirectional: keys behind a query (j > start + i) have buckets of their own,
- *       buckets .. 2 buckets - 1, by their distance; otherwise they count as distance 0.
+ *       left of the scores beside a bias of 1e8 or more, and rows whose keys all have one weigh them alike.
+ *   bucket_first   HOST array of `buckets` first distances in ascending order from 0, the last one at most SJVP_CTX_MAX_DISTANCE; a
+ *       distance has the last bucket that does not begin beyond it (of equal ones all but the last are empty).  bidirectional: keys
+ *       behind a query (j > start + i) have buckets of their own, buckets .. 2 buckets - 1, by their distance; otherwise they count as
+ *       distance 0.
  *   o_rest (or NULL)   what the rounding of o left, 16 bits to an element in a form of its own, for the backward.  A forward that is
  *       given it forms o with probabilities of 16 bits or more (22 or 24 where the table is fp32) and stores what 22 (fp16, down to
- *       steps of 2^-35) or 24 bits hold of it; the backward needs it
- *       for rowsum(dO * o), of which dS is a small difference where attention is sharp, and which the gradient of an fp32 table
- *       (formed to some 1e-6 with it) is a sum over.
+ *       steps of 2^-35) or 24 bits hold of it; the backward needs it for rowsum(dO * o), of which dS is a small difference where
+ *       attention is sharp, and which the gradient of an fp32 table (formed to some 1e-6 with it) is a sum over.
  *   lse   [B,Hq,Lq][2] fp32 contiguous: m, l of each row with lse_i = m ln 2 + ln l, two numbers, since one would lose l beside large
  *       scores or biases; the forward takes NULL where no backward follows.
  *   dO   fp16: dS = P (dP - delta) is rounded to fp16 on its way into dQ and dK, so that losses are scaled as usual with this type.

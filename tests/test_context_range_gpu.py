@@ -106,6 +106,19 @@ def test_weights_of_large_scores_sum_to_one(shape, dtype):
     assert bool(((total - rows).abs() <= limit).all()), float((total - rows).abs().max() / limit)
 
 
+@pytest.mark.parametrize("value", [-1e4, -1e5, -1e6, 1e6])
+@pytest.mark.parametrize("shape", FORMS)
+def test_weights_beside_a_large_bias_sum_to_one(shape, value):
+    """As above, with a bias that leaves some of the scores: forward and backward round score plus bias alike."""
+    B, H, G, Lq, Lk, _ = shape
+    x = make(*shape, FP16, seed=6, table=(32, torch.float32))
+    x["table"][:] = value
+    x["dO"] = torch.ones_like(x["dO"])
+    total, rows = run(x, max_distance=60)["dv"].cpu().double().sum(1), G * Lq
+    limit = (2 * torch.finfo(FP16).eps / 2 + 2.0 ** -14) * rows + 2.0 ** -25 * Lk * (1 + rows)
+    assert bool(((total - rows).abs() <= limit).all()), float((total - rows).abs().max() / limit)
+
+
 def off_in_norm(x, **options):
     """How far the table's gradient is off, relative to its norm."""
     want = orc.attention(**x, **options)[0]["dtable"]
