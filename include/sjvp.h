@@ -48,7 +48,7 @@
 extern "C" {
 #endif
 
-#define SJVP_VERSION 1
+#define SJVP_VERSION 2   /* 2: lse of sjvp_ctx has two numbers to a row */
 
 enum sjvp_dtype { SJVP_BF16 = 0, SJVP_FP16 = 1, SJVP_FP32 = 2, SJVP_FP32_BF16 = 3 };
 
