@@ -45,11 +45,11 @@ def listed():
         # The LM1B network's batch with its sentences packed in place of padded.
         _packed("packed_train_lm1b", "packed_train", 64, 128, 0.125, 0, 12, 1, 64, "bf16", False),
         # Training on long documents with shared key heads.
-        _packed("packed_train_long", "packed_train", 4, 6144, 0.25, 0, 16, 4, 128, "bf16", True),
+        _packed("packed_train_long", "packed_train", 4, 6000, 0.25, 0, 16, 4, 128, "bf16", True),
         # Two long prompts before their first token is drawn.
         _packed("packed_prompt_long", "packed_forward", 2, 8192, 0.6, 0, 16, 8, 128, "bf16", True),
         # A generation step writes one token of each sequence.
-        _paged("paged_write_step", "paged_write", 64, 1, 4096, 0.25, 16, 4, 128, "bf16", 16, "e4m3"),
+        _paged("paged_write_step", "paged_write", 64, 1, 4096, 0.3, 16, 4, 128, "bf16", 16, "e4m3"),
         # Whole prompts are written.
         _paged("paged_write_prompt", "paged_write", 8, 4096, 4096, 0.5, 32, 4, 128, "bf16", 64, "e4m3"),
         # A few short sequences are read back, pages of a size that is no power of two.
