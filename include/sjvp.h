@@ -66,7 +66,8 @@ enum sjvp_status {
                                 sjvp_fwd_rotary / sjvp_bwd_rotary: a shape, dtype or table they do not serve */
     SJVP_ERR_SCALE = -10,    /* scale negative, infinite or NaN (0 selects the default)      */
     SJVP_ERR_SCRATCH = -11,  /* sjvp_bwd_noalloc: problem beyond SJVP_NOALLOC_MAX_ROWS, or no static scratch on this device */
-    SJVP_ERR_BUCKETS = -12   /* sjvp_ctx_*: a bucket count or list of first distances that is not served */
+    SJVP_ERR_BUCKETS = -12,  /* sjvp_ctx_*: a bucket count or list of first distances that is not served */
+    SJVP_ERR_PAGES = -13     /* sjvp_paged_*: a cache that is not served */
 };
 
 /* Indices into the stride tables: strides[3*i + {0,1,2}] = (batch, head, sequence) strides in
@@ -333,6 +334,81 @@ typedef struct sjvp_ctx {
 size_t sjvp_ctx_workspace_bytes(const sjvp_ctx* t, int backward);
 int sjvp_ctx_fwd(const sjvp_ctx* t, int dtype, void* stream);
 int sjvp_ctx_bwd(const sjvp_ctx* t, int dtype, void* stream);
+
+/*
+ * Attention over packed sequences, with its backward, and over a paged cache; SJVP_BF16 or SJVP_FP16 tensors, without tangents:
+ *   s[i][j] = scale q_i.k_j for the keys j of the query's own sequence (causal: up to the query's own position),
+ *   p = softmax over j,   o_i = sum_j p[i][j] v_j
+ * B sequences stand one behind the other in tensors [T,H,D] (views by the strides of head and row in elements, unit last stride, any
+ * alignment of the rows; the row stride of an input of two rows or more below 2^24).  offsets, a device array [B+1] in ascending order,
+ * says where: sequence b has the rows offsets[b] .. offsets[b+1]-1.  Sequences may be empty.  Results of rows in front of the first
+ * sequence and behind the last one are zeros, and what stands in inputs there is not used.  Hq is a multiple of Hkv; query head h reads key head
+ * h / (Hq / Hkv).  T * Hq < 2^31, T and B up to 2^29.
+ */
+enum sjvp_packed_tensor { SJVP_S_Q = 0, SJVP_S_K, SJVP_S_V, SJVP_S_O, SJVP_S_DO, SJVP_S_DQ, SJVP_S_DK, SJVP_S_DV, SJVP_S_COUNT };
+/*
+ * Whole sequences: q, o, dO, dq [T,Hq,D]; k, v, dk, dv [T,Hkv,D].
+ *   lse   [Hq][T][2] fp32: m, l of each row as sjvp_ctx_fwd() stores them; the forward takes NULL where no backward follows.
+ *   dk, dv   both or neither (then without the launch that makes them)
+ *   A row that sees one key has exactly no gradient of its score.  Sums are fp32, in a fixed order.
+ * strides[2*i + {0,1}]: (head, row) strides of tensor i of sjvp_packed_tensor.  scale 0: 1/sqrt(D).  The workspace is device memory of
+ * sjvp_packed_workspace_bytes() bytes, 16-byte aligned (0: none is needed).
+ */
+typedef struct sjvp_packed {
+    const void *q, *k, *v;
+    void* o;
+    const void* dO;
+    void *dq, *dk, *dv;
+    int64_t strides[SJVP_S_COUNT * 2];
+    float* lse;
+    const int32_t* offsets;
+    void* workspace;
+    size_t workspace_bytes;
+    int32_t B, T, Hq, Hkv, D, causal;
+    float scale;
+} sjvp_packed;
+size_t sjvp_packed_workspace_bytes(const sjvp_packed* t, int backward);
+int sjvp_packed_fwd(const sjvp_packed* t, int dtype, void* stream);
+int sjvp_packed_bwd(const sjvp_packed* t, int dtype, void* stream);
+
+/*
+ * A cache in pages.  k_pages, v_pages: [pages, Hkv, page_size, D] with the byte strides (page, head, row) page_strides[0..2], the same of both;
+ * numbers of the tensors' 16-bit type (D a multiple of 8), or, with k_scales and v_scales, of 8 bits (e4m3; D a multiple of 16), of which each 32 columns
+ * of a row have a power of two 2^(code - 127), code an unsigned byte of [pages, Hkv, page_size, ceil(D/32)] with the byte strides
+ * page_strides[3..5].  Rows of k_pages and v_pages start on 16-byte boundaries.
+ *   tables   device array [B][table_pages] with the row stride table_stride: position x of sequence b stands in row x % page_size of page
+ *       tables[b][x / page_size].  A number that is none of the cache's pages reads as zeros and takes no writes.
+ *   lengths  device array [B]: the tokens that the cache holds of a sequence, those of the call among them; clamped to what the table has.
+ *   offsets  as above, of the call's new tokens: the last offsets[b+1] - offsets[b] ones of sequence b.  NULL: T = B, one each.
+ * sjvp_paged_write: k, v [T,Hkv,D] (strides (head, row) of SJVP_P_K, SJVP_P_V) to their places in the pages.  A page that is written to belongs to
+ *   one sequence.  8 bits: the exponent of 32 columns is the least one by which none of their finite numbers goes beyond 448, within -117 .. 120
+ *   (bf16) or -15 .. 8 (fp16), so that every 8-bit number stands for one of the 16-bit type; numbers are rounded to nearest even, and at the
+ *   largest exponent end at 240; what is not finite becomes NaN.
+ * sjvp_paged_read: what the cache holds, to k, v [B,size,Hkv,D] (strides (head, row, batch) at SJVP_P_K, SJVP_P_V), zeros behind a length.
+ * sjvp_paged_attention: q, o [T,Hq,D]: the new tokens on all that the cache holds of their sequence, causal; token i of n new ones has the position
+ *   length - n + i; one in front of position 0 sees nothing, and o is zero.
+ * strides[3*i + {0,1,2}]: (head, row, batch) strides in elements of tensor i of sjvp_paged_tensor.  The workspace of sjvp_paged_attention is
+ * device memory of sjvp_paged_workspace_bytes() bytes, 16-byte aligned (0: none is needed).  No counterpart in the reference.
+ */
+enum sjvp_paged_tensor { SJVP_P_Q = 0, SJVP_P_O, SJVP_P_K, SJVP_P_V, SJVP_P_COUNT };
+typedef struct sjvp_paged {
+    const void* q;
+    void *o, *k, *v;
+    int64_t strides[SJVP_P_COUNT * 3];
+    void *k_pages, *v_pages, *k_scales, *v_scales;
+    int64_t page_strides[6];
+    const int32_t *tables, *lengths, *offsets;
+    int64_t table_stride;
+    void* workspace;
+    size_t workspace_bytes;
+    int32_t pages, page_size, table_pages;
+    int32_t B, T, Hq, Hkv, D, size;
+    float scale;
+} sjvp_paged;
+size_t sjvp_paged_workspace_bytes(const sjvp_paged* t);
+int sjvp_paged_write(const sjvp_paged* t, int dtype, void* stream);
+int sjvp_paged_read(const sjvp_paged* t, int dtype, void* stream);
+int sjvp_paged_attention(const sjvp_paged* t, int dtype, void* stream);
 
 /* Static, NUL-terminated description of a status code. */
 const char* sjvp_strerror(int status);

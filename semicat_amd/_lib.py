@@ -28,6 +28,7 @@ SJVP_ERR_ROTARY = -9
 SJVP_ERR_SCALE = -10
 SJVP_ERR_SCRATCH = -11
 SJVP_ERR_BUCKETS = -12
+SJVP_ERR_PAGES = -13
 SJVP_NOALLOC_MAX_ROWS = 1 << 20
 
 SJVP_BWD_ROW = 1
@@ -44,6 +45,9 @@ SJVP_CTX_MAX_BUCKETS = 256
 SJVP_CTX_MAX_DISTANCE = 1024
 SJVP_CTX_MAX_POSITION = 1 << 29
 
+S_TENSORS = ("q", "k", "v", "o", "dO", "dq", "dk", "dv")
+P_TENSORS = ("q", "o", "k", "v")
+
 SJVP_REPAIR_OFF = 0
 SJVP_REPAIR_AUTO = 1
 SJVP_REPAIR_ALWAYS = 2
@@ -51,6 +55,8 @@ SJVP_REPAIR_ALWAYS = 2
 EXPORTS = ("sjvp_fwd", "sjvp_bwd", "sjvp_bwd_parts", "sjvp_bwd_noalloc", "sjvp_fwd_rotary", "sjvp_bwd_rotary", "sjvp_bwd_workspace_bytes", "sjvp_rope",
            "sjvp_adaln_fwd", "sjvp_adaln_bwd", "sjvp_adaln_workspace_floats", "sjvp_gelu", "sjvp_cast",
            "sjvp_ctx_fwd", "sjvp_ctx_bwd", "sjvp_ctx_workspace_bytes",
+           "sjvp_packed_fwd", "sjvp_packed_bwd", "sjvp_packed_workspace_bytes",
+           "sjvp_paged_write", "sjvp_paged_read", "sjvp_paged_attention", "sjvp_paged_workspace_bytes",
            "sjvp_set_row_sum_repair", "sjvp_strerror", "sjvp_version", "sjvp_build_id")
 
 
@@ -73,6 +79,23 @@ class Ctx(ctypes.Structure):
                 + [("bucket_first", ctypes.c_void_p), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t)]
                 + [(n, ctypes.c_int32) for n in ("query_start0", "table_dtype", "buckets", "bidirectional", "causal",
                                                  "B", "Hq", "Hkv", "Lq", "Lk", "D")]
+                + [("scale", ctypes.c_float)])
+
+
+class Packed(ctypes.Structure):
+    """``struct sjvp_packed``."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in S_TENSORS] + [("strides", ctypes.c_int64 * (2 * len(S_TENSORS)))]
+                + [(n, ctypes.c_void_p) for n in ("lse", "offsets", "workspace")] + [("workspace_bytes", ctypes.c_size_t)]
+                + [(n, ctypes.c_int32) for n in ("B", "T", "Hq", "Hkv", "D", "causal")] + [("scale", ctypes.c_float)])
+
+
+class Paged(ctypes.Structure):
+    """``struct sjvp_paged``."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in P_TENSORS] + [("strides", ctypes.c_int64 * (3 * len(P_TENSORS)))]
+                + [(n, ctypes.c_void_p) for n in ("k_pages", "v_pages", "k_scales", "v_scales")] + [("page_strides", ctypes.c_int64 * 6)]
+                + [(n, ctypes.c_void_p) for n in ("tables", "lengths", "offsets")]
+                + [("table_stride", ctypes.c_int64), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t)]
+                + [(n, ctypes.c_int32) for n in ("pages", "page_size", "table_pages", "B", "T", "Hq", "Hkv", "D", "size")]
                 + [("scale", ctypes.c_float)])
 
 
@@ -136,6 +159,14 @@ def load() -> ctypes.CDLL:
             lib.sjvp_ctx_fwd.restype = lib.sjvp_ctx_bwd.restype = i
             lib.sjvp_ctx_workspace_bytes.argtypes = [ctx, i]
             lib.sjvp_ctx_workspace_bytes.restype = ctypes.c_size_t
+            packed, paged = ctypes.POINTER(Packed), ctypes.POINTER(Paged)
+            lib.sjvp_packed_fwd.argtypes = lib.sjvp_packed_bwd.argtypes = [packed, i, vp]
+            lib.sjvp_packed_workspace_bytes.argtypes = [packed, i]
+            lib.sjvp_paged_write.argtypes = lib.sjvp_paged_read.argtypes = lib.sjvp_paged_attention.argtypes = [paged, i, vp]
+            lib.sjvp_paged_workspace_bytes.argtypes = [paged]
+            for fn in (lib.sjvp_packed_fwd, lib.sjvp_packed_bwd, lib.sjvp_paged_write, lib.sjvp_paged_read, lib.sjvp_paged_attention):
+                fn.restype = i
+            lib.sjvp_packed_workspace_bytes.restype = lib.sjvp_paged_workspace_bytes.restype = ctypes.c_size_t
             lib.sjvp_set_row_sum_repair.argtypes = [i]
             lib.sjvp_set_row_sum_repair.restype = i
             lib.sjvp_strerror.argtypes = [i]

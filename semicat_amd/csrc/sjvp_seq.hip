@@ -1,0 +1,178 @@
+// C ABI of the attention over packed sequences and over a paged cache: checks, how the work is split, and the launches.
+#include <climits>
+#include <cmath>
+
+#include "sjvp_seq_launch.hpp"
+
+namespace sjvp {
+namespace {
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+constexpr int64_t kMostThreads = UINT32_MAX;  // of a launch
+
+bool strides_ok(const CtxView& v, int rows) { return rows <= 1 || (v.sl >= 0 && v.sl < 1 << 24); }
+
+// what the calls have in common
+int seq_common(SeqParams& p, int B, int T, int Hq, int Hkv, int D, float scale) {
+    if (B < 1 || T < 1 || Hq < 1 || Hkv < 1 || Hq % Hkv || B > kCtxMost || T > kCtxMost || (int64_t)T * Hq > INT_MAX) return SJVP_ERR_SHAPE;
+    if (D < 16 || D > 128) return SJVP_ERR_HEAD_DIM;
+    if (!(scale >= 0.0f) || !std::isfinite(scale)) return SJVP_ERR_SCALE;
+    p.B = B, p.T = T, p.Hq = Hq, p.Hkv = Hkv, p.G = Hq / Hkv, p.D = D;
+    p.scale = scale == 0.0f ? 1.0f / std::sqrt(static_cast<float>(D)) : scale;
+    p.c = p.scale * kLog2e;
+    // blocks of 32 rows over all heads and splits, 256 threads each
+    return (seq_slots(p, p.G, 32) * Hkv) * 64 > kMostThreads / 256 * 64 ? SJVP_ERR_SHAPE : SJVP_OK;
+}
+
+int packed_params(const sjvp_packed* t, SeqParams& p) {
+    if (!t) return SJVP_ERR_NULL;
+    const int rc = seq_common(p, t->B, t->T, t->Hq, t->Hkv, t->D, t->scale);
+    if (rc != SJVP_OK) return rc;
+    CtxView* views[SJVP_S_COUNT] = {&p.q, &p.k, &p.v, &p.o, &p.g, &p.dq, &p.dk, &p.dv};
+    const void* ptrs[SJVP_S_COUNT] = {t->q, t->k, t->v, t->o, t->dO, t->dq, t->dk, t->dv};
+    for (int i = 0; i < SJVP_S_COUNT; ++i) *views[i] = {static_cast<elem_t*>(const_cast<void*>(ptrs[i])), 0, t->strides[2 * i], t->strides[2 * i + 1]};
+    for (CtxView* v : {&p.q, &p.k, &p.v, &p.g}) {
+        if (v->ptr && !strides_ok(*v, t->T)) return SJVP_ERR_SHAPE;
+        if (t->T == 1) v->sl = t->D;  // (one row: no stride)
+    }
+    p.lse = t->lse, p.offsets = t->offsets, p.causal = t->causal != 0;
+    return SJVP_OK;
+}
+
+int paged_params(const sjvp_paged* t, SeqParams& p, int T) {
+    if (!t) return SJVP_ERR_NULL;
+    const int rc = seq_common(p, t->B, T, t->Hq, t->Hkv, t->D, t->scale);
+    if (rc != SJVP_OK) return rc;
+    const bool e4m3 = t->k_scales || t->v_scales;
+    if (t->pages < 1 || t->page_size < 1 || t->page_size > kCtxMost || t->table_pages < 1 || t->D % (e4m3 ? 16 : 8)) return SJVP_ERR_PAGES;
+    if (!t->k_pages || !t->v_pages || !t->tables || !t->lengths || !t->k_scales != !t->v_scales) return SJVP_ERR_NULL;
+    for (int i = 0; i < 3; ++i)
+        if (t->page_strides[i] % 16 || t->page_strides[i] < 0) return SJVP_ERR_PAGES;
+    if (reinterpret_cast<uintptr_t>(t->k_pages) % 16 || reinterpret_cast<uintptr_t>(t->v_pages) % 16) return SJVP_ERR_PAGES;
+    CtxView* views[SJVP_P_COUNT] = {&p.q, &p.o, &p.k, &p.v};
+    const void* ptrs[SJVP_P_COUNT] = {t->q, t->o, t->k, t->v};
+    for (int i = 0; i < SJVP_P_COUNT; ++i)
+        *views[i] = {static_cast<elem_t*>(const_cast<void*>(ptrs[i])), t->strides[3 * i + 2], t->strides[3 * i], t->strides[3 * i + 1]};
+    p.lengths = t->lengths, p.offsets = t->offsets, p.causal = 1;
+    SeqPages& g = p.pages;
+    g.k = static_cast<unsigned char*>(t->k_pages), g.v = static_cast<unsigned char*>(t->v_pages);
+    g.ks = static_cast<unsigned char*>(t->k_scales), g.vs = static_cast<unsigned char*>(t->v_scales);
+    g.sp = t->page_strides[0], g.sh = t->page_strides[1], g.sr = t->page_strides[2];
+    g.scale_sp = t->page_strides[3], g.scale_sh = t->page_strides[4], g.scale_sr = t->page_strides[5];
+    g.table = t->tables, g.table_stride = t->table_stride;
+    g.pages = t->pages, g.size = t->page_size;
+    g.capacity = (int)std::min<int64_t>((int64_t)t->table_pages * t->page_size, kCtxMost);
+    g.shift = 0;
+    while ((1u << g.shift) < (uint32_t)g.size) ++g.shift;
+    g.magic = (uint32_t)(((uint64_t(1) << (31 + g.shift)) + g.size - 1) / g.size);
+    return SJVP_OK;
+}
+
+// How a call of the paged attention is served.  seq_few splits long sequences over workgroups and takes any number of rows; seq_fwd, whose
+// four waves share their tiles, takes the longer sequences where blocks of 128 rows fill half of the compute units.
+struct PagedPlan {
+    bool few = true, many = false;
+    int splits = 1;
+    size_t stat = 0, part = 0, used = 0, total = 0;  // floats
+};
+
+PagedPlan paged_plan(const SeqParams& p) {
+    PagedPlan plan;
+    const int64_t rows = (int64_t)p.T * p.G;
+    plan.many = p.T > p.B && 2 * ceil_div(rows, kCtxOwned) * p.Hkv > compute_units();
+    const int64_t blocks = (p.B + rows / 32) * p.Hkv;
+    plan.splits = (int)std::max<int64_t>(1, std::min<int64_t>({8 * (int64_t)compute_units() / blocks, p.pages.capacity / 512, 64}));
+    if (plan.splits > 1) {
+        const auto take = [&](int64_t floats) {
+            const size_t at = plan.total;
+            plan.total += (size_t)(floats + 3) / 4 * 4;
+            return at;
+        };
+        const int64_t places = p.Hkv * (plan.many ? (int64_t)(p.B + 2) * kSeqFew : rows);
+        plan.stat = take(2 * plan.splits * places);
+        plan.part = take(plan.splits * places * ctx_padded(p.D));
+        plan.used = take(places);
+    }
+    return plan;
+}
+
+int seq_workspace(void* ws, size_t bytes, size_t floats) {
+    return floats == 0 || (ws && bytes >= 4 * floats && reinterpret_cast<uintptr_t>(ws) % 16 == 0) ? SJVP_OK : SJVP_ERR_WORKSPACE;
+}
+
+}  // namespace
+}  // namespace sjvp
+
+extern "C" {
+
+using namespace sjvp;
+
+size_t sjvp_packed_workspace_bytes(const sjvp_packed* t, int backward) {
+    SeqParams p{};
+    return backward && packed_params(t, p) == SJVP_OK ? 4 * 3 * (size_t)p.Hq * p.T : 0;
+}
+
+int sjvp_packed_fwd(const sjvp_packed* t, int dtype, void* stream) {
+    SeqParams p{};
+    const int rc = packed_params(t, p);
+    if (rc != SJVP_OK) return rc;
+    if (dtype != SJVP_BF16 && dtype != SJVP_FP16) return SJVP_ERR_DTYPE;
+    if (!t->q || !t->k || !t->v || !t->o || !t->offsets) return SJVP_ERR_NULL;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    return dtype == SJVP_BF16 ? seq_packed_fwd<Bf16>(p, s) : seq_packed_fwd<Fp16>(p, s);
+}
+
+int sjvp_packed_bwd(const sjvp_packed* t, int dtype, void* stream) {
+    SeqParams p{};
+    const int rc = packed_params(t, p);
+    if (rc != SJVP_OK) return rc;
+    if (dtype != SJVP_BF16 && dtype != SJVP_FP16) return SJVP_ERR_DTYPE;
+    if (!t->q || !t->k || !t->v || !t->o || !t->dO || !t->dq || !t->dk != !t->dv || !t->lse || !t->offsets) return SJVP_ERR_NULL;
+    if (seq_workspace(t->workspace, t->workspace_bytes, 3 * (size_t)p.Hq * p.T) != SJVP_OK) return SJVP_ERR_WORKSPACE;
+    p.folded = static_cast<float*>(t->workspace);
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    return dtype == SJVP_BF16 ? seq_packed_bwd<Bf16>(p, s) : seq_packed_bwd<Fp16>(p, s);
+}
+
+size_t sjvp_paged_workspace_bytes(const sjvp_paged* t) {
+    SeqParams p{};
+    return t && paged_params(t, p, t->T) == SJVP_OK ? 4 * paged_plan(p).total : 0;
+}
+
+int sjvp_paged_write(const sjvp_paged* t, int dtype, void* stream) {
+    SeqParams p{};
+    const int rc = t ? paged_params(t, p, t->T) : SJVP_ERR_NULL;
+    if (rc != SJVP_OK) return rc;
+    if (dtype != SJVP_BF16 && dtype != SJVP_FP16) return SJVP_ERR_DTYPE;
+    if (!t->k || !t->v || (!t->offsets && t->T != t->B)) return SJVP_ERR_NULL;
+    return paged_copy(p, p.pages.ks, dtype == SJVP_FP16, true, static_cast<hipStream_t>(stream));
+}
+
+int sjvp_paged_read(const sjvp_paged* t, int dtype, void* stream) {
+    SeqParams p{};
+    const int rc = paged_params(t, p, 1);
+    if (rc != SJVP_OK) return rc;
+    if (dtype != SJVP_BF16 && dtype != SJVP_FP16) return SJVP_ERR_DTYPE;
+    if (!t->k || !t->v) return SJVP_ERR_NULL;
+    if (t->size < 1 || t->size > kCtxMost || (int64_t)t->B * t->size > kMostThreads / 64 - kCtxWaves) return SJVP_ERR_SHAPE;
+    p.most = t->size;
+    return paged_copy(p, p.pages.ks, dtype == SJVP_FP16, false, static_cast<hipStream_t>(stream));
+}
+
+int sjvp_paged_attention(const sjvp_paged* t, int dtype, void* stream) {
+    SeqParams p{};
+    const int rc = t ? paged_params(t, p, t->T) : SJVP_ERR_NULL;
+    if (rc != SJVP_OK) return rc;
+    if (dtype != SJVP_BF16 && dtype != SJVP_FP16) return SJVP_ERR_DTYPE;
+    if (!t->q || !t->o || (!t->offsets && t->T != t->B)) return SJVP_ERR_NULL;
+    const PagedPlan plan = paged_plan(p);
+    if (seq_workspace(t->workspace, t->workspace_bytes, plan.total) != SJVP_OK) return SJVP_ERR_WORKSPACE;
+    float* ws = static_cast<float*>(t->workspace);
+    p.splits = plan.splits;
+    p.stat = ws + plan.stat, p.part = ws + plan.part, p.used = reinterpret_cast<int*>(ws + plan.used);
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    return dtype == SJVP_BF16 ? seq_paged<Bf16>(p, p.pages.ks, plan.few, plan.many, s) : seq_paged<Fp16>(p, p.pages.ks, plan.few, plan.many, s);
+}
+
+}  // extern "C"

@@ -1,0 +1,308 @@
+// Attention over packed sequences and over a paged cache: parameters and device building blocks (kernels: sjvp_seq_fwd.hpp,
+// sjvp_seq_bwd.hpp, sjvp_paged.hip; tile algebra: sjvp_ctx.hpp).
+//
+//   s[i][j] = scale q_i.k_j    for the keys j of the query's own sequence, causal: up to its own position
+//   p = softmax over j,  o_i = sum_j p[i][j] v_j
+//
+// Sequences stand one behind the other in tensors of T rows; offsets [B+1] say where.  The rows in front of the first one and behind
+// the last one are two more segments, without keys, so that every row of a result is written by the same code: segment 0 is
+// [0, offsets[0]), segment x in 1 .. B is sequence x - 1, segment B + 1 ends at T.  Offsets are clamped to T; what is not ascending
+// gives rows of no use, none out of bounds.
+//
+// Which segment a workgroup serves is found on the device, so that the host reads no lengths: blocks of R rows of a segment take the slots
+//   floor(offset / R) + segment, ...
+// which never meet, since floor(a / R) + ceil(n / R) <= floor((a + n) / R) + 1; the slot of a workgroup gives its segment by a search of 64
+// places at a time.  T / R + B + 2 slots hold all blocks, at most B + 2 of them idle.
+#pragma once
+#include "sjvp_ctx.hpp"
+
+namespace sjvp {
+
+// Pages of a cache: [pages, heads, size, D] numbers of 16 or 8 bits, the latter with a power of two for each 32 columns (8-bit exponents
+// [pages, heads, size, ceil(D / 32)]).  Strides in bytes, the same of K and V.  Position x of sequence b stands in row x % size of page
+// table[b][x / size]; a page number that the cache has not reads as zeros.
+struct SeqPages {
+    unsigned char *k, *v, *ks, *vs;
+    int64_t sp, sh, sr, scale_sp, scale_sh, scale_sr;
+    const int* table;
+    int64_t table_stride;
+    int pages, size, capacity;  // capacity: positions that a row of the table has
+    uint32_t magic, shift;      // x / size = mulhi(2 x, magic) >> shift below 2^30
+    __device__ __forceinline__ int page_of(int x) const { return (int)(__umulhi(2u * (uint32_t)x, magic) >> shift); }
+};
+
+constexpr int kSeqFew = 64;  // rows of a sequence that seq_few serves beside seq_fwd
+
+struct SeqParams {
+    CtxView q, k, v, o, g, dq, dk, dv;  // [T,H,D], sb unused
+    float *lse, *folded;                // [Hq,T][2]: (m, l) of each row; [3][Hq,T]: row_stat_folded, -delta
+    float *part, *stat;                 // sums of split work: [splits][seq_places] of HD floats, and their (maximum, sum)
+    int* used;                          // splits that a row's sums stand in (0: in none)
+    const int *offsets, *lengths;       // offsets null: one row each
+    int B, T, Hq, Hkv, G, D, causal;
+    float scale, c;                     // c = scale * log2(e)
+    int slots, splits;
+    int least, most;                    // query rows (of all heads of a group) of the sequences that a launch serves
+    SeqPages pages;
+};
+
+__device__ __forceinline__ int seq_offset(const SeqParams& p, int x) {
+    if (x == 0) return 0;
+    if (x >= p.B + 2) return p.T;
+    return min(max(p.offsets ? p.offsets[x - 1] : x - 1, 0), p.T);
+}
+
+// The block of R rows (of `heads` rows to a token) that a workgroup serves.
+struct SeqBlock {
+    int segment, token, tokens, row0;  // first token and number of tokens of the segment; first row of the block within it
+    bool some;
+};
+template <int R>
+__device__ __forceinline__ SeqBlock seq_block(const SeqParams& p, int slot, int heads, int lane) {
+    int lo = 0, hi = p.B + 2;  // the segment lies in [lo, hi)
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 63) / 64, x = lo + lane * step;
+        const bool there = x < hi && seq_offset(p, x) * heads / R + x <= slot;
+        const int n = __popcll(__builtin_amdgcn_ballot_w64(there || lane == 0));
+        lo += (n - 1) * step;
+        hi = min(hi, lo + step);
+    }
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    SeqBlock b;
+    b.segment = lo;
+    b.token = __builtin_amdgcn_readfirstlane(seq_offset(p, lo));
+    b.tokens = max(0, __builtin_amdgcn_readfirstlane(seq_offset(p, lo + 1)) - b.token);
+    b.row0 = (slot - (b.token * heads / R + lo)) * R;
+    b.some = b.row0 >= 0 && b.row0 < b.tokens * heads;  // (descending offsets may lead to a segment that begins behind the slot)
+    return b;
+}
+
+// Keys of a segment and the position of its first query among them.
+template <bool PAGED>
+struct SeqKeys {
+    int keys, start;
+    __device__ __forceinline__ SeqKeys(const SeqParams& p, const SeqBlock& b) {
+        const bool sequence = b.segment >= 1 && b.segment <= p.B;
+        if constexpr (PAGED) {
+            keys = sequence ? min(max(p.lengths[b.segment - 1], 0), p.pages.capacity) : 0;
+            start = keys - b.tokens;
+        } else {
+            keys = sequence ? b.tokens : 0;
+            start = 0;
+        }
+    }
+    // keys that query i sees
+    __device__ __forceinline__ int seen(const SeqParams& p, int i) const { return p.causal ? max(0, min(keys, start + i + 1)) : keys; }
+};
+
+// Two 8-bit numbers of a word, times a power of two, as two 16-bit ones.
+template <typename T>
+__device__ __forceinline__ uint32_t from_e4m3(uint32_t word, float scale, bool high) {
+    if constexpr (std::is_same_v<T, Bf16>) {
+        return high ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word, scale, true))
+                    : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word, scale, false));
+    } else {
+        return high ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(word, scale, true))
+                    : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(word, scale, false));
+    }
+}
+template <typename T>
+__device__ __forceinline__ u32x4 from_e4m3_8(uint32_t a, uint32_t b, float scale) {
+    return u32x4{from_e4m3<T>(a, scale, false), from_e4m3<T>(a, scale, true), from_e4m3<T>(b, scale, false), from_e4m3<T>(b, scale, true)};
+}
+// 2^(code - 127)
+__device__ __forceinline__ float scale_of(uint32_t code) { return __uint_as_float(code << 23); }
+
+// 16 bytes of zeros, for the lanes of a copy that have no row.
+static __device__ const u32x4 kZeroPiece = {0u, 0u, 0u, 0u};
+
+// Tiles of 64 keys and values on their way to LDS by four waves.  look() is called a tile ahead of request(), request() ahead of use,
+// deliver() where the places are read next, behind it arrived() and a barrier.
+// From a contiguous tensor (rows of a segment):
+template <int HD, bool DMA>
+struct SeqFeed {
+    static constexpr bool kDma = DMA;
+    TileFeed<HD, DMA> kf, vf;
+    const elem_t *k, *v;
+    __device__ __forceinline__ SeqFeed(const SeqParams& p, const SeqBlock& b, int hk, int tid)
+        : kf(p.k.sl, p.D, tid), vf(p.v.sl, p.D, tid), k(p.k.head(0, hk) + b.token * p.k.sl), v(p.v.head(0, hk) + b.token * p.v.sl) {}
+    __device__ __forceinline__ void look(const SeqParams&, int, int) {}
+    __device__ __forceinline__ void request(const SeqParams& p, int t, int keys, elem_t* kp, elem_t* vp, int wave) {
+        kf.request(k + (int64_t)t * kCtxTile * p.k.sl, p.k.sl, keys - t * kCtxTile, p.D, kp, wave);
+        vf.request(v + (int64_t)t * kCtxTile * p.v.sl, p.v.sl, keys - t * kCtxTile, p.D, vp, wave);
+    }
+    __device__ __forceinline__ void deliver(const SeqParams& p, elem_t* kp, elem_t* vp, int tid) {
+        kf.deliver(kp, p.D, tid), vf.deliver(vp, p.D, tid);
+    }
+    __device__ __forceinline__ void arrived() { kf.arrived(); }
+};
+
+// From the pages of a cache, 16-bit numbers (D is a multiple of 8 and rows are aligned): every lane of an LDS-DMA copy has an address of its
+// own, so a tile may lie in any number of pages.
+template <int HD, bool DMA>
+struct PageFeed {
+    static constexpr bool kDma = DMA;
+    static constexpr int CH = HD / 8, N = kCtxTile * CH / kCtxThreads;
+    u32x4 kr[DMA ? 1 : N], vr[DMA ? 1 : N];
+    int page[N], row[N];
+    const int* table;
+    int64_t head;
+    int x;
+    __device__ __forceinline__ PageFeed(const SeqParams& p, const SeqBlock& b, int hk, int tid)
+        : table(p.pages.table + (b.segment - 1) * p.pages.table_stride), head(hk * p.pages.sh), x(tid) {}
+    __device__ __forceinline__ void look(const SeqParams& p, int t, int keys) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int key = t * kCtxTile + (x + kCtxThreads * i) / CH, at = p.pages.page_of(key);
+            page[i] = key < keys ? table[at] : -1;
+            row[i] = key - at * p.pages.size;
+        }
+    }
+    __device__ __forceinline__ void request(const SeqParams& p, int, int, elem_t* kp, elem_t* vp, int wave) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int r = (x + kCtxThreads * i) / CH, c = DMA ? (x + kCtxThreads * i) % CH ^ swz<HD>(r) : (x + kCtxThreads * i) % CH;
+            const bool ok = (uint32_t)page[i] < (uint32_t)p.pages.pages && 8 * c < p.D;
+            const int64_t at = page[i] * p.pages.sp + head + row[i] * p.pages.sr + 16 * c;
+            const void* none = &kZeroPiece;
+            const void *from_k = ok ? p.pages.k + at : none, *from_v = ok ? p.pages.v + at : none;
+            if constexpr (DMA) {
+                dma16(from_k, lds_addr(kp) + 16 * (64 * wave + kCtxThreads * i));
+                dma16(from_v, lds_addr(vp) + 16 * (64 * wave + kCtxThreads * i));
+            } else {
+                kr[i] = *static_cast<const u32x4*>(from_k), vr[i] = *static_cast<const u32x4*>(from_v);
+            }
+        }
+    }
+    __device__ __forceinline__ void deliver(const SeqParams&, elem_t* kp, elem_t* vp, int) {
+        if constexpr (!DMA) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int y = x + kCtxThreads * i, at = (y / CH) * Tile<HD, false>::kLd + 8 * (y % CH);
+                *reinterpret_cast<u32x4*>(kp + at) = kr[i], *reinterpret_cast<u32x4*>(vp + at) = vr[i];
+            }
+        }
+    }
+    __device__ __forceinline__ void arrived() {
+        if constexpr (DMA) __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+    }
+};
+
+// From pages of 8-bit numbers (D is a multiple of 16), which become 16-bit ones on their way, once for the four waves.
+template <typename T, int HD>
+struct PageFeed8 {
+    static constexpr bool kDma = false;
+    static constexpr int PC = HD / 16, N = (kCtxTile * PC + kCtxThreads - 1) / kCtxThreads;
+    u32x4 kr[N], vr[N];
+    uint32_t ks[N], vs[N];
+    int page[N], row[N];
+    const int* table;
+    int64_t head, scale_head;
+    int x;
+    __device__ __forceinline__ PageFeed8(const SeqParams& p, const SeqBlock& b, int hk, int tid)
+        : table(p.pages.table + (b.segment - 1) * p.pages.table_stride), head(hk * p.pages.sh), scale_head(hk * p.pages.scale_sh), x(tid) {}
+    __device__ __forceinline__ void look(const SeqParams& p, int t, int keys) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int r = (x + kCtxThreads * i) / PC, key = t * kCtxTile + r, at = p.pages.page_of(key);
+            page[i] = r < kCtxTile && key < keys ? table[at] : -1;
+            row[i] = key - at * p.pages.size;
+        }
+    }
+    __device__ __forceinline__ void request(const SeqParams& p, int, int, elem_t*, elem_t*, int) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int c = (x + kCtxThreads * i) % PC;
+            const bool ok = (uint32_t)page[i] < (uint32_t)p.pages.pages && 16 * c < p.D;
+            const int64_t at = page[i] * p.pages.sp + head + row[i] * p.pages.sr + 16 * c;
+            const int64_t sat = page[i] * p.pages.scale_sp + scale_head + row[i] * p.pages.scale_sr + c / 2;
+            const void* none = &kZeroPiece;
+            kr[i] = *static_cast<const u32x4*>(ok ? p.pages.k + at : none), vr[i] = *static_cast<const u32x4*>(ok ? p.pages.v + at : none);
+            ks[i] = *static_cast<const uint8_t*>(ok ? p.pages.ks + sat : none), vs[i] = *static_cast<const uint8_t*>(ok ? p.pages.vs + sat : none);
+        }
+    }
+    __device__ __forceinline__ void deliver(const SeqParams&, elem_t* kp, elem_t* vp, int) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int y = x + kCtxThreads * i, at = (y / PC) * Tile<HD, false>::kLd + 16 * (y % PC);
+            if (kCtxTile * PC % kCtxThreads && y >= kCtxTile * PC) break;
+            const float a = scale_of(ks[i]), b = scale_of(vs[i]);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                *reinterpret_cast<u32x4*>(kp + at + 8 * j) = from_e4m3_8<T>(kr[i][2 * j], kr[i][2 * j + 1], a);
+                *reinterpret_cast<u32x4*>(vp + at + 8 * j) = from_e4m3_8<T>(vr[i][2 * j], vr[i][2 * j + 1], b);
+            }
+        }
+    }
+    __device__ __forceinline__ void arrived() {}
+};
+
+// Running maximum and sum of a row, as in the attention on keys of another length: raised only past 2^8.
+template <int HD>
+struct SeqSums {
+    f32x16 acc[HD / 32];
+    float m, ref, l;  // maximum (-inf: no key yet), what is subtracted (finite), sum of this lane's half
+
+    __device__ __forceinline__ SeqSums() : acc{}, m(-INFINITY), ref(0.0f), l(0.0f) {}
+
+    // Scores of 32 N keys to exponentials; keys from `left` on are not seen (masked).
+    template <bool MASKED, int N>
+    __device__ __forceinline__ void take(f32x16 (&s)[N], float c, int left, int h) {
+        if constexpr (MASKED) {
+#pragma unroll
+            for (int u = 0; u < N; ++u)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (32 * u + tile_row(r, 0) >= left - 4 * h) s[u][r] = -INFINITY;
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int u = 0; u < N; ++u)
+#pragma unroll
+            for (int r = u ? 0 : 1; r < 16; ++r) top = fmaxf(top, s[u][r]);
+        top *= c;
+        if (__builtin_amdgcn_ballot_w64(top > m + 8.0f)) {
+            const float grown = fmaxf(m, halves_max(top));
+            const float now = grown == -INFINITY ? 0.0f : grown;
+            const float f = m == -INFINITY ? 0.0f : fast_exp2(ref - now);
+            m = grown, ref = now;
+            l *= f;
+#pragma unroll
+            for (int dt = 0; dt < HD / 32; ++dt) acc[dt] *= f;
+        }
+        float sum = 0.0f;
+#pragma unroll
+        for (int u = 0; u < N; ++u)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[u][r] = fast_exp2(__builtin_fmaf(s[u][r], c, -ref));
+                sum += s[u][r];
+            }
+        l += sum;
+    }
+};
+
+// Sums of a wave's own 32 rows, OUT^T, as rows in memory whose places `at` gives, through the wave's own LDS region of [32][HD + 8].
+template <typename T, int HD, typename F>
+__device__ __forceinline__ void store_rows_at(const f32x16* acc, float factor, int rows, elem_t* region, int lane, int D, F&& at) {
+    elem_t* mine = region + (lane & 31) * (HD + 8) + 4 * (lane >> 5);
+#pragma unroll
+    for (int dt = 0; dt < HD / 32; ++dt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float x[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = factor == 0.0f ? 0.0f : acc[dt][4 * i + j] * factor;  // (sums of rows without a result may be NaN)
+            *reinterpret_cast<u32x2*>(mine + 32 * dt + 8 * i) = u32x2{T::pack2(x[0], x[1]), T::pack2(x[2], x[3])};
+        }
+    wave_exchange();
+    constexpr int CH = HD / 8;
+#pragma unroll
+    for (int x0 = 0; x0 < 32 * CH; x0 += 64) {
+        const int x = x0 + lane, row = x / CH, c8 = 8 * (x % CH);
+        if (row < rows) store_chunk(at(row), *reinterpret_cast<const u32x4*>(region + row * (HD + 8) + c8), c8, D);
+    }
+    wave_exchange();
+}
+
+}  // namespace sjvp

@@ -1,0 +1,229 @@
+// Backward kernels of the attention over packed sequences (sjvp_seq.hpp).
+//
+//   dP = dO V^T,  delta = rowsum(dO * O),  dS = P (dP - delta)
+//   dQ = scale dS K,  dK = scale sum_heads dS^T Q,  dV = sum_heads P^T dO
+//
+// A row-owned launch (dQ, delta) and a column-owned one (dK, dV), both of which recompute P: 3 + 4 contractions against the 5 of a
+// single launch, whose dQ would be summed over workgroups by atomics in an order that changes from run to run.
+#pragma once
+#include "sjvp_seq_fwd.hpp"
+
+namespace sjvp {
+
+// 32 rows' numbers in LDS as the registers of a score tile
+__device__ __forceinline__ f32x16 seq_of_rows(const float* rows, int h) {
+    f32x16 x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const f32x4 four = *reinterpret_cast<const f32x4*>(rows + 8 * i + 4 * h);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[4 * i + j] = four[j];
+    }
+    return x;
+}
+
+// Row-owned: four waves of 32 query rows (of the heads that share a key head) share tiles of 64 keys.
+template <typename T, int HD, bool DMA>
+__global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 3 : 2) void seq_bwd_row(SeqParams p) {
+    if constexpr (DMA) __builtin_assume(p.D % 8 == 0);
+    extern __shared__ __align__(16) unsigned char smem[];
+    constexpr int kTile = Tile<HD, DMA>::kElems;
+    elem_t* tiles = reinterpret_cast<elem_t*>(smem);  // K [2], V [2]
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+    const int hk = blockIdx.x % p.Hkv, slot = p.causal ? p.slots - 1 - (int)(blockIdx.x / p.Hkv) : blockIdx.x / p.Hkv;
+    const SeqBlock b = seq_block<kCtxOwned>(p, slot, p.G, lane);
+    if (!b.some) return;
+    const int all = b.tokens * p.G;
+    const SeqKeys<false> keys(p, b);
+    const int r0 = b.row0 + 32 * wave, rows = min(max(all - r0, 0), 32);
+    const SeqRow mine(p, hk, min(r0 + (lane & 31), all - 1));
+    const bool ok = (lane & 31) < rows;
+    const int limit = keys.seen(p, mine.token);
+    const int n = keys.seen(p, (min(b.row0 + kCtxOwned, all) - 1) / p.G), whole = keys.seen(p, b.row0 / p.G);
+    const int n_wave = rows > 0 ? keys.seen(p, (r0 + rows - 1) / p.G) : 0;
+    const int nt = (n + kCtxTile - 1) / kCtxTile;
+    SeqFeed<HD, DMA> feed(p, b, hk, tid);
+    const Tile<HD, DMA> at(lane);
+    const auto k_place = [&](int t) { return tiles + (t & 1) * kTile; };
+    const auto v_place = [&](int t) { return tiles + (2 + (t & 1)) * kTile; };
+    if (nt) feed.request(p, 0, n, k_place(0), v_place(0), wave);
+
+    const int64_t token = b.token + mine.token, stat = (int64_t)mine.hq * p.T + token;
+    const f32x2 ml = ok && limit > 0 ? *reinterpret_cast<const f32x2*>(p.lse + 2 * stat) : f32x2{0.0f, 0.0f};
+    const bool some = ml[1] != 0.0f;       // a row that sees no key has no gradient, whatever its cotangent,
+    const bool scored = some && limit != 1;  // one that sees one key none of its score: exactly none, not what rounding leaves
+    u32x4 own_q[HD / 16], own_g[HD / 16];
+    own_operands<HD>(own_q, p.q.head(0, mine.hq) + token * p.q.sl, ok, h, p.D);
+    own_operands<HD>(own_g, p.g.head(0, mine.hq) + token * p.g.sl, some, h, p.D);
+    float delta = 0.0f;
+    {
+        const elem_t* o = p.o.head(0, mine.hq) + token * p.o.sl;
+#pragma unroll
+        for (int c = 0; c < HD / 16; ++c) {
+            const u32x4 x = some ? load_chunk(o, 16 * c + 8 * h, p.D) : u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int e = 0; e < 32; e += 16) delta += T::to_float((elem_t)(own_g[c][j] >> e)) * T::to_float((elem_t)(x[j] >> e));
+        }
+        delta = halves_sum(delta);
+    }
+    if (h == 0 && ok) {
+        const int64_t every = (int64_t)p.Hq * p.T;
+        const f32x2 folded = row_stat_folded(ml);
+        p.folded[stat] = folded[0], p.folded[every + stat] = folded[1], p.folded[2 * every + stat] = -delta;
+    }
+    const f32x2 less_factor = row_stat(ml);
+    const float less = less_factor[0], factor = less_factor[1], less_delta = -delta * factor;  // P (dP - delta) = exponential * (factor dP + less_delta)
+    if (nt) feed.deliver(p, k_place(0), v_place(0), tid);
+    feed.arrived();
+    workgroup_barrier();
+    f32x16 acc[HD / 32] = {};
+    const auto tile = [&](int t, auto masked) {
+        const int key = t * kCtxTile;
+        const bool more = t + 1 < nt;
+        if (more) feed.request(p, t + 1, n, k_place(t + 1), v_place(t + 1), wave);
+        if (key < n_wave) {
+            f32x16 s[2], ds[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                s[u] = scores<T>(at, k_place(t), 32 * u, own_q);
+                ds[u] = scores<T>(at, v_place(t), 32 * u, own_g);
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    ds[u][r] = fast_exp2(__builtin_fmaf(s[u][r], p.c, -less)) * __builtin_fmaf(ds[u][r], factor, less_delta);
+                    if constexpr (decltype(masked)::value)
+                        if (32 * u + tile_row(r, 0) >= limit - key - 4 * h) ds[u][r] = 0.0f;
+                }
+                add_columns<T>(acc, at, k_place(t), 32 * u, ds[u]);
+            }
+        }
+        if (more) feed.deliver(p, k_place(t + 1), v_place(t + 1), tid);
+        feed.arrived();
+        workgroup_barrier();
+    };
+    const int free = min(whole / kCtxTile, nt);
+    int t = 0;
+    for (; t < free; ++t) tile(t, std::false_type{});
+    for (; t < nt; ++t) tile(t, std::true_type{});
+    store_rows_at<T, HD>(acc, scored ? p.scale : 0.0f, rows, tiles + wave * 32 * (HD + 8), lane, p.D, [&](int row) {
+        const SeqRow to(p, hk, r0 + row);
+        return p.dq.head(0, to.hq) + (int64_t)(b.token + to.token) * p.dq.sl;
+    });
+}
+
+// Column-owned: four waves of 32 keys share tiles of 64 query rows, over all heads that read the key head.
+template <typename T, int HD, bool DMA>
+__global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void seq_bwd_col(SeqParams p) {
+    if constexpr (DMA) __builtin_assume(p.D % 8 == 0);
+    extern __shared__ __align__(16) unsigned char smem[];
+    constexpr int kTile = Tile<HD, DMA>::kElems;
+    elem_t* tiles = reinterpret_cast<elem_t*>(smem);             // [2][Q, dO]
+    float* stats = reinterpret_cast<float*>(tiles + 4 * kTile);  // [2][row_stat_folded, -delta][64]
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+    const int hk = blockIdx.x % p.Hkv, slot = blockIdx.x / p.Hkv;
+    const SeqBlock b = seq_block<kCtxOwned>(p, slot, 1, lane);
+    if (!b.some) return;
+    const SeqKeys<false> keys(p, b);
+    const int k0 = b.row0 + 32 * wave, key = k0 + (lane & 31);
+    const bool ok = key < keys.keys;
+    u32x4 own_k[HD / 16], own_v[HD / 16];
+    own_operands<HD>(own_k, p.k.head(0, hk) + (int64_t)(b.token + key) * p.k.sl, ok, h, p.D);
+    own_operands<HD>(own_v, p.v.head(0, hk) + (int64_t)(b.token + key) * p.v.sl, ok, h, p.D);
+    // tiles of query rows that see a key of the workgroup, head by head
+    const int ta = p.causal ? b.row0 / kCtxTile : 0, tb = (keys.keys + kCtxTile - 1) / kCtxTile, per_head = max(0, tb - ta);
+    const int nx = p.G * per_head;
+
+    TileFeed<HD, DMA> qf(p.q.sl, p.D, tid), gf(p.g.sl, p.D, tid);
+    const Tile<HD, DMA> at(lane);
+    float stat = 0.0f;
+    const auto place = [&](int x) { return tiles + (x & 1) * 2 * kTile; };
+    const auto request = [&](int x) {
+        const int hq = hk * p.G + x / per_head, r0 = (ta + x % per_head) * kCtxTile;
+        const int64_t token = b.token + r0;
+        qf.request(p.q.head(0, hq) + token * p.q.sl, p.q.sl, b.tokens - r0, p.D, place(x), wave);
+        gf.request(p.g.head(0, hq) + token * p.g.sl, p.g.sl, b.tokens - r0, p.D, place(x) + kTile, wave);
+        if (tid < 3 * kCtxTile) {
+            const int i = tid & (kCtxTile - 1);
+            const float* from = p.folded + (tid / kCtxTile * (int64_t)p.Hq + hq) * p.T + token;
+            stat = r0 + i < b.tokens ? from[i] : tid < kCtxTile ? INFINITY : tid < 2 * kCtxTile ? 1.0f : 0.0f;
+        }
+    };
+    const auto deliver = [&](int x) {
+        qf.deliver(place(x), p.D, tid);
+        gf.deliver(place(x) + kTile, p.D, tid);
+        if (tid < 3 * kCtxTile) stats[(x & 1) * (kCtxStats / 2) + tid] = stat;
+    };
+    if (nx) {
+        request(0);
+        deliver(0);
+        qf.arrived();
+    }
+    f32x16 dk[HD / 32] = {}, dv[HD / 32] = {};
+    constexpr bool kFactors = HD > 64;
+    const auto tile = [&](int x, auto masked) {
+        const int r0 = (ta + x % per_head) * kCtxTile;
+        if (x + 1 < nx) request(x + 1);
+        const elem_t* Q = place(x);
+        const float* st = stats + (x & 1) * (kCtxStats / 2);
+        if (k0 < keys.keys && !(decltype(masked)::value && r0 + kCtxTile <= k0)) {
+            const bool factors = __builtin_amdgcn_ballot_w64(st[kCtxTile + lane] != 1.0f);
+            f32x16 s[2], ds[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                s[u] = scores<T>(at, Q, 32 * u, own_k);
+                ds[u] = scores<T>(at, Q + kTile, 32 * u, own_v, seq_of_rows(st + 2 * kCtxTile + 32 * u, h));
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const f32x4 less = *reinterpret_cast<const f32x4*>(st + 32 * u + 8 * i + 4 * h);
+                    f32x4 factor;
+                    if constexpr (kFactors) factor = *reinterpret_cast<const f32x4*>(st + kCtxTile + 32 * u + 8 * i + 4 * h);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        float y = fast_exp2(__builtin_fmaf(s[u][4 * i + j], p.c, -less[j]));
+                        if constexpr (kFactors) y *= factor[j];
+                        ds[u][4 * i + j] *= y;
+                        if constexpr (decltype(masked)::value)
+                            if (32 * u + 8 * i + j < key - r0 - 4 * h) y = 0.0f, ds[u][4 * i + j] = 0.0f;  // a row ahead of the key
+                        s[u][4 * i + j] = y;
+                    }
+                }
+                if (!kFactors && factors) {
+                    const f32x16 factor = seq_of_rows(st + kCtxTile + 32 * u, h);
+                    s[u] *= factor, ds[u] *= factor;
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                add_columns<T>(dv, at, Q + kTile, 32 * u, s[u]);
+                add_columns<T>(dk, at, Q, 32 * u, ds[u]);
+            }
+        }
+        if (x + 1 < nx) deliver(x + 1);
+        qf.arrived();
+        workgroup_barrier();
+    };
+    workgroup_barrier();
+    // causal: the rows of the block's own positions stand in a head's first two tiles
+    const int near = p.causal ? min(kCtxOwned / kCtxTile, per_head) : 0;
+    for (int x = 0; x < nx;) {
+        const int first = x;
+        for (; x < first + near; ++x) tile(x, std::true_type{});
+        for (; x < first + per_head; ++x) tile(x, std::false_type{});
+    }
+    const bool scored = ok && keys.keys != 1;
+    const int out_rows = min(max(b.tokens - k0, 0), 32);
+    elem_t* region = tiles + wave * 32 * (HD + 8);
+    store_rows_at<T, HD>(dk, scored ? p.scale : 0.0f, out_rows, region, lane, p.D,
+                         [&](int row) { return p.dk.head(0, hk) + (int64_t)(b.token + k0 + row) * p.dk.sl; });
+    store_rows_at<T, HD>(dv, ok ? 1.0f : 0.0f, out_rows, region, lane, p.D,
+                         [&](int row) { return p.dv.head(0, hk) + (int64_t)(b.token + k0 + row) * p.dv.sl; });
+}
+
+}  // namespace sjvp

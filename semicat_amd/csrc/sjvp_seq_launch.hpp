@@ -1,0 +1,21 @@
+// Launches of the attention over packed sequences and over a paged cache, for the translation units.
+#pragma once
+#include "sjvp_ctx_launch.hpp"
+#include "sjvp_seq.hpp"
+
+namespace sjvp {
+
+// Blocks of R rows that the segments of a call can have (see seq_block).
+inline int64_t seq_slots(const SeqParams& p, int heads, int R) { return (int64_t)p.T * heads / R + p.B + 2; }
+
+inline bool seq_dma(const SeqParams& p, const CtxView& a, const CtxView& b) {
+    return p.D % 8 == 0 && ctx_padded(p.D) != 96 && ctx_aligned(a) && ctx_aligned(b);
+}
+
+template <typename T> int seq_packed_fwd(SeqParams p, hipStream_t stream);
+template <typename T> int seq_packed_bwd(SeqParams p, hipStream_t stream);
+// e4m3: pages of 8-bit numbers; few, many: which of the two kernels serve the call
+template <typename T> int seq_paged(SeqParams p, bool e4m3, bool few, bool many, hipStream_t stream);
+int paged_copy(const SeqParams& p, bool e4m3, bool fp16, bool write, hipStream_t stream);
+
+}  // namespace sjvp

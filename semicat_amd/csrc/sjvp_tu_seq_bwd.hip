@@ -1,0 +1,26 @@
+// Translation unit: backward kernels of the attention over packed sequences for one element type (SJVP_T).
+#include "sjvp_seq_bwd.hpp"
+#include "sjvp_seq_launch.hpp"
+
+namespace sjvp {
+
+template <>
+int seq_packed_bwd<SJVP_T>(SeqParams p, hipStream_t stream) {
+    const bool row_dma = seq_dma(p, p.k, p.v), col_dma = seq_dma(p, p.q, p.g);
+    p.splits = 1, p.least = 0, p.most = INT_MAX;
+    p.slots = (int)seq_slots(p, p.G, kCtxOwned);
+    int rc = ctx_by_head(p.D, row_dma, [&](auto hd, auto dma) {
+        constexpr int HD = decltype(hd)::value;
+        constexpr bool DMA = decltype(dma)::value;
+        return launch(seq_bwd_row<SJVP_T, HD, DMA>, p.slots * p.Hkv, ctx_tiles_bytes(HD, DMA), stream, p, kCtxThreads);
+    });
+    if (rc != SJVP_OK || !p.dk.ptr) return rc;
+    p.slots = (int)seq_slots(p, 1, kCtxOwned);
+    return ctx_by_head(p.D, col_dma, [&](auto hd, auto dma) {
+        constexpr int HD = decltype(hd)::value;
+        constexpr bool DMA = decltype(dma)::value;
+        return launch(seq_bwd_col<SJVP_T, HD, DMA>, p.slots * p.Hkv, ctx_tiles_bytes(HD, DMA) + 4 * kCtxStats, stream, p, kCtxThreads);
+    });
+}
+
+}  // namespace sjvp
