@@ -195,7 +195,8 @@ def _load_host(lib: ctypes.CDLL):
                 (lib.sjvp_fwd, lib.sjvp_fwd_rotary, lib.sjvp_bwd_parts, lib.sjvp_bwd_rotary,
                  lib.sjvp_bwd_workspace_bytes, lib.sjvp_cast, lib.sjvp_adaln_fwd, lib.sjvp_adaln_bwd,
                  lib.sjvp_adaln_workspace_floats, lib.sjvp_gelu, lib.sjvp_rope, lib.sjvp_ctx_fwd, lib.sjvp_ctx_bwd,
-                 lib.sjvp_ctx_workspace_bytes)))
+                 lib.sjvp_ctx_workspace_bytes, lib.sjvp_packed_fwd, lib.sjvp_packed_bwd, lib.sjvp_packed_workspace_bytes,
+                 lib.sjvp_paged_write, lib.sjvp_paged_read, lib.sjvp_paged_attention, lib.sjvp_paged_workspace_bytes)))
     return host
 
 

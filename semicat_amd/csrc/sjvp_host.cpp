@@ -40,6 +40,13 @@ struct Abi {
     decltype(&sjvp_ctx_fwd) ctx_fwd = nullptr;
     decltype(&sjvp_ctx_bwd) ctx_bwd = nullptr;
     decltype(&sjvp_ctx_workspace_bytes) ctx_workspace_bytes = nullptr;
+    decltype(&sjvp_packed_fwd) packed_fwd = nullptr;
+    decltype(&sjvp_packed_bwd) packed_bwd = nullptr;
+    decltype(&sjvp_packed_workspace_bytes) packed_workspace_bytes = nullptr;
+    decltype(&sjvp_paged_write) paged_write = nullptr;
+    decltype(&sjvp_paged_read) paged_read = nullptr;
+    decltype(&sjvp_paged_attention) paged_attention = nullptr;
+    decltype(&sjvp_paged_workspace_bytes) paged_workspace_bytes = nullptr;
 };
 Abi abi;  // filled once by bind() when the library is loaded
 
@@ -781,11 +788,310 @@ PyObject* context(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// What a packed attention call has beside its differentiable tensors.
+struct PackedOptions {
+    Tensor offsets;
+    bool causal = true;
+    float scale = 0.0f;
+    mutable int status = SJVP_OK;  // of a forward that its node has thrown
+};
+
+// whether the kernels take the stride of an input's rows
+bool row_stride(const Tensor& x) { return x.size(0) <= 1 || x.stride(0) < 1 << 24; }
+
+void packed_view(sjvp_packed& t, int at, const Tensor& x) {  // [T,H,D] as (head, row)
+    t.strides[2 * at] = x.stride(1), t.strides[2 * at + 1] = x.stride(0);
+}
+
+sjvp_packed packed_struct(const Tensor& q, const Tensor& k, const Tensor& v, const PackedOptions& options) {
+    sjvp_packed t{};
+    t.T = static_cast<int>(q.size(0)), t.Hq = static_cast<int>(q.size(1)), t.D = static_cast<int>(q.size(2)), t.Hkv = static_cast<int>(k.size(1));
+    t.B = static_cast<int>(options.offsets.size(0)) - 1;
+    t.q = q.data_ptr(), t.k = k.data_ptr(), t.v = v.data_ptr();
+    t.offsets = static_cast<const int32_t*>(options.offsets.data_ptr());
+    t.causal = options.causal, t.scale = options.scale;
+    packed_view(t, SJVP_S_Q, q), packed_view(t, SJVP_S_K, k), packed_view(t, SJVP_S_V, v);
+    return t;
+}
+
+// lse: for a backward to follow, or null
+Tensor packed_forward(const Tensor& q, const Tensor& k, const Tensor& v, const PackedOptions& options, Tensor* lse, int& status) {
+    const c10::DeviceGuard guard(q.device());
+    const Maker make_tensor{q.device()};
+    Tensor o = make_tensor(q.sizes(), q.scalar_type());
+    sjvp_packed t = packed_struct(q, k, v, options);
+    if (lse) {
+        *lse = make_tensor({q.size(1), q.size(0), 2}, at::kFloat);
+        t.lse = static_cast<float*>(lse->data_ptr());
+    }
+    t.o = o.data_ptr();
+    packed_view(t, SJVP_S_O, o);
+    status = abi.packed_fwd(&t, type_tag(q.scalar_type()), c10::hip::getCurrentHIPStream(q.device().index()).stream());
+    return o;
+}
+
+// As NoSecondDerivative, of the packed attention.
+struct NoSecondPacked : torch::autograd::Function<NoSecondPacked> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext*, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+                                                  torch::autograd::variable_list* grads) {
+        return std::move(*grads);
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext*, torch::autograd::variable_list) {
+        TORCH_CHECK_NOT_IMPLEMENTED(false, "double backward of packed attention is not implemented");
+    }
+};
+
+struct PackedNode : torch::autograd::Function<PackedNode> {
+    static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const PackedOptions* options) {
+        Tensor lse;
+        int status;
+        Tensor o = packed_forward(q, k, v, *options, &lse, status);
+        options->status = status;
+        TORCH_CHECK(status == SJVP_OK, "sjvp status ", status, " from the packed attention kernels");
+        ctx->save_for_backward({q, k, v, options->offsets, o, lse});
+        ctx->saved_data["causal"] = options->causal;
+        ctx->saved_data["scale"] = static_cast<double>(options->scale);
+        ctx->set_materialize_grads(false);
+        return o;
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list cotangents) {
+        torch::autograd::variable_list grads(4);
+        if (!cotangents[0].defined()) return grads;
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &o = saved[4], &lse = saved[5];
+        const PackedOptions options{saved[3], ctx->saved_data["causal"].toBool(), static_cast<float>(ctx->saved_data["scale"].toDouble())};
+        const bool record = at::GradMode::is_enabled();
+        {
+            const at::NoGradGuard no_grad;
+            const c10::DeviceGuard guard(q.device());
+            const Tensor g = cotangents[0].stride(2) == 1 && row_stride(cotangents[0]) ? cotangents[0] : cotangents[0].contiguous();
+            const Maker make_tensor{q.device()};
+            sjvp_packed t = packed_struct(q, k, v, options);
+            t.lse = static_cast<float*>(lse.data_ptr()), t.o = o.data_ptr(), t.dO = g.data_ptr();
+            packed_view(t, SJVP_S_O, o), packed_view(t, SJVP_S_DO, g);
+            grads[0] = make_tensor(q.sizes(), q.scalar_type());
+            t.dq = grads[0].data_ptr();
+            packed_view(t, SJVP_S_DQ, grads[0]);
+            if (ctx->needs_input_grad(1) || ctx->needs_input_grad(2)) {
+                grads[1] = make_tensor(k.sizes(), k.scalar_type());
+                grads[2] = make_tensor(v.sizes(), v.scalar_type());
+                t.dk = grads[1].data_ptr(), t.dv = grads[2].data_ptr();
+                packed_view(t, SJVP_S_DK, grads[1]), packed_view(t, SJVP_S_DV, grads[2]);
+            }
+            t.workspace_bytes = abi.packed_workspace_bytes(&t, 1);
+            const Tensor workspace = make_tensor({static_cast<int64_t>(t.workspace_bytes)}, at::kByte);
+            t.workspace = workspace.data_ptr();
+            const int status = abi.packed_bwd(&t, type_tag(q.scalar_type()), c10::hip::getCurrentHIPStream(q.device().index()).stream());
+            TORCH_CHECK(status == SJVP_OK, "sjvp status ", status, " from the packed attention kernels");
+        }
+        if (record) {
+            torch::autograd::variable_list made;
+            for (int i = 0; i < 3; ++i)
+                if (grads[i].defined()) made.push_back(grads[i]);
+            made = NoSecondPacked::apply(q, k, v, cotangents[0], &made);
+            for (int i = 0, n = 0; i < 3; ++i)
+                if (grads[i].defined()) grads[i] = made[n++];
+        }
+        for (int i = 0; i < 3; ++i)
+            if (grads[i].defined() && !ctx->needs_input_grad(i)) grads[i] = Tensor();
+        return grads;
+    }
+};
+
+// obj as an int32 array of a call, contiguous, or nullptr
+const Tensor* index_array(PyObject* obj, int64_t least, c10::Device device) {
+    const Tensor* x = plain(obj);
+    if (!x || x->dim() != 1 || x->size(0) < least || x->size(0) > kMostRows || x->scalar_type() != at::kInt || x->device() != device || !x->is_contiguous()) return nullptr;
+    return x;
+}
+
+// obj as [T,H,D] rows of 16-bit numbers, or nullptr
+const Tensor* packed_rows(PyObject* obj) {
+    const Tensor* x = plain(obj);
+    if (!x || x->dim() != 3 || x->numel() == 0 || x->stride(2) != 1 || !row_stride(*x) || x->size(0) > kMostRows || x->size(1) > kMostRows ||
+        x->size(0) * x->size(1) > INT_MAX || x->size(2) < 16 || x->size(2) > 128 || (x->scalar_type() != at::kBFloat16 && x->scalar_type() != at::kHalf) ||
+        x->_fw_grad(0).defined())
+        return nullptr;
+    return x;
+}
+
+// packed(q, k, v, offsets, causal, scale) -> output: [T,H,D] tensors
+PyObject* packed(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 6 || !abi.packed_fwd) return none();
+    const Tensor* in[3];
+    for (int i = 0; i < 3; ++i) {
+        in[i] = packed_rows(a[i]);
+        if (!in[i] || in[i]->scalar_type() != in[0]->scalar_type() || in[i]->device() != in[0]->device()) return none();
+    }
+    const Tensor &q = *in[0], &k = *in[1], &v = *in[2];
+    if (k.sizes() != v.sizes() || k.size(0) != q.size(0) || k.size(2) != q.size(2) || q.size(1) % k.size(1)) return none();
+    const Tensor* offsets = index_array(a[3], 2, q.device());
+    PackedOptions options;
+    options.scale = scale_arg(a[5]);
+    if (!offsets || options.scale < 0.0f || (a[4] != Py_True && a[4] != Py_False)) return none();
+    options.offsets = *offsets, options.causal = a[4] == Py_True;
+    Tensor o;
+    int status = SJVP_OK;
+    {
+        pybind11::gil_scoped_release no_gil;
+        if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad())) {
+            try {
+                o = PackedNode::apply(q, k, v, &options);
+            } catch (const c10::Error&) {
+                if (options.status == SJVP_OK) throw;
+                status = options.status;  // (raised as every other status)
+            }
+        } else o = packed_forward(q, k, v, options, nullptr, status);
+    }
+    if (status != SJVP_OK) return PyLong_FromLong(status);
+    return THPVariable_Wrap(std::move(o));
+    END_HANDLE_TH_ERRORS
+}
+
+// The cache and the sequences of a paged call: a = k, v, k_scales, v_scales, dtype, tables, lengths, offsets (all but the first two, dtype,
+// tables and lengths may be None).  T: the call's rows, negative where it has none.
+struct PagedCall {
+    sjvp_paged t{};
+    at::ScalarType dtype = at::kBFloat16;
+    c10::Device device{c10::kCPU};
+
+    bool take(PyObject* const* a, int64_t T) {
+        const Tensor *k = plain(a[0]), *v = plain(a[1]);
+        const bool scaled = a[2] != Py_None;
+        if (!k || !v || k->dim() != 4 || k->sizes() != v->sizes() || k->stride(3) != 1 || v->stride(3) != 1 || k->device() != v->device() ||
+            k->scalar_type() != v->scalar_type() || scaled != (a[3] != Py_None) || !THPDtype_Check(a[4]))
+            return false;
+        dtype = reinterpret_cast<THPDtype*>(a[4])->scalar_type, device = k->device();
+        if ((dtype != at::kBFloat16 && dtype != at::kHalf) || k->scalar_type() != (scaled ? at::kFloat8_e4m3fn : dtype)) return false;
+        const int item = scaled ? 1 : 2;
+        for (int d = 0; d < 4; ++d)
+            if (k->size(d) < 1 || k->size(d) > kMostRows) return false;
+        const auto place = [](const Tensor& x, int d) { return x.size(d) > 1 ? x.stride(d) : 0; };
+        constexpr int dims[3] = {0, 1, 2};
+        for (int d : dims) {
+            if (place(*k, d) != place(*v, d)) return false;
+            t.page_strides[d] = place(*k, d) * item;
+        }
+        t.k_pages = k->data_ptr(), t.v_pages = v->data_ptr();
+        if (scaled) {
+            const Tensor* s[2] = {plain(a[2]), plain(a[3])};
+            for (const Tensor* x : s) {
+                if (!x || x->dim() != 4 || x->device() != device || x->element_size() != 1 || x->stride(3) != 1 || x->size(3) != (k->size(3) + 31) / 32) return false;
+                for (int d : dims)
+                    if (x->size(d) != k->size(d) || place(*x, d) != place(*s[0], d)) return false;
+            }
+            for (int d : dims) t.page_strides[3 + d] = place(*s[0], d);
+            t.k_scales = s[0]->data_ptr(), t.v_scales = s[1]->data_ptr();
+        }
+        t.pages = static_cast<int>(k->size(0)), t.Hkv = static_cast<int>(k->size(1)), t.page_size = static_cast<int>(k->size(2)), t.D = static_cast<int>(k->size(3));
+        t.Hq = t.Hkv;
+        const Tensor* tables = plain(a[5]);
+        if (!tables || tables->dim() != 2 || tables->size(0) < 1 || tables->size(1) < 1 || tables->size(0) > kMostRows || tables->size(1) > kMostRows ||
+            tables->scalar_type() != at::kInt || tables->device() != device || (tables->size(1) > 1 && tables->stride(1) != 1))
+            return false;
+        const int64_t B = tables->size(0);
+        t.tables = static_cast<const int32_t*>(tables->data_ptr()), t.table_stride = tables->stride(0), t.table_pages = static_cast<int>(tables->size(1));
+        const Tensor* lengths = index_array(a[6], B, device);
+        if (!lengths || lengths->size(0) != B) return false;
+        t.lengths = static_cast<const int32_t*>(lengths->data_ptr());
+        if (a[7] != Py_None) {
+            const Tensor* offsets = index_array(a[7], B + 1, device);
+            if (!offsets || offsets->size(0) != B + 1) return false;
+            t.offsets = static_cast<const int32_t*>(offsets->data_ptr());
+        } else if (T >= 0 && T != B) {
+            return false;
+        }
+        t.B = static_cast<int>(B), t.T = static_cast<int>(std::max<int64_t>(T, 0));
+        return true;
+    }
+    // [T,H,D] rows of the call
+    bool rows(const Tensor& x, int64_t heads) const { return x.scalar_type() == dtype && x.device() == device && x.size(1) == heads && x.size(2) == t.D; }
+    void put(int at, const Tensor& x) { t.strides[3 * at] = x.stride(1), t.strides[3 * at + 1] = x.stride(0); }
+    void* stream() const { return c10::hip::getCurrentHIPStream(device.index()).stream(); }
+};
+
+bool wants_gradient(const Tensor& x) { return x.requires_grad() && at::GradMode::is_enabled(); }
+
+// paged_attention(q, cache and sequences as PagedCall takes them, scale) -> output
+PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 10 || !abi.paged_attention) return none();
+    const Tensor* q = packed_rows(a[0]);
+    PagedCall call;
+    if (!q || wants_gradient(*q) || !call.take(a + 1, q->size(0)) || q->size(1) % call.t.Hkv || !call.rows(*q, q->size(1))) return none();
+    call.t.scale = scale_arg(a[9]);
+    if (call.t.scale < 0.0f) return none();
+    Tensor o;
+    int status;
+    {
+        pybind11::gil_scoped_release no_gil;
+        const c10::DeviceGuard guard(call.device);
+        const Maker make_tensor{call.device};
+        o = make_tensor(q->sizes(), call.dtype);
+        call.t.Hq = static_cast<int>(q->size(1)), call.t.q = q->data_ptr(), call.t.o = o.data_ptr();
+        call.put(SJVP_P_Q, *q), call.put(SJVP_P_O, o);
+        call.t.workspace_bytes = abi.paged_workspace_bytes(&call.t);
+        const Tensor workspace = call.t.workspace_bytes ? make_tensor({static_cast<int64_t>(call.t.workspace_bytes)}, at::kByte) : Tensor();
+        call.t.workspace = workspace.defined() ? workspace.data_ptr() : nullptr;
+        status = abi.paged_attention(&call.t, type_tag(call.dtype), call.stream());
+    }
+    if (status != SJVP_OK) return PyLong_FromLong(status);
+    return THPVariable_Wrap(std::move(o));
+    END_HANDLE_TH_ERRORS
+}
+
+// paged_write(k, v, cache and sequences) -> status
+PyObject* paged_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 10 || !abi.paged_write) return none();
+    const Tensor *k = packed_rows(a[0]), *v = packed_rows(a[1]);
+    PagedCall call;
+    if (!k || !v || wants_gradient(*k) || wants_gradient(*v) || !call.take(a + 2, k->size(0)) || k->sizes() != v->sizes() ||
+        !call.rows(*k, call.t.Hkv) || !call.rows(*v, call.t.Hkv))
+        return none();
+    const c10::DeviceGuard guard(call.device);
+    call.t.k = k->data_ptr(), call.t.v = v->data_ptr();
+    call.put(SJVP_P_K, *k), call.put(SJVP_P_V, *v);
+    return PyLong_FromLong(abi.paged_write(&call.t, type_tag(call.dtype), call.stream()));
+    END_HANDLE_TH_ERRORS
+}
+
+// paged_read(cache and sequences, size) -> (k, v)
+PyObject* paged_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 9 || !abi.paged_read || !PyLong_CheckExact(a[8])) return none();
+    const long size = PyLong_AsLong(a[8]);
+    if (PyErr_Occurred()) PyErr_Clear();
+    PagedCall call;
+    if (size < 1 || size > kMostRows || !call.take(a, -1)) return none();
+    Tensor out[2];
+    int status;
+    {
+        pybind11::gil_scoped_release no_gil;
+        const c10::DeviceGuard guard(call.device);
+        const Maker make_tensor{call.device};
+        for (int i = 0; i < 2; ++i) {
+            out[i] = make_tensor({call.t.B, size, call.t.Hkv, call.t.D}, call.dtype);
+            int64_t* strides = call.t.strides + 3 * (SJVP_P_K + i);
+            strides[0] = out[i].stride(2), strides[1] = out[i].stride(1), strides[2] = out[i].stride(0);
+        }
+        call.t.size = static_cast<int>(size), call.t.k = out[0].data_ptr(), call.t.v = out[1].data_ptr();
+        status = abi.paged_read(&call.t, type_tag(call.dtype), call.stream());
+    }
+    if (status != SJVP_OK) return PyLong_FromLong(status);
+    PyObject* res = PyTuple_New(2);
+    if (!res) return nullptr;
+    for (int i = 0; i < 2; ++i) PyTuple_SET_ITEM(res, i, THPVariable_Wrap(std::move(out[i])));
+    return res;
+    END_HANDLE_TH_ERRORS
+}
+
 // bind(addresses of the entry points, in the order of Abi)
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
-    constexpr int kEntries = 14;
+    constexpr int kEntries = 21;
     if (n != kEntries) {
-        PyErr_SetString(PyExc_TypeError, "bind() takes fourteen addresses");
+        PyErr_SetString(PyExc_TypeError, "bind() takes twenty-one addresses");
         return nullptr;
     }
     void* p[kEntries];
@@ -811,7 +1117,14 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
            reinterpret_cast<decltype(abi.rope)>(p[10]),
            reinterpret_cast<decltype(abi.ctx_fwd)>(p[11]),
            reinterpret_cast<decltype(abi.ctx_bwd)>(p[12]),
-           reinterpret_cast<decltype(abi.ctx_workspace_bytes)>(p[13])};
+           reinterpret_cast<decltype(abi.ctx_workspace_bytes)>(p[13]),
+           reinterpret_cast<decltype(abi.packed_fwd)>(p[14]),
+           reinterpret_cast<decltype(abi.packed_bwd)>(p[15]),
+           reinterpret_cast<decltype(abi.packed_workspace_bytes)>(p[16]),
+           reinterpret_cast<decltype(abi.paged_write)>(p[17]),
+           reinterpret_cast<decltype(abi.paged_read)>(p[18]),
+           reinterpret_cast<decltype(abi.paged_attention)>(p[19]),
+           reinterpret_cast<decltype(abi.paged_workspace_bytes)>(p[20])};
     return none();
 }
 
@@ -828,6 +1141,10 @@ PyMethodDef methods[] = {
     {"gelu", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(gelu)), METH_FASTCALL, nullptr},
     {"rope", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rope)), METH_FASTCALL, nullptr},
     {"context", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(context)), METH_FASTCALL, nullptr},
+    {"packed", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(packed)), METH_FASTCALL, nullptr},
+    {"paged_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(paged_attention)), METH_FASTCALL, nullptr},
+    {"paged_write", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(paged_write)), METH_FASTCALL, nullptr},
+    {"paged_read", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(paged_read)), METH_FASTCALL, nullptr},
     {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(bind)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 

@@ -17,9 +17,9 @@ int seq_packed_fwd<SJVP_T>(SeqParams p, hipStream_t stream) {
 template <>
 int seq_paged<SJVP_T>(SeqParams p, bool e4m3, bool few, bool many, hipStream_t stream) {
     const int splits = p.splits;
-    return ctx_by_head(p.D, true, [&](auto hd, auto dma) {
+    const auto with = [&](auto hd) {
         constexpr int HD = decltype(hd)::value;
-        constexpr bool DMA = decltype(dma)::value;
+        constexpr bool DMA = HD != 96;  // (twelve pieces to a row do not fit the permutation of LDS-DMA tiles)
         int rc = SJVP_OK;
         if (few) {
             p.slots = (int)seq_slots(p, p.G, 32), p.least = 0, p.most = many ? kSeqFew : INT_MAX;
@@ -40,7 +40,13 @@ int seq_paged<SJVP_T>(SeqParams p, bool e4m3, bool few, bool many, hipStream_t s
         while (slices < splits && slices < 16) slices *= 2;
         const int64_t rows = p.Hkv * (many ? (int64_t)(p.B + 2) * kSeqFew : (int64_t)p.T * p.G), per = 16 / slices;
         return launch(seq_join<SJVP_T, HD>, (int)((rows + per - 1) / per), 0, stream, p, kCtxThreads);
-    });
+    };
+    switch (ctx_padded(p.D)) {
+        case 32: return with(std::integral_constant<int, 32>{});
+        case 64: return with(std::integral_constant<int, 64>{});
+        case 96: return with(std::integral_constant<int, 96>{});
+        default: return with(std::integral_constant<int, 128>{});
+    }
 }
 
 }  // namespace sjvp

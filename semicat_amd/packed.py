@@ -178,6 +178,10 @@ def packed_attention(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor, causal: b
     gradients there are zeros.  The lengths are not looked at by the host.  ``causal`` hides the tokens behind a query.  ``Hq`` is a
     multiple of ``Hkv``; query head ``h`` reads key head ``h // (Hq // Hkv)``.  ``scale`` defaults to ``1/sqrt(D)``.  bfloat16 and float16,
     16 <= D <= 128; other types are computed in bfloat16 and handed back as they came."""
+    if _on_gpu(q):
+        o = _lib.host().packed(q, k, v, offsets, bool(causal), scale)
+        if o is not None:
+            return _host_result(o)
     for t in (q, k, v):
         if fwAD.unpack_dual(t).tangent is not None:
             raise NotImplementedError("forward mode of packed attention is not implemented")

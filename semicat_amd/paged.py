@@ -21,7 +21,7 @@ import torch.autograd.forward_ad as fwAD
 from torch import Tensor
 
 from . import _lib
-from .kernels import _scale_arg
+from .kernels import _host_result, _on_gpu, _scale_arg
 from .packed import _DTYPES, _check_indices, _check_offsets, _check_query, _check_rows
 
 GROUP = 32  # columns of a row that share a scale
@@ -89,6 +89,9 @@ class PagedCache:
             strides += places(k_scales)
         self.k, self.v, self.k_scales, self.v_scales, self.dtype = k, v, k_scales, v_scales, dtype
         self._strides = strides + (0,) * (6 - len(strides))
+
+    def _storage(self):
+        return self.k, self.v, self.k_scales, self.v_scales, self.dtype
 
     pages = property(lambda self: self.k.shape[0])
     heads = property(lambda self: self.k.shape[1])
@@ -160,6 +163,10 @@ def paged_write(cache: PagedCache, k: Tensor, v: Tensor, tables: Tensor, lengths
     """Writes the new tokens' ``k`` and ``v`` ``[T,Hkv,D]`` to the last positions of their sequences: token ``i`` of ``n`` new ones of a
     sequence has the position ``length - n + i``.  A page that is written to must belong to one sequence.  Tensors of another type than the cache's are
     rounded to it first."""
+    if _on_gpu(k):
+        status = _lib.host().paged_write(k, v, *cache._storage(), tables, lengths, offsets)
+        if status is not None:
+            return _lib.check(status)
     _no_gradient("paged_write", k, v)
     if k.ndim != 3:
         raise AssertionError(f"k must have three dimensions, got {tuple(k.shape)}")
@@ -181,6 +188,10 @@ def paged_write(cache: PagedCache, k: Tensor, v: Tensor, tables: Tensor, lengths
 def paged_read(cache: PagedCache, tables: Tensor, lengths: Tensor, size: int) -> Tuple[Tensor, Tensor]:
     """What the cache holds of each sequence's first ``size`` positions: ``(k, v)`` ``[B,size,Hkv,D]``, zeros behind a sequence, as
     :func:`semicat_amd.cross_attention` takes them with ``key_lengths``."""
+    if _on_gpu(cache.k):
+        both = _lib.host().paged_read(*cache._storage(), tables, lengths, None, size)
+        if both is not None:
+            return _host_result(both)
     t = _describe(cache, tables, lengths, None, -1)
     t.size = size
     k, v = (torch.empty((tables.shape[0], size, cache.heads, cache.head_dim), device=cache.k.device, dtype=cache.dtype) for _ in range(2))
@@ -198,6 +209,10 @@ def paged_attention(q: Tensor, cache: PagedCache, tables: Tensor, lengths: Tenso
     ``[T,Hq,D]``; rows that see nothing, and rows outside the sequences, are zeros.  ``Hq`` is a multiple of the cache's heads, ``scale``
     defaults to ``1/sqrt(D)``.  Sequences with one new token and with whole chunks of a prompt may stand in one call.  ``q`` of
     another type than the cache's is computed in the cache's and handed back as it came."""
+    if _on_gpu(q):
+        o = _lib.host().paged_attention(q, *cache._storage(), tables, lengths, offsets, scale)
+        if o is not None:
+            return _host_result(o)
     _no_gradient("paged_attention", q)
     dtype = q.dtype
     q = q if dtype == cache.dtype else q.to(cache.dtype)
