@@ -21,8 +21,8 @@ int seq_common(SeqParams& p, int B, int T, int Hq, int Hkv, int D, float scale) 
     p.B = B, p.T = T, p.Hq = Hq, p.Hkv = Hkv, p.G = Hq / Hkv, p.D = D;
     p.scale = scale == 0.0f ? 1.0f / std::sqrt(static_cast<float>(D)) : scale;
     p.c = p.scale * kLog2e;
-    // blocks of 32 rows over all heads and splits, 256 threads each
-    return (seq_slots(p, p.G, 32) * Hkv) * 64 > kMostThreads / 256 * 64 ? SJVP_ERR_SHAPE : SJVP_OK;
+    // blocks of 16 rows of all heads, 256 threads each (splits are made of launches of few blocks alone)
+    return seq_slots(p, p.G, 16) * Hkv > kMostThreads / 256 ? SJVP_ERR_SHAPE : SJVP_OK;
 }
 
 int packed_params(const sjvp_packed* t, SeqParams& p) {
@@ -63,6 +63,8 @@ int paged_params(const sjvp_paged* t, SeqParams& p, int T) {
     g.table = t->tables, g.table_stride = t->table_stride;
     g.pages = t->pages, g.size = t->page_size;
     g.capacity = (int)std::min<int64_t>((int64_t)t->table_pages * t->page_size, kCtxMost);
+    const int groups = (t->D + 31) / 32;
+    g.scale_words = (((uintptr_t)g.ks | (uintptr_t)g.vs | (uintptr_t)g.scale_sp | (uintptr_t)g.scale_sh | (uintptr_t)g.scale_sr) & (groups - 1)) == 0;
     g.shift = 0;
     while ((1u << g.shift) < (uint32_t)g.size) ++g.shift;
     g.magic = (uint32_t)(((uint64_t(1) << (31 + g.shift)) + g.size - 1) / g.size);

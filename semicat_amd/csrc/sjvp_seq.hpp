@@ -27,6 +27,7 @@ struct SeqPages {
     const int* table;
     int64_t table_stride;
     int pages, size, capacity;  // capacity: positions that a row of the table has
+    int scale_words;            // the exponents of a row are one word of memory (32 or 16 bits)
     uint32_t magic, shift;      // x / size = mulhi(2 x, magic) >> shift below 2^30
     __device__ __forceinline__ int page_of(int x) const { return (int)(__umulhi(2u * (uint32_t)x, magic) >> shift); }
 };
@@ -116,6 +117,26 @@ __device__ __forceinline__ float scale_of(uint32_t code) { return __uint_as_floa
 // 16 bytes of zeros, for the lanes of a copy that have no row.
 static __device__ const u32x4 kZeroPiece = {0u, 0u, 0u, 0u};
 
+// A load from memory.  (Of a pointer that is one of two, the compiler does not know that neither points to LDS; the loads that it makes then count as LDS
+// reads too, so that every wait for LDS waits for them: B=2 Hq=16 Hkv=2 four tokens on 32769 D=128 32 us.)
+template <typename V>
+__device__ __forceinline__ V global(const void* at) {
+    return *(const __attribute__((address_space(1))) V*)(uintptr_t)at;
+}
+
+// The exponent codes of a row, a byte to each 32 columns.
+template <int GROUPS>
+__device__ __forceinline__ uint32_t scale_codes(const void* at, bool words) {
+    if constexpr (GROUPS == 4)
+        if (words) return global<uint32_t>(at);
+    if constexpr (GROUPS == 2)
+        if (words) return global<uint16_t>(at);
+    uint32_t codes = 0;
+#pragma unroll
+    for (int i = 0; i < GROUPS; ++i) codes |= (uint32_t)global<uint8_t>(static_cast<const uint8_t*>(at) + i) << (8 * i);
+    return codes;
+}
+
 // Tiles of 64 keys and values on their way to LDS by four waves.  look() is called a tile ahead of request(), request() ahead of use,
 // deliver() where the places are read next, behind it arrived() and a barrier.
 // From a contiguous tensor (rows of a segment):
@@ -170,7 +191,7 @@ struct PageFeed {
                 dma16(from_k, lds_addr(kp) + 16 * (64 * wave + kCtxThreads * i));
                 dma16(from_v, lds_addr(vp) + 16 * (64 * wave + kCtxThreads * i));
             } else {
-                kr[i] = *static_cast<const u32x4*>(from_k), vr[i] = *static_cast<const u32x4*>(from_v);
+                kr[i] = global<u32x4>(from_k), vr[i] = global<u32x4>(from_v);
             }
         }
     }
@@ -217,8 +238,8 @@ struct PageFeed8 {
             const int64_t at = page[i] * p.pages.sp + head + row[i] * p.pages.sr + 16 * c;
             const int64_t sat = page[i] * p.pages.scale_sp + scale_head + row[i] * p.pages.scale_sr + c / 2;
             const void* none = &kZeroPiece;
-            kr[i] = *static_cast<const u32x4*>(ok ? p.pages.k + at : none), vr[i] = *static_cast<const u32x4*>(ok ? p.pages.v + at : none);
-            ks[i] = *static_cast<const uint8_t*>(ok ? p.pages.ks + sat : none), vs[i] = *static_cast<const uint8_t*>(ok ? p.pages.vs + sat : none);
+            kr[i] = global<u32x4>(ok ? p.pages.k + at : none), vr[i] = global<u32x4>(ok ? p.pages.v + at : none);
+            ks[i] = global<uint8_t>(ok ? p.pages.ks + sat : none), vs[i] = global<uint8_t>(ok ? p.pages.vs + sat : none);
         }
     }
     __device__ __forceinline__ void deliver(const SeqParams&, elem_t* kp, elem_t* vp, int) {

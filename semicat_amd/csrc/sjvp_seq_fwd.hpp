@@ -1,6 +1,7 @@
 // Forward kernels of the attention over packed sequences and over a paged cache (sjvp_seq.hpp).
 #pragma once
 #include "sjvp_seq.hpp"
+#include "sjvp_w16.hpp"
 
 namespace sjvp {
 
@@ -99,136 +100,199 @@ __device__ __forceinline__ int64_t seq_place(const SeqParams& p, const SeqBlock&
     return hk * seq_group(p) + (p.most == kSeqFew ? (int64_t)b.segment * kSeqFew : (int64_t)b.token * p.G) + row;
 }
 
-// Few rows: 32 rows to a block and waves that share out its keys: each runs over tiles of 32 keys of its own, K straight from memory into
-// the operand's registers, V through a region of LDS that no other wave reads, so that nothing but the end is synchronised.  The sums of
-// the waves are joined in LDS; with several splits of the keys they go to memory for seq_join.
-// E4M3: the cache's numbers have 8 bits; a lane's 16 bytes of K are the two halves of 32 columns then, and q is read in that order.
-template <typename T, int HD, bool E4M3, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, HD <= 64 ? 4 : 2) void seq_few(SeqParams p) {
+// Maximum and sum over the four lanes (l, l ^ 16, l ^ 32, l ^ 48) of a row.
+__device__ __forceinline__ float quarters_max(float x) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return halves_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ __forceinline__ float quarters_sum(float x) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return halves_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
+// Few rows: 16 or 32 rows to a block (NC sets of 16) and waves that share out its keys: each runs over tiles of 32 keys of its own, K straight from
+// memory into the operand's registers, V through a region of LDS that no other wave reads, so that nothing but the end is synchronised.  The
+// sums of the waves are joined in LDS; with several splits of the keys they go to memory for seq_join.
+//
+// The matrix instructions are 16x16x32 (tile algebra in sjvp_w16.hpp), so that a step of a group of heads, some four to sixteen rows, leaves
+// little of them idle, and a wave needs 128 registers at most: four waves to a SIMD hold twice as many loads in flight as the 32-wide form did.
+// E4M3: the cache's numbers have 8 bits; a lane's 16 bytes are columns of two chunks of 32 then, and q is read in that order.
+template <typename T, int HD, bool E4M3, int NC, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, NC == 1 ? (E4M3 || HD <= 96 ? 4 : 3) : HD <= 64 ? 4 : 2) void seq_few(SeqParams p) {
     extern __shared__ __align__(16) unsigned char smem[];
-    constexpr int kRegion = 32 * (HD + 8), kSum = HD + 4, CH = HD / 8;
-    elem_t* region = reinterpret_cast<elem_t*>(smem);  // [WAVES] V tiles, then the waves' sums [WAVES][32][HD + 4] fp32
+    constexpr int R = 16 * NC, kLd = HD + 8, kSum = HD + 4, CH = HD / 8, KC = HD / 32, DT = HD / 16;
+    elem_t* region = reinterpret_cast<elem_t*>(smem);  // [WAVES][32] rows of V, then the waves' sums [WAVES][R][HD + 4] fp32
     float* sums = reinterpret_cast<float*>(smem);
-    float* stats = sums + WAVES * 32 * kSum;  // [WAVES][32] maximum, then sum
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+    float* stats = sums + WAVES * R * kSum;  // [WAVES][R] maximum, then sum
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), y = lane & 15, g = lane >> 4;
     const int hk = blockIdx.x % p.Hkv, x = blockIdx.x / p.Hkv, slot = x % p.slots, split = x / p.slots;
-    const SeqBlock b = seq_block<32>(p, slot, p.G, lane);
+    const SeqBlock b = seq_block<R>(p, slot, p.G, lane);
     const int all = b.tokens * p.G;
     if (!b.some || all < p.least || all > p.most) return;
     const SeqKeys<true> keys(p, b);
-    const int r0 = b.row0, rows = min(all - r0, 32);
-    const SeqRow mine(p, hk, min(r0 + (lane & 31), all - 1));
-    const int limit = keys.seen(p, mine.token), n = keys.seen(p, (r0 + rows - 1) / p.G), whole = keys.seen(p, r0 / p.G);
+    const int r0 = b.row0, rows = min(all - r0, R);
+    const int n = keys.seen(p, (r0 + rows - 1) / p.G), whole = keys.seen(p, r0 / p.G);
     const SeqSplit part((n + 31) / 32, p.splits, split);
     if (split >= part.used) return;
 
-    u32x4 own[HD / 16];
-    {
+    // column of the eight numbers that step c of a contraction over the head dimension has in this lane
+    const auto column = [&](int c) { return !E4M3 || (KC % 2 && c == KC - 1) ? 32 * c + 8 * g : 64 * (c / 2) + 16 * g + 8 * (c % 2); };
+    u32x4 own[NC][KC];
+    int limit[NC];
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+        const SeqRow mine(p, hk, min(r0 + 16 * i + y, all - 1));
+        limit[i] = keys.seen(p, mine.token);
         const elem_t* q = p.q.head(0, mine.hq) + (int64_t)(b.token + mine.token) * p.q.sl;
 #pragma unroll
-        for (int c = 0; c < HD / 16; ++c) {
-            const int c8 = E4M3 ? 32 * (c / 2) + 16 * h + 8 * (c % 2) : 16 * c + 8 * h;
-            own[c] = (lane & 31) < rows ? load_chunk(q, c8, p.D) : u32x4{0u, 0u, 0u, 0u};
-        }
+        for (int c = 0; c < KC; ++c) own[i][c] = 16 * i + y < rows ? load_chunk(q, column(c), p.D) : u32x4{0u, 0u, 0u, 0u};
     }
-    constexpr int NK = E4M3 ? HD / 32 : HD / 16, PC = E4M3 ? HD / 16 : CH, NV = 32 * PC / 64;  // 16-byte pieces: K of a lane, V of a row, V of a lane
-    u32x4 kr[NK], vr[NV];
-    uint32_t ks[E4M3 ? NK : 1], vs[E4M3 ? NV : 1];
+    // K and V of the rows 16 u + lane % 16 of a tile: pieces of 16 bytes, the last one of an odd number of 8-bit chunks of 8
+    constexpr int NP = E4M3 ? (KC + 1) / 2 : KC;
+    u32x4 kr[2][NP], vr[2][NP];
+    uint32_t ks[2] = {}, vs[2] = {};
     const int* table = p.pages.table + (b.segment - 1) * p.pages.table_stride;
-    const int64_t head = hk * p.pages.sh, scale_head = hk * p.pages.scale_sh;
+    const unsigned char *kp = p.pages.k + hk * p.pages.sh, *vp = p.pages.v + hk * p.pages.sh;
+    const unsigned char *ksp = p.pages.ks + hk * p.pages.scale_sh, *vsp = p.pages.vs + hk * p.pages.scale_sh;
     const void* none = &kZeroPiece;
-    // the page of key t * 32 + lane % 32
+    int page[2];
     const auto look = [&](int t) {
-        const int key = 32 * t + (lane & 31);
-        return key < n ? table[p.pages.page_of(key)] : -1;
-    };
-    const auto load = [&](int t, int page) {
-        const int key = 32 * t + (lane & 31), row = key - p.pages.page_of(key) * p.pages.size;
-        const bool there = (uint32_t)page < (uint32_t)p.pages.pages;
-        const int64_t at = page * p.pages.sp + head + row * p.pages.sr, sat = E4M3 ? page * p.pages.scale_sp + scale_head + row * p.pages.scale_sr : 0;
 #pragma unroll
-        for (int c = 0; c < NK; ++c) {
-            const int byte = 32 * c + 16 * h;  // (columns of 16 bits: 16 c + 8 h)
-            const bool ok = there && byte < (E4M3 ? p.D : 2 * p.D);
-            kr[c] = *static_cast<const u32x4*>(ok ? p.pages.k + at + byte : none);
-            if constexpr (E4M3) ks[c] = *static_cast<const uint8_t*>(ok ? p.pages.ks + sat + c : none);
-        }
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int y = lane + 64 * i, r = y / PC, c = y % PC, vkey = 32 * t + r, vrow = vkey - p.pages.page_of(vkey) * p.pages.size;
-            const int vpage = __shfl(page, r);
-            const bool ok = (uint32_t)vpage < (uint32_t)p.pages.pages && 16 * c < (E4M3 ? p.D : 2 * p.D);
-            vr[i] = *static_cast<const u32x4*>(ok ? p.pages.v + vpage * p.pages.sp + head + vrow * p.pages.sr + 16 * c : none);
-            if constexpr (E4M3)
-                vs[i] = *static_cast<const uint8_t*>(ok ? p.pages.vs + vpage * p.pages.scale_sp + scale_head + vrow * p.pages.scale_sr + c / 2 : none);
+        for (int u = 0; u < 2; ++u) {
+            const int key = 32 * t + 16 * u + y;
+            page[u] = key < n ? table[p.pages.page_of(key)] : -1;
         }
     };
-    int t = part.first + wave, page = t < part.end ? look(t) : -1;
-    if (t < part.end) load(t, page);
-    if (t + WAVES < part.end) page = look(t + WAVES);
-    SeqSums<HD> st;
-    elem_t* V = region + wave * kRegion;
-    const Tile<HD, false> tile(lane);
+    const auto load = [&](int t) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int key = 32 * t + 16 * u + y, row = key - p.pages.page_of(key) * p.pages.size;
+            const bool there = (uint32_t)page[u] < (uint32_t)p.pages.pages;
+            const int64_t at = page[u] * p.pages.sp + row * p.pages.sr;
+#pragma unroll
+            for (int c = 0; c < NP; ++c) {
+                if (E4M3 && KC % 2 && c == NP - 1) {
+                    const int byte = 32 * (KC - 1) + 8 * g;
+                    const bool ok = there && byte < p.D;
+                    const u32x2 a = global<u32x2>(ok ? kp + at + byte : none), d = global<u32x2>(ok ? vp + at + byte : none);
+                    kr[u][c] = u32x4{a[0], a[1], 0u, 0u}, vr[u][c] = u32x4{d[0], d[1], 0u, 0u};
+                } else {
+                    const int byte = 64 * c + 16 * g;
+                    const bool ok = there && byte < (E4M3 ? p.D : 2 * p.D);
+                    kr[u][c] = global<u32x4>(ok ? kp + at + byte : none);
+                    vr[u][c] = global<u32x4>(ok ? vp + at + byte : none);
+                }
+            }
+            if constexpr (E4M3) {
+                const int64_t sat = page[u] * p.pages.scale_sp + row * p.pages.scale_sr;
+                ks[u] = scale_codes<KC>(there ? ksp + sat : none, p.pages.scale_words);
+                vs[u] = scale_codes<KC>(there ? vsp + sat : none, p.pages.scale_words);
+            }
+        }
+    };
+    // step c's eight numbers of a row, from its pieces
+    const auto operand = [&](const u32x4* r, uint32_t codes, int c) {
+        if constexpr (!E4M3) return r[c];
+        if (KC % 2 && c == KC - 1) return from_e4m3_8<T>(r[c / 2][0], r[c / 2][1], scale_of(codes >> (8 * c) & 0xffu));
+        // columns 64 (c / 2) + 16 g ..: the first or the second group of 32 of the pair
+        return from_e4m3_8<T>(r[c / 2][2 * (c % 2)], r[c / 2][2 * (c % 2) + 1], scale_of(codes >> (16 * (c / 2) + 8 * (g >> 1)) & 0xffu));
+    };
+    int t = part.first + wave;
+    if (t < part.end) {
+        look(t);
+        load(t);
+    }
+    if (t + WAVES < part.end) look(t + WAVES);
+    f32x4 acc[NC][DT] = {};
+    float m[NC], ref[NC], l[NC];
+#pragma unroll
+    for (int i = 0; i < NC; ++i) m[i] = -INFINITY, ref[i] = 0.0f, l[i] = 0.0f;
+    elem_t* V = region + wave * 32 * kLd;
+    // transposing reads: lane 4j + i of 16 supplies row 4g + j, columns 4i .. 4i+3, lane i receives column i
+    const elem_t* tr = V + (4 * g + (y >> 2)) * kLd + 4 * (y & 3);
     for (; t < part.end; t += WAVES) {
-        f32x16 s[1] = {};
+        f32x4 s[NC][2] = {};
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int y = lane + 64 * i;
-            if constexpr (E4M3) {
-                elem_t* to = V + (y / PC) * (HD + 8) + 16 * (y % PC);
-                const float scale = scale_of(vs[i]);
-                *reinterpret_cast<u32x4*>(to) = from_e4m3_8<T>(vr[i][0], vr[i][1], scale);
-                *reinterpret_cast<u32x4*>(to + 8) = from_e4m3_8<T>(vr[i][2], vr[i][3], scale);
-            } else {
-                *reinterpret_cast<u32x4*>(V + (y / PC) * (HD + 8) + 8 * (y % PC)) = vr[i];
-            }
-        }
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int c = 0; c < NK; ++c) {
-            if constexpr (E4M3) {
-                const float scale = scale_of(ks[c]);
-                s[0] = Mma32<T>::run(from_e4m3_8<T>(kr[c][0], kr[c][1], scale), own[2 * c], s[0]);
-                s[0] = Mma32<T>::run(from_e4m3_8<T>(kr[c][2], kr[c][3], scale), own[2 * c + 1], s[0]);
-            } else {
-                s[0] = Mma32<T>::run(kr[c], own[c], s[0]);
+            for (int c = 0; c < KC; ++c) {
+                *reinterpret_cast<u32x4*>(V + (16 * u + y) * kLd + column(c)) = operand(vr[u], vs[u], c);
+                const u32x4 k = operand(kr[u], ks[u], c);
+#pragma unroll
+                for (int i = 0; i < NC; ++i) s[i][u] = T::mfma16(k, own[i][c], s[i][u]);
             }
-        }
         if (t + WAVES < part.end) {
-            load(t + WAVES, page);
-            if (t + 2 * WAVES < part.end) page = look(t + 2 * WAVES);
+            load(t + WAVES);
+            if (t + 2 * WAVES < part.end) look(t + 2 * WAVES);
         }
-        if (32 * t + 32 <= whole) st.template take<false>(s, p.c, 0, h);
-        else st.template take<true>(s, p.c, limit - 32 * t, h);
+        const bool masked = 32 * t + 32 > whole;
+        u32x4 pr[NC];
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            if (masked) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (32 * t + 16 * u + 4 * g + j >= limit[i]) s[i][u][j] = -INFINITY;
+            }
+            float top = s[i][0][0];
+#pragma unroll
+            for (int j = 1; j < 8; ++j) top = fmaxf(top, s[i][j >> 2][j & 3]);
+            top *= p.c;
+            if (__builtin_amdgcn_ballot_w64(top > m[i] + 8.0f)) {
+                const float grown = fmaxf(m[i], quarters_max(top)), now = grown == -INFINITY ? 0.0f : grown;
+                const float f = m[i] == -INFINITY ? 0.0f : fast_exp2(ref[i] - now);
+                m[i] = grown, ref[i] = now;
+                l[i] *= f;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) acc[i][d] *= f;
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    s[i][u][j] = fast_exp2(__builtin_fmaf(s[i][u][j], p.c, -ref[i]));
+                    l[i] += s[i][u][j];
+                }
+            pr[i] = pack_b16<T>(s[i][0], s[i][1]);
+        }
         wave_exchange();
-        add_columns<T>(st.acc, tile, V, 0, s[0]);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+            typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+            const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tr + 16 * d)));
+            const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tr + 16 * kLd + 16 * d)));
+            const u32x4 v = {lo[0], lo[1], hi[0], hi[1]};
+#pragma unroll
+            for (int i = 0; i < NC; ++i) acc[i][d] = T::mfma16(v, pr[i], acc[i][d]);
+        }
         wave_exchange();
     }
-    const float l = halves_sum(st.l);
     workgroup_barrier();  // the sums take the place of the V tiles
-    if (h == 0) {
-        stats[wave * 32 + lane] = st.m == -INFINITY ? -INFINITY : st.ref;
-        stats[(WAVES + wave) * 32 + lane] = l;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+        const float sum = quarters_sum(l[i]);
+        if (g == 0) {
+            stats[wave * R + 16 * i + y] = m[i] == -INFINITY ? -INFINITY : ref[i];
+            stats[(WAVES + wave) * R + 16 * i + y] = sum;
+        }
+#pragma unroll
+        for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(sums + (wave * R + 16 * i + y) * kSum + 16 * d + 4 * g) = acc[i][d];
     }
-    float* out = sums + (wave * 32 + (lane & 31)) * kSum + 4 * h;
-#pragma unroll
-    for (int dt = 0; dt < HD / 32; ++dt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            *reinterpret_cast<f32x4*>(out + 32 * dt + 8 * i) =
-                f32x4{st.acc[dt][4 * i], st.acc[dt][4 * i + 1], st.acc[dt][4 * i + 2], st.acc[dt][4 * i + 3]};
     workgroup_barrier();
-    for (int y = tid; y < rows * CH; y += 64 * WAVES) {
-        const int row = y / CH, c8 = 8 * (y % CH);
+    for (int z = tid; z < rows * CH; z += 64 * WAVES) {
+        const int row = z / CH, c8 = 8 * (z % CH);
         float top = -INFINITY, sum = 0.0f, o[8] = {};
 #pragma unroll
-        for (int k = 0; k < WAVES; ++k) top = fmaxf(top, stats[k * 32 + row]);
-        const float ref = top == -INFINITY ? 0.0f : top;
+        for (int k = 0; k < WAVES; ++k) top = fmaxf(top, stats[k * R + row]);
+        const float base = top == -INFINITY ? 0.0f : top;
 #pragma unroll
         for (int k = 0; k < WAVES; ++k) {
-            const float f = fast_exp2(stats[k * 32 + row] - ref);
-            sum += f * stats[(WAVES + k) * 32 + row];
+            const float f = fast_exp2(stats[k * R + row] - base);
+            sum += f * stats[(WAVES + k) * R + row];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) o[j] += f * sums[(k * 32 + row) * kSum + c8 + j];
+            for (int j = 0; j < 8; ++j) o[j] += f * sums[(k * R + row) * kSum + c8 + j];
         }
         const SeqRow to(p, hk, r0 + row);
         if (p.splits > 1) {

@@ -1,5 +1,7 @@
 // Launches of the attention over packed sequences and over a paged cache, for the translation units.
 #pragma once
+#include <algorithm>
+#include <climits>
 #include "sjvp_ctx_launch.hpp"
 #include "sjvp_seq.hpp"
 
@@ -7,6 +9,9 @@ namespace sjvp {
 
 // Blocks of R rows that the segments of a call can have (see seq_block).
 inline int64_t seq_slots(const SeqParams& p, int heads, int R) { return (int64_t)p.T * heads / R + p.B + 2; }
+
+// Sets of 16 rows to a block of seq_few.
+inline int seq_sets(const SeqParams& p) { return (int64_t)p.T * p.G <= 16 * (int64_t)p.B ? 1 : 2; }
 
 inline bool seq_dma(const SeqParams& p, const CtxView& a, const CtxView& b) {
     return p.D % 8 == 0 && ctx_padded(p.D) != 96 && ctx_aligned(a) && ctx_aligned(b);

@@ -22,10 +22,17 @@ int seq_paged<SJVP_T>(SeqParams p, bool e4m3, bool few, bool many, hipStream_t s
         constexpr bool DMA = HD != 96;  // (twelve pieces to a row do not fit the permutation of LDS-DMA tiles)
         int rc = SJVP_OK;
         if (few) {
-            p.slots = (int)seq_slots(p, p.G, 32), p.least = 0, p.most = many ? kSeqFew : INT_MAX;
-            const int grid = p.slots * p.Hkv * splits, smem = kCtxWaves * 32 * (HD + 4 + 2) * 4;
-            rc = e4m3 ? launch(seq_few<SJVP_T, HD, true, kCtxWaves>, grid, smem, stream, p, kCtxThreads)
-                      : launch(seq_few<SJVP_T, HD, false, kCtxWaves>, grid, smem, stream, p, kCtxThreads);
+            const auto run = [&](auto sets, auto bits8) {
+                constexpr int NC = decltype(sets)::value;
+                p.slots = (int)seq_slots(p, p.G, 16 * NC), p.least = 0, p.most = many ? kSeqFew : INT_MAX;
+                const int smem = kCtxWaves * std::max(32 * (HD + 8) * 2, 16 * NC * (HD + 4 + 2) * 4);
+                return launch(seq_few<SJVP_T, HD, decltype(bits8)::value, NC, kCtxWaves>, p.slots * p.Hkv * splits, smem, stream, p, kCtxThreads);
+            };
+            const std::integral_constant<int, 1> one;
+            const std::integral_constant<int, 2> two;
+            const std::true_type yes;
+            const std::false_type no;
+            rc = seq_sets(p) == 1 ? e4m3 ? run(one, yes) : run(one, no) : e4m3 ? run(two, yes) : run(two, no);
             if (rc != SJVP_OK) return rc;
         }
         if (many) {
