@@ -1,6 +1,7 @@
 // C ABI of the attention over packed sequences and over a paged cache: checks, how the work is split, and the launches.
 #include <climits>
 #include <cmath>
+#include <cstdlib>
 
 #include "sjvp_seq_launch.hpp"
 
@@ -75,7 +76,7 @@ int paged_params(const sjvp_paged* t, SeqParams& p, int T) {
 // four waves share their tiles, takes the longer sequences where blocks of 128 rows fill half of the compute units.
 struct PagedPlan {
     bool few = true, many = false;
-    int splits = 1;
+    int splits = 1, split_tiles = 1;
     size_t stat = 0, part = 0, used = 0, total = 0;  // floats
 };
 
@@ -84,7 +85,8 @@ PagedPlan paged_plan(const SeqParams& p) {
     const int64_t rows = (int64_t)p.T * p.G;
     plan.many = p.T > p.B && 2 * ceil_div(rows, kCtxOwned) * p.Hkv > compute_units();
     const int64_t blocks = (p.B + rows / 32) * p.Hkv;
-    plan.splits = (int)std::max<int64_t>(1, std::min<int64_t>({8 * (int64_t)compute_units() / blocks, p.pages.capacity / 512, 64}));
+    plan.split_tiles = 8;
+    plan.splits = (int)std::max<int64_t>(1, std::min<int64_t>({8 * (int64_t)compute_units() / blocks, p.pages.capacity / (32 * plan.split_tiles), 128}));
     if (plan.splits > 1) {
         const auto take = [&](int64_t floats) {
             const size_t at = plan.total;
@@ -96,6 +98,22 @@ PagedPlan paged_plan(const SeqParams& p) {
         plan.part = take(plan.splits * places * ctx_padded(p.D));
         plan.used = take(places);
     }
+    return plan;
+}
+
+// The backward of whole sequences: the column-owned launch is split over the heads that share a key head.
+struct PackedPlan {
+    int splits = 1;
+    size_t part = 0, total = 0;  // floats
+};
+
+PackedPlan packed_plan(const SeqParams& p) {
+    PackedPlan plan;
+    const int64_t blocks = (p.T / kCtxOwned + 1) * (int64_t)p.Hkv;
+    static const int CU = getenv("CUX") ? atoi(getenv("CUX")) : 4; // XXX
+    plan.splits = (int)std::max<int64_t>(1, std::min<int64_t>(CU * (int64_t)compute_units() / blocks, p.G));
+    plan.part = (3 * (size_t)p.Hq * p.T + 3) / 4 * 4;
+    plan.total = plan.part + (plan.splits > 1 ? 2 * (size_t)plan.splits * p.Hkv * p.T * ctx_padded(p.D) : 0);
     return plan;
 }
 
@@ -112,7 +130,7 @@ using namespace sjvp;
 
 size_t sjvp_packed_workspace_bytes(const sjvp_packed* t, int backward) {
     SeqParams p{};
-    return backward && packed_params(t, p) == SJVP_OK ? 4 * 3 * (size_t)p.Hq * p.T : 0;
+    return backward && packed_params(t, p) == SJVP_OK ? 4 * packed_plan(p).total : 0;
 }
 
 int sjvp_packed_fwd(const sjvp_packed* t, int dtype, void* stream) {
@@ -131,8 +149,9 @@ int sjvp_packed_bwd(const sjvp_packed* t, int dtype, void* stream) {
     if (rc != SJVP_OK) return rc;
     if (dtype != SJVP_BF16 && dtype != SJVP_FP16) return SJVP_ERR_DTYPE;
     if (!t->q || !t->k || !t->v || !t->o || !t->dO || !t->dq || !t->dk != !t->dv || !t->lse || !t->offsets) return SJVP_ERR_NULL;
-    if (seq_workspace(t->workspace, t->workspace_bytes, 3 * (size_t)p.Hq * p.T) != SJVP_OK) return SJVP_ERR_WORKSPACE;
-    p.folded = static_cast<float*>(t->workspace);
+    const PackedPlan plan = packed_plan(p);
+    if (seq_workspace(t->workspace, t->workspace_bytes, plan.total) != SJVP_OK) return SJVP_ERR_WORKSPACE;
+    p.splits = plan.splits, p.folded = static_cast<float*>(t->workspace), p.part = p.folded + plan.part;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     return dtype == SJVP_BF16 ? seq_packed_bwd<Bf16>(p, s) : seq_packed_bwd<Fp16>(p, s);
 }
@@ -171,7 +190,7 @@ int sjvp_paged_attention(const sjvp_paged* t, int dtype, void* stream) {
     const PagedPlan plan = paged_plan(p);
     if (seq_workspace(t->workspace, t->workspace_bytes, plan.total) != SJVP_OK) return SJVP_ERR_WORKSPACE;
     float* ws = static_cast<float*>(t->workspace);
-    p.splits = plan.splits;
+    p.splits = plan.splits, p.split_tiles = plan.split_tiles;
     p.stat = ws + plan.stat, p.part = ws + plan.part, p.used = reinterpret_cast<int*>(ws + plan.used);
     const hipStream_t s = static_cast<hipStream_t>(stream);
     return dtype == SJVP_BF16 ? seq_paged<Bf16>(p, p.pages.ks, plan.few, plan.many, s) : seq_paged<Fp16>(p, p.pages.ks, plan.few, plan.many, s);

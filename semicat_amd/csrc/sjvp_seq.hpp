@@ -42,7 +42,7 @@ struct SeqParams {
     const int *offsets, *lengths;       // offsets null: one row each
     int B, T, Hq, Hkv, G, D, causal;
     float scale, c;                     // c = scale * log2(e)
-    int slots, splits;
+    int slots, splits, split_tiles;     // split_tiles: tiles of 32 keys that a split has at least
     int least, most;                    // query rows (of all heads of a group) of the sequences that a launch serves
     SeqPages pages;
 };
@@ -53,27 +53,33 @@ __device__ __forceinline__ int seq_offset(const SeqParams& p, int x) {
     return min(max(p.offsets ? p.offsets[x - 1] : x - 1, 0), p.T);
 }
 
-// The block of R rows (of `heads` rows to a token) that a workgroup serves.
+// The block of R rows (of `heads` rows to a token) that a workgroup serves, and the length that the cache has of its sequence.  In the last step of the
+// search the lanes hold the offsets and lengths of neighbouring segments, so that a workgroup waits for memory once (up to 62 sequences) before it
+// knows its rows and keys.
 struct SeqBlock {
     int segment, token, tokens, row0;  // first token and number of tokens of the segment; first row of the block within it
+    int held;
     bool some;
 };
-template <int R>
+template <int R, bool PAGED = false>
 __device__ __forceinline__ SeqBlock seq_block(const SeqParams& p, int slot, int heads, int lane) {
     int lo = 0, hi = p.B + 2;  // the segment lies in [lo, hi)
-    while (hi - lo > 1) {
+    while (hi - lo > 64) {
         const int step = (hi - lo + 63) / 64, x = lo + lane * step;
         const bool there = x < hi && seq_offset(p, x) * heads / R + x <= slot;
         const int n = __popcll(__builtin_amdgcn_ballot_w64(there || lane == 0));
         lo += (n - 1) * step;
         hi = min(hi, lo + step);
     }
-    lo = __builtin_amdgcn_readfirstlane(lo);
+    const int x = lo + lane, at = seq_offset(p, x), next = seq_offset(p, x + 1);
+    const int held = PAGED && x >= 1 && x <= p.B ? p.lengths[x - 1] : 0;
+    const int mine = __popcll(__builtin_amdgcn_ballot_w64(lane == 0 || (x < hi && at * heads / R + x <= slot))) - 1;
     SeqBlock b;
-    b.segment = lo;
-    b.token = __builtin_amdgcn_readfirstlane(seq_offset(p, lo));
-    b.tokens = max(0, __builtin_amdgcn_readfirstlane(seq_offset(p, lo + 1)) - b.token);
-    b.row0 = (slot - (b.token * heads / R + lo)) * R;
+    b.segment = __builtin_amdgcn_readfirstlane(lo + mine);
+    b.token = __builtin_amdgcn_readlane(at, mine);
+    b.tokens = max(0, __builtin_amdgcn_readlane(next, mine) - b.token);
+    b.held = __builtin_amdgcn_readlane(held, mine);
+    b.row0 = (slot - (b.token * heads / R + b.segment)) * R;
     b.some = b.row0 >= 0 && b.row0 < b.tokens * heads;  // (descending offsets may lead to a segment that begins behind the slot)
     return b;
 }
@@ -85,7 +91,7 @@ struct SeqKeys {
     __device__ __forceinline__ SeqKeys(const SeqParams& p, const SeqBlock& b) {
         const bool sequence = b.segment >= 1 && b.segment <= p.B;
         if constexpr (PAGED) {
-            keys = sequence ? min(max(p.lengths[b.segment - 1], 0), p.pages.capacity) : 0;
+            keys = sequence ? min(max(b.held, 0), p.pages.capacity) : 0;
             start = keys - b.tokens;
         } else {
             keys = sequence ? b.tokens : 0;

@@ -135,34 +135,41 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 3 : 2) void seq_bwd_row(Seq
     });
 }
 
-// Column-owned: four waves of 32 keys share tiles of 64 query rows, over all heads that read the key head.
-template <typename T, int HD, bool DMA>
-__global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void seq_bwd_col(SeqParams p) {
+// Column-owned: groups of 32 keys share tiles of 64 query rows, over all heads that read the key head (or, with splits, over a part of them).  A group is
+// one wave, or two that take 32 rows of a tile each and add their sums up in the end: at D = 128 the sums and operands of 32 keys fill the
+// registers of two waves to a SIMD either way, and two waves fill each other's gaps.
+template <typename T, int HD, bool DMA, int PAIR>
+__global__ __launch_bounds__(kCtxThreads * PAIR, HD <= 64 ? 2 * PAIR : PAIR) void seq_bwd_col(SeqParams p) {
     if constexpr (DMA) __builtin_assume(p.D % 8 == 0);
     extern __shared__ __align__(16) unsigned char smem[];
-    constexpr int kTile = Tile<HD, DMA>::kElems;
+    constexpr int kTile = Tile<HD, DMA>::kElems, NT = kCtxThreads * PAIR, U = 2 / PAIR;
     elem_t* tiles = reinterpret_cast<elem_t*>(smem);             // [2][Q, dO]
-    float* stats = reinterpret_cast<float*>(tiles + 4 * kTile);  // [2][row_stat_folded, -delta][64]
+    elem_t* mine = tiles + 4 * kTile;                            // PAIR == 2: K [2], V [2] of the workgroup's keys
+    float* stats = reinterpret_cast<float*>(mine + (PAIR == 2 ? 4 * kTile : 0));  // [2][row_stat_folded, -delta][64]
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
-    const int hk = blockIdx.x % p.Hkv, slot = blockIdx.x / p.Hkv;
+    const int group = wave % kCtxWaves, half = wave / kCtxWaves;
+    const int hk = blockIdx.x % p.Hkv, slot = blockIdx.x / p.Hkv % p.slots, split = blockIdx.x / p.Hkv / p.slots;
     const SeqBlock b = seq_block<kCtxOwned>(p, slot, 1, lane);
     if (!b.some) return;
     const SeqKeys<false> keys(p, b);
-    const int k0 = b.row0 + 32 * wave, key = k0 + (lane & 31);
+    const int k0 = b.row0 + 32 * group, key = k0 + (lane & 31);
     const bool ok = key < keys.keys;
-    u32x4 own_k[HD / 16], own_v[HD / 16];
-    own_operands<HD>(own_k, p.k.head(0, hk) + (int64_t)(b.token + key) * p.k.sl, ok, h, p.D);
-    own_operands<HD>(own_v, p.v.head(0, hk) + (int64_t)(b.token + key) * p.v.sl, ok, h, p.D);
+    u32x4 own_k[PAIR == 1 ? HD / 16 : 1], own_v[PAIR == 1 ? HD / 16 : 1];
+    if constexpr (PAIR == 1) {
+        own_operands<HD>(own_k, p.k.head(0, hk) + (int64_t)(b.token + key) * p.k.sl, ok, h, p.D);
+        own_operands<HD>(own_v, p.v.head(0, hk) + (int64_t)(b.token + key) * p.v.sl, ok, h, p.D);
+    }
     // tiles of query rows that see a key of the workgroup, head by head
     const int ta = p.causal ? b.row0 / kCtxTile : 0, tb = (keys.keys + kCtxTile - 1) / kCtxTile, per_head = max(0, tb - ta);
-    const int nx = p.G * per_head;
+    const int first_head = hk * p.G + p.G * split / p.splits, heads = hk * p.G + p.G * (split + 1) / p.splits - first_head;
+    const int nx = heads * per_head;
 
-    TileFeed<HD, DMA> qf(p.q.sl, p.D, tid), gf(p.g.sl, p.D, tid);
+    TileFeed<HD, DMA, NT> qf(p.q.sl, p.D, tid), gf(p.g.sl, p.D, tid);
     const Tile<HD, DMA> at(lane);
     float stat = 0.0f;
     const auto place = [&](int x) { return tiles + (x & 1) * 2 * kTile; };
     const auto request = [&](int x) {
-        const int hq = hk * p.G + x / per_head, r0 = (ta + x % per_head) * kCtxTile;
+        const int hq = first_head + x / per_head, r0 = (ta + x % per_head) * kCtxTile;
         const int64_t token = b.token + r0;
         qf.request(p.q.head(0, hq) + token * p.q.sl, p.q.sl, b.tokens - r0, p.D, place(x), wave);
         gf.request(p.g.head(0, hq) + token * p.g.sl, p.g.sl, b.tokens - r0, p.D, place(x) + kTile, wave);
@@ -180,8 +187,28 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void seq_bwd_col(Seq
     if (nx) {
         request(0);
         deliver(0);
+        if constexpr (PAIR == 2) {
+            TileFeed<HD, DMA, NT> kf(p.k.sl, p.D, tid), vf(p.v.sl, p.D, tid);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int k = b.row0 + i * kCtxTile;
+                kf.request(p.k.head(0, hk) + (int64_t)(b.token + k) * p.k.sl, p.k.sl, keys.keys - k, p.D, mine + i * kTile, wave);
+                vf.request(p.v.head(0, hk) + (int64_t)(b.token + k) * p.v.sl, p.v.sl, keys.keys - k, p.D, mine + (2 + i) * kTile, wave);
+                kf.deliver(mine + i * kTile, p.D, tid);
+                vf.deliver(mine + (2 + i) * kTile, p.D, tid);
+            }
+        }
         qf.arrived();
     }
+    const elem_t *own_kt = mine + group / 2 * kTile, *own_vt = own_kt + 2 * kTile;
+    const int own_row = 32 * (group & 1);
+    // scores of 32 rows of a tile and the wave's keys
+    const auto products = [&](const elem_t* rows, int row, const u32x4* own, const elem_t* own_tile, f32x16 x) {
+        if constexpr (PAIR == 1) return scores<T>(at, rows, row, own, x);
+#pragma unroll
+        for (int c = 0; c < HD / 16; ++c) x = Mma32<T>::run(at.rows(rows, row, c), at.rows(own_tile, own_row, c), x);
+        return x;
+    };
     f32x16 dk[HD / 32] = {}, dv[HD / 32] = {};
     constexpr bool kFactors = HD > 64;
     const auto tile = [&](int x, auto masked) {
@@ -189,40 +216,42 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void seq_bwd_col(Seq
         if (x + 1 < nx) request(x + 1);
         const elem_t* Q = place(x);
         const float* st = stats + (x & 1) * (kCtxStats / 2);
-        if (k0 < keys.keys && !(decltype(masked)::value && r0 + kCtxTile <= k0)) {
-            const bool factors = __builtin_amdgcn_ballot_w64(st[kCtxTile + lane] != 1.0f);
-            f32x16 s[2], ds[2];
+        const bool factors = !kFactors && __builtin_amdgcn_ballot_w64(st[kCtxTile + lane] != 1.0f);
+        const int row0 = PAIR == 2 ? 32 * half : 0, end = row0 + 32 * U;  // rows of the tile that are this wave's
+        if (k0 < keys.keys && !(decltype(masked)::value && r0 + end <= k0)) {
+            f32x16 s[U], ds[U];
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                s[u] = scores<T>(at, Q, 32 * u, own_k);
-                ds[u] = scores<T>(at, Q + kTile, 32 * u, own_v, seq_of_rows(st + 2 * kCtxTile + 32 * u, h));
+            for (int u = 0; u < U; ++u) {
+                s[u] = products(Q, row0 + 32 * u, own_k, own_kt, f32x16{});
+                ds[u] = products(Q + kTile, row0 + 32 * u, own_v, own_vt, seq_of_rows(st + 2 * kCtxTile + row0 + 32 * u, h));
             }
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
+            for (int u = 0; u < U; ++u) {
+                const float* sr = st + row0 + 32 * u;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const f32x4 less = *reinterpret_cast<const f32x4*>(st + 32 * u + 8 * i + 4 * h);
+                    const f32x4 less = *reinterpret_cast<const f32x4*>(sr + 8 * i + 4 * h);
                     f32x4 factor;
-                    if constexpr (kFactors) factor = *reinterpret_cast<const f32x4*>(st + kCtxTile + 32 * u + 8 * i + 4 * h);
+                    if constexpr (kFactors) factor = *reinterpret_cast<const f32x4*>(sr + kCtxTile + 8 * i + 4 * h);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         float y = fast_exp2(__builtin_fmaf(s[u][4 * i + j], p.c, -less[j]));
                         if constexpr (kFactors) y *= factor[j];
                         ds[u][4 * i + j] *= y;
                         if constexpr (decltype(masked)::value)
-                            if (32 * u + 8 * i + j < key - r0 - 4 * h) y = 0.0f, ds[u][4 * i + j] = 0.0f;  // a row ahead of the key
+                            if (row0 + 32 * u + 8 * i + j < key - r0 - 4 * h) y = 0.0f, ds[u][4 * i + j] = 0.0f;  // a row ahead of the key
                         s[u][4 * i + j] = y;
                     }
                 }
                 if (!kFactors && factors) {
-                    const f32x16 factor = seq_of_rows(st + kCtxTile + 32 * u, h);
+                    const f32x16 factor = seq_of_rows(sr + kCtxTile, h);
                     s[u] *= factor, ds[u] *= factor;
                 }
             }
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                add_columns<T>(dv, at, Q + kTile, 32 * u, s[u]);
-                add_columns<T>(dk, at, Q, 32 * u, ds[u]);
+            for (int u = 0; u < U; ++u) {
+                add_columns<T>(dv, at, Q + kTile, row0 + 32 * u, s[u]);
+                add_columns<T>(dk, at, Q, row0 + 32 * u, ds[u]);
             }
         }
         if (x + 1 < nx) deliver(x + 1);
@@ -239,11 +268,64 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 2 : 1) void seq_bwd_col(Seq
     }
     const bool scored = ok && keys.keys != 1;
     const int out_rows = min(max(b.tokens - k0, 0), 32);
-    elem_t* region = tiles + wave * 32 * (HD + 8);
-    store_rows_at<T, HD>(dk, scored ? p.scale : 0.0f, out_rows, region, lane, p.D,
-                         [&](int row) { return p.dk.head(0, hk) + (int64_t)(b.token + k0 + row) * p.dk.sl; });
-    store_rows_at<T, HD>(dv, ok ? 1.0f : 0.0f, out_rows, region, lane, p.D,
-                         [&](int row) { return p.dv.head(0, hk) + (int64_t)(b.token + k0 + row) * p.dv.sl; });
+    elem_t* region = tiles + group * 32 * (HD + 8);
+    const auto finish = [&](f32x16* sum, bool some, float factor, const CtxView& out, int which) {
+        if constexpr (PAIR == 2) {
+            // [group][register][lane]: the sums of the second waves take the place of the tiles
+            f32x4* there = reinterpret_cast<f32x4*>(tiles) + group * (HD / 32) * 4 * 64 + lane;
+            if (half)
+#pragma unroll
+                for (int dt = 0; dt < HD / 32; ++dt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        there[(4 * dt + i) * 64] = f32x4{sum[dt][4 * i], sum[dt][4 * i + 1], sum[dt][4 * i + 2], sum[dt][4 * i + 3]};
+            workgroup_barrier();
+            if (!half)
+#pragma unroll
+                for (int dt = 0; dt < HD / 32; ++dt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const f32x4 other = there[(4 * dt + i) * 64];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) sum[dt][4 * i + j] += other[j];
+                    }
+            workgroup_barrier();
+        }
+        if (half == 0) {
+            if (p.splits > 1) {
+                const int64_t place = ((int64_t)(2 * split + which) * p.Hkv + hk) * p.T + b.token + k0;
+                store_part<HD>(sum, some, p.part + place * HD, out_rows, lane);
+            } else {
+                store_rows_at<T, HD>(sum, some ? factor : 0.0f, out_rows, region, lane, p.D,
+                                     [&](int row) { return out.head(0, hk) + (int64_t)(b.token + k0 + row) * out.sl; });
+            }
+        }
+        if constexpr (PAIR == 2) workgroup_barrier();
+    };
+    finish(dk, scored, p.scale, p.dk, 0);
+    finish(dv, ok, 1.0f, p.dv, 1);
+}
+
+// Adds up the splits of seq_bwd_col, eight columns to a thread, in a fixed order.
+template <typename T, int HD>
+__global__ __launch_bounds__(kCtxThreads) void seq_sum(SeqParams p) {
+    constexpr int CH = HD / 8;
+    const int64_t x = (int64_t)blockIdx.x * kCtxThreads + threadIdx.x, rows = (int64_t)p.Hkv * p.T, place = x / CH;  // [dk, dv][Hkv][T]
+    const int c8 = 8 * (int)(x % CH);
+    if (place >= 2 * rows) return;
+    float y[8] = {};
+    for (int s = 0; s < p.splits; ++s) {
+        const f32x4* from = reinterpret_cast<const f32x4*>(p.part + (2 * s * rows + place) * HD + c8);
+        const f32x4 a = from[0], c = from[1];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] += a[j], y[4 + j] += c[j];
+    }
+    const bool v = place >= rows;
+    const int64_t row = v ? place - rows : place;
+    const float f = v ? 1.0f : p.scale;
+    const CtxView& out = v ? p.dv : p.dk;
+    store_chunk(out.head(0, (int)(row / p.T)) + row % p.T * out.sl,
+                u32x4{T::pack2(f * y[0], f * y[1]), T::pack2(f * y[2], f * y[3]), T::pack2(f * y[4], f * y[5]), T::pack2(f * y[6], f * y[7])}, c8, p.D);
 }
 
 }  // namespace sjvp

@@ -22,7 +22,7 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 4 : 2) void seq_fwd(SeqPara
     elem_t* tiles = reinterpret_cast<elem_t*>(smem);  // K [2], V [2]
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
     const int hk = blockIdx.x % p.Hkv, slot = p.causal ? p.slots - 1 - (int)(blockIdx.x / p.Hkv) : blockIdx.x / p.Hkv;  // causal: long rows first
-    const SeqBlock b = seq_block<kCtxOwned>(p, slot, p.G, lane);
+    const SeqBlock b = seq_block<kCtxOwned, PAGED>(p, slot, p.G, lane);
     const int all = b.tokens * p.G;
     if (!b.some || all < p.least || all > p.most) return;
     const SeqKeys<PAGED> keys(p, b);
@@ -81,12 +81,11 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 4 : 2) void seq_fwd(SeqPara
     });
 }
 
-// Splits of the tiles of 32 keys of a sequence: of kSeqLeast tiles or more, as many as the launch has at most.
-constexpr int kSeqLeast = 16;
+// Splits of the tiles of 32 keys of a sequence: of split_tiles or more, as many as the launch has at most.
 struct SeqSplit {
     int used, first, end;
-    __device__ __forceinline__ SeqSplit(int tiles, int splits, int split) {
-        const int per = max(kSeqLeast, (tiles + splits - 1) / splits);
+    __device__ __forceinline__ SeqSplit(const SeqParams& p, int tiles, int split) {
+        const int per = max(p.split_tiles, (tiles + p.splits - 1) / p.splits);
         used = max(1, (tiles + per - 1) / per);
         first = min(split * per, tiles), end = min(first + per, tiles);
     }
@@ -126,13 +125,13 @@ __global__ __launch_bounds__(64 * WAVES, NC == 1 ? (E4M3 || HD <= 96 ? 4 : 3) : 
     float* stats = sums + WAVES * R * kSum;  // [WAVES][R] maximum, then sum
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), y = lane & 15, g = lane >> 4;
     const int hk = blockIdx.x % p.Hkv, x = blockIdx.x / p.Hkv, slot = x % p.slots, split = x / p.slots;
-    const SeqBlock b = seq_block<R>(p, slot, p.G, lane);
+    const SeqBlock b = seq_block<R, true>(p, slot, p.G, lane);
     const int all = b.tokens * p.G;
     if (!b.some || all < p.least || all > p.most) return;
     const SeqKeys<true> keys(p, b);
     const int r0 = b.row0, rows = min(all - r0, R);
     const int n = keys.seen(p, (r0 + rows - 1) / p.G), whole = keys.seen(p, r0 / p.G);
-    const SeqSplit part((n + 31) / 32, p.splits, split);
+    const SeqSplit part(p, (n + 31) / 32, split);
     if (split >= part.used) return;
 
     // column of the eight numbers that step c of a contraction over the head dimension has in this lane
