@@ -143,13 +143,129 @@ __device__ __forceinline__ uint32_t scale_codes(const void* at, bool words) {
     return codes;
 }
 
+// A tile of 64 looped rows in LDS, and where this lane reads its operands (tile algebra: sjvp_ctx.hpp).  Rows are unpadded (D in 65 to 96 have rows
+// of 128 columns) and the 16-byte pieces of a row are permuted by it, for both kinds of reads.  LDS serves 256 bytes a cycle: 16 lanes of a
+// row-major read, so 16 neighbouring rows have to be in different places; and 32 lanes of a transposing read, which are four neighbouring rows of 64 bytes,
+// so these four have to be too.  (The permutation of sjvp_device.hpp has the four rows in one or two places, for which the
+// counters show six cycles lost to each transposing read of eight, half of the time that LDS was busy.)
+//
+// The places of a tile are LDS addresses in registers, which move to the tile's next place; what else differs from read to read is constant
+// and stands in the instruction.
+template <int HD>
+struct SeqTile {
+    static constexpr int kLd = HD == 96 ? 128 : HD, kElems = kCtxTile * kLd, kBytes = 2 * kElems, PP = kLd / 8;
+    uint32_t row[HD / 16], lo[HD / 32], hi[HD / 32];
+
+    static __device__ __forceinline__ int swz(int row) {
+        if constexpr (kLd == 128) return (row & 3) << 2 | (row >> 2 & 3);
+        if constexpr (kLd == 64) return (row >> 1 & 1) << 2 | (row >> 2 & 3);
+        return row >> 2 & 3;
+    }
+    __device__ __forceinline__ SeqTile(const elem_t* tile, int lane) {
+        const uint32_t base = lds_addr(tile);
+        const int y = lane & 31, h = lane >> 5, i16 = lane & 15;
+#pragma unroll
+        for (int c = 0; c < HD / 16; ++c) row[c] = base + 2 * (y * kLd + 8 * ((2 * c + h) ^ swz(y)));
+        // within 16 lanes of a transposing read lane 4j + i supplies row j, columns 4i .. 4i+3, and lane n receives column n
+        const int r = 4 * h + (i16 >> 2), chunk = 2 * ((lane >> 4) & 1) + ((i16 & 3) >> 1);
+#pragma unroll
+        for (int z = 0; z < HD / 32; ++z) {
+            lo[z] = base + 2 * (r * kLd + 8 * ((chunk + 4 * z) ^ swz(r)) + 4 * (i16 & 1));
+            hi[z] = base + 2 * ((r + 8) * kLd + 8 * ((chunk + 4 * z) ^ swz(r + 8)) + 4 * (i16 & 1));
+        }
+    }
+    __device__ __forceinline__ void move(int bytes) {
+#pragma unroll
+        for (int c = 0; c < HD / 16; ++c) row[c] += bytes;
+#pragma unroll
+        for (int z = 0; z < HD / 32; ++z) lo[z] += bytes, hi[z] += bytes;
+    }
+    template <typename V>
+    static __device__ __forceinline__ V __attribute__((address_space(3)))* at(uint32_t address) {
+        return (V __attribute__((address_space(3)))*)address;
+    }
+    // A operand: 32 rows, chunk c of 16 columns.  from: bytes from the place to the first of the rows (whole multiples of 16 of them)
+    __device__ __forceinline__ u32x4 rows(int from, int c) const { return *at<const u32x4>(row[c] + from); }
+    // A operand of an output contraction: columns 32 dt .. 32 dt + 31 over 16 rows
+    __device__ __forceinline__ u32x4 columns(int from, int dt) const {
+        const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(at<s16x4>(lo[dt] + from)));
+        const u32x2 b = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(at<s16x4>(hi[dt] + from)));
+        return u32x4{a[0], a[1], b[0], b[1]};
+    }
+    // scores of 32 rows and this lane's own row
+    template <typename T>
+    __device__ __forceinline__ f32x16 scores(int from, const u32x4* own, f32x16 s = {}) const {
+#pragma unroll
+        for (int c = 0; c < HD / 16; ++c) s = Mma32<T>::run(rows(from, c), own[c], s);
+        return s;
+    }
+    // OUT^T += A^T B for a score tile of 32 rows
+    template <typename T>
+    __device__ __forceinline__ void add_columns(f32x16* acc, int from, const f32x16& s) const {
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            const u32x4 b = pack_scores<T>(s, m);
+#pragma unroll
+            for (int dt = 0; dt < HD / 32; ++dt) acc[dt] = Mma32<T>::run(columns(from + m * 16 * kLd * 2, dt), b, acc[dt]);
+        }
+    }
+};
+
+// A tile of 64 rows of a tensor on its way to LDS by NT threads: by LDS-DMA where rows start on 16-byte boundaries, through registers at any
+// alignment otherwise.
+template <int HD, bool DMA, int NT = kCtxThreads>
+struct RowFeed {
+    using At = SeqTile<HD>;
+    static constexpr int PP = At::PP, N = kCtxTile * PP / NT;
+    static_assert(kCtxTile * PP % NT == 0, "every thread copies whole pieces");
+    u32x4 r[DMA ? 1 : N];
+    uint32_t offset[N];
+
+    __device__ __forceinline__ RowFeed(int64_t sl, int D, int tid) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int x = tid + NT * i, row = x / PP, c = x % PP;
+            offset[i] = chunk_offset(row, 8 * (DMA ? c ^ At::swz(row) : c), sl, D);
+        }
+    }
+    __device__ __forceinline__ void request(const elem_t* base, int64_t sl, int rows, int D, elem_t* place, int wave) {
+        if constexpr (DMA) {
+            const u32x4 from = rows_words(base, sl, rows, D);
+            // (as TileFeed::request)
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                asm volatile("s_mov_b32 m0, %2\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
+                             :
+                             : "v"(offset[i]), "s"(from), "s"(__builtin_amdgcn_readfirstlane(lds_addr(place) + 16 * (64 * wave + NT * i)))
+                             : "memory");
+        } else {
+            const Rows from = make_rows(base, sl, rows, D);
+#pragma unroll
+            for (int i = 0; i < N; ++i) r[i] = read_chunk(from, offset[i]);
+        }
+    }
+    __device__ __forceinline__ void deliver(elem_t* place, int D, int tid) {
+        if constexpr (!DMA) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int x = tid + NT * i, row = x / PP, c = x % PP;
+                if (D % 8) r[i] = chunk_shifted(r[i], 8 * c, D);
+                *reinterpret_cast<u32x4*>(place + row * At::kLd + 8 * (c ^ At::swz(row))) = r[i];
+            }
+        }
+    }
+    static __device__ __forceinline__ void arrived() {
+        if constexpr (DMA) __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+    }
+};
+
 // Tiles of 64 keys and values on their way to LDS by four waves.  look() is called a tile ahead of request(), request() ahead of use,
 // deliver() where the places are read next, behind it arrived() and a barrier.
 // From a contiguous tensor (rows of a segment):
 template <int HD, bool DMA>
 struct SeqFeed {
     static constexpr bool kDma = DMA;
-    TileFeed<HD, DMA> kf, vf;
+    RowFeed<HD, DMA> kf, vf;
     const elem_t *k, *v;
     __device__ __forceinline__ SeqFeed(const SeqParams& p, const SeqBlock& b, int hk, int tid)
         : kf(p.k.sl, p.D, tid), vf(p.v.sl, p.D, tid), k(p.k.head(0, hk) + b.token * p.k.sl), v(p.v.head(0, hk) + b.token * p.v.sl) {}
@@ -166,11 +282,11 @@ struct SeqFeed {
 
 // From the pages of a cache, 16-bit numbers (D is a multiple of 8 and rows are aligned): every lane of an LDS-DMA copy has an address of its
 // own, so a tile may lie in any number of pages.
-template <int HD, bool DMA>
+template <int HD>
 struct PageFeed {
-    static constexpr bool kDma = DMA;
-    static constexpr int CH = HD / 8, N = kCtxTile * CH / kCtxThreads;
-    u32x4 kr[DMA ? 1 : N], vr[DMA ? 1 : N];
+    using At = SeqTile<HD>;
+    static constexpr bool kDma = true;
+    static constexpr int CH = At::PP, N = kCtxTile * CH / kCtxThreads;
     int page[N], row[N];
     const int* table;
     int64_t head;
@@ -188,36 +304,23 @@ struct PageFeed {
     __device__ __forceinline__ void request(const SeqParams& p, int, int, elem_t* kp, elem_t* vp, int wave) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int r = (x + kCtxThreads * i) / CH, c = DMA ? (x + kCtxThreads * i) % CH ^ swz<HD>(r) : (x + kCtxThreads * i) % CH;
+            const int r = (x + kCtxThreads * i) / CH, c = (x + kCtxThreads * i) % CH ^ At::swz(r);
             const bool ok = (uint32_t)page[i] < (uint32_t)p.pages.pages && 8 * c < p.D;
             const int64_t at = page[i] * p.pages.sp + head + row[i] * p.pages.sr + 16 * c;
             const void* none = &kZeroPiece;
             const void *from_k = ok ? p.pages.k + at : none, *from_v = ok ? p.pages.v + at : none;
-            if constexpr (DMA) {
-                dma16(from_k, lds_addr(kp) + 16 * (64 * wave + kCtxThreads * i));
-                dma16(from_v, lds_addr(vp) + 16 * (64 * wave + kCtxThreads * i));
-            } else {
-                kr[i] = global<u32x4>(from_k), vr[i] = global<u32x4>(from_v);
-            }
+            dma16(from_k, lds_addr(kp) + 16 * (64 * wave + kCtxThreads * i));
+            dma16(from_v, lds_addr(vp) + 16 * (64 * wave + kCtxThreads * i));
         }
     }
-    __device__ __forceinline__ void deliver(const SeqParams&, elem_t* kp, elem_t* vp, int) {
-        if constexpr (!DMA) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const int y = x + kCtxThreads * i, at = (y / CH) * Tile<HD, false>::kLd + 8 * (y % CH);
-                *reinterpret_cast<u32x4*>(kp + at) = kr[i], *reinterpret_cast<u32x4*>(vp + at) = vr[i];
-            }
-        }
-    }
-    __device__ __forceinline__ void arrived() {
-        if constexpr (DMA) __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
-    }
+    __device__ __forceinline__ void deliver(const SeqParams&, elem_t*, elem_t*, int) {}
+    __device__ __forceinline__ void arrived() { __builtin_amdgcn_s_waitcnt(0x0F70); }  // vmcnt(0)
 };
 
 // From pages of 8-bit numbers (D is a multiple of 16), which become 16-bit ones on their way, once for the four waves.
 template <typename T, int HD>
 struct PageFeed8 {
+    using At = SeqTile<HD>;
     static constexpr bool kDma = false;
     static constexpr int PC = HD / 16, N = (kCtxTile * PC + kCtxThreads - 1) / kCtxThreads;
     u32x4 kr[N], vr[N];
@@ -251,13 +354,14 @@ struct PageFeed8 {
     __device__ __forceinline__ void deliver(const SeqParams&, elem_t* kp, elem_t* vp, int) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int y = x + kCtxThreads * i, at = (y / PC) * Tile<HD, false>::kLd + 16 * (y % PC);
+            const int y = x + kCtxThreads * i, r = y / PC, c = y % PC;
             if (kCtxTile * PC % kCtxThreads && y >= kCtxTile * PC) break;
             const float a = scale_of(ks[i]), b = scale_of(vs[i]);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                *reinterpret_cast<u32x4*>(kp + at + 8 * j) = from_e4m3_8<T>(kr[i][2 * j], kr[i][2 * j + 1], a);
-                *reinterpret_cast<u32x4*>(vp + at + 8 * j) = from_e4m3_8<T>(vr[i][2 * j], vr[i][2 * j + 1], b);
+                const int at = r * At::kLd + 8 * ((2 * c + j) ^ At::swz(r));
+                *reinterpret_cast<u32x4*>(kp + at) = from_e4m3_8<T>(kr[i][2 * j], kr[i][2 * j + 1], a);
+                *reinterpret_cast<u32x4*>(vp + at) = from_e4m3_8<T>(vr[i][2 * j], vr[i][2 * j + 1], b);
             }
         }
     }

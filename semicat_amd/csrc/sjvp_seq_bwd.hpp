@@ -27,7 +27,7 @@ template <typename T, int HD, bool DMA>
 __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 3 : 2) void seq_bwd_row(SeqParams p) {
     if constexpr (DMA) __builtin_assume(p.D % 8 == 0);
     extern __shared__ __align__(16) unsigned char smem[];
-    constexpr int kTile = Tile<HD, DMA>::kElems;
+    constexpr int kTile = SeqTile<HD>::kElems;
     elem_t* tiles = reinterpret_cast<elem_t*>(smem);  // K [2], V [2]
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
     const int hk = blockIdx.x % p.Hkv, slot = p.causal ? p.slots - 1 - (int)(blockIdx.x / p.Hkv) : blockIdx.x / p.Hkv;
@@ -43,7 +43,8 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 3 : 2) void seq_bwd_row(Seq
     const int n_wave = rows > 0 ? keys.seen(p, (r0 + rows - 1) / p.G) : 0;
     const int nt = (n + kCtxTile - 1) / kCtxTile;
     SeqFeed<HD, DMA> feed(p, b, hk, tid);
-    const Tile<HD, DMA> at(lane);
+    SeqTile<HD> at(tiles, lane);
+    constexpr int kHalf = 32 * SeqTile<HD>::kLd * 2, kBytes = SeqTile<HD>::kBytes;
     const auto k_place = [&](int t) { return tiles + (t & 1) * kTile; };
     const auto v_place = [&](int t) { return tiles + (2 + (t & 1)) * kTile; };
     if (nt) feed.request(p, 0, n, k_place(0), v_place(0), wave);
@@ -72,7 +73,7 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 3 : 2) void seq_bwd_row(Seq
         workgroup_barrier();
         for (int u = 0; u < 2 * nt; ++u) {
             if (32 * u >= n_wave) break;
-            const f32x16 s = scores<T>(at, k_place(u >> 1), 32 * (u & 1), own_q), dp = scores<T>(at, v_place(u >> 1), 32 * (u & 1), own_g);
+            const f32x16 s = at.template scores<T>(u * kHalf, own_q), dp = at.template scores<T>(2 * kBytes + u * kHalf, own_g);
 #pragma unroll
             for (int r = 0; r < 16; ++r)
                 if (32 * u + tile_row(r, 0) < limit - 4 * h) delta = __builtin_fmaf(fast_exp2(__builtin_fmaf(s[r], p.c, -less)), dp[r], delta);
@@ -99,6 +100,7 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 3 : 2) void seq_bwd_row(Seq
     }
     const float less_delta = -delta * factor;  // P (dP - delta) = exponential * (factor dP + less_delta)
     f32x16 acc[HD / 32] = {};
+    int step = kBytes;
     const auto tile = [&](int t, auto masked) {
         const int key = t * kCtxTile;
         const bool more = t + 1 < nt;
@@ -107,8 +109,8 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 3 : 2) void seq_bwd_row(Seq
             f32x16 s[2], ds[2];
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                s[u] = scores<T>(at, k_place(t), 32 * u, own_q);
-                ds[u] = scores<T>(at, v_place(t), 32 * u, own_g);
+                s[u] = at.template scores<T>(u * kHalf, own_q);
+                ds[u] = at.template scores<T>(2 * kBytes + u * kHalf, own_g);
             }
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
@@ -118,9 +120,11 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 3 : 2) void seq_bwd_row(Seq
                     if constexpr (decltype(masked)::value)
                         if (32 * u + tile_row(r, 0) >= limit - key - 4 * h) ds[u][r] = 0.0f;
                 }
-                add_columns<T>(acc, at, k_place(t), 32 * u, ds[u]);
+                at.template add_columns<T>(acc, u * kHalf, ds[u]);
             }
         }
+        at.move(step);
+        step = -step;
         if (more) feed.deliver(p, k_place(t + 1), v_place(t + 1), tid);
         feed.arrived();
         workgroup_barrier();
@@ -142,7 +146,7 @@ template <typename T, int HD, bool DMA, int PAIR>
 __global__ __launch_bounds__(kCtxThreads * PAIR, HD <= 64 ? 2 * PAIR : PAIR) void seq_bwd_col(SeqParams p) {
     if constexpr (DMA) __builtin_assume(p.D % 8 == 0);
     extern __shared__ __align__(16) unsigned char smem[];
-    constexpr int kTile = Tile<HD, DMA>::kElems, NT = kCtxThreads * PAIR, U = 2 / PAIR;
+    constexpr int kTile = SeqTile<HD>::kElems, NT = kCtxThreads * PAIR, U = 2 / PAIR;
     elem_t* tiles = reinterpret_cast<elem_t*>(smem);             // [2][Q, dO]
     elem_t* mine = tiles + 4 * kTile;                            // PAIR == 2: K [2], V [2] of the workgroup's keys
     float* stats = reinterpret_cast<float*>(mine + (PAIR == 2 ? 4 * kTile : 0));  // [2][row_stat_folded, -delta][64]
@@ -164,12 +168,12 @@ __global__ __launch_bounds__(kCtxThreads * PAIR, HD <= 64 ? 2 * PAIR : PAIR) voi
     const int first_head = hk * p.G + p.G * split / p.splits, heads = hk * p.G + p.G * (split + 1) / p.splits - first_head;
     const int nx = heads * per_head;
 
-    TileFeed<HD, DMA, NT> qf(p.q.sl, p.D, tid), gf(p.g.sl, p.D, tid);
-    const Tile<HD, DMA> at(lane);
+    RowFeed<HD, DMA, NT> qf(p.q.sl, p.D, tid), gf(p.g.sl, p.D, tid);
+    constexpr int kHalf = 32 * SeqTile<HD>::kLd * 2, kBytes = SeqTile<HD>::kBytes;
+    SeqTile<HD> at(tiles + (PAIR == 2 ? half * (kHalf / 2) : 0), lane);  // (a pair's second wave: rows 32 .. 63)
     float stat = 0.0f;
     const auto place = [&](int x) { return tiles + (x & 1) * 2 * kTile; };
-    const auto request = [&](int x) {
-        const int hq = first_head + x / per_head, r0 = (ta + x % per_head) * kCtxTile;
+    const auto request = [&](int x, int hq, int r0) {
         const int64_t token = b.token + r0;
         qf.request(p.q.head(0, hq) + token * p.q.sl, p.q.sl, b.tokens - r0, p.D, place(x), wave);
         gf.request(p.g.head(0, hq) + token * p.g.sl, p.g.sl, b.tokens - r0, p.D, place(x) + kTile, wave);
@@ -185,10 +189,10 @@ __global__ __launch_bounds__(kCtxThreads * PAIR, HD <= 64 ? 2 * PAIR : PAIR) voi
         if (tid < 3 * kCtxTile) stats[(x & 1) * (kCtxStats / 2) + tid] = stat;
     };
     if (nx) {
-        request(0);
+        request(0, first_head, ta * kCtxTile);
         deliver(0);
         if constexpr (PAIR == 2) {
-            TileFeed<HD, DMA, NT> kf(p.k.sl, p.D, tid), vf(p.v.sl, p.D, tid);
+            RowFeed<HD, DMA, NT> kf(p.k.sl, p.D, tid), vf(p.v.sl, p.D, tid);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int k = b.row0 + i * kCtxTile;
@@ -200,21 +204,26 @@ __global__ __launch_bounds__(kCtxThreads * PAIR, HD <= 64 ? 2 * PAIR : PAIR) voi
         }
         qf.arrived();
     }
-    const elem_t *own_kt = mine + group / 2 * kTile, *own_vt = own_kt + 2 * kTile;
-    const int own_row = 32 * (group & 1);
-    // scores of 32 rows of a tile and the wave's keys
-    const auto products = [&](const elem_t* rows, int row, const u32x4* own, const elem_t* own_tile, f32x16 x) {
-        if constexpr (PAIR == 1) return scores<T>(at, rows, row, own, x);
+    // scores of 32 rows of a tile and the wave's keys (32 group .. of the two tiles of K, or of V behind them)
+    uint32_t own[HD / 16];
 #pragma unroll
-        for (int c = 0; c < HD / 16; ++c) x = Mma32<T>::run(at.rows(rows, row, c), at.rows(own_tile, own_row, c), x);
+    for (int c = 0; c < HD / 16; ++c) own[c] = at.row[c] - half * kHalf + 4 * kBytes + group * kHalf;
+    const auto products = [&](int from, const u32x4* own_rows, int own_from, f32x16 x) {
+        if constexpr (PAIR == 1) return at.template scores<T>(from, own_rows, x);
+#pragma unroll
+        for (int c = 0; c < HD / 16; ++c) x = Mma32<T>::run(at.rows(from, c), *SeqTile<HD>::template at<const u32x4>(own[c] + own_from), x);
         return x;
     };
     f32x16 dk[HD / 32] = {}, dv[HD / 32] = {};
     constexpr bool kFactors = HD > 64;
-    const auto tile = [&](int x, auto masked) {
-        const int r0 = (ta + x % per_head) * kCtxTile;
-        if (x + 1 < nx) request(x + 1);
-        const elem_t* Q = place(x);
+    int step = 2 * kBytes;
+    // x: tiles before this one; hq, t: the head and the tile of its rows
+    const auto tile = [&](int x, int hq, int t, auto masked) {
+        const int r0 = t * kCtxTile;
+        if (x + 1 < nx) {
+            const bool last = t + 1 == tb;
+            request(x + 1, last ? hq + 1 : hq, (last ? ta : t + 1) * kCtxTile);
+        }
         const float* st = stats + (x & 1) * (kCtxStats / 2);
         const bool factors = !kFactors && __builtin_amdgcn_ballot_w64(st[kCtxTile + lane] != 1.0f);
         const int row0 = PAIR == 2 ? 32 * half : 0, end = row0 + 32 * U;  // rows of the tile that are this wave's
@@ -222,8 +231,8 @@ __global__ __launch_bounds__(kCtxThreads * PAIR, HD <= 64 ? 2 * PAIR : PAIR) voi
             f32x16 s[U], ds[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                s[u] = products(Q, row0 + 32 * u, own_k, own_kt, f32x16{});
-                ds[u] = products(Q + kTile, row0 + 32 * u, own_v, own_vt, seq_of_rows(st + 2 * kCtxTile + row0 + 32 * u, h));
+                s[u] = products(u * kHalf, own_k, 0, f32x16{});
+                ds[u] = products(kBytes + u * kHalf, own_v, 2 * kBytes, seq_of_rows(st + 2 * kCtxTile + row0 + 32 * u, h));
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
@@ -250,10 +259,12 @@ __global__ __launch_bounds__(kCtxThreads * PAIR, HD <= 64 ? 2 * PAIR : PAIR) voi
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                add_columns<T>(dv, at, Q + kTile, row0 + 32 * u, s[u]);
-                add_columns<T>(dk, at, Q, row0 + 32 * u, ds[u]);
+                at.template add_columns<T>(dv, kBytes + u * kHalf, s[u]);
+                at.template add_columns<T>(dk, u * kHalf, ds[u]);
             }
         }
+        at.move(step);
+        step = -step;
         if (x + 1 < nx) deliver(x + 1);
         qf.arrived();
         workgroup_barrier();
@@ -261,10 +272,10 @@ __global__ __launch_bounds__(kCtxThreads * PAIR, HD <= 64 ? 2 * PAIR : PAIR) voi
     workgroup_barrier();
     // causal: the rows of the block's own positions stand in a head's first two tiles
     const int near = p.causal ? min(kCtxOwned / kCtxTile, per_head) : 0;
-    for (int x = 0; x < nx;) {
-        const int first = x;
-        for (; x < first + near; ++x) tile(x, std::true_type{});
-        for (; x < first + per_head; ++x) tile(x, std::false_type{});
+    for (int x = 0, hq = first_head; x < nx; ++hq) {
+        int t = ta;
+        for (; t < ta + near; ++t) tile(x++, hq, t, std::true_type{});
+        for (; t < tb; ++t) tile(x++, hq, t, std::false_type{});
     }
     const bool scored = ok && keys.keys != 1;
     const int out_rows = min(max(b.tokens - k0, 0), 32);

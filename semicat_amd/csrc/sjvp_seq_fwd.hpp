@@ -17,8 +17,7 @@ template <typename T, int HD, bool PAGED, typename FEED>
 __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 4 : 2) void seq_fwd(SeqParams p) {
     if constexpr (FEED::kDma) __builtin_assume(p.D % 8 == 0);
     extern __shared__ __align__(16) unsigned char smem[];
-    constexpr bool DMA = FEED::kDma;
-    constexpr int kTile = Tile<HD, DMA>::kElems;
+    constexpr int kTile = SeqTile<HD>::kElems;
     elem_t* tiles = reinterpret_cast<elem_t*>(smem);  // K [2], V [2]
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
     const int hk = blockIdx.x % p.Hkv, slot = p.causal ? p.slots - 1 - (int)(blockIdx.x / p.Hkv) : blockIdx.x / p.Hkv;  // causal: long rows first
@@ -37,7 +36,7 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 4 : 2) void seq_fwd(SeqPara
     own_operands<HD>(own, p.q.head(0, mine.hq) + (int64_t)(b.token + mine.token) * p.q.sl, ok, h, p.D);
     const int nt = (n + kCtxTile - 1) / kCtxTile;
     FEED feed(p, b, hk, tid);
-    const Tile<HD, DMA> at(lane);
+    SeqTile<HD> at(tiles, lane);
     const auto k_place = [&](int t) { return tiles + (t & 1) * kTile; };
     const auto v_place = [&](int t) { return tiles + (2 + (t & 1)) * kTile; };
     if (nt) {
@@ -49,6 +48,8 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 4 : 2) void seq_fwd(SeqPara
     feed.arrived();
     workgroup_barrier();
     SeqSums<HD> st;
+    constexpr int kHalf = 32 * SeqTile<HD>::kLd * 2, kV = 2 * SeqTile<HD>::kBytes;
+    int step = SeqTile<HD>::kBytes;
     const auto tile = [&](int t, auto masked) {
         const bool more = t + 1 < nt;
         if (more) {
@@ -58,11 +59,13 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 4 : 2) void seq_fwd(SeqPara
         if (t * kCtxTile < n_wave) {
             f32x16 s[2];
 #pragma unroll
-            for (int u = 0; u < 2; ++u) s[u] = scores<T>(at, k_place(t), 32 * u, own);
+            for (int u = 0; u < 2; ++u) s[u] = at.template scores<T>(u * kHalf, own);
             st.template take<decltype(masked)::value>(s, p.c, limit - t * kCtxTile, h);
 #pragma unroll
-            for (int u = 0; u < 2; ++u) add_columns<T>(st.acc, at, v_place(t), 32 * u, s[u]);
+            for (int u = 0; u < 2; ++u) at.template add_columns<T>(st.acc, kV + u * kHalf, s[u]);
         }
+        at.move(step);
+        step = -step;
         if (more) feed.deliver(p, k_place(t + 1), v_place(t + 1), tid);
         feed.arrived();
         workgroup_barrier();

@@ -2,6 +2,7 @@
 #pragma once
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 #include "sjvp_ctx_launch.hpp"
 #include "sjvp_seq.hpp"
 
@@ -13,8 +14,22 @@ inline int64_t seq_slots(const SeqParams& p, int heads, int R) { return (int64_t
 // Sets of 16 rows to a block of seq_few.
 inline int seq_sets(const SeqParams& p) { return (int64_t)p.T * p.G <= 16 * (int64_t)p.B ? 1 : 2; }
 
-inline bool seq_dma(const SeqParams& p, const CtxView& a, const CtxView& b) {
-    return p.D % 8 == 0 && ctx_padded(p.D) != 96 && ctx_aligned(a) && ctx_aligned(b);
+inline bool seq_dma(const SeqParams& p, const CtxView& a, const CtxView& b) { return p.D % 8 == 0 && ctx_aligned(a) && ctx_aligned(b); }
+inline int seq_tiles_bytes(int HD) { return 4 * kCtxTile * (HD == 96 ? 128 : HD) * 2; }
+
+// Calls f with the padded head dimension, and, where it is wanted, whether tiles come by LDS-DMA, as constants.
+template <typename F>
+int seq_by_head(int D, F&& f) {
+    switch (ctx_padded(D)) {
+        case 32: return f(std::integral_constant<int, 32>{});
+        case 64: return f(std::integral_constant<int, 64>{});
+        case 96: return f(std::integral_constant<int, 96>{});
+        default: return f(std::integral_constant<int, 128>{});
+    }
+}
+template <typename F>
+int seq_by_head(int D, bool dma, F&& f) {
+    return seq_by_head(D, [&](auto hd) { return dma ? f(hd, std::true_type{}) : f(hd, std::false_type{}); });
 }
 
 template <typename T> int seq_packed_fwd(SeqParams p, hipStream_t stream);

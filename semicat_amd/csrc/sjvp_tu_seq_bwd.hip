@@ -9,19 +9,19 @@ int seq_packed_bwd<SJVP_T>(SeqParams p, hipStream_t stream) {
     const bool row_dma = seq_dma(p, p.k, p.v), col_dma = seq_dma(p, p.q, p.g) && row_dma;  // (at D = 128 the column-owned one has K and V in LDS too)
     const int splits = p.splits;
     p.slots = (int)seq_slots(p, p.G, kCtxOwned);
-    int rc = ctx_by_head(p.D, row_dma, [&](auto hd, auto dma) {
+    int rc = seq_by_head(p.D, row_dma, [&](auto hd, auto dma) {
         constexpr int HD = decltype(hd)::value;
         constexpr bool DMA = decltype(dma)::value;
-        return launch(seq_bwd_row<SJVP_T, HD, DMA>, p.slots * p.Hkv, ctx_tiles_bytes(HD, DMA), stream, p, kCtxThreads);
+        return launch(seq_bwd_row<SJVP_T, HD, DMA>, p.slots * p.Hkv, seq_tiles_bytes(HD), stream, p, kCtxThreads);
     });
     if (rc != SJVP_OK || !p.dk.ptr) return rc;
     p.slots = (int)seq_slots(p, 1, kCtxOwned);
     p.splits = splits;
-    return ctx_by_head(p.D, col_dma, [&](auto hd, auto dma) {
+    return seq_by_head(p.D, col_dma, [&](auto hd, auto dma) {
         constexpr int HD = decltype(hd)::value;
         constexpr bool DMA = decltype(dma)::value;
-        constexpr int PAIR = HD == 128 ? 2 : 1;
-        const int rc = launch(seq_bwd_col<SJVP_T, HD, DMA, PAIR>, p.slots * p.Hkv * p.splits, PAIR * ctx_tiles_bytes(HD, DMA) + 4 * kCtxStats, stream, p, kCtxThreads * PAIR);
+        constexpr int PAIR = HD > 64 ? 2 : 1;
+        const int rc = launch(seq_bwd_col<SJVP_T, HD, DMA, PAIR>, p.slots * p.Hkv * p.splits, PAIR * seq_tiles_bytes(HD) + 4 * kCtxStats, stream, p, kCtxThreads * PAIR);
         if (rc != SJVP_OK || p.splits == 1) return rc;
         return launch(seq_sum<SJVP_T, HD>, (int)((2 * (int64_t)p.Hkv * p.T * (HD / 8) + kCtxThreads - 1) / kCtxThreads), 0, stream, p, kCtxThreads);
     });
