@@ -72,31 +72,33 @@ int paged_params(const sjvp_paged* t, SeqParams& p, int T) {
     return SJVP_OK;
 }
 
-// How a call of the paged attention is served.  seq_few splits long sequences over workgroups and takes any number of rows; seq_fwd, whose
-// four waves share their tiles, takes the longer sequences where blocks of 128 rows fill half of the compute units.
-struct PagedPlan {
-    bool few = true, many = false;
-    int splits = 1, split_tiles = 1;
-    size_t stat = 0, part = 0, used = 0, total = 0;  // floats
-};
-
 PagedPlan paged_plan(const SeqParams& p) {
     PagedPlan plan;
-    const int64_t rows = (int64_t)p.T * p.G;
-    plan.many = p.T > p.B && 2 * ceil_div(rows, kCtxOwned) * p.Hkv > compute_units();
-    const int64_t blocks = (p.B + rows / 32) * p.Hkv;
-    plan.split_tiles = 8;
-    plan.splits = (int)std::max<int64_t>(1, std::min<int64_t>({8 * (int64_t)compute_units() / blocks, p.pages.capacity / (32 * plan.split_tiles), 128}));
-    if (plan.splits > 1) {
-        const auto take = [&](int64_t floats) {
-            const size_t at = plan.total;
-            plan.total += (size_t)(floats + 3) / 4 * 4;
-            return at;
-        };
-        const int64_t places = p.Hkv * (plan.many ? (int64_t)(p.B + 2) * kSeqFew : rows);
-        plan.stat = take(2 * plan.splits * places);
-        plan.part = take(plan.splits * places * ctx_padded(p.D));
-        plan.used = take(places);
+    const int64_t rows = (int64_t)p.T * p.G, cu = compute_units(), keys = p.pages.capacity;
+    const auto take = [&](int64_t floats) {
+        const size_t at = plan.total;
+        plan.total += (size_t)(floats + 3) / 4 * 4;
+        return at;
+    };
+    const auto scratch = [&](PagedPart& part, int64_t places) {
+        if (part.splits <= 1) return;
+        part.stat = take(2 * part.splits * places);
+        part.part = take(part.splits * places * ctx_padded(p.D));
+        part.used = take(places);
+    };
+    const auto splits = [](int64_t wanted, int64_t most, int64_t limit) { return (int)std::max<int64_t>(1, std::min<int64_t>({wanted, most, limit})); };
+    const int64_t many = ceil_div(rows, kCtxOwned) * p.Hkv;
+    plan.has_many = p.T > p.B && 2 * many > cu;
+    plan.has_few = !plan.has_many || rows < 256 * (int64_t)p.B;
+    if (plan.has_few) {
+        plan.few.split_tiles = 8;
+        plan.few.splits = splits(8 * cu / ((p.B + rows / 32) * p.Hkv), keys / (32 * plan.few.split_tiles), 128);
+        scratch(plan.few, p.Hkv * (plan.has_many ? (int64_t)(p.B + 2) * kSeqFew : rows));
+    }
+    if (plan.has_many) {
+        plan.many.split_tiles = 32;
+        plan.many.splits = splits(8 * cu / many, keys / (kCtxTile * plan.many.split_tiles), 16);
+        scratch(plan.many, p.Hkv * rows);
     }
     return plan;
 }
@@ -110,7 +112,7 @@ struct PackedPlan {
 PackedPlan packed_plan(const SeqParams& p) {
     PackedPlan plan;
     const int64_t blocks = (p.T / kCtxOwned + 1) * (int64_t)p.Hkv;
-    static const int CU = getenv("CUX") ? atoi(getenv("CUX")) : 4; // XXX
+    static const int CU = getenv("CUY") ? atoi(getenv("CUY")) : 4; // XXX
     plan.splits = (int)std::max<int64_t>(1, std::min<int64_t>(CU * (int64_t)compute_units() / blocks, p.G));
     plan.part = (3 * (size_t)p.Hq * p.T + 3) / 4 * 4;
     plan.total = plan.part + (plan.splits > 1 ? 2 * (size_t)plan.splits * p.Hkv * p.T * ctx_padded(p.D) : 0);
@@ -189,11 +191,9 @@ int sjvp_paged_attention(const sjvp_paged* t, int dtype, void* stream) {
     if (!t->q || !t->o || (!t->offsets && t->T != t->B)) return SJVP_ERR_NULL;
     const PagedPlan plan = paged_plan(p);
     if (seq_workspace(t->workspace, t->workspace_bytes, plan.total) != SJVP_OK) return SJVP_ERR_WORKSPACE;
-    float* ws = static_cast<float*>(t->workspace);
-    p.splits = plan.splits, p.split_tiles = plan.split_tiles;
-    p.stat = ws + plan.stat, p.part = ws + plan.part, p.used = reinterpret_cast<int*>(ws + plan.used);
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    return dtype == SJVP_BF16 ? seq_paged<Bf16>(p, p.pages.ks, plan.few, plan.many, s) : seq_paged<Fp16>(p, p.pages.ks, plan.few, plan.many, s);
+    float* ws = static_cast<float*>(t->workspace);
+    return dtype == SJVP_BF16 ? seq_paged<Bf16>(p, plan, ws, p.pages.ks, s) : seq_paged<Fp16>(p, plan, ws, p.pages.ks, s);
 }
 
 }  // extern "C"

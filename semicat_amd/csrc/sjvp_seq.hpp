@@ -38,11 +38,11 @@ struct SeqParams {
     CtxView q, k, v, o, g, dq, dk, dv;  // [T,H,D], sb unused
     float *lse, *folded;                // [Hq,T][2]: (m, l) of each row; [3][Hq,T]: row_stat_folded, -delta
     float *part, *stat;                 // sums of split work: [splits][seq_places] of HD floats, and their (maximum, sum)
-    int* used;                          // splits that a row's sums stand in (0: in none)
+    int *used, *used_many;              // splits that a row's sums stand in (0: in none); seq_few beside a split seq_fwd: those of seq_fwd
     const int *offsets, *lengths;       // offsets null: one row each
     int B, T, Hq, Hkv, G, D, causal;
     float scale, c;                     // c = scale * log2(e)
-    int slots, splits, split_tiles;     // split_tiles: tiles of 32 keys that a split has at least
+    int slots, splits, split_tiles;     // split_tiles: tiles (of 32 keys, seq_fwd: of 64) that a split has at least
     int least, most;                    // query rows (of all heads of a group) of the sequences that a launch serves
     SeqPages pages;
 };
@@ -277,6 +277,14 @@ struct SeqFeed {
     __device__ __forceinline__ void deliver(const SeqParams& p, elem_t* kp, elem_t* vp, int tid) {
         kf.deliver(kp, p.D, tid), vf.deliver(vp, p.D, tid);
     }
+    __device__ __forceinline__ void request_k(const SeqParams& p, int t, int keys, elem_t* kp, int wave) {
+        kf.request(k + (int64_t)t * kCtxTile * p.k.sl, p.k.sl, keys - t * kCtxTile, p.D, kp, wave);
+    }
+    __device__ __forceinline__ void request_v(const SeqParams& p, int t, int keys, elem_t* vp, int wave) {
+        vf.request(v + (int64_t)t * kCtxTile * p.v.sl, p.v.sl, keys - t * kCtxTile, p.D, vp, wave);
+    }
+    __device__ __forceinline__ void deliver_k(const SeqParams& p, elem_t* kp, int tid) { kf.deliver(kp, p.D, tid); }
+    __device__ __forceinline__ void deliver_v(const SeqParams& p, elem_t* vp, int tid) { vf.deliver(vp, p.D, tid); }
     __device__ __forceinline__ void arrived() { kf.arrived(); }
 };
 
@@ -376,9 +384,9 @@ struct SeqSums {
 
     __device__ __forceinline__ SeqSums() : acc{}, m(-INFINITY), ref(0.0f), l(0.0f) {}
 
-    // Scores of 32 N keys to exponentials; keys from `left` on are not seen (masked).
+    // The rows' maxima with the scores of 32 N keys; keys from `left` on are not seen (masked).
     template <bool MASKED, int N>
-    __device__ __forceinline__ void take(f32x16 (&s)[N], float c, int left, int h) {
+    __device__ __forceinline__ void raise(f32x16 (&s)[N], float c, int left, int h) {
         if constexpr (MASKED) {
 #pragma unroll
             for (int u = 0; u < N; ++u)
@@ -401,6 +409,9 @@ struct SeqSums {
 #pragma unroll
             for (int dt = 0; dt < HD / 32; ++dt) acc[dt] *= f;
         }
+    }
+    template <int N>
+    __device__ __forceinline__ void exponentials(f32x16 (&s)[N], float c) {
         float sum = 0.0f;
 #pragma unroll
         for (int u = 0; u < N; ++u)
@@ -410,6 +421,11 @@ struct SeqSums {
                 sum += s[u][r];
             }
         l += sum;
+    }
+    template <bool MASKED, int N>
+    __device__ __forceinline__ void take(f32x16 (&s)[N], float c, int left, int h) {
+        raise<MASKED>(s, c, left, h);
+        exponentials(s, c);
     }
 };
 

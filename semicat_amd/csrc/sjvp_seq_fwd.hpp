@@ -12,15 +12,35 @@ struct SeqRow {
     __device__ __forceinline__ SeqRow(const SeqParams& p, int hk, int row) : token(row / p.G), hq(hk * p.G + row % p.G) {}
 };
 
+// Splits of the tiles of a sequence's keys: of split_tiles or more, as many as the launch has at most.
+struct SeqSplit {
+    int used, first, end;
+    __device__ __forceinline__ SeqSplit(const SeqParams& p, int tiles, int split) {
+        const int per = max(p.split_tiles, (tiles + p.splits - 1) / p.splits);
+        used = max(1, (tiles + per - 1) / per);
+        first = min(split * per, tiles), end = min(first + per, tiles);
+    }
+};
+
+// Where the sums of a row stand between seq_few and seq_join: by token, or, where seq_few serves the short sequences of a call alone
+// (p.most is kSeqFew), by segment, kSeqFew rows to each.
+__device__ __forceinline__ int64_t seq_group(const SeqParams& p) { return p.most == kSeqFew ? (int64_t)(p.B + 2) * kSeqFew : (int64_t)p.T * p.G; }
+__device__ __forceinline__ int64_t seq_places(const SeqParams& p) { return p.Hkv * seq_group(p); }
+__device__ __forceinline__ int64_t seq_place(const SeqParams& p, const SeqBlock& b, int hk, int row) {
+    return hk * seq_group(p) + (p.most == kSeqFew ? (int64_t)b.segment * kSeqFew : (int64_t)b.token * p.G) + row;
+}
+
 // Many rows: four waves of 32 rows share tiles of 64 keys, two tiles of K and V in LDS, one barrier to a tile.
 template <typename T, int HD, bool PAGED, typename FEED>
 __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 4 : 2) void seq_fwd(SeqParams p) {
     if constexpr (FEED::kDma) __builtin_assume(p.D % 8 == 0);
     extern __shared__ __align__(16) unsigned char smem[];
     constexpr int kTile = SeqTile<HD>::kElems;
+    constexpr bool kAhead = !PAGED && FEED::kDma && HD == 128;
     elem_t* tiles = reinterpret_cast<elem_t*>(smem);  // K [2], V [2]
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
-    const int hk = blockIdx.x % p.Hkv, slot = p.causal ? p.slots - 1 - (int)(blockIdx.x / p.Hkv) : blockIdx.x / p.Hkv;  // causal: long rows first
+    const int hk = blockIdx.x % p.Hkv, x = blockIdx.x / p.Hkv, split = PAGED ? x / p.slots : 0;
+    const int slot = p.causal ? p.slots - 1 - (x - split * p.slots) : x;  // causal: long rows first
     const SeqBlock b = seq_block<kCtxOwned, PAGED>(p, slot, p.G, lane);
     const int all = b.tokens * p.G;
     if (!b.some || all < p.least || all > p.most) return;
@@ -32,22 +52,79 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 4 : 2) void seq_fwd(SeqPara
     const int n = keys.seen(p, (min(b.row0 + kCtxOwned, all) - 1) / p.G), whole = keys.seen(p, b.row0 / p.G);  // keys of the last, the first row
     const int n_wave = rows > 0 ? keys.seen(p, (r0 + rows - 1) / p.G) : 0;
 
+    const SeqSplit part(p, (n + kCtxTile - 1) / kCtxTile, split);
+    if (PAGED && split >= part.used) return;
     u32x4 own[HD / 16];
     own_operands<HD>(own, p.q.head(0, mine.hq) + (int64_t)(b.token + mine.token) * p.q.sl, ok, h, p.D);
-    const int nt = (n + kCtxTile - 1) / kCtxTile;
+    const int t0 = PAGED ? part.first : 0, nt = PAGED ? part.end : (n + kCtxTile - 1) / kCtxTile;
     FEED feed(p, b, hk, tid);
     SeqTile<HD> at(tiles, lane);
+    SeqSums<HD> st;
+    if constexpr (kAhead) {
     const auto k_place = [&](int t) { return tiles + (t & 1) * kTile; };
     const auto v_place = [&](int t) { return tiles + (2 + (t & 1)) * kTile; };
+    // K runs a tile ahead of V, so that the scores of the next tile are made beside the exponentials of this one.
     if (nt) {
         feed.look(p, 0, n);
-        feed.request(p, 0, n, k_place(0), v_place(0), wave);
-        if (nt > 1) feed.look(p, 1, n);
-        feed.deliver(p, k_place(0), v_place(0), tid);
+        feed.request_k(p, 0, n, k_place(0), wave);
+        feed.request_v(p, 0, n, v_place(0), wave);
+        feed.deliver_k(p, k_place(0), tid);
+        feed.deliver_v(p, v_place(0), tid);
+        if (nt > 1) {
+            feed.look(p, 1, n);
+            feed.request_k(p, 1, n, k_place(1), wave);
+            feed.deliver_k(p, k_place(1), tid);
+        }
     }
     feed.arrived();
     workgroup_barrier();
-    SeqSums<HD> st;
+    constexpr int kHalf = 32 * SeqTile<HD>::kLd * 2, kV = 2 * SeqTile<HD>::kBytes;
+    int step = SeqTile<HD>::kBytes;
+    f32x16 s[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) s[u] = at.template scores<T>(u * kHalf, own);
+    workgroup_barrier();
+    const auto tile = [&](int t, auto masked) {
+        if (t + 1 < nt) feed.request_v(p, t + 1, n, v_place(t + 1), wave);
+        if (t + 2 < nt) {
+            feed.look(p, t + 2, n);
+            feed.request_k(p, t + 2, n, k_place(t), wave);
+        }
+        at.move(step);
+        if (t * kCtxTile < n_wave) {
+            st.template raise<decltype(masked)::value>(s, p.c, limit - t * kCtxTile, h);
+            f32x16 next[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) next[u] = at.template scores<T>(u * kHalf, own);
+            st.exponentials(s, p.c);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                at.template add_columns<T>(st.acc, kV - step + u * kHalf, s[u]);
+                s[u] = next[u];
+            }
+        }
+        step = -step;
+        if (t + 1 < nt) feed.deliver_v(p, v_place(t + 1), tid);
+        if (t + 2 < nt) feed.deliver_k(p, k_place(t), tid);
+        feed.arrived();
+        workgroup_barrier();
+    };
+    // (the tiles that all rows see as a whole have a loop without masks)
+    const int free = min(whole / kCtxTile, nt);
+    int t = 0;
+    for (; t < free; ++t) tile(t, std::false_type{});
+    for (; t < nt; ++t) tile(t, std::true_type{});
+    } else {
+    const auto k_place = [&](int t) { return tiles + ((t - t0) & 1) * kTile; };
+    const auto v_place = [&](int t) { return tiles + (2 + ((t - t0) & 1)) * kTile; };
+    if (t0 < nt) {
+        feed.look(p, t0, n);
+        feed.request(p, t0, n, k_place(t0), v_place(t0), wave);
+        if (t0 + 1 < nt) feed.look(p, t0 + 1, n);
+        feed.deliver(p, k_place(t0), v_place(t0), tid);
+    }
+    feed.arrived();
+    workgroup_barrier();
     constexpr int kHalf = 32 * SeqTile<HD>::kLd * 2, kV = 2 * SeqTile<HD>::kBytes;
     int step = SeqTile<HD>::kBytes;
     const auto tile = [&](int t, auto masked) {
@@ -72,34 +149,35 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 4 : 2) void seq_fwd(SeqPara
     };
     // (the tiles that all rows see as a whole have a loop without masks)
     const int free = min(whole / kCtxTile, nt);
-    int t = 0;
+    int t = t0;
     for (; t < free; ++t) tile(t, std::false_type{});
     for (; t < nt; ++t) tile(t, std::true_type{});
+    }
     const float both = halves_sum(st.l), l = limit > 0 ? both : 0.0f, f = l == 0.0f ? 0.0f : 1.0f / l;
     if (p.lse && h == 0 && ok)
         *reinterpret_cast<f32x2*>(p.lse + 2 * ((int64_t)mine.hq * p.T + b.token + mine.token)) = f32x2{l == 0.0f ? 0.0f : st.ref, l};
+    if constexpr (PAGED) {
+        if (p.splits > 1 && ok) {
+            const int64_t place = seq_place(p, b, hk, r0 + (lane & 31));
+            if (split == 0 && h == 0) p.used[place] = part.used > 1 ? part.used : 0;
+            if (part.used > 1) {
+                const int64_t at = split * seq_places(p) + place;
+                if (h == 0) p.stat[2 * at] = st.m == -INFINITY ? -INFINITY : st.ref, p.stat[2 * at + 1] = both;
+                float* out = p.part + at * HD + 4 * h;
+#pragma unroll
+                for (int dt = 0; dt < HD / 32; ++dt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        *reinterpret_cast<f32x4*>(out + 32 * dt + 8 * i) =
+                            f32x4{st.acc[dt][4 * i], st.acc[dt][4 * i + 1], st.acc[dt][4 * i + 2], st.acc[dt][4 * i + 3]};
+            }
+        }
+        if (part.used > 1) return;
+    }
     store_rows_at<T, HD>(st.acc, f, rows, tiles + wave * 32 * (HD + 8), lane, p.D, [&](int row) {
         const SeqRow to(p, hk, r0 + row);
         return p.o.head(0, to.hq) + (int64_t)(b.token + to.token) * p.o.sl;
     });
-}
-
-// Splits of the tiles of 32 keys of a sequence: of split_tiles or more, as many as the launch has at most.
-struct SeqSplit {
-    int used, first, end;
-    __device__ __forceinline__ SeqSplit(const SeqParams& p, int tiles, int split) {
-        const int per = max(p.split_tiles, (tiles + p.splits - 1) / p.splits);
-        used = max(1, (tiles + per - 1) / per);
-        first = min(split * per, tiles), end = min(first + per, tiles);
-    }
-};
-
-// Where the sums of a row stand between seq_few and seq_join: by token, or, where seq_few serves the short sequences of a call alone
-// (p.most is kSeqFew), by segment, kSeqFew rows to each.
-__device__ __forceinline__ int64_t seq_group(const SeqParams& p) { return p.most == kSeqFew ? (int64_t)(p.B + 2) * kSeqFew : (int64_t)p.T * p.G; }
-__device__ __forceinline__ int64_t seq_places(const SeqParams& p) { return p.Hkv * seq_group(p); }
-__device__ __forceinline__ int64_t seq_place(const SeqParams& p, const SeqBlock& b, int hk, int row) {
-    return hk * seq_group(p) + (p.most == kSeqFew ? (int64_t)b.segment * kSeqFew : (int64_t)b.token * p.G) + row;
 }
 
 // Maximum and sum over the four lanes (l, l ^ 16, l ^ 32, l ^ 48) of a row.
@@ -297,6 +375,7 @@ __global__ __launch_bounds__(64 * WAVES, NC == 1 ? (E4M3 || HD <= 96 ? 4 : 3) : 
             for (int j = 0; j < 8; ++j) o[j] += f * sums[(k * R + row) * kSum + c8 + j];
         }
         const SeqRow to(p, hk, r0 + row);
+        if (p.used_many && split == 0 && c8 == 0) p.used_many[hk * (int64_t)p.T * p.G + (int64_t)b.token * p.G + r0 + row] = 0;
         if (p.splits > 1) {
             const int64_t place = seq_place(p, b, hk, r0 + row);
             if (split == 0 && c8 == 0) p.used[place] = part.used > 1 ? part.used : 0;
@@ -317,7 +396,7 @@ __global__ __launch_bounds__(64 * WAVES, NC == 1 ? (E4M3 || HD <= 96 ? 4 : 3) : 
     }
 }
 
-// Joins the splits of seq_few: 16 threads to the columns of a row (eight each), `slices` of them to the splits, which meet in LDS.
+// Joins the splits of seq_few or seq_fwd: 16 threads to the columns of a row (eight each), `slices` of them to the splits, which meet in LDS.
 template <typename T, int HD>
 __global__ __launch_bounds__(kCtxThreads) void seq_join(SeqParams p) {
     __shared__ float met[kCtxThreads / 16][16][11];

@@ -34,8 +34,19 @@ int seq_by_head(int D, bool dma, F&& f) {
 
 template <typename T> int seq_packed_fwd(SeqParams p, hipStream_t stream);
 template <typename T> int seq_packed_bwd(SeqParams p, hipStream_t stream);
-// e4m3: pages of 8-bit numbers; few, many: which of the two kernels serve the call
-template <typename T> int seq_paged(SeqParams p, bool e4m3, bool few, bool many, hipStream_t stream);
+// How a call of the paged attention is served: by seq_few, which splits long sequences over workgroups and takes any number of rows, or, where
+// blocks of 128 rows fill half of the compute units, the longer sequences by seq_fwd.  Scratch of each: places in floats.
+struct PagedPart {
+    int splits = 1, split_tiles = 1;
+    size_t stat = 0, part = 0, used = 0;
+};
+struct PagedPlan {
+    bool has_few = true, has_many = false;
+    PagedPart few, many;
+    size_t total = 0;
+};
+// e4m3: pages of 8-bit numbers
+template <typename T> int seq_paged(SeqParams p, const PagedPlan& plan, float* ws, bool e4m3, hipStream_t stream);
 int paged_copy(const SeqParams& p, bool e4m3, bool fp16, bool write, hipStream_t stream);
 
 }  // namespace sjvp

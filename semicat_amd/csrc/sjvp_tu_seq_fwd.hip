@@ -15,37 +15,45 @@ int seq_packed_fwd<SJVP_T>(SeqParams p, hipStream_t stream) {
 }
 
 template <>
-int seq_paged<SJVP_T>(SeqParams p, bool e4m3, bool few, bool many, hipStream_t stream) {
-    const int splits = p.splits;
+int seq_paged<SJVP_T>(SeqParams p, const PagedPlan& plan, float* ws, bool e4m3, hipStream_t stream) {
+    SeqParams m = p;
+    const auto put = [&](SeqParams& x, const PagedPart& part, int least, int most) {
+        x.least = least, x.most = most, x.splits = part.splits, x.split_tiles = part.split_tiles;
+        x.stat = ws + part.stat, x.part = ws + part.part, x.used = reinterpret_cast<int*>(ws + part.used);
+    };
+    put(p, plan.few, 0, plan.has_many ? kSeqFew : INT_MAX);
+    put(m, plan.many, plan.has_few ? kSeqFew + 1 : 0, INT_MAX);
+    p.used_many = plan.has_many && plan.many.splits > 1 ? m.used : nullptr;
     return seq_by_head(p.D, [&](auto hd) {
         constexpr int HD = decltype(hd)::value;
+        const auto few = [&](auto sets, auto bits8) {
+            constexpr int NC = decltype(sets)::value;
+            p.slots = (int)seq_slots(p, p.G, 16 * NC);
+            const int smem = kCtxWaves * std::max(32 * (HD + 8) * 2, 16 * NC * (HD + 4 + 2) * 4);
+            return launch(seq_few<SJVP_T, HD, decltype(bits8)::value, NC, kCtxWaves>, p.slots * p.Hkv * p.splits, smem, stream, p, kCtxThreads);
+        };
+        const auto join = [&](const SeqParams& x) {
+            if (x.splits == 1) return (int)SJVP_OK;
+            int slices = 1;  // as in the kernel
+            while (slices < x.splits && slices < 16) slices *= 2;
+            const int64_t rows = x.Hkv * (x.most == kSeqFew ? (int64_t)(x.B + 2) * kSeqFew : (int64_t)x.T * x.G), per = 16 / slices;
+            return launch(seq_join<SJVP_T, HD>, (int)((rows + per - 1) / per), 0, stream, x, kCtxThreads);
+        };
+        const std::integral_constant<int, 1> one;
+        const std::integral_constant<int, 2> two;
+        const std::true_type yes;
+        const std::false_type no;
         int rc = SJVP_OK;
-        if (few) {
-            const auto run = [&](auto sets, auto bits8) {
-                constexpr int NC = decltype(sets)::value;
-                p.slots = (int)seq_slots(p, p.G, 16 * NC), p.least = 0, p.most = many ? kSeqFew : INT_MAX;
-                const int smem = kCtxWaves * std::max(32 * (HD + 8) * 2, 16 * NC * (HD + 4 + 2) * 4);
-                return launch(seq_few<SJVP_T, HD, decltype(bits8)::value, NC, kCtxWaves>, p.slots * p.Hkv * splits, smem, stream, p, kCtxThreads);
-            };
-            const std::integral_constant<int, 1> one;
-            const std::integral_constant<int, 2> two;
-            const std::true_type yes;
-            const std::false_type no;
-            rc = seq_sets(p) == 1 ? e4m3 ? run(one, yes) : run(one, no) : e4m3 ? run(two, yes) : run(two, no);
-            if (rc != SJVP_OK) return rc;
+        if (plan.has_few) {
+            rc = seq_sets(p) == 1 ? e4m3 ? few(one, yes) : few(one, no) : e4m3 ? few(two, yes) : few(two, no);
+            if (rc == SJVP_OK) rc = join(p);
         }
-        if (many) {
-            SeqParams m = p;
-            m.slots = (int)seq_slots(p, p.G, kCtxOwned), m.least = few ? kSeqFew + 1 : 0, m.most = INT_MAX;
-            rc = e4m3 ? launch(seq_fwd<SJVP_T, HD, true, PageFeed8<SJVP_T, HD>>, m.slots * p.Hkv, seq_tiles_bytes(HD), stream, m, kCtxThreads)
-                      : launch(seq_fwd<SJVP_T, HD, true, PageFeed<HD>>, m.slots * p.Hkv, seq_tiles_bytes(HD), stream, m, kCtxThreads);
-            if (rc != SJVP_OK) return rc;
-        }
-        if (!few || splits == 1) return rc;
-        int slices = 1;  // as in the kernel
-        while (slices < splits && slices < 16) slices *= 2;
-        const int64_t rows = p.Hkv * (many ? (int64_t)(p.B + 2) * kSeqFew : (int64_t)p.T * p.G), per = 16 / slices;
-        return launch(seq_join<SJVP_T, HD>, (int)((rows + per - 1) / per), 0, stream, p, kCtxThreads);
+        if (rc != SJVP_OK || !plan.has_many) return rc;
+        m.slots = (int)seq_slots(m, m.G, kCtxOwned);
+        const int grid = m.slots * m.Hkv * m.splits;
+        rc = e4m3 ? launch(seq_fwd<SJVP_T, HD, true, PageFeed8<SJVP_T, HD>>, grid, seq_tiles_bytes(HD), stream, m, kCtxThreads)
+                  : launch(seq_fwd<SJVP_T, HD, true, PageFeed<HD>>, grid, seq_tiles_bytes(HD), stream, m, kCtxThreads);
+        return rc == SJVP_OK ? join(m) : rc;
     });
 }
 
