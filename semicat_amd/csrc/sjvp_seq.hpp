@@ -84,6 +84,43 @@ __device__ __forceinline__ SeqBlock seq_block(const SeqParams& p, int slot, int 
     return b;
 }
 
+__device__ __forceinline__ int lanes_sum(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x128, 0xf, 0xf, false);  // turned by 8, 4, 2, 1 of 16
+    x += __builtin_amdgcn_update_dpp(0, x, 0x124, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x122, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x121, 0xf, 0xf, false);
+    return __builtin_amdgcn_readlane(x, 0) + __builtin_amdgcn_readlane(x, 16) + __builtin_amdgcn_readlane(x, 32) + __builtin_amdgcn_readlane(x, 48);
+}
+
+// The same for causal launches, whose blocks take the longer the further they are from the front of their sequence (or, with `back`, from its
+// end): the rank-th block in descending order of that distance, over all sequences, so that the launch does not end with long ones.  With up to 62
+// sequences; with more the plain order does.  C(j) blocks have a distance of j or more; j with C(j) > rank >= C(j + 1) is the block's.
+template <int R>
+__device__ __forceinline__ SeqBlock seq_block_long_first(const SeqParams& p, int rank, int heads, bool back, int lane) {
+    if (!p.causal) return seq_block<R>(p, rank, heads, lane);
+    if (p.B + 2 > 64) return seq_block<R>(p, back ? rank : p.slots - 1 - rank, heads, lane);
+    const int at = seq_offset(p, min(lane, p.B + 2)), tokens = lane < p.B + 2 ? max(0, seq_offset(p, lane + 1) - at) : 0;
+    const int blocks = (tokens * heads + R - 1) / R;
+    int lo = 0, hi = 1;
+    while (__builtin_amdgcn_ballot_w64(blocks > hi)) hi *= 2;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (lanes_sum(max(0, blocks - mid)) > rank) lo = mid;
+        else hi = mid;
+    }
+    const int left = rank - lanes_sum(max(0, blocks - lo - 1));
+    const uint64_t those = __builtin_amdgcn_ballot_w64(blocks > lo);
+    const uint64_t one = __builtin_amdgcn_ballot_w64(blocks > lo && __popcll(those & ((uint64_t(1) << lane) - 1)) == left);
+    SeqBlock b;
+    b.some = one != 0;
+    b.segment = one ? __builtin_ctzll(one) : 0;
+    b.token = __builtin_amdgcn_readlane(at, b.segment);
+    b.tokens = __builtin_amdgcn_readlane(tokens, b.segment);
+    b.row0 = (back ? __builtin_amdgcn_readlane(blocks, b.segment) - 1 - lo : lo) * R;
+    b.held = 0;
+    return b;
+}
+
 // Keys of a segment and the position of its first query among them.
 template <bool PAGED>
 struct SeqKeys {
@@ -141,6 +178,22 @@ __device__ __forceinline__ uint32_t scale_codes(const void* at, bool words) {
 #pragma unroll
     for (int i = 0; i < GROUPS; ++i) codes |= (uint32_t)global<uint8_t>(static_cast<const uint8_t*>(at) + i) << (8 * i);
     return codes;
+}
+
+// Orders the instructions of a stretch without branches: LDS reads run `AHEAD` groups of READS ahead of the STEPS groups of MFMAS matrix
+// instructions that use them.  (Left to itself the compiler puts a read right in front of its use where registers are short, and every matrix
+// instruction waits for LDS.)
+template <int STEPS, int READS, int MFMAS, int AHEAD>
+__device__ __forceinline__ void reads_ahead() {
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+#pragma unroll
+    for (int i = 0; i < STEPS - AHEAD; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, MFMAS, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) __builtin_amdgcn_sched_group_barrier(0x008, MFMAS, 0);
 }
 
 // A tile of 64 looped rows in LDS, and where this lane reads its operands (tile algebra: sjvp_ctx.hpp).  Rows are unpadded (D in 65 to 96 have rows

@@ -8,6 +8,10 @@
 #pragma once
 #include "sjvp_seq_fwd.hpp"
 
+#ifndef XC
+#define XC 2
+#define XD 1
+#endif
 namespace sjvp {
 
 // 32 rows' numbers in LDS as the registers of a score tile
@@ -30,8 +34,8 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 3 : 2) void seq_bwd_row(Seq
     constexpr int kTile = SeqTile<HD>::kElems;
     elem_t* tiles = reinterpret_cast<elem_t*>(smem);  // K [2], V [2]
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
-    const int hk = blockIdx.x % p.Hkv, slot = p.causal ? p.slots - 1 - (int)(blockIdx.x / p.Hkv) : blockIdx.x / p.Hkv;
-    const SeqBlock b = seq_block<kCtxOwned>(p, slot, p.G, lane);
+    const int hk = blockIdx.x % p.Hkv;
+    const SeqBlock b = seq_block_long_first<kCtxOwned>(p, blockIdx.x / p.Hkv, p.G, false, lane);
     if (!b.some) return;
     const int all = b.tokens * p.G;
     const SeqKeys<false> keys(p, b);
@@ -152,8 +156,8 @@ __global__ __launch_bounds__(kCtxThreads * PAIR, HD <= 64 ? 2 * PAIR : PAIR) voi
     float* stats = reinterpret_cast<float*>(mine + (PAIR == 2 ? 4 * kTile : 0));  // [2][row_stat_folded, -delta][64]
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
     const int group = wave % kCtxWaves, half = wave / kCtxWaves;
-    const int hk = blockIdx.x % p.Hkv, slot = blockIdx.x / p.Hkv % p.slots, split = blockIdx.x / p.Hkv / p.slots;
-    const SeqBlock b = seq_block<kCtxOwned>(p, slot, 1, lane);
+    const int hk = blockIdx.x % p.Hkv, x = blockIdx.x / p.Hkv, split = x % p.splits;  // (splits side by side: they are equally long)
+    const SeqBlock b = seq_block_long_first<kCtxOwned>(p, x / p.splits, 1, true, lane);
     if (!b.some) return;
     const SeqKeys<false> keys(p, b);
     const int k0 = b.row0 + 32 * group, key = k0 + (lane & 31);
@@ -229,10 +233,23 @@ __global__ __launch_bounds__(kCtxThreads * PAIR, HD <= 64 ? 2 * PAIR : PAIR) voi
         const int row0 = PAIR == 2 ? 32 * half : 0, end = row0 + 32 * U;  // rows of the tile that are this wave's
         if (k0 < keys.keys && !(decltype(masked)::value && r0 + end <= k0)) {
             f32x16 s[U], ds[U];
+            if constexpr (PAIR == 2 && XC > 0) {
+            s[0] = f32x16{};
+            ds[0] = seq_of_rows(st + 2 * kCtxTile + row0, h);
+#pragma unroll
+            for (int c = 0; c < HD / 16; ++c) {
+                s[0] = Mma32<T>::run(at.rows(0, c), *SeqTile<HD>::template at<const u32x4>(own[c]), s[0]);
+                ds[0] = Mma32<T>::run(at.rows(kBytes, c), *SeqTile<HD>::template at<const u32x4>(own[c] + 2 * kBytes), ds[0]);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+            reads_ahead<HD / 16, 4, 2, XD>();
+            __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
+            } else {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 s[u] = products(u * kHalf, own_k, 0, f32x16{});
                 ds[u] = products(kBytes + u * kHalf, own_v, 2 * kBytes, seq_of_rows(st + 2 * kCtxTile + row0 + 32 * u, h));
+            }
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
@@ -262,6 +279,7 @@ __global__ __launch_bounds__(kCtxThreads * PAIR, HD <= 64 ? 2 * PAIR : PAIR) voi
                 at.template add_columns<T>(dv, kBytes + u * kHalf, s[u]);
                 at.template add_columns<T>(dk, u * kHalf, ds[u]);
             }
+            if constexpr (PAIR == 2 && XC > 0) reads_ahead<HD / 8, 2, 1, XC>();
         }
         at.move(step);
         step = -step;
@@ -272,10 +290,10 @@ __global__ __launch_bounds__(kCtxThreads * PAIR, HD <= 64 ? 2 * PAIR : PAIR) voi
     workgroup_barrier();
     // causal: the rows of the block's own positions stand in a head's first two tiles
     const int near = p.causal ? min(kCtxOwned / kCtxTile, per_head) : 0;
-    for (int x = 0, hq = first_head; x < nx; ++hq) {
+    for (int done = 0, hq = first_head; done < nx; ++hq) {
         int t = ta;
-        for (; t < ta + near; ++t) tile(x++, hq, t, std::true_type{});
-        for (; t < tb; ++t) tile(x++, hq, t, std::false_type{});
+        for (; t < ta + near; ++t) tile(done++, hq, t, std::true_type{});
+        for (; t < tb; ++t) tile(done++, hq, t, std::false_type{});
     }
     const bool scored = ok && keys.keys != 1;
     const int out_rows = min(max(b.tokens - k0, 0), 32);

@@ -40,8 +40,8 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 4 : 2) void seq_fwd(SeqPara
     elem_t* tiles = reinterpret_cast<elem_t*>(smem);  // K [2], V [2]
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
     const int hk = blockIdx.x % p.Hkv, x = blockIdx.x / p.Hkv, split = PAGED ? x / p.slots : 0;
-    const int slot = p.causal ? p.slots - 1 - (x - split * p.slots) : x;  // causal: long rows first
-    const SeqBlock b = seq_block<kCtxOwned, PAGED>(p, slot, p.G, lane);
+    const SeqBlock b = PAGED ? seq_block<kCtxOwned, true>(p, p.slots - 1 - (x - split * p.slots), p.G, lane)
+                             : seq_block_long_first<kCtxOwned>(p, x, p.G, false, lane);
     const int all = b.tokens * p.G;
     if (!b.some || all < p.least || all > p.most) return;
     const SeqKeys<PAGED> keys(p, b);
