@@ -8,10 +8,6 @@
 #pragma once
 #include "sjvp_seq_fwd.hpp"
 
-#ifndef XC
-#define XC 2
-#define XD 1
-#endif
 namespace sjvp {
 
 // 32 rows' numbers in LDS as the registers of a score tile
@@ -111,11 +107,15 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 3 : 2) void seq_bwd_row(Seq
         if (more) feed.request(p, t + 1, n, k_place(t + 1), v_place(t + 1), wave);
         if (key < n_wave) {
             f32x16 s[2], ds[2];
+            s[0] = s[1] = ds[0] = ds[1] = f32x16{};
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                s[u] = at.template scores<T>(u * kHalf, own_q);
-                ds[u] = at.template scores<T>(2 * kBytes + u * kHalf, own_g);
-            }
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int c = 0; c < HD / 16; ++c) {
+                    s[u] = Mma32<T>::run(at.rows(u * kHalf, c), own_q[c], s[u]);
+                    ds[u] = Mma32<T>::run(at.rows(2 * kBytes + u * kHalf, c), own_g[c], ds[u]);
+                }
+            reads_ahead<HD / 8, 2, 2, 2>();
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
 #pragma unroll
@@ -233,7 +233,7 @@ __global__ __launch_bounds__(kCtxThreads * PAIR, HD <= 64 ? 2 * PAIR : PAIR) voi
         const int row0 = PAIR == 2 ? 32 * half : 0, end = row0 + 32 * U;  // rows of the tile that are this wave's
         if (k0 < keys.keys && !(decltype(masked)::value && r0 + end <= k0)) {
             f32x16 s[U], ds[U];
-            if constexpr (PAIR == 2 && XC > 0) {
+            if constexpr (PAIR == 2) {
             s[0] = f32x16{};
             ds[0] = seq_of_rows(st + 2 * kCtxTile + row0, h);
 #pragma unroll
@@ -242,7 +242,7 @@ __global__ __launch_bounds__(kCtxThreads * PAIR, HD <= 64 ? 2 * PAIR : PAIR) voi
                 ds[0] = Mma32<T>::run(at.rows(kBytes, c), *SeqTile<HD>::template at<const u32x4>(own[c] + 2 * kBytes), ds[0]);
             }
             __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
-            reads_ahead<HD / 16, 4, 2, XD>();
+            reads_ahead<HD / 16, 4, 2, 1>();
             __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
             } else {
 #pragma unroll
@@ -279,7 +279,7 @@ __global__ __launch_bounds__(kCtxThreads * PAIR, HD <= 64 ? 2 * PAIR : PAIR) voi
                 at.template add_columns<T>(dv, kBytes + u * kHalf, s[u]);
                 at.template add_columns<T>(dk, u * kHalf, ds[u]);
             }
-            if constexpr (PAIR == 2 && XC > 0) reads_ahead<HD / 8, 2, 1, XC>();
+            if constexpr (PAIR == 2) reads_ahead<HD / 8, 2, 1, 2>();
         }
         at.move(step);
         step = -step;
