@@ -1,7 +1,6 @@
 // C ABI of the attention over packed sequences and over a paged cache: checks, how the work is split, and the launches.
 #include <climits>
 #include <cmath>
-#include <cstdlib>
 
 #include "sjvp_seq_launch.hpp"
 
@@ -112,8 +111,7 @@ struct PackedPlan {
 PackedPlan packed_plan(const SeqParams& p) {
     PackedPlan plan;
     const int64_t blocks = (p.T / kCtxOwned + 1) * (int64_t)p.Hkv;
-    static const int CU = getenv("CUY") ? atoi(getenv("CUY")) : 4; // XXX
-    plan.splits = (int)std::max<int64_t>(1, std::min<int64_t>(CU * (int64_t)compute_units() / blocks, p.G));
+    plan.splits = (int)std::max<int64_t>(1, std::min<int64_t>(4 * (int64_t)compute_units() / blocks, p.G));
     plan.part = (3 * (size_t)p.Hq * p.T + 3) / 4 * 4;
     plan.total = plan.part + (plan.splits > 1 ? 2 * (size_t)plan.splits * p.Hkv * p.T * ctx_padded(p.D) : 0);
     return plan;

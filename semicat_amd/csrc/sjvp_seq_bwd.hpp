@@ -143,195 +143,255 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 3 : 2) void seq_bwd_row(Seq
     });
 }
 
-// Column-owned: groups of 32 keys share tiles of 64 query rows, over all heads that read the key head (or, with splits, over a part of them).  A group is
-// one wave, or two that take 32 rows of a tile each and add their sums up in the end: at D = 128 the sums and operands of 32 keys fill the
-// registers of two waves to a SIMD either way, and two waves fill each other's gaps.
-template <typename T, int HD, bool DMA, int PAIR>
-__global__ __launch_bounds__(kCtxThreads * PAIR, HD <= 64 ? 2 * PAIR : PAIR) void seq_bwd_col(SeqParams p) {
-    if constexpr (DMA) __builtin_assume(p.D % 8 == 0);
-    extern __shared__ __align__(16) unsigned char smem[];
-    constexpr int kTile = SeqTile<HD>::kElems, NT = kCtxThreads * PAIR, U = 2 / PAIR;
-    elem_t* tiles = reinterpret_cast<elem_t*>(smem);             // [2][Q, dO]
-    elem_t* mine = tiles + 4 * kTile;                            // PAIR == 2: K [2], V [2] of the workgroup's keys
-    float* stats = reinterpret_cast<float*>(mine + (PAIR == 2 ? 4 * kTile : 0));  // [2][row_stat_folded, -delta][64]
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
-    const int group = wave % kCtxWaves, half = wave / kCtxWaves;
-    const int hk = blockIdx.x % p.Hkv, x = blockIdx.x / p.Hkv, split = x % p.splits;  // (splits side by side: they are equally long)
-    const SeqBlock b = seq_block_long_first<kCtxOwned>(p, x / p.splits, 1, true, lane);
-    if (!b.some) return;
-    const SeqKeys<false> keys(p, b);
-    const int k0 = b.row0 + 32 * group, key = k0 + (lane & 31);
-    const bool ok = key < keys.keys;
-    u32x4 own_k[PAIR == 1 ? HD / 16 : 1], own_v[PAIR == 1 ? HD / 16 : 1];
-    if constexpr (PAIR == 1) {
-        own_operands<HD>(own_k, p.k.head(0, hk) + (int64_t)(b.token + key) * p.k.sl, ok, h, p.D);
-        own_operands<HD>(own_v, p.v.head(0, hk) + (int64_t)(b.token + key) * p.v.sl, ok, h, p.D);
+// What the column-owned launches have in common: the block of keys, the heads of a split, and the tiles of 64 query rows that see a key of the block,
+// head by head.
+struct SeqCols {
+    int hk, split, ta, tb, first_head, heads, tiles;
+    SeqBlock b;
+    __device__ __forceinline__ SeqCols(const SeqParams& p, int lane)
+        : hk(blockIdx.x % p.Hkv), split(blockIdx.x / p.Hkv % p.splits),  // (splits side by side: they are equally long)
+          b(seq_block_long_first<kCtxOwned>(p, blockIdx.x / p.Hkv / p.splits, 1, true, lane)) {
+        const int keys = SeqKeys<false>(p, b).keys;
+        ta = p.causal ? b.row0 / kCtxTile : 0, tb = (keys + kCtxTile - 1) / kCtxTile;
+        first_head = hk * p.G + p.G * split / p.splits, heads = hk * p.G + p.G * (split + 1) / p.splits - first_head;
+        tiles = heads * max(0, tb - ta);
     }
-    // tiles of query rows that see a key of the workgroup, head by head
-    const int ta = p.causal ? b.row0 / kCtxTile : 0, tb = (keys.keys + kCtxTile - 1) / kCtxTile, per_head = max(0, tb - ta);
-    const int first_head = hk * p.G + p.G * split / p.splits, heads = hk * p.G + p.G * (split + 1) / p.splits - first_head;
-    const int nx = heads * per_head;
+};
 
-    RowFeed<HD, DMA, NT> qf(p.q.sl, p.D, tid), gf(p.g.sl, p.D, tid);
-    constexpr int kHalf = 32 * SeqTile<HD>::kLd * 2, kBytes = SeqTile<HD>::kBytes;
-    SeqTile<HD> at(tiles + (PAIR == 2 ? half * (kHalf / 2) : 0), lane);  // (a pair's second wave: rows 32 .. 63)
-    float stat = 0.0f;
-    const auto place = [&](int x) { return tiles + (x & 1) * 2 * kTile; };
-    const auto request = [&](int x, int hq, int r0) {
+// Tiles of Q and dO (one behind the other in LDS) with the statistics of their rows, requested by NT threads.
+template <int HD, bool DMA, int NT>
+struct ColFeed {
+    RowFeed<HD, DMA, NT> qf, gf;
+    float stat;
+    __device__ __forceinline__ ColFeed(const SeqParams& p, int tid) : qf(p.q.sl, p.D, tid), gf(p.g.sl, p.D, tid), stat(0.0f) {}
+    __device__ __forceinline__ void request(const SeqParams& p, const SeqBlock& b, int hq, int r0, elem_t* place, int tid, int wave) {
         const int64_t token = b.token + r0;
-        qf.request(p.q.head(0, hq) + token * p.q.sl, p.q.sl, b.tokens - r0, p.D, place(x), wave);
-        gf.request(p.g.head(0, hq) + token * p.g.sl, p.g.sl, b.tokens - r0, p.D, place(x) + kTile, wave);
+        qf.request(p.q.head(0, hq) + token * p.q.sl, p.q.sl, b.tokens - r0, p.D, place, wave);
+        gf.request(p.g.head(0, hq) + token * p.g.sl, p.g.sl, b.tokens - r0, p.D, place + SeqTile<HD>::kElems, wave);
         if (tid < 3 * kCtxTile) {
             const int i = tid & (kCtxTile - 1);
             const float* from = p.folded + (tid / kCtxTile * (int64_t)p.Hq + hq) * p.T + token;
             stat = r0 + i < b.tokens ? from[i] : tid < kCtxTile ? INFINITY : tid < 2 * kCtxTile ? 1.0f : 0.0f;
         }
-    };
-    const auto deliver = [&](int x) {
-        qf.deliver(place(x), p.D, tid);
-        gf.deliver(place(x) + kTile, p.D, tid);
-        if (tid < 3 * kCtxTile) stats[(x & 1) * (kCtxStats / 2) + tid] = stat;
-    };
-    if (nx) {
-        request(0, first_head, ta * kCtxTile);
-        deliver(0);
-        if constexpr (PAIR == 2) {
-            RowFeed<HD, DMA, NT> kf(p.k.sl, p.D, tid), vf(p.v.sl, p.D, tid);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int k = b.row0 + i * kCtxTile;
-                kf.request(p.k.head(0, hk) + (int64_t)(b.token + k) * p.k.sl, p.k.sl, keys.keys - k, p.D, mine + i * kTile, wave);
-                vf.request(p.v.head(0, hk) + (int64_t)(b.token + k) * p.v.sl, p.v.sl, keys.keys - k, p.D, mine + (2 + i) * kTile, wave);
-                kf.deliver(mine + i * kTile, p.D, tid);
-                vf.deliver(mine + (2 + i) * kTile, p.D, tid);
-            }
-        }
-        qf.arrived();
     }
-    // scores of 32 rows of a tile and the wave's keys (32 group .. of the two tiles of K, or of V behind them)
-    uint32_t own[HD / 16];
+    __device__ __forceinline__ void deliver(const SeqParams& p, elem_t* place, float* stats, int tid) {
+        qf.deliver(place, p.D, tid);
+        gf.deliver(place + SeqTile<HD>::kElems, p.D, tid);
+        if (tid < 3 * kCtxTile) stats[tid] = stat;
+    }
+};
+
+// P and dS of 32 rows from their scores and dP - delta.  st: [row_stat_folded, -delta][64] from the first of the rows on; key: this lane's, from that row on.
+template <bool MASKED, bool FACTORS>
+__device__ __forceinline__ void col_probabilities(f32x16& s, f32x16& ds, const float* st, float c, int key, int h) {
 #pragma unroll
-    for (int c = 0; c < HD / 16; ++c) own[c] = at.row[c] - half * kHalf + 4 * kBytes + group * kHalf;
-    const auto products = [&](int from, const u32x4* own_rows, int own_from, f32x16 x) {
-        if constexpr (PAIR == 1) return at.template scores<T>(from, own_rows, x);
+    for (int i = 0; i < 4; ++i) {
+        const f32x4 less = *reinterpret_cast<const f32x4*>(st + 8 * i + 4 * h);
+        f32x4 factor;
+        if constexpr (FACTORS) factor = *reinterpret_cast<const f32x4*>(st + kCtxTile + 8 * i + 4 * h);
 #pragma unroll
-        for (int c = 0; c < HD / 16; ++c) x = Mma32<T>::run(at.rows(from, c), *SeqTile<HD>::template at<const u32x4>(own[c] + own_from), x);
-        return x;
-    };
+        for (int j = 0; j < 4; ++j) {
+            float y = fast_exp2(__builtin_fmaf(s[4 * i + j], c, -less[j]));
+            if constexpr (FACTORS) y *= factor[j];
+            ds[4 * i + j] *= y;
+            if constexpr (MASKED)
+                if (8 * i + j < key - 4 * h) y = 0.0f, ds[4 * i + j] = 0.0f;  // a row ahead of the key
+            s[4 * i + j] = y;
+        }
+    }
+}
+
+// dK or dV of a wave's 32 keys to where they go: the result, or a split's sums.
+template <typename T, int HD>
+__device__ __forceinline__ void store_col(const SeqParams& p, const SeqCols& w, f32x16* sum, bool some, float factor, const CtxView& out, int which, int k0,
+                                          elem_t* region, int lane) {
+    const int rows = min(max(w.b.tokens - k0, 0), 32);
+    if (p.splits > 1) {
+        const int64_t place = ((int64_t)(2 * w.split + which) * p.Hkv + w.hk) * p.T + w.b.token + k0;
+        store_part<HD>(sum, some, p.part + place * HD, rows, lane);
+    } else {
+        store_rows_at<T, HD>(sum, some ? factor : 0.0f, rows, region, lane, p.D,
+                             [&](int row) { return out.head(0, w.hk) + (int64_t)(w.b.token + k0 + row) * out.sl; });
+    }
+}
+
+// Column-owned: four waves of 32 keys share tiles of 64 query rows, over all heads that read the key head (or, with splits, over a part of them).
+template <typename T, int HD, bool DMA>
+__global__ __launch_bounds__(kCtxThreads, 2) void seq_bwd_col(SeqParams p) {
+    if constexpr (DMA) __builtin_assume(p.D % 8 == 0);
+    extern __shared__ __align__(16) unsigned char smem[];
+    constexpr int kTile = SeqTile<HD>::kElems, kHalf = 32 * SeqTile<HD>::kLd * 2, kBytes = SeqTile<HD>::kBytes;
+    elem_t* tiles = reinterpret_cast<elem_t*>(smem);             // [2][Q, dO]
+    float* stats = reinterpret_cast<float*>(tiles + 4 * kTile);  // [2][row_stat_folded, -delta][64]
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+    const SeqCols w(p, lane);
+    if (!w.b.some) return;
+    const int keys = SeqKeys<false>(p, w.b).keys, k0 = w.b.row0 + 32 * wave, key = k0 + (lane & 31);
+    const bool ok = key < keys;
+    u32x4 own_k[HD / 16], own_v[HD / 16];
+    own_operands<HD>(own_k, p.k.head(0, w.hk) + (int64_t)(w.b.token + key) * p.k.sl, ok, h, p.D);
+    own_operands<HD>(own_v, p.v.head(0, w.hk) + (int64_t)(w.b.token + key) * p.v.sl, ok, h, p.D);
+    ColFeed<HD, DMA, kCtxThreads> feed(p, tid);
+    SeqTile<HD> at(tiles, lane);
+    const auto place = [&](int x) { return tiles + (x & 1) * 2 * kTile; };
+    const auto st_place = [&](int x) { return stats + (x & 1) * (kCtxStats / 2); };
+    if (w.tiles) {
+        feed.request(p, w.b, w.first_head, w.ta * kCtxTile, place(0), tid, wave);
+        feed.deliver(p, place(0), st_place(0), tid);
+        feed.qf.arrived();
+    }
     f32x16 dk[HD / 32] = {}, dv[HD / 32] = {};
-    constexpr bool kFactors = HD > 64;
     int step = 2 * kBytes;
     // x: tiles before this one; hq, t: the head and the tile of its rows
     const auto tile = [&](int x, int hq, int t, auto masked) {
         const int r0 = t * kCtxTile;
-        if (x + 1 < nx) {
-            const bool last = t + 1 == tb;
-            request(x + 1, last ? hq + 1 : hq, (last ? ta : t + 1) * kCtxTile);
+        const bool more = x + 1 < w.tiles;
+        if (more) {
+            const bool last = t + 1 == w.tb;
+            feed.request(p, w.b, last ? hq + 1 : hq, (last ? w.ta : t + 1) * kCtxTile, place(x + 1), tid, wave);
         }
-        const float* st = stats + (x & 1) * (kCtxStats / 2);
-        const bool factors = !kFactors && __builtin_amdgcn_ballot_w64(st[kCtxTile + lane] != 1.0f);
-        const int row0 = PAIR == 2 ? 32 * half : 0, end = row0 + 32 * U;  // rows of the tile that are this wave's
-        if (k0 < keys.keys && !(decltype(masked)::value && r0 + end <= k0)) {
-            f32x16 s[U], ds[U];
-            if constexpr (PAIR == 2) {
-            s[0] = f32x16{};
-            ds[0] = seq_of_rows(st + 2 * kCtxTile + row0, h);
+        if (k0 < keys && !(decltype(masked)::value && r0 + kCtxTile <= k0)) {
+            const float* st = st_place(x);
+            const bool factors = __builtin_amdgcn_ballot_w64(st[kCtxTile + lane] != 1.0f);
+            f32x16 s[2], ds[2];
 #pragma unroll
-            for (int c = 0; c < HD / 16; ++c) {
-                s[0] = Mma32<T>::run(at.rows(0, c), *SeqTile<HD>::template at<const u32x4>(own[c]), s[0]);
-                ds[0] = Mma32<T>::run(at.rows(kBytes, c), *SeqTile<HD>::template at<const u32x4>(own[c] + 2 * kBytes), ds[0]);
-            }
-            __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
-            reads_ahead<HD / 16, 4, 2, 1>();
-            __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
-            } else {
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                s[u] = products(u * kHalf, own_k, 0, f32x16{});
-                ds[u] = products(kBytes + u * kHalf, own_v, 2 * kBytes, seq_of_rows(st + 2 * kCtxTile + row0 + 32 * u, h));
-            }
+            for (int u = 0; u < 2; ++u) {
+                s[u] = at.template scores<T>(u * kHalf, own_k);
+                ds[u] = at.template scores<T>(kBytes + u * kHalf, own_v, seq_of_rows(st + 2 * kCtxTile + 32 * u, h));
             }
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const float* sr = st + row0 + 32 * u;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const f32x4 less = *reinterpret_cast<const f32x4*>(sr + 8 * i + 4 * h);
-                    f32x4 factor;
-                    if constexpr (kFactors) factor = *reinterpret_cast<const f32x4*>(sr + kCtxTile + 8 * i + 4 * h);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        float y = fast_exp2(__builtin_fmaf(s[u][4 * i + j], p.c, -less[j]));
-                        if constexpr (kFactors) y *= factor[j];
-                        ds[u][4 * i + j] *= y;
-                        if constexpr (decltype(masked)::value)
-                            if (row0 + 32 * u + 8 * i + j < key - r0 - 4 * h) y = 0.0f, ds[u][4 * i + j] = 0.0f;  // a row ahead of the key
-                        s[u][4 * i + j] = y;
-                    }
-                }
-                if (!kFactors && factors) {
-                    const f32x16 factor = seq_of_rows(sr + kCtxTile, h);
+            for (int u = 0; u < 2; ++u) {
+                col_probabilities<decltype(masked)::value, false>(s[u], ds[u], st + 32 * u, p.c, key - r0 - 32 * u, h);
+                if (factors) {
+                    const f32x16 factor = seq_of_rows(st + kCtxTile + 32 * u, h);
                     s[u] *= factor, ds[u] *= factor;
                 }
             }
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
+            for (int u = 0; u < 2; ++u) {
                 at.template add_columns<T>(dv, kBytes + u * kHalf, s[u]);
                 at.template add_columns<T>(dk, u * kHalf, ds[u]);
             }
-            if constexpr (PAIR == 2) reads_ahead<HD / 8, 2, 1, 2>();
         }
         at.move(step);
         step = -step;
-        if (x + 1 < nx) deliver(x + 1);
-        qf.arrived();
+        if (more) feed.deliver(p, place(x + 1), st_place(x + 1), tid);
+        feed.qf.arrived();
         workgroup_barrier();
     };
     workgroup_barrier();
     // causal: the rows of the block's own positions stand in a head's first two tiles
-    const int near = p.causal ? min(kCtxOwned / kCtxTile, per_head) : 0;
-    for (int done = 0, hq = first_head; done < nx; ++hq) {
-        int t = ta;
-        for (; t < ta + near; ++t) tile(done++, hq, t, std::true_type{});
-        for (; t < tb; ++t) tile(done++, hq, t, std::false_type{});
+    const int near = p.causal ? min(kCtxOwned / kCtxTile, w.tb - w.ta) : 0;
+    for (int done = 0, hq = w.first_head; done < w.tiles; ++hq) {
+        int t = w.ta;
+        for (; t < w.ta + near; ++t) tile(done++, hq, t, std::true_type{});
+        for (; t < w.tb; ++t) tile(done++, hq, t, std::false_type{});
     }
-    const bool scored = ok && keys.keys != 1;
-    const int out_rows = min(max(b.tokens - k0, 0), 32);
+    elem_t* region = tiles + wave * 32 * (HD + 8);
+    store_col<T, HD>(p, w, dk, ok && keys != 1, p.scale, p.dk, 0, k0, region, lane);
+    store_col<T, HD>(p, w, dv, ok, 1.0f, p.dv, 1, k0, region, lane);
+}
+
+// The same above D = 64, where the sums and operands of 32 keys are more than the registers of two waves to a SIMD: K and V stand in LDS, and a group
+// of 32 keys has two waves, with 32 rows of a tile each, whose sums are added up in the end.
+template <typename T, int HD, bool DMA>
+__global__ __launch_bounds__(2 * kCtxThreads, 2) void seq_bwd_col_pair(SeqParams p) {
+    if constexpr (DMA) __builtin_assume(p.D % 8 == 0);
+    extern __shared__ __align__(16) unsigned char smem[];
+    constexpr int kTile = SeqTile<HD>::kElems, kHalf = 32 * SeqTile<HD>::kLd * 2, kBytes = SeqTile<HD>::kBytes, NT = 2 * kCtxThreads;
+    elem_t* tiles = reinterpret_cast<elem_t*>(smem);             // [2][Q, dO]
+    elem_t* mine = tiles + 4 * kTile;                            // K [2], V [2]
+    float* stats = reinterpret_cast<float*>(mine + 4 * kTile);   // [2][row_stat_folded, -delta][64]
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+    const int group = wave % kCtxWaves, half = wave / kCtxWaves;
+    const SeqCols w(p, lane);
+    if (!w.b.some) return;
+    const int keys = SeqKeys<false>(p, w.b).keys, k0 = w.b.row0 + 32 * group, key = k0 + (lane & 31);
+    const bool ok = key < keys;
+    ColFeed<HD, DMA, NT> feed(p, tid);
+    SeqTile<HD> at(tiles + half * (kHalf / 2), lane);  // (the second wave: rows 32 .. 63)
+    const auto place = [&](int x) { return tiles + (x & 1) * 2 * kTile; };
+    const auto st_place = [&](int x) { return stats + (x & 1) * (kCtxStats / 2); };
+    if (w.tiles) {
+        feed.request(p, w.b, w.first_head, w.ta * kCtxTile, place(0), tid, wave);
+        feed.deliver(p, place(0), st_place(0), tid);
+        RowFeed<HD, DMA, NT> kf(p.k.sl, p.D, tid), vf(p.v.sl, p.D, tid);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int k = w.b.row0 + i * kCtxTile;
+            kf.request(p.k.head(0, w.hk) + (int64_t)(w.b.token + k) * p.k.sl, p.k.sl, keys - k, p.D, mine + i * kTile, wave);
+            vf.request(p.v.head(0, w.hk) + (int64_t)(w.b.token + k) * p.v.sl, p.v.sl, keys - k, p.D, mine + (2 + i) * kTile, wave);
+            kf.deliver(mine + i * kTile, p.D, tid);
+            vf.deliver(mine + (2 + i) * kTile, p.D, tid);
+        }
+        feed.qf.arrived();
+    }
+    uint32_t own[HD / 16];  // LDS addresses of the wave's rows of K; V two tiles behind
+#pragma unroll
+    for (int c = 0; c < HD / 16; ++c) own[c] = at.row[c] - half * kHalf + 4 * kBytes + group * kHalf;
+    f32x16 dk[HD / 32] = {}, dv[HD / 32] = {};
+    int step = 2 * kBytes;
+    const auto tile = [&](int x, int hq, int t, auto masked) {
+        const int r0 = t * kCtxTile + 32 * half;  // the wave's rows
+        const bool more = x + 1 < w.tiles;
+        if (more) {
+            const bool last = t + 1 == w.tb;
+            feed.request(p, w.b, last ? hq + 1 : hq, (last ? w.ta : t + 1) * kCtxTile, place(x + 1), tid, wave);
+        }
+        if (k0 < keys && !(decltype(masked)::value && r0 + 32 <= k0)) {
+            const float* st = st_place(x) + 32 * half;
+            f32x16 s = {}, ds = seq_of_rows(st + 2 * kCtxTile, h);
+#pragma unroll
+            for (int c = 0; c < HD / 16; ++c) {
+                s = Mma32<T>::run(at.rows(0, c), *SeqTile<HD>::template at<const u32x4>(own[c]), s);
+                ds = Mma32<T>::run(at.rows(kBytes, c), *SeqTile<HD>::template at<const u32x4>(own[c] + 2 * kBytes), ds);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);  // (-delta)
+            reads_ahead<HD / 16, 4, 2, 1>();
+            __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);  // (the other statistics)
+            col_probabilities<decltype(masked)::value, true>(s, ds, st, p.c, key - r0, h);
+            at.template add_columns<T>(dv, kBytes, s);
+            at.template add_columns<T>(dk, 0, ds);
+            reads_ahead<HD / 8, 2, 1, 2>();
+        }
+        at.move(step);
+        step = -step;
+        if (more) feed.deliver(p, place(x + 1), st_place(x + 1), tid);
+        feed.qf.arrived();
+        workgroup_barrier();
+    };
+    workgroup_barrier();
+    const int near = p.causal ? min(kCtxOwned / kCtxTile, w.tb - w.ta) : 0;
+    for (int done = 0, hq = w.first_head; done < w.tiles; ++hq) {
+        int t = w.ta;
+        for (; t < w.ta + near; ++t) tile(done++, hq, t, std::true_type{});
+        for (; t < w.tb; ++t) tile(done++, hq, t, std::false_type{});
+    }
     elem_t* region = tiles + group * 32 * (HD + 8);
     const auto finish = [&](f32x16* sum, bool some, float factor, const CtxView& out, int which) {
-        if constexpr (PAIR == 2) {
-            // [group][register][lane]: the sums of the second waves take the place of the tiles
-            f32x4* there = reinterpret_cast<f32x4*>(tiles) + group * (HD / 32) * 4 * 64 + lane;
-            if (half)
+        // [group][register][lane]: the sums of the second waves take the place of the tiles
+        f32x4* there = reinterpret_cast<f32x4*>(tiles) + group * (HD / 32) * 4 * 64 + lane;
+        if (half)
 #pragma unroll
-                for (int dt = 0; dt < HD / 32; ++dt)
+            for (int dt = 0; dt < HD / 32; ++dt)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        there[(4 * dt + i) * 64] = f32x4{sum[dt][4 * i], sum[dt][4 * i + 1], sum[dt][4 * i + 2], sum[dt][4 * i + 3]};
-            workgroup_barrier();
-            if (!half)
+                for (int i = 0; i < 4; ++i)
+                    there[(4 * dt + i) * 64] = f32x4{sum[dt][4 * i], sum[dt][4 * i + 1], sum[dt][4 * i + 2], sum[dt][4 * i + 3]};
+        workgroup_barrier();
+        if (!half)
 #pragma unroll
-                for (int dt = 0; dt < HD / 32; ++dt)
+            for (int dt = 0; dt < HD / 32; ++dt)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const f32x4 other = there[(4 * dt + i) * 64];
+                for (int i = 0; i < 4; ++i) {
+                    const f32x4 other = there[(4 * dt + i) * 64];
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) sum[dt][4 * i + j] += other[j];
-                    }
-            workgroup_barrier();
-        }
-        if (half == 0) {
-            if (p.splits > 1) {
-                const int64_t place = ((int64_t)(2 * split + which) * p.Hkv + hk) * p.T + b.token + k0;
-                store_part<HD>(sum, some, p.part + place * HD, out_rows, lane);
-            } else {
-                store_rows_at<T, HD>(sum, some ? factor : 0.0f, out_rows, region, lane, p.D,
-                                     [&](int row) { return out.head(0, hk) + (int64_t)(b.token + k0 + row) * out.sl; });
-            }
-        }
-        if constexpr (PAIR == 2) workgroup_barrier();
+                    for (int j = 0; j < 4; ++j) sum[dt][4 * i + j] += other[j];
+                }
+        workgroup_barrier();
+        if (!half) store_col<T, HD>(p, w, sum, some, factor, out, which, k0, region, lane);
+        workgroup_barrier();
     };
-    finish(dk, scored, p.scale, p.dk, 0);
+    finish(dk, ok && keys != 1, p.scale, p.dk, 0);
     finish(dv, ok, 1.0f, p.dv, 1);
 }
 

@@ -20,8 +20,10 @@ int seq_packed_bwd<SJVP_T>(SeqParams p, hipStream_t stream) {
     return seq_by_head(p.D, col_dma, [&](auto hd, auto dma) {
         constexpr int HD = decltype(hd)::value;
         constexpr bool DMA = decltype(dma)::value;
-        constexpr int PAIR = HD > 64 ? 2 : 1;
-        const int rc = launch(seq_bwd_col<SJVP_T, HD, DMA, PAIR>, p.slots * p.Hkv * p.splits, PAIR * seq_tiles_bytes(HD) + 4 * kCtxStats, stream, p, kCtxThreads * PAIR);
+        const int grid = p.slots * p.Hkv * p.splits;
+        int rc;
+        if constexpr (HD > 64) rc = launch(seq_bwd_col_pair<SJVP_T, HD, DMA>, grid, 2 * seq_tiles_bytes(HD) + 4 * kCtxStats, stream, p, 2 * kCtxThreads);
+        else rc = launch(seq_bwd_col<SJVP_T, HD, DMA>, grid, seq_tiles_bytes(HD) + 4 * kCtxStats, stream, p, kCtxThreads);
         if (rc != SJVP_OK || p.splits == 1) return rc;
         return launch(seq_sum<SJVP_T, HD>, (int)((2 * (int64_t)p.Hkv * p.T * (HD / 8) + kCtxThreads - 1) / kCtxThreads), 0, stream, p, kCtxThreads);
     });
