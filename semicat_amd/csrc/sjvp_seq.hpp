@@ -482,6 +482,35 @@ struct SeqSums {
     }
 };
 
+// Infinities and NaN in values that a causal row does not see: a contraction makes NaN of them by a probability of zero, for every row of the tile.
+// Tiles that some rows see in part are looked at before they are used; such numbers are added to the rows that see them one by one, and
+// taken out of the tile.
+template <typename T> constexpr uint32_t kExponents = std::is_same_v<T, Bf16> ? 0x7f807f80u : 0x7c007c00u;
+// bits 15 and 31: whether the numbers of a pair are not finite
+template <typename T>
+__device__ __forceinline__ uint32_t not_finite(uint32_t pair) {
+    return ((pair & kExponents<T>) + (std::is_same_v<T, Bf16> ? 0x00800080u : 0x04000400u)) & 0x80008000u;
+}
+template <typename T>
+__device__ __forceinline__ bool any_not_finite(u32x4 x) {
+    return (not_finite<T>(x[0]) | not_finite<T>(x[1]) | not_finite<T>(x[2]) | not_finite<T>(x[3])) != 0;
+}
+template <typename T>
+__device__ __forceinline__ u32x4 only_finite(u32x4 x) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] &= ~((not_finite<T>(x[i]) >> 15) * 0xffffu);
+    return x;
+}
+// What is not finite of four numbers in LDS.  (Behind a wall, so that it takes few registers.)
+template <typename T>
+__device__ __forceinline__ f32x4 only_not_finite(const elem_t* from) {
+    u32x2 x = *reinterpret_cast<const u32x2*>(from);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) x[i] &= (not_finite<T>(x[i]) >> 15) * 0xffffu;
+    asm volatile("" ::: "memory");
+    return f32x4{T::to_float((elem_t)x[0]), T::to_float((elem_t)(x[0] >> 16)), T::to_float((elem_t)x[1]), T::to_float((elem_t)(x[1] >> 16))};
+}
+
 // Sums of a wave's own 32 rows, OUT^T, as rows in memory whose places `at` gives, through the wave's own LDS region of [32][HD + 8].
 template <typename T, int HD, typename F>
 __device__ __forceinline__ void store_rows_at(const f32x16* acc, float factor, int rows, elem_t* region, int lane, int D, F&& at) {

@@ -60,98 +60,103 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 4 : 2) void seq_fwd(SeqPara
     FEED feed(p, b, hk, tid);
     SeqTile<HD> at(tiles, lane);
     SeqSums<HD> st;
-    if constexpr (kAhead) {
-    const auto k_place = [&](int t) { return tiles + (t & 1) * kTile; };
-    const auto v_place = [&](int t) { return tiles + (2 + (t & 1)) * kTile; };
-    // K runs a tile ahead of V, so that the scores of the next tile are made beside the exponentials of this one.
-    if (nt) {
-        feed.look(p, 0, n);
-        feed.request_k(p, 0, n, k_place(0), wave);
-        feed.request_v(p, 0, n, v_place(0), wave);
-        feed.deliver_k(p, k_place(0), tid);
-        feed.deliver_v(p, v_place(0), tid);
-        if (nt > 1) {
-            feed.look(p, 1, n);
-            feed.request_k(p, 1, n, k_place(1), wave);
-            feed.deliver_k(p, k_place(1), tid);
-        }
-    }
-    feed.arrived();
-    workgroup_barrier();
     constexpr int kHalf = 32 * SeqTile<HD>::kLd * 2, kV = 2 * SeqTile<HD>::kBytes;
     int step = SeqTile<HD>::kBytes;
-    f32x16 s[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) s[u] = at.template scores<T>(u * kHalf, own);
-    workgroup_barrier();
-    const auto tile = [&](int t, auto masked) {
-        if (t + 1 < nt) feed.request_v(p, t + 1, n, v_place(t + 1), wave);
-        if (t + 2 < nt) {
-            feed.look(p, t + 2, n);
-            feed.request_k(p, t + 2, n, k_place(t), wave);
-        }
-        at.move(step);
-        if (t * kCtxTile < n_wave) {
-            st.template raise<decltype(masked)::value>(s, p.c, limit - t * kCtxTile, h);
-            f32x16 next[2];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) next[u] = at.template scores<T>(u * kHalf, own);
-            st.exponentials(s, p.c);
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                at.template add_columns<T>(st.acc, kV - step + u * kHalf, s[u]);
-                s[u] = next[u];
-            }
-        }
-        step = -step;
-        if (t + 1 < nt) feed.deliver_v(p, v_place(t + 1), tid);
-        if (t + 2 < nt) feed.deliver_k(p, k_place(t), tid);
-        feed.arrived();
-        workgroup_barrier();
-    };
-    // (the tiles that all rows see as a whole have a loop without masks)
-    const int free = min(whole / kCtxTile, nt);
-    int t = 0;
-    for (; t < free; ++t) tile(t, std::false_type{});
-    for (; t < nt; ++t) tile(t, std::true_type{});
-    } else {
     const auto k_place = [&](int t) { return tiles + ((t - t0) & 1) * kTile; };
     const auto v_place = [&](int t) { return tiles + (2 + ((t - t0) & 1)) * kTile; };
-    if (t0 < nt) {
-        feed.look(p, t0, n);
-        feed.request(p, t0, n, k_place(t0), v_place(t0), wave);
-        if (t0 + 1 < nt) feed.look(p, t0 + 1, n);
-        feed.deliver(p, k_place(t0), v_place(t0), tid);
-    }
-    feed.arrived();
-    workgroup_barrier();
-    constexpr int kHalf = 32 * SeqTile<HD>::kLd * 2, kV = 2 * SeqTile<HD>::kBytes;
-    int step = SeqTile<HD>::kBytes;
-    const auto tile = [&](int t, auto masked) {
-        const bool more = t + 1 < nt;
-        if (more) {
-            feed.request(p, t + 1, n, k_place(t + 1), v_place(t + 1), wave);
-            if (t + 2 < nt) feed.look(p, t + 2, n);
-        }
-        if (t * kCtxTile < n_wave) {
-            f32x16 s[2];
+    // tile t's values that are not finite
+    const auto care = [&](int t) {
+        elem_t* V = v_place(t);
+        bool some = false;
+        for (int x = tid; x < kTile / 8; x += kCtxThreads) some = some || any_not_finite<T>(reinterpret_cast<const u32x4*>(V)[x]);
+        if (!workgroup_barrier_or(some)) return;
+        for (int j = 0; j < min(limit - t * kCtxTile, kCtxTile); ++j) {
+            const elem_t* from = V + j * SeqTile<HD>::kLd + 4 * h;
 #pragma unroll
-            for (int u = 0; u < 2; ++u) s[u] = at.template scores<T>(u * kHalf, own);
-            st.template take<decltype(masked)::value>(s, p.c, limit - t * kCtxTile, h);
+            for (int c = 0; c < HD / 8; ++c) {
+                const f32x4 more = only_not_finite<T>(from + 8 * (c ^ SeqTile<HD>::swz(j)));
 #pragma unroll
-            for (int u = 0; u < 2; ++u) at.template add_columns<T>(st.acc, kV + u * kHalf, s[u]);
+                for (int i = 0; i < 4; ++i) st.acc[c / 4][4 * (c % 4) + i] += more[i];
+            }
         }
-        at.move(step);
-        step = -step;
-        if (more) feed.deliver(p, k_place(t + 1), v_place(t + 1), tid);
-        feed.arrived();
+        workgroup_barrier();
+        for (int x = tid; x < kTile / 8; x += kCtxThreads) {
+            u32x4* piece = reinterpret_cast<u32x4*>(V) + x;
+            *piece = only_finite<T>(*piece);
+        }
         workgroup_barrier();
     };
-    // (the tiles that all rows see as a whole have a loop without masks)
-    const int free = min(whole / kCtxTile, nt);
-    int t = t0;
-    for (; t < free; ++t) tile(t, std::false_type{});
-    for (; t < nt; ++t) tile(t, std::true_type{});
+    // the tiles that all rows see as a whole have a loop without masks
+    const int free = max(min(whole / kCtxTile, nt), t0);
+    const auto walk = [&](auto&& tile) {
+        int t = t0;
+        for (; t < free; ++t) tile(t, std::false_type{});
+        for (; t < nt; ++t) tile(t, std::true_type{});
+    };
+    if constexpr (kAhead) {
+        // K runs a tile ahead of V, so that the scores of the next tile are made beside the exponentials of this one.
+        if (nt) {
+            feed.request_k(p, 0, n, k_place(0), wave);
+            feed.request_v(p, 0, n, v_place(0), wave);
+            if (nt > 1) feed.request_k(p, 1, n, k_place(1), wave);
+        }
+        feed.arrived();
+        workgroup_barrier();
+        f32x16 s[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) s[u] = at.template scores<T>(u * kHalf, own);
+        workgroup_barrier();
+        walk([&](int t, auto masked) {
+            if (t + 1 < nt) feed.request_v(p, t + 1, n, v_place(t + 1), wave);
+            if (t + 2 < nt) feed.request_k(p, t + 2, n, k_place(t), wave);
+            if (decltype(masked)::value && p.causal) care(t);
+            at.move(step);
+            if (t * kCtxTile < n_wave) {
+                st.template raise<decltype(masked)::value>(s, p.c, limit - t * kCtxTile, h);
+                f32x16 next[2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) next[u] = at.template scores<T>(u * kHalf, own);
+                st.exponentials(s, p.c);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    at.template add_columns<T>(st.acc, kV - step + u * kHalf, s[u]);
+                    s[u] = next[u];
+                }
+            }
+            step = -step;
+            feed.arrived();
+            workgroup_barrier();
+        });
+    } else {
+        if (t0 < nt) {
+            feed.look(p, t0, n);
+            feed.request(p, t0, n, k_place(t0), v_place(t0), wave);
+            if (t0 + 1 < nt) feed.look(p, t0 + 1, n);
+            feed.deliver(p, k_place(t0), v_place(t0), tid);
+        }
+        feed.arrived();
+        workgroup_barrier();
+        walk([&](int t, auto masked) {
+            const bool more = t + 1 < nt;
+            if (more) {
+                feed.request(p, t + 1, n, k_place(t + 1), v_place(t + 1), wave);
+                if (t + 2 < nt) feed.look(p, t + 2, n);
+            }
+            if (decltype(masked)::value && p.causal) care(t);
+            if (t * kCtxTile < n_wave) {
+                f32x16 s[2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) s[u] = at.template scores<T>(u * kHalf, own);
+                st.template take<decltype(masked)::value>(s, p.c, limit - t * kCtxTile, h);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) at.template add_columns<T>(st.acc, kV + u * kHalf, s[u]);
+            }
+            at.move(step);
+            step = -step;
+            if (more) feed.deliver(p, k_place(t + 1), v_place(t + 1), tid);
+            feed.arrived();
+            workgroup_barrier();
+        });
     }
     const float both = halves_sum(st.l), l = limit > 0 ? both : 0.0f, f = l == 0.0f ? 0.0f : 1.0f / l;
     if (p.lse && h == 0 && ok)
@@ -306,6 +311,24 @@ __global__ __launch_bounds__(64 * WAVES, NC == 1 ? (E4M3 || HD <= 96 ? 4 : 3) : 
             if (t + 2 * WAVES < part.end) look(t + 2 * WAVES);
         }
         const bool masked = 32 * t + 32 > whole;
+        if (masked && whole < n) {
+            wave_exchange();
+            bool some = false;
+            for (int x = lane; x < 32 * CH; x += 64) some = some || any_not_finite<T>(*reinterpret_cast<const u32x4*>(V + x / CH * kLd + 8 * (x % CH)));
+            if (__builtin_amdgcn_ballot_w64(some)) {
+                for (int j = 0; j < 32; ++j)
+#pragma unroll
+                    for (int i = 0; i < NC; ++i)
+                        if (32 * t + j < limit[i])
+#pragma unroll
+                            for (int d = 0; d < DT; ++d) acc[i][d] += only_not_finite<T>(V + j * kLd + 16 * d + 4 * g);
+                wave_exchange();
+                for (int x = lane; x < 32 * CH; x += 64) {
+                    u32x4* piece = reinterpret_cast<u32x4*>(V + x / CH * kLd + 8 * (x % CH));
+                    *piece = only_finite<T>(*piece);
+                }
+            }
+        }
         u32x4 pr[NC];
 #pragma unroll
         for (int i = 0; i < NC; ++i) {

@@ -117,6 +117,29 @@ def test_rows_of_nobody_are_not_used(bad):
     check(run(x, offsets, True), clean, offsets, True)
 
 
+@pytest.mark.parametrize("D,G", [(64, 1), (128, 2), (48, 4), (96, 1), (20, 2)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_numbers_that_a_row_does_not_see(D, G, bad):
+    """Tokens with infinities or NaN among their numbers do not reach the tokens in front of them (but for the last bits: rows of a wave raise
+    their maxima together)."""
+    from semicat_amd import packed_attention
+    offsets, hurt = offsets_of([70, 1, 300, 129]), {0: 33, 2: 130, 3: 128}  # (sequence: its first such token)
+    x = make(offsets[-1], 4, G, D, BF16)
+    at = torch.tensor(offsets, dtype=torch.int32, device="cuda")
+    want, sizes = orc.packed(x["q"], x["k"], x["v"], offsets, True)
+    limit = orc.limit(want["o"], sizes["o"], BF16)
+    for b, i in hurt.items():
+        x["v"][offsets[b] + i, :, 3], x["v"][offsets[b + 1] - 1] = bad, bad
+        x["k"][offsets[b] + i, :, 1] = bad
+        x["q"][offsets[b] + i, 0] = bad
+    got = packed_attention(*(x[n].cuda() for n in "qkv"), at).cpu()
+    off = (got.double() - want["o"]).abs()
+    for b, (s, e) in enumerate(zip(offsets, offsets[1:])):
+        i = s + hurt.get(b, e - s)
+        assert bool((off[s:i] <= limit[s:i]).all()), b
+        assert not got[i:e].isfinite().all(-1).any(), b
+
+
 def test_neighbours_do_not_mix():
     """NaN in one sequence stays there."""
     offsets = offsets_of([40, 50, 60])

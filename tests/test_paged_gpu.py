@@ -261,6 +261,43 @@ def test_numbers_of_nobody_are_not_used(quantized):
     assert torch.equal(attend(cache, q, tables, held, None), want)
 
 
+@pytest.mark.parametrize("quantized", [True, False])
+@pytest.mark.parametrize("new,held", [([5, 1, 3], [40, 33, 70]), ([300, 17, 200], [900, 17, 1400]), ([90] * 30, [100 + 20 * i for i in range(30)])])
+def test_numbers_that_a_token_does_not_see(new, held, quantized):
+    """The last token's keys and values are not finite: only its own output is not."""
+    size, H, D = 16, 8, 64
+    pages = sum(-(-n // size) for n in held) + 1
+    cache = cache_of(pages, size, 4, D, BF16, quantized)
+    tables = tables_of(held, size, pages)
+    offsets = offsets_of(new)
+    q = normal(sum(new), H, D, dtype=BF16)
+    want, sizes = orc.paged(q, held_rows(cache, tables, held, "k"), held_rows(cache, tables, held, "v"), held, offsets)
+    bad = torch.tensor([float("nan")], dtype=BF16).view(torch.uint8) if not quantized else torch.tensor([127], dtype=torch.uint8)
+    for b, n in enumerate(held):
+        page, row = int(tables[b, (n - 1) // size]), (n - 1) % size
+        for t in (cache.k, cache.v):
+            t.view(torch.uint8)[page, :, row] = bad.repeat(D).cuda()
+    got = attend(cache, q, tables, held, offsets)
+    last = torch.zeros(sum(new), dtype=torch.bool)
+    last[torch.tensor(offsets[1:]) - 1] = True
+    off = (got.double() - want).abs()
+    assert bool((off <= orc.limit(want, sizes, BF16))[~last].all()) and got[last].isnan().all()
+
+
+def test_rows_of_nobody_beside_many():
+    """Rows outside the sequences are zeros whichever launch they fall to."""
+    new, held = [300] * 12 + [3], [400] * 13
+    cache = cache_of(13 * 25 + 1, 16, 4, 64, BF16, True)
+    tables = tables_of(held, 16, 13 * 25 + 1)
+    for front, behind in ((1, 2), (200, 300)):
+        offsets = [n + front for n in offsets_of(new)]
+        q = normal(offsets[-1] + behind, 16, 64, dtype=BF16)
+        got = attend(cache, q, tables, held, offsets)
+        assert not got[:front].any() and not got[-behind:].any()
+        inner = attend(cache, q[front:-behind], tables, held, offsets_of(new))
+        assert torch.equal(got[front:-behind], inner)
+
+
 def test_places_in_memory():
     """A cache in slices of a caller's tensors, tensors of any stride, a table that is a slice of a larger one."""
     from semicat_amd import PagedCache, paged_attention, paged_write
