@@ -9,7 +9,8 @@ namespace {
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-constexpr int64_t kMostThreads = UINT32_MAX;  // of a launch
+// a launch has fewer than 2^32 threads
+int seq_grid(int64_t blocks, int threads) { return blocks > UINT32_MAX / threads ? SJVP_ERR_SHAPE : SJVP_OK; }
 
 bool strides_ok(const CtxView& v, int rows) { return rows <= 1 || (v.sl >= 0 && v.sl < 1 << 24); }
 
@@ -21,8 +22,22 @@ int seq_common(SeqParams& p, int B, int T, int Hq, int Hkv, int D, float scale) 
     p.B = B, p.T = T, p.Hq = Hq, p.Hkv = Hkv, p.G = Hq / Hkv, p.D = D;
     p.scale = scale == 0.0f ? 1.0f / std::sqrt(static_cast<float>(D)) : scale;
     p.c = p.scale * kLog2e;
-    // blocks of 16 rows of all heads, 256 threads each (splits are made of launches of few blocks alone)
-    return seq_slots(p, p.G, 16) * Hkv > kMostThreads / 256 ? SJVP_ERR_SHAPE : SJVP_OK;
+    return SJVP_OK;
+}
+
+// The backward of whole sequences: the column-owned launch is split over the heads that share a key head.
+struct PackedPlan {
+    int splits = 1;
+    size_t part = 0, total = 0;  // floats
+};
+
+PackedPlan packed_plan(const SeqParams& p) {
+    PackedPlan plan;
+    const int64_t blocks = (p.T / kCtxOwned + 1) * (int64_t)p.Hkv;
+    plan.splits = (int)std::max<int64_t>(1, std::min<int64_t>(4 * (int64_t)compute_units() / blocks, p.G));
+    plan.part = (3 * (size_t)p.Hq * p.T + 3) / 4 * 4;
+    plan.total = plan.part + (plan.splits > 1 ? 2 * (size_t)plan.splits * p.Hkv * p.T * ctx_padded(p.D) : 0);
+    return plan;
 }
 
 int packed_params(const sjvp_packed* t, SeqParams& p) {
@@ -37,7 +52,8 @@ int packed_params(const sjvp_packed* t, SeqParams& p) {
         if (t->T == 1) v->sl = t->D;  // (one row: no stride)
     }
     p.lse = t->lse, p.offsets = t->offsets, p.causal = t->causal != 0;
-    return SJVP_OK;
+    if (seq_grid(seq_slots(p, p.G, kCtxOwned) * p.Hkv, kCtxThreads) != SJVP_OK) return SJVP_ERR_SHAPE;
+    return seq_grid(seq_slots(p, 1, kCtxOwned) * p.Hkv * packed_plan(p).splits, 2 * kCtxThreads);
 }
 
 int paged_params(const sjvp_paged* t, SeqParams& p, int T) {
@@ -102,19 +118,10 @@ PagedPlan paged_plan(const SeqParams& p) {
     return plan;
 }
 
-// The backward of whole sequences: the column-owned launch is split over the heads that share a key head.
-struct PackedPlan {
-    int splits = 1;
-    size_t part = 0, total = 0;  // floats
-};
-
-PackedPlan packed_plan(const SeqParams& p) {
-    PackedPlan plan;
-    const int64_t blocks = (p.T / kCtxOwned + 1) * (int64_t)p.Hkv;
-    plan.splits = (int)std::max<int64_t>(1, std::min<int64_t>(4 * (int64_t)compute_units() / blocks, p.G));
-    plan.part = (3 * (size_t)p.Hq * p.T + 3) / 4 * 4;
-    plan.total = plan.part + (plan.splits > 1 ? 2 * (size_t)plan.splits * p.Hkv * p.T * ctx_padded(p.D) : 0);
-    return plan;
+// (splits are made of launches of few blocks alone, so that those of one split are the most)
+int attention_params(const sjvp_paged* t, SeqParams& p) {
+    const int rc = paged_params(t, p, t->T);
+    return rc != SJVP_OK ? rc : seq_grid(seq_slots(p, p.G, 16 * seq_sets(p)) * p.Hkv, kCtxThreads);
 }
 
 int seq_workspace(void* ws, size_t bytes, size_t floats) {
@@ -158,7 +165,7 @@ int sjvp_packed_bwd(const sjvp_packed* t, int dtype, void* stream) {
 
 size_t sjvp_paged_workspace_bytes(const sjvp_paged* t) {
     SeqParams p{};
-    return t && paged_params(t, p, t->T) == SJVP_OK ? 4 * paged_plan(p).total : 0;
+    return t && attention_params(t, p) == SJVP_OK ? 4 * paged_plan(p).total : 0;
 }
 
 int sjvp_paged_write(const sjvp_paged* t, int dtype, void* stream) {
@@ -167,6 +174,7 @@ int sjvp_paged_write(const sjvp_paged* t, int dtype, void* stream) {
     if (rc != SJVP_OK) return rc;
     if (dtype != SJVP_BF16 && dtype != SJVP_FP16) return SJVP_ERR_DTYPE;
     if (!t->k || !t->v || (!t->offsets && t->T != t->B)) return SJVP_ERR_NULL;
+    if (seq_grid(t->T, 64) != SJVP_OK) return SJVP_ERR_SHAPE;  // (a wave to a token)
     return paged_copy(p, p.pages.ks, dtype == SJVP_FP16, true, static_cast<hipStream_t>(stream));
 }
 
@@ -176,14 +184,14 @@ int sjvp_paged_read(const sjvp_paged* t, int dtype, void* stream) {
     if (rc != SJVP_OK) return rc;
     if (dtype != SJVP_BF16 && dtype != SJVP_FP16) return SJVP_ERR_DTYPE;
     if (!t->k || !t->v) return SJVP_ERR_NULL;
-    if (t->size < 1 || t->size > kCtxMost || (int64_t)t->B * t->size > kMostThreads / 64 - kCtxWaves) return SJVP_ERR_SHAPE;
+    if (t->size < 1 || t->size > kCtxMost || seq_grid((int64_t)t->B * t->size, 64) != SJVP_OK) return SJVP_ERR_SHAPE;
     p.most = t->size;
     return paged_copy(p, p.pages.ks, dtype == SJVP_FP16, false, static_cast<hipStream_t>(stream));
 }
 
 int sjvp_paged_attention(const sjvp_paged* t, int dtype, void* stream) {
     SeqParams p{};
-    const int rc = t ? paged_params(t, p, t->T) : SJVP_ERR_NULL;
+    const int rc = t ? attention_params(t, p) : SJVP_ERR_NULL;
     if (rc != SJVP_OK) return rc;
     if (dtype != SJVP_BF16 && dtype != SJVP_FP16) return SJVP_ERR_DTYPE;
     if (!t->q || !t->o || (!t->offsets && t->T != t->B)) return SJVP_ERR_NULL;

@@ -196,6 +196,35 @@ __device__ __forceinline__ void reads_ahead() {
     for (int i = 0; i < AHEAD; ++i) __builtin_amdgcn_sched_group_barrier(0x008, MFMAS, 0);
 }
 
+// Infinities and NaN in rows that a causal query (or key) does not see: a contraction makes NaN of them by a probability of zero, for every query
+// of the tile.  Tiles that some queries see in part are looked at before they are used; such numbers are added one by one to what sees
+// them, and taken out of the tile.  The backward finds them in the scores, the forward, whose values no score has met, in LDS.
+template <typename T> constexpr uint32_t kExponents = std::is_same_v<T, Bf16> ? 0x7f807f80u : 0x7c007c00u;
+// bits 15 and 31: whether the numbers of a pair are not finite
+template <typename T>
+__device__ __forceinline__ uint32_t not_finite(uint32_t pair) {
+    return ((pair & kExponents<T>) + (std::is_same_v<T, Bf16> ? 0x00800080u : 0x04000400u)) & 0x80008000u;
+}
+template <typename T>
+__device__ __forceinline__ bool any_not_finite(u32x4 x) {
+    return (not_finite<T>(x[0]) | not_finite<T>(x[1]) | not_finite<T>(x[2]) | not_finite<T>(x[3])) != 0;
+}
+template <typename T>
+__device__ __forceinline__ u32x4 only_finite(u32x4 x) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] &= ~((not_finite<T>(x[i]) >> 15) * 0xffffu);
+    return x;
+}
+// What is not finite of four numbers in LDS.  (Behind a wall, so that it takes few registers.)
+template <typename T>
+__device__ __forceinline__ f32x4 only_not_finite(const elem_t* from) {
+    u32x2 x = *reinterpret_cast<const u32x2*>(from);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) x[i] &= (not_finite<T>(x[i]) >> 15) * 0xffffu;
+    asm volatile("" ::: "memory");
+    return f32x4{T::to_float((elem_t)x[0]), T::to_float((elem_t)(x[0] >> 16)), T::to_float((elem_t)x[1]), T::to_float((elem_t)(x[1] >> 16))};
+}
+
 // A tile of 64 looped rows in LDS, and where this lane reads its operands (tile algebra: sjvp_ctx.hpp).  Rows are unpadded (D in 65 to 96 have rows
 // of 128 columns) and the 16-byte pieces of a row are permuted by it, for both kinds of reads.  LDS serves 256 bytes a cycle: 16 lanes of a
 // row-major read, so 16 neighbouring rows have to be in different places; and 32 lanes of a transposing read, which are four neighbouring rows of 64 bytes,
@@ -336,8 +365,6 @@ struct SeqFeed {
     __device__ __forceinline__ void request_v(const SeqParams& p, int t, int keys, elem_t* vp, int wave) {
         vf.request(v + (int64_t)t * kCtxTile * p.v.sl, p.v.sl, keys - t * kCtxTile, p.D, vp, wave);
     }
-    __device__ __forceinline__ void deliver_k(const SeqParams& p, elem_t* kp, int tid) { kf.deliver(kp, p.D, tid); }
-    __device__ __forceinline__ void deliver_v(const SeqParams& p, elem_t* vp, int tid) { vf.deliver(vp, p.D, tid); }
     __device__ __forceinline__ void arrived() { kf.arrived(); }
 };
 
@@ -456,7 +483,7 @@ struct SeqSums {
         if (__builtin_amdgcn_ballot_w64(top > m + 8.0f)) {
             const float grown = fmaxf(m, halves_max(top));
             const float now = grown == -INFINITY ? 0.0f : grown;
-            const float f = m == -INFINITY ? 0.0f : fast_exp2(ref - now);
+            const float f = m == -INFINITY ? 1.0f : fast_exp2(ref - now);  // (no sums yet but infinities, of the careful tiles)
             m = grown, ref = now;
             l *= f;
 #pragma unroll
@@ -482,33 +509,32 @@ struct SeqSums {
     }
 };
 
-// Infinities and NaN in values that a causal row does not see: a contraction makes NaN of them by a probability of zero, for every row of the tile.
-// Tiles that some rows see in part are looked at before they are used; such numbers are added to the rows that see them one by one, and
-// taken out of the tile.
-template <typename T> constexpr uint32_t kExponents = std::is_same_v<T, Bf16> ? 0x7f807f80u : 0x7c007c00u;
-// bits 15 and 31: whether the numbers of a pair are not finite
-template <typename T>
-__device__ __forceinline__ uint32_t not_finite(uint32_t pair) {
-    return ((pair & kExponents<T>) + (std::is_same_v<T, Bf16> ? 0x00800080u : 0x04000400u)) & 0x80008000u;
+// Of a tile of 64 rows: whether some of this thread's pieces are not finite; out += factor times what is not finite of the rows [first, end); the finite
+// numbers alone.
+template <typename T, int HD, int NT>
+__device__ __forceinline__ bool tile_not_finite(const elem_t* tile, int tid) {
+    bool some = false;
+    for (int x = tid; x < SeqTile<HD>::kElems / 8; x += NT) some = some || any_not_finite<T>(reinterpret_cast<const u32x4*>(tile)[x]);
+    return some;
 }
-template <typename T>
-__device__ __forceinline__ bool any_not_finite(u32x4 x) {
-    return (not_finite<T>(x[0]) | not_finite<T>(x[1]) | not_finite<T>(x[2]) | not_finite<T>(x[3])) != 0;
-}
-template <typename T>
-__device__ __forceinline__ u32x4 only_finite(u32x4 x) {
+template <typename T, int HD>
+__device__ __forceinline__ void add_not_finite(f32x16* out, const elem_t* tile, int first, int end, float factor, int h) {
+    for (int j = first; j < end; ++j) {
+        const elem_t* from = tile + j * SeqTile<HD>::kLd + 4 * h;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] &= ~((not_finite<T>(x[i]) >> 15) * 0xffffu);
-    return x;
-}
-// What is not finite of four numbers in LDS.  (Behind a wall, so that it takes few registers.)
-template <typename T>
-__device__ __forceinline__ f32x4 only_not_finite(const elem_t* from) {
-    u32x2 x = *reinterpret_cast<const u32x2*>(from);
+        for (int c = 0; c < HD / 8; ++c) {
+            const f32x4 more = only_not_finite<T>(from + 8 * (c ^ SeqTile<HD>::swz(j)));
 #pragma unroll
-    for (int i = 0; i < 2; ++i) x[i] &= (not_finite<T>(x[i]) >> 15) * 0xffffu;
-    asm volatile("" ::: "memory");
-    return f32x4{T::to_float((elem_t)x[0]), T::to_float((elem_t)(x[0] >> 16)), T::to_float((elem_t)x[1]), T::to_float((elem_t)(x[1] >> 16))};
+            for (int i = 0; i < 4; ++i) out[c / 4][4 * (c % 4) + i] = __builtin_fmaf(factor, more[i], out[c / 4][4 * (c % 4) + i]);
+        }
+    }
+}
+template <typename T, int HD, int NT>
+__device__ __forceinline__ void keep_finite(elem_t* tile, int tid) {
+    for (int x = tid; x < SeqTile<HD>::kElems / 8; x += NT) {
+        u32x4* piece = reinterpret_cast<u32x4*>(tile) + x;
+        *piece = only_finite<T>(*piece);
+    }
 }
 
 // Sums of a wave's own 32 rows, OUT^T, as rows in memory whose places `at` gives, through the wave's own LDS region of [32][HD + 8].

@@ -22,6 +22,22 @@ __device__ __forceinline__ f32x16 seq_of_rows(const float* rows, int h) {
     return x;
 }
 
+// Whether one of a wave's scores is not finite.
+__device__ __forceinline__ bool some_not_finite(const f32x16& a, const f32x16& b) {
+    float zero = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) zero = __builtin_fmaf(a[r], 0.0f, __builtin_fmaf(b[r], 0.0f, zero));
+    return __builtin_amdgcn_ballot_w64(zero != 0.0f) != 0;
+}
+
+// Whether some wave says so, in the x-th tile, behind whose contractions is a barrier.  (One that leaves copies to LDS in flight, unlike a barrier
+// with a reduction.)
+__device__ __forceinline__ bool some_wave(int* last, int x, bool some, int lane) {
+    if (some && lane == 0) *last = x + 1;
+    workgroup_barrier();
+    return __builtin_amdgcn_readfirstlane(*last) == x + 1;
+}
+
 // Row-owned: four waves of 32 query rows (of the heads that share a key head) share tiles of 64 keys.
 template <typename T, int HD, bool DMA>
 __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 3 : 2) void seq_bwd_row(SeqParams p) {
@@ -29,6 +45,7 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 3 : 2) void seq_bwd_row(Seq
     extern __shared__ __align__(16) unsigned char smem[];
     constexpr int kTile = SeqTile<HD>::kElems;
     elem_t* tiles = reinterpret_cast<elem_t*>(smem);  // K [2], V [2]
+    __shared__ int hurt;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
     const int hk = blockIdx.x % p.Hkv;
     const SeqBlock b = seq_block_long_first<kCtxOwned>(p, blockIdx.x / p.Hkv, p.G, false, lane);
@@ -48,6 +65,7 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 3 : 2) void seq_bwd_row(Seq
     const auto k_place = [&](int t) { return tiles + (t & 1) * kTile; };
     const auto v_place = [&](int t) { return tiles + (2 + (t & 1)) * kTile; };
     if (nt) feed.request(p, 0, n, k_place(0), v_place(0), wave);
+    if (tid == 0) hurt = 0;
 
     const int64_t token = b.token + mine.token, stat = (int64_t)mine.hq * p.T + token;
     const f32x2 ml = ok && limit > 0 ? *reinterpret_cast<const f32x2*>(p.lse + 2 * stat) : f32x2{0.0f, 0.0f};
@@ -105,9 +123,10 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 3 : 2) void seq_bwd_row(Seq
         const int key = t * kCtxTile;
         const bool more = t + 1 < nt;
         if (more) feed.request(p, t + 1, n, k_place(t + 1), v_place(t + 1), wave);
+        f32x16 s[2], ds[2];
+        s[0] = s[1] = ds[0] = ds[1] = f32x16{};
+        bool some = false;
         if (key < n_wave) {
-            f32x16 s[2], ds[2];
-            s[0] = s[1] = ds[0] = ds[1] = f32x16{};
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -116,6 +135,7 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 3 : 2) void seq_bwd_row(Seq
                     ds[u] = Mma32<T>::run(at.rows(2 * kBytes + u * kHalf, c), own_g[c], ds[u]);
                 }
             reads_ahead<HD / 8, 2, 2, 2>();
+            if constexpr (decltype(masked)::value) some = some_not_finite(s[0], s[1]);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
 #pragma unroll
@@ -124,8 +144,20 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 3 : 2) void seq_bwd_row(Seq
                     if constexpr (decltype(masked)::value)
                         if (32 * u + tile_row(r, 0) >= limit - key - 4 * h) ds[u][r] = 0.0f;
                 }
-                at.template add_columns<T>(acc, u * kHalf, ds[u]);
+                if constexpr (!decltype(masked)::value) at.template add_columns<T>(acc, u * kHalf, ds[u]);
             }
+        }
+        if constexpr (decltype(masked)::value) {
+            // (a hidden row of V has ended in a zero of dS, one of K would meet that zero in the contraction)
+            if (p.causal && some_wave(&hurt, t, some, lane)) {
+                add_not_finite<T, HD>(acc, k_place(t), 0, min(limit - key, kCtxTile), 0.0f, h);
+                workgroup_barrier();
+                keep_finite<T, HD, kCtxThreads>(k_place(t), tid);
+                workgroup_barrier();
+            }
+            if (key < n_wave)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) at.template add_columns<T>(acc, u * kHalf, ds[u]);
         }
         at.move(step);
         step = -step;
@@ -201,6 +233,17 @@ __device__ __forceinline__ void col_probabilities(f32x16& s, f32x16& ds, const f
     }
 }
 
+// What is not finite of a tile of Q and dO: of the rows [first, end) to this lane's key, and out of the tile.
+template <typename T, int HD, int NT>
+__device__ __forceinline__ void col_care(f32x16* dk, f32x16* dv, elem_t* tile, int first, int end, int tid, int h) {
+    add_not_finite<T, HD>(dk, tile, first, end, 0.0f, h);
+    add_not_finite<T, HD>(dv, tile + SeqTile<HD>::kElems, first, end, 1.0f, h);
+    workgroup_barrier();
+    keep_finite<T, HD, NT>(tile, tid);
+    keep_finite<T, HD, NT>(tile + SeqTile<HD>::kElems, tid);
+    workgroup_barrier();
+}
+
 // dK or dV of a wave's 32 keys to where they go: the result, or a split's sums.
 template <typename T, int HD>
 __device__ __forceinline__ void store_col(const SeqParams& p, const SeqCols& w, f32x16* sum, bool some, float factor, const CtxView& out, int which, int k0,
@@ -223,6 +266,7 @@ __global__ __launch_bounds__(kCtxThreads, 2) void seq_bwd_col(SeqParams p) {
     constexpr int kTile = SeqTile<HD>::kElems, kHalf = 32 * SeqTile<HD>::kLd * 2, kBytes = SeqTile<HD>::kBytes;
     elem_t* tiles = reinterpret_cast<elem_t*>(smem);             // [2][Q, dO]
     float* stats = reinterpret_cast<float*>(tiles + 4 * kTile);  // [2][row_stat_folded, -delta][64]
+    __shared__ int hurt;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
     const SeqCols w(p, lane);
     if (!w.b.some) return;
@@ -242,6 +286,7 @@ __global__ __launch_bounds__(kCtxThreads, 2) void seq_bwd_col(SeqParams p) {
     }
     f32x16 dk[HD / 32] = {}, dv[HD / 32] = {};
     int step = 2 * kBytes;
+    if (tid == 0) hurt = 0;
     // x: tiles before this one; hq, t: the head and the tile of its rows
     const auto tile = [&](int x, int hq, int t, auto masked) {
         const int r0 = t * kCtxTile;
@@ -250,23 +295,31 @@ __global__ __launch_bounds__(kCtxThreads, 2) void seq_bwd_col(SeqParams p) {
             const bool last = t + 1 == w.tb;
             feed.request(p, w.b, last ? hq + 1 : hq, (last ? w.ta : t + 1) * kCtxTile, place(x + 1), tid, wave);
         }
-        if (k0 < keys && !(decltype(masked)::value && r0 + kCtxTile <= k0)) {
+        const bool used = k0 < keys && !(decltype(masked)::value && r0 + kCtxTile <= k0);
+        f32x16 s[2], ds[2];
+        bool some = false;
+        if (used) {
             const float* st = st_place(x);
             const bool factors = __builtin_amdgcn_ballot_w64(st[kCtxTile + lane] != 1.0f);
-            f32x16 s[2], ds[2];
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 s[u] = at.template scores<T>(u * kHalf, own_k);
                 ds[u] = at.template scores<T>(kBytes + u * kHalf, own_v, seq_of_rows(st + 2 * kCtxTile + 32 * u, h));
             }
+            if constexpr (decltype(masked)::value) some = some_not_finite(s[0], s[1]) || some_not_finite(ds[0], ds[1]);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                col_probabilities<decltype(masked)::value, false>(s[u], ds[u], st + 32 * u, p.c, key - r0 - 32 * u, h);
-                if (factors) {
+                constexpr bool kMasked = decltype(masked)::value;  // (factors may be NaN: ahead of the mask)
+                col_probabilities<kMasked, kMasked>(s[u], ds[u], st + 32 * u, p.c, key - r0 - 32 * u, h);
+                if (!kMasked && factors) {
                     const f32x16 factor = seq_of_rows(st + kCtxTile + 32 * u, h);
                     s[u] *= factor, ds[u] *= factor;
                 }
             }
+        }
+        if constexpr (decltype(masked)::value)
+            if (some_wave(&hurt, x, some, lane)) col_care<T, HD, kCtxThreads>(dk, dv, place(x), max(key - r0, 0), kCtxTile, tid, h);
+        if (used) {
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 at.template add_columns<T>(dv, kBytes + u * kHalf, s[u]);
@@ -302,6 +355,7 @@ __global__ __launch_bounds__(2 * kCtxThreads, 2) void seq_bwd_col_pair(SeqParams
     elem_t* tiles = reinterpret_cast<elem_t*>(smem);             // [2][Q, dO]
     elem_t* mine = tiles + 4 * kTile;                            // K [2], V [2]
     float* stats = reinterpret_cast<float*>(mine + 4 * kTile);   // [2][row_stat_folded, -delta][64]
+    __shared__ int hurt;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
     const int group = wave % kCtxWaves, half = wave / kCtxWaves;
     const SeqCols w(p, lane);
@@ -331,6 +385,7 @@ __global__ __launch_bounds__(2 * kCtxThreads, 2) void seq_bwd_col_pair(SeqParams
     for (int c = 0; c < HD / 16; ++c) own[c] = at.row[c] - half * kHalf + 4 * kBytes + group * kHalf;
     f32x16 dk[HD / 32] = {}, dv[HD / 32] = {};
     int step = 2 * kBytes;
+    if (tid == 0) hurt = 0;
     const auto tile = [&](int x, int hq, int t, auto masked) {
         const int r0 = t * kCtxTile + 32 * half;  // the wave's rows
         const bool more = x + 1 < w.tiles;
@@ -338,9 +393,12 @@ __global__ __launch_bounds__(2 * kCtxThreads, 2) void seq_bwd_col_pair(SeqParams
             const bool last = t + 1 == w.tb;
             feed.request(p, w.b, last ? hq + 1 : hq, (last ? w.ta : t + 1) * kCtxTile, place(x + 1), tid, wave);
         }
-        if (k0 < keys && !(decltype(masked)::value && r0 + 32 <= k0)) {
+        const bool used = k0 < keys && !(decltype(masked)::value && r0 + 32 <= k0);
+        f32x16 s = {}, ds;
+        bool some = false;
+        if (used) {
             const float* st = st_place(x) + 32 * half;
-            f32x16 s = {}, ds = seq_of_rows(st + 2 * kCtxTile, h);
+            ds = seq_of_rows(st + 2 * kCtxTile, h);
 #pragma unroll
             for (int c = 0; c < HD / 16; ++c) {
                 s = Mma32<T>::run(at.rows(0, c), *SeqTile<HD>::template at<const u32x4>(own[c]), s);
@@ -349,7 +407,12 @@ __global__ __launch_bounds__(2 * kCtxThreads, 2) void seq_bwd_col_pair(SeqParams
             __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);  // (-delta)
             reads_ahead<HD / 16, 4, 2, 1>();
             __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);  // (the other statistics)
+            if constexpr (decltype(masked)::value) some = some_not_finite(s, ds);
             col_probabilities<decltype(masked)::value, true>(s, ds, st, p.c, key - r0, h);
+        }
+        if constexpr (decltype(masked)::value)
+            if (some_wave(&hurt, x, some, lane)) col_care<T, HD, NT>(dk, dv, place(x), max(key - t * kCtxTile, 32 * half), 32 * half + 32, tid, h);
+        if (used) {
             at.template add_columns<T>(dv, kBytes, s);
             at.template add_columns<T>(dk, 0, ds);
             reads_ahead<HD / 8, 2, 1, 2>();

@@ -67,23 +67,10 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 4 : 2) void seq_fwd(SeqPara
     // tile t's values that are not finite
     const auto care = [&](int t) {
         elem_t* V = v_place(t);
-        bool some = false;
-        for (int x = tid; x < kTile / 8; x += kCtxThreads) some = some || any_not_finite<T>(reinterpret_cast<const u32x4*>(V)[x]);
-        if (!workgroup_barrier_or(some)) return;
-        for (int j = 0; j < min(limit - t * kCtxTile, kCtxTile); ++j) {
-            const elem_t* from = V + j * SeqTile<HD>::kLd + 4 * h;
-#pragma unroll
-            for (int c = 0; c < HD / 8; ++c) {
-                const f32x4 more = only_not_finite<T>(from + 8 * (c ^ SeqTile<HD>::swz(j)));
-#pragma unroll
-                for (int i = 0; i < 4; ++i) st.acc[c / 4][4 * (c % 4) + i] += more[i];
-            }
-        }
+        if (!workgroup_barrier_or(tile_not_finite<T, HD, kCtxThreads>(V, tid))) return;
+        add_not_finite<T, HD>(st.acc, V, 0, min(limit - t * kCtxTile, kCtxTile), 1.0f, h);
         workgroup_barrier();
-        for (int x = tid; x < kTile / 8; x += kCtxThreads) {
-            u32x4* piece = reinterpret_cast<u32x4*>(V) + x;
-            *piece = only_finite<T>(*piece);
-        }
+        keep_finite<T, HD, kCtxThreads>(V, tid);
         workgroup_barrier();
     };
     // the tiles that all rows see as a whole have a loop without masks
@@ -345,7 +332,7 @@ __global__ __launch_bounds__(64 * WAVES, NC == 1 ? (E4M3 || HD <= 96 ? 4 : 3) : 
             top *= p.c;
             if (__builtin_amdgcn_ballot_w64(top > m[i] + 8.0f)) {
                 const float grown = fmaxf(m[i], quarters_max(top)), now = grown == -INFINITY ? 0.0f : grown;
-                const float f = m[i] == -INFINITY ? 0.0f : fast_exp2(ref[i] - now);
+                const float f = m[i] == -INFINITY ? 1.0f : fast_exp2(ref[i] - now);
                 m[i] = grown, ref[i] = now;
                 l[i] *= f;
 #pragma unroll

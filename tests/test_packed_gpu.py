@@ -140,6 +140,40 @@ def test_numbers_that_a_row_does_not_see(D, G, bad):
         assert not got[i:e].isfinite().all(-1).any(), b
 
 
+@pytest.mark.parametrize("D,G", [(64, 1), (128, 2), (48, 4), (96, 1), (20, 2), (128, 8)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_gradients_of_numbers_that_a_row_does_not_see(D, G, bad):
+    """Infinities and NaN of a key or value do not reach the gradients of queries in front of it, those of a query or of its
+    result's gradient not the keys behind it."""
+    from semicat_amd import packed_attention
+    offsets = offsets_of([70, 200, 300, 129, 260])
+    hurt_keys, hurt_rows = {0: 33, 2: 130, 3: 128}, {1: 70, 4: 128}  # (sequence: the token)
+    x = make(offsets[-1], 8, G, D, BF16)
+    at = torch.tensor(offsets, dtype=torch.int32, device="cuda")
+    want, sizes = orc.packed(x["q"], x["k"], x["v"], offsets, True, x["dO"])
+    for b, i in hurt_keys.items():
+        x["k"][offsets[b] + i, :, 5] = bad
+        x["v"][offsets[b] + i, :, 3], x["v"][offsets[b + 1] - 1] = bad, bad
+    for b, i in hurt_rows.items():
+        x["q"][offsets[b] + i, :, 7], x["dO"][offsets[b] + i, :, 9] = bad, bad
+    leaves = [x[n].cuda().requires_grad_() for n in "qkv"]
+    grads = torch.autograd.grad(packed_attention(*leaves, at), leaves, x["dO"].cuda())
+    for name, t in zip(("dq", "dk", "dv"), grads):
+        off, limit = (t.cpu().double() - want[name]).abs(), orc.limit(want[name], sizes[name], BF16)
+        for b, (s, e) in enumerate(zip(offsets, offsets[1:])):
+            clean = torch.arange(s, e)
+            if b in hurt_keys:
+                i = s + hurt_keys[b]
+                clean, rest = clean[:i - s if name == "dq" else 0], torch.arange(i, e) if name == "dq" else clean
+            else:
+                i = s + hurt_rows[b]
+                clean, rest = (clean[clean != i], torch.tensor([i])) if name == "dq" else (clean[i - s + 1:], torch.arange(s, i + 1))
+            assert bool((off[clean] <= limit[clean]).all()), (name, b)
+            if name == "dv" and b in hurt_keys and bad == bad:
+                continue  # (a score of -inf is a probability of zero)
+            assert not t.cpu()[rest].isfinite().all(-1).any(), (name, b)
+
+
 def test_neighbours_do_not_mix():
     """NaN in one sequence stays there."""
     offsets = offsets_of([40, 50, 60])
