@@ -509,14 +509,7 @@ struct SeqSums {
     }
 };
 
-// Of a tile of 64 rows: whether some of this thread's pieces are not finite; out += factor times what is not finite of the rows [first, end); the finite
-// numbers alone.
-template <typename T, int HD, int NT>
-__device__ __forceinline__ bool tile_not_finite(const elem_t* tile, int tid) {
-    bool some = false;
-    for (int x = tid; x < SeqTile<HD>::kElems / 8; x += NT) some = some || any_not_finite<T>(reinterpret_cast<const u32x4*>(tile)[x]);
-    return some;
-}
+// Of a tile of 64 rows: out += factor times what is not finite of the rows [first, end); the finite numbers alone.
 template <typename T, int HD>
 __device__ __forceinline__ void add_not_finite(f32x16* out, const elem_t* tile, int first, int end, float factor, int h) {
     for (int j = first; j < end; ++j) {

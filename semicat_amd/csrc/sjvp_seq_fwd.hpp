@@ -64,13 +64,27 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 4 : 2) void seq_fwd(SeqPara
     int step = SeqTile<HD>::kBytes;
     const auto k_place = [&](int t) { return tiles + ((t - t0) & 1) * kTile; };
     const auto v_place = [&](int t) { return tiles + (2 + ((t - t0) & 1)) * kTile; };
-    // tile t's values that are not finite
+    // tile t's values that are not finite  (written out here: through the functions that the backward calls, which do the same, the compiler places
+    // the loops so that two prompts of 5000 and 8192 tokens, Hq=16 Hkv=2 D=128, take 355 us in place of 346)
     const auto care = [&](int t) {
         elem_t* V = v_place(t);
-        if (!workgroup_barrier_or(tile_not_finite<T, HD, kCtxThreads>(V, tid))) return;
-        add_not_finite<T, HD>(st.acc, V, 0, min(limit - t * kCtxTile, kCtxTile), 1.0f, h);
+        bool some = false;
+        for (int x = tid; x < kTile / 8; x += kCtxThreads) some = some || any_not_finite<T>(reinterpret_cast<const u32x4*>(V)[x]);
+        if (!workgroup_barrier_or(some)) return;
+        for (int j = 0; j < min(limit - t * kCtxTile, kCtxTile); ++j) {
+            const elem_t* from = V + j * SeqTile<HD>::kLd + 4 * h;
+#pragma unroll
+            for (int c = 0; c < HD / 8; ++c) {
+                const f32x4 more = only_not_finite<T>(from + 8 * (c ^ SeqTile<HD>::swz(j)));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) st.acc[c / 4][4 * (c % 4) + i] += more[i];
+            }
+        }
         workgroup_barrier();
-        keep_finite<T, HD, kCtxThreads>(V, tid);
+        for (int x = tid; x < kTile / 8; x += kCtxThreads) {
+            u32x4* piece = reinterpret_cast<u32x4*>(V) + x;
+            *piece = only_finite<T>(*piece);
+        }
         workgroup_barrier();
     };
     // the tiles that all rows see as a whole have a loop without masks
