@@ -103,15 +103,23 @@ PagedPlan paged_plan(const SeqParams& p) {
     };
     const auto splits = [](int64_t wanted, int64_t most, int64_t limit) { return (int)std::max<int64_t>(1, std::min<int64_t>({wanted, most, limit})); };
     const int64_t many = ceil_div(rows, kCtxOwned) * p.Hkv;
-    plan.has_many = p.T > p.B && 2 * many > cu;
+    // seq_fwd's blocks of 128 rows, where the sequences have 128 rows on average (H=28 G=4 D=64 e4m3, 37 sequences of 0 to 32 new tokens on up to 2490:
+    // 86 us with it, 41 without; 46 of up to 125, G=8: 26 and 50) and are many enough, which for a long cache is fewer blocks, each split over its keys
+    // (16 heads, 512 tokens on 32768: 190 us, 276 by seq_few; five sequences of 463 tokens, 95 blocks: 23 and 15).  Sequences of few rows
+    // have seq_few beside it unless 256 rows on average make such unlikely (one decodes while another's prompt is read).
+    plan.has_many = rows >= 128 * (int64_t)p.B && p.T > p.B && (keys < 1024 ? 2 : 8) * many > cu;
     plan.has_few = !plan.has_many || rows < 256 * (int64_t)p.B;
     if (plan.has_few) {
-        plan.few.split_tiles = 8;
-        plan.few.splits = splits(8 * cu / ((p.B + rows / 32) * p.Hkv), keys / (32 * plan.few.split_tiles), 128);
+        // Splits of 256 keys or more, 512 of 8 bits, which take half of the bytes (a token each of 11 sequences of 604, 17 heads: 16.3 us at 256, 12.9; of
+        // 21600 tokens of 16 bits, two heads: 15.3 and 17.8 at 384): as many as give eight workgroups to a compute unit (57 sequences of up to 20
+        // tokens on up to 10334, D=64: 54 us, 62 with half as many).  Below 768 keys the join costs more (16 tokens on 600, 8 heads: 14.9 us split, 12.3).
+        plan.few.split_tiles = p.pages.ks ? 16 : 8;
+        plan.few.splits = keys < 768 ? 1 : splits(8 * cu / ((p.B + rows / 32) * p.Hkv), keys / (32 * plan.few.split_tiles), 128);
         scratch(plan.few, p.Hkv * (plan.has_many ? (int64_t)(p.B + 2) * kSeqFew : rows));
     }
     if (plan.has_many) {
-        plan.many.split_tiles = 32;
+        // Splits of 2048 keys (1024: eight prompts of 512 tokens on up to 8192, 212 us in place of 187), of 512 where there are few blocks.
+        plan.many.split_tiles = 2 * many > cu ? 32 : 8;
         plan.many.splits = splits(8 * cu / many, keys / (kCtxTile * plan.many.split_tiles), 16);
         scratch(plan.many, p.Hkv * rows);
     }

@@ -84,6 +84,17 @@ __device__ __forceinline__ SeqBlock seq_block(const SeqParams& p, int slot, int 
     return b;
 }
 
+// Beside a launch that serves the longer sequences, kSeqFew / R slots to a segment.
+template <int R>
+__device__ __forceinline__ SeqBlock seq_block_few(const SeqParams& p, int slot) {
+    SeqBlock b;
+    b.segment = slot / (kSeqFew / R), b.row0 = slot % (kSeqFew / R) * R;
+    b.token = seq_offset(p, b.segment), b.tokens = max(0, seq_offset(p, b.segment + 1) - b.token);
+    b.held = b.segment >= 1 && b.segment <= p.B ? p.lengths[b.segment - 1] : 0;
+    b.some = b.row0 < b.tokens * p.G;
+    return b;
+}
+
 __device__ __forceinline__ int lanes_sum(int x) {
     x += __builtin_amdgcn_update_dpp(0, x, 0x128, 0xf, 0xf, false);  // turned by 8, 4, 2, 1 of 16
     x += __builtin_amdgcn_update_dpp(0, x, 0x124, 0xf, 0xf, false);
@@ -118,6 +129,45 @@ __device__ __forceinline__ SeqBlock seq_block_long_first(const SeqParams& p, int
     b.tokens = __builtin_amdgcn_readlane(tokens, b.segment);
     b.row0 = (back ? __builtin_amdgcn_readlane(blocks, b.segment) - 1 - lo : lo) * R;
     b.held = 0;
+    return b;
+}
+
+// Sum over the lanes up to this one.
+__device__ __forceinline__ int lanes_scan(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // from 1, 2, 4, 8 lanes below in a row of 16
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // the last lane of a row to the next row
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // that of the first half to the second one
+    return x;
+}
+
+// The blocks of the paged attention in descending order of their sequences' keys (in 16 classes), for the same reason, over the sequences that the
+// launch serves; a sequence's last block first.
+template <int R, int TILE>
+__device__ __forceinline__ SeqBlock seq_block_most_keys_first(const SeqParams& p, int rank, int lane) {
+    if (p.B + 2 > 64) return seq_block<R, true>(p, p.slots - 1 - rank, p.G, lane);
+    const int at = seq_offset(p, min(lane, p.B + 2)), tokens = lane < p.B + 2 ? max(0, seq_offset(p, lane + 1) - at) : 0;
+    const int held = lane >= 1 && lane <= p.B ? p.lengths[lane - 1] : 0, rows = tokens * p.G;
+    const int blocks = rows >= p.least && rows <= p.most ? (rows + R - 1) / R : 0;
+    int key = min(max(held, 0), p.pages.capacity) / TILE;
+    while (__builtin_amdgcn_ballot_w64(key > 15)) key >>= 1;
+    int lo = 0, hi = 16;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (lanes_sum(key >= mid ? blocks : 0) > rank) lo = mid;
+        else hi = mid;
+    }
+    const int left = rank - lanes_sum(key > lo ? blocks : 0), upto = lanes_scan(key == lo ? blocks : 0);
+    const uint64_t those = __builtin_amdgcn_ballot_w64(upto > left);
+    SeqBlock b;
+    b.some = those != 0;
+    b.segment = those ? __builtin_ctzll(those) : 0;
+    b.token = __builtin_amdgcn_readlane(at, b.segment);
+    b.tokens = __builtin_amdgcn_readlane(tokens, b.segment);
+    b.held = __builtin_amdgcn_readlane(held, b.segment);
+    b.row0 = (__builtin_amdgcn_readlane(upto, b.segment) - 1 - left) * R;
     return b;
 }
 

@@ -40,7 +40,7 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 4 : 2) void seq_fwd(SeqPara
     elem_t* tiles = reinterpret_cast<elem_t*>(smem);  // K [2], V [2]
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
     const int hk = blockIdx.x % p.Hkv, x = blockIdx.x / p.Hkv, split = PAGED ? x / p.slots : 0;
-    const SeqBlock b = PAGED ? seq_block<kCtxOwned, true>(p, p.slots - 1 - (x - split * p.slots), p.G, lane)
+    const SeqBlock b = PAGED ? seq_block_most_keys_first<kCtxOwned, kCtxTile>(p, x - split * p.slots, lane)
                              : seq_block_long_first<kCtxOwned>(p, x, p.G, false, lane);
     const int all = b.tokens * p.G;
     if (!b.some || all < p.least || all > p.most) return;
@@ -69,7 +69,10 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 4 : 2) void seq_fwd(SeqPara
     const auto care = [&](int t) {
         elem_t* V = v_place(t);
         bool some = false;
-        for (int x = tid; x < kTile / 8; x += kCtxThreads) some = some || any_not_finite<T>(reinterpret_cast<const u32x4*>(V)[x]);
+        for (int x = tid; x < kTile / 8; x += kCtxThreads) {
+            const int row = x / SeqTile<HD>::PP, c = x % SeqTile<HD>::PP ^ SeqTile<HD>::swz(row);
+            if (HD == SeqTile<HD>::kLd || 8 * c < HD) some = some || any_not_finite<T>(reinterpret_cast<const u32x4*>(V)[x]);  // (not what pads a row)
+        }
         if (!workgroup_barrier_or(some)) return;
         for (int j = 0; j < min(limit - t * kCtxTile, kCtxTile); ++j) {
             const elem_t* from = V + j * SeqTile<HD>::kLd + 4 * h;
@@ -212,9 +215,9 @@ __global__ __launch_bounds__(64 * WAVES, NC == 1 ? (E4M3 || HD <= 96 ? 4 : 3) : 
     float* stats = sums + WAVES * R * kSum;  // [WAVES][R] maximum, then sum
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), y = lane & 15, g = lane >> 4;
     const int hk = blockIdx.x % p.Hkv, x = blockIdx.x / p.Hkv, slot = x % p.slots, split = x / p.slots;
-    const SeqBlock b = seq_block<R, true>(p, slot, p.G, lane);
+    const SeqBlock b = p.most == kSeqFew ? seq_block_few<R>(p, slot) : seq_block<R, true>(p, slot, p.G, lane);
     const int all = b.tokens * p.G;
-    if (!b.some || all < p.least || all > p.most) return;
+    if (!b.some || all > p.most) return;
     const SeqKeys<true> keys(p, b);
     const int r0 = b.row0, rows = min(all - r0, R);
     const int n = keys.seen(p, (r0 + rows - 1) / p.G), whole = keys.seen(p, r0 / p.G);

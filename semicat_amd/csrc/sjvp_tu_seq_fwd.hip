@@ -28,9 +28,18 @@ int seq_paged<SJVP_T>(SeqParams p, const PagedPlan& plan, float* ws, bool e4m3, 
         constexpr int HD = decltype(hd)::value;
         const auto few = [&](auto sets, auto bits8) {
             constexpr int NC = decltype(sets)::value;
-            p.slots = (int)seq_slots(p, p.G, 16 * NC);
-            const int smem = kCtxWaves * std::max(32 * (HD + 8) * 2, 16 * NC * (HD + 4 + 2) * 4);
-            return launch(seq_few<SJVP_T, HD, decltype(bits8)::value, NC, kCtxWaves>, p.slots * p.Hkv * p.splits, smem, stream, p, kCtxThreads);
+            p.slots = (int)(plan.has_many ? (int64_t)(p.B + 2) * (kSeqFew / (16 * NC)) : seq_slots(p, p.G, 16 * NC));
+            const auto run = [&](auto waves) {
+                constexpr int WAVES = decltype(waves)::value;
+                const int smem = WAVES * std::max(32 * (HD + 8) * 2, 16 * NC * (HD + 4 + 2) * 4);
+                return launch(seq_few<SJVP_T, HD, decltype(bits8)::value, NC, WAVES>, p.slots * p.Hkv * p.splits, smem, stream, p, 64 * WAVES);
+            };
+            // Short caches: a workgroup of one wave, of which four times as many run at once (123 tokens on up to 43 each, 23 heads of 112: 12.6 us in place
+            // of 20.9; 11 sequences of 71 tokens on 71, 32 heads of 128: 15.1 and 21.0); a few of them are faster with four waves (36 sequences
+            // of 8 tokens on up to 65, 9 heads: 8.5 us and 11.1).
+            const int64_t keys = p.pages.capacity;
+            const bool alone = keys <= 64 || (keys <= 512 && 32 * (int64_t)p.slots * p.Hkv >= keys * compute_units());
+            return alone ? run(std::integral_constant<int, 1>{}) : run(std::integral_constant<int, kCtxWaves>{});
         };
         const auto join = [&](const SeqParams& x) {
             if (x.splits == 1) return (int)SJVP_OK;

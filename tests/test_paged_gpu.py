@@ -222,6 +222,41 @@ def test_many_rows_of_many_sequences():
 
 
 @pytest.mark.parametrize("quantized", [True, False])
+@pytest.mark.parametrize("most,B,H,G,D,dtype", [(40, 50, 4, 1, 64, BF16), (64, 9, 4, 2, 128, FP16), (1, 70, 3, 3, 16, BF16), (200, 150, 32, 1, 48, BF16),
+                                                 (120, 64, 40, 2, 96, FP16), (130, 40, 40, 1, 112, BF16)])
+def test_short_caches(most, B, H, G, D, dtype, quantized):
+    """Caches that a wave reads by itself, and their neighbours."""
+    g = torch.Generator().manual_seed(most)
+    held = torch.randint(0, most + 1, (B,), generator=g).tolist()
+    held[0], held[-1] = most, 0
+    new = [min(n, int(torch.randint(0, 1 + min(most, 12), (1,), generator=g))) for n in held]
+    pages = sum(-(-n // 8) for n in held) + 3
+    cache = cache_of(pages, 8, H // G, D, dtype, quantized)
+    tables = tables_of(held, 8, pages, extra=0)
+    check_attention(cache, normal(sum(new), H, D, dtype=dtype), tables, held, offsets_of(new))
+    check_attention(cache, normal(B, H, D, dtype=dtype), tables, held, None)
+
+
+@pytest.mark.parametrize("quantized", [True, False])
+@pytest.mark.parametrize("B,G,D,dtype", [(7, 4, 128, BF16), (62, 2, 64, FP16), (63, 2, 96, BF16), (1, 8, 80, BF16)])
+def test_chunks_on_caches_of_all_lengths(B, G, D, dtype, quantized):
+    """Blocks of 128 rows in the order of their sequences' lengths, up to 62 sequences, and in the plain order with more."""
+    g = torch.Generator().manual_seed(B)
+    new = [int(n) for n in torch.randint(128 // G, 512 // G, (B,), generator=g)]
+    held = [n + int(m) for n, m in zip(new, torch.randint(0, 3000 if B < 10 else 200, (B,), generator=g))]
+    new[B // 2] = 0
+    if B > 2:
+        held[1], held[2] = held[0], 0
+        new[2] = 3  # (more new tokens than the cache has)
+    H = 12 * G if B < 10 else 2 * G
+    pages = sum(-(-n // 64) for n in held) + 3
+    cache = cache_of(pages, 64, H // G, D, dtype, quantized)
+    tables = tables_of(held, 64, pages)
+    new[1 % B] = min(new[1 % B], held[1 % B])
+    check_attention(cache, normal(max(1, sum(new)), H, D, dtype=dtype)[:sum(new)], tables, held, offsets_of(new))
+
+
+@pytest.mark.parametrize("quantized", [True, False])
 def test_pages_that_the_cache_has_not(quantized):
     """They read as zeros and take no writes; lengths beyond the table end there."""
     from semicat_amd import paged_read, paged_write
