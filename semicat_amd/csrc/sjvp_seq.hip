@@ -25,7 +25,9 @@ int seq_common(SeqParams& p, int B, int T, int Hq, int Hkv, int D, float scale) 
     return SJVP_OK;
 }
 
-// The backward of whole sequences: the column-owned launch is split over the heads that share a key head.
+// The backward of whole sequences: the column-owned launch is split over the heads that share a key head, as far as four workgroups to a compute unit
+// (four sequences of 1024 to 2048 tokens, Hq=32 Hkv=4 D=128, forward and backward: 476 us; one 677, two 489, eight 494; of 1500 to 6000, Hq=16: 1244,
+// 1364, 1358 and 1286).
 struct PackedPlan {
     int splits = 1;
     size_t part = 0, total = 0;  // floats

@@ -11,7 +11,8 @@ namespace sjvp {
 // Blocks of R rows that the segments of a call can have (see seq_block).
 inline int64_t seq_slots(const SeqParams& p, int heads, int R) { return (int64_t)p.T * heads / R + p.B + 2; }
 
-// Sets of 16 rows to a block of seq_few.
+// Sets of 16 rows to a block of seq_few: one where a sequence has up to 16 rows on average, which leaves registers for four waves to a SIMD (a token each of
+// 64 sequences on 1200 to 4096, Hq=16 Hkv=4 D=128 e4m3: 41.5 us, two sets 48.2; six tokens of 16, 24 rows: 25.9 and 22.3).
 inline int seq_sets(const SeqParams& p) { return (int64_t)p.T * p.G <= 16 * (int64_t)p.B ? 1 : 2; }
 
 inline bool seq_dma(const SeqParams& p, const CtxView& a, const CtxView& b) { return p.D % 8 == 0 && ctx_aligned(a) && ctx_aligned(b); }

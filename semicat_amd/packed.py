@@ -175,7 +175,8 @@ def packed_attention(q: Tensor, k: Tensor, v: Tensor, offsets: Tensor, causal: b
 
     ``offsets`` (int32 ``[sequences + 1]``, ascending, on the GPU) says where: sequence ``b`` has the rows ``offsets[b]`` up to
     ``offsets[b + 1]``; sequences may be empty.  Rows in front of the first sequence and behind the last one are not used, results and
-    gradients there are zeros.  The lengths are not looked at by the host.  ``causal`` hides the tokens behind a query.  ``Hq`` is a
+    gradients there are zeros.  The lengths are not looked at by the host.  ``causal`` hides the tokens behind a query: infinities and
+    NaN among them reach neither its result nor its gradient.  ``Hq`` is a
     multiple of ``Hkv``; query head ``h`` reads key head ``h // (Hq // Hkv)``.  ``scale`` defaults to ``1/sqrt(D)``.  bfloat16 and float16,
     16 <= D <= 128; other types are computed in bfloat16 and handed back as they came."""
     if _on_gpu(q):

@@ -207,7 +207,8 @@ def paged_attention(q: Tensor, cache: PagedCache, tables: Tensor, lengths: Tenso
     """Attention of the new tokens ``q`` ``[T,Hq,D]`` on all tokens that the cache holds of their sequences, causal: token ``i`` of ``n`` new ones
     has the position ``length - n + i`` and sees the positions up to its own, which :func:`paged_write` has filled before.  Returns
     ``[T,Hq,D]``; rows that see nothing, and rows outside the sequences, are zeros.  ``Hq`` is a multiple of the cache's heads, ``scale``
-    defaults to ``1/sqrt(D)``.  Sequences with one new token and with whole chunks of a prompt may stand in one call.  ``q`` of
+    defaults to ``1/sqrt(D)``.  Sequences with one new token and with whole chunks of a prompt may stand in one call.  What the
+    pages hold behind a token's position, NaN included, does not reach its result.  ``q`` of
     another type than the cache's is computed in the cache's and handed back as it came."""
     if _on_gpu(q):
         o = _lib.host().paged_attention(q, *cache._storage(), tables, lengths, offsets, scale)

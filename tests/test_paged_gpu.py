@@ -256,6 +256,18 @@ def test_chunks_on_caches_of_all_lengths(B, G, D, dtype, quantized):
     check_attention(cache, normal(max(1, sum(new)), H, D, dtype=dtype)[:sum(new)], tables, held, offsets_of(new))
 
 
+@pytest.mark.parametrize("D,dtype", [(128, BF16), (48, FP16)])
+@pytest.mark.parametrize("G,few", [(4, (7, 8, 9)), (1, (31, 32, 33)), (8, (3, 4, 5))])
+def test_the_border_of_few_rows(G, few, D, dtype):
+    """Sequences of 32 rows and their neighbours in number beside long ones, split over the keys or not."""
+    new = [*few, 1, 0, 700 // G, *few, 2100 // G]
+    for more in (0, 2500):
+        held = [n + more * (i % 2) for i, n in enumerate(new)]
+        pages = sum(-(-n // 16) for n in held) + 3
+        cache = cache_of(pages, 16, 8, D, dtype, True)
+        check_attention(cache, normal(sum(new), 8 * G, D, dtype=dtype), tables_of(held, 16, pages), held, offsets_of(new))
+
+
 @pytest.mark.parametrize("quantized", [True, False])
 def test_pages_that_the_cache_has_not(quantized):
     """They read as zeros and take no writes; lengths beyond the table end there."""
