@@ -56,7 +56,7 @@ __device__ __forceinline__ uint32_t to_e4m3(u32x4 a, u32x4 b, u32x4& codes) {
 }
 
 // A wave writes one token: its rows of K and V of all heads, 16 bytes of a page to a lane.  A lane quantises 16 columns, so that a group of 32 needs one
-// exchange.  Eight prompts of 2048 to 4096 tokens, 8 heads of 128, e4m3: 28 us = 5.6 TB/s, the vector unit busy all the while; one token each
+// exchange.  Eight prompts of 2048 to 4096 tokens, 8 heads of 128, e4m3: 28 us = 5.4 TB/s, the vector unit busy all the while; one token each
 // of 64 sequences: 4.5 us, those of any launch.
 template <typename T, bool E4M3>
 __global__ __launch_bounds__(kCtxThreads) void paged_write(SeqParams p) {

@@ -261,7 +261,7 @@ __device__ __forceinline__ void store_col(const SeqParams& p, const SeqCols& w, 
 }
 
 // Column-owned: four waves of 32 keys share tiles of 64 query rows, over all heads that read the key head (or, with splits, over a part of them).  Own K and V
-// stay in registers.  64 sequences of 16 to 128 tokens, 12 heads, D=64, whole: 18.4 us = 2.6 TB/s, one tile to a workgroup.
+// stay in registers.  64 sequences of 16 to 128 tokens, 12 heads, D=64, whole: 18.4 us = 2.3 TB/s, one tile to a workgroup.
 template <typename T, int HD, bool DMA>
 __global__ __launch_bounds__(kCtxThreads, 2) void seq_bwd_col(SeqParams p) {
     if constexpr (DMA) __builtin_assume(p.D % 8 == 0);
@@ -463,7 +463,8 @@ __global__ __launch_bounds__(2 * kCtxThreads, 2) void seq_bwd_col_pair(SeqParams
     finish(dv, ok, 1.0f, p.dv, 1);
 }
 
-// Adds up the splits of seq_bwd_col, eight columns to a thread, in a fixed order.  Two splits of 15000 tokens, four heads of 128: 23 us = 5.3 TB/s.
+// Adds up the splits of seq_bwd_col, eight columns to a thread, in a fixed order.  Two splits of 15000 tokens, four heads of 128: 154 MB in 23 us, from the caches in
+// part.
 template <typename T, int HD>
 __global__ __launch_bounds__(kCtxThreads) void seq_sum(SeqParams p) {
     constexpr int CH = HD / 8;

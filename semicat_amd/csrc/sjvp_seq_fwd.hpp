@@ -36,7 +36,7 @@ __device__ __forceinline__ int64_t seq_place(const SeqParams& p, const SeqBlock&
 //
 // Bound by the matrix unit and the exponentials alike: two prompts of 4915 and 8192 tokens, Hq=16 Hkv=2 D=128, causal, 346 us = 1.09 PFLOP/s (a
 // 16384^3 product: 1.36), the matrix unit busy 59 % and the vector unit 58 %; 64 sequences of 16 to 128 tokens, 12 heads, D=64, whole, 12.5 us =
-// 3.8 TB/s, where a workgroup is one or two tiles and its start and end.  On pages (eight prompts of 128 to 512 tokens on 2048 to 8192, Hq=16
+// 2.3 TB/s, where a workgroup is one or two tiles and its start and end.  On pages (eight prompts of 128 to 512 tokens on 2048 to 8192, Hq=16
 // Hkv=4 D=128 e4m3) 166 us and 20 for the join, 0.64 PFLOP/s: a tile of 8-bit numbers goes through registers, with 10 vector instructions to a matrix
 // instruction in place of 7 (16-bit pages, by LDS-DMA, are as fast: 165), and a launch whose workgroups are 2.1 times what runs at once.
 template <typename T, int HD, bool PAGED, typename FEED>
@@ -214,7 +214,7 @@ __device__ __forceinline__ float quarters_sum(float x) {
 // The matrix instructions are 16x16x32 (tile algebra in sjvp_w16.hpp), so that a step of a group of heads, some four to sixteen rows, leaves
 // little of them idle, and a wave needs 128 registers at most: four waves to a SIMD hold twice as many loads in flight as the 32-wide form did.
 //
-// Bound by memory where sequences are many (a token each of 64 sequences of 2048 to 8192, Hq=16 Hkv=4 D=128 e4m3: 75 us = 4.8 TB/s, a copy makes
+// Bound by memory where sequences are many (a token each of 64 sequences of 2048 to 8192, Hq=16 Hkv=4 D=128 e4m3: 75 us = 4.6 TB/s, a copy makes
 // 5.2), by the latency of offsets, tables and two tiles one behind the other where they are few (four tokens on 29491 and 32769, Hq=16 Hkv=2, 16 bits: 20 us,
 // 3.2 TB/s; a token on 128: 5 us).
 // E4M3: the cache's numbers have 8 bits; a lane's 16 bytes are columns of two chunks of 32 then, and q is read in that order.
@@ -437,7 +437,7 @@ __global__ __launch_bounds__(64 * WAVES, NC == 1 ? (E4M3 || HD <= 96 ? 4 : 3) : 
 
 // Joins the splits of seq_few or seq_fwd: 16 threads to the columns of a row (eight each), `slices` of them to the splits, which meet in LDS.  A launch of
 // its own, 4 to 7 us for few rows, whose least is 4: a join by the last workgroup would need counters that start at zero, which is a launch
-// too.  87 MB of the sums of 16384 tokens' chunks in 19 us = 4.6 TB/s.
+// too.  41000 rows of 128 in one to four splits, some 60 MB of sums: 19 us = 3.7 TB/s.
 template <typename T, int HD>
 __global__ __launch_bounds__(kCtxThreads) void seq_join(SeqParams p) {
     __shared__ float met[kCtxThreads / 16][16][11];
