@@ -324,3 +324,68 @@ def test_a_captured_backward_replays():
         for t, n in zip((o, *grads), ("o", "dq", "dk", "dv")):
             assert torch.equal(t, want[n]), n
         run(x, offsets, False)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_thousands_of_sequences(causal):
+    g = torch.Generator().manual_seed(0)
+    offsets = offsets_of(torch.randint(0, 3, (4200,), generator=g).tolist(), 3)  # (a search in three steps)
+    x = make(offsets[-1] + 2, 1, 1, 16, BF16)
+    check(run(x, offsets, causal), x, offsets, causal)
+
+
+@pytest.mark.parametrize("D,G", [(64, 2), (128, 1), (36, 2)])
+def test_broadcast_inputs(D, G):
+    """Keys, values and cotangents that are one row seen many times: the same numbers as their copies, gradients summed over the broadcast."""
+    from semicat_amd import packed_attention
+    T, offsets = 200, offsets_of([150, 50])
+    x = make(T, 4, G, D, BF16)
+    at = torch.tensor(offsets, dtype=torch.int32, device="cuda")
+    q = x["q"].cuda()
+    for shape in ((1, 1, D), (T, 1, D), (1, 4 // G, D)):
+        k, v = (x[n][:shape[0], :shape[1]].cuda() for n in "kv")
+        cot = x["dO"][:shape[0], :1].cuda().expand(T, 4, D)
+        wide = [t.expand(T, 4 // G, D) for t in (k, v)]
+        leaves = [q.clone().requires_grad_(), *(t.clone().requires_grad_() for t in wide)]
+        want = torch.autograd.grad(packed_attention(*leaves, at), leaves, cot.contiguous())
+        leaves = [q.clone().requires_grad_(), *(t.clone().requires_grad_() for t in (k, v))]
+        got = torch.autograd.grad(packed_attention(leaves[0], *(t.expand(T, 4 // G, D) for t in leaves[1:]), at), leaves, cot)
+        assert torch.equal(got[0], want[0])
+        for a, b, t in zip(got[1:], want[1:], (k, v)):
+            assert torch.equal(a, b.sum_to_size(t.shape))
+
+
+def test_function_transforms():
+    from semicat_amd import packed_attention
+    offsets = offsets_of([40, 33])
+    x = make(73, 2, 1, 64, BF16)
+    want = run(x, offsets, True)
+    at = torch.tensor(offsets, dtype=torch.int32, device="cuda")
+    q, k, v, dO = (x[n].cuda() for n in ("q", "k", "v", "dO"))
+    o, pull = torch.func.vjp(lambda *t: packed_attention(*t, at), q, k, v)
+    assert torch.equal(o, want["o"])
+    for a, n in zip(pull(dO), ("dq", "dk", "dv")):
+        assert torch.equal(a, want[n])
+    with pytest.raises(NotImplementedError):
+        torch.func.jvp(lambda t: packed_attention(t, k, v, at), (q,), (q,))
+    with pytest.raises(Exception):
+        torch.func.vmap(lambda t: packed_attention(t, k, v, at))(q[None])
+    torch.cuda.synchronize()
+
+
+def test_places_beyond_32_bits():
+    """The last rows of tensors of more than 4 GiB."""
+    from semicat_amd import packed_attention
+    T, H, D, tail = 2_200_000, 8, 128, 330
+    x = make(tail, H, 1, D, BF16)
+    big = {n: torch.zeros(T, H, D, dtype=BF16, device="cuda") for n in x}
+    for n, t in x.items():
+        big[n][T - tail:] = t.cuda()
+    results = []
+    for tensors, first in (({n: t.cuda() for n, t in x.items()}, 0), (big, T - tail)):
+        at = torch.tensor([first, first + 200, first + tail], dtype=torch.int32, device="cuda")
+        leaves = [tensors[n].requires_grad_() for n in "qkv"]
+        o = packed_attention(*leaves, at)
+        results.append([o.detach(), *torch.autograd.grad(o, leaves, tensors["dO"])])
+    for small, large in zip(*results):
+        assert torch.equal(small, large[T - tail:]) and not large[:T - tail].any()
