@@ -375,7 +375,7 @@ int sjvp_packed_bwd(const sjvp_packed* t, int dtype, void* stream);
  * A cache in pages.  k_pages, v_pages: [pages, Hkv, page_size, D] with the byte strides (page, head, row) page_strides[0..2], the same of both;
  * numbers of the tensors' 16-bit type (D a multiple of 8), or, with k_scales and v_scales, of 8 bits (e4m3; D a multiple of 16), of which each 32 columns
  * of a row have a power of two 2^(code - 127), code an unsigned byte of [pages, Hkv, page_size, ceil(D/32)] with the byte strides
- * page_strides[3..5].  Rows of k_pages and v_pages start on 16-byte boundaries.
+ * page_strides[3..5].  Rows of k_pages and v_pages start on 16-byte boundaries; strides between pages and between rows are below 2^32.
  *   tables   device array [B][table_pages] with the row stride table_stride: position x of sequence b stands in row x % page_size of page
  *       tables[b][x / page_size].  A number that is none of the cache's pages reads as zeros and takes no writes.
  *   lengths  device array [B]: the tokens that the cache holds of a sequence, those of the call among them; clamped to what the table has.

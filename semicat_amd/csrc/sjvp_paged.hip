@@ -71,7 +71,7 @@ __global__ __launch_bounds__(kCtxThreads) void paged_write(SeqParams p) {
     if ((uint32_t)page >= (uint32_t)p.pages.pages) return;
     constexpr int kColumns = E4M3 ? 16 : 8;
     const int per = E4M3 ? (p.D + 31) / 32 * 2 : p.D / 8;  // (E4M3: the lanes of a group stand side by side)
-    const int64_t to = page * p.pages.sp + row * p.pages.sr, scale_to = page * p.pages.scale_sp + row * p.pages.scale_sr;
+    const int64_t to = p.pages.at(page, row), scale_to = p.pages.scale_at(page, row);
     for (int x0 = 0; x0 < 2 * p.Hkv * per; x0 += 64) {
         const int x = x0 + lane, unit = x % per, hx = x / per, v = hx >= p.Hkv, head = v ? hx - p.Hkv : hx, c = kColumns * unit;
         const bool ok = hx < 2 * p.Hkv && c < p.D;
@@ -104,7 +104,7 @@ __global__ __launch_bounds__(kCtxThreads) void paged_read(SeqParams p) {
     const bool there = (uint32_t)page < (uint32_t)p.pages.pages;
     constexpr int kColumns = E4M3 ? 16 : 8;
     const int per = p.D / kColumns, row = position - at * p.pages.size;
-    const int64_t from = page * p.pages.sp + row * p.pages.sr, scale_from = page * p.pages.scale_sp + row * p.pages.scale_sr;
+    const int64_t from = p.pages.at(page, row), scale_from = p.pages.scale_at(page, row);
     for (int x = lane; x < 2 * p.Hkv * per; x += 64) {
         const int unit = x % per, hx = x / per, v = hx >= p.Hkv, head = v ? hx - p.Hkv : hx, c = kColumns * unit;
         elem_t* to = (v ? p.v : p.k).head(b, head) + position * (v ? p.v : p.k).sl;

@@ -67,6 +67,8 @@ int paged_params(const sjvp_paged* t, SeqParams& p, int T) {
     if (!t->k_pages || !t->v_pages || !t->tables || !t->lengths || !t->k_scales != !t->v_scales) return SJVP_ERR_NULL;
     for (int i = 0; i < 3; ++i)
         if (t->page_strides[i] % 16 || t->page_strides[i] < 0) return SJVP_ERR_PAGES;
+    for (int i : {0, 2, 3, 5})
+        if (t->page_strides[i] < 0 || t->page_strides[i] > UINT32_MAX) return SJVP_ERR_PAGES;
     if (reinterpret_cast<uintptr_t>(t->k_pages) % 16 || reinterpret_cast<uintptr_t>(t->v_pages) % 16) return SJVP_ERR_PAGES;
     CtxView* views[SJVP_P_COUNT] = {&p.q, &p.o, &p.k, &p.v};
     const void* ptrs[SJVP_P_COUNT] = {t->q, t->o, t->k, t->v};
@@ -76,8 +78,8 @@ int paged_params(const sjvp_paged* t, SeqParams& p, int T) {
     SeqPages& g = p.pages;
     g.k = static_cast<unsigned char*>(t->k_pages), g.v = static_cast<unsigned char*>(t->v_pages);
     g.ks = static_cast<unsigned char*>(t->k_scales), g.vs = static_cast<unsigned char*>(t->v_scales);
-    g.sp = t->page_strides[0], g.sh = t->page_strides[1], g.sr = t->page_strides[2];
-    g.scale_sp = t->page_strides[3], g.scale_sh = t->page_strides[4], g.scale_sr = t->page_strides[5];
+    g.sp = (uint32_t)t->page_strides[0], g.sh = t->page_strides[1], g.sr = (uint32_t)t->page_strides[2];
+    g.scale_sp = (uint32_t)t->page_strides[3], g.scale_sh = t->page_strides[4], g.scale_sr = (uint32_t)t->page_strides[5];
     g.table = t->tables, g.table_stride = t->table_stride;
     g.pages = t->pages, g.size = t->page_size;
     g.capacity = (int)std::min<int64_t>((int64_t)t->table_pages * t->page_size, kCtxMost);

@@ -23,12 +23,18 @@ namespace sjvp {
 // table[b][x / size]; a page number that the cache has not reads as zeros.
 struct SeqPages {
     unsigned char *k, *v, *ks, *vs;
-    int64_t sp, sh, sr, scale_sp, scale_sh, scale_sr;
+    int64_t sh, scale_sh;
+    uint32_t sp, sr, scale_sp, scale_sr;  // (of 32 bits: an instruction to a product in place of four; 79 sequences of up to 11 tokens on 1280 to
+                                          // 5120, 16 heads of 32, e4m3: 62 us in place of 70)
     const int* table;
     int64_t table_stride;
     int pages, size, capacity;  // capacity: positions that a row of the table has
     int scale_words;            // the exponents of a row are one word of memory (32 or 16 bits)
     uint32_t magic, shift;      // x / size = mulhi(2 x, magic) >> shift below 2^30
+    __device__ __forceinline__ int64_t at(int page, int row) const { return (int64_t)((uint64_t)(uint32_t)page * sp + (uint64_t)(uint32_t)row * sr); }
+    __device__ __forceinline__ int64_t scale_at(int page, int row) const {
+        return (int64_t)((uint64_t)(uint32_t)page * scale_sp + (uint64_t)(uint32_t)row * scale_sr);
+    }
     __device__ __forceinline__ int page_of(int x) const { return (int)(__umulhi(2u * (uint32_t)x, magic) >> shift); }
 };
 
@@ -445,7 +451,7 @@ struct PageFeed {
         for (int i = 0; i < N; ++i) {
             const int r = (x + kCtxThreads * i) / CH, c = (x + kCtxThreads * i) % CH ^ At::swz(r);
             const bool ok = (uint32_t)page[i] < (uint32_t)p.pages.pages && 8 * c < p.D;
-            const int64_t at = page[i] * p.pages.sp + head + row[i] * p.pages.sr + 16 * c;
+            const int64_t at = p.pages.at(page[i], row[i]) + head + 16 * c;
             const void* none = &kZeroPiece;
             const void *from_k = ok ? p.pages.k + at : none, *from_v = ok ? p.pages.v + at : none;
             dma16(from_k, lds_addr(kp) + 16 * (64 * wave + kCtxThreads * i));
@@ -483,8 +489,8 @@ struct PageFeed8 {
         for (int i = 0; i < N; ++i) {
             const int c = (x + kCtxThreads * i) % PC;
             const bool ok = (uint32_t)page[i] < (uint32_t)p.pages.pages && 16 * c < p.D;
-            const int64_t at = page[i] * p.pages.sp + head + row[i] * p.pages.sr + 16 * c;
-            const int64_t sat = page[i] * p.pages.scale_sp + scale_head + row[i] * p.pages.scale_sr + c / 2;
+            const int64_t at = p.pages.at(page[i], row[i]) + head + 16 * c;
+            const int64_t sat = p.pages.scale_at(page[i], row[i]) + scale_head + c / 2;
             const void* none = &kZeroPiece;
             kr[i] = global<u32x4>(ok ? p.pages.k + at : none), vr[i] = global<u32x4>(ok ? p.pages.v + at : none);
             ks[i] = global<uint8_t>(ok ? p.pages.ks + sat : none), vs[i] = global<uint8_t>(ok ? p.pages.vs + sat : none);

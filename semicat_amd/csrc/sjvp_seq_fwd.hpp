@@ -269,7 +269,7 @@ __global__ __launch_bounds__(64 * WAVES, NC == 1 ? (E4M3 || HD <= 96 ? 4 : 3) : 
         for (int u = 0; u < 2; ++u) {
             const int key = 32 * t + 16 * u + y, row = key - p.pages.page_of(key) * p.pages.size;
             const bool there = (uint32_t)page[u] < (uint32_t)p.pages.pages;
-            const int64_t at = page[u] * p.pages.sp + row * p.pages.sr;
+            const int64_t at = p.pages.at(page[u], row);
 #pragma unroll
             for (int c = 0; c < NP; ++c) {
                 if (E4M3 && KC % 2 && c == NP - 1) {
@@ -285,7 +285,7 @@ __global__ __launch_bounds__(64 * WAVES, NC == 1 ? (E4M3 || HD <= 96 ? 4 : 3) : 
                 }
             }
             if constexpr (E4M3) {
-                const int64_t sat = page[u] * p.pages.scale_sp + row * p.pages.scale_sr;
+                const int64_t sat = p.pages.scale_at(page[u], row);
                 ks[u] = scale_codes<KC>(there ? ksp + sat : none, p.pages.scale_words);
                 vs[u] = scale_codes<KC>(there ? vsp + sat : none, p.pages.scale_words);
             }

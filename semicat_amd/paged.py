@@ -52,8 +52,8 @@ class PagedCache:
     @classmethod
     def of(cls, k: Tensor, v: Tensor, k_scales: Optional[Tensor] = None, v_scales: Optional[Tensor] = None,
            dtype: Optional[torch.dtype] = None) -> "PagedCache":
-        """A cache in tensors that the caller has, of any strides whose pages, heads and rows are multiples of 16 bytes apart, the same of k and v.
-        ``dtype``: the 16-bit type that quantised numbers stand for (bfloat16 if not said)."""
+        """A cache in tensors that the caller has, of any strides whose pages, heads and rows are multiples of 16 bytes apart, pages
+        and rows less than 4 GiB, the same of k and v.  ``dtype``: the 16-bit type that quantised numbers stand for (bfloat16 if not said)."""
         cache = cls.__new__(cls)
         cache._take(k, v, k_scales, v_scales, dtype)
         return cache
@@ -87,6 +87,8 @@ class PagedCache:
             if k_scales.device != k.device or places(k_scales) != places(v_scales):
                 raise AssertionError("scales of k and v must have the same strides, on the pages' device")
             strides += places(k_scales)
+        if any(not 0 <= s < 1 << 32 for i, s in enumerate(strides) if i % 3 != 1):
+            raise AssertionError("pages, and the rows of a page, must be less than 4 GiB apart")
         self.k, self.v, self.k_scales, self.v_scales, self.dtype = k, v, k_scales, v_scales, dtype
         self._strides = strides + (0,) * (6 - len(strides))
 

@@ -163,6 +163,8 @@ def test_cache_of_the_caller_s_tensors():
     (AssertionError, lambda: PagedCache.of(*[_t(4, 2, 8, 40)[..., 4:36]] * 2)),          # 8 bytes off
     (AssertionError, lambda: PagedCache.of(_t(4, 2, 8, 32), _t(4, 8, 2, 32).transpose(1, 2))),
     (AssertionError, lambda: PagedCache.of(*[_t(4, 2, 32, 8).transpose(2, 3)] * 2)),
+    (AssertionError, lambda: PagedCache.of(*[torch.empty_strided((2, 2, 8, 32), (1 << 31, 256, 32, 1), dtype=BF16, device="meta")] * 2)),
+    (AssertionError, lambda: PagedCache.of(*[torch.empty_strided((2, 2, 8, 32), (256, 512, 1 << 31, 1), dtype=BF16, device="meta")] * 2)),
     (RuntimeError, lambda: paged_read(PagedCache(4, 8, 2, 32, device="cpu"), _i(3, 2), _i(3), 4)),
     (AssertionError, lambda: paged_read(_cache(), _i(3), _i(3), 4)),
     (TypeError, lambda: paged_read(_cache(), _i(3, 2, dtype=torch.int64), _i(3), 4)),
@@ -272,6 +274,11 @@ def test_status_of_the_paged_cache_beyond_the_fields():
         assert getattr(lib, fn)(None, 0, None) == _lib.SJVP_ERR_NULL
     for fn in ("write", "read", "attention"):
         assert call(fn, 2) == _lib.SJVP_ERR_DTYPE
+    for i in (0, 2, 3, 5):
+        for stride in (1 << 32, -16):
+            t = _pages(k_scales=64, v_scales=64)
+            t.page_strides[i] = stride
+            assert lib.sjvp_paged_read(ctypes.byref(t), 0, None) == _lib.SJVP_ERR_PAGES
     for stride, status in ((8, _lib.SJVP_ERR_PAGES), (-16, _lib.SJVP_ERR_PAGES)):
         for i in range(3):
             t = _pages()
