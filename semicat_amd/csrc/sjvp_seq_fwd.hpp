@@ -38,7 +38,8 @@ __device__ __forceinline__ int64_t seq_place(const SeqParams& p, const SeqBlock&
 // 16384^3 product: 1.36), the matrix unit busy 59 % and the vector unit 58 %; 64 sequences of 16 to 128 tokens, 12 heads, D=64, whole, 12.5 us =
 // 2.3 TB/s, where a workgroup is one or two tiles and its start and end.  On pages (eight prompts of 128 to 512 tokens on 2048 to 8192, Hq=16
 // Hkv=4 D=128 e4m3) 166 us and 20 for the join, 0.64 PFLOP/s: a tile of 8-bit numbers goes through registers, with 10 vector instructions to a matrix
-// instruction in place of 7 (16-bit pages, by LDS-DMA, are as fast: 165), and a launch whose workgroups are 2.1 times what runs at once.
+// instruction in place of 7; 16-bit pages, by LDS-DMA, are as fast: with two waves to a SIMD a wave's contractions, exponentials and waits for the next
+// tile stand one behind the other for the most part.
 template <typename T, int HD, bool PAGED, typename FEED>
 __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 4 : 2) void seq_fwd(SeqParams p) {
     if constexpr (FEED::kDma) __builtin_assume(p.D % 8 == 0);
@@ -212,7 +213,8 @@ __device__ __forceinline__ float quarters_sum(float x) {
 // sums of the waves are joined in LDS; with several splits of the keys they go to memory for seq_join.
 //
 // The matrix instructions are 16x16x32 (tile algebra in sjvp_w16.hpp), so that a step of a group of heads, some four to sixteen rows, leaves
-// little of them idle, and a wave needs 128 registers at most: four waves to a SIMD hold twice as many loads in flight as the 32-wide form did.
+// little of them idle, and with one set of rows a wave needs 128 registers (16-bit numbers above D = 96: 162): four (three) waves to a SIMD hold
+// twice as many loads in flight as the 32-wide form did.
 //
 // Bound by memory where sequences are many (a token each of 64 sequences of 2048 to 8192, Hq=16 Hkv=4 D=128 e4m3: 75 us = 4.6 TB/s, a copy makes
 // 5.2), by the latency of offsets, tables and two tiles one behind the other where they are few (four tokens on 29491 and 32769, Hq=16 Hkv=2, 16 bits: 20 us,
