@@ -8,7 +8,7 @@
 
 namespace sjvp {
 
-// The segment that holds a token: the last one that does not begin behind it.
+// The segment that holds a token: the last one that does not begin behind it.  (Of offsets that descend it may begin behind the token or end before it.)
 __device__ __forceinline__ int seq_segment(const SeqParams& p, int token, int lane) {
     int lo = 0, hi = p.B + 2;
     while (hi - lo > 1) {
@@ -64,8 +64,9 @@ __global__ __launch_bounds__(kCtxThreads) void paged_write(SeqParams p) {
     if (token >= p.T) return;
     const int segment = seq_segment(p, token, lane);
     if (segment < 1 || segment > p.B) return;
-    const int first = seq_offset(p, segment), keys = min(max(p.lengths[segment - 1], 0), p.pages.capacity);
-    const int position = keys - max(0, seq_offset(p, segment + 1) - first) + token - first;
+    const int first = seq_offset(p, segment), end = seq_offset(p, segment + 1), keys = min(max(p.lengths[segment - 1], 0), p.pages.capacity);
+    if (token < first || token >= end) return;  // (offsets that descend; a position would lie behind the length, and its page outside the table)
+    const int position = keys - (end - first) + token - first;
     if (position < 0) return;
     const int at = p.pages.page_of(position), page = p.pages.table[(segment - 1) * p.pages.table_stride + at], row = position - at * p.pages.size;
     if ((uint32_t)page >= (uint32_t)p.pages.pages) return;
