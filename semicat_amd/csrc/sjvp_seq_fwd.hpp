@@ -435,7 +435,7 @@ __global__ __launch_bounds__(64 * WAVES, NC == 1 ? (E4M3 || HD <= 96 ? 4 : 3) : 
                 continue;
             }
         }
-        const float f = sum == 0.0f || top == -INFINITY ? 0.0f : 1.0f / sum;
+        const float f = sum == 0.0f ? 0.0f : 1.0f / sum;  // (a row that sees nothing sums to exactly zero; of scores that are all NaN the maximum is none either)
         u32x4 r;
 #pragma unroll
         for (int j = 0; j < 4; ++j) r[j] = T::pack2(f == 0.0f ? 0.0f : o[2 * j] * f, f == 0.0f ? 0.0f : o[2 * j + 1] * f);
@@ -496,7 +496,7 @@ __global__ __launch_bounds__(kCtxThreads) void seq_join(SeqParams p) {
         const float* other = met[group + s][threadIdx.x & 15];
         add(other[0], other[1], other + 2);
     }
-    const float f = sum == 0.0f || top == -INFINITY ? 0.0f : 1.0f / sum;
+    const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
     u32x4 o;
 #pragma unroll
     for (int j = 0; j < 4; ++j) o[j] = T::pack2(f == 0.0f ? 0.0f : y[2 * j] * f, f == 0.0f ? 0.0f : y[2 * j + 1] * f);

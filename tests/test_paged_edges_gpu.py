@@ -1,9 +1,9 @@
-"""The paged cache where a call's description of its sequences ends: offsets that descend."""
+"""The paged cache where a call's description of its sequences ends, offsets that descend, and NaN among what a row does see."""
 import pytest
 import torch
 
 from semicat_amd import paged_attention, paged_write
-from tests.test_paged_gpu import BF16, cache_of, ints, normal
+from tests.test_paged_gpu import BF16, attend, cache_of, ints, normal, offsets_of, tables_of
 
 pytestmark = pytest.mark.gpu
 
@@ -33,3 +33,61 @@ def test_offsets_that_descend_reach_no_other_pages(offsets, quantized):
         o = paged_attention(normal(T, 4, 64, dtype=BF16, seed=3).cuda(), pages, tables, ints(held), ints(offsets))
         torch.cuda.synchronize()
         assert o.shape == (T, 4, 64)
+
+
+NAN_CASES = [  # held, new, heads, group, head dimension
+    ([1, 7, 33, 0, 64, 257], None, 4, 2, 64),                                # seq_few, whole
+    ([1, 40, 17], [1, 6, 5], 4, 4, 128),
+    ([5000, 1, 3000, 700], None, 8, 4, 128),                                 # split
+    ([4000, 6, 900], [4, 9, 2], 8, 2, 64),                                   # (more new tokens than are held)
+    ([30] * 40, [20] * 40, 4, 1, 48),                                        # workgroups of one wave
+    ([900, 17, 1400], [300, 17, 200], 8, 2, 64),                             # blocks of 128 rows
+    ([8000, 5000], [700, 500], 32, 4, 128),                                  # split
+    ([5000, 1, 3333, 900, 2048, 2], [1000, 1, 900, 700, 17, 2], 16, 4, 64),  # both launches
+]
+
+
+@pytest.mark.parametrize("quantized", [True, False])
+@pytest.mark.parametrize("held,new,H,G,D", NAN_CASES)
+def test_nan_queries_have_nan_results(held, new, H, G, D, quantized):
+    """A NaN in a query makes all of its scores NaN: its result is NaN, in whichever launch and split, and zero only where it sees nothing."""
+    pages = sum(-(-n // 16) for n in held) + 3
+    cache = cache_of(pages, 16, H // G, D, BF16, quantized)
+    tables = tables_of(held, 16, pages)
+    offsets = offsets_of(new or [1] * len(held))
+    q = normal(offsets[-1], H, D, dtype=BF16)
+    want = attend(cache, q, tables, held, new and offsets)
+    seen, spoilt = torch.zeros(q.shape[:2], dtype=torch.bool), torch.zeros(q.shape[:2], dtype=torch.bool)
+    for b, n in enumerate(held):
+        count = offsets[b + 1] - offsets[b]
+        for i in range(count):
+            seen[offsets[b] + i] = n - count + i >= 0
+        for i in {0, count // 2, count - 1}:
+            spoilt[offsets[b] + i, (b + i) % H] = True
+    q[spoilt, D // 2] = float("nan")
+    got = attend(cache, q, tables, held, new and offsets)
+    assert got[spoilt & seen].isnan().all() and not got[~seen].any()
+    assert torch.equal(got[~spoilt], want[~spoilt])
+
+
+@pytest.mark.parametrize("quantized", [True, False])
+@pytest.mark.parametrize("held,new,H,G,D", NAN_CASES)
+def test_rows_whose_keys_are_all_nan(held, new, H, G, D, quantized):
+    """A sequence with NaN in all its keys, one of one key among them, has NaN results; the others keep theirs."""
+    pages = sum(-(-n // 16) for n in held) + 3
+    cache = cache_of(pages, 16, H // G, D, BF16, quantized)
+    tables = tables_of(held, 16, pages)
+    offsets = offsets_of(new or [1] * len(held))
+    q = normal(offsets[-1], H, D, dtype=BF16)
+    want = attend(cache, q, tables, held, new and offsets)
+    bad = torch.tensor([0x7f], dtype=torch.uint8) if quantized else torch.tensor([float("nan")], dtype=BF16)
+    nan = torch.zeros(offsets[-1], dtype=torch.bool)
+    for b, n in enumerate(held):
+        if b % 2 == 0:
+            mine = tables[b, :-(-n // 16)].long().cuda()
+            (cache.k.view(torch.uint8) if quantized else cache.k)[mine, :, :, 3] = bad.cuda()
+            count = offsets[b + 1] - offsets[b]
+            for i in range(count):
+                nan[offsets[b] + i] = n - count + i >= 0
+    got = attend(cache, q, tables, held, new and offsets)
+    assert got[nan].isnan().all() and torch.equal(got[~nan], want[~nan])
