@@ -378,7 +378,8 @@ int sjvp_packed_bwd(const sjvp_packed* t, int dtype, void* stream);
  * page_strides[3..5].  Rows of k_pages and v_pages start on 16-byte boundaries; strides between pages and between rows are below 2^32.
  *   tables   device array [B][table_pages] with the row stride table_stride: position x of sequence b stands in row x % page_size of page
  *       tables[b][x / page_size].  A number that is none of the cache's pages reads as zeros and takes no writes.
- *   lengths  device array [B]: the tokens that the cache holds of a sequence, those of the call among them; clamped to what the table has.
+ *   lengths  device array [B]: the tokens that the cache holds of a sequence, those of the call among them.  Positions that the table has not
+ *       (from table_pages * page_size on, at most 2^29) take no writes and hold no keys.
  *   offsets  as above, of the call's new tokens: the last offsets[b+1] - offsets[b] ones of sequence b.  NULL: T = B, one each.
  * sjvp_paged_write: k, v [T,Hkv,D] (strides (head, row) of SJVP_P_K, SJVP_P_V) to their places in the pages.  A page that is written to belongs to
  *   one sequence.  8 bits: the exponent of 32 columns is the least one by which none of their finite numbers goes beyond 448, within -117 .. 120

@@ -64,10 +64,10 @@ __global__ __launch_bounds__(kCtxThreads) void paged_write(SeqParams p) {
     if (token >= p.T) return;
     const int segment = seq_segment(p, token, lane);
     if (segment < 1 || segment > p.B) return;
-    const int first = seq_offset(p, segment), end = seq_offset(p, segment + 1), keys = min(max(p.lengths[segment - 1], 0), p.pages.capacity);
+    const int first = seq_offset(p, segment), end = seq_offset(p, segment + 1), length = max(p.lengths[segment - 1], 0);
     if (token < first || token >= end) return;  // (offsets that descend; a position would lie behind the length, and its page outside the table)
-    const int position = keys - (end - first) + token - first;
-    if (position < 0) return;
+    const int position = length - (end - first) + token - first;
+    if (position < 0 || position >= p.pages.capacity) return;
     const int at = p.pages.page_of(position), page = p.pages.table[(segment - 1) * p.pages.table_stride + at], row = position - at * p.pages.size;
     if ((uint32_t)page >= (uint32_t)p.pages.pages) return;
     constexpr int kColumns = E4M3 ? 16 : 8;

@@ -185,8 +185,9 @@ struct SeqKeys {
     __device__ __forceinline__ SeqKeys(const SeqParams& p, const SeqBlock& b) {
         const bool sequence = b.segment >= 1 && b.segment <= p.B;
         if constexpr (PAGED) {
-            keys = sequence ? min(max(b.held, 0), p.pages.capacity) : 0;
-            start = keys - b.tokens;
+            const int length = sequence ? max(b.held, 0) : 0;
+            keys = min(length, p.pages.capacity);
+            start = length - b.tokens;  // (a length beyond the table: the positions that the table has not hold no keys)
         } else {
             keys = sequence ? b.tokens : 0;
             start = 0;

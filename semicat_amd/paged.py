@@ -8,8 +8,8 @@ olsdavis/semicat, which generates whole sequences.
 All of them take the same description of the sequences: ``tables`` (int32 ``[B,P]``, position ``x`` of sequence ``b`` stands in row
 ``x % page_size`` of page ``tables[b, x // page_size]``), ``lengths`` (int32 ``[B]``, the tokens of each sequence with those of the call) and
 ``offsets`` (int32 ``[B+1]``, where the call's new tokens of each sequence stand in its ``[T,...]`` tensors, as in
-:func:`semicat_amd.packed_attention`; None: one token of each sequence).  A page number that the cache has not reads as zeros and takes no writes.
-The host looks at none of them.  None of the ops has a gradient.
+:func:`semicat_amd.packed_attention`; None: one token of each sequence).  A page number that the cache has not reads as zeros and takes no writes;
+positions behind the end of a table (a length of more than ``P * page_size``) take no writes and hold no keys.  The host looks at none of them.  None of the ops has a gradient.
 """
 from __future__ import annotations
 

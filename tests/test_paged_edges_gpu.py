@@ -1,9 +1,10 @@
-"""The paged cache where a call's description of its sequences ends, offsets that descend, and NaN among what a row does see."""
+"""The paged cache where a call's description of its sequences ends, offsets that descend and lengths beyond the table, and NaN among what a row does see."""
 import pytest
 import torch
 
-from semicat_amd import paged_attention, paged_write
-from tests.test_paged_gpu import BF16, attend, cache_of, ints, normal, offsets_of, tables_of
+from oracle import packed_oracle as orc
+from semicat_amd import paged_attention, paged_read, paged_write
+from tests.test_paged_gpu import BF16, attend, cache_of, held_rows, ints, normal, offsets_of, tables_of
 
 pytestmark = pytest.mark.gpu
 
@@ -91,3 +92,37 @@ def test_rows_whose_keys_are_all_nan(held, new, H, G, D, quantized):
                 nan[offsets[b] + i] = n - count + i >= 0
     got = attend(cache, q, tables, held, new and offsets)
     assert got[nan].isnan().all() and torch.equal(got[~nan], want[~nan])
+
+
+@pytest.mark.parametrize("quantized", [True, False])
+@pytest.mark.parametrize("more,new", [((1, 0, 3), (1, 1, 1)), ((5, 2, 0), (4, 9, 30)), ((100, 1, 1 << 30), (100, 40, 60)), ((0, 60, 0), (0, 64, 1))])
+def test_tokens_behind_their_table(more, new, quantized):
+    """A token has the position length - n + i, also where the length goes beyond the table: behind its end it is not written, and what stands in the
+    table stays; its query sees all of the table, one within it the positions up to its own."""
+    size, H, D, room = 8, 2, 64, 64
+    cache = cache_of(26, size, H, D, BF16, quantized)
+    tables = torch.randperm(26, generator=torch.Generator().manual_seed(5))[:24].view(3, 8).int()
+    held, offsets = [room + m for m in more], offsets_of(new)
+    k, v = normal(sum(new), H, D, dtype=BF16), normal(sum(new), H, D, dtype=BF16, seed=2)
+    want = bits(cache)
+    paged_write(cache, k.cuda(), v.cuda(), tables.cuda(), ints(held), ints(offsets))
+    for b, n in enumerate(new):
+        for i in range(n):
+            x = held[b] - n + i
+            if x < room:
+                page, row = int(tables[b, x // size]), x % size
+                for j, numbers in enumerate((k[offsets[b] + i], v[offsets[b] + i])):
+                    if quantized:
+                        want[j][page, :, row], want[2 + j][page, :, row] = orc.quantise(numbers)
+                    else:
+                        want[j][page, :, row] = numbers.contiguous().view(torch.uint8)
+    assert all(torch.equal(a, b) for a, b in zip(bits(cache), want))
+    rows = {which: held_rows(cache, tables, [room] * 3, which) for which in "kv"}
+    for got, which in zip(paged_read(cache, tables.cuda(), ints(held), room + 2), "kv"):
+        assert not got[:, room:].any()
+        assert all(torch.equal(got[b, :room].cpu().double(), rows[which][b]) for b in range(3))
+    for H in (4, 16):
+        q = normal(sum(new), H, D, dtype=BF16, seed=7)
+        got = attend(cache, q, tables, held, offsets)
+        value, sizes = orc.paged(q, rows["k"], rows["v"], held, offsets)
+        assert bool(((got.double() - value).abs() <= orc.limit(value, sizes, BF16)).all())
