@@ -949,6 +949,10 @@ PyObject* packed(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+bool wants_gradient(const Tensor& x) { return x.requires_grad() && at::GradMode::is_enabled(); }
+// (raised by the general form)
+bool differentiated(const Tensor& x) { return wants_gradient(x) || x._fw_grad(0).defined(); }
+
 // The cache and the sequences of a paged call: a = k, v, k_scales, v_scales, dtype, tables, lengths, offsets (all but the first two, dtype,
 // tables and lengths may be None).  T: the call's rows, negative where it has none.
 struct PagedCall {
@@ -960,7 +964,7 @@ struct PagedCall {
         const Tensor *k = plain(a[0]), *v = plain(a[1]);
         const bool scaled = a[2] != Py_None;
         if (!k || !v || k->dim() != 4 || k->sizes() != v->sizes() || k->stride(3) != 1 || v->stride(3) != 1 || k->device() != v->device() ||
-            k->scalar_type() != v->scalar_type() || scaled != (a[3] != Py_None) || !THPDtype_Check(a[4]))
+            k->scalar_type() != v->scalar_type() || scaled != (a[3] != Py_None) || !THPDtype_Check(a[4]) || differentiated(*k) || differentiated(*v))
             return false;
         dtype = reinterpret_cast<THPDtype*>(a[4])->scalar_type, device = k->device();
         if ((dtype != at::kBFloat16 && dtype != at::kHalf) || k->scalar_type() != (scaled ? at::kFloat8_e4m3fn : dtype)) return false;
@@ -977,7 +981,9 @@ struct PagedCall {
         if (scaled) {
             const Tensor* s[2] = {plain(a[2]), plain(a[3])};
             for (const Tensor* x : s) {
-                if (!x || x->dim() != 4 || x->device() != device || x->element_size() != 1 || x->stride(3) != 1 || x->size(3) != (k->size(3) + 31) / 32) return false;
+                if (!x || x->dim() != 4 || x->device() != device || x->element_size() != 1 || x->stride(3) != 1 || x->size(3) != (k->size(3) + 31) / 32 ||
+                    differentiated(*x))
+                    return false;
                 for (int d : dims)
                     if (x->size(d) != k->size(d) || place(*x, d) != place(*s[0], d)) return false;
             }
@@ -1010,8 +1016,6 @@ struct PagedCall {
     void put(int at, const Tensor& x) { t.strides[3 * at] = x.stride(1), t.strides[3 * at + 1] = x.stride(0); }
     void* stream() const { return c10::hip::getCurrentHIPStream(device.index()).stream(); }
 };
-
-bool wants_gradient(const Tensor& x) { return x.requires_grad() && at::GradMode::is_enabled(); }
 
 // paged_attention(q, cache and sequences as PagedCall takes them, scale) -> output
 PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {

@@ -9,7 +9,8 @@ All of them take the same description of the sequences: ``tables`` (int32 ``[B,P
 ``x % page_size`` of page ``tables[b, x // page_size]``), ``lengths`` (int32 ``[B]``, the tokens of each sequence with those of the call) and
 ``offsets`` (int32 ``[B+1]``, where the call's new tokens of each sequence stand in its ``[T,...]`` tensors, as in
 :func:`semicat_amd.packed_attention`; None: one token of each sequence).  A page number that the cache has not reads as zeros and takes no writes;
-positions behind the end of a table (a length of more than ``P * page_size``) take no writes and hold no keys.  The host looks at none of them.  None of the ops has a gradient.
+positions behind the end of a table (a length of more than ``P * page_size``) take no writes and hold no keys.  The host looks at none of them.  None of the ops has a gradient: with an input, or a tensor of the
+cache, that requires one they raise, as they do with forward-mode tangents.
 """
 from __future__ import annotations
 
@@ -152,8 +153,8 @@ def _launch(fn: str, t: _lib.Paged, cache: PagedCache) -> None:
         _lib.check(getattr(lib, fn)(ctypes.byref(t), _DTYPES[cache.dtype], stream))
 
 
-def _no_gradient(what: str, *tensors: Tensor) -> None:
-    for t in tensors:
+def _no_gradient(what: str, cache: PagedCache, *tensors: Tensor) -> None:
+    for t in (*tensors, *(x for x in cache._storage()[:4] if x is not None)):
         if fwAD.unpack_dual(t).tangent is not None:
             raise NotImplementedError(f"forward mode of {what} is not implemented")
         if t.requires_grad and torch.is_grad_enabled():
@@ -169,7 +170,7 @@ def paged_write(cache: PagedCache, k: Tensor, v: Tensor, tables: Tensor, lengths
         status = _lib.host().paged_write(k, v, *cache._storage(), tables, lengths, offsets)
         if status is not None:
             return _lib.check(status)
-    _no_gradient("paged_write", k, v)
+    _no_gradient("paged_write", cache, k, v)
     if k.ndim != 3:
         raise AssertionError(f"k must have three dimensions, got {tuple(k.shape)}")
     t = _describe(cache, tables, lengths, offsets, k.shape[0])
@@ -194,6 +195,7 @@ def paged_read(cache: PagedCache, tables: Tensor, lengths: Tensor, size: int) ->
         both = _lib.host().paged_read(*cache._storage(), tables, lengths, None, size)
         if both is not None:
             return _host_result(both)
+    _no_gradient("paged_read", cache)
     t = _describe(cache, tables, lengths, None, -1)
     t.size = size
     k, v = (torch.empty((tables.shape[0], size, cache.heads, cache.head_dim), device=cache.k.device, dtype=cache.dtype) for _ in range(2))
@@ -216,7 +218,7 @@ def paged_attention(q: Tensor, cache: PagedCache, tables: Tensor, lengths: Tenso
         o = _lib.host().paged_attention(q, *cache._storage(), tables, lengths, offsets, scale)
         if o is not None:
             return _host_result(o)
-    _no_gradient("paged_attention", q)
+    _no_gradient("paged_attention", cache, q)
     dtype = q.dtype
     q = q if dtype == cache.dtype else q.to(cache.dtype)
     _check_query(q)

@@ -1,0 +1,62 @@
+"""CPU tests of the packed sequences and the paged cache: gradients that are not there raise."""
+import pytest
+import torch
+import torch.autograd.forward_ad as fwAD
+
+from semicat_amd import PagedCache, paged, paged_attention, paged_read, paged_write
+from tests.test_packed import BF16, E8, FP8, _Gpu, _i, _q, _t
+
+
+@pytest.fixture(autouse=True)
+def _general_form(monkeypatch):
+    monkeypatch.setattr(paged, "_on_gpu", lambda q: False)
+
+
+def _storage(scales):
+    if not scales:
+        return [_t(4, 2, 8, 32), _t(4, 2, 8, 32)]
+    return [torch.zeros(4, 2, 8, d, dtype=torch.uint8).view(t).as_subclass(_Gpu) for d, t in ((32, FP8), (32, FP8), (1, E8), (1, E8))]
+
+
+CALLS = {"attention": lambda cache: paged_attention(_q(), cache, _i(3, 2), _i(3), _i(4)), "read": lambda cache: paged_read(cache, _i(3, 2), _i(3), 4),
+         "write": lambda cache: paged_write(cache, _q(), _q(), _i(3, 2), _i(3), _i(4))}
+
+
+@pytest.mark.parametrize("which", range(2))
+@pytest.mark.parametrize("call", CALLS)
+@pytest.mark.parametrize("scales", [False, True])
+def test_no_gradient_through_the_cache(monkeypatch, call, scales, which):
+    launched = []
+    monkeypatch.setattr(paged, "_launch", lambda *a: launched.append(a))
+    tensors = _storage(scales)
+    tensors[which].requires_grad_()
+    cache = PagedCache.of(*tensors)
+    with pytest.raises(NotImplementedError):
+        CALLS[call](cache)
+    assert not launched
+    with torch.no_grad():
+        CALLS[call](cache)
+    assert len(launched) == 1
+
+
+@pytest.mark.parametrize("which", range(2))
+@pytest.mark.parametrize("call", CALLS)
+def test_no_forward_mode_through_the_cache(monkeypatch, call, which):
+    monkeypatch.setattr(paged, "_launch", lambda *a: pytest.fail("launched"))
+    tensors = [torch.zeros(4, 2, 8, 32, dtype=BF16) for _ in range(2)]
+    with fwAD.dual_level():
+        tensors[which] = fwAD.make_dual(tensors[which], torch.ones_like(tensors[which]))
+        cache = PagedCache.of(*tensors)
+        with pytest.raises(NotImplementedError):
+            CALLS[call](cache)
+
+
+def test_dual_levels_without_tangents(monkeypatch):
+    """Tensors of 8 bits have none, and are looked at all the same."""
+    launched = []
+    monkeypatch.setattr(paged, "_launch", lambda *a: launched.append(a))
+    with fwAD.dual_level():
+        for call in CALLS.values():
+            for scales in (False, True):
+                call(PagedCache.of(*_storage(scales)))
+    assert len(launched) == 6

@@ -1,9 +1,10 @@
-"""The paged cache where a call's description of its sequences ends, offsets that descend and lengths beyond the table, and NaN among what a row does see."""
+"""The paged cache at its edges: offsets that descend, lengths beyond the table, NaN among what a row sees, gradients that are not there."""
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 
 from oracle import packed_oracle as orc
-from semicat_amd import paged_attention, paged_read, paged_write
+from semicat_amd import paged, paged_attention, paged_read, paged_write
 from tests.test_paged_gpu import BF16, attend, cache_of, held_rows, ints, normal, offsets_of, tables_of
 
 pytestmark = pytest.mark.gpu
@@ -126,3 +127,33 @@ def test_tokens_behind_their_table(more, new, quantized):
         got = attend(cache, q, tables, held, offsets)
         value, sizes = orc.paged(q, rows["k"], rows["v"], held, offsets)
         assert bool(((got.double() - value).abs() <= orc.limit(value, sizes, BF16)).all())
+
+
+@pytest.mark.parametrize("quantized", [True, False])
+@pytest.mark.parametrize("name", ["k", "v"])
+def test_no_gradient_through_the_cache(monkeypatch, name, quantized):
+    """A cache whose tensors require gradients, or have tangents, is refused, by the host extension as by the general form; without recording it serves."""
+    cache = cache_of(3, 16, 2, 64, BF16, quantized)
+    tables, lengths, q, k = ints([[0, 1, 2]]), ints([40]), normal(1, 4, 64, dtype=BF16).cuda(), normal(1, 2, 64, dtype=BF16).cuda()
+    calls = (lambda: paged_write(cache, k, k, tables, lengths), lambda: paged_attention(q, cache, tables, lengths),
+             lambda: paged_read(cache, tables, lengths, 40)[0])
+    want = [call() for call in calls]
+    pages = getattr(cache, name)
+    for general in (False, True):
+        if general:
+            monkeypatch.setattr(paged, "_on_gpu", lambda q: False)
+        pages.requires_grad_()
+        for call in calls:
+            with pytest.raises(NotImplementedError):
+                call()
+        with torch.no_grad():
+            got = [call() for call in calls]
+        assert torch.equal(got[1], want[1]) and torch.equal(got[2], want[2])
+        pages.requires_grad_(False)
+        if not quantized:
+            with fwAD.dual_level():
+                setattr(cache, name, fwAD.make_dual(pages, torch.ones_like(pages)))
+                for call in calls:
+                    with pytest.raises(NotImplementedError):
+                        call()
+                setattr(cache, name, pages)
