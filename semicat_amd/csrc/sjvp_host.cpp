@@ -959,6 +959,7 @@ struct PagedCall {
     sjvp_paged t{};
     at::ScalarType dtype = at::kBFloat16;
     c10::Device device{c10::kCPU};
+    const Tensor* storage[4] = {};  // k, v, k_scales, v_scales
 
     bool take(PyObject* const* a, int64_t T) {
         const Tensor *k = plain(a[0]), *v = plain(a[1]);
@@ -978,6 +979,7 @@ struct PagedCall {
             t.page_strides[d] = place(*k, d) * item;
         }
         t.k_pages = k->data_ptr(), t.v_pages = v->data_ptr();
+        storage[0] = k, storage[1] = v;
         if (scaled) {
             const Tensor* s[2] = {plain(a[2]), plain(a[3])};
             for (const Tensor* x : s) {
@@ -989,6 +991,7 @@ struct PagedCall {
             }
             for (int d : dims) t.page_strides[3 + d] = place(*s[0], d);
             t.k_scales = s[0]->data_ptr(), t.v_scales = s[1]->data_ptr();
+            storage[2] = s[0], storage[3] = s[1];
         }
         t.pages = static_cast<int>(k->size(0)), t.Hkv = static_cast<int>(k->size(1)), t.page_size = static_cast<int>(k->size(2)), t.D = static_cast<int>(k->size(3));
         t.Hq = t.Hkv;
@@ -1015,6 +1018,11 @@ struct PagedCall {
     bool rows(const Tensor& x, int64_t heads) const { return x.scalar_type() == dtype && x.device() == device && x.size(1) == heads && x.size(2) == t.D; }
     void put(int at, const Tensor& x) { t.strides[3 * at] = x.stride(1), t.strides[3 * at + 1] = x.stride(0); }
     void* stream() const { return c10::hip::getCurrentHIPStream(device.index()).stream(); }
+    // a change in place, for what autograd has saved of the cache's tensors
+    void changed() const {
+        for (const Tensor* x : storage)
+            if (x && !x->is_inference()) x->unsafeGetTensorImpl()->bump_version();
+    }
 };
 
 // paged_attention(q, cache and sequences as PagedCall takes them, scale) -> output
@@ -1057,7 +1065,9 @@ PyObject* paged_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const c10::DeviceGuard guard(call.device);
     call.t.k = k->data_ptr(), call.t.v = v->data_ptr();
     call.put(SJVP_P_K, *k), call.put(SJVP_P_V, *v);
-    return PyLong_FromLong(abi.paged_write(&call.t, type_tag(call.dtype), call.stream()));
+    const int status = abi.paged_write(&call.t, type_tag(call.dtype), call.stream());
+    if (status == SJVP_OK) call.changed();
+    return PyLong_FromLong(status);
     END_HANDLE_TH_ERRORS
 }
 

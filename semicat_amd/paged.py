@@ -165,7 +165,7 @@ def _no_gradient(what: str, cache: PagedCache, *tensors: Tensor) -> None:
 def paged_write(cache: PagedCache, k: Tensor, v: Tensor, tables: Tensor, lengths: Tensor, offsets: Optional[Tensor] = None) -> None:
     """Writes the new tokens' ``k`` and ``v`` ``[T,Hkv,D]`` to the last positions of their sequences: token ``i`` of ``n`` new ones of a
     sequence has the position ``length - n + i``.  A page that is written to must belong to one sequence.  Tensors of another type than the cache's are
-    rounded to it first."""
+    rounded to it first.  The cache's tensors count as changed in place."""
     if _on_gpu(k):
         status = _lib.host().paged_write(k, v, *cache._storage(), tables, lengths, offsets)
         if status is not None:
@@ -185,6 +185,8 @@ def paged_write(cache: PagedCache, k: Tensor, v: Tensor, tables: Tensor, lengths
         return
     _put(t, 2, k), _put(t, 3, v)
     _launch("sjvp_paged_write", t, cache)
+    # (a change in place, for what autograd has saved of these tensors)
+    torch.autograd.graph.increment_version([x for x in cache._storage()[:4] if x is not None])
 
 
 @torch._dynamo.disable

@@ -1,4 +1,4 @@
-"""CPU tests of the packed sequences and the paged cache: gradients that are not there raise."""
+"""CPU tests of the packed sequences and the paged cache: gradients that are not there raise, a write is a change in place."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fwAD
@@ -60,3 +60,20 @@ def test_dual_levels_without_tangents(monkeypatch):
             for scales in (False, True):
                 call(PagedCache.of(*_storage(scales)))
     assert len(launched) == 6
+
+
+@pytest.mark.parametrize("scales", [False, True])
+def test_a_write_counts_as_a_change_in_place(monkeypatch, scales):
+    monkeypatch.setattr(paged, "_launch", lambda *a: None)
+    tensors = _storage(scales)
+    cache = PagedCache.of(*tensors)
+    versions = lambda: [t._version for t in tensors]
+    before = versions()
+    paged_attention(_q(), cache, _i(3, 2), _i(3), _i(4)), paged_read(cache, _i(3, 2), _i(3), 4)
+    paged_write(cache, _q(T=0), _q(T=0), _i(3, 2), _i(3), _i(4))
+    assert versions() == before
+    paged_write(cache, _q(), _q(), _i(3, 2), _i(3), _i(4))
+    assert all(now > was for now, was in zip(versions(), before))
+    with torch.inference_mode():
+        kept = PagedCache.of(*_storage(scales))  # (such tensors have no count)
+        paged_write(kept, _q(), _q(), _i(3, 2), _i(3), _i(4))

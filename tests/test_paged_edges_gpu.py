@@ -1,10 +1,11 @@
-"""The paged cache at its edges: offsets that descend, lengths beyond the table, NaN among what a row sees, gradients that are not there."""
+"""The paged cache at its edges: offsets that descend, lengths beyond the table, NaN among what a row sees, gradients that are not there, the count of
+changes in place."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fwAD
 
 from oracle import packed_oracle as orc
-from semicat_amd import paged, paged_attention, paged_read, paged_write
+from semicat_amd import PagedCache, paged, paged_attention, paged_read, paged_write
 from tests.test_paged_gpu import BF16, attend, cache_of, held_rows, ints, normal, offsets_of, tables_of
 
 pytestmark = pytest.mark.gpu
@@ -157,3 +158,31 @@ def test_no_gradient_through_the_cache(monkeypatch, name, quantized):
                     with pytest.raises(NotImplementedError):
                         call()
                 setattr(cache, name, pages)
+
+
+@pytest.mark.parametrize("quantized", [True, False])
+@pytest.mark.parametrize("general", [False, True])
+def test_a_write_counts_as_a_change_in_place(monkeypatch, general, quantized):
+    """What autograd has saved of a cache's tensors, or of what they are views of, is not used after a write has changed it."""
+    if general:
+        monkeypatch.setattr(paged, "_on_gpu", lambda q: False)
+    cache = cache_of(3, 16, 2, 64, BF16, quantized)
+    tables, lengths, k = ints([[0, 1, 2]]), ints([40]), normal(1, 2, 64, dtype=BF16).cuda()
+    tensors = [t for t in (cache.k, cache.v, cache.k_scales, cache.v_scales) if t is not None]
+    before = [t._version for t in tensors]
+    paged_read(cache, tables, lengths, 40), paged_attention(normal(1, 4, 64, dtype=BF16).cuda(), cache, tables, lengths)
+    assert [t._version for t in tensors] == before
+    paged_write(cache, k, k, tables, lengths)
+    assert all(t._version > n for t, n in zip(tensors, before))
+    if not quantized:
+        room = torch.zeros(2, 3, 2, 16, 64, dtype=BF16, device="cuda")
+        views = PagedCache.of(room[0], room[1])
+        weight = torch.ones((), dtype=BF16, device="cuda", requires_grad=True)
+        y = (room * weight).float().sum()
+        paged_write(views, k, k, tables, lengths)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    with torch.inference_mode():
+        kept = PagedCache(3, 16, 2, 64, BF16, quantized)
+    paged_write(kept, k, k, tables, lengths)  # (its tensors have no count)
+    assert paged_read(kept, tables, lengths, 40)[0][0, 39].any()
