@@ -125,6 +125,8 @@ def packed_backward(q: Tensor, k: Tensor, v: Tensor, o: Tensor, lse: Tensor, dO:
     dq, dk, dv = _like(q), *((_like(k), _like(v)) if with_keys else (None, None))
     if q.numel():
         _call(True, (q, k, v, o, dO, dq, dk, dv), lse, offsets, causal, scale)
+    elif with_keys:
+        dk.zero_(), dv.zero_()  # (keys that no query reads)
     return dq, dk, dv
 
 

@@ -1,9 +1,9 @@
-"""CPU tests of the packed sequences and the paged cache: gradients that are not there raise, a write is a change in place."""
+"""CPU tests of the packed sequences and the paged cache: gradients that are not there raise, a write is a change in place, calls without query rows."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fwAD
 
-from semicat_amd import PagedCache, paged, paged_attention, paged_read, paged_write
+from semicat_amd import PagedCache, packed, packed_attention, packed_backward, packed_forward, paged, paged_attention, paged_read, paged_write
 from tests.test_packed import BF16, E8, FP8, _Gpu, _i, _q, _t
 
 
@@ -77,3 +77,30 @@ def test_a_write_counts_as_a_change_in_place(monkeypatch, scales):
     with torch.inference_mode():
         kept = PagedCache.of(*_storage(scales))  # (such tensors have no count)
         paged_write(kept, _q(), _q(), _i(3, 2), _i(3), _i(4))
+
+
+@pytest.fixture
+def filled_memory():
+    """New tensors hold NaN until they are written."""
+    torch.use_deterministic_algorithms(True)
+    yield
+    torch.use_deterministic_algorithms(False)
+
+
+@pytest.mark.parametrize("H,T", [(0, 6), (0, 0), (2, 0)])
+def test_calls_without_query_rows(filled_memory, H, T):
+    """Keys that no query reads have gradients of zero."""
+    q, k = _q(T=T, H=H), _q(T=T)
+    o, lse = packed_forward(q, k, k, _i(2))
+    assert o.shape == (T, H, 32) and lse.shape == (H, T, 2)
+    dq, dk, dv = packed_backward(q, k, k, o, lse.as_subclass(_Gpu), _q(T=T, H=H), _i(2))
+    assert dq.shape == q.shape and dk.shape == dv.shape == k.shape
+    assert not dk.any() and not dv.any()
+    assert packed_backward(q, k, k, o, lse.as_subclass(_Gpu), _q(T=T, H=H), _i(2), with_keys=False)[1:] == (None, None)
+
+
+def test_training_without_query_heads(filled_memory, monkeypatch):
+    monkeypatch.setattr(packed, "_on_gpu", lambda q: False)
+    q, k, v = (_q(T=6, H=h).requires_grad_() for h in (0, 2, 2))
+    grads = torch.autograd.grad(packed_attention(q, k, v, _i(2)).float().sum(), [q, k, v])
+    assert [g.shape for g in grads] == [t.shape for t in (q, k, v)] and not any(g.any() for g in grads)
