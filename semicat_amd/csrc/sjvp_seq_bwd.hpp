@@ -123,7 +123,7 @@ __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 3 : 2) void seq_bwd_row(Seq
     int step = kBytes;
     const auto tile = [&](int t, auto masked) {
         const int key = t * kCtxTile;
-        const bool more = t + 1 < nt;
+        const bool more = t + 1 < nt && !at_once;  // (both tiles of a short block are there, and other waves may still read the second one for delta)
         if (more) feed.request(p, t + 1, n, k_place(t + 1), v_place(t + 1), wave);
         f32x16 s[2], ds[2];
         s[0] = s[1] = ds[0] = ds[1] = f32x16{};
