@@ -349,7 +349,7 @@ __global__ __launch_bounds__(kCtxThreads, 2) void seq_bwd_col(SeqParams p) {
 }
 
 // The same above D = 64, where the sums and operands of 32 keys are more than the registers of two waves to a SIMD: K and V stand in LDS, and a group
-// of 32 keys has two waves, with 32 rows of a tile each, whose sums are added up in the end.  One workgroup to a compute unit (134 KB of LDS).  The
+// of 32 keys has two waves, with 32 rows of a tile each, whose sums are added up in the end.  One workgroup to a compute unit (133 KB of LDS).  The
 // sequences above at D=128: 655 us = 0.85 PFLOP/s, the matrix unit busy 44 %, LDS the most of the rest: five reads to two matrix instructions, none
 // of which meets another in a bank.  (K and V in registers with eight waves: 982 us, spills.)
 template <typename T, int HD, bool DMA>

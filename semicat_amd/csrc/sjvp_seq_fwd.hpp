@@ -38,7 +38,7 @@ __device__ __forceinline__ int64_t seq_place(const SeqParams& p, const SeqBlock&
 // 16384^3 product: 1.36), the matrix unit busy 59 % and the vector unit 58 %; 64 sequences of 16 to 128 tokens, 12 heads, D=64, whole, 12.5 us =
 // 2.3 TB/s, where a workgroup is one or two tiles and its start and end.  On pages (eight prompts of 128 to 512 tokens on 2048 to 8192, Hq=16
 // Hkv=4 D=128 e4m3) 166 us and 20 for the join, 0.64 PFLOP/s: a tile of 8-bit numbers goes through registers, with 10 vector instructions to a matrix
-// instruction in place of 7; 16-bit pages, by LDS-DMA, are as fast: with two waves to a SIMD a wave's contractions, exponentials and waits for the next
+// instruction in place of 7; 16-bit pages, by LDS-DMA, take 171 us in place of 180 with the join: with two waves to a SIMD a wave's contractions, exponentials and waits for the next
 // tile stand one behind the other for the most part.
 template <typename T, int HD, bool PAGED, typename FEED>
 __global__ __launch_bounds__(kCtxThreads, HD <= 64 ? 4 : 2) void seq_fwd(SeqParams p) {
@@ -435,7 +435,8 @@ __global__ __launch_bounds__(64 * WAVES, NC == 1 ? (E4M3 || HD <= 96 ? 4 : 3) : 
                 continue;
             }
         }
-        const float f = sum == 0.0f ? 0.0f : 1.0f / sum;  // (a row that sees nothing sums to exactly zero; of scores that are all NaN the maximum is none either)
+        // (a row that sees nothing sums to exactly zero; scores that are all NaN have no maximum either)
+        const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
         u32x4 r;
 #pragma unroll
         for (int j = 0; j < 4; ++j) r[j] = T::pack2(f == 0.0f ? 0.0f : o[2 * j] * f, f == 0.0f ? 0.0f : o[2 * j + 1] * f);

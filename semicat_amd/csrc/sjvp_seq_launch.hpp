@@ -36,7 +36,8 @@ int seq_by_head(int D, bool dma, F&& f) {
 template <typename T> int seq_packed_fwd(SeqParams p, hipStream_t stream);
 template <typename T> int seq_packed_bwd(SeqParams p, hipStream_t stream);
 // How a call of the paged attention is served: by seq_few, which splits long sequences over workgroups and takes any number of rows, or, where
-// blocks of 128 rows fill half of the compute units, the longer sequences by seq_fwd.  Scratch of each: places in floats.
+// the sequences have 128 rows on average and blocks of 128 rows fill half of the compute units (an eighth with tables of 1024 positions or more), the longer
+// sequences by seq_fwd (paged_plan).  Scratch of each: places in floats.
 struct PagedPart {
     int splits = 1, split_tiles = 1;
     size_t stat = 0, part = 0, used = 0;
